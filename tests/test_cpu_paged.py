@@ -1,0 +1,81 @@
+"""Ops on shared pages: the CPU statement against dense attention, and what is refused."""
+import pytest
+import torch
+
+from scirust_b200.ops import paged
+
+BF = torch.bfloat16
+
+
+def batch(B=3, H=4, Hkv=2, dh=64, page=8, prefix=20, tails=(1, 9, 4), new=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    shared = prefix // page
+    own = [(prefix + t + page - 1) // page - shared for t in tails]
+    total = shared + sum(own) + 2
+    order = torch.randperm(total, generator=g).int()
+    table = torch.zeros((B, shared + max(own)), dtype=torch.int32)
+    at = shared
+    for b, n in enumerate(own):
+        table[b, :shared] = order[:shared]
+        table[b, shared:shared + n] = order[at:at + n]
+        at += n
+    rows = [1] * B if new is None else new
+    cu = None if new is None else torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32)
+    return dict(q=torch.randn(sum(rows), H * dh, generator=g).to(BF), pool=torch.randn(total, 2, Hkv, page, dh, generator=g).to(BF),
+                block_table=table, page=page, seq_len=torch.tensor([prefix + t for t in tails], dtype=torch.int32),
+                prefix_table=order[:shared].contiguous(), prefix_len=prefix, H=H, Hkv=Hkv, dh=dh, cu_q=cu)
+
+
+@pytest.mark.parametrize("new", [None, [1, 9, 3]])
+def test_statement_is_dense_attention(new):
+    a = batch(new=new)
+    out = paged.shared_prefix_attention(**a)
+    at = 0
+    for b, n in enumerate(new or [1, 1, 1]):
+        L = int(a["seq_len"][b])
+        kv = a["pool"][a["block_table"][b].long()].double().permute(1, 2, 0, 3, 4).reshape(2, 2, -1, 64)[:, :, :L]
+        for i in range(n):
+            limit = L - n + i + 1
+            q = a["q"][at].double().view(2, 2, 64)
+            p = torch.softmax(q @ kv[0, :, :limit].transpose(1, 2) / 8, -1)
+            want = (p @ kv[1, :, :limit]).reshape(-1)
+            assert torch.allclose(out[at].double(), want, atol=2 ** -7 * float(want.abs().max()))
+            at += 1
+
+
+def test_empty_sequences_and_rows_of_no_sequence():
+    a = batch(new=[1, 9, 3])
+    a["seq_len"][1] = 0
+    out = paged.shared_prefix_attention(**a)
+    assert not out[1:10].any() and bool(out[0].any()) and bool(out[10:].any())
+    a = batch(new=[1, 9, 3])
+    a["q"] = torch.cat([a["q"], a["q"][:2]])
+    out = paged.shared_prefix_attention(**a)
+    assert not out[13:].any()
+    kept = paged.shared_prefix_attention(**a, out=torch.full_like(out, 3.0))
+    assert torch.equal(kept[:13], out[:13]) and bool((kept[13:] == 3).all())
+
+
+@pytest.mark.parametrize("change", [
+    dict(H=3), dict(page=16), dict(dh=32), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(prefix_len=-1),
+    dict(prefix_len=30), dict(seq_len=torch.ones(2, dtype=torch.int32)), dict(cu_q=torch.zeros(3, dtype=torch.int32)),
+    dict(q=torch.zeros(4, 256, dtype=BF)), dict(q=torch.zeros(3, 255, dtype=BF)), dict(out=torch.zeros(3, 255, dtype=BF)),
+    dict(block_table=torch.zeros(3, dtype=torch.int32))])
+def test_refusals(change):
+    with pytest.raises(ValueError):
+        paged.shared_prefix_attention(**{**batch(), **change})
+
+
+def test_entry_point_refuses():
+    """Sizes and pointers are looked at before anything is launched."""
+    from scirust_b200.ops import _lib
+    ok = dict(q=16, ldq=256, pool=16, n_blocks=4, table=16, max_blocks=4, page=64, seq_len=16, prefix_table=16, prefix=64, cu=None, B=2, NT=2,
+              H=4, Hkv=2, dh=64, units=4, scale=0.125, ws=16, ws_bytes=1 << 30, out=16, ldo=256, fill=1, status=16, stream=None)
+    for change, what in ((dict(B=0), "bad argument"), (dict(NT=3), "bad argument"), (dict(H=5), "bad argument"), (dict(dh=96), "bad argument"),
+                         (dict(page=12), "bad argument"), (dict(page=4), "bad argument"), (dict(prefix=32), "bad argument"),
+                         (dict(prefix_table=None), "bad argument"), (dict(scale=0.0), "bad argument"), (dict(scale=float("nan")), "bad argument"),
+                         (dict(ws_bytes=100), "bad argument"), (dict(H=260), "bad argument"), (dict(q=24), "misaligned"), (dict(ldq=257), "misaligned"),
+                         (dict(out=8), "misaligned"), (dict(ldo=260), "misaligned"), (dict(n_blocks=1 << 24), "size beyond"),
+                         (dict(max_blocks=1 << 25), "size beyond"), (dict(B=1 << 22, NT=1 << 22, max_blocks=1 << 12), "size beyond")):
+        with pytest.raises(_lib.NativeError, match=what):
+            _lib.call("sb_shared_prefix_attention", *{**ok, **change}.values())

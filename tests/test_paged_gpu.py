@@ -1,0 +1,229 @@
+"""Ops on pages that sequences share, against 64-bit statements."""
+import math
+
+import pytest
+import torch
+
+from scirust_b200.ops import _lib, paged
+
+pytestmark = pytest.mark.gpu
+BF, F64 = torch.bfloat16, torch.float64
+DEV = "cuda"
+
+
+def batch(B, H, Hkv, dh, page, prefix, tails, new=None, seed=0, spare=3, q_pad=8):
+    """Inputs of a batch: tails[b] positions behind the prefix, of which the last new[b] are rows (default: one each)."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    shared = prefix // page
+    own = [max(0, (prefix + t + page - 1) // page - shared) for t in tails]
+    total = shared + sum(own) + spare
+    order = torch.randperm(total, generator=g, device=DEV).int()
+    table = torch.full((B, shared + max(own + [1])), -1, dtype=torch.int32, device=DEV)
+    at = shared
+    for b, n in enumerate(own):
+        table[b, :shared] = order[:shared]
+        table[b, shared:shared + n] = order[at:at + n]
+        at += n
+    pool = torch.randn((total, 2, Hkv, page, dh), generator=g, device=DEV).to(BF)
+    rows = [1] * B if new is None else new
+    q = (torch.randn((sum(rows), H * dh + q_pad), generator=g, device=DEV) * 1.5).to(BF)
+    cu = None if new is None else torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32, device=DEV)
+    return dict(q=q, pool=pool, block_table=table, page=page, seq_len=torch.tensor([prefix + t for t in tails], dtype=torch.int32, device=DEV),
+                prefix_table=order[:shared].contiguous(), prefix_len=prefix, H=H, Hkv=Hkv, dh=dh, cu_q=cu)
+
+
+def statement(a, scale=None):
+    """(o, bound): 64 bits, and how far an element may be off. P is rounded to bf16 (half a step of 2^-8) and weighs v, the answer is
+    rounded once more; a score is a sum of dh products in 32 bits, each addition off by a step of 2^-23 of the sum of magnitudes, which
+    the exponential passes on as a relative error of a weight and of their sum."""
+    H, Hkv, dh, page = a["H"], a["Hkv"], a["dh"], a["page"]
+    scale = dh ** -0.5 if scale is None else scale
+    n = a["q"].shape[0]
+    o, bound = torch.zeros((n, Hkv, H // Hkv, dh), dtype=F64, device=DEV), torch.zeros((n, Hkv, H // Hkv, dh), dtype=F64, device=DEV)
+    ends = list(range(n + 1)) if a["cu_q"] is None else a["cu_q"].tolist()
+    for b, length in enumerate(a["seq_len"].tolist()):
+        t0, t1 = ends[b], ends[b + 1]
+        for t in range(t0, t1):
+            limit = length - (t1 - t0) + (t - t0) + 1
+            if limit <= 0:
+                continue
+            pos = torch.arange(limit, device=DEV)
+            kv = a["pool"][a["block_table"][b].long()[pos // page], :, :, pos % page].to(F64)
+            q = a["q"][t, :H * dh].to(F64).reshape(Hkv, H // Hkv, dh)
+            s = torch.einsum("kgd,jkd->kgj", q, kv[:, 0]) * scale
+            size = torch.einsum("kgd,jkd->kgj", q.abs(), kv[:, 0].abs()) * scale
+            p = torch.softmax(s, -1)
+            o[t] = torch.einsum("kgj,jkd->kgd", p, kv[:, 1])
+            mean = torch.einsum("kgj,jkd->kgd", p, kv[:, 1].abs())
+            slip = 2 * dh * 2.0 ** -23 * size.amax(-1, keepdim=True)
+            bound[t] = 2.0 ** -8 * (mean + o[t].abs()) + slip * mean + 1e-6
+    return o.reshape(n, -1), bound.reshape(n, -1)
+
+
+def check(a, **kw):
+    out = paged.shared_prefix_attention(**a, **kw)
+    _lib.check_status(out.device)
+    want, bound = statement(a, kw.get("scale"))
+    off = (out.to(F64) - want).abs() / bound.clamp_min(1e-30)
+    assert bool((off <= 1).all()), f"off by up to {float(off.nan_to_num(9e9).max()):.2f} of the bound"
+    return out
+
+
+HEADS = [(16, 4, 64), (32, 8, 128), (4, 1, 128), (8, 8, 64), (6, 2, 128), (20, 1, 64)]
+
+
+@pytest.mark.parametrize("H,Hkv,dh", HEADS)
+@pytest.mark.parametrize("page,prefix,tails", [
+    (64, 128, [1, 64, 65, 3]), (64, 1000, [1, 5, 200, 24, 25, 88]), (16, 333, [1, 7, 40]), (8, 80, [9]), (128, 640, [1, 129, 300]),
+    (32, 31, [1, 64]), (64, 0, [1, 63, 64, 130]), (192, 400, [20, 700]), (40, 200, [1, 41, 90])])
+def test_one_row_each(H, Hkv, dh, page, prefix, tails):
+    check(batch(len(tails), H, Hkv, dh, page, prefix, tails))
+
+
+@pytest.mark.parametrize("H,Hkv,dh", HEADS[:3] + [(6, 2, 128)])
+@pytest.mark.parametrize("page,prefix,tails,new", [
+    (64, 512, [64, 10, 1, 33], [64, 10, 1, 5]), (64, 1000, [30, 7, 7], [30, 0, 7]), (16, 333, [70, 70], [70, 3]),
+    (64, 200, [500], [500]), (64, 0, [150, 1, 64], [150, 1, 64]), (128, 300, [3, 260, 9], [3, 200, 9]), (8, 100, [1, 1, 1], [1, 1, 1])])
+def test_ragged_rows(H, Hkv, dh, page, prefix, tails, new):
+    check(batch(len(tails), H, Hkv, dh, page, prefix, tails, new))
+
+
+def test_rows_before_the_first_position_and_empty_sequences():
+    a = batch(5, 16, 4, 64, 64, 256, [10, 1, 5, 70, 3])
+    a["seq_len"] = torch.tensor([266, 0, 100, 326, 256], dtype=torch.int32, device=DEV)     # empty, inside the prefix, its last position
+    out = check(a)
+    assert not out[1].any()
+    a = batch(3, 16, 4, 64, 64, 128, [40, 6, 4], [40, 6, 4])
+    a["seq_len"] = torch.tensor([20, 3, 0], dtype=torch.int32, device=DEV)                  # more rows than positions
+    out = check(a)
+    assert not out[:20].any() and not out[40:43].any() and not out[46:].any() and bool(out[43].any())
+    a = batch(3, 16, 4, 64, 64, 0, [4, 6, 4])
+    a["seq_len"] = torch.zeros(3, dtype=torch.int32, device=DEV)
+    assert not check(a).any()
+
+
+@pytest.mark.parametrize("new", [None, [1, 9, 1, 30]])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -3.3895e38])
+def test_what_no_row_sees_may_hold_anything(new, junk):
+    a = batch(4, 8, 2, 128, 16, 100, [1, 9, 50, 30], new)
+    page = a["page"]
+    table = a["block_table"].cpu()
+    seen = torch.zeros(a["pool"].shape[0], page, dtype=torch.bool)
+    for b, length in enumerate(a["seq_len"].tolist()):
+        pos = torch.arange(length)
+        seen[table[b].long()[pos // page], pos % page] = True
+    a["pool"].masked_fill_(~seen.to(DEV)[:, None, None, :, None], junk)
+    check(a)
+
+
+def test_scores_far_apart():
+    a = batch(6, 16, 4, 64, 64, 320, [1, 9, 50, 30, 77, 128])
+    a["q"] *= 20                                   # scores of a few hundred: one position has all the weight
+    check(a)
+    check(batch(6, 16, 4, 64, 64, 320, [1, 9, 50, 30, 77, 128]), scale=0.01)
+
+
+def test_weights_of_the_lowest_value_mask():
+    """A row whose scores are all near the lowest bf16 value still has weights that sum to one."""
+    a = batch(2, 4, 4, 64, 64, 128, [5, 70])
+    a["q"].fill_(-3e19)
+    a["pool"][:, 0] = 3e18                         # q.k = -9e37 * 64, beyond 32 bits only after 64 products
+    a["pool"][:, 0, :, :, 1:] = 0
+    out = check(a)
+    assert bool(out.any())
+
+
+def test_rows_of_no_sequence():
+    a = batch(3, 16, 4, 64, 64, 256, [9, 5, 20], [9, 5, 20])
+    a["q"] = torch.cat([a["q"], a["q"][:7]])
+    a["cu_q"] += 3                                 # three rows in front of the first sequence, four behind the last
+    a["q"] = a["q"].roll(3, 0).contiguous()
+    out = check(a)
+    assert not out[:3].any() and not out[-4:].any()
+    kept = torch.full_like(out, 7.0)
+    assert paged.shared_prefix_attention(**a, out=kept) is kept
+    assert torch.equal(kept[3:-4], out[3:-4]) and bool((kept[:3] == 7).all()) and bool((kept[-4:] == 7).all())
+
+
+def test_offsets_that_make_no_sense_stay_inside():
+    a = batch(4, 16, 4, 64, 64, 256, [9, 5, 20, 2], [9, 5, 20, 2])
+    a["cu_q"] = torch.tensor([0, 30, 10, 9000, -5], dtype=torch.int32, device=DEV)
+    guard = torch.full((a["q"].shape[0] + 8, 1024), 7.0, dtype=BF, device=DEV)
+    out = paged.shared_prefix_attention(**a, out=guard[4:-4])
+    _lib.check_status(out.device)
+    assert bool((guard[:4] == 7).all()) and bool((guard[-4:] == 7).all())
+
+
+def test_pages_outside_the_pool_read_as_zeros():
+    a = batch(3, 16, 4, 64, 64, 128, [70, 5, 300])
+    bad = dict(a, block_table=a["block_table"].clone())
+    bad["block_table"][0, 2:] = torch.tensor([1 << 30, -7, 5000, 2 ** 31 - 1, 0], device=DEV)[:bad["block_table"].shape[1] - 2].int()
+    out = paged.shared_prefix_attention(**bad)
+    _lib.check_status(out.device)
+    assert torch.equal(out[1:], paged.shared_prefix_attention(**a)[1:]) and bool(out.isfinite().all())
+
+
+def test_strides_of_rows_and_of_the_answer():
+    a = batch(5, 16, 4, 64, 64, 256, [10, 1, 5, 70, 3])
+    wide = torch.zeros((5, 4096), dtype=BF, device=DEV)
+    wide[:, 8:8 + 1024] = a["q"][:, :1024]
+    want = check(a)
+    answer = torch.zeros((5, 2048), dtype=BF, device=DEV)
+    out = paged.shared_prefix_attention(**dict(a, q=wide[:, 8:]), out=answer[:, 512:1536])
+    assert torch.equal(out, want) and not answer[:, :512].any() and not answer[:, 1536:].any()
+
+
+def test_long_prefix_many_sequences():
+    check(batch(64, 8, 2, 64, 64, 6000, [1 + 7 * b % 190 for b in range(64)]))
+    check(batch(130, 4, 1, 128, 64, 700, [1 + 11 * b % 300 for b in range(130)]))
+
+
+def test_more_sequences_than_a_cta_plans_for():
+    check(batch(1100, 4, 1, 64, 64, 130, [1 + b % 90 for b in range(1100)]))
+
+
+def test_offsets_beyond_32_bits():
+    """Pages whose elements lie past 2^31 of the pool (5.4 GB)."""
+    H, Hkv, dh, page = 8, 8, 128, 64
+    a = batch(2, H, Hkv, dh, page, 128, [100, 7])
+    far = torch.empty((20600, 2, Hkv, page, dh), dtype=BF, device=DEV)
+    assert far.numel() > 1 << 31
+    n = a["pool"].shape[0]
+    far[-n:] = a["pool"]
+    move = 20600 - n
+    b = dict(a, pool=far, block_table=a["block_table"] + move, prefix_table=a["prefix_table"] + move)
+    assert torch.equal(paged.shared_prefix_attention(**b), check(a))
+
+
+def test_same_bits_again_on_another_stream_and_in_a_graph():
+    a = batch(9, 32, 8, 128, 64, 1000, [1 + 30 * b for b in range(9)])
+    want = check(a, max_len=1300)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [paged.shared_prefix_attention(**a, max_len=1300) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(o, want) for o in outs)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            o = paged.shared_prefix_attention(**a, max_len=1300)
+        graphs.append((g, o))
+    a["seq_len"] -= 17                              # lengths and pages are read by the replay
+    a["seq_len"].clamp_(min=1000)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):                              # both graphs at once
+        for (g, _), s in zip(graphs, (one, two)):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    want = check(a, max_len=1300)
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want)
+
+
+def test_what_a_bound_of_the_lengths_is_for():
+    """max_len sizes the launch; lengths beyond it are still answered."""
+    a = batch(3, 16, 4, 64, 64, 256, [300, 5, 700])
+    assert torch.allclose(check(a, max_len=1).float(), check(a).float(), atol=0.05)
