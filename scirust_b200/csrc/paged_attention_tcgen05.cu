@@ -7,8 +7,8 @@
 // o_i not divided by l_i, join as m = max m_i, w_i = exp(scale (m_i - m)), o = sum w_i o_i / sum w_i l_i (here m_i is a maximum of q.k).
 //
 // Both parts are the same work for a CTA: a tile of 128 rows (tokens times the query heads of one kv head), a table of pages and a
-// range of 64-position blocks of keys. An item is all of that for one tile of rows:
-//   shared: (kv head, tile of consecutive tokens, whatever their sequences), blocks [0, P / 64)
+// range of 128-position blocks of keys. An item is all of that for one tile of rows:
+//   shared: (kv head, tile of consecutive tokens, whatever their sequences), blocks [0, P / 128)
 //   own:    (sequence, tile of its tokens, kv head), blocks of [P, limit of its last row)
 // Where the sequences bring a whole tile of rows each there is nothing to share, and their own items start at position 0.
 // The blocks of all items form one line, which is dealt out evenly over the CTAs; what lies in a CTA's share of an item is a piece.
@@ -18,34 +18,52 @@
 #include "api.h"
 #include "dependent.cuh"
 #include "per_device.h"
+#include <limits.h>
+#include <type_traits>
 
 namespace sb {
 
 int num_sms();
+int make_tmap_3d_bf16_box(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t pitch1, uint64_t pitch2,
+                          uint32_t box0, uint32_t box1, uint32_t box2);
 int make_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t ld,
                       uint32_t box_inner, uint32_t box_outer);
 
 namespace spa {
 
 constexpr int BM = 128;        // rows of a tile
-constexpr int BN = 64;         // positions of a block
-constexpr int THREADS = 192;   // producer, issuer, four softmax warps
-constexpr int TMEM_COLS = 256;
-constexpr int MAX_DIRECT = 1024;   // sequences of one token each whose plan every CTA makes for itself, in shared memory
+constexpr int BN = 128;        // positions of a block
+constexpr int HALF = BN / 2;   // columns of P that are handed over at once
+constexpr int THREADS = 384;   // loaders of rows and K, and of V, issuers of both products, two lanes of four softmax warps
+// Registers a thread: 168 at launch for all three warpgroups, shared out as 72 + 2 x 216.
+constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;
+static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * 168, "the shares draw on the registers of the launch");
+constexpr int TMEM_COLS = 512;
+constexpr int QUEUE = 4;       // pieces that the producer may be ahead
+constexpr int ITEM_UNITS = 2;
+// A row's reference may lag behind its maximum until a weight passes 2^8: then O is rescaled, in the first blocks of a piece mostly. What
+// is summed is the weight after its rounding to bf16, the one that multiplies V, so a row that one position dominates loses nothing.
+constexpr float RESCALE_GAP = 8.f;
 constexpr float LOWEST = -3.402823466e38f;   // reference of a row that has seen nothing: 2^(-inf - LOWEST) is 0
 
 template <int DH>
 struct Cfg {
   static constexpr int NCH = DH / 64;                // 64-column chunks of a head
-  static constexpr int SLOTS = DH == 128 ? 4 : 8;    // ring of K and V blocks
-  static constexpr int Q_BYTES = BM * DH * 2;
   static constexpr int KV_BYTES = BN * DH * 2;
-  static constexpr int PLAN_BYTES = (2 * MAX_DIRECT + 2) * 4;
-  static constexpr int SMEM_BYTES = Q_BYTES + SLOTS * KV_BYTES + 256 /* barriers */ + PLAN_BYTES + 1024 /* alignment */;
-  static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
-  // tensor memory: scores, two buffers of P as bf16 pairs, O
-  static constexpr int COL_S = 0, COL_P = BN, COL_O = COL_P + 2 * (BN / 2);
-  static_assert(COL_O + DH <= TMEM_COLS, "tensor memory");
+  static constexpr int SB = DH == 64 ? 2 : 1;        // score accumulators: one that the lanes take turns with at 128, one each at 64
+  // Shared memory holds two tiles of the rows that the largest tile of the batch has, and as many blocks of K and V as go in beside them.
+  static constexpr int MAX_SLOTS = DH == 128 ? 7 : 14;
+  static constexpr int BAR_BYTES = (8 * (2 * MAX_SLOTS + 2 * QUEUE + 2 + 2 + 2 + 2 + 4 + 2 + 4 + 4) + 8 + 15) / 16 * 16;
+  static constexpr int FIXED_BYTES = BAR_BYTES + QUEUE * 32 + BM * 8 + 1024 /* alignment */;
+  static int slots(int q_rows) {
+    const int n = (227 * 1024 - FIXED_BYTES - 2 * q_rows * DH * 2) / KV_BYTES;
+    return n < MAX_SLOTS ? n : MAX_SLOTS;
+  }
+  static int smem_bytes(int q_rows) { return 2 * q_rows * DH * 2 + slots(q_rows) * KV_BYTES + FIXED_BYTES; }
+  static_assert((227 * 1024 - FIXED_BYTES - 2 * BM * DH * 2) / KV_BYTES >= 5, "three blocks of K and two of V beside two full tiles");
+  // tensor memory: scores, P of each lane as bf16 pairs, O of each lane
+  static constexpr int COL_P = SB * BN, COL_O = COL_P + 2 * (BN / 2);
+  static_assert(COL_O + 2 * DH <= TMEM_COLS, "tensor memory");
 };
 
 // What the plan says of an item of its own: tokens [t0, t0 + n), sequence, position behind the last one that a row sees.
@@ -55,7 +73,8 @@ struct Pair {
 
 struct Header {        // at the start of the workspace
   int units, units_shared, q_lo, q_hi, pairs;
-  int pad[3];
+  int least;           // no row sees fewer positions
+  int pad[2];
 };
 
 struct Params {
@@ -69,6 +88,9 @@ struct Params {
   int prefix;          // shared positions: whole pages; 0 where every sequence's own items start at 0
   int page, n_blocks, box;
   int B, NT, H, Hkv, G, TT;
+  int q_tokens;        // of the box that brings a tile of rows
+  int q_rows;          // of a tile in shared memory, a multiple of 8; the tensor core reads 128, those behind are rows of no one
+  int ks, vs;          // blocks of K and V in shared memory
   float scale_log2;
   __nv_bfloat16* out;
   long long ldo;
@@ -79,7 +101,7 @@ struct Params {
   int* row_limit;      // [NT]
   int* row_pair;       // [NT], -1: of no sequence
   float* whole;        // [2][NT][H][dh], and [2][NT][H][2] behind it: items that were not cut
-  float* cut;          // [2 * CTAs][128][dh], and [2 * CTAs][128][2] behind it: first and last pieces of the CTAs
+  float* cut;          // [2 * CTAs][256][dh], and [2 * CTAs][256][2] behind it: first and last pieces of the CTAs
   int max_pairs;
   int* status;
 };
@@ -89,25 +111,80 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 32 bytes, a whole sector.
+__device__ __forceinline__ void st_global_v8(float* to, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// Wait of a whole warp, all lanes with one result; bounded like mbar_wait, in fewer instructions: the kernel below is bound by what it
+// has to fetch of its own code where a CTA goes through many short pieces (with mbar_wait at every wait 136 KB).
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > kLocalWaitNs || *reinterpret_cast<volatile int*>(status) != 0)) {
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+  return true;
+}
+// Lane 0's value: the same for the whole warp, as the compiler then knows.
+__device__ __forceinline__ uint32_t same(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// The even deal of `units` over `ctas`: the first `rem` of them get one more.
+// a / d for 0 <= a < 2^31, d > 0: the compiler's own division takes three times the instructions.
+__device__ __forceinline__ int quotient(int a, int d) {
+  int q = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(d)));
+  int r = a - q * d;
+#pragma unroll 1
+  while (r < 0) { --q; r += d; }
+#pragma unroll 1
+  while (r >= d) { ++q; r -= d; }
+  return q;
+}
+
+// The even deal of `units` over `ctas`: the first `rem` of them get one more. Two units at least, so that a CTA between the ends of an
+// item has a block of it, whose two units may lie with two CTAs (the first unit's CTA has the block).
 struct Deal {
-  int per, rem;
-  __device__ Deal(int units, int ctas) : per(units / ctas), rem(units - units / ctas * ctas) {}
-  __device__ int begin(int c) const { return c * per + min(c, rem); }
+  int units, per, rem;
+  __device__ Deal(int units_, int ctas) : units(units_) {
+    ctas = min(ctas, max(1, units >> 1));
+    per = quotient(units, ctas);
+    rem = units - per * ctas;
+  }
+  __device__ int begin(int c) const { return min(units, c * per + min(c, rem)); }
   __device__ int owner(int u) const {
     const int edge = rem * (per + 1);
-    return u < edge ? u / (per + 1) : rem + (u - edge) / per;      // per == 0: all units lie below the edge
+    const bool low = u < edge;
+    return quotient(low ? u : u - edge, low ? per + 1 : max(per, 1)) + (low ? 0 : rem);
   }
 };
 
 __device__ __forceinline__ int blocks_of(int positions) { return positions > 0 ? (positions + BN - 1) / BN : 0; }
+// Units that an item takes in the line: one for a block of one tile of rows, two for a block of two, and what an item costs besides
+// its blocks in front of them.
+__device__ __forceinline__ int units_of(int positions, int n_tok, int TT) {
+  return positions > 0 ? (positions + BN - 1) / BN * (n_tok > TT ? 2 : 1) + ITEM_UNITS : 0;
+}
+
+// The shared items of one kv head: tiles of two times TT tokens, the last of which may have one tile of rows.
+struct Shared {
+  int tiles, size, last, head;        // items of a head, units of an item and of the last one, of a head
+  __device__ Shared(int prefix, int tokens, int TT) {
+    tiles = prefix > 0 ? quotient(tokens + 2 * TT - 1, 2 * TT) : 0;
+    size = units_of(prefix, 2 * TT, TT);
+    last = units_of(prefix, tokens - (tiles - 1) * 2 * TT, TT);
+    head = tiles > 0 ? (tiles - 1) * size + last : 0;
+  }
+};
 
 // Inclusive sum over a warp.
 __device__ __forceinline__ int warp_scan(int v, int lane) {
@@ -119,85 +196,119 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
   return v;
 }
 
-// A piece of an item, as all roles of a CTA see it.
+// A piece of an item. The producer finds a CTA's pieces, one after the other, and hands them to the other warps.
 struct Piece {
-  int h, t0, n_tok, kbase, kend, j0, j1;   // blocks [j0, j1) of kbase + 64 j, positions below kend
-  const int* table;
-  bool shared, cut, first;                 // cut: only a part of its item; first: the first piece of this CTA
+  int h, t0, n_tok, kbase, kend, j0, j1;   // blocks [j0, j1) of kbase + 128 j, positions below kend
+  int flags;                               // and the sequence, whose table it is, from SEQUENCE on
 };
+// CUT: not all of its item; FIRST: begins where the CTA's share does; SHORT: some row may end inside
+constexpr int PIECE_SHARED = 1, PIECE_CUT = 2, PIECE_FIRST = 4, PIECE_SHORT = 8, SEQUENCE = 4;
 
+// A CTA's pieces, found by a whole warp. The plan of a batch of one token a sequence is summed up on the way, 32 sequences at a time;
+// anything else has been planned (plan_kernel).
 struct Walk {
   const Params& p;
-  const int* cum;
-  const int* len;        // lengths of sequences of one token each, or null: pairs come from the plan
-  int units_shared, q_lo, q_hi, tiles_q, blocks_shared, pairs;
+  const Shared shared;
+  int units_shared, q_lo, q_hi, pairs;
   int u, u1, u_first;
-  int pair_at;
+  int window, c_lo, c_hi;        // pairs window + lane: units of one kv head before and behind
+  int4 info;
 
-  __device__ Walk(const Params& p_, const int* cum_, const int* len_, const Header& h, int u0, int u1_)
-      : p(p_), cum(cum_), len(len_), units_shared(h.units_shared), q_lo(h.q_lo), q_hi(h.q_hi),
-        tiles_q((h.q_hi - h.q_lo + p_.TT - 1) / p_.TT), blocks_shared(blocks_of(p_.prefix)), pairs(h.pairs), u(u0), u1(u1_),
-        u_first(u0), pair_at(-1) {}
+  __device__ Walk(const Params& p_, const Header& h, int u0, int u1_)
+      : p(p_), shared(p_.prefix, h.q_hi - h.q_lo, p_.TT), units_shared(h.units_shared), q_lo(h.q_lo), q_hi(h.q_hi), pairs(h.pairs), u(u0),
+        u1(u1_), u_first(u0), window(-1), c_lo(0), c_hi(0), info(make_int4(0, 0, 0, 0)) {}
 
-  __device__ bool next(Piece& x) {
-    if (u >= u1) return false;
-    int off, size;
-    if (u < units_shared) {
-      size = blocks_shared;
-      const int item = u / size;
-      off = u - item * size;
-      x.h = item / tiles_q;
-      x.t0 = q_lo + (item - x.h * tiles_q) * p.TT;
-      x.n_tok = min(p.TT, q_hi - x.t0);
-      x.kbase = 0;
-      x.kend = p.prefix;
-      x.table = p.prefix_table;
-      x.shared = true;
-    } else {
-      const int v = u - units_shared;
-      if (pair_at < 0) {                        // last pair that starts at v or before
-        int lo = 0, hi = pairs - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (cum[mid] * p.Hkv <= v) lo = mid; else hi = mid - 1;
-        }
-        pair_at = lo;
-      }
-      while (cum[pair_at + 1] * p.Hkv <= v) ++pair_at;      // v lies below the last pair's end
-      size = cum[pair_at + 1] - cum[pair_at];
-      const int rest = v - cum[pair_at] * p.Hkv;
-      x.h = rest / size;
-      off = rest - x.h * size;
-      int b;
-      if (len) {
-        b = pair_at;
-        x.t0 = b; x.n_tok = 1; x.kend = len[b];
-      } else {
-        const int4 i = *reinterpret_cast<const int4*>(p.pair + pair_at);
-        x.t0 = i.x; x.n_tok = i.y; x.kend = i.w;
-        b = i.z;
-      }
-      x.kbase = p.prefix;
-      x.table = p.block_table + static_cast<size_t>(b) * p.max_blocks;
-      x.shared = false;
+  __device__ void planned(int from, int lane) {
+    window = from;
+    const int i = from + lane;
+    c_lo = c_hi = -1;
+    if (i < pairs) {
+      c_lo = p.cum[i];
+      c_hi = p.cum[i + 1];
+      info = *reinterpret_cast<const int4*>(p.pair + i);
     }
-    x.j0 = off;
-    x.j1 = min(size, off + (u1 - u));
-    x.cut = x.j1 - x.j0 != size;
-    x.first = u == u_first;
-    u += x.j1 - x.j0;
-    return true;
+  }
+  __device__ void summed(int from, int lane, int before) {
+    window = from;
+    const int b = from + lane;
+    const int len = b < pairs ? clampi(p.seq_len[b], 0, p.max_blocks * p.page) : 0;
+    const int n = units_of(len - p.prefix, 1, p.TT);
+    c_hi = before + warp_scan(n, lane);
+    c_lo = c_hi - n;
+    info = make_int4(b, 1, b, len);
+  }
+
+  // False: no more pieces.
+  __device__ bool next(Piece& x) {
+    const int lane = threadIdx.x & 31;
+    for (;;) {
+      if (u >= u1) return false;
+      int off, size;
+      x.flags = u == u_first ? PIECE_FIRST : 0;
+      if (u < units_shared) {
+        x.h = quotient(u, shared.head);
+        const int rest = u - x.h * shared.head;
+        const int tile = min(quotient(rest, shared.size), shared.tiles - 1);
+        off = rest - tile * shared.size;
+        size = tile == shared.tiles - 1 ? shared.last : shared.size;
+        x.t0 = q_lo + tile * 2 * p.TT;
+        x.n_tok = min(2 * p.TT, q_hi - x.t0);
+        x.kbase = 0;
+        x.kend = p.prefix;
+        x.flags |= PIECE_SHARED;
+      } else {
+        const int v = u - units_shared;
+        if (window < 0) {
+          if (p.pair) {                           // last pair that starts at v or before
+            int lo = 0, hi = pairs - 1;
+            while (lo < hi) {
+              const int mid = (lo + hi + 1) >> 1;
+              if (p.cum[mid] * p.Hkv <= v) lo = mid; else hi = mid - 1;
+            }
+            planned(lo, lane);
+          } else {
+            summed(0, lane, 0);
+          }
+        }
+        unsigned open;
+        while (!(open = __ballot_sync(0xffffffffu, c_hi * p.Hkv > v))) {   // v lies below the last pair's end
+          if (window >= pairs) return false;
+          if (p.pair) planned(window + 32, lane);
+          else summed(window + 32, lane, __shfl_sync(0xffffffffu, c_hi, 31));
+        }
+        const int l = __ffs(open) - 1;
+        const int before = __shfl_sync(0xffffffffu, c_lo, l);
+        size = __shfl_sync(0xffffffffu, c_hi, l) - before;
+        const int rest = v - before * p.Hkv;
+        x.h = quotient(rest, size);
+        off = rest - x.h * size;
+        x.t0 = __shfl_sync(0xffffffffu, info.x, l);
+        x.n_tok = __shfl_sync(0xffffffffu, info.y, l);
+        x.kend = __shfl_sync(0xffffffffu, info.w, l);
+        x.kbase = p.prefix;
+        x.flags |= __shfl_sync(0xffffffffu, info.z, l) << SEQUENCE;
+      }
+      const int stop = min(size, off + (u1 - u));
+      u += stop - off;
+      // a block belongs to the CTA that has its first unit
+      const int two = x.n_tok > p.TT ? 1 : 0;
+      x.j0 = (max(0, off - ITEM_UNITS) + two) >> two;
+      x.j1 = (max(0, stop - ITEM_UNITS) + two) >> two;
+      if (x.j1 == x.j0) continue;
+      if (x.j1 - x.j0 != (size - ITEM_UNITS) >> two) x.flags |= PIECE_CUT;
+      return true;
+    }
   }
 };
 
 // Plan of a ragged batch, or of more sequences than the CTAs plan for themselves: one CTA.
 __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   __shared__ int s_warp[32];
-  __shared__ int s_hi, s_pairs, s_sum;
+  __shared__ int s_hi, s_pairs, s_sum, s_least;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   pdl_wait();
-  if (tid == 0) { s_hi = p.cu_q ? clampi(p.cu_q[0], 0, p.NT) : 0; s_pairs = 0; s_sum = 0; }
+  if (tid == 0) { s_hi = p.cu_q ? clampi(p.cu_q[0], 0, p.NT) : 0; s_pairs = 0; s_sum = 0; s_least = INT_MAX; }
   for (int t = tid; t < p.NT; t += 1024) { p.row_limit[t] = 0; p.row_pair[t] = -1; }
   __syncthreads();
   const int q_lo = s_hi;
@@ -226,7 +337,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
     if (tid == 1023) s_hi = max(before, top);
     start = max(start, before);
     const int n = b < p.B ? max(0, end - start) : 0;
-    int tiles = (n + p.TT - 1) / p.TT;
+    const int span = 2 * p.TT;             // tokens of an item
+    int tiles = (n + span - 1) / span;
     const int scan = warp_scan(tiles, lane);
     if (lane == 31) s_warp[warp] = scan;
     __syncthreads();
@@ -237,12 +349,13 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
     if (tid == 1023) s_pairs = min(at + tiles, p.max_pairs);
     if (b < p.B) {
       const int len = clampi(p.seq_len[b], 0, cap);
+      if (n > 0) atomicMin(&s_least, len - n + 1);
       for (int i = 0; i < tiles && at + i < p.max_pairs; ++i) {
         Pair x;
-        x.t0 = start + i * p.TT;
-        x.n = min(p.TT, n - i * p.TT);
+        x.t0 = start + i * span;
+        x.n = min(span, n - i * span);
         x.b = b;
-        x.kend = len - n + i * p.TT + x.n;
+        x.kend = len - n + i * span + x.n;
         *reinterpret_cast<int4*>(p.pair + at + i) = make_int4(x.t0, x.n, x.b, x.kend);
       }
     }
@@ -258,7 +371,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   }
   for (int i0 = 0; i0 < pairs; i0 += 1024) {
     const int i = i0 + tid;
-    const int n = i < pairs ? blocks_of(p.pair[i].kend - p.prefix) : 0;
+    const int n = i < pairs ? units_of(p.pair[i].kend - p.prefix, p.pair[i].n, p.TT) : 0;
     const int scan = warp_scan(n, lane);
     if (lane == 31) s_warp[warp] = scan;
     __syncthreads();
@@ -271,45 +384,108 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   }
   if (tid == 0) {
     p.cum[pairs] = s_sum;
-    const int shared = p.Hkv * ((q_hi - q_lo + p.TT - 1) / p.TT) * blocks_of(p.prefix);
+    const int shared = p.Hkv * Shared(p.prefix, q_hi - q_lo, p.TT).head;
     p.hdr->units = shared + p.Hkv * s_sum;
     p.hdr->units_shared = shared;
     p.hdr->q_lo = q_lo; p.hdr->q_hi = q_hi; p.hdr->pairs = pairs;
+    p.hdr->least = s_least;
   }
 }
 
+// What brings the blocks of K, or of V, whole warp.
+struct Ring {
+  uint8_t* at;
+  uint64_t *full, *empty;
+  const int* table;
+  int slots, slot, head, from, row;        // lane i: first row in the pool of box (from + i)
+  uint32_t phase;
+
+  __device__ Ring(uint8_t* at_, uint64_t* full_, uint64_t* empty_, int slots_)
+      : at(at_), full(full_), empty(empty_), table(nullptr), slots(slots_), slot(0), head(0), from(0), row(0), phase(0) {}
+
+  __device__ void piece(const Params& p, const Piece& x, int head_) {
+    table = x.flags & PIECE_SHARED ? p.prefix_table : p.block_table + static_cast<size_t>(x.flags >> SEQUENCE) * p.max_blocks;
+    head = head_;
+    from = -(1 << 30);
+  }
+
+  template <int DH>
+  __device__ bool load(const Params& p, const CUtensorMap& tmap, const Piece& x, int j) {
+    const int lane = threadIdx.x & 31, nbx = BN / p.box, bx0 = j * nbx;       // boxes of a block, at most 16
+    if (bx0 + nbx > from + 32) {              // nbx divides 32: a block's boxes are fetched together
+      from = bx0;
+      const int pos = x.kbase + (from + lane) * p.box, at_page = quotient(pos, p.page);
+      int page = pos < x.kend ? table[at_page] : 0;
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.n_blocks)) page = p.n_blocks;   // reads as zeros
+      row = (page * 2 * p.Hkv + head) * p.page + pos - at_page * p.page;
+    }
+    if (!wait(&empty[slot], phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) return false;
+    const int live = min(nbx, (x.kend - x.kbase - j * BN + p.box - 1) / p.box);     // boxes with a position below kend
+    if (lane == 0) mbar_arrive_expect_tx(&full[slot], live * p.box * DH * 2);
+    __syncwarp();
+    const int i = lane - (bx0 - from);
+    if (i >= 0 && i < live) {
+      uint8_t* to = at + slot * (BN * DH * 2) + i * p.box * 128;
+#pragma unroll
+      for (int c = 0; c < DH / 64; ++c) tma_load_2d(to + c * (BN * 128), &tmap, &full[slot], c * 64, row);
+    }
+    __syncwarp();
+    if (++slot == slots) { slot = 0; phase ^= 1; }
+    return true;
+  }
+};
+
 template <int DH>
-__global__ void __launch_bounds__(THREADS, 2)
-attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, 1)
+attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap q_tile, const __grid_constant__ CUtensorMap q_token,
+              const __grid_constant__ Params p) {
   using C = Cfg<DH>;
-  constexpr int SLOTS = C::SLOTS;
+  const int KS = p.ks, VS = p.vs;
+  const int q_chunk = p.q_rows * 128, q_bytes = q_chunk * C::NCH;      // a 64-column chunk of a tile of rows, the tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = sQ + C::Q_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + SLOTS * C::KV_BYTES);   // [SLOTS]
-  uint64_t* empty = full + SLOTS;        // [SLOTS]
-  uint64_t* q_full = empty + SLOTS;      // rows of a piece are in shared memory (4 warp arrivals)
-  uint64_t* s_full = q_full + 1;         // scores of a block are in tensor memory
-  uint64_t* s_free = s_full + 1;         // and in registers (4 warp arrivals)
-  uint64_t* p_full = s_free + 1;         // [2] P of a block is in tensor memory and O rescaled (4 warp arrivals)
-  uint64_t* pv_done = p_full + 2;        // P V of a block has completed
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 1);
-  int* s_cum = reinterpret_cast<int*>(ring + SLOTS * C::KV_BYTES + 256);     // [B + 1]
-  int* s_len = s_cum + MAX_DIRECT + 1;                                       // [B]
-  static_assert((2 * SLOTS + 7) * 8 + 4 <= 256, "barriers");
+  uint8_t* sK = sQ + 2 * q_bytes;
+  uint8_t* sV = sK + KS * C::KV_BYTES;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sV + VS * C::KV_BYTES);      // [KS]
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;       // [VS]
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* x_full = v_empty + VS;       // [QUEUE] a piece is in the queue
+  uint64_t* x_empty = x_full + QUEUE;    // [QUEUE] and has been read (loader of V, issuers, eight softmax warps)
+  uint64_t* q_full = x_empty + QUEUE;    // [2] rows of every second piece are in shared memory
+  uint64_t* q_empty = q_full + 2;        // [2] and have been multiplied
+  uint64_t* s_full = q_empty + 2;        // [2] scores of a lane's block are in tensor memory
+  uint64_t* s_free = s_full + 2;         // [SB] the scores that lay in this accumulator are in registers (4 warp arrivals)
+  uint64_t* p_full = s_free + 2;         // [2][2] a half of a lane's P is in tensor memory, O rescaled (4 warp arrivals)
+  uint64_t* pv_done = p_full + 4;        // [2] P V of a lane's block has completed
+  uint64_t* o_full = pv_done + 2;        // [4] a quarter of the rows: lane 1 has its sum ready for lane 0
+  uint64_t* o_free = o_full + 4;         // [4] and lane 0 has read it
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_free + 4);
+  Piece* queue = reinterpret_cast<Piece*>(sV + VS * C::KV_BYTES + C::BAR_BYTES);
+  float2* s_ml = reinterpret_cast<float2*>(queue + QUEUE);                    // [BM] maximum and sum of lane 1
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    mbar_init(q_full, 4);
-    mbar_init(s_full, 1);
-    mbar_init(s_free, 4);
-    mbar_init(&p_full[0], 4);
-    mbar_init(&p_full[1], 4);
-    mbar_init(pv_done, 1);
+    for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    for (int s = 0; s < QUEUE; ++s) { mbar_init(&x_full[s], 1); mbar_init(&x_empty[s], 11); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_free[s], 4);
+      mbar_init(&pv_done[s], 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_full[s], 1);
+      mbar_init(&o_free[s], 1);
+    }
     fence_barrier_init();
     fence_proxy_async_smem();
     prefetch_tmap(&tmap);
+    prefetch_tmap(&q_tile);
+    prefetch_tmap(&q_token);
   }
   if (warp == 1) {
     tmem_alloc(tmem_holder, TMEM_COLS);
@@ -322,266 +498,371 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   pdl_trigger();
   pdl_wait();
 
-  // ---- plan: one token per sequence is summed up here, anything else has been by plan_kernel
-  const bool direct = p.pair == nullptr;
-  Header hdr;
-  if (direct) {
-    if (warp == 0) {
+  // Pieces as the other warps get them from warp 0; j1 == 0 is the end. A piece of more rows than a tile has gives each lane a
+  // tile, and both take every block; of one tile both take the rows, and every second block. The lanes take turns throughout: `steps`
+  // counts what both have taken (a block of a lane is a step).
+  int at = 0;
+  uint32_t at_phase = 0;
+  auto take = [&](Piece& x) -> bool {
+    if (!wait(&x_full[at], at_phase, p.status, ST_TIMEOUT_MISC)) return false;
+    const int4* from = reinterpret_cast<const int4*>(queue + at);
+    const int4 a = from[0], b = from[1];
+    x.h = a.x; x.t0 = a.y; x.n_tok = a.z; x.kbase = a.w;
+    x.kend = b.x; x.j0 = b.y; x.j1 = b.z; x.flags = b.w;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&x_empty[at]);
+    if (++at == QUEUE) { at = 0; at_phase ^= 1; }
+    return x.j1 != 0;
+  };
+  Piece x = {};
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+  if (warp == 0) {
+    // -------------------------------- pieces, their rows, and K --------------------------------
+    Header hdr;
+    if (p.pair) {
+      hdr.units = p.hdr->units; hdr.units_shared = p.hdr->units_shared;
+      hdr.q_lo = p.hdr->q_lo; hdr.q_hi = p.hdr->q_hi; hdr.pairs = p.hdr->pairs; hdr.least = p.hdr->least;
+    } else {
       const int cap = p.max_blocks * p.page;
-      int base = 0;
+      int sum = 0, least = INT_MAX;
+#pragma unroll 1
       for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int b = b0 + lane;
-        const int len = b < p.B ? clampi(p.seq_len[b], 0, cap) : 0;
-        const int n = blocks_of(len - p.prefix);
+        const int len = b < p.B ? clampi(p.seq_len[b], 0, cap) : INT_MAX;
+        const int n = b < p.B ? units_of(len - p.prefix, 1, p.TT) : 0;
+        least = min(least, len);
         const int scan = warp_scan(n, lane);
-        if (b < p.B) {
-          s_cum[b] = base + scan - n;
-          s_len[b] = len;
-          if (blockIdx.x == 0) { p.cum[b] = base + scan - n; }
-        }
-        base += __shfl_sync(0xffffffffu, scan, 31);
+        if (blockIdx.x == 0 && b < p.B) p.cum[b] = sum + scan - n;        // for the joining launch
+        sum += __shfl_sync(0xffffffffu, scan, 31);
       }
+      hdr.q_lo = 0; hdr.q_hi = p.B; hdr.pairs = p.B; hdr.least = __reduce_min_sync(0xffffffffu, least);
+      hdr.units_shared = p.Hkv * Shared(p.prefix, p.B, p.TT).head;
+      hdr.units = hdr.units_shared + p.Hkv * sum;
+      if (blockIdx.x == 0 && lane == 0) {
+        p.cum[p.B] = sum;
+        p.hdr->units = hdr.units; p.hdr->units_shared = hdr.units_shared;
+        p.hdr->q_lo = 0; p.hdr->q_hi = p.B; p.hdr->pairs = p.B;
+      }
+    }
+    const Deal deal(hdr.units, gridDim.x);
+    Walk walk(p, hdr, deal.begin(blockIdx.x), deal.begin(blockIdx.x + 1));
+    Ring k(sK, k_full, k_empty, KS);
+    int n_pieces = 0;
+    bool ok = true, both = false;
+    while (ok) {
+      const bool more = walk.next(x);
+      if (!more) x.j0 = x.j1 = 0;
+      if (hdr.least < x.kend) x.flags |= PIECE_SHORT;
+      ok = wait(&x_empty[at], at_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
+      if (!ok) break;
       if (lane == 0) {
-        s_cum[p.B] = base;
-        if (blockIdx.x == 0) p.cum[p.B] = base;
+        int4* to = reinterpret_cast<int4*>(queue + at);
+        to[0] = make_int4(x.h, x.t0, x.n_tok, x.kbase);
+        to[1] = make_int4(x.kend, x.j0, x.j1, x.flags);
+        mbar_arrive(&x_full[at]);
       }
-    }
-    __syncthreads();
-    hdr.q_lo = 0; hdr.q_hi = p.B; hdr.pairs = p.B;
-    hdr.units_shared = p.Hkv * ((p.B + p.TT - 1) / p.TT) * blocks_of(p.prefix);
-    hdr.units = hdr.units_shared + p.Hkv * s_cum[p.B];
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      p.hdr->units = hdr.units; p.hdr->units_shared = hdr.units_shared;
-      p.hdr->q_lo = 0; p.hdr->q_hi = p.B; p.hdr->pairs = p.B;
-    }
-  } else {
-    hdr.units = p.hdr->units; hdr.units_shared = p.hdr->units_shared;
-    hdr.q_lo = p.hdr->q_lo; hdr.q_hi = p.hdr->q_hi; hdr.pairs = p.hdr->pairs;
-  }
-  const Deal deal(hdr.units, gridDim.x);
-  Walk walk(p, direct ? s_cum : p.cum, direct ? s_len : nullptr, hdr, deal.begin(blockIdx.x), deal.begin(blockIdx.x + 1));
-  Piece x;
-
-  if (warp == 0) {
-    // ------------------------------------ TMA producer ------------------------------------
-    // Blocks arrive in the order in which the issuer takes them: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1) of a piece.
-    int slot = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    const int nbx = BN / p.box;               // boxes of a block, at most 8
-    while (ok && walk.next(x)) {
-      int fetched = -(1 << 30), page_of_lane = 0;      // lane i: page of box (fetched + i)
-      int fetched_v = -(1 << 30), page_of_lane_v = 0;
-      auto load = [&](int j, bool v, int& at, int& pages) -> bool {
-        if (!mbar_wait_warp(&empty[slot], phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) return false;
-        const int bx0 = j * nbx;
-        if (bx0 < at || bx0 + nbx > at + 32) {         // nbx divides 32: a block's boxes are fetched together
-          at = bx0;
-          const int pos = x.kbase + (at + lane) * p.box;
-          pages = pos < x.kend ? x.table[pos / p.page] : 0;
-          if (static_cast<unsigned>(pages) >= static_cast<unsigned>(p.n_blocks)) pages = p.n_blocks;   // reads as zeros
+      __syncwarp();
+      if (++at == QUEUE) { at = 0; at_phase ^= 1; }
+      if (!more) break;
+      const bool two = x.n_tok > p.TT;
+      k.piece(p, x, x.h);
+#pragma unroll 1
+      for (int j = x.j0; j < x.j1 && ok; ++j) {
+        ok = k.template load<DH>(p, tmap, x, j);
+        if (j > x.j0) continue;
+        // Rows of a piece of one tile go to either half of the space, while those of the piece before are multiplied; two tiles take both.
+        // So the piece before the last has been multiplied, and where both halves are needed the last too.
+#pragma unroll 1
+        for (int before = 2; before >= (two || both ? 1 : 2); --before) {
+          const int piece = n_pieces - before;
+          ok = ok && (piece < 0 || wait(&q_empty[piece & 1], (piece >> 1) & 1, p.status, ST_TIMEOUT_EMPTY));
         }
-        const int live = min(nbx, (x.kend - x.kbase - j * BN + p.box - 1) / p.box);     // boxes with a position below kend
-        uint8_t* to = ring + slot * C::KV_BYTES;
-        if (lane == 0) mbar_arrive_expect_tx(&full[slot], live * p.box * DH * 2);
-        for (int i = 0; i < live; ++i) {
-          const int blk = __shfl_sync(0xffffffffu, pages, bx0 + i - at);
-          if (lane == 0) {
-            const int row = (blk * 2 * p.Hkv + (v ? p.Hkv : 0) + x.h) * p.page + (x.kbase + (bx0 + i) * p.box) % p.page;
-#pragma unroll
-            for (int c = 0; c < C::NCH; ++c)
-              tma_load_2d(to + c * (BN * 128) + i * p.box * 128, &tmap, &full[slot], c * 64, row);
+        both = two;
+        if (ok && lane == 0) {
+          // The box of a tile brings its tokens and, behind the last of them, rows of others that no one reads.
+          const bool one = x.n_tok == 1;
+          const int tiles = two ? 2 : 1, bytes = (one ? 1 : p.q_tokens) * p.G * 128;
+          uint64_t* bar = &q_full[n_pieces & 1];
+          mbar_arrive_expect_tx(bar, tiles * C::NCH * bytes);
+#pragma unroll 1
+          for (int i = 0; i < tiles * C::NCH; ++i) {
+            const int tile = i / C::NCH, c = i % C::NCH;
+            tma_load_3d(sQ + (two ? tile : n_pieces & 1) * q_bytes + c * q_chunk, one ? &q_token : &q_tile, bar, c * 64, x.h * p.G,
+                        x.t0 + tile * p.TT);
           }
         }
         __syncwarp();
-        if (++slot == SLOTS) { slot = 0; phase ^= 1; }
-        return true;
-      };
-      ok = load(x.j0, false, fetched, page_of_lane);
-      for (int j = x.j0; j < x.j1 && ok; ++j) {
-        if (j + 1 < x.j1) ok = load(j + 1, false, fetched, page_of_lane);
-        ok = ok && load(j, true, fetched_v, page_of_lane_v);
       }
+      ++n_pieces;
+    }
+  } else if (warp == 3) {
+    // -------------------------------- V --------------------------------
+    Ring v(sV, v_full, v_empty, VS);
+    bool ok = true;
+    while (ok && take(x)) {
+      v.piece(p, x, p.Hkv + x.h);
+#pragma unroll 1
+      for (int j = x.j0; j < x.j1 && ok; ++j) ok = v.template load<DH>(p, tmap, x, j);
     }
   } else if (warp == 1) {
-    // ------------------------------------- MMA issuer -------------------------------------
+    // ------------------------------------- S = Q K^T -------------------------------------
+    // The two products have a warp each: what one of them waits for, asks and counts (half of the time of a single warp for both) the
+    // tensor core spends on the other's. The warp walks its loop as a whole and one lane issues; what an instruction is given comes from
+    // lane 0 by a shuffle, so that it is known to be the same for the warp and stays in uniform registers.
     const bool leader = elect_one();
-    constexpr uint32_t idesc_s = make_idesc_bf16(BM, BN, false, false);
-    constexpr uint32_t idesc_o = make_idesc_bf16(BM, DH, false, true);
-    int slot = 0, n_blocks = 0, n_pieces = 0;      // blocks whose scores were issued, pieces begun
-    uint32_t phase = 0;
+    constexpr uint32_t idesc = make_idesc_bf16(BM, BN, false, false);
+    constexpr uint64_t desc = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16);
+    const uint32_t a_q = smem_u32(sQ), a_k = smem_u32(sK), chunk = same(q_chunk >> 4);
+    int ks = 0, n_pieces = 0, steps = 0;
+    uint32_t kph = 0;
     bool ok = true;
-    const uint64_t dq = make_smem_desc(smem_u32(sQ), 16, 1024);
-    auto advance = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
-    auto scores = [&]() -> bool {                  // S = Q K^T
-      if (!mbar_wait_warp(&full[slot], phase, p.status, ST_TIMEOUT_FULL)) return false;
-      if (n_blocks > 0 && !mbar_wait_warp(s_free, (n_blocks - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY)) return false;
-      tc_fence_after();
-      const uint64_t dk = make_smem_desc(smem_u32(ring + slot * C::KV_BYTES), 16, 1024);
-      if (leader) {
+    while (ok && take(x)) {
+      const int half = n_pieces & 1;
+      const bool two = same(x.n_tok > p.TT ? 1 : 0);
+      const int n = same((x.j1 - x.j0) << (two ? 1 : 0));
+      ok = wait(&q_full[half], (n_pieces >> 1) & 1, p.status, ST_TIMEOUT_MISC);
+#pragma unroll 1
+      for (int i = 0; i < n && ok; ++i, ++steps) {
+        const int L = steps & 1;
+        const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;      // the block's first step, its last
+        const int before = C::SB == 1 ? steps : steps >> 1;                        // scores that were in this accumulator
+        const uint32_t q_lo = same((a_q + (two ? L : half) * q_bytes) >> 4), k_lo = same((a_k + ks * C::KV_BYTES) >> 4);
+        const uint32_t to = same(tmem + (C::SB == 1 ? 0 : L * BN));
+        if (uses) ok = wait(&k_full[ks], kph, p.status, ST_TIMEOUT_FULL);
+        if (before > 0) ok = ok && wait(&s_free[C::SB == 1 ? 0 : L], (before - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k)
-          umma_bf16_ss(tmem + C::COL_S, smem_desc_at(dq, (k >> 2) * (BM * 128) + (k & 3) * 32),
-                       smem_desc_at(dk, (k >> 2) * (BN * 128) + (k & 3) * 32), idesc_s, k > 0 ? 1u : 0u);
-        umma_commit(s_full);
-        umma_commit(&empty[slot]);
-      }
-      ++n_blocks;
-      advance();
-      return true;
-    };
-    auto values = [&](int i, int live, bool begins) -> bool {     // O (+)= P V of block i, of which `live` positions count
-      if (!mbar_wait_warp(&full[slot], phase, p.status, ST_TIMEOUT_FULL)) return false;
-      uint8_t* v = ring + slot * C::KV_BYTES;
-      if (live < BN) {
-        // The weights of positions behind the end are zero, but what lies there may be no number: zero times it would be none either.
-        for (int c = lane; c < (BN - live) * (DH / 8); c += 32) {
-          const int row = live + c / (DH / 8), w = c % (DH / 8);       // rows are whole, so their swizzle does not matter
-          *reinterpret_cast<uint4*>(v + (w >> 3) * (BN * 128) + row * 128 + (w & 7) * 16) = make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < DH / 16; ++k)
+            umma_bf16_ss(to, desc | (q_lo + (k >> 2) * chunk + (k & 3) * 2), desc | (k_lo + (k >> 2) * (BN * 8) + (k & 3) * 2), idesc,
+                         k > 0 ? 1u : 0u);
+          umma_commit(&s_full[L]);
+          if (frees) umma_commit(&k_empty[ks]);
+          if (i == n - 1) umma_commit(&q_empty[half]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
+        if (frees) {
+          if (++ks == KS) { ks = 0; kph ^= 1; }
+        }
       }
-      if (!mbar_wait_warp(&p_full[i & 1], (i >> 1) & 1, p.status, ST_TIMEOUT_MISC)) return false;
-      tc_fence_after();
-      const uint64_t dv = make_smem_desc(smem_u32(v), BN * 128, 1024);
-      if (leader) {
-#pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          umma_bf16_ts(tmem + C::COL_O, tmem + C::COL_P + (i & 1) * (BN / 2) + k * 8, smem_desc_at(dv, k * (16 * 128)), idesc_o,
-                       (!begins || k > 0) ? 1u : 0u);
-        umma_commit(pv_done);
-        umma_commit(&empty[slot]);
-      }
-      advance();
-      return true;
-    };
-    while (ok && walk.next(x)) {
-      ok = mbar_wait_warp(q_full, n_pieces & 1, p.status, ST_TIMEOUT_MISC);
       ++n_pieces;
-      const int i0 = n_blocks;
-      ok = ok && scores();
-      for (int j = x.j0; j < x.j1 && ok; ++j) {
-        if (j + 1 < x.j1) ok = scores();
-        ok = ok && values(i0 + j - x.j0, min(BN, x.kend - x.kbase - j * BN), j == x.j0);
-      }
     }
   } else {
+    // ------------------------------------- O (+)= P V -------------------------------------
+    const bool leader = elect_one();
+    constexpr uint32_t idesc = make_idesc_bf16(BM, DH, false, true);
+    constexpr uint64_t desc = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61) | (static_cast<uint64_t>(BN * 8) << 16);
+    const uint32_t a_v = smem_u32(sV);
+    int vs = 0, steps = 0;
+    uint32_t vph = 0;
+    bool ok = true;
+    while (ok && take(x)) {
+      const bool two = same(x.n_tok > p.TT ? 1 : 0);
+      const int n = same((x.j1 - x.j0) << (two ? 1 : 0)), first_live = same(x.kend - x.kbase - x.j0 * BN);
+#pragma unroll 1
+      for (int i = 0; i < n && ok; ++i, ++steps) {
+        const int L = steps & 1, turn = steps >> 1;            // every second step is this lane's
+        const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;
+        const int live = min(BN, first_live - (two ? i >> 1 : i) * BN);            // positions that count
+        const uint32_t v_lo = same((a_v + vs * C::KV_BYTES) >> 4), o = same(tmem + C::COL_O + L * DH),
+                       w = same(tmem + C::COL_P + L * (BN / 2)), begins = same(i < 2 ? 1 : 0);
+        if (uses) {
+          ok = wait(&v_full[vs], vph, p.status, ST_TIMEOUT_FULL);
+          if (ok && (live & 15)) {
+            // A product takes 16 positions. The weights of those behind the end are zero, but what lies there may be no number, and zero
+            // times it would be none either.
+            uint8_t* v = sV + vs * C::KV_BYTES;
+#pragma unroll 1
+            for (int c = lane; c < (16 - (live & 15)) * (DH / 8); c += 32) {
+              const int row = live + c / (DH / 8), e = c % (DH / 8);       // rows are whole, so their swizzle does not matter
+              *reinterpret_cast<uint4*>(v + (e >> 3) * (BN * 128) + row * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && wait(&p_full[2 * L + h], turn & 1, p.status, ST_TIMEOUT_MISC);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int k2 = 0; k2 < HALF / 16; ++k2) {
+              const int k = h * (HALF / 16) + k2;
+              if (k * 16 < live) umma_bf16_ts(o, w + k * 8, desc | (v_lo + k * 128), idesc, (!begins || k > 0) ? 1u : 0u);
+            }
+          }
+        }
+        if (!ok) break;
+        if (leader) {
+          umma_commit(&pv_done[L]);
+          if (frees) umma_commit(&v_empty[vs]);
+        }
+        if (frees) {
+          if (++vs == VS) { vs = 0; vph ^= 1; }
+        }
+      }
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     // ------------------------------------ softmax warps ------------------------------------
+    const int L = (warp >> 2) - 1;         // lane
     const int quarter = warp & 3;          // lanes of tensor memory that this warp may read
     const int r = quarter * 32 + lane;     // row of the tile
-    const int tok = r / p.G, g = r - tok * p.G;
-    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t tm_S = tmem + C::COL_S + lane_off, tm_O = tmem + C::COL_O + lane_off;
+    const int row_tok = quotient(r, p.G), g = r - row_tok * p.G;
+    const uint32_t tm = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t tm_S = tm + (C::SB == 1 ? 0 : L * BN), tm_P = tm + C::COL_P + L * (BN / 2), tm_O = tm + C::COL_O + L * DH;
     const float sl2 = p.scale_log2;
-    int n_blocks = 0;
-    auto load_q = [&](const Piece& y) {
-      if (tok < y.n_tok) {
-        const uint4* from = reinterpret_cast<const uint4*>(p.q + (y.t0 + tok) * p.ldq + (y.h * p.G + g) * DH);
-        uint8_t* to = sQ + r * 128;
-#pragma unroll
-        for (int c = 0; c < DH / 8; ++c)
-          *reinterpret_cast<uint4*>(to + (c >> 3) * (BM * 128) + (((c & 7) ^ (r & 7)) << 4)) = from[c];
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    };
-    bool more = walk.next(x);
-    if (more) load_q(x);
-    while (more) {
-      const bool active = quarter * 32 < x.n_tok * p.G;      // whether any row of this warp counts
-      const bool valid = tok < x.n_tok;
+    int n = 0, steps = 0, n_join = 0;      // this lane's blocks; both lanes'; pieces whose lanes were joined
+    bool pending = false;                  // lane 1: its O waits to be read by lane 0
+    while (take(x)) {
+      const bool two = x.n_tok > p.TT;
+      const int nb = x.j1 - x.j0;
+      const int first = two ? 0 : (L ^ steps) & 1, step = two ? 1 : 2;           // this lane's blocks
+      steps += two ? 2 * nb : nb;
+      if (first >= nb) continue;
+      const int toks = two ? min(p.TT, x.n_tok - L * p.TT) : x.n_tok, tok = row_tok + (two ? L * p.TT : 0);
+      const bool active = quarter * 32 < toks * p.G;      // whether any row of this warp counts
+      const bool valid = row_tok < toks;
       const int t = x.t0 + tok;
       // positions that the row sees of this piece's
-      const int limit = valid ? min(x.kend, direct ? s_len[t] : p.row_limit[t]) : x.kend;
+      int limit = x.kend;
+      if (valid) {
+        if (!(x.flags & PIECE_SHARED)) limit -= x.n_tok - 1 - tok;
+        else if (x.flags & PIECE_SHORT) limit = min(limit, p.pair ? p.row_limit[t] : p.seq_len[t]);
+      }
       float m_ref = LOWEST, l = 0.f;
-      for (int j = x.j0; j < x.j1; ++j, ++n_blocks) {
-        mbar_wait_converged(s_full, n_blocks & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+      for (int i = first; i < nb; i += step, ++n) {
+        // Waits in this loop may give up (the status word says so) but do not end it: lanes that left it one by one would be
+        // missing at the warp barriers below.
+        wait(&s_full[L], n & 1, p.status, ST_TIMEOUT_TMEM_FULL);
         if (!active) {
           __syncwarp();
-          if (lane == 0) { mbar_arrive(s_free); mbar_arrive(&p_full[n_blocks & 1]); }
+          if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
+          // P V of the block before: its P was complete then, so these arrivals are this block's
+          if (n > 0) wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+          if (pending) {                   // as below
+            wait(&o_free[quarter], (n_join - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
+            pending = false;
+          }
+          __syncwarp();
+          if (lane == 0) { mbar_arrive(&p_full[2 * L]); mbar_arrive(&p_full[2 * L + 1]); }
           continue;
         }
         tc_fence_after();
         uint32_t v[BN];
         __syncwarp();
-        tmem_ld_32x32_converged(tm_S, v);
-        tmem_ld_32x32_converged(tm_S + 32, v + 32);
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32_converged(tm_S + c * 32, v + c * 32);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
-        const int lim = limit - (x.kbase + j * BN);          // columns from here on are masked
-        if (lim < BN) {
+        if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
+        const int lim = limit - (x.kbase + (x.j0 + i) * BN);          // columns from here on are masked
+        const int live = x.kend - (x.kbase + (x.j0 + i) * BN);        // for every row
+        if (__any_sync(0xffffffffu, lim < BN)) {
 #pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (i >= lim) v[i] = 0xff800000u;
+          for (int c = 0; c < BN; ++c)
+            if (c >= lim) v[c] = 0xff800000u;
         }
         float m4[4] = {LOWEST, LOWEST, LOWEST, LOWEST};
 #pragma unroll
-        for (int i = 0; i < BN; i += 2)
-          m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        for (int c = 0; c < BN; c += 2)
+          m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         const float m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        const bool grow = m_blk > m_ref;
+        const bool grow = (m_blk - m_ref) * sl2 > RESCALE_GAP || m_ref == LOWEST;
         const float alpha = grow ? ex2((m_ref - m_blk) * sl2) : 1.f;
         if (grow) m_ref = m_blk;
         const float neg_m = -m_ref;
-        if (j > x.j0) {
-          mbar_wait_converged(pv_done, (n_blocks - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+        if (n > 0) {                       // P V of the block before has read P and updated O
+          wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
           tc_fence_after();
-          if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
+          if (i > first && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
             for (int c = 0; c < DH / 32; ++c) {
               uint32_t o[32];
               tmem_ld_32x32_converged(tm_O + c * 32, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) mul2(o[i], o[i + 1], alpha, alpha);
+              for (int e = 0; e < 32; e += 2) mul2(o[e], o[e + 1], alpha, alpha);
               tmem_st_32x32_converged(tm_O + c * 32, o);
             }
           }
         }
-        float sum4[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t pk[BN / 2];
-#pragma unroll
-        for (int i = 0; i < BN; i += 2) {
-          // Subtracted before it is scaled: one fused step leaves the rounding of scale * m between a row's largest score and zero,
-          // which is everything once scores are beyond 2^24.
-          fma2(v[i], v[i + 1], 1.f, neg_m);
-          mul2(v[i], v[i + 1], sl2, sl2);
-          const float e0 = ex2(__uint_as_float(v[i])), e1 = ex2(__uint_as_float(v[i + 1]));
-          add2(sum4[i & 6], sum4[(i & 6) + 1], __float_as_uint(e0), __float_as_uint(e1));
-          pk[i >> 1] = pack_bf16x2(e0, e1);
+        if (pending) {                     // O of the piece before is about to be overwritten
+          wait(&o_free[quarter], (n_join - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
+          pending = false;
         }
-        tmem_st_32x32(tmem + C::COL_P + (n_blocks & 1) * (BN / 2) + lane_off, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[n_blocks & 1]);
+        float sum4[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && live <= HALF) {    // nothing of it is multiplied
+            if (lane == 0) mbar_arrive(&p_full[2 * L + 1]);
+            break;
+          }
+          uint32_t pk[HALF / 2];
+#pragma unroll
+          for (int c2 = 0; c2 < HALF; c2 += 2) {
+            const int c = h * HALF + c2;
+            // Subtracted before it is scaled: one fused step leaves the rounding of scale * m between a row's largest score and zero,
+            // which is everything once scores are beyond 2^24.
+            fma2(v[c], v[c + 1], 1.f, neg_m);
+            mul2(v[c], v[c + 1], sl2, sl2);
+            const float e0 = ex2(__uint_as_float(v[c])), e1 = ex2(__uint_as_float(v[c + 1]));
+            const uint32_t w = pack_bf16x2(e0, e1);
+            add2(sum4[c & 6], sum4[(c & 6) + 1], w << 16, w & 0xffff0000u);
+            pk[c2 >> 1] = w;
+          }
+          tmem_st_32x32(tm_P + h * (HALF / 2), pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * L + h]);
+        }
         const float sum = ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) + ((sum4[4] + sum4[5]) + (sum4[6] + sum4[7]));
         l = __fadd_rn(__fmul_rn(l, alpha), sum);
       }
-      // all products of this piece with its rows are done: the next piece's may take their place
-      const Piece y = x;
-      more = walk.next(x);
-      if (more) load_q(x);
       if (!active) continue;
-      mbar_wait_warp(pv_done, (n_blocks - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+      const bool joins = !two && nb > 1;        // both lanes have a sum of these rows
+      wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
       tc_fence_after();
-      const int head = y.h * p.G + g;
-      const bool out_now = !y.cut && p.prefix == 0;
+      if (joins && L == 1) {
+        s_ml[r] = make_float2(m_ref, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_full[quarter]);
+        ++n_join;
+        pending = true;
+        continue;
+      }
+      float w0 = 1.f, w1 = 0.f;
+      if (joins) {
+        wait(&o_full[quarter], n_join & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+        tc_fence_after();
+        const float2 y = s_ml[r];
+        const float m = fmaxf(m_ref, y.x);
+        w0 = ex2((m_ref - m) * sl2);
+        w1 = ex2((y.x - m) * sl2);
+        m_ref = m;
+        l = __fmaf_rn(w0, l, __fmul_rn(w1, y.y));
+      }
+      const int head = x.h * p.G + g;
+      const bool cut = x.flags & PIECE_CUT;
+      const bool out_now = !cut && p.prefix == 0;
       float* to = nullptr;
       if (valid && !out_now) {
-        size_t row;
+        size_t row, rows;
         float* base;
-        size_t rows;
-        if (y.cut) {
-          row = static_cast<size_t>(2 * blockIdx.x + (y.first ? 0 : 1)) * BM + r;
-          rows = static_cast<size_t>(2) * gridDim.x * BM;
+        if (cut) {
+          row = static_cast<size_t>(2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1)) * (2 * BM) + (two ? L * BM : 0) + r;
+          rows = static_cast<size_t>(2) * gridDim.x * (2 * BM);
           base = p.cut;
         } else {
-          row = (static_cast<size_t>(y.shared ? 0 : p.NT) + t) * p.H + head;
+          row = (static_cast<size_t>(x.flags & PIECE_SHARED ? 0 : p.NT) + t) * p.H + head;
           rows = static_cast<size_t>(2) * p.NT * p.H;
           base = p.whole;
         }
@@ -589,30 +870,44 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         *reinterpret_cast<float2*>(base + rows * DH + row * 2) = make_float2(m_ref, l);
       }
       const float inv_l = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < DH; c0 += 64) {
+        uint32_t o[64];
+        __syncwarp();
 #pragma unroll
-      for (int c = 0; c < DH / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32(tm_O + c * 32, o);
+        for (int c = 0; c < 64; c += 32) tmem_ld_32x32_converged(tm_O + c0 + c, o + c);
+        if (joins) {
+          uint32_t o1[64];
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) tmem_ld_32x32_converged(tm_O + DH + c0 + c, o1 + c);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            o[e] = __float_as_uint(__fmaf_rn(w0, __uint_as_float(o[e]), __fmul_rn(w1, __uint_as_float(o1[e]))));
+        }
         tmem_ld_wait();
         if (valid && out_now) {
-          __nv_bfloat16* orow = p.out + t * p.ldo + head * DH + c * 32;
+          __nv_bfloat16* orow = p.out + t * p.ldo + head * DH + c0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int e = 0; e < 8; ++e) {
             uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(o[i * 8 + 0]) * inv_l, __uint_as_float(o[i * 8 + 1]) * inv_l);
-            w.y = pack_bf16x2(__uint_as_float(o[i * 8 + 2]) * inv_l, __uint_as_float(o[i * 8 + 3]) * inv_l);
-            w.z = pack_bf16x2(__uint_as_float(o[i * 8 + 4]) * inv_l, __uint_as_float(o[i * 8 + 5]) * inv_l);
-            w.w = pack_bf16x2(__uint_as_float(o[i * 8 + 6]) * inv_l, __uint_as_float(o[i * 8 + 7]) * inv_l);
-            *reinterpret_cast<uint4*>(orow + i * 8) = w;
+            w.x = pack_bf16x2(__uint_as_float(o[e * 8 + 0]) * inv_l, __uint_as_float(o[e * 8 + 1]) * inv_l);
+            w.y = pack_bf16x2(__uint_as_float(o[e * 8 + 2]) * inv_l, __uint_as_float(o[e * 8 + 3]) * inv_l);
+            w.z = pack_bf16x2(__uint_as_float(o[e * 8 + 4]) * inv_l, __uint_as_float(o[e * 8 + 5]) * inv_l);
+            w.w = pack_bf16x2(__uint_as_float(o[e * 8 + 6]) * inv_l, __uint_as_float(o[e * 8 + 7]) * inv_l);
+            *reinterpret_cast<uint4*>(orow + e * 8) = w;
           }
         } else if (valid) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(to + c * 32 + i * 4) = make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+          for (int e = 0; e < 64; e += 8) st_global_v8(to + c0 + e, o + e);
         }
-        __syncwarp();
       }
+      __syncwarp();
       tc_fence_before();      // O is in registers before the next piece's first P is handed over
+      if (joins) {
+        if (lane == 0) mbar_arrive(&o_free[quarter]);
+        ++n_join;
+      }
     }
   }
 
@@ -622,115 +917,151 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
 }
 
-// Joins the parts of a row: one CTA of four warps for each (token, head), the warps take every fourth part and add theirs in order.
-template <int DH>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, int ctas) {
+// Joins the parts of a row. A CTA has the heads of a (token, kv head), which have the same parts; WAYS warps share those of a row and
+// read a batch at a time, and their sums meet in shared memory.
+template <int DH, int WAYS>
+__global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant__ Params p, int ctas) {
   constexpr int F = DH / 32;               // columns of a lane
-  __shared__ float s_o[4][DH];
-  __shared__ float s_m[4], s_l[4];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x, head = blockIdx.y, h = head / p.G;
+  constexpr int ROWS = 4, BATCH = WAYS > 1 ? 4 : 8;       // rows, parts at a time
+  using Vec = typename std::conditional<F == 4, float4, float2>::type;
+  __shared__ float s_o[WAYS > 1 ? ROWS : 1][WAYS][DH];
+  __shared__ float2 s_ml[ROWS][WAYS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS, slot = warp / WAYS;
+  const int t = blockIdx.x, h = blockIdx.y;
   pdl_trigger();
   pdl_wait();
-  const Header hdr = *p.hdr;
   const int pair = p.pair ? p.row_pair[t] : t;
-  __nv_bfloat16* to = p.out + t * p.ldo + head * DH;
+  const int units = p.hdr->units, units_shared = p.hdr->units_shared, q_lo = p.hdr->q_lo, q_hi = p.hdr->q_hi;
   if (pair < 0) {                          // a row of no sequence
-    if (p.fill && threadIdx.x < DH) to[threadIdx.x] = __float2bfloat16_rn(0.f);
+    if (p.fill)
+      for (int i = threadIdx.x; i < p.G * DH; i += 128 * WAYS) p.out[t * p.ldo + h * p.G * DH + i] = __float2bfloat16_rn(0.f);
     return;
   }
-  const Deal deal(hdr.units, ctas);
-  // the row's two items: [begin, end) in the line of blocks, row inside the tile
-  int beg[2], end[2], row[2];
-  {
-    const int blocks = blocks_of(p.prefix), tiles_q = (hdr.q_hi - hdr.q_lo + p.TT - 1) / p.TT;
-    const int tile = (t - hdr.q_lo) / p.TT;
-    beg[0] = (h * tiles_q + tile) * blocks;
-    end[0] = beg[0] + blocks;
-    row[0] = (t - hdr.q_lo - tile * p.TT) * p.G + head - h * p.G;
-    const int before = p.cum[pair], size = p.cum[pair + 1] - before;
-    beg[1] = hdr.units_shared + before * p.Hkv + h * size;
-    end[1] = beg[1] + size;
-    row[1] = (t - (p.pair ? p.pair[pair].t0 : t)) * p.G + head - h * p.G;
-  }
-  int c0[2], n[2];
-#pragma unroll
+  const Deal deal(units, ctas);
+  // The row's two items: parts, where the first lies and those of the CTAs behind it, which begin with theirs.
+  const Shared shared(p.prefix, q_hi - q_lo, p.TT);
+  int n[2];
+  const float* from[2];
+  const float2* ml[2];
+  int jump[2];                             // rows from the first part to the second, which is 4 * BM in front of the third
+#pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    const bool some = end[i] > beg[i];
-    c0[i] = some ? deal.owner(beg[i]) : 0;
-    n[i] = some ? deal.owner(end[i] - 1) - c0[i] + 1 : 0;
+    int beg, size, t0, tokens;
+    if (i == 0) {
+      const int tile = quotient(t - q_lo, 2 * p.TT);
+      beg = h * shared.head + tile * shared.size;
+      size = tile == shared.tiles - 1 ? shared.last : shared.size;
+      t0 = q_lo + tile * 2 * p.TT;
+      tokens = min(2 * p.TT, q_hi - t0);
+      if (p.prefix == 0) size = 0;
+    } else {
+      const int before = p.cum[pair];
+      size = p.cum[pair + 1] - before;
+      beg = units_shared + before * p.Hkv + h * size;
+      t0 = p.pair ? p.pair[pair].t0 : t;
+      tokens = p.pair ? p.pair[pair].n : 1;
+    }
+    const int two = tokens > p.TT ? 1 : 0, tok = t - t0;
+    int count = 0, skip = 0;
+    size_t at = 0;
+    bool cut = false;
+    if (size > 0) {
+      const int first = beg + ITEM_UNITS, c0 = deal.owner(first);
+      count = deal.owner(first + ((((size - ITEM_UNITS) >> two) - 1) << two)) - c0 + 1;
+      cut = count > 1;
+      const bool odd = deal.begin(c0) < beg;         // the second piece of its CTA
+      skip = odd ? 2 * BM : 4 * BM;
+      at = cut ? static_cast<size_t>(2 * c0 + (odd ? 1 : 0)) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
+               : (static_cast<size_t>(i ? p.NT : 0) + t) * p.H + h * p.G;
+    }
+    const size_t rows = cut ? static_cast<size_t>(4) * ctas * BM : static_cast<size_t>(2) * p.NT * p.H;
+    const float* base = cut ? p.cut : p.whole;
+    const float* o = base + at * DH + lane * F;
+    const float2* m = reinterpret_cast<const float2*>(base + rows * DH) + at;
+    if (i == 0) { n[0] = count; from[0] = o; ml[0] = m; jump[0] = skip; }
+    else { n[1] = count; from[1] = o; ml[1] = m; jump[1] = skip; }
   }
   if (p.prefix == 0 && n[1] == 1) return;  // written out by its CTA
   const int parts = n[0] + n[1];
-  const size_t rows_cut = static_cast<size_t>(2) * ctas * BM, rows_whole = static_cast<size_t>(2) * p.NT * p.H;
-  auto part = [&](int k, const float*& o, const float*& ml) {
-    const int i = k < n[0] ? 0 : 1;
-    if (n[i] == 1) {
-      const size_t at = (static_cast<size_t>(i ? p.NT : 0) + t) * p.H + head;
-      o = p.whole + at * DH;
-      ml = p.whole + rows_whole * DH + at * 2;
-    } else {
-      const int c = c0[i] + k - (i ? n[0] : 0);
-      const size_t at = static_cast<size_t>(2 * c + (deal.begin(c) >= beg[i] ? 0 : 1)) * BM + row[i];
-      o = p.cut + at * DH;
-      ml = p.cut + rows_cut * DH + at * 2;
-    }
-  };
-  float m = LOWEST, l = 0.f, acc[F];
+#pragma unroll 1
+  for (int g0 = 0; g0 < p.G; g0 += ROWS) {
+    const int g = g0 + slot;
+    float m = LOWEST, l = 0.f, acc[F];
 #pragma unroll
-  for (int f = 0; f < F; ++f) acc[f] = 0.f;
-  // this warp's parts: a lane looks up one of up to 32, then all lanes read them one after the other
-  for (int k0 = warp; k0 < parts; k0 += 4 * 32) {
-    const int k = k0 + 4 * lane;
-    const float* o = nullptr;
-    float2 x = make_float2(LOWEST, 0.f);
-    if (k < parts) {
-      const float* ml;
-      part(k, o, ml);
-      x = *reinterpret_cast<const float2*>(ml);
-    }
-    float top = x.x;
+    for (int f = 0; f < F; ++f) acc[f] = 0.f;
+    if (g < p.G) {
+#pragma unroll 1
+      for (int k0 = way; k0 < parts; k0 += WAYS * BATCH) {
+        Vec o[BATCH];
+        float2 x[BATCH];
 #pragma unroll
-    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    if (top > m) {
-      const float a = ex2((m - top) * p.scale_log2);
-      l *= a;
+        for (int b = 0; b < BATCH; ++b) {
+          const int k = k0 + b * WAYS;
+          const bool own = k >= n[0];
+          const int c = own ? k - n[0] : k;
+          const int row = g + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
+          x[b] = make_float2(LOWEST, 0.f);
+          o[b] = Vec{};
+          if (k < parts) {
+            o[b] = *reinterpret_cast<const Vec*>((own ? from[1] : from[0]) + static_cast<size_t>(row) * DH);
+            x[b] = (own ? ml[1] : ml[0])[row];
+          }
+        }
+        float top = m;
 #pragma unroll
-      for (int f = 0; f < F; ++f) acc[f] *= a;
-      m = top;
-    }
-    const float w = ex2((x.x - m) * p.scale_log2);
-    float sum = w * x.y;
+        for (int b = 0; b < BATCH; ++b) top = fmaxf(top, x[b].x);
+        const float a = ex2((m - top) * p.scale_log2);
+        l *= a;
 #pragma unroll
-    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    l += sum;
-    const int count = min(32, (parts - k0 + 3) / 4);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), i));
-      const float wi = __shfl_sync(0xffffffffu, w, i);
+        for (int f = 0; f < F; ++f) acc[f] *= a;
+        m = top;
 #pragma unroll
-      for (int f = 0; f < F; f += 2) {
-        const float2 y = *reinterpret_cast<const float2*>(from + lane * F + f);
-        acc[f] = fmaf(wi, y.x, acc[f]);
-        acc[f + 1] = fmaf(wi, y.y, acc[f + 1]);
+        for (int b = 0; b < BATCH; ++b) {            // a part that is none has no weight: l is 0 and so is o
+          const float w = ex2((x[b].x - m) * p.scale_log2);
+          l = fmaf(w, x[b].y, l);
+          acc[0] = fmaf(w, o[b].x, acc[0]);
+          acc[1] = fmaf(w, o[b].y, acc[1]);
+          if constexpr (F == 4) {
+            acc[2] = fmaf(w, o[b].z, acc[2]);
+            acc[3] = fmaf(w, o[b].w, acc[3]);
+          }
+        }
       }
     }
-  }
+    if constexpr (WAYS > 1) {
+      if (g < p.G) {
 #pragma unroll
-  for (int f = 0; f < F; ++f) s_o[warp][lane * F + f] = acc[f];
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-  __syncthreads();
-  if (threadIdx.x < DH) {
-    const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float sum = 0.f, o = 0.f;
+        for (int f = 0; f < F; ++f) s_o[slot][way][lane * F + f] = acc[f];
+        if (lane == 0) s_ml[slot][way] = make_float2(m, l);
+      }
+      __syncthreads();
+      if (g < p.G && way == 0) {
+        float top = m;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = ex2((s_m[w] - top) * p.scale_log2);
-      sum = fmaf(a, s_l[w], sum);
-      o = fmaf(a, s_o[w][threadIdx.x], o);
+        for (int w = 1; w < WAYS; ++w) top = fmaxf(top, s_ml[slot][w].x);
+        const float a = ex2((m - top) * p.scale_log2);
+        l *= a;
+#pragma unroll
+        for (int f = 0; f < F; ++f) acc[f] *= a;
+#pragma unroll
+        for (int w = 1; w < WAYS; ++w) {
+          const float2 y = s_ml[slot][w];
+          const float b = ex2((y.x - top) * p.scale_log2);
+          l = fmaf(b, y.y, l);
+#pragma unroll
+          for (int f = 0; f < F; ++f) acc[f] = fmaf(b, s_o[slot][w][lane * F + f], acc[f]);
+        }
+      }
+      __syncthreads();
     }
-    to[threadIdx.x] = __float2bfloat16_rn(sum > 0.f ? o / sum : 0.f);
+    if (g < p.G && way == 0) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      __nv_bfloat16* to = p.out + t * p.ldo + (h * p.G + g) * DH + lane * F;
+      if constexpr (F == 4)
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+      else
+        *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    }
   }
 }
 
@@ -745,21 +1076,32 @@ struct Layout {
     row_pair = limit + (planned ? up(static_cast<size_t>(NT) * 4) : 0);
     whole = row_pair + (planned ? up(static_cast<size_t>(NT) * 4) : 0);
     cut = whole + (shared ? up(static_cast<size_t>(2) * NT * H * (dh + 2) * 4) : 0);
-    total = cut + up(static_cast<size_t>(2) * ctas * BM * (dh + 2) * 4);
+    total = cut + up(static_cast<size_t>(4) * ctas * BM * (dh + 2) * 4);
   }
 };
 
 template <int DH>
-static int launch(const CUtensorMap& tm, const Params& p, int ctas, cudaStream_t s) {
+static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
+  CUtensorMap q_tile, q_token;
+  // (64 columns, the query heads of a kv head, tokens): the rows of a tile in the order in which it has them
+  int rc = make_tmap_3d_bf16_box(&q_tile, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, p.q_tokens);
+  if (!rc) rc = make_tmap_3d_bf16_box(&q_token, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, 1);
+  if (rc) return rc;
   static PerDeviceOnce attr;
-  if (allow_smem(attr, attend_kernel<DH>, Cfg<DH>::SMEM_BYTES, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  if (allow_smem(attr, attend_kernel<DH>, 227 * 1024, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  const int slots = Cfg<DH>::slots(p.q_rows);
+  p.vs = slots / 2;
+  p.ks = slots - p.vs;
   if (p.pair && launch_dep(plan_kernel, dim3(1), dim3(1024), 0, s, p) != cudaSuccess) return SB_ERR_LAUNCH;
-  if (launch_dep(attend_kernel<DH>, dim3(ctas), dim3(THREADS), Cfg<DH>::SMEM_BYTES, s, tm, p) != cudaSuccess) return SB_ERR_LAUNCH;
-  return launch_dep(join_kernel<DH>, dim3(p.NT, p.H), dim3(128), 0, s, p, ctas) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  if (launch_dep(attend_kernel<DH>, dim3(ctas), dim3(THREADS), Cfg<DH>::smem_bytes(p.q_rows), s, tm, q_tile, q_token, p) != cudaSuccess) return SB_ERR_LAUNCH;
+  // few rows have many parts each
+  const bool few = static_cast<long long>(p.NT) * p.Hkv <= 256;
+  return (few ? launch_dep(join_kernel<DH, 4>, dim3(p.NT, p.Hkv), dim3(512), 0, s, p, ctas)
+              : launch_dep(join_kernel<DH, 1>, dim3(p.NT, p.Hkv), dim3(128), 0, s, p, ctas)) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 static int ctas_for(long long units) {
-  const long long most = 2ll * num_sms();
+  const long long most = num_sms();
   return static_cast<int>(units < 1 ? 1 : units < most ? units : most);
 }
 
@@ -768,12 +1110,12 @@ static int ctas_for(long long units) {
 
 using namespace sb;
 
-// Bytes of workspace that sb_shared_prefix_attention needs (16-byte aligned); 0 where it would refuse the sizes.
+// Bytes of workspace that sb_shared_prefix_attention needs (32-byte aligned); 0 where it would refuse the sizes.
 extern "C" size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv, int dh, int ragged, int shared) {
   if (NT <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > spa::BM) return 0;
-  const bool planned = ragged || B > spa::MAX_DIRECT;
-  const int max_pairs = ragged ? B + NT / (spa::BM / (H / Hkv)) : B;
-  return spa::Layout(NT, H, dh, 2 * num_sms(), max_pairs, planned, shared != 0).total;
+  const bool planned = ragged;
+  const int max_pairs = ragged ? B + NT / (2 * (spa::BM / (H / Hkv))) : B;
+  return spa::Layout(NT, H, dh, num_sms(), max_pairs, planned, shared != 0).total;
 }
 
 // q: bf16 [NT, ldq], query heads first, positions already rotated in. pool: n_blocks pages [2, Hkv, page, dh], page a multiple of 8.
@@ -790,7 +1132,7 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
       !(scale > 0.f) || !status || !workspace)
     return SB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (ldq & 7) || (reinterpret_cast<uintptr_t>(out) & 15) || (ldo & 7) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15))
+      (reinterpret_cast<uintptr_t>(workspace) & 31))
     return SB_ERR_ALIGN;
   const uint64_t rows = static_cast<uint64_t>(n_blocks) * 2 * Hkv * page;
   // coordinates of the pool's rows, and of the page behind the last that stands for a bad one; positions; the line of blocks
@@ -798,10 +1140,10 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
       H > 65535)
     return SB_ERR_TOO_LARGE;
   const int G = H / Hkv, TT = spa::BM / G;
-  const bool planned = cu_q || B > spa::MAX_DIRECT;
-  const int max_pairs = cu_q ? B + NT / TT : B;
+  const bool planned = cu_q != nullptr;
+  const int max_pairs = cu_q ? B + NT / (2 * TT) : B;
   const uint64_t cap = static_cast<uint64_t>(max_blocks) * page;
-  if (static_cast<uint64_t>(Hkv) * max_pairs * (cap / spa::BN + 1) + static_cast<uint64_t>(Hkv) * (NT / TT + 1) * (prefix / spa::BN + 1) >=
+  if (static_cast<uint64_t>(Hkv) * max_pairs * (2 * cap / spa::BN + 2 + spa::ITEM_UNITS) + static_cast<uint64_t>(Hkv) * (NT / (2 * TT) + 1) * (2 * prefix / spa::BN + 2 + spa::ITEM_UNITS) >=
       (1ull << 31))
     return SB_ERR_TOO_LARGE;
   const int ctas = spa::ctas_for(max_units);
@@ -818,6 +1160,8 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   p.block_table = block_table; p.max_blocks = max_blocks; p.seq_len = seq_len; p.prefix_table = prefix_table; p.cu_q = cu_q;
   p.prefix = prefix; p.page = page; p.n_blocks = n_blocks; p.box = box;
   p.B = B; p.NT = NT; p.H = H; p.Hkv = Hkv; p.G = G; p.TT = TT;
+  p.q_tokens = NT < TT ? NT : TT;
+  p.q_rows = (G * p.q_tokens + 7) / 8 * 8;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo; p.fill = fill;
   p.hdr = reinterpret_cast<spa::Header*>(ws);

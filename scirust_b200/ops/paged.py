@@ -15,7 +15,7 @@ vp, i32, i64, f32, sz = _lib.vp, _lib.i32, _lib.i64, _lib.f32, _lib.sz
 _lib.register("sb_shared_prefix_attention", [vp, i64, vp, i32, vp, i32, i32, vp, vp, i32, vp, i32, i32, i32, i32, i32, i64, f32, vp, sz,
                                              vp, i64, i32, vp, vp])
 
-TILE_ROWS, BLOCK = 128, 64          # rows of a tile, positions of a block of keys
+TILE_ROWS, BLOCK = 128, 128          # rows of a tile, positions of a block of keys
 
 
 def shared_prefix_attention_ref(q, pool, block_table, page, seq_len, prefix_table, prefix_len, H, Hkv, dh, scale=None, cu_q=None):
@@ -127,5 +127,5 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
               page, seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
               B, n, H, Hkv, dh, units, scale, ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(0), int(fill),
               _lib.status_word(device).data_ptr(), _lib.stream())
-    _g.launch_count += 2 if cu_q is None and B <= 1024 else 3
+    _g.launch_count += 2 if cu_q is None else 3
     return out

@@ -70,7 +70,7 @@ def test_entry_point_refuses():
     """Sizes and pointers are looked at before anything is launched."""
     from scirust_b200.ops import _lib
     ok = dict(q=16, ldq=256, pool=16, n_blocks=4, table=16, max_blocks=4, page=64, seq_len=16, prefix_table=16, prefix=64, cu=None, B=2, NT=2,
-              H=4, Hkv=2, dh=64, units=4, scale=0.125, ws=16, ws_bytes=1 << 30, out=16, ldo=256, fill=1, status=16, stream=None)
+              H=4, Hkv=2, dh=64, units=4, scale=0.125, ws=32, ws_bytes=1 << 30, out=16, ldo=256, fill=1, status=16, stream=None)
     for change, what in ((dict(B=0), "bad argument"), (dict(NT=3), "bad argument"), (dict(H=5), "bad argument"), (dict(dh=96), "bad argument"),
                          (dict(page=12), "bad argument"), (dict(page=4), "bad argument"), (dict(prefix=32), "bad argument"),
                          (dict(prefix_table=None), "bad argument"), (dict(scale=0.0), "bad argument"), (dict(scale=float("nan")), "bad argument"),

@@ -60,6 +60,15 @@ def statement(a, scale=None):
     return o.reshape(n, -1), bound.reshape(n, -1)
 
 
+@pytest.fixture(autouse=True)
+def _poisoned(monkeypatch):
+    """Workspaces and answers begin as NaN and between fences, so that a part which is read and was not written shows."""
+    monkeypatch.setattr(_lib, "DEBUG_POISON", True)
+    yield
+    torch.cuda.synchronize()
+    _lib.check_canaries()
+
+
 def check(a, **kw):
     out = paged.shared_prefix_attention(**a, **kw)
     _lib.check_status(out.device)
@@ -227,3 +236,13 @@ def test_what_a_bound_of_the_lengths_is_for():
     """max_len sizes the launch; lengths beyond it are still answered."""
     a = batch(3, 16, 4, 64, 64, 256, [300, 5, 700])
     assert torch.allclose(check(a, max_len=1).float(), check(a).float(), atol=0.05)
+
+
+@pytest.mark.parametrize("B,tail", [(16, 256), (33, 400), (64, 512), (300, 130)])
+def test_many_short_pieces_a_cta(B, tail):
+    """CTAs that go from piece to piece, of one block and of several, of one tile of rows and of two."""
+    g = torch.Generator().manual_seed(B)
+    tails = torch.randint(1, tail, (B,), generator=g).tolist()
+    check(batch(B, 32, 8, 128, 64, 1000, tails))
+    new = [min(t, 1 + b % 70) for b, t in enumerate(tails)]
+    check(batch(B, 8, 2, 64, 16, 300, tails, new))
