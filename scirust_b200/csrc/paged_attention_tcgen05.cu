@@ -88,6 +88,7 @@ struct Params {
   int prefix;          // shared positions: whole pages; 0 where every sequence's own items start at 0
   int page, n_blocks, box;
   int B, NT, H, Hkv, G, TT;
+  int split;           // a row has four parts of an item, one of every fourth of a block's positions: 1 those of its own, 2 of both
   int q_tokens;        // of the box that brings a tile of rows
   int q_rows;          // of a tile in shared memory, a multiple of 8; the tensor core reads 128, those behind are rows of no one
   int ks, vs;          // blocks of K and V in shared memory
@@ -100,7 +101,7 @@ struct Params {
   Pair* pair;
   int* row_limit;      // [NT]
   int* row_pair;       // [NT], -1: of no sequence
-  float* whole;        // [2][NT][H][dh], and [2][NT][H][2] behind it: items that were not cut
+  float* whole;        // [slots][NT][H][dh], and [slots][NT][H][2] behind it: items that were not cut, shared and then own
   float* cut;          // [2 * CTAs][256][dh], and [2 * CTAs][256][2] behind it: first and last pieces of the CTAs
   int max_pairs;
   int* status;
@@ -206,6 +207,16 @@ constexpr int PIECE_SHARED = 1, PIECE_CUT = 2, PIECE_FIRST = 4, PIECE_SHORT = 8,
 
 // A CTA's pieces, found by a whole warp. The plan of a batch of one token a sequence is summed up on the way, 32 sequences at a time;
 // anything else has been planned (plan_kernel).
+// Slots of the rows of items that were not cut: of shared items, then of own ones.
+__host__ __device__ __forceinline__ int own_slot(const Params& p) { return p.prefix == 0 ? 0 : p.split & 2 ? 4 : 1; }
+__host__ __device__ __forceinline__ int whole_slots(const Params& p) { return own_slot(p) + (p.split ? 4 : 1); }
+
+// Whether the four quarters of the tile (the softmax warps of a lane) have the same rows, up to eight, and a fourth of the positions of
+// each block: the few rows of a sequence of one token would keep one warp of a lane busy, and both lanes' on one scheduler.
+__device__ __forceinline__ bool is_split(const Params& p, const Piece& x) {
+  return (x.flags & PIECE_SHARED ? p.split & 2 : p.split & 1) != 0;
+}
+
 struct Walk {
   const Params& p;
   const Shared shared;
@@ -622,6 +633,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       const int half = n_pieces & 1;
       const bool two = same(x.n_tok > p.TT ? 1 : 0);
       const int n = same((x.j1 - x.j0) << (two ? 1 : 0));
+      // eight rows for every eight of the tile, where its four quarters take the same rows
+      const uint64_t desc_q = desc & ~(same(is_split(p, x) ? 1 : 0) ? 0x3fffull << 32 : 0ull);
       ok = wait(&q_full[half], (n_pieces >> 1) & 1, p.status, ST_TIMEOUT_MISC);
 #pragma unroll 1
       for (int i = 0; i < n && ok; ++i, ++steps) {
@@ -637,7 +650,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         if (leader) {
 #pragma unroll
           for (int k = 0; k < DH / 16; ++k)
-            umma_bf16_ss(to, desc | (q_lo + (k >> 2) * chunk + (k & 3) * 2), desc | (k_lo + (k >> 2) * (BN * 8) + (k & 3) * 2), idesc,
+            umma_bf16_ss(to, desc_q | (q_lo + (k >> 2) * chunk + (k & 3) * 2), desc | (k_lo + (k >> 2) * (BN * 8) + (k & 3) * 2), idesc,
                          k > 0 ? 1u : 0u);
           umma_commit(&s_full[L]);
           if (frees) umma_commit(&k_empty[ks]);
@@ -713,7 +726,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int L = (warp >> 2) - 1;         // lane
     const int quarter = warp & 3;          // lanes of tensor memory that this warp may read
     const int r = quarter * 32 + lane;     // row of the tile
-    const int row_tok = quotient(r, p.G), g = r - row_tok * p.G;
+    const int tile_tok = quotient(r, p.G), tile_g = r - tile_tok * p.G;
+    const int lane_tok = quotient(lane, p.G), lane_g = lane - lane_tok * p.G;      // split
     const uint32_t tm = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t tm_S = tm + (C::SB == 1 ? 0 : L * BN), tm_P = tm + C::COL_P + L * (BN / 2), tm_O = tm + C::COL_O + L * DH;
     const float sl2 = p.scale_log2;
@@ -725,8 +739,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       const int first = two ? 0 : (L ^ steps) & 1, step = two ? 1 : 2;           // this lane's blocks
       steps += two ? 2 * nb : nb;
       if (first >= nb) continue;
+      const bool split = is_split(p, x);
+      const int row_tok = split ? lane_tok : tile_tok, g = split ? lane_g : tile_g;
       const int toks = two ? min(p.TT, x.n_tok - L * p.TT) : x.n_tok, tok = row_tok + (two ? L * p.TT : 0);
-      const bool active = quarter * 32 < toks * p.G;      // whether any row of this warp counts
+      const bool active = split || quarter * 32 < toks * p.G;      // whether any row of this warp counts
       const bool valid = row_tok < toks;
       const int t = x.t0 + tok;
       // positions that the row sees of this piece's
@@ -754,74 +770,111 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           continue;
         }
         tc_fence_after();
-        uint32_t v[BN];
-        __syncwarp();
-#pragma unroll
-        for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32_converged(tm_S + c * 32, v + c * 32);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
         const int lim = limit - (x.kbase + (x.j0 + i) * BN);          // columns from here on are masked
-        const int live = x.kend - (x.kbase + (x.j0 + i) * BN);        // for every row
-        if (__any_sync(0xffffffffu, lim < BN)) {
-#pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (c >= lim) v[c] = 0xff800000u;
-        }
-        float m4[4] = {LOWEST, LOWEST, LOWEST, LOWEST};
-#pragma unroll
-        for (int c = 0; c < BN; c += 2)
-          m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-        const float m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        const bool grow = (m_blk - m_ref) * sl2 > RESCALE_GAP || m_ref == LOWEST;
-        const float alpha = grow ? ex2((m_ref - m_blk) * sl2) : 1.f;
-        if (grow) m_ref = m_blk;
-        const float neg_m = -m_ref;
-        if (n > 0) {                       // P V of the block before has read P and updated O
-          wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
-          tc_fence_after();
-          if (i > first && __any_sync(0xffffffffu, grow)) {
+        float m_blk, sum4[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        // The row's reference for this block, P V of the lane's block before, which frees P, and O, if the reference has moved; the factor
+        // of what the row has so far.
+        auto turn = [&]() -> float {
+          const bool grow = (m_blk - m_ref) * sl2 > RESCALE_GAP || m_ref == LOWEST;
+          const float alpha = grow ? ex2((m_ref - m_blk) * sl2) : 1.f;
+          if (grow) m_ref = m_blk;
+          if (n > 0) {
+            wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+            tc_fence_after();
+            if (i > first && __any_sync(0xffffffffu, grow)) {
 #pragma unroll 1
-            for (int c = 0; c < DH / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32_converged(tm_O + c * 32, o);
-              tmem_ld_wait();
+              for (int c = 0; c < DH / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32_converged(tm_O + c * 32, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) mul2(o[e], o[e + 1], alpha, alpha);
-              tmem_st_32x32_converged(tm_O + c * 32, o);
+                for (int e = 0; e < 32; e += 2) mul2(o[e], o[e + 1], alpha, alpha);
+                tmem_st_32x32_converged(tm_O + c * 32, o);
+              }
             }
           }
-        }
-        if (pending) {                     // O of the piece before is about to be overwritten
-          wait(&o_free[quarter], (n_join - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
-          pending = false;
-        }
-        float sum4[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == 1 && live <= HALF) {    // nothing of it is multiplied
-            if (lane == 0) mbar_arrive(&p_full[2 * L + 1]);
-            break;
+          if (pending) {                   // O of the piece before is about to be overwritten
+            wait(&o_free[quarter], (n_join - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
+            pending = false;
           }
-          uint32_t pk[HALF / 2];
+          return alpha;
+        };
+        // Weights of two columns, as bf16. Scores are subtracted before they are scaled: one fused step leaves the rounding of scale * m
+        // between a row's largest score and zero, which is everything once scores are beyond 2^24.
+        auto weigh = [&](uint32_t& a, uint32_t& b, int c) -> uint32_t {
+          fma2(a, b, 1.f, -m_ref);
+          mul2(a, b, sl2, sl2);
+          const uint32_t w = pack_bf16x2(ex2(__uint_as_float(a)), ex2(__uint_as_float(b)));
+          add2(sum4[c & 6], sum4[(c & 6) + 1], w << 16, w & 0xffff0000u);
+          return w;
+        };
+        float alpha;
+        if (split) {
+          uint32_t v[32];
+          tmem_ld_32x32(tm_S + quarter * 32, v);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
+          m_blk = LOWEST;
 #pragma unroll
-          for (int c2 = 0; c2 < HALF; c2 += 2) {
-            const int c = h * HALF + c2;
-            // Subtracted before it is scaled: one fused step leaves the rounding of scale * m between a row's largest score and zero,
-            // which is everything once scores are beyond 2^24.
-            fma2(v[c], v[c + 1], 1.f, neg_m);
-            mul2(v[c], v[c + 1], sl2, sl2);
-            const float e0 = ex2(__uint_as_float(v[c])), e1 = ex2(__uint_as_float(v[c + 1]));
-            const uint32_t w = pack_bf16x2(e0, e1);
-            add2(sum4[c & 6], sum4[(c & 6) + 1], w << 16, w & 0xffff0000u);
-            pk[c2 >> 1] = w;
+          for (int c = 0; c < 32; c += 2) {
+            if (quarter * 32 + c >= lim) v[c] = 0xff800000u;
+            if (quarter * 32 + c + 1 >= lim) v[c + 1] = 0xff800000u;
+            m_blk = max3(m_blk, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
           }
-          tmem_st_32x32(tm_P + h * (HALF / 2), pk);
+          alpha = turn();
+          uint32_t pk[32];
+          if (i == first) {                // the weights of the others' positions stay zero
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pk[c] = 0;
+            tmem_st_32x32(tm_P, pk);
+            tmem_st_32x32(tm_P + 32, pk);
+            tmem_st_wait();
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) pk[c >> 1] = weigh(v[c], v[c + 1], c);
+          tmem_st_32x16(tm_P + quarter * 16, pk);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * L + h]);
+          if (lane == 0) { mbar_arrive(&p_full[2 * L]); mbar_arrive(&p_full[2 * L + 1]); }
+        } else {
+          uint32_t v[BN];
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32_converged(tm_S + c * 32, v + c * 32);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
+          if (__any_sync(0xffffffffu, lim < BN)) {
+#pragma unroll
+            for (int c = 0; c < BN; ++c)
+              if (c >= lim) v[c] = 0xff800000u;
+          }
+          float m4[4] = {LOWEST, LOWEST, LOWEST, LOWEST};
+#pragma unroll
+          for (int c = 0; c < BN; c += 2)
+            m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+          m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          alpha = turn();
+          const int live = x.kend - (x.kbase + (x.j0 + i) * BN);      // positions that any row sees
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && live <= HALF) {    // nothing of it is multiplied
+              if (lane == 0) mbar_arrive(&p_full[2 * L + 1]);
+              break;
+            }
+            uint32_t pk[HALF / 2];
+#pragma unroll
+            for (int c2 = 0; c2 < HALF; c2 += 2) pk[c2 >> 1] = weigh(v[h * HALF + c2], v[h * HALF + c2 + 1], h * HALF + c2);
+            tmem_st_32x32(tm_P + h * (HALF / 2), pk);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * L + h]);
+          }
         }
         const float sum = ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) + ((sum4[4] + sum4[5]) + (sum4[6] + sum4[7]));
         l = __fadd_rn(__fmul_rn(l, alpha), sum);
@@ -852,7 +905,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       }
       const int head = x.h * p.G + g;
       const bool cut = x.flags & PIECE_CUT;
-      const bool out_now = !cut && p.prefix == 0;
+      const bool out_now = !cut && p.prefix == 0 && !split;
       float* to = nullptr;
       if (valid && !out_now) {
         size_t row, rows;
@@ -862,8 +915,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           rows = static_cast<size_t>(2) * gridDim.x * (2 * BM);
           base = p.cut;
         } else {
-          row = (static_cast<size_t>(x.flags & PIECE_SHARED ? 0 : p.NT) + t) * p.H + head;
-          rows = static_cast<size_t>(2) * p.NT * p.H;
+          const int slot = (x.flags & PIECE_SHARED ? 0 : own_slot(p)) + (split ? quarter : 0);
+          row = (static_cast<size_t>(slot) * p.NT + t) * p.H + head;
+          rows = static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
           base = p.whole;
         }
         to = base + row * DH;
@@ -944,6 +998,7 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
   const float* from[2];
   const float2* ml[2];
   int jump[2];                             // rows from the first part to the second, which is 4 * BM in front of the third
+  int fold[2], apart[2];                   // log2 of the parts that a CTA has of an item, rows between them
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
     int beg, size, t0, tokens;
@@ -962,6 +1017,7 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
       tokens = p.pair ? p.pair[pair].n : 1;
     }
     const int two = tokens > p.TT ? 1 : 0, tok = t - t0;
+    const int log = p.split & (i ? 1 : 2) ? 2 : 0;
     int count = 0, skip = 0;
     size_t at = 0;
     bool cut = false;
@@ -972,16 +1028,17 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
       const bool odd = deal.begin(c0) < beg;         // the second piece of its CTA
       skip = odd ? 2 * BM : 4 * BM;
       at = cut ? static_cast<size_t>(2 * c0 + (odd ? 1 : 0)) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
-               : (static_cast<size_t>(i ? p.NT : 0) + t) * p.H + h * p.G;
+               : (static_cast<size_t>(i ? own_slot(p) : 0) * p.NT + t) * p.H + h * p.G;
     }
-    const size_t rows = cut ? static_cast<size_t>(4) * ctas * BM : static_cast<size_t>(2) * p.NT * p.H;
+    const size_t rows = cut ? static_cast<size_t>(4) * ctas * BM : static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
     const float* base = cut ? p.cut : p.whole;
     const float* o = base + at * DH + lane * F;
     const float2* m = reinterpret_cast<const float2*>(base + rows * DH) + at;
-    if (i == 0) { n[0] = count; from[0] = o; ml[0] = m; jump[0] = skip; }
-    else { n[1] = count; from[1] = o; ml[1] = m; jump[1] = skip; }
+    const int gap = cut ? 32 : p.NT * p.H;
+    if (i == 0) { n[0] = count << log; from[0] = o; ml[0] = m; jump[0] = skip; fold[0] = log; apart[0] = gap; }
+    else { n[1] = count << log; from[1] = o; ml[1] = m; jump[1] = skip; fold[1] = log; apart[1] = gap; }
   }
-  if (p.prefix == 0 && n[1] == 1) return;  // written out by its CTA
+  if (p.prefix == 0 && !p.split && n[1] == 1) return;  // written out by its CTA
   const int parts = n[0] + n[1];
 #pragma unroll 1
   for (int g0 = 0; g0 < p.G; g0 += ROWS) {
@@ -998,8 +1055,8 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
         for (int b = 0; b < BATCH; ++b) {
           const int k = k0 + b * WAYS;
           const bool own = k >= n[0];
-          const int c = own ? k - n[0] : k;
-          const int row = g + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
+          const int e = own ? k - n[0] : k, c = e >> (own ? fold[1] : fold[0]), f = e - (c << (own ? fold[1] : fold[0]));
+          const int row = g + f * (own ? apart[1] : apart[0]) + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
           x[b] = make_float2(LOWEST, 0.f);
           o[b] = Vec{};
           if (k < parts) {
@@ -1068,14 +1125,14 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
 // Bytes of the parts of the workspace, in the order in which they lie.
 struct Layout {
   size_t cum, pair, limit, row_pair, whole, cut, total;
-  Layout(long long NT, int H, int dh, int ctas, int max_pairs, bool planned, bool shared) {
+  Layout(long long NT, int H, int dh, int ctas, int max_pairs, bool planned, int slots) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     cum = up(sizeof(Header));
     pair = cum + up((static_cast<size_t>(max_pairs) + 1) * 4);
     limit = pair + (planned ? up(static_cast<size_t>(max_pairs) * sizeof(Pair)) : 0);
     row_pair = limit + (planned ? up(static_cast<size_t>(NT) * 4) : 0);
     whole = row_pair + (planned ? up(static_cast<size_t>(NT) * 4) : 0);
-    cut = whole + (shared ? up(static_cast<size_t>(2) * NT * H * (dh + 2) * 4) : 0);
+    cut = whole + up(static_cast<size_t>(slots) * NT * H * (dh + 2) * 4);
     total = cut + up(static_cast<size_t>(4) * ctas * BM * (dh + 2) * 4);
   }
 };
@@ -1110,12 +1167,23 @@ static int ctas_for(long long units) {
 
 using namespace sb;
 
+// What the sizes of a call decide.
+static void sizes(spa::Params& p, int NT, int B, int H, int Hkv, int prefix, bool ragged) {
+  p.B = B; p.NT = NT; p.H = H; p.Hkv = Hkv; p.prefix = prefix;
+  p.G = H / Hkv; p.TT = spa::BM / p.G;
+  p.q_tokens = NT < p.TT ? NT : p.TT;
+  p.q_rows = (p.G * p.q_tokens + 7) / 8 * 8;
+  p.max_pairs = ragged ? B + NT / (2 * p.TT) : B;
+  p.split = ragged || p.G > 8 ? 0 : NT * p.G > 8 ? 1 : 3;
+}
+static int slots_of(const spa::Params& p) { return p.prefix > 0 || p.split ? spa::whole_slots(p) : 0; }
+
 // Bytes of workspace that sb_shared_prefix_attention needs (32-byte aligned); 0 where it would refuse the sizes.
-extern "C" size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv, int dh, int ragged, int shared) {
+extern "C" size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv, int dh, int ragged, int prefix) {
   if (NT <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > spa::BM) return 0;
-  const bool planned = ragged;
-  const int max_pairs = ragged ? B + NT / (2 * (spa::BM / (H / Hkv))) : B;
-  return spa::Layout(NT, H, dh, num_sms(), max_pairs, planned, shared != 0).total;
+  spa::Params p;
+  sizes(p, NT, B, H, Hkv, prefix, ragged != 0);
+  return spa::Layout(NT, H, dh, num_sms(), p.max_pairs, ragged != 0, slots_of(p)).total;
 }
 
 // q: bf16 [NT, ldq], query heads first, positions already rotated in. pool: n_blocks pages [2, Hkv, page, dh], page a multiple of 8.
@@ -1139,15 +1207,16 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   if (rows + 2ull * Hkv * page >= (1ull << 31) || static_cast<uint64_t>(max_blocks) * page >= (1ull << 30) ||
       H > 65535)
     return SB_ERR_TOO_LARGE;
-  const int G = H / Hkv, TT = spa::BM / G;
   const bool planned = cu_q != nullptr;
-  const int max_pairs = cu_q ? B + NT / (2 * TT) : B;
+  spa::Params p;
+  sizes(p, NT, B, H, Hkv, prefix, planned);
+  const int TT = p.TT, max_pairs = p.max_pairs;
   const uint64_t cap = static_cast<uint64_t>(max_blocks) * page;
   if (static_cast<uint64_t>(Hkv) * max_pairs * (2 * cap / spa::BN + 2 + spa::ITEM_UNITS) + static_cast<uint64_t>(Hkv) * (NT / (2 * TT) + 1) * (2 * prefix / spa::BN + 2 + spa::ITEM_UNITS) >=
       (1ull << 31))
     return SB_ERR_TOO_LARGE;
   const int ctas = spa::ctas_for(max_units);
-  const spa::Layout at(NT, H, dh, ctas, max_pairs, planned, prefix > 0);
+  const spa::Layout at(NT, H, dh, ctas, max_pairs, planned, slots_of(p));
   if (at.total > workspace_bytes) return SB_ERR_ARG;
   int box = 64;
   while (page % box) box >>= 1;
@@ -1155,13 +1224,9 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   const int rc = make_tmap_2d_bf16(&tm, pool, dh, rows, dh, 64, box);
   if (rc) return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  spa::Params p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq;
   p.block_table = block_table; p.max_blocks = max_blocks; p.seq_len = seq_len; p.prefix_table = prefix_table; p.cu_q = cu_q;
-  p.prefix = prefix; p.page = page; p.n_blocks = n_blocks; p.box = box;
-  p.B = B; p.NT = NT; p.H = H; p.Hkv = Hkv; p.G = G; p.TT = TT;
-  p.q_tokens = NT < TT ? NT : TT;
-  p.q_rows = (G * p.q_tokens + 7) / 8 * 8;
+  p.page = page; p.n_blocks = n_blocks; p.box = box;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo; p.fill = fill;
   p.hdr = reinterpret_cast<spa::Header*>(ws);
@@ -1171,7 +1236,6 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   p.row_pair = planned ? reinterpret_cast<int*>(ws + at.row_pair) : nullptr;
   p.whole = reinterpret_cast<float*>(ws + at.whole);
   p.cut = reinterpret_cast<float*>(ws + at.cut);
-  p.max_pairs = max_pairs;
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dh == 64 ? spa::launch<64>(tm, p, ctas, s) : spa::launch<128>(tm, p, ctas, s);

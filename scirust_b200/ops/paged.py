@@ -46,10 +46,10 @@ def shared_prefix_attention_ref(q, pool, block_table, page, seq_len, prefix_tabl
 
 
 @functools.lru_cache(maxsize=4096)       # a function of the device and the sizes
-def _workspace_bytes(device, NT, B, H, Hkv, dh, ragged, shared):
+def _workspace_bytes(device, NT, B, H, Hkv, dh, ragged, prefix):
     fn = _lib.cuda().sb_shared_prefix_attention_bytes
     fn.argtypes, fn.restype = [i32] * 7, sz
-    return fn(NT, B, H, Hkv, dh, int(ragged), int(shared))
+    return fn(NT, B, H, Hkv, dh, int(ragged), prefix)
 
 
 def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, prefix_len, H, Hkv, dh, scale=None, cu_q=None,
@@ -122,7 +122,7 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     pairs = B if cu_q is None else B + n // per_tile
     L = max_blocks * page if max_len is None else min(int(max_len), max_blocks * page)
     units = Hkv * (tiles * -(-prefix // BLOCK) + pairs * max(0, -(-(L - prefix) // BLOCK)))
-    ws = _lib.empty(_workspace_bytes(device, n, B, H, Hkv, dh, cu_q is not None, prefix > 0), torch.uint8, device)
+    ws = _lib.empty(_workspace_bytes(device, n, B, H, Hkv, dh, cu_q is not None, prefix), torch.uint8, device)
     _lib.call("sb_shared_prefix_attention", q.data_ptr(), q.stride(0), pool.data_ptr(), pool.shape[0], block_table.data_ptr(), max_blocks,
               page, seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
               B, n, H, Hkv, dh, units, scale, ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(0), int(fill),
