@@ -90,6 +90,7 @@ struct Params {
   int B, NT, H, Hkv, G, TT;
   int split;           // a row has four parts of an item, one of every fourth of a block's positions: 1 those of its own, 2 of both
   int q_tokens;        // of the box that brings a tile of rows
+  int by_token;        // whether there is a box of one token too
   int q_rows;          // of a tile in shared memory, a multiple of 8; the tensor core reads 128, those behind are rows of no one
   int ks, vs;          // blocks of K and V in shared memory
   float scale_log2;
@@ -593,7 +594,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         both = two;
         if (ok && lane == 0) {
           // The box of a tile brings its tokens and, behind the last of them, rows of others that no one reads.
-          const bool one = x.n_tok == 1;
+          const bool one = x.n_tok == 1 && p.by_token;
           const int tiles = two ? 2 : 1, bytes = (one ? 1 : p.q_tokens) * p.G * 128;
           uint64_t* bar = &q_full[n_pieces & 1];
           mbar_arrive_expect_tx(bar, tiles * C::NCH * bytes);
@@ -971,24 +972,29 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
 }
 
-// Joins the parts of a row. A CTA has the heads of a (token, kv head), which have the same parts; WAYS warps share those of a row and
-// read a batch at a time, and their sums meet in shared memory.
-template <int DH, int WAYS>
+// Joins the parts of rows. The heads of a (token, kv head) have the same parts, so they are looked up once. PACKED, for many rows of few
+// parts: a warp has the rows of a (token, kv head), two at a time, and a CTA four of these. Otherwise a CTA has them, four at a time, a
+// row to WAYS warps, which share its parts; their sums meet in shared memory.
+template <int DH, int WAYS, bool PACKED>
 __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant__ Params p, int ctas) {
   constexpr int F = DH / 32;               // columns of a lane
-  constexpr int ROWS = 4, BATCH = WAYS > 1 ? 4 : 8;       // rows, parts at a time
+  static_assert(WAYS == 1 || !PACKED, "");
+  constexpr int ROWS = PACKED ? 1 : 4, AT_ONCE = PACKED ? 2 : 1, BATCH = PACKED || WAYS > 1 ? 4 : 8;       // rows a CTA, a warp; parts at a time
   using Vec = typename std::conditional<F == 4, float4, float2>::type;
   __shared__ float s_o[WAYS > 1 ? ROWS : 1][WAYS][DH];
   __shared__ float2 s_ml[ROWS][WAYS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS, slot = warp / WAYS;
-  const int t = blockIdx.x, h = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS, slot = PACKED ? 0 : warp / WAYS;
+  const int job = PACKED ? blockIdx.x * 4 + warp : blockIdx.x;
+  const int t = quotient(job, p.Hkv), h = job - t * p.Hkv;
   pdl_trigger();
   pdl_wait();
+  if (t >= p.NT) return;
   const int pair = p.pair ? p.row_pair[t] : t;
   const int units = p.hdr->units, units_shared = p.hdr->units_shared, q_lo = p.hdr->q_lo, q_hi = p.hdr->q_hi;
   if (pair < 0) {                          // a row of no sequence
     if (p.fill)
-      for (int i = threadIdx.x; i < p.G * DH; i += 128 * WAYS) p.out[t * p.ldo + h * p.G * DH + i] = __float2bfloat16_rn(0.f);
+      for (int i = PACKED ? lane : threadIdx.x; i < p.G * DH; i += PACKED ? 32 : 32 * ROWS * WAYS)
+        p.out[t * p.ldo + h * p.G * DH + i] = __float2bfloat16_rn(0.f);
     return;
   }
   const Deal deal(units, ctas);
@@ -1041,83 +1047,96 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
   if (p.prefix == 0 && !p.split && n[1] == 1) return;  // written out by its CTA
   const int parts = n[0] + n[1];
 #pragma unroll 1
-  for (int g0 = 0; g0 < p.G; g0 += ROWS) {
-    const int g = g0 + slot;
-    float m = LOWEST, l = 0.f, acc[F];
+  for (int g0 = 0; g0 < p.G; g0 += ROWS * AT_ONCE) {
+    const int g = g0 + slot;               // this warp's rows: g, and g + 1
+    float m[AT_ONCE], l[AT_ONCE], acc[AT_ONCE][F];
 #pragma unroll
-    for (int f = 0; f < F; ++f) acc[f] = 0.f;
-    if (g < p.G) {
+    for (int r = 0; r < AT_ONCE; ++r) {
+      m[r] = LOWEST;
+      l[r] = 0.f;
+#pragma unroll
+      for (int f = 0; f < F; ++f) acc[r][f] = 0.f;
+    }
 #pragma unroll 1
-      for (int k0 = way; k0 < parts; k0 += WAYS * BATCH) {
-        Vec o[BATCH];
-        float2 x[BATCH];
+    for (int k0 = way; k0 < parts; k0 += WAYS * BATCH) {
+      Vec o[AT_ONCE][BATCH];
+      float2 x[AT_ONCE][BATCH];
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-          const int k = k0 + b * WAYS;
-          const bool own = k >= n[0];
-          const int e = own ? k - n[0] : k, c = e >> (own ? fold[1] : fold[0]), f = e - (c << (own ? fold[1] : fold[0]));
-          const int row = g + f * (own ? apart[1] : apart[0]) + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
-          x[b] = make_float2(LOWEST, 0.f);
-          o[b] = Vec{};
-          if (k < parts) {
-            o[b] = *reinterpret_cast<const Vec*>((own ? from[1] : from[0]) + static_cast<size_t>(row) * DH);
-            x[b] = (own ? ml[1] : ml[0])[row];
+      for (int b = 0; b < BATCH; ++b) {
+        const int k = k0 + b * WAYS;
+        const bool own = k >= n[0];
+        const int e = own ? k - n[0] : k, log = own ? fold[1] : fold[0], c = e >> log;
+        const int row = g + (e - (c << log)) * (own ? apart[1] : apart[0]) + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
+        const float* at_o = (own ? from[1] : from[0]) + static_cast<long long>(row) * DH;
+        const float2* at_ml = (own ? ml[1] : ml[0]) + row;
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r) {
+          x[r][b] = make_float2(LOWEST, 0.f);
+          o[r][b] = Vec{};
+          if (k < parts && g + r < p.G) {
+            o[r][b] = *reinterpret_cast<const Vec*>(at_o + r * DH);
+            x[r][b] = at_ml[r];
           }
         }
-        float top = m;
+      }
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) top = fmaxf(top, x[b].x);
-        const float a = ex2((m - top) * p.scale_log2);
-        l *= a;
+      for (int r = 0; r < AT_ONCE; ++r) {
+        float top = m[r];
 #pragma unroll
-        for (int f = 0; f < F; ++f) acc[f] *= a;
-        m = top;
+        for (int b = 0; b < BATCH; ++b) top = fmaxf(top, x[r][b].x);
+        const float a = ex2((m[r] - top) * p.scale_log2);
+        l[r] *= a;
+#pragma unroll
+        for (int f = 0; f < F; ++f) acc[r][f] *= a;
+        m[r] = top;
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {            // a part that is none has no weight: l is 0 and so is o
-          const float w = ex2((x[b].x - m) * p.scale_log2);
-          l = fmaf(w, x[b].y, l);
-          acc[0] = fmaf(w, o[b].x, acc[0]);
-          acc[1] = fmaf(w, o[b].y, acc[1]);
+          const float w = ex2((x[r][b].x - top) * p.scale_log2);
+          l[r] = fmaf(w, x[r][b].y, l[r]);
+          acc[r][0] = fmaf(w, o[r][b].x, acc[r][0]);
+          acc[r][1] = fmaf(w, o[r][b].y, acc[r][1]);
           if constexpr (F == 4) {
-            acc[2] = fmaf(w, o[b].z, acc[2]);
-            acc[3] = fmaf(w, o[b].w, acc[3]);
+            acc[r][2] = fmaf(w, o[r][b].z, acc[r][2]);
+            acc[r][3] = fmaf(w, o[r][b].w, acc[r][3]);
           }
         }
       }
     }
     if constexpr (WAYS > 1) {
-      if (g < p.G) {
 #pragma unroll
-        for (int f = 0; f < F; ++f) s_o[slot][way][lane * F + f] = acc[f];
-        if (lane == 0) s_ml[slot][way] = make_float2(m, l);
-      }
+      for (int f = 0; f < F; ++f) s_o[slot][way][lane * F + f] = acc[0][f];
+      if (lane == 0) s_ml[slot][way] = make_float2(m[0], l[0]);
       __syncthreads();
-      if (g < p.G && way == 0) {
-        float top = m;
+      if (way == 0) {
+        float top = m[0];
 #pragma unroll
         for (int w = 1; w < WAYS; ++w) top = fmaxf(top, s_ml[slot][w].x);
-        const float a = ex2((m - top) * p.scale_log2);
-        l *= a;
+        const float a = ex2((m[0] - top) * p.scale_log2);
+        l[0] *= a;
 #pragma unroll
-        for (int f = 0; f < F; ++f) acc[f] *= a;
-#pragma unroll
+        for (int f = 0; f < F; ++f) acc[0][f] *= a;
+#pragma unroll 1
         for (int w = 1; w < WAYS; ++w) {
           const float2 y = s_ml[slot][w];
           const float b = ex2((y.x - top) * p.scale_log2);
-          l = fmaf(b, y.y, l);
+          l[0] = fmaf(b, y.y, l[0]);
 #pragma unroll
-          for (int f = 0; f < F; ++f) acc[f] = fmaf(b, s_o[slot][w][lane * F + f], acc[f]);
+          for (int f = 0; f < F; ++f) acc[0][f] = fmaf(b, s_o[slot][w][lane * F + f], acc[0][f]);
         }
       }
       __syncthreads();
     }
-    if (g < p.G && way == 0) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      __nv_bfloat16* to = p.out + t * p.ldo + (h * p.G + g) * DH + lane * F;
-      if constexpr (F == 4)
-        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-      else
-        *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+    for (int r = 0; r < AT_ONCE; ++r) {
+      if (g + r < p.G && way == 0) {
+        const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+        __nv_bfloat16* to = p.out + t * p.ldo + (h * p.G + g + r) * DH + lane * F;
+        if constexpr (F == 4)
+          *reinterpret_cast<uint2*>(to) =
+              make_uint2(pack_bf16x2(acc[r][0] * inv, acc[r][1] * inv), pack_bf16x2(acc[r][2] * inv, acc[r][3] * inv));
+        else
+          *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(acc[r][0] * inv, acc[r][1] * inv);
+      }
     }
   }
 }
@@ -1142,8 +1161,11 @@ static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
   CUtensorMap q_tile, q_token;
   // (64 columns, the query heads of a kv head, tokens): the rows of a tile in the order in which it has them
   int rc = make_tmap_3d_bf16_box(&q_tile, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, p.q_tokens);
-  if (!rc) rc = make_tmap_3d_bf16_box(&q_token, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, 1);
+  // a map takes a microsecond to make: up to eight tokens a box of one saves less
+  p.by_token = p.q_tokens > 8;
+  if (!rc && p.by_token) rc = make_tmap_3d_bf16_box(&q_token, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, 1);
   if (rc) return rc;
+  if (!p.by_token) q_token = q_tile;
   static PerDeviceOnce attr;
   if (allow_smem(attr, attend_kernel<DH>, 227 * 1024, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
   const int slots = Cfg<DH>::slots(p.q_rows);
@@ -1151,10 +1173,11 @@ static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
   p.ks = slots - p.vs;
   if (p.pair && launch_dep(plan_kernel, dim3(1), dim3(1024), 0, s, p) != cudaSuccess) return SB_ERR_LAUNCH;
   if (launch_dep(attend_kernel<DH>, dim3(ctas), dim3(THREADS), Cfg<DH>::smem_bytes(p.q_rows), s, tm, q_tile, q_token, p) != cudaSuccess) return SB_ERR_LAUNCH;
+  const long long jobs = static_cast<long long>(p.NT) * p.Hkv;
   // few rows have many parts each
-  const bool few = static_cast<long long>(p.NT) * p.Hkv <= 256;
-  return (few ? launch_dep(join_kernel<DH, 4>, dim3(p.NT, p.Hkv), dim3(512), 0, s, p, ctas)
-              : launch_dep(join_kernel<DH, 1>, dim3(p.NT, p.Hkv), dim3(128), 0, s, p, ctas)) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  return (p.pair        ? launch_dep(join_kernel<DH, 1, true>, dim3((jobs + 3) / 4), dim3(128), 0, s, p, ctas)
+          : jobs <= 256 ? launch_dep(join_kernel<DH, 4, false>, dim3(jobs), dim3(512), 0, s, p, ctas)
+                        : launch_dep(join_kernel<DH, 1, false>, dim3(jobs), dim3(128), 0, s, p, ctas)) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 static int ctas_for(long long units) {
@@ -1205,7 +1228,7 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   const uint64_t rows = static_cast<uint64_t>(n_blocks) * 2 * Hkv * page;
   // coordinates of the pool's rows, and of the page behind the last that stands for a bad one; positions; the line of blocks
   if (rows + 2ull * Hkv * page >= (1ull << 31) || static_cast<uint64_t>(max_blocks) * page >= (1ull << 30) ||
-      H > 65535)
+      static_cast<uint64_t>(NT) * Hkv >= (1ull << 31))
     return SB_ERR_TOO_LARGE;
   const bool planned = cu_q != nullptr;
   spa::Params p;

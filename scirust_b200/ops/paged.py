@@ -45,6 +45,21 @@ def shared_prefix_attention_ref(q, pool, block_table, page, seq_len, prefix_tabl
     return out
 
 
+_ws: dict = {}
+
+
+def _workspace(n, device, stream):
+    """``(buffer, its bytes)`` of at least ``n`` bytes. Calls on one stream follow one another and share one; what is being captured into
+    a graph gets its own from the graph's pool, since graphs captured on one stream may be replayed at once on two."""
+    if _lib.DEBUG_POISON or torch._C._cuda_isCurrentStreamCapturing():
+        return _lib.empty(n, torch.uint8, device), n
+    key = (device.index, stream)
+    w = _ws.get(key)
+    if w is None or w[1] < n:
+        w = _ws[key] = (torch.empty(n, dtype=torch.uint8, device=device), n)
+    return w
+
+
 @functools.lru_cache(maxsize=4096)       # a function of the device and the sizes
 def _workspace_bytes(device, NT, B, H, Hkv, dh, ragged, prefix):
     fn = _lib.cuda().sb_shared_prefix_attention_bytes
@@ -68,17 +83,18 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     Positions that no row of a sequence sees may hold anything, infinities and NaN included. Among the new tokens of one call that
     holds for keys; a value that is not finite reaches the rows in front of it too, as in ``attention_fwd``."""
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    B, n = seq_len.shape[0], q.shape[0]
+    (n, width), (B,), (rows, max_blocks) = q.shape, seq_len.shape, block_table.shape
+    n_blocks, *layout = pool.shape
     prefix = int(prefix_len) // page * page if prefix_table is not None else 0
-    if H % Hkv or H <= 0 or page <= 0 or prefix_len < 0 or not scale > 0.0:
+    if H <= 0 or H % Hkv or page <= 0 or prefix_len < 0 or not scale > 0.0:
         raise ValueError("shared_prefix_attention: heads must divide by kv heads, page and scale be positive")
-    if pool.dim() != 5 or tuple(pool.shape[1:]) != (2, Hkv, page, dh) or block_table.dim() != 2 or block_table.shape[0] != B:
+    if layout != [2, Hkv, page, dh] or rows != B:
         raise ValueError("shared_prefix_attention: pool must be [n_blocks, 2, Hkv, page, dh] and block_table [B, pages]")
-    if q.dim() != 2 or q.shape[1] < H * dh or (cu_q is None and n != B) or (cu_q is not None and cu_q.shape != (B + 1,)):
+    if width < H * dh or (n != B if cu_q is None else cu_q.shape != (B + 1,)):
         raise ValueError("shared_prefix_attention: q must be [rows, >= H*dh], one row a sequence or rows counted by cu_q [B + 1]")
     if prefix and prefix_table.numel() * page < prefix:
         raise ValueError("shared_prefix_attention: prefix_table is shorter than the prefix")
-    if out is not None and tuple(out.shape) != (n, H * dh):
+    if out is not None and out.shape != (n, H * dh):
         raise ValueError("shared_prefix_attention: out must be [rows, H*dh]")
     if not q.is_cuda:
         o = shared_prefix_attention_ref(q, pool, block_table, page, seq_len, prefix_table, prefix_len, H, Hkv, dh, scale, cu_q).to(BF)
@@ -94,38 +110,44 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
         with torch.cuda.device(device):
             return shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, prefix_len, H, Hkv, dh, scale, cu_q,
                                            max_len, out)
-    if q.dtype != BF or pool.dtype != BF or (out is not None and out.dtype != BF):
+    if q.dtype is not BF or pool.dtype is not BF or (out is not None and out.dtype is not BF):
         raise ValueError("shared_prefix_attention: q, pool and out must be bf16")
-    if dh not in (64, 128) or H // Hkv > TILE_ROWS or page % 8:
+    if (dh != 128 and dh != 64) or H > TILE_ROWS * Hkv or page % 8:
         raise ValueError("shared_prefix_attention: head dimension 64 or 128, up to 128 query heads per kv head, pages of a multiple of 8")
-    # torch.int32 and one device: a pointer to anything else would be read as what it is not
-    for t in (block_table, seq_len, prefix_table if prefix else None, cu_q):
-        if t is not None and (t.dtype != torch.int32 or t.device != device or not t.is_contiguous()):
-            raise ValueError("shared_prefix_attention: tables, lengths and offsets must be contiguous int32 on the device of q")
-    if pool.device != device or not pool.is_contiguous() or q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
-        raise ValueError("shared_prefix_attention: pool contiguous and on the device of q, rows of q contiguous and 16-byte aligned")
-    fill = out is None
-    if fill:
-        out = _lib.empty((n, H * dh), BF, device)
-    elif out.device != device or out.stride(1) != 1 or out.stride(0) % 8 or out.data_ptr() % 16:
-        raise ValueError("shared_prefix_attention: rows of out contiguous, 16-byte aligned and on the device of q")
+    # a pointer to anything but 32-bit integers on this device would be read as what it is not
+    i = torch.int32
+    if not (block_table.dtype is i and seq_len.dtype is i and (not prefix or prefix_table.dtype is i) and (cu_q is None or cu_q.dtype is i)
+            and block_table.is_contiguous() and seq_len.is_contiguous() and (not prefix or prefix_table.is_contiguous())
+            and (cu_q is None or cu_q.is_contiguous())):
+        raise ValueError("shared_prefix_attention: tables, lengths and offsets must be contiguous and int32")
+    if not (block_table.device == seq_len.device == pool.device == device and (not prefix or prefix_table.device == device)
+            and (cu_q is None or cu_q.device == device) and (out is None or out.device == device)):
+        raise ValueError("shared_prefix_attention: all tensors must be on the device of q")
+    (ldq, unit), q_at = q.stride(), q.data_ptr()
+    if unit != 1 or ldq % 8 or q_at % 16 or not pool.is_contiguous():
+        raise ValueError("shared_prefix_attention: pool must be contiguous, rows of q contiguous and 16-byte aligned")
+    if out is None:
+        fill, ldo = 1, H * dh
+        out = _lib.empty((n, ldo), BF, device)
+    else:
+        fill, (ldo, unit) = 0, out.stride()
+        if unit != 1 or ldo % 8 or out.data_ptr() % 16:
+            raise ValueError("shared_prefix_attention: rows of out must be contiguous and 16-byte aligned")
     if n == 0:
         return out
-    max_blocks = block_table.shape[1]
     if B == 0 or max_blocks == 0:
         return out.zero_() if fill or cu_q is None else out
-    G = H // Hkv
-    per_tile = TILE_ROWS // G
+    per_tile = TILE_ROWS // (H // Hkv)
     if cu_q is not None and n >= B * per_tile:
         prefix = 0                                  # the sequences fill tiles by themselves: nothing to gain from a part in common
-    tiles = -(-n // per_tile)
-    pairs = B if cu_q is None else B + n // per_tile
     L = max_blocks * page if max_len is None else min(int(max_len), max_blocks * page)
-    units = Hkv * (tiles * -(-prefix // BLOCK) + pairs * max(0, -(-(L - prefix) // BLOCK)))
-    ws = _lib.empty(_workspace_bytes(device, n, B, H, Hkv, dh, cu_q is not None, prefix), torch.uint8, device)
-    _lib.call("sb_shared_prefix_attention", q.data_ptr(), q.stride(0), pool.data_ptr(), pool.shape[0], block_table.data_ptr(), max_blocks,
-              page, seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
-              B, n, H, Hkv, dh, units, scale, ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(0), int(fill),
-              _lib.status_word(device).data_ptr(), _lib.stream())
+    pairs = B if cu_q is None else B + n // per_tile
+    units = Hkv * (-(-n // per_tile) * -(-prefix // BLOCK) + pairs * max(0, -(-(L - prefix) // BLOCK)))
+    stream = _lib.stream()
+    ws, ws_bytes = _workspace(_workspace_bytes(device.index, n, B, H, Hkv, dh, cu_q is not None, prefix), device, stream)
+    _lib.call("sb_shared_prefix_attention", q_at, ldq, pool.data_ptr(), n_blocks, block_table.data_ptr(), max_blocks, page,
+              seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
+              B, n, H, Hkv, dh, units, scale, ws.data_ptr(), ws_bytes, out.data_ptr(), ldo, fill,
+              _lib.status_word(device).data_ptr(), stream)
     _g.launch_count += 2 if cu_q is None else 3
     return out
