@@ -4,7 +4,7 @@
 //   s_j = scale q.k_j,  m = max s_j,  l = sum exp(s_j - m),  o = sum exp(s_j - m) v_j / l,   j < limit;   limit <= 0: o = 0.
 // Positions below P (the whole pages of the prefix) are the same for all sequences, so the sum is taken in two parts: the rows of all
 // sequences against one copy of K and V, and each sequence's rows against what it has for itself. Parts (m_i, l_i, o_i) of a row,
-// o_i not divided by l_i, join as m = max m_i, w_i = exp(scale (m_i - m)), o = sum w_i o_i / sum w_i l_i (here m_i is a maximum of q.k).
+// o_i not divided by l_i, join as m = max m_i, w_i = 2^(m_i - m), o = sum w_i o_i / sum w_i l_i (scores in units of log 2).
 //
 // Both parts are the same work for a CTA: a tile of 128 rows (tokens times the query heads of one kv head), a table of pages and a
 // range of 128-position blocks of keys. An item is all of that for one tile of rows:
@@ -41,9 +41,10 @@ static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * 168, "the shares draw on the 
 constexpr int TMEM_COLS = 512;
 constexpr int QUEUE = 4;       // pieces that the producer may be ahead
 constexpr int ITEM_UNITS = 2;
-// A row's reference may lag behind its maximum until a weight passes 2^8: then O is rescaled, in the first blocks of a piece mostly. What
-// is summed is the weight after its rounding to bf16, the one that multiplies V, so a row that one position dominates loses nothing.
-constexpr float RESCALE_GAP = 8.f;
+// A row's reference is its running maximum, so its largest weight is 1 and loses nothing when weights become bf16, and the sum is one of
+// weights before that. A reference that may lag behind by 2^8 saves rescales of O: 2 us of 64 (64 sequences behind 16384 positions), for an
+// error of 2.2e-3 in place of 2.0e-3 on unit scores and 1.3e-3 in place of 0.5e-3 on scores of four times the spread; with a sum of the
+// rounded weights that is 1.0e-3, but the sum costs 5 to 12 us of 65 to 105.
 constexpr float LOWEST = -3.402823466e38f;   // reference of a row that has seen nothing: 2^(-inf - LOWEST) is 0
 
 template <int DH>
@@ -776,9 +777,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         // The row's reference for this block, P V of the lane's block before, which frees P, and O, if the reference has moved; the factor
         // of what the row has so far.
         auto turn = [&]() -> float {
-          const bool grow = (m_blk - m_ref) * sl2 > RESCALE_GAP || m_ref == LOWEST;
-          const float alpha = grow ? ex2((m_ref - m_blk) * sl2) : 1.f;
-          if (grow) m_ref = m_blk;
+          const float m_new = m_blk * sl2;
+          const bool grow = m_new > m_ref;
+          const float alpha = grow ? ex2(m_ref - m_new) : 1.f;
+          if (grow) m_ref = m_new;
           if (n > 0) {
             wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
             tc_fence_after();
@@ -800,14 +802,21 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           }
           return alpha;
         };
-        // Weights of two columns, as bf16. Scores are subtracted before they are scaled: one fused step leaves the rounding of scale * m
-        // between a row's largest score and zero, which is everything once scores are beyond 2^24.
+        // Weights of two columns, as bf16. Scale and difference are one fused step, whose exponent is off from the rounded reference by up
+        // to half a step of it: nothing, unless scores are beyond 2^24. Those are scaled beforehand, rounded as the reference was.
+        float factor = sl2;
+        auto scaled_first = [&](uint32_t* u, auto count) {
+          if (__any_sync(0xffffffffu, fabsf(m_ref) > 16777216.f && m_ref != LOWEST)) {
+#pragma unroll
+            for (int c = 0; c < decltype(count)::value; c += 2) mul2(u[c], u[c + 1], sl2, sl2);
+            factor = 1.f;
+          }
+        };
         auto weigh = [&](uint32_t& a, uint32_t& b, int c) -> uint32_t {
-          fma2(a, b, 1.f, -m_ref);
-          mul2(a, b, sl2, sl2);
-          const uint32_t w = pack_bf16x2(ex2(__uint_as_float(a)), ex2(__uint_as_float(b)));
-          add2(sum4[c & 6], sum4[(c & 6) + 1], w << 16, w & 0xffff0000u);
-          return w;
+          fma2(a, b, factor, -m_ref);
+          const float e0 = ex2(__uint_as_float(a)), e1 = ex2(__uint_as_float(b));
+          add2(sum4[c & 6], sum4[(c & 6) + 1], __float_as_uint(e0), __float_as_uint(e1));
+          return pack_bf16x2(e0, e1);
         };
         float alpha;
         if (split) {
@@ -825,6 +834,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
             m_blk = max3(m_blk, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
           }
           alpha = turn();
+          scaled_first(v, std::integral_constant<int, 32>{});
           uint32_t pk[32];
           if (i == first) {                // the weights of the others' positions stay zero
 #pragma unroll
@@ -860,6 +870,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
             m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
           m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           alpha = turn();
+          scaled_first(v, std::integral_constant<int, BN>{});
           const int live = x.kend - (x.kbase + (x.j0 + i) * BN);      // positions that any row sees
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -899,8 +910,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         tc_fence_after();
         const float2 y = s_ml[r];
         const float m = fmaxf(m_ref, y.x);
-        w0 = ex2((m_ref - m) * sl2);
-        w1 = ex2((y.x - m) * sl2);
+        w0 = ex2(m_ref - m);
+        w1 = ex2(y.x - m);
         m_ref = m;
         l = __fmaf_rn(w0, l, __fmul_rn(w1, y.y));
       }
@@ -1084,14 +1095,14 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
         float top = m[r];
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) top = fmaxf(top, x[r][b].x);
-        const float a = ex2((m[r] - top) * p.scale_log2);
+        const float a = ex2(m[r] - top);
         l[r] *= a;
 #pragma unroll
         for (int f = 0; f < F; ++f) acc[r][f] *= a;
         m[r] = top;
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {            // a part that is none has no weight: l is 0 and so is o
-          const float w = ex2((x[r][b].x - top) * p.scale_log2);
+          const float w = ex2(x[r][b].x - top);
           l[r] = fmaf(w, x[r][b].y, l[r]);
           acc[r][0] = fmaf(w, o[r][b].x, acc[r][0]);
           acc[r][1] = fmaf(w, o[r][b].y, acc[r][1]);
@@ -1111,14 +1122,14 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
         float top = m[0];
 #pragma unroll
         for (int w = 1; w < WAYS; ++w) top = fmaxf(top, s_ml[slot][w].x);
-        const float a = ex2((m[0] - top) * p.scale_log2);
+        const float a = ex2(m[0] - top);
         l[0] *= a;
 #pragma unroll
         for (int f = 0; f < F; ++f) acc[0][f] *= a;
 #pragma unroll 1
         for (int w = 1; w < WAYS; ++w) {
           const float2 y = s_ml[slot][w];
-          const float b = ex2((y.x - top) * p.scale_log2);
+          const float b = ex2(y.x - top);
           l[0] = fmaf(b, y.y, l[0]);
 #pragma unroll
           for (int f = 0; f < F; ++f) acc[0][f] = fmaf(b, s_o[slot][w][lane * F + f], acc[0][f]);
