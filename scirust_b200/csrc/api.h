@@ -125,6 +125,9 @@ int sb_cast(const void* in, void* out, size_t n, int to_bf16, float scale, void*
 int sb_multi_cast_f32_bf16(const void* const* srcs, const unsigned long long* dst_offs, const unsigned long long* ns, int count, void* dst, int accumulate, void* stream);
 int sb_sumsq_no_alloc(const void* g, size_t n, int is_bf16, float* out, int accumulate, void* stream);
 
+// page_copy.cu
+int sb_copy_pages(const void* const* src, void* const* dst, int layers, const int* from, const int* to, int n, int src_blocks, int dst_blocks, long long page_bytes, int segs, long long seg_bytes, long long seg_pitch, void* stream_);
+
 // paged_attention_tcgen05.cu
 size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv, int dh, int ragged, int prefix);
 int sb_shared_prefix_attention(const void* q, long long ldq, const void* pool, int n_blocks, const int* block_table, int max_blocks, int page, const int* seq_len, const int* prefix_table, int prefix, const int* cu_q, int B, int NT, int H, int Hkv, int dh, long long max_units, float scale, void* workspace, size_t workspace_bytes, void* out, long long ldo, int fill, int* status, void* stream);

@@ -1,7 +1,9 @@
-"""Ops on a paged KV cache whose sequences share pages (csrc/paged_attention_tcgen05.cu): the attention of a batch behind a common
-prefix. CPU tensors take the fp32 PyTorch statement of the same arithmetic."""
+"""Ops on a paged KV cache whose sequences share pages: the attention of a batch behind a common prefix
+(csrc/paged_attention_tcgen05.cu), and copies of pages in all layers' pools (csrc/page_copy.cu). CPU tensors take the PyTorch statement
+of the same arithmetic."""
 from __future__ import annotations
 
+import ctypes as C
 import functools
 import math
 
@@ -14,6 +16,8 @@ BF = torch.bfloat16
 vp, i32, i64, f32, sz = _lib.vp, _lib.i32, _lib.i64, _lib.f32, _lib.sz
 _lib.register("sb_shared_prefix_attention", [vp, i64, vp, i32, vp, i32, i32, vp, vp, i32, vp, i32, i32, i32, i32, i32, i64, f32, vp, sz,
                                              vp, i64, i32, vp, vp])
+
+_lib.register("sb_copy_pages", [vp, vp, i32, vp, vp, i32, i32, i32, i64, i32, i64, i64, vp])
 
 TILE_ROWS, BLOCK = 128, 128          # rows of a tile, positions of a block of keys
 
@@ -151,3 +155,82 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
               _lib.status_word(device).data_ptr(), stream)
     _g.launch_count += 2 if cu_q is None else 3
     return out
+
+
+class PagePools:
+    """The pools of a cache's layers, checked once: tensors of one shape ``[n_blocks, ..., page, width]``, type and device, each contiguous.
+    It holds on to the tensors; one that is replaced in the cache needs a new handle."""
+
+    def __init__(self, pools):
+        self.pools = list(pools)
+        if not self.pools or self.pools[0].dim() < 3:
+            raise ValueError("PagePools: at least one pool of [n_blocks, ..., page, width]")
+        p = self.pools[0]
+        self.shape, self.dtype, self.device = tuple(p.shape), p.dtype, p.device
+        for t in self.pools:
+            if tuple(t.shape) != self.shape or t.dtype != self.dtype or t.device != self.device or not t.is_contiguous():
+                raise ValueError("PagePools: contiguous pools of one shape, type and device")
+        self.n_blocks, self.page = self.shape[0], self.shape[-2]
+        self.heads = math.prod(self.shape[1:-2])                      # of K and of V
+        self.row_bytes = self.shape[-1] * p.element_size()            # of a position of a head
+        self.page_bytes = self.heads * self.page * self.row_bytes
+        self._table = (C.c_void_p * len(self.pools))(*[t.data_ptr() for t in self.pools])
+        self.table = C.addressof(self._table)
+
+    def __len__(self):
+        return len(self.pools)
+
+
+def _page_ids(ids, n_blocks, what):
+    ids = [int(i) for i in (ids.tolist() if torch.is_tensor(ids) else ids)]
+    if any(not 0 <= i < n_blocks for i in ids):
+        raise ValueError(f"copy_pages: {what} page outside the pool")
+    return ids
+
+
+def copy_pages(pools, src, dst, rows=None, out=None):
+    """Copies page ``src[i]`` to page ``dst[i]`` in every layer's pool, or to ``dst[i]`` of the pools ``out``; with ``rows`` only the first
+    ``rows`` positions of each page. ``pools`` (and ``out``) is a ``PagePools`` or a list of pools.
+
+    A source may be copied many times; a destination must occur once and, in the same pools, be no source. Ids from the host (a list, a CPU
+    tensor) are checked for that. Ids on the device (int32) are taken as they are, so that a captured call can be replayed with others;
+    ids outside the pools are skipped there, as padding may be."""
+    pools = pools if isinstance(pools, PagePools) else PagePools(pools)
+    to = pools if out is None else out if isinstance(out, PagePools) else PagePools(out)
+    if to is not pools and (len(to) != len(pools) or to.shape[1:] != pools.shape[1:] or to.dtype != pools.dtype or to.device != pools.device):
+        raise ValueError("copy_pages: out must be as many pools of the same pages, type and device")
+    if rows is not None and not 0 <= rows <= pools.page:
+        raise ValueError("copy_pages: rows must be between 0 and the positions of a page")
+    device = pools.device
+    on_device = device.type == "cuda" and torch.is_tensor(src) and torch.is_tensor(dst) and src.is_cuda and dst.is_cuda
+    if on_device:
+        if (src.dtype is not torch.int32 or dst.dtype is not torch.int32 or src.shape != dst.shape or src.dim() != 1
+                or not src.is_contiguous() or not dst.is_contiguous() or src.device != device or dst.device != device):
+            raise ValueError("copy_pages: page ids on the device must be two contiguous int32 vectors of one length, beside the pools")
+    else:
+        src, dst = _page_ids(src, pools.n_blocks, "source"), _page_ids(dst, to.n_blocks, "destination")
+        if len(src) != len(dst) or len(set(dst)) != len(dst):
+            raise ValueError("copy_pages: as many destinations as sources, each once")
+        same = {t.data_ptr() for t in pools.pools} & {t.data_ptr() for t in to.pools}
+        if same and set(src) & set(dst):
+            raise ValueError("copy_pages: a page is both source and destination")
+    n = len(src)
+    if n == 0 or rows == 0 or pools.page_bytes == 0:
+        return
+    rows = pools.page if rows is None else rows
+    if device.type != "cuda":
+        a, b = torch.tensor(src, device=device), torch.tensor(dst, device=device)
+        for s, d in zip(pools.pools, to.pools):
+            d[b, ..., :rows, :] = s[a, ..., :rows, :]
+        return
+    if device.index != _lib.current_device():
+        with torch.cuda.device(device):
+            return copy_pages(pools, src, dst, rows, to)
+    if not on_device:
+        src, dst = torch.tensor([src, dst], dtype=torch.int32).to(device)
+    pitch = pools.page * pools.row_bytes
+    whole = rows == pools.page
+    _lib.call("sb_copy_pages", pools.table, to.table, len(pools), src.data_ptr(), dst.data_ptr(), n, pools.n_blocks, to.n_blocks,
+              pools.page_bytes, 1 if whole else pools.heads, pools.page_bytes if whole else rows * pools.row_bytes,
+              pools.page_bytes if whole else pitch, _lib.stream())
+    _g.launch_count += -(-len(pools) // 64)

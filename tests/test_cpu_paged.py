@@ -79,3 +79,45 @@ def test_entry_point_refuses():
                          (dict(max_blocks=1 << 25), "size beyond"), (dict(B=1 << 22, NT=1 << 22, max_blocks=1 << 12), "size beyond")):
         with pytest.raises(_lib.NativeError, match=what):
             _lib.call("sb_shared_prefix_attention", *{**ok, **change}.values())
+
+
+def test_copy_pages_statement():
+    pools = [torch.randn(6, 2, 1, 4, 8) for _ in range(2)]
+    before = [p.clone() for p in pools]
+    paged.copy_pages(pools, [1, 1, 0], [3, 5, 4], rows=3)
+    for p, b in zip(pools, before):
+        for s, d in ((1, 3), (1, 5), (0, 4)):
+            assert torch.equal(p[d, :, :, :3], b[s, :, :, :3]) and torch.equal(p[d, :, :, 3:], b[d, :, :, 3:])
+        assert torch.equal(p[:3], b[:3])
+    other = [torch.zeros(2, 2, 1, 4, 8) for _ in range(2)]
+    paged.copy_pages(pools, [1, 4], [1, 0], out=other)
+    assert all(torch.equal(o[1], p[1]) and torch.equal(o[0], p[4]) for o, p in zip(other, pools))
+    paged.copy_pages(pools, [], [])
+
+
+@pytest.mark.parametrize("args,kw", [
+    (([0], [6]), {}), (([-1], [2]), {}), (([0, 1], [2, 2]), {}), (([0, 1], [1, 2]), {}), (([0], [1, 2]), {}), (([0], [1]), dict(rows=5)),
+    (([0], [1]), dict(rows=-1)), (([0], [1]), dict(out=[torch.zeros(6, 2, 1, 4, 8)])),
+    (([0], [1]), dict(out=[torch.zeros(6, 2, 1, 2, 8)] * 2)), (([0], [1]), dict(out=[torch.zeros(6, 2, 1, 4, 8, dtype=BF)] * 2))])
+def test_copy_pages_refusals(args, kw):
+    with pytest.raises(ValueError):
+        paged.copy_pages([torch.zeros(6, 2, 1, 4, 8) for _ in range(2)], *args, **kw)
+
+
+def test_page_pools_refusals():
+    for bad in ([], [torch.zeros(3, 4)], [torch.zeros(3, 2, 4, 8), torch.zeros(3, 2, 4, 7)], [torch.zeros(3, 2, 8, 4).transpose(2, 3)],
+                [torch.zeros(3, 2, 4, 8), torch.zeros(3, 2, 4, 8, dtype=BF)]):
+        with pytest.raises(ValueError):
+            paged.PagePools(bad)
+
+
+def test_copy_entry_point_refuses():
+    import ctypes
+    from scirust_b200.ops import _lib
+    table = ctypes.addressof((ctypes.c_void_p * 1)(16))
+    ok = dict(src=table, dst=table, layers=1, a=16, b=16, n=1, sb=4, db=4, page=1024, segs=1, seg=1024, pitch=1024, stream=None)
+    for change, what in ((dict(src=None), "bad argument"), (dict(layers=0), "bad argument"), (dict(n=0), "bad argument"),
+                         (dict(sb=0), "bad argument"), (dict(seg=0), "bad argument"), (dict(segs=2, seg=512, pitch=500), "bad argument"),
+                         (dict(segs=3, seg=512, pitch=512), "bad argument"), (dict(page=1 << 31, seg=512), "size beyond")):
+        with pytest.raises(_lib.NativeError, match=what):
+            _lib.call("sb_copy_pages", *{**ok, **change}.values())

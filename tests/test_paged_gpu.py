@@ -246,3 +246,75 @@ def test_many_short_pieces_a_cta(B, tail):
     check(batch(B, 32, 8, 128, 64, 1000, tails))
     new = [min(t, 1 + b % 70) for b, t in enumerate(tails)]
     check(batch(B, 8, 2, 64, 16, 300, tails, new))
+
+
+# ---------------------------------------------------------------------------------------------- copies of pages
+def _copied(pools, src, dst, rows, out=None):
+    """Each pool as it should be, one copy at a time."""
+    want = [(o if out is not None else p).clone() for p, o in zip(pools, out or pools)]
+    for w, p in zip(want, pools):
+        for a, b in zip(src, dst):
+            w[b, ..., :rows, :] = p[a, ..., :rows, :]
+    return want
+
+
+@pytest.mark.parametrize("shape,dtype", [((40, 2, 8, 64, 128), BF), ((33, 2, 3, 16, 64), BF), ((21, 2, 1, 8, 80), torch.float16),
+                                         ((17, 2, 2, 5, 7), torch.uint8), ((19, 2, 2, 3, 6), torch.int16), ((9, 4, 1), torch.float32)])
+@pytest.mark.parametrize("rows", [None, 1, 3])
+def test_copies_of_pages(shape, dtype, rows):
+    g = torch.Generator(device=DEV).manual_seed(1)
+    pools = [torch.randint(0, 100, shape, generator=g, device=DEV).to(dtype) for _ in range(3)]
+    order = torch.randperm(shape[0], generator=torch.Generator().manual_seed(2)).tolist()
+    n = shape[0] // 3
+    for src, dst in ((order[:n], order[n:2 * n]), ([order[0]] * n, order[n:2 * n]), (order[:1], order[1:2])):
+        for ids in (lambda v: v, lambda v: torch.tensor(v), lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)):
+            want = _copied(pools, src, dst, rows or shape[-2])
+            got = [p.clone() for p in pools]
+            paged.copy_pages(paged.PagePools(got), ids(src), ids(dst), rows=rows)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        other = [torch.zeros((n + 2, *shape[1:]), dtype=dtype, device=DEV) for _ in pools]
+        into = list(range(n + 1, n + 1 - len(src), -1))
+        want = _copied(pools, src, into, rows or shape[-2], other)
+        paged.copy_pages(pools, src, into, rows=rows, out=other)
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+def test_copies_skip_what_is_outside_and_take_many_layers():
+    pools = [torch.randn(12, 2, 2, 16, 64, device=DEV).to(BF) for _ in range(70)]
+    want = _copied(pools, [3, 4], [7, 8], 16)
+    src = torch.tensor([3, -1, 12, 5, 4, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    dst = torch.tensor([7, 0, 1, -5, 8, 2], dtype=torch.int32, device=DEV)
+    paged.copy_pages(pools, src, dst)
+    assert all(torch.equal(a, b) for a, b in zip(pools, want))
+
+
+def test_copies_beyond_32_bits():
+    pool = torch.empty((20600, 2, 8, 64, 128), dtype=BF, device=DEV)
+    pool[-4:] = torch.randn(4, 2, 8, 64, 128, device=DEV)
+    pool[3:5] = 0
+    paged.copy_pages([pool], [20599, 20597], [3, 20598])
+    assert torch.equal(pool[3], pool[20599]) and torch.equal(pool[20598], pool[20597]) and not pool[4].any()
+
+
+def test_copies_in_a_graph_take_new_ids():
+    pools = [torch.randn(12, 2, 2, 16, 64, device=DEV).to(BF) for _ in range(2)]
+    src, dst = torch.tensor([1, 2], dtype=torch.int32, device=DEV), torch.tensor([8, 9], dtype=torch.int32, device=DEV)
+    handle = paged.PagePools(pools)
+    paged.copy_pages(handle, src, dst)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        paged.copy_pages(handle, src, dst)
+    src.copy_(torch.tensor([3, 4]))
+    dst.copy_(torch.tensor([10, 11]))
+    want = _copied(pools, [3, 4], [10, 11], 16)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(pools, want))
+
+
+def test_many_copies():
+    """More copies than a grid has rows."""
+    pool = torch.arange(140000, device=DEV, dtype=torch.int32).reshape(-1, 1, 1, 1).repeat(1, 1, 2, 4)
+    n = 70000
+    paged.copy_pages([pool], torch.arange(n, dtype=torch.int32, device=DEV), torch.arange(n, 2 * n, dtype=torch.int32, device=DEV))
+    assert torch.equal(pool[:n], pool[n:])
