@@ -7,7 +7,9 @@
 //
 // Bound by memory: each byte is read and written once. A CTA copies up to 32 KB of one page of one layer, eight 16-byte words a thread, all
 // of whose loads are under way before the first store; layers are the slowest grid index, so a page that goes to many (a fork) is read
-// from L2 by all but the first.
+// from L2 by all but the first. 128 pages of 256 KB in eight layers 83 us, 0.99 of the copy rate; 301 pages of 8 KB in 32 layers 26.9, 0.90;
+// 40 of 64 positions to 16 pages in 32 layers 18.5, of which 84 MB are writes (four copies a CTA, which hold a source that stays the same
+// in registers, gained nothing and cost the first of these 2 us).
 #include "api.h"
 #include "dependent.cuh"
 
@@ -22,6 +24,7 @@ struct Params {
   const int *from, *to;
   int n, src_blocks, dst_blocks, segs;
   long long page_words, seg_words, seg_pitch_words;
+  int step_segs, step_words;                       // THREADS words further on: segments, and words into the one behind them
 };
 
 // One segment: no division.
@@ -32,6 +35,18 @@ __global__ void __launch_bounds__(THREADS) copy_pages_kernel(const __grid_consta
   const long long words = p.seg_words * p.segs, first = static_cast<long long>(blockIdx.x) * (THREADS * WORDS) + threadIdx.x;
   const W* src = static_cast<const W*>(p.src[blockIdx.z]);
   W* dst = static_cast<W*>(p.dst[blockIdx.z]);
+  long long at[WORDS];
+  {
+    int seg = ONE ? 0 : static_cast<int>(static_cast<unsigned>(first) / static_cast<unsigned>(p.seg_words));      // words < 2^31 (host)
+    long long in = first - seg * p.seg_words;
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+      at[k] = ONE ? first + k * THREADS : seg * p.seg_pitch_words + in;
+      seg += p.step_segs;
+      in += p.step_words;
+      if (in >= p.seg_words) { in -= p.seg_words; ++seg; }
+    }
+  }
   for (int i = blockIdx.y; i < p.n; i += gridDim.y) {
     const int a = p.from[i], b = p.to[i];
     if (static_cast<unsigned>(a) >= static_cast<unsigned>(p.src_blocks) || static_cast<unsigned>(b) >= static_cast<unsigned>(p.dst_blocks))
@@ -39,18 +54,9 @@ __global__ void __launch_bounds__(THREADS) copy_pages_kernel(const __grid_consta
     const W* s = src + a * p.page_words;
     W* d = dst + b * p.page_words;
     W v[WORDS];
-    long long at[WORDS];
 #pragma unroll
-    for (int k = 0; k < WORDS; ++k) {
-      const long long w = first + k * THREADS;
-      if (ONE) {
-        at[k] = w;
-      } else {
-        const unsigned seg = static_cast<unsigned>(w) / static_cast<unsigned>(p.seg_words);      // words < 2^31 (host)
-        at[k] = w + seg * (p.seg_pitch_words - p.seg_words);
-      }
-      if (w < words) v[k] = s[at[k]];
-    }
+    for (int k = 0; k < WORDS; ++k)
+      if (first + k * THREADS < words) v[k] = s[at[k]];
 #pragma unroll
     for (int k = 0; k < WORDS; ++k)
       if (first + k * THREADS < words) d[at[k]] = v[k];
@@ -64,6 +70,8 @@ static int launch(Params p, int layers, const void* const* src, void* const* dst
   p.seg_words = seg_bytes / sizeof(W);
   p.seg_pitch_words = seg_pitch / sizeof(W);
   const long long words = p.seg_words * p.segs, chunks = (words + THREADS * WORDS - 1) / (THREADS * WORDS);
+  p.step_segs = static_cast<int>(THREADS / p.seg_words);
+  p.step_words = static_cast<int>(THREADS % p.seg_words);
   for (int l0 = 0; l0 < layers; l0 += MAX_LAYERS) {
     const int n = layers - l0 < MAX_LAYERS ? layers - l0 : MAX_LAYERS;
     for (int l = 0; l < n; ++l) {

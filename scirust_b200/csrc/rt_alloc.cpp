@@ -3,7 +3,8 @@
 //  * BlockAllocator: fixed-size KV-cache pages with a LIFO free list and per-sequence block lists
 //    (the reference's paged cache keeps a block table per sequence and grows it page by page:
 //    scirust-core/src/nn/paged_attention.rs:21-147). Freed pages are reused most-recent-first so
-//    a workload's physical layout is reproducible.
+//    a workload's physical layout is reproducible. A page may have several owners (sequences with a
+//    common prefix); it returns to the list with the last of them.
 //  * Arena: a bump allocator over one preallocated device buffer with mark/release, used for the
 //    step-scoped workspace instead of one allocation per op (the reference's op-chain allocates an
 //    output for every op: scirust-cuda/src/chain.rs:1049-1052; its CPU arenas:
@@ -15,6 +16,8 @@
 
 struct SbBlockAlloc {
   std::vector<int32_t> free_list;
+  std::vector<int32_t> more;      // owners of a page beyond the first
+  std::vector<uint8_t> used;
   int32_t n_blocks;
 };
 struct SbArena {
@@ -25,9 +28,17 @@ extern "C" {
 
 SbBlockAlloc* sbrt_balloc_new(int32_t n_blocks) {
   if (n_blocks <= 0) return nullptr;
-  SbBlockAlloc* a = new SbBlockAlloc();
+  SbBlockAlloc* a = nullptr;
+  try {                                   // memory that runs out is an error of the caller's call, not one of C++
+    a = new SbBlockAlloc();
+    a->free_list.reserve(n_blocks);
+    a->more.assign(n_blocks, 0);
+    a->used.assign(n_blocks, 0);
+  } catch (...) {
+    delete a;
+    return nullptr;
+  }
   a->n_blocks = n_blocks;
-  a->free_list.reserve(n_blocks);
   for (int32_t i = n_blocks - 1; i >= 0; --i) a->free_list.push_back(i);  // block 0 is handed out first
   return a;
 }
@@ -39,16 +50,85 @@ int32_t sbrt_balloc_alloc(SbBlockAlloc* a, int32_t n, int32_t* out) {
   for (int32_t i = 0; i < n; ++i) {
     out[i] = a->free_list.back();
     a->free_list.pop_back();
+    a->used[out[i]] = 1;
+    a->more[out[i]] = 0;
   }
   return 0;
 }
-// Returns blocks to the pool; ids outside the pool are rejected (-1) and nothing is freed.
+// Gives up one owner of each block (an id may occur several times); the last owner's returns to the pool. Ids outside the pool, and more
+// blocks than are out, are rejected (-1) and nothing is freed.
 int32_t sbrt_balloc_free(SbBlockAlloc* a, const int32_t* ids, int32_t n) {
   for (int32_t i = 0; i < n; ++i)
     if (ids[i] < 0 || ids[i] >= a->n_blocks) return -1;
-  if (a->free_list.size() + static_cast<size_t>(n) > static_cast<size_t>(a->n_blocks)) return -1;
-  for (int32_t i = 0; i < n; ++i) a->free_list.push_back(ids[i]);
+  std::vector<int32_t> back;
+  try {
+    back.reserve(n > 0 ? n : 0);
+  } catch (...) {
+    return -1;
+  }
+  for (int32_t i = 0; i < n; ++i) {
+    if (a->more[ids[i]] > 0) --a->more[ids[i]];
+    else back.push_back(ids[i]);
+  }
+  if (a->free_list.size() + back.size() > static_cast<size_t>(a->n_blocks)) {
+    // as they were: an id keeps its last owner in `back`, so what it had beyond is the times that it occurs less those
+    for (int32_t i = 0; i < n; ++i) ++a->more[ids[i]];
+    for (int32_t id : back) --a->more[id];
+    return -1;
+  }
+  for (int32_t id : back) {
+    a->free_list.push_back(id);           // within what is reserved
+    a->used[id] = 0;
+  }
   return 0;
+}
+// One more owner for each block (an id may occur several times); -1, and none, if one of them is not in use.
+int32_t sbrt_balloc_share(SbBlockAlloc* a, const int32_t* ids, int32_t n) {
+  for (int32_t i = 0; i < n; ++i)
+    if (ids[i] < 0 || ids[i] >= a->n_blocks || !a->used[ids[i]]) return -1;
+  for (int32_t i = 0; i < n; ++i) ++a->more[ids[i]];
+  return 0;
+}
+// Owners of a block, 0 if it is free, -1 if there is none of this id.
+int32_t sbrt_balloc_owners(const SbBlockAlloc* a, int32_t id) {
+  if (id < 0 || id >= a->n_blocks) return -1;
+  return a->used[id] ? a->more[id] + 1 : 0;
+}
+// Numbers the blocks in use anew, ascending from 0, in a pool of n_blocks: to[id] gets the new id of block id, or -1 if it is free, and the
+// return value is how many are in use. A block below that number keeps its id, the others take the lowest free ones in ascending order.
+// -1, and nothing changes, if they are more than n_blocks. Blocks are then handed out from the lowest on.
+int32_t sbrt_balloc_compact(SbBlockAlloc* a, int32_t n_blocks, int32_t* to) {
+  int32_t live = 0;
+  for (int32_t i = 0; i < a->n_blocks; ++i) live += a->used[i];
+  if (n_blocks <= 0 || live > n_blocks) return -1;
+  std::vector<int32_t> more, list;
+  std::vector<uint8_t> used;
+  try {
+    more.assign(n_blocks, 0);
+    used.assign(n_blocks, 0);
+    list.reserve(n_blocks);
+  } catch (...) {
+    return -1;
+  }
+  int32_t hole = 0;
+  for (int32_t i = 0; i < a->n_blocks; ++i) {
+    to[i] = -1;
+    if (!a->used[i]) continue;
+    if (i < live) {
+      to[i] = i;
+    } else {
+      while (a->used[hole]) ++hole;
+      to[i] = hole++;
+    }
+    more[to[i]] = a->more[i];
+  }
+  for (int32_t i = 0; i < live; ++i) used[i] = 1;
+  for (int32_t i = n_blocks - 1; i >= live; --i) list.push_back(i);
+  a->n_blocks = n_blocks;
+  a->more.swap(more);
+  a->used.swap(used);
+  a->free_list.swap(list);
+  return live;
 }
 
 SbArena* sbrt_arena_new(uint64_t capacity) {

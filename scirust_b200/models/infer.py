@@ -24,7 +24,7 @@ import torch
 from .. import ops
 from ..generate import SamplingParams
 from ..ops.sampling import DeviceSampler
-from ..ops import _lib, attention as att, decode as D, gemm as G
+from ..ops import _lib, attention as att, decode as D, gemm as G, paged
 from .sciagent import BF, GQADecoder, SciAgentConfig
 
 
@@ -42,6 +42,12 @@ class BlockAllocator:
         lib.sbrt_balloc_alloc.restype = C.c_int32
         lib.sbrt_balloc_free.argtypes = [C.c_void_p, C.c_void_p, C.c_int32]
         lib.sbrt_balloc_free.restype = C.c_int32
+        lib.sbrt_balloc_share.argtypes = [C.c_void_p, C.c_void_p, C.c_int32]
+        lib.sbrt_balloc_share.restype = C.c_int32
+        lib.sbrt_balloc_owners.argtypes = [C.c_void_p, C.c_int32]
+        lib.sbrt_balloc_owners.restype = C.c_int32
+        lib.sbrt_balloc_compact.argtypes = [C.c_void_p, C.c_int32, C.c_void_p]
+        lib.sbrt_balloc_compact.restype = C.c_int32
         self._lib = lib
         self._h = lib.sbrt_balloc_new(n_blocks)
         if not self._h:
@@ -56,6 +62,30 @@ class BlockAllocator:
         if self._lib.sbrt_balloc_alloc(self._h, n, buf) != 0:
             raise MemoryError(f"KV cache exhausted: {n} pages requested, {self.num_free()} free")
         return list(buf[:n])
+
+    def share(self, ids) -> None:
+        """One more owner for each of these pages, which are in use: ``free`` returns a page when its last owner gives it up."""
+        ids = list(ids)
+        buf = (C.c_int32 * max(len(ids), 1))(*ids)
+        if self._lib.sbrt_balloc_share(self._h, buf, len(ids)) != 0:
+            raise ValueError("only pages in use can be shared")
+
+    def owners(self, page: int) -> int:
+        """How many own the page; 0 if it is free."""
+        n = int(self._lib.sbrt_balloc_owners(self._h, page))
+        if n < 0:
+            raise ValueError("no such page")
+        return n
+
+    def compact(self, n_blocks: int | None = None) -> list:
+        """Numbers the pages in use anew from 0 on, in a pool of ``n_blocks`` (default: as many as now): the new id of every page, -1 for a
+        free one. The lowest ids stay as they are, the others move into the holes."""
+        n = self.n_blocks if n_blocks is None else n_blocks
+        to = (C.c_int32 * self.n_blocks)()
+        if self._lib.sbrt_balloc_compact(self._h, n, to) < 0:
+            raise MemoryError(f"{self.n_blocks - self.num_free()} pages in use do not fit into {n}")
+        self.n_blocks = n
+        return list(to)
 
     def free(self, ids) -> None:
         ids = list(ids)
@@ -103,6 +133,54 @@ class PagedKVCache:
         self.alloc.free(self.owned[seq])
         self.owned[seq] = []
         self.table_host[seq].zero_()
+
+    def fork(self, src: int, seqs, n_tokens: int) -> None:
+        """Gives the sequences ``seqs``, which have no pages, the first ``n_tokens`` positions of ``src``. Whole pages are shared: each counts
+        its owners and is free again with the last of them. A page that the positions do not fill is copied for every sequence, as far as it is
+        filled, since each writes on in its own. ``commit`` makes the tables known to the device, as after ``reserve``."""
+        seqs = list(seqs)
+        whole, rest = divmod(n_tokens, self.page)
+        if not 0 <= src < self.max_batch or n_tokens < 0 or len(self.owned[src]) < whole + bool(rest):
+            raise ValueError("fork: the sequence does not hold so many positions")
+        if len(set(seqs)) != len(seqs) or any(not 0 <= s < self.max_batch or self.owned[s] for s in seqs):
+            raise ValueError("fork: to different sequences of the cache without pages")
+        last = self.alloc.alloc(len(seqs)) if rest else []
+        self.alloc.share(self.owned[src][:whole] * len(seqs))
+        for i, s in enumerate(seqs):
+            self.owned[s] = self.owned[src][:whole] + last[i:i + 1]
+            self.table_host[s, :len(self.owned[s])] = torch.tensor(self.owned[s], dtype=torch.int32)
+        if last:
+            paged.copy_pages(paged.PagePools(self.pools), [self.owned[src][whole]] * len(seqs), last, rows=rest)
+
+    def _renumber(self, to) -> None:
+        for s, ids in enumerate(self.owned):
+            self.owned[s] = [to[i] for i in ids]
+            if ids:
+                self.table_host[s, :len(ids)] = torch.tensor(self.owned[s], dtype=torch.int32)
+        self.commit()
+
+    def compact(self) -> int:
+        """Moves pages so that those in use have the lowest ids, and returns how many they are. Tables that the caller has of its own (a copy
+        of a row of ``block_table``, the page ids of a shared prefix) have to be read again."""
+        to = self.alloc.compact()
+        moves = [(a, b) for a, b in enumerate(to) if b not in (-1, a)]
+        paged.copy_pages(paged.PagePools(self.pools), [a for a, _ in moves], [b for _, b in moves])
+        self._renumber(to)
+        return sum(b >= 0 for b in to)
+
+    def resize(self, n_blocks: int) -> None:
+        """Pools of ``n_blocks`` pages, more or fewer, with what the sequences hold; MemoryError if that is more. Pages are numbered anew as
+        by ``compact``, and the pools are other tensors: what was captured into a graph with the old ones still uses those."""
+        old = self.pools
+        live = self.alloc.n_blocks - self.alloc.num_free()
+        if n_blocks < max(live, 1):
+            raise MemoryError(f"{live} pages in use do not fit into {n_blocks}")
+        new = [torch.zeros((n_blocks, *p.shape[1:]), dtype=p.dtype, device=p.device) for p in old]
+        to = self.alloc.compact(n_blocks)
+        pairs = [(a, b) for a, b in enumerate(to) if b >= 0]
+        paged.copy_pages(paged.PagePools(old), [a for a, _ in pairs], [b for _, b in pairs], out=paged.PagePools(new))
+        self.pools[:] = new
+        self._renumber(to)
 
 
 class _WidenAhead:
