@@ -350,18 +350,32 @@ class InferenceEngine:
         cache.commit()
         seq_of = torch.arange(B, dtype=torch.int32, device=self.dev).repeat_interleave(P)
         pos = torch.arange(P, dtype=torch.int32, device=self.dev).repeat(B)
-        x = ops.embed_fwd(self.embed, tok.reshape(-1))
+        x = self._prompt_layers(tok.reshape(-1), seq_of, pos,
+                                lambda li, qkv: att.attention_fwd(qkv, B, P, H, Hkv, dh, causal=True, want_lse=False)[0])
+        last = x.view(B, P, -1)[:, -1, :].contiguous()
+        logits = self.logits[:B]
+        self._head(last, logits, rms_weight=self.rms_final)
+        D.argmax_rows(logits, out_tokens=self.tokens[:B])
+        cache.seq_len[:B] = P
+        return logits
+
+    def _prompt_layers(self, tok, seq_of, pos, attend):
+        """All layers over prompt tokens: ``tok`` [n], token i at position ``pos[i]`` of sequence ``seq_of[i]``. Keys and values go to the
+        cache, then ``attend(layer, qkv)`` is the attention. Returns the residual stream [n, d]."""
+        cfg, cache = self.cfg, self.cache
+        H, Hkv, dh, n = self.H, self.Hkv, cfg.head_dim, tok.shape[0]
+        x = ops.embed_fwd(self.embed, tok)
         products = self._products()
         gates = products in GATED_PRODUCTS
-        ahead = products == _OWN_PRODUCTS and x.is_cuda and B * P < self._ahead_below
-        plan = _WidenAhead(self.layers if ahead else [], B * P)
+        ahead = products == _OWN_PRODUCTS and x.is_cuda and n < self._ahead_below
+        plan = _WidenAhead(self.layers if ahead else [], n)
 
         def attention(li, l, x):
             h, _ = ops.rmsnorm_fwd(x, l["rms1"], cfg.eps, want_inv=False)
             w, kw = plan.product(l["wqkv"])
             qkv = self._linear(h, w, **kw)
             D.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table, cache.page, seq_of, pos)
-            a, _ = att.attention_fwd(qkv, B, P, H, Hkv, dh, causal=True, want_lse=False)
+            a = attend(li, qkv)
             w, kw = plan.product(l["wo"])
             return self._proj_out(a, w, x, site="attn", **kw)
 
@@ -379,13 +393,8 @@ class InferenceEngine:
             x = plan.run(attention, li, l, x)
             x = plan.run(feed_forward, l, x)
         if plan.ran_out:
-            self._ahead_below = B * P
-        last = x.view(B, P, -1)[:, -1, :].contiguous()
-        logits = self.logits[:B]
-        self._head(last, logits, rms_weight=self.rms_final)
-        D.argmax_rows(logits, out_tokens=self.tokens[:B])
-        cache.seq_len[:B] = P
-        return logits
+            self._ahead_below = n
+        return x
 
     def _head(self, hn, logits, rms_weight=None):
         """logits[M, V] (fp32) = norm(hn) @ head; ``rms_weight`` asks for the final RMSNorm to be
@@ -424,8 +433,12 @@ class InferenceEngine:
                 qkv = self._linear(h, l["wqkv"])
             D.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table, cache.page,
                              seq_of, pos)
-            a = D.decode_attention(qkv, cache.pools[li], cache.block_table, cache.page, self._len_plus1[:B], H, Hkv,
-                                   dh, max_len=max_len, stream=stream)
+            if self._shared is not None:
+                a = paged.shared_prefix_attention(qkv, cache.pools[li], cache.block_table[:B], cache.page, self._len_plus1[:B], *self._shared,
+                                                  H, Hkv, dh, max_len=max_len)
+            else:
+                a = D.decode_attention(qkv, cache.pools[li], cache.block_table, cache.page, self._len_plus1[:B], H, Hkv,
+                                       dh, max_len=max_len, stream=stream)
             x = self._proj_out(a, l["wo"], x, site="attn")
             if small:
                 gu = D.gemv(x, l["wgu"], rms_weight=l["rms2"], eps=cfg.eps)
@@ -491,10 +504,6 @@ class InferenceEngine:
         for b in range(B):
             self.cache.reserve(b, P + max_new)
         self.cache.commit()
-        out = torch.zeros((B, max_new), dtype=torch.int64, device=self.dev)
-        self._seq_of = torch.arange(self.max_batch, dtype=torch.int32, device=self.dev)
-        self._len_plus1 = torch.zeros(self.max_batch, dtype=torch.int32, device=self.dev)
-        self._generated = None
         sampler = None
         if not greedy:
             sampler = DeviceSampler(params, B, self.cfg.vocab_size, [seed + b for b in range(B)], self.dev,
@@ -502,12 +511,20 @@ class InferenceEngine:
             sampler.set_history(prompts)
             sampler.sample(logits[:B], out_tokens=self.tokens[:B])
             sampler.push(self.tokens[:B])
+        return self._decode_steps(B, P, max_new, sampler)
+
+    def _decode_steps(self, B: int, P: int, max_new: int, sampler):
+        """The tokens [B, max_new] from the first one, which is in ``self.tokens``, on; the longest of the sequences holds ``P``."""
+        out = torch.zeros((B, max_new), dtype=torch.int64, device=self.dev)
+        self._seq_of = torch.arange(self.max_batch, dtype=torch.int32, device=self.dev)
+        self._len_plus1 = torch.zeros(self.max_batch, dtype=torch.int32, device=self.dev)
+        self._generated = None
         out[:, 0] = self.tokens[:B]
         max_len = P + max_new
         stream = self._streams(B, P + 1)
 
         def crosses(i):
-            return max_new - i >= self.RECAPTURE_STEPS and self._streams(B, P + i) != stream
+            return self._shared is None and max_new - i >= self.RECAPTURE_STEPS and self._streams(B, P + i) != stream
 
         if self.use_graph and max_new > 2:
             # one eager step on the capture stream warms every workspace (they are kept per stream, and nothing may be
@@ -547,6 +564,89 @@ class InferenceEngine:
                 self._step_eager(B, max_len, sampler, stream=stream)
                 out[:, i] = self.tokens[:B]
         _lib.check_status(self.dev) if self.dev.type == "cuda" else None
+        return out
+
+    # ------------------------------------------------------------------ many sequences from one prefix
+    _shared = None                       # (page ids, positions) of the prefix that the sequences of the running generation have in common
+
+    def _shares(self, B: int, P: int) -> bool:
+        """Whether the attention that reads a common prefix of ``P`` positions once beats ``decode_attention``, which reads it for each of
+        ``B`` sequences (from the cache of the chip, while it fits). Its second launch costs about 5 us, so what the others need not read
+        again has to be worth that. us in a graph, 32 positions behind the prefix, decode / shared, 32 / 8 heads of 128:
+        4 x 2048 13.8 / 14.1, 4 x 4096 18.1 / 16.8, 8 x 1024 13.9 / 15.3, 8 x 2048 18.4 / 15.5, 16 x 512 14.3 / 15.6, 16 x 1024 18.9 / 16.4,
+        64 x 256 22.7 / 29.7, 64 x 1024 49.4 / 31.6, 64 x 8192 304 / 42.7, 2 x 8192 17.3 / 20.2; 16 / 16 heads of 64: 16 x 512 15.1 / 15.4,
+        16 x 1024 21.6 / 19.3, 64 x 512 29.5 / 39.4, 64 x 1024 51.8 / 42.4; 8 / 1 heads of 128: 64 x 1024 16.7 / 19.3, 64 x 2048 21.2 / 21.0."""
+        return P >= 1024 and (B - 1) * P * self.Hkv * self.cfg.head_dim * 4 >= 45 << 20
+
+    def generate_shared(self, prefix: torch.Tensor, suffixes, max_new: int, params: SamplingParams | None = None, seed: int = 0):
+        """Generation for sequences that begin alike. ``prefix`` [P] goes through the model once, and its pages of the cache are shared;
+        ``suffixes`` is how many samples of it are wanted, or what each sequence has behind it: a matrix [B, S], or a list of B vectors of
+        any lengths, empty ones too. Sequence b samples from the stream seeded with ``seed + b``. Returns int64 [B, max_new].
+
+        The same tokens as ``generate`` on the whole prompts, but for roundings (another kernel reads the prefix)."""
+        params = params or SamplingParams()
+        prefix = prefix.reshape(-1)
+        P = prefix.numel()
+        if isinstance(suffixes, int):
+            suffixes = [prefix[:0]] * suffixes
+        suffixes = [torch.as_tensor(s).reshape(-1).to(prefix.dtype) for s in suffixes]
+        B, lens = len(suffixes), [s.numel() for s in suffixes]
+        if B < 1 or P < 1 or max_new < 1:
+            raise ValueError("a prefix, one sequence and one new token at least")
+        longest = P + max(lens)
+        if B > self.max_batch or longest + max_new > self.max_seq:
+            raise ValueError("request exceeds the engine's max_batch / max_seq")
+        cache, dev = self.cache, self.dev
+        for b in range(self.max_batch):                # pages that another generation has left
+            if cache.owned[b]:
+                cache.release(b)
+        logits = self.prefill(prefix[None]).clone()
+        cache.fork(0, range(1, B), P)
+        for b in range(B):
+            cache.reserve(b, P + lens[b] + max_new)
+        cache.commit()
+        greedy = params.temperature <= 0.0 and params.repetition_penalty <= 1.0
+        shared = (cache.block_table[0, :P // cache.page].clone(), P)
+        logits = self._extend(suffixes, lens, P, shared, logits.expand(B, -1))
+        sampler = None
+        if greedy:
+            D.argmax_rows(logits, out_tokens=self.tokens[:B])
+        else:
+            sampler = DeviceSampler(params, B, self.cfg.vocab_size, [seed + b for b in range(B)], dev, history_len=longest + max_new)
+            sampler.history[:, :P] = prefix.to(dev)
+            for b, s in enumerate(suffixes):
+                sampler.history[b, P:P + lens[b]] = s.to(dev)
+            sampler.n_hist.copy_(torch.tensor([P + n for n in lens], dtype=torch.int32))
+            sampler.sample(logits, out_tokens=self.tokens[:B])
+            sampler.push(self.tokens[:B])
+        cache.seq_len[:B] = torch.tensor([P + n for n in lens], dtype=torch.int32, device=dev)
+        self._shared = shared if self._shares(B, P) else None
+        try:
+            return self._decode_steps(B, longest, max_new, sampler)
+        finally:
+            self._shared = None
+
+    def _extend(self, suffixes, lens, P, shared, logits):
+        """The layers over what the sequences have behind the prefix, all in one pass; returns their last positions' logits [B, V], those
+        given where a sequence has nothing."""
+        B, cache, dev = len(lens), self.cache, self.dev
+        out = self.logits[:B]
+        out.copy_(logits)
+        if sum(lens) == 0:
+            return out
+        tok = torch.cat(suffixes).to(dev)
+        n = torch.tensor(lens, dtype=torch.int32)
+        ends = torch.cat([n[:1] * 0, n.cumsum(0, dtype=torch.int32)])
+        seq_of = torch.arange(B, dtype=torch.int32).repeat_interleave(n.long())
+        pos = torch.arange(tok.numel(), dtype=torch.int32) - ends[:-1].repeat_interleave(n.long()) + P
+        seq_of, pos, cu, total = seq_of.to(dev), pos.to(torch.int32).to(dev), ends.to(dev), (n + P).to(dev)
+        x = self._prompt_layers(tok, seq_of, pos, lambda li, qkv: paged.shared_prefix_attention(
+            qkv, cache.pools[li], cache.block_table[:B], cache.page, total, *shared, self.H, self.Hkv, self.cfg.head_dim, cu_q=cu, max_len=P + max(lens)))
+        some = [b for b in range(B) if lens[b]]
+        last = x[torch.tensor([int(ends[b + 1]) - 1 for b in some], device=dev)].contiguous()
+        got = torch.empty((len(some), out.shape[1]), dtype=out.dtype, device=dev)
+        self._head(last, got, rms_weight=self.rms_final)
+        out[torch.tensor(some, device=dev)] = got
         return out
 
 

@@ -318,3 +318,45 @@ def test_many_copies():
     n = 70000
     paged.copy_pages([pool], torch.arange(n, dtype=torch.int32, device=DEV), torch.arange(n, 2 * n, dtype=torch.int32, device=DEV))
     assert torch.equal(pool[:n], pool[n:])
+
+
+@pytest.mark.parametrize("P, lens", [(100, (5, 0, 130, 1)), (256, (0, 0, 0)), (9, (3, 40))])
+def test_generation_behind_a_shared_prefix(monkeypatch, P, lens):
+    """Prefill, fork, attention over the suffixes and decode steps together: each call of the attention against its statement, the graph
+    against eager steps, and the first logits against those of whole prompts (about 40 roundings of 2^-9 rms on either side of a
+    difference, independent: 2^-9 * sqrt(80) = 0.017 of the logits' size; twice that is allowed)."""
+    from scirust_b200.generate import SamplingParams
+    from scirust_b200.models.infer import InferenceEngine
+    from scirust_b200.models.sciagent import GQADecoder, SciAgentConfig
+    model = GQADecoder(SciAgentConfig(256, 256, 2, 4, 2, 384, 512, 10000.0), device=DEV, seed=5, init_std=0.08)
+    g = torch.Generator().manual_seed(P)
+    prefix = torch.randint(1, 256, (P,), generator=g).to(DEV)
+    suffixes = [torch.randint(1, 256, (n,), generator=g).to(DEV) for n in lens]
+    B, calls, op = len(lens), [], paged.shared_prefix_attention
+
+    def checked(q, pool, table, page, length, prefix_table, prefix_len, H, Hkv, dh, cu_q=None, max_len=None):
+        o = op(q, pool, table, page, length, prefix_table, prefix_len, H, Hkv, dh, cu_q=cu_q, max_len=max_len)
+        o64, bound = statement(dict(q=q, pool=pool, block_table=table, page=page, seq_len=length, H=H, Hkv=Hkv, dh=dh, cu_q=cu_q))
+        assert bool(((o.to(F64) - o64).abs() <= bound).all())
+        calls.append(cu_q is not None)
+        return o
+
+    eager = InferenceEngine(model, max_batch=B + 1, max_seq=512, page=16, use_graph=False)
+    graph = InferenceEngine(model, max_batch=B + 1, max_seq=512, page=16)
+    for e in (eager, graph):
+        monkeypatch.setattr(e, "_shares", lambda B, P: True)
+    for params in (None, SamplingParams(0.9, 20, 0.95, 1.1)):
+        with monkeypatch.context() as m:
+            m.setattr(paged, "shared_prefix_attention", checked)
+            want = eager.generate_shared(prefix, suffixes, 6, params, seed=2)
+        assert sum(calls) == (2 if sum(lens) else 0) and len(calls) - sum(calls) == 2 * 5
+        calls.clear()
+        for _ in range(2):
+            assert torch.equal(graph.generate_shared(prefix, suffixes, 6, params, seed=2), want)
+    seen = []
+    monkeypatch.setattr(eager, "_decode_steps", lambda *a: seen.append(eager.logits[:B].float().clone()))
+    eager.generate_shared(prefix, suffixes, 6)
+    for b in range(B):
+        whole = graph.prefill(torch.cat([prefix, suffixes[b]])[None])[0].float()
+        assert (seen[0][b] - whole).norm() <= 0.034 * whole.norm()
+        graph.cache.release(0)
