@@ -162,12 +162,20 @@ def cmd_infer(a):
     if not ids:
         sys.stderr.write("error: empty prompt\n")
         return EXIT_VALIDATION
-    eng = InferenceEngine(model, quant=a.quant, max_batch=1, max_seq=len(ids) + a.max_new + 1)
+    samples = getattr(a, "samples", 1)
+    if samples < 1:
+        sys.stderr.write("error: --samples must be positive\n")
+        return EXIT_VALIDATION
+    eng = InferenceEngine(model, quant=a.quant, max_batch=samples, max_seq=len(ids) + a.max_new + 1)
     params = SamplingParams(a.temperature, a.top_k, a.top_p, a.repetition_penalty)
-    out = eng.generate(torch.tensor([ids]), a.max_new, params, seed=a.seed)[0].tolist()
-    if 0 in out:
-        out = out[:out.index(0)]      # token 0 stops generation
-    print(tok.decode(out) if tok else " ".join(str(t) for t in out))
+    if samples == 1:
+        outs = eng.generate(torch.tensor([ids]), a.max_new, params, seed=a.seed).tolist()
+    else:                             # sample b draws from the stream of seed + b; the prompt is computed and read once
+        outs = eng.generate_shared(torch.tensor(ids), samples, a.max_new, params, seed=a.seed).tolist()
+    for out in outs:
+        if 0 in out:
+            out = out[:out.index(0)]  # token 0 stops generation
+        print(tok.decode(out) if tok else " ".join(str(t) for t in out))
     return EXIT_OK
 
 
@@ -734,6 +742,7 @@ def build_parser():
         sp.add_argument("--tokenizer", default="")
         sp.add_argument("--prompt", default="")
         sp.add_argument("--max-new", type=int, default=32)
+        sp.add_argument("--samples", type=int, default=1, help="continuations of the prompt, one a line")
         sp.add_argument("--temperature", type=float, default=0.0)
         sp.add_argument("--top-k", type=int, default=0)
         sp.add_argument("--top-p", type=float, default=1.0)

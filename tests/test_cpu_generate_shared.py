@@ -60,6 +60,18 @@ def test_refusals(model):
             eng.generate_shared(*args)
 
 
+def test_command_prints_a_line_for_each_sample(model, tmp_path, capsys):
+    from scirust_b200 import cli
+    from scirust_b200.io import checkpoint as CK
+    CK.save_sciagent_checkpoint(model, tmp_path / "step_1", step=1, loss=0.0, lr=0.0)
+    args = ["infer", "--checkpoint", str(tmp_path / "step_1"), "--prompt", "1 2 3 4 5 6 7 8 9", "--max-new", "4", "--device", "cpu"]
+    assert cli.run(args) == 0
+    one = capsys.readouterr().out.splitlines()
+    assert cli.run(args + ["--samples", "3"]) == 0
+    assert capsys.readouterr().out.splitlines() == one * 3           # greedy
+    assert cli.run(args + ["--samples", "0"]) != 0
+
+
 @pytest.mark.parametrize("H, Hkv, B, P, want", [(32, 8, 4, 2048, False), (32, 8, 4, 4096, True), (32, 8, 2, 8192, False), (32, 8, 8, 1024, False),
                                                 (32, 8, 16, 1024, True), (32, 8, 64, 512, False), (8, 1, 64, 1024, False), (8, 1, 64, 2048, True)])
 def test_rule_of_which_attention_runs(H, Hkv, B, P, want):
