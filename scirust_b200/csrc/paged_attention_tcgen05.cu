@@ -40,7 +40,8 @@ constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * 168, "the shares draw on the registers of the launch");
 constexpr int TMEM_COLS = 512;
 constexpr int QUEUE = 4;       // pieces that the producer may be ahead
-constexpr int ITEM_UNITS = 2;
+// What an item costs besides its blocks, in units (below): where a row has four parts, with one tile, with two.
+constexpr int ITEM_SPLIT = 2, ITEM_ONE = 3, ITEM_TWO = 5;
 // A row's reference is its running maximum, so its largest weight is 1 and loses nothing when weights become bf16, and the sum is one of
 // weights before that. A reference that may lag behind by 2^8 saves rescales of O: 2 us of 64 (64 sequences behind 16384 positions), for an
 // error of 2.2e-3 in place of 2.0e-3 on unit scores and 1.3e-3 in place of 0.5e-3 on scores of four times the spread; with a sum of the
@@ -72,8 +73,8 @@ struct Pair {
   int t0, n, b, kend;
 };
 
-struct Header {        // at the start of the workspace
-  int units, units_shared, q_lo, q_hi, pairs;
+struct Header {        // at the start of the workspace, of a batch that has been planned
+  int units_shared, units_own, q_lo, q_hi, pairs;
   int least;           // no row sees fewer positions
   int pad[2];
 };
@@ -103,8 +104,11 @@ struct Params {
   Pair* pair;
   int* row_limit;      // [NT]
   int* row_pair;       // [NT], -1: of no sequence
+  int2* part;          // [Hkv][shared tiles] and then [pairs][Hkv]: CTAs that have a piece of the item; the first of these, times two, 1 for its second piece
+  int* row_t0;         // [NT] first token of its pair
   float* whole;        // [slots][NT][H][dh], and [slots][NT][H][2] behind it: items that were not cut, shared and then own
   float* cut;          // [2 * CTAs][256][dh], and [2 * CTAs][256][2] behind it: first and last pieces of the CTAs
+  int shared_items;    // entries of `part` that shared items have
   int max_pairs;
   int* status;
 };
@@ -154,37 +158,56 @@ __device__ __forceinline__ int quotient(int a, int d) {
   return q;
 }
 
-// The even deal of `units` over `ctas`: the first `rem` of them get one more. Two units at least, so that a CTA between the ends of an
-// item has a block of it, whose two units may lie with two CTAs (the first unit's CTA has the block).
+__device__ __forceinline__ int blocks_of(int positions) { return positions > 0 ? (positions + BN - 1) / BN : 0; }
+// An item lies in the line with one unit for a block of one tile of rows, two for a block of two, and in front of them what it costs
+// besides its blocks.
+__device__ __forceinline__ int head_units(int n_tok, int TT, bool split) { return split ? ITEM_SPLIT : n_tok > TT ? ITEM_TWO : ITEM_ONE; }
+__device__ __forceinline__ int units_of(int positions, int n_tok, int TT, bool split) {
+  return positions > 0 ? (blocks_of(positions) << (n_tok > TT ? 1 : 0)) + head_units(n_tok, TT, split) : 0;
+}
+
+// The deal of the line over the CTAs: shared items to the first of them, own ones to the others, the units of either evenly. A CTA also
+// has to begin a piece that its neighbour's share has cut, which is dearer for shared items (of two tiles) than for own ones (of a few
+// rows). With U and V units, `more` units dearer: U / n + more = V / (ctas - n) for n CTAs.
+// At least two units a CTA, so that one between the ends of an item has a block of it, whose two units may lie with two CTAs (the first
+// unit's CTA has the block).
 struct Deal {
-  int units, per, rem;
-  __device__ Deal(int units_, int ctas) : units(units_) {
-    ctas = min(ctas, max(1, units >> 1));
-    per = quotient(units, ctas);
-    rem = units - per * ctas;
+  int shared, ctas[2], per[2], rem[2];     // units of the first part of the line
+  __device__ Deal(int units_shared, int units_own, int grid, int more) : shared(units_shared) {
+    int n = units_shared > 0 ? grid : 0;
+    if (units_shared > 0 && units_own > 0) {
+      const float U = units_shared, V = units_own, N = grid, b = more * N - U - V;
+      n = clampi(__float2int_ru(2.f * U * N / (sqrtf(b * b + 4.f * more * U * N) - b)), 1, grid - 1);
+    }
+    ctas[0] = n;
+    ctas[1] = grid - n;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int units = i ? units_own : units_shared, share = max(1, min(ctas[i], units >> 1));
+      per[i] = quotient(units, share);
+      rem[i] = units - per[i] * share;
+    }
   }
-  __device__ int begin(int c) const { return min(units, c * per + min(c, rem)); }
+  // The share of CTA c is [begin, end) of the line.
+  __device__ void share(int c, int units_own, int& begin, int& end) const {
+    const int i = c < ctas[0] ? 0 : 1, k = i ? c - ctas[0] : c, units = i ? units_own : shared, from = i ? shared : 0;
+    begin = from + min(units, k * per[i] + min(k, rem[i]));
+    end = from + min(units, (k + 1) * per[i] + min(k + 1, rem[i]));
+  }
   __device__ int owner(int u) const {
-    const int edge = rem * (per + 1);
-    const bool low = u < edge;
-    return quotient(low ? u : u - edge, low ? per + 1 : max(per, 1)) + (low ? 0 : rem);
+    const int i = u < shared ? 0 : 1, v = i ? u - shared : u, edge = rem[i] * (per[i] + 1);
+    const bool low = v < edge;
+    return (i ? ctas[0] : 0) + quotient(low ? v : v - edge, low ? per[i] + 1 : max(per[i], 1)) + (low ? 0 : rem[i]);
   }
 };
-
-__device__ __forceinline__ int blocks_of(int positions) { return positions > 0 ? (positions + BN - 1) / BN : 0; }
-// Units that an item takes in the line: one for a block of one tile of rows, two for a block of two, and what an item costs besides
-// its blocks in front of them.
-__device__ __forceinline__ int units_of(int positions, int n_tok, int TT) {
-  return positions > 0 ? (positions + BN - 1) / BN * (n_tok > TT ? 2 : 1) + ITEM_UNITS : 0;
-}
 
 // The shared items of one kv head: tiles of two times TT tokens, the last of which may have one tile of rows.
 struct Shared {
   int tiles, size, last, head;        // items of a head, units of an item and of the last one, of a head
-  __device__ Shared(int prefix, int tokens, int TT) {
+  __device__ Shared(int prefix, int tokens, int TT, bool split) {
     tiles = prefix > 0 ? quotient(tokens + 2 * TT - 1, 2 * TT) : 0;
-    size = units_of(prefix, 2 * TT, TT);
-    last = units_of(prefix, tokens - (tiles - 1) * 2 * TT, TT);
+    size = units_of(prefix, 2 * TT, TT, false);
+    last = units_of(prefix, tokens - (tiles - 1) * 2 * TT, TT, split);
     head = tiles > 0 ? (tiles - 1) * size + last : 0;
   }
 };
@@ -224,12 +247,13 @@ struct Walk {
   const Shared shared;
   int units_shared, q_lo, q_hi, pairs;
   int u, u1, u_first;
+  int begin, last, index;        // of the item: where it lies in the line, the first unit of its last block, its entry of p.part
   int window, c_lo, c_hi;        // pairs window + lane: units of one kv head before and behind
   int4 info;
 
   __device__ Walk(const Params& p_, const Header& h, int u0, int u1_)
-      : p(p_), shared(p_.prefix, h.q_hi - h.q_lo, p_.TT), units_shared(h.units_shared), q_lo(h.q_lo), q_hi(h.q_hi), pairs(h.pairs), u(u0),
-        u1(u1_), u_first(u0), window(-1), c_lo(0), c_hi(0), info(make_int4(0, 0, 0, 0)) {}
+      : p(p_), shared(p_.prefix, h.q_hi - h.q_lo, p_.TT, (p_.split & 2) != 0), units_shared(h.units_shared), q_lo(h.q_lo), q_hi(h.q_hi), pairs(h.pairs), u(u0),
+        u1(u1_), u_first(u0), begin(0), last(0), index(0), window(-1), c_lo(0), c_hi(0), info(make_int4(0, 0, 0, 0)) {}
 
   __device__ void planned(int from, int lane) {
     window = from;
@@ -245,7 +269,7 @@ struct Walk {
     window = from;
     const int b = from + lane;
     const int len = b < pairs ? clampi(p.seq_len[b], 0, p.max_blocks * p.page) : 0;
-    const int n = units_of(len - p.prefix, 1, p.TT);
+    const int n = units_of(len - p.prefix, 1, p.TT, p.split & 1);
     c_hi = before + warp_scan(n, lane);
     c_lo = c_hi - n;
     info = make_int4(b, 1, b, len);
@@ -266,6 +290,7 @@ struct Walk {
         size = tile == shared.tiles - 1 ? shared.last : shared.size;
         x.t0 = q_lo + tile * 2 * p.TT;
         x.n_tok = min(2 * p.TT, q_hi - x.t0);
+        index = x.h * shared.tiles + tile;
         x.kbase = 0;
         x.kend = p.prefix;
         x.flags |= PIECE_SHARED;
@@ -299,16 +324,20 @@ struct Walk {
         x.n_tok = __shfl_sync(0xffffffffu, info.y, l);
         x.kend = __shfl_sync(0xffffffffu, info.w, l);
         x.kbase = p.prefix;
+        index = p.shared_items + (window + l) * p.Hkv + x.h;
         x.flags |= __shfl_sync(0xffffffffu, info.z, l) << SEQUENCE;
       }
       const int stop = min(size, off + (u1 - u));
+      begin = u - off;
       u += stop - off;
       // a block belongs to the CTA that has its first unit
       const int two = x.n_tok > p.TT ? 1 : 0;
-      x.j0 = (max(0, off - ITEM_UNITS) + two) >> two;
-      x.j1 = (max(0, stop - ITEM_UNITS) + two) >> two;
+      const int head = head_units(x.n_tok, p.TT, is_split(p, x)), blocks = (size - head) >> two;
+      x.j0 = (max(0, off - head) + two) >> two;
+      x.j1 = (max(0, stop - head) + two) >> two;
       if (x.j1 == x.j0) continue;
-      if (x.j1 - x.j0 != (size - ITEM_UNITS) >> two) x.flags |= PIECE_CUT;
+      if (x.j1 - x.j0 != blocks) x.flags |= PIECE_CUT;
+      last = begin + head + ((blocks - 1) << two);
       return true;
     }
   }
@@ -380,11 +409,12 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
     for (int r = lane; r < x.y; r += 32) {
       p.row_limit[x.x + r] = x.w - x.y + r + 1;
       p.row_pair[x.x + r] = i;
+      p.row_t0[x.x + r] = x.x;
     }
   }
   for (int i0 = 0; i0 < pairs; i0 += 1024) {
     const int i = i0 + tid;
-    const int n = i < pairs ? units_of(p.pair[i].kend - p.prefix, p.pair[i].n, p.TT) : 0;
+    const int n = i < pairs ? units_of(p.pair[i].kend - p.prefix, p.pair[i].n, p.TT, false) : 0;
     const int scan = warp_scan(n, lane);
     if (lane == 31) s_warp[warp] = scan;
     __syncthreads();
@@ -397,9 +427,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   }
   if (tid == 0) {
     p.cum[pairs] = s_sum;
-    const int shared = p.Hkv * Shared(p.prefix, q_hi - q_lo, p.TT).head;
-    p.hdr->units = shared + p.Hkv * s_sum;
-    p.hdr->units_shared = shared;
+    p.hdr->units_shared = p.Hkv * Shared(p.prefix, q_hi - q_lo, p.TT, false).head;
+    p.hdr->units_own = p.Hkv * s_sum;
     p.hdr->q_lo = q_lo; p.hdr->q_hi = q_hi; p.hdr->pairs = pairs;
     p.hdr->least = s_least;
   }
@@ -535,7 +564,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     // -------------------------------- pieces, their rows, and K --------------------------------
     Header hdr;
     if (p.pair) {
-      hdr.units = p.hdr->units; hdr.units_shared = p.hdr->units_shared;
+      hdr.units_shared = p.hdr->units_shared; hdr.units_own = p.hdr->units_own;
       hdr.q_lo = p.hdr->q_lo; hdr.q_hi = p.hdr->q_hi; hdr.pairs = p.hdr->pairs; hdr.least = p.hdr->least;
     } else {
       const int cap = p.max_blocks * p.page;
@@ -544,23 +573,19 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int b = b0 + lane;
         const int len = b < p.B ? clampi(p.seq_len[b], 0, cap) : INT_MAX;
-        const int n = b < p.B ? units_of(len - p.prefix, 1, p.TT) : 0;
+        const int n = b < p.B ? units_of(len - p.prefix, 1, p.TT, p.split & 1) : 0;
         least = min(least, len);
-        const int scan = warp_scan(n, lane);
-        if (blockIdx.x == 0 && b < p.B) p.cum[b] = sum + scan - n;        // for the joining launch
-        sum += __shfl_sync(0xffffffffu, scan, 31);
+        sum += __reduce_add_sync(0xffffffffu, n);
       }
       hdr.q_lo = 0; hdr.q_hi = p.B; hdr.pairs = p.B; hdr.least = __reduce_min_sync(0xffffffffu, least);
-      hdr.units_shared = p.Hkv * Shared(p.prefix, p.B, p.TT).head;
-      hdr.units = hdr.units_shared + p.Hkv * sum;
-      if (blockIdx.x == 0 && lane == 0) {
-        p.cum[p.B] = sum;
-        p.hdr->units = hdr.units; p.hdr->units_shared = hdr.units_shared;
-        p.hdr->q_lo = 0; p.hdr->q_hi = p.B; p.hdr->pairs = p.B;
-      }
+      hdr.units_shared = p.Hkv * Shared(p.prefix, p.B, p.TT, (p.split & 2) != 0).head;
+      hdr.units_own = p.Hkv * sum;
     }
-    const Deal deal(hdr.units, gridDim.x);
-    Walk walk(p, hdr, deal.begin(blockIdx.x), deal.begin(blockIdx.x + 1));
+    const Deal deal(hdr.units_shared, hdr.units_own, gridDim.x,
+                    head_units(hdr.q_hi - hdr.q_lo, p.TT, (p.split & 2) != 0) - head_units(1, p.TT, p.split & 1));
+    int u0, u1;
+    deal.share(blockIdx.x, hdr.units_own, u0, u1);
+    Walk walk(p, hdr, u0, u1);
     Ring k(sK, k_full, k_empty, KS);
     int n_pieces = 0;
     bool ok = true, both = false;
@@ -579,6 +604,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       __syncwarp();
       if (++at == QUEUE) { at = 0; at_phase ^= 1; }
       if (!more) break;
+      if (x.j0 == 0 && lane == 0)          // for the joining launch
+        p.part[walk.index] = make_int2(x.flags & PIECE_CUT ? deal.owner(walk.last) - static_cast<int>(blockIdx.x) + 1 : 1,
+                                       2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1));
       const bool two = x.n_tok > p.TT;
       k.piece(p, x, x.h);
 #pragma unroll 1
@@ -1001,59 +1029,52 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
   pdl_wait();
   if (t >= p.NT) return;
   const int pair = p.pair ? p.row_pair[t] : t;
-  const int units = p.hdr->units, units_shared = p.hdr->units_shared, q_lo = p.hdr->q_lo, q_hi = p.hdr->q_hi;
   if (pair < 0) {                          // a row of no sequence
     if (p.fill)
       for (int i = PACKED ? lane : threadIdx.x; i < p.G * DH; i += PACKED ? 32 : 32 * ROWS * WAYS)
         p.out[t * p.ldo + h * p.G * DH + i] = __float2bfloat16_rn(0.f);
     return;
   }
-  const Deal deal(units, ctas);
   // The row's two items: parts, where the first lies and those of the CTAs behind it, which begin with theirs.
-  const Shared shared(p.prefix, q_hi - q_lo, p.TT);
+  int q_lo = 0, q_hi = p.NT, t0 = t, kend;
+  if (p.pair) {
+    q_lo = p.hdr->q_lo;
+    q_hi = p.hdr->q_hi;
+    t0 = p.row_t0[t];
+    kend = p.pair[pair].kend;
+  } else {
+    kend = clampi(p.seq_len[t], 0, p.max_blocks * p.page);
+  }
+  const int2 own = p.part[p.shared_items + pair * p.Hkv + h];
+  int2 common = make_int2(0, 0);
+  int first = 0;                           // token of the shared item
+  if (p.prefix > 0) {
+    const int tile = quotient(t - q_lo, 2 * p.TT);
+    common = p.part[h * quotient(q_hi - q_lo + 2 * p.TT - 1, 2 * p.TT) + tile];
+    first = q_lo + tile * 2 * p.TT;
+  }
   int n[2];
   const float* from[2];
   const float2* ml[2];
   int jump[2];                             // rows from the first part to the second, which is 4 * BM in front of the third
   int fold[2], apart[2];                   // log2 of the parts that a CTA has of an item, rows between them
-#pragma unroll 1
+#pragma unroll
   for (int i = 0; i < 2; ++i) {
-    int beg, size, t0, tokens;
-    if (i == 0) {
-      const int tile = quotient(t - q_lo, 2 * p.TT);
-      beg = h * shared.head + tile * shared.size;
-      size = tile == shared.tiles - 1 ? shared.last : shared.size;
-      t0 = q_lo + tile * 2 * p.TT;
-      tokens = min(2 * p.TT, q_hi - t0);
-      if (p.prefix == 0) size = 0;
-    } else {
-      const int before = p.cum[pair];
-      size = p.cum[pair + 1] - before;
-      beg = units_shared + before * p.Hkv + h * size;
-      t0 = p.pair ? p.pair[pair].t0 : t;
-      tokens = p.pair ? p.pair[pair].n : 1;
-    }
-    const int two = tokens > p.TT ? 1 : 0, tok = t - t0;
-    const int log = p.split & (i ? 1 : 2) ? 2 : 0;
-    int count = 0, skip = 0;
-    size_t at = 0;
-    bool cut = false;
-    if (size > 0) {
-      const int first = beg + ITEM_UNITS, c0 = deal.owner(first);
-      count = deal.owner(first + ((((size - ITEM_UNITS) >> two) - 1) << two)) - c0 + 1;
-      cut = count > 1;
-      const bool odd = deal.begin(c0) < beg;         // the second piece of its CTA
-      skip = odd ? 2 * BM : 4 * BM;
-      at = cut ? static_cast<size_t>(2 * c0 + (odd ? 1 : 0)) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
-               : (static_cast<size_t>(i ? own_slot(p) : 0) * p.NT + t) * p.H + h * p.G;
-    }
+    // in bounds even where a wait of the other launch has given up and the entry is none
+    int2 x = i ? own : common;
+    x.y = clampi(x.y, 0, 2 * ctas - 1);
+    const int count = i && kend <= p.prefix ? 0 : clampi(x.x, 0, ctas - (x.y >> 1)), tok = t - (i ? t0 : first), log = p.split & (i ? 1 : 2) ? 2 : 0;
+    const bool cut = count > 1;
+    const size_t at = cut ? static_cast<size_t>(x.y) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
+                          : (static_cast<size_t>(i ? own_slot(p) : 0) * p.NT + t) * p.H + h * p.G;
     const size_t rows = cut ? static_cast<size_t>(4) * ctas * BM : static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
     const float* base = cut ? p.cut : p.whole;
-    const float* o = base + at * DH + lane * F;
-    const float2* m = reinterpret_cast<const float2*>(base + rows * DH) + at;
-    const int gap = cut ? 32 : p.NT * p.H;
-    if (i == 0) { n[0] = count << log; from[0] = o; ml[0] = m; jump[0] = skip; fold[0] = log; apart[0] = gap; }
-    else { n[1] = count << log; from[1] = o; ml[1] = m; jump[1] = skip; fold[1] = log; apart[1] = gap; }
+    n[i] = count << log;
+    from[i] = base + at * DH + lane * F;
+    ml[i] = reinterpret_cast<const float2*>(base + rows * DH) + at;
+    jump[i] = x.y & 1 ? 2 * BM : 4 * BM;
+    fold[i] = log;
+    apart[i] = cut ? 32 : p.NT * p.H;
   }
   if (p.prefix == 0 && !p.split && n[1] == 1) return;  // written out by its CTA
   const int parts = n[0] + n[1];
@@ -1154,14 +1175,17 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
 
 // Bytes of the parts of the workspace, in the order in which they lie.
 struct Layout {
-  size_t cum, pair, limit, row_pair, whole, cut, total;
-  Layout(long long NT, int H, int dh, int ctas, int max_pairs, bool planned, int slots) {
+  size_t cum, pair, limit, row_pair, row_t0, part, whole, cut, total;
+  Layout(long long NT, int H, int Hkv, int dh, int ctas, int max_pairs, int shared_items, bool planned, int slots) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    cum = up(sizeof(Header));
-    pair = cum + up((static_cast<size_t>(max_pairs) + 1) * 4);
+    const size_t rows = planned ? up(static_cast<size_t>(NT) * 4) : 0;
+    cum = planned ? up(sizeof(Header)) : 0;
+    pair = cum + (planned ? up((static_cast<size_t>(max_pairs) + 1) * 4) : 0);
     limit = pair + (planned ? up(static_cast<size_t>(max_pairs) * sizeof(Pair)) : 0);
-    row_pair = limit + (planned ? up(static_cast<size_t>(NT) * 4) : 0);
-    whole = row_pair + (planned ? up(static_cast<size_t>(NT) * 4) : 0);
+    row_pair = limit + rows;
+    row_t0 = row_pair + rows;
+    part = row_t0 + rows;
+    whole = part + up((static_cast<size_t>(max_pairs) * Hkv + shared_items) * sizeof(int2));
     cut = whole + up(static_cast<size_t>(slots) * NT * H * (dh + 2) * 4);
     total = cut + up(static_cast<size_t>(4) * ctas * BM * (dh + 2) * 4);
   }
@@ -1193,7 +1217,7 @@ static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
 
 static int ctas_for(long long units) {
   const long long most = num_sms();
-  return static_cast<int>(units < 1 ? 1 : units < most ? units : most);
+  return static_cast<int>(units < 2 ? 2 : units < most ? units : most);      // one for either part of the line
 }
 
 }  // namespace spa
@@ -1208,6 +1232,7 @@ static void sizes(spa::Params& p, int NT, int B, int H, int Hkv, int prefix, boo
   p.q_tokens = NT < p.TT ? NT : p.TT;
   p.q_rows = (p.G * p.q_tokens + 7) / 8 * 8;
   p.max_pairs = ragged ? B + NT / (2 * p.TT) : B;
+  p.shared_items = prefix > 0 ? Hkv * (NT / (2 * p.TT) + 1) : 0;
   p.split = ragged || p.G > 8 ? 0 : NT * p.G > 8 ? 1 : 3;
 }
 static int slots_of(const spa::Params& p) { return p.prefix > 0 || p.split ? spa::whole_slots(p) : 0; }
@@ -1217,7 +1242,7 @@ extern "C" size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv
   if (NT <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > spa::BM) return 0;
   spa::Params p;
   sizes(p, NT, B, H, Hkv, prefix, ragged != 0);
-  return spa::Layout(NT, H, dh, num_sms(), p.max_pairs, ragged != 0, slots_of(p)).total;
+  return spa::Layout(NT, H, Hkv, dh, num_sms(), p.max_pairs, p.shared_items, ragged != 0, slots_of(p)).total;
 }
 
 // q: bf16 [NT, ldq], query heads first, positions already rotated in. pool: n_blocks pages [2, Hkv, page, dh], page a multiple of 8.
@@ -1246,11 +1271,11 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   sizes(p, NT, B, H, Hkv, prefix, planned);
   const int TT = p.TT, max_pairs = p.max_pairs;
   const uint64_t cap = static_cast<uint64_t>(max_blocks) * page;
-  if (static_cast<uint64_t>(Hkv) * max_pairs * (2 * cap / spa::BN + 2 + spa::ITEM_UNITS) + static_cast<uint64_t>(Hkv) * (NT / (2 * TT) + 1) * (2 * prefix / spa::BN + 2 + spa::ITEM_UNITS) >=
-      (1ull << 31))
+  const uint64_t own = 2 * cap / spa::BN + 2 + spa::ITEM_TWO, common = 2 * prefix / spa::BN + 2 + spa::ITEM_TWO;     // units of an item
+  if (Hkv * (max_pairs * own + (NT / (2 * TT) + 1) * common) >= (1ull << 31))
     return SB_ERR_TOO_LARGE;
   const int ctas = spa::ctas_for(max_units);
-  const spa::Layout at(NT, H, dh, ctas, max_pairs, planned, slots_of(p));
+  const spa::Layout at(NT, H, Hkv, dh, ctas, max_pairs, p.shared_items, planned, slots_of(p));
   if (at.total > workspace_bytes) return SB_ERR_ARG;
   int box = 64;
   while (page % box) box >>= 1;
@@ -1263,10 +1288,12 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   p.page = page; p.n_blocks = n_blocks; p.box = box;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo; p.fill = fill;
-  p.hdr = reinterpret_cast<spa::Header*>(ws);
-  p.cum = reinterpret_cast<int*>(ws + at.cum);
+  p.hdr = planned ? reinterpret_cast<spa::Header*>(ws) : nullptr;
+  p.cum = planned ? reinterpret_cast<int*>(ws + at.cum) : nullptr;
   p.pair = planned ? reinterpret_cast<spa::Pair*>(ws + at.pair) : nullptr;
   p.row_limit = planned ? reinterpret_cast<int*>(ws + at.limit) : nullptr;
+  p.row_t0 = planned ? reinterpret_cast<int*>(ws + at.row_t0) : nullptr;
+  p.part = reinterpret_cast<int2*>(ws + at.part);
   p.row_pair = planned ? reinterpret_cast<int*>(ws + at.row_pair) : nullptr;
   p.whole = reinterpret_cast<float*>(ws + at.whole);
   p.cut = reinterpret_cast<float*>(ws + at.cut);
