@@ -33,15 +33,17 @@ namespace spa {
 
 constexpr int BM = 128;        // rows of a tile
 constexpr int BN = 128;        // positions of a block
+constexpr int BN_LOG = 7;
 constexpr int HALF = BN / 2;   // columns of P that are handed over at once
 constexpr int THREADS = 384;   // loaders of rows and K, and of V, issuers of both products, two lanes of four softmax warps
 // Registers a thread: 168 at launch for all three warpgroups, shared out as 72 + 2 x 216.
 constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * 168, "the shares draw on the registers of the launch");
 constexpr int TMEM_COLS = 512;
+constexpr int FEW = 8;         // rows of an item whose products are taken the other way round
 constexpr int QUEUE = 4;       // pieces that the producer may be ahead
-// What an item costs besides its blocks, in units (below): where a row has four parts, with one tile, with two.
-constexpr int ITEM_SPLIT = 2, ITEM_ONE = 3, ITEM_TWO = 5;
+// What an item costs besides its blocks, in units (below): of few rows, of one tile, of two.
+constexpr int ITEM_FEW = 2, ITEM_ONE = 3, ITEM_TWO = 5;
 // A row's reference is its running maximum, so its largest weight is 1 and loses nothing when weights become bf16, and the sum is one of
 // weights before that. A reference that may lag behind by 2^8 saves rescales of O: 2 us of 64 (64 sequences behind 16384 positions), for an
 // error of 2.2e-3 in place of 2.0e-3 on unit scores and 1.3e-3 in place of 0.5e-3 on scores of four times the spread; with a sum of the
@@ -55,8 +57,8 @@ struct Cfg {
   static constexpr int SB = DH == 64 ? 2 : 1;        // score accumulators: one that the lanes take turns with at 128, one each at 64
   // Shared memory holds two tiles of the rows that the largest tile of the batch has, and as many blocks of K and V as go in beside them.
   static constexpr int MAX_SLOTS = DH == 128 ? 7 : 14;
-  static constexpr int BAR_BYTES = (8 * (2 * MAX_SLOTS + 2 * QUEUE + 2 + 2 + 2 + 2 + 4 + 2 + 4 + 4) + 8 + 15) / 16 * 16;
-  static constexpr int FIXED_BYTES = BAR_BYTES + QUEUE * 32 + BM * 8 + 1024 /* alignment */;
+  static constexpr int BAR_BYTES = (8 * (2 * MAX_SLOTS + 2 * QUEUE + 2 + 2 + 2 + 2 + 4 + 2 + 4 + 4 + 2) + 8 + 15) / 16 * 16;
+  static constexpr int FIXED_BYTES = BAR_BYTES + QUEUE * 32 + BM * 8 + 2 * 2 * 4 * FEW * 4 + 1024 /* alignment */;
   static int slots(int q_rows) {
     const int n = (227 * 1024 - FIXED_BYTES - 2 * q_rows * DH * 2) / KV_BYTES;
     return n < MAX_SLOTS ? n : MAX_SLOTS;
@@ -79,6 +81,20 @@ struct Header {        // at the start of the workspace, of a batch that has bee
   int pad[2];
 };
 
+// a / d for 0 <= a < 2^31 by a multiplication, where the host knows d: m = 2^k / d rounded up with k = 31 + log2 d rounded up, so that
+// m d - 2^k < 2^(k - 31).
+struct Divisor {
+  unsigned m;
+  int shift;
+  __host__ void set(int d) {
+    int log = 0;
+    while ((1ll << log) < d) ++log;
+    shift = 31 + log;
+    m = static_cast<unsigned>(((1ull << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int of(int a) const { return static_cast<int>((static_cast<unsigned long long>(a) * m) >> shift); }
+};
+
 struct Params {
   const __nv_bfloat16* q;
   long long ldq;
@@ -88,9 +104,10 @@ struct Params {
   const int* prefix_table;
   const int* cu_q;
   int prefix;          // shared positions: whole pages; 0 where every sequence's own items start at 0
-  int page, n_blocks, box;
+  int page, n_blocks, box_log;
+  Divisor by_page, by_heads, by_span;     // page, Hkv, 2 TT
   int B, NT, H, Hkv, G, TT;
-  int split;           // a row has four parts of an item, one of every fourth of a block's positions: 1 those of its own, 2 of both
+  int few;             // items whose products are taken the other way round: 1 a sequence's own, 2 shared ones (few_rows)
   int q_tokens;        // of the box that brings a tile of rows
   int by_token;        // whether there is a box of one token too
   int q_rows;          // of a tile in shared memory, a multiple of 8; the tensor core reads 128, those behind are rows of no one
@@ -129,14 +146,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+constexpr int kTries = 1 << 21;
 // Wait of a whole warp, all lanes with one result; bounded like mbar_wait, in fewer instructions: the kernel below is bound by what it
 // has to fetch of its own code where a CTA goes through many short pieces (with mbar_wait at every wait 136 KB).
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  const uint64_t t0 = globaltimer_ns();
+  int tries = 0;
 #pragma unroll 1
   while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
-    if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > kLocalWaitNs || *reinterpret_cast<volatile int*>(status) != 0)) {
+    // a try takes 20 cycles at least, some thousand as a rule
+    if (++tries > kTries || ((tries & 15) == 0 && __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(status) != 0))) {
       atomicCAS(status, 0, code);
       return false;
     }
@@ -147,23 +165,19 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status
 __device__ __forceinline__ uint32_t same(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// a / d for 0 <= a < 2^31, d > 0: the compiler's own division takes three times the instructions.
+// a / d for 0 <= a < 2^31, d > 0 and results below 2^20, where the estimate is off by one at most: the compiler's own division takes four
+// times the instructions.
 __device__ __forceinline__ int quotient(int a, int d) {
-  int q = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(d)));
-  int r = a - q * d;
-#pragma unroll 1
-  while (r < 0) { --q; r += d; }
-#pragma unroll 1
-  while (r >= d) { ++q; r -= d; }
-  return q;
+  const int q = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(d))), r = a - q * d;
+  return q - (r < 0) + (r >= d);
 }
 
 __device__ __forceinline__ int blocks_of(int positions) { return positions > 0 ? (positions + BN - 1) / BN : 0; }
 // An item lies in the line with one unit for a block of one tile of rows, two for a block of two, and in front of them what it costs
 // besides its blocks.
-__device__ __forceinline__ int head_units(int n_tok, int TT, bool split) { return split ? ITEM_SPLIT : n_tok > TT ? ITEM_TWO : ITEM_ONE; }
-__device__ __forceinline__ int units_of(int positions, int n_tok, int TT, bool split) {
-  return positions > 0 ? (blocks_of(positions) << (n_tok > TT ? 1 : 0)) + head_units(n_tok, TT, split) : 0;
+__device__ __forceinline__ int head_units(int n_tok, int TT, bool few) { return few ? ITEM_FEW : n_tok > TT ? ITEM_TWO : ITEM_ONE; }
+__device__ __forceinline__ int units_of(int positions, int n_tok, int TT, bool few) {
+  return positions > 0 ? (blocks_of(positions) << (n_tok > TT ? 1 : 0)) + head_units(n_tok, TT, few) : 0;
 }
 
 // The deal of the line over the CTAs: shared items to the first of them, own ones to the others, the units of either evenly. A CTA also
@@ -171,47 +185,48 @@ __device__ __forceinline__ int units_of(int positions, int n_tok, int TT, bool s
 // rows). With U and V units, `more` units dearer: U / n + more = V / (ctas - n) for n CTAs.
 // At least two units a CTA, so that one between the ends of an item has a block of it, whose two units may lie with two CTAs (the first
 // unit's CTA has the block).
-struct Deal {
-  int shared, ctas[2], per[2], rem[2];     // units of the first part of the line
-  __device__ Deal(int units_shared, int units_own, int grid, int more) : shared(units_shared) {
-    int n = units_shared > 0 ? grid : 0;
+struct Deal {                              // the part of it that CTA c has a share of
+  int from, units, first, per, rem;        // where it begins in the line, its units, its first CTA
+  __device__ Deal(int units_shared, int units_own, int grid, int c, int more) {
+    int n = units_shared > 0 ? grid : 0;   // CTAs of the shared part
     if (units_shared > 0 && units_own > 0) {
       const float U = units_shared, V = units_own, N = grid, b = more * N - U - V;
       n = clampi(__float2int_ru(2.f * U * N / (sqrtf(b * b + 4.f * more * U * N) - b)), 1, grid - 1);
     }
-    ctas[0] = n;
-    ctas[1] = grid - n;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int units = i ? units_own : units_shared, share = max(1, min(ctas[i], units >> 1));
-      per[i] = quotient(units, share);
-      rem[i] = units - per[i] * share;
-    }
+    const bool own = c >= n;
+    from = own ? units_shared : 0;
+    units = own ? units_own : units_shared;
+    first = own ? n : 0;
+    const int share = max(1, min(own ? grid - n : n, units >> 1));
+    per = units / share;                   // may be large
+    rem = units - per * share;
   }
-  // The share of CTA c is [begin, end) of the line.
-  __device__ void share(int c, int units_own, int& begin, int& end) const {
-    const int i = c < ctas[0] ? 0 : 1, k = i ? c - ctas[0] : c, units = i ? units_own : shared, from = i ? shared : 0;
-    begin = from + min(units, k * per[i] + min(k, rem[i]));
-    end = from + min(units, (k + 1) * per[i] + min(k + 1, rem[i]));
-  }
+  __device__ int begin(int c) const { return from + min(units, (c - first) * per + min(c - first, rem)); }
   __device__ int owner(int u) const {
-    const int i = u < shared ? 0 : 1, v = i ? u - shared : u, edge = rem[i] * (per[i] + 1);
+    const int v = u - from, edge = rem * (per + 1);
     const bool low = v < edge;
-    return (i ? ctas[0] : 0) + quotient(low ? v : v - edge, low ? per[i] + 1 : max(per[i], 1)) + (low ? 0 : rem[i]);
+    return first + quotient(low ? v : v - edge, low ? per + 1 : max(per, 1)) + (low ? 0 : rem);
   }
 };
 
 // The shared items of one kv head: tiles of two times TT tokens, the last of which may have one tile of rows.
 struct Shared {
   int tiles, size, last, head;        // items of a head, units of an item and of the last one, of a head
-  __device__ Shared(int prefix, int tokens, int TT, bool split) {
-    tiles = prefix > 0 ? quotient(tokens + 2 * TT - 1, 2 * TT) : 0;
+  __device__ Shared(const Params& p, int tokens) {
+    const int prefix = p.prefix, TT = p.TT;
+    const bool few = p.few & 2;
+    tiles = prefix > 0 ? p.by_span.of(tokens + 2 * TT - 1) : 0;
     size = units_of(prefix, 2 * TT, TT, false);
-    last = units_of(prefix, tokens - (tiles - 1) * 2 * TT, TT, split);
+    last = units_of(prefix, tokens - (tiles - 1) * 2 * TT, TT, few);
     head = tiles > 0 ? (tiles - 1) * size + last : 0;
   }
 };
 
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
 // Inclusive sum over a warp.
 __device__ __forceinline__ int warp_scan(int v, int lane) {
 #pragma unroll
@@ -233,46 +248,52 @@ constexpr int PIECE_SHARED = 1, PIECE_CUT = 2, PIECE_FIRST = 4, PIECE_SHORT = 8,
 // A CTA's pieces, found by a whole warp. The plan of a batch of one token a sequence is summed up on the way, 32 sequences at a time;
 // anything else has been planned (plan_kernel).
 // Slots of the rows of items that were not cut: of shared items, then of own ones.
-__host__ __device__ __forceinline__ int own_slot(const Params& p) { return p.prefix == 0 ? 0 : p.split & 2 ? 4 : 1; }
-__host__ __device__ __forceinline__ int whole_slots(const Params& p) { return own_slot(p) + (p.split ? 4 : 1); }
+__host__ __device__ __forceinline__ int own_slot(const Params& p) { return p.prefix == 0 ? 0 : 1; }
+__host__ __device__ __forceinline__ int whole_slots(const Params& p) { return own_slot(p) + 1; }
 
-// Whether the four quarters of the tile (the softmax warps of a lane) have the same rows, up to eight, and a fourth of the positions of
-// each block: the few rows of a sequence of one token would keep one warp of a lane busy, and both lanes' on one scheduler.
-__device__ __forceinline__ bool is_split(const Params& p, const Piece& x) {
-  return (x.flags & PIECE_SHARED ? p.split & 2 : p.split & 1) != 0;
+// Whether the products are taken the other way round, S^T = K Q^T and O^T = V^T P^T, of up to eight rows (a sequence of one token has as
+// many as query heads share a kv head). In a tile of 128 rows they would be lanes 0 to 7 of one warp, which would go through 128 columns
+// of scores and dh of O one by one; here a thread has a position, or a column of O, of all rows, an eighth of the instructions.
+template <bool PLANNED>
+__device__ __forceinline__ bool few_rows(const Params& p, const Piece& x) {
+  return !PLANNED && (x.flags & PIECE_SHARED ? p.few & 2 : p.few & 1) != 0;
 }
 
+// The items from one on are gone through without a division or a search: a warp that looks for every piece anew takes 4000 cycles for
+// one, as long as the others take for a piece of one block.
+template <bool PLANNED>
 struct Walk {
   const Params& p;
   const Shared shared;
   int units_shared, q_lo, q_hi, pairs;
   int u, u1, u_first;
-  int begin, last, index;        // of the item: where it lies in the line, the first unit of its last block, its entry of p.part
+  int h, tile, size;             // the item: kv head; tile of shared items, or lane that has the pair; units
+  int last, index;               // the first unit of its last block, its entry of p.part
   int window, c_lo, c_hi;        // pairs window + lane: units of one kv head before and behind
   int4 info;
 
-  __device__ Walk(const Params& p_, const Header& h, int u0, int u1_)
-      : p(p_), shared(p_.prefix, h.q_hi - h.q_lo, p_.TT, (p_.split & 2) != 0), units_shared(h.units_shared), q_lo(h.q_lo), q_hi(h.q_hi), pairs(h.pairs), u(u0),
-        u1(u1_), u_first(u0), begin(0), last(0), index(0), window(-1), c_lo(0), c_hi(0), info(make_int4(0, 0, 0, 0)) {}
+  __device__ Walk(const Params& p_, const Header& hd, int u0, int u1_)
+      : p(p_), shared(p_, hd.q_hi - hd.q_lo), units_shared(hd.units_shared), q_lo(hd.q_lo), q_hi(hd.q_hi),
+        pairs(hd.pairs), u(u0), u1(u1_), u_first(u0), h(0), tile(0), size(0), last(0), index(0), window(-32), c_lo(0), c_hi(0),
+        info(make_int4(0, 0, 0, 0)) {}
 
-  __device__ void planned(int from, int lane) {
-    window = from;
-    const int i = from + lane;
-    c_lo = c_hi = -1;
-    if (i < pairs) {
-      c_lo = p.cum[i];
-      c_hi = p.cum[i + 1];
-      info = *reinterpret_cast<const int4*>(p.pair + i);
+  // The pairs behind those of the window.
+  __device__ void advance(int lane) {
+    const int before = window < 0 || PLANNED ? 0 : __shfl_sync(0xffffffffu, c_hi, 31), i = (window += 32) + lane;
+    if (PLANNED) {
+      c_lo = c_hi = -1;
+      if (i < pairs) {
+        c_lo = p.cum[i];
+        c_hi = p.cum[i + 1];
+        info = *reinterpret_cast<const int4*>(p.pair + i);
+      }
+    } else {
+      const int len = i < pairs ? clampi(p.seq_len[i], 0, p.max_blocks * p.page) : 0;
+      const int n = units_of(len - p.prefix, 1, p.TT, p.few & 1);
+      c_hi = before + warp_scan(n, lane);
+      c_lo = c_hi - n;
+      info = make_int4(i, 1, i, len);
     }
-  }
-  __device__ void summed(int from, int lane, int before) {
-    window = from;
-    const int b = from + lane;
-    const int len = b < pairs ? clampi(p.seq_len[b], 0, p.max_blocks * p.page) : 0;
-    const int n = units_of(len - p.prefix, 1, p.TT, p.split & 1);
-    c_hi = before + warp_scan(n, lane);
-    c_lo = c_hi - n;
-    info = make_int4(b, 1, b, len);
   }
 
   // False: no more pieces.
@@ -280,59 +301,73 @@ struct Walk {
     const int lane = threadIdx.x & 31;
     for (;;) {
       if (u >= u1) return false;
-      int off, size;
-      x.flags = u == u_first ? PIECE_FIRST : 0;
+      int off = 0;
+      x.flags = 0;
       if (u < units_shared) {
-        x.h = quotient(u, shared.head);
-        const int rest = u - x.h * shared.head;
-        const int tile = min(quotient(rest, shared.size), shared.tiles - 1);
-        off = rest - tile * shared.size;
+        if (u == u_first) {
+          h = quotient(u, shared.head);
+          const int rest = u - h * shared.head;
+          tile = min(quotient(rest, shared.size), shared.tiles - 1);
+          off = rest - tile * shared.size;
+        } else if (++tile == shared.tiles) {
+          tile = 0;
+          ++h;
+        }
         size = tile == shared.tiles - 1 ? shared.last : shared.size;
         x.t0 = q_lo + tile * 2 * p.TT;
         x.n_tok = min(2 * p.TT, q_hi - x.t0);
-        index = x.h * shared.tiles + tile;
+        index = h * shared.tiles + tile;
         x.kbase = 0;
         x.kend = p.prefix;
-        x.flags |= PIECE_SHARED;
+        x.flags = PIECE_SHARED;
       } else {
-        const int v = u - units_shared;
-        if (window < 0) {
-          if (p.pair) {                           // last pair that starts at v or before
+        // the first lane whose pair has units beyond v
+        int v = -1;
+        unsigned mask = 0;                        // nothing in the window yet
+        if (u == u_first) {
+          v = u - units_shared;
+          if (PLANNED) {                           // last pair that starts at v or before
             int lo = 0, hi = pairs - 1;
             while (lo < hi) {
               const int mid = (lo + hi + 1) >> 1;
               if (p.cum[mid] * p.Hkv <= v) lo = mid; else hi = mid - 1;
             }
-            planned(lo, lane);
-          } else {
-            summed(0, lane, 0);
+            window = lo - 32;
+          }
+        } else if (++h == p.Hkv) {
+          mask = tile == 31 ? 0u : 0xffffffffu << (tile + 1);
+        }
+        if (u == u_first || h == p.Hkv) {
+          unsigned open;
+          while (!(open = __ballot_sync(0xffffffffu, c_hi * p.Hkv > v && c_hi > c_lo) & mask)) {
+            if (window + 32 >= pairs) return false;
+            advance(lane);
+            mask = 0xffffffffu;
+          }
+          tile = __ffs(open) - 1;
+          const int before = __shfl_sync(0xffffffffu, c_lo, tile);
+          size = __shfl_sync(0xffffffffu, c_hi, tile) - before;
+          h = 0;
+          if (u == u_first) {
+            const int rest = v - before * p.Hkv;
+            h = quotient(rest, size);
+            off = rest - h * size;
           }
         }
-        unsigned open;
-        while (!(open = __ballot_sync(0xffffffffu, c_hi * p.Hkv > v))) {   // v lies below the last pair's end
-          if (window >= pairs) return false;
-          if (p.pair) planned(window + 32, lane);
-          else summed(window + 32, lane, __shfl_sync(0xffffffffu, c_hi, 31));
-        }
-        const int l = __ffs(open) - 1;
-        const int before = __shfl_sync(0xffffffffu, c_lo, l);
-        size = __shfl_sync(0xffffffffu, c_hi, l) - before;
-        const int rest = v - before * p.Hkv;
-        x.h = quotient(rest, size);
-        off = rest - x.h * size;
-        x.t0 = __shfl_sync(0xffffffffu, info.x, l);
-        x.n_tok = __shfl_sync(0xffffffffu, info.y, l);
-        x.kend = __shfl_sync(0xffffffffu, info.w, l);
+        x.t0 = __shfl_sync(0xffffffffu, info.x, tile);
+        x.n_tok = __shfl_sync(0xffffffffu, info.y, tile);
+        x.kend = __shfl_sync(0xffffffffu, info.w, tile);
         x.kbase = p.prefix;
-        index = p.shared_items + (window + l) * p.Hkv + x.h;
-        x.flags |= __shfl_sync(0xffffffffu, info.z, l) << SEQUENCE;
+        index = p.shared_items + (window + tile) * p.Hkv + h;
+        x.flags = __shfl_sync(0xffffffffu, info.z, tile) << SEQUENCE;
       }
-      const int stop = min(size, off + (u1 - u));
-      begin = u - off;
+      x.h = h;
+      if (u == u_first) x.flags |= PIECE_FIRST;
+      const int stop = min(size, off + (u1 - u)), begin = u - off;
       u += stop - off;
       // a block belongs to the CTA that has its first unit
       const int two = x.n_tok > p.TT ? 1 : 0;
-      const int head = head_units(x.n_tok, p.TT, is_split(p, x)), blocks = (size - head) >> two;
+      const int head = head_units(x.n_tok, p.TT, few_rows<PLANNED>(p, x)), blocks = (size - head) >> two;
       x.j0 = (max(0, off - head) + two) >> two;
       x.j1 = (max(0, stop - head) + two) >> two;
       if (x.j1 == x.j0) continue;
@@ -427,47 +462,70 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   }
   if (tid == 0) {
     p.cum[pairs] = s_sum;
-    p.hdr->units_shared = p.Hkv * Shared(p.prefix, q_hi - q_lo, p.TT, false).head;
+    p.hdr->units_shared = p.Hkv * Shared(p, q_hi - q_lo).head;
     p.hdr->units_own = p.Hkv * s_sum;
     p.hdr->q_lo = q_lo; p.hdr->q_hi = q_hi; p.hdr->pairs = pairs;
     p.hdr->least = s_least;
   }
 }
 
-// What brings the blocks of K, or of V, whole warp.
+// What brings the blocks of K, or of V, whole warp. The table is read ahead: 32 boxes of the piece while the 32 in front of them are
+// brought, and the first of the next piece while this one is.
+struct Boxes {
+  int from, page, in;            // lane i: page of box (from + i) of a piece, and where in it the box begins
+};
 struct Ring {
   uint8_t* at;
   uint64_t *full, *empty;
   const int* table;
-  int slots, slot, head, from, row;        // lane i: first row in the pool of box (from + i)
+  int slots, slot, head, row;    // lane i: first row in the pool of its box
   uint32_t phase;
+  Boxes now, then;
 
   __device__ Ring(uint8_t* at_, uint64_t* full_, uint64_t* empty_, int slots_)
-      : at(at_), full(full_), empty(empty_), table(nullptr), slots(slots_), slot(0), head(0), from(0), row(0), phase(0) {}
+      : at(at_), full(full_), empty(empty_), table(nullptr), slots(slots_), slot(0), head(0), row(0), phase(0) {}
 
-  __device__ void piece(const Params& p, const Piece& x, int head_) {
-    table = x.flags & PIECE_SHARED ? p.prefix_table : p.block_table + static_cast<size_t>(x.flags >> SEQUENCE) * p.max_blocks;
+  __device__ static const int* table_of(const Params& p, const Piece& x) {
+    return x.flags & PIECE_SHARED ? p.prefix_table : p.block_table + static_cast<size_t>(x.flags >> SEQUENCE) * p.max_blocks;
+  }
+  __device__ static Boxes boxes(const Params& p, const Piece& x, const int* table, int from) {
+    const int pos = x.kbase + ((from + static_cast<int>(threadIdx.x & 31)) << p.box_log), at_page = p.by_page.of(pos);
+    Boxes b;
+    b.from = from;
+    b.in = pos - at_page * p.page;
+    b.page = pos < x.kend ? table[at_page] : 0;
+    return b;
+  }
+  __device__ static Boxes first(const Params& p, const Piece& x) { return boxes(p, x, table_of(p, x), x.j0 << (BN_LOG - p.box_log)); }
+
+  __device__ void rows(const Params& p) {
+    const int page = static_cast<unsigned>(now.page) >= static_cast<unsigned>(p.n_blocks) ? p.n_blocks : now.page;   // reads as zeros
+    row = (page * 2 * p.Hkv + head) * p.page + now.in;
+  }
+  __device__ void piece(const Params& p, const Piece& x, int head_, const Boxes& first_) {
+    table = table_of(p, x);
     head = head_;
-    from = -(1 << 30);
+    now = first_;
+    then.from = -1;
+    rows(p);
   }
 
   template <int DH>
   __device__ bool load(const Params& p, const CUtensorMap& tmap, const Piece& x, int j) {
-    const int lane = threadIdx.x & 31, nbx = BN / p.box, bx0 = j * nbx;       // boxes of a block, at most 16
-    if (bx0 + nbx > from + 32) {              // nbx divides 32: a block's boxes are fetched together
-      from = bx0;
-      const int pos = x.kbase + (from + lane) * p.box, at_page = quotient(pos, p.page);
-      int page = pos < x.kend ? table[at_page] : 0;
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.n_blocks)) page = p.n_blocks;   // reads as zeros
-      row = (page * 2 * p.Hkv + head) * p.page + pos - at_page * p.page;
+    const int lane = threadIdx.x & 31, nbx = BN >> p.box_log, bx0 = j << (BN_LOG - p.box_log);       // boxes of a block, at most 16
+    if (bx0 >= now.from + 32) {               // nbx divides 32: a block's boxes are read together
+      now = then;
+      rows(p);
+      then.from = -1;
     }
+    if (then.from < 0 && (now.from + 32) << p.box_log < x.kend - x.kbase) then = boxes(p, x, table, now.from + 32);
     if (!wait(&empty[slot], phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) return false;
-    const int live = min(nbx, (x.kend - x.kbase - j * BN + p.box - 1) / p.box);     // boxes with a position below kend
-    if (lane == 0) mbar_arrive_expect_tx(&full[slot], live * p.box * DH * 2);
+    const int live = min(nbx, (x.kend - x.kbase - j * BN + (1 << p.box_log) - 1) >> p.box_log);     // boxes with a position below kend
+    if (lane == 0) mbar_arrive_expect_tx(&full[slot], (live * DH * 2) << p.box_log);
     __syncwarp();
-    const int i = lane - (bx0 - from);
+    const int i = lane - (bx0 - now.from);
     if (i >= 0 && i < live) {
-      uint8_t* to = at + slot * (BN * DH * 2) + i * p.box * 128;
+      uint8_t* to = at + slot * (BN * DH * 2) + (i << p.box_log) * 128;
 #pragma unroll
       for (int c = 0; c < DH / 64; ++c) tma_load_2d(to + c * (BN * 128), &tmap, &full[slot], c * 64, row);
     }
@@ -477,7 +535,7 @@ struct Ring {
   }
 };
 
-template <int DH>
+template <int DH, bool PLANNED>
 __global__ void __launch_bounds__(THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap q_tile, const __grid_constant__ CUtensorMap q_token,
               const __grid_constant__ Params p) {
@@ -502,22 +560,31 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   uint64_t* pv_done = p_full + 4;        // [2] P V of a lane's block has completed
   uint64_t* o_full = pv_done + 2;        // [4] a quarter of the rows: lane 1 has its sum ready for lane 0
   uint64_t* o_free = o_full + 4;         // [4] and lane 0 has read it
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_free + 4);
+  uint64_t* r_full = o_free + 4;         // [2] few rows: what the warps of a lane tell each other is in shared memory (4 warp arrivals)
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(r_full + 2);
   Piece* queue = reinterpret_cast<Piece*>(sV + VS * C::KV_BYTES + C::BAR_BYTES);
-  float2* s_ml = reinterpret_cast<float2*>(queue + QUEUE);                    // [BM] maximum and sum of lane 1
+  // maximum and sum: [BM] of lane 1; of few rows [lane][warp][row]
+  float2* s_ml = reinterpret_cast<float2*>(queue + QUEUE);
+  float* s_max = reinterpret_cast<float*>(s_ml + BM);                         // [lane][block, even or odd][warp][row]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+#pragma unroll 1
     for (int s = 0; s < VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+#pragma unroll 1
     for (int s = 0; s < QUEUE; ++s) { mbar_init(&x_full[s], 1); mbar_init(&x_empty[s], 11); }
+#pragma unroll 1
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&s_free[s], 4);
       mbar_init(&pv_done[s], 1);
+      mbar_init(&r_full[s], 4);
     }
+#pragma unroll 1
     for (int s = 0; s < 4; ++s) {
       mbar_init(&p_full[s], 4);
       mbar_init(&o_full[s], 1);
@@ -563,7 +630,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   if (warp == 0) {
     // -------------------------------- pieces, their rows, and K --------------------------------
     Header hdr;
-    if (p.pair) {
+    if (PLANNED) {
       hdr.units_shared = p.hdr->units_shared; hdr.units_own = p.hdr->units_own;
       hdr.q_lo = p.hdr->q_lo; hdr.q_hi = p.hdr->q_hi; hdr.pairs = p.hdr->pairs; hdr.least = p.hdr->least;
     } else {
@@ -573,42 +640,49 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int b = b0 + lane;
         const int len = b < p.B ? clampi(p.seq_len[b], 0, cap) : INT_MAX;
-        const int n = b < p.B ? units_of(len - p.prefix, 1, p.TT, p.split & 1) : 0;
+        const int n = b < p.B ? units_of(len - p.prefix, 1, p.TT, p.few & 1) : 0;
         least = min(least, len);
         sum += __reduce_add_sync(0xffffffffu, n);
       }
       hdr.q_lo = 0; hdr.q_hi = p.B; hdr.pairs = p.B; hdr.least = __reduce_min_sync(0xffffffffu, least);
-      hdr.units_shared = p.Hkv * Shared(p.prefix, p.B, p.TT, (p.split & 2) != 0).head;
+      hdr.units_shared = p.Hkv * Shared(p, p.B).head;
       hdr.units_own = p.Hkv * sum;
     }
-    const Deal deal(hdr.units_shared, hdr.units_own, gridDim.x,
-                    head_units(hdr.q_hi - hdr.q_lo, p.TT, (p.split & 2) != 0) - head_units(1, p.TT, p.split & 1));
-    int u0, u1;
-    deal.share(blockIdx.x, hdr.units_own, u0, u1);
-    Walk walk(p, hdr, u0, u1);
+    const Deal deal(hdr.units_shared, hdr.units_own, gridDim.x, blockIdx.x,
+                    head_units(hdr.q_hi - hdr.q_lo, p.TT, (p.few & 2) != 0) - head_units(1, p.TT, p.few & 1));
+    Walk<PLANNED> walk(p, hdr, deal.begin(blockIdx.x), deal.begin(blockIdx.x + 1));
     Ring k(sK, k_full, k_empty, KS);
     int n_pieces = 0;
-    bool ok = true, both = false;
+    bool ok = true, both = false, begun = false;
+    Piece y = {};                          // the piece behind x
+    Boxes first = {};
     while (ok) {
-      const bool more = walk.next(x);
-      if (!more) x.j0 = x.j1 = 0;
-      if (hdr.least < x.kend) x.flags |= PIECE_SHORT;
-      ok = wait(&x_empty[at], at_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
-      if (!ok) break;
-      if (lane == 0) {
-        int4* to = reinterpret_cast<int4*>(queue + at);
-        to[0] = make_int4(x.h, x.t0, x.n_tok, x.kbase);
-        to[1] = make_int4(x.kend, x.j0, x.j1, x.flags);
-        mbar_arrive(&x_full[at]);
+      if (begun) {
+        x = y;
+        if (hdr.least < x.kend) x.flags |= PIECE_SHORT;
+        ok = wait(&x_empty[at], at_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
+        if (!ok) break;
+        if (lane == 0) {
+          int4* to = reinterpret_cast<int4*>(queue + at);
+          to[0] = make_int4(x.h, x.t0, x.n_tok, x.kbase);
+          to[1] = make_int4(x.kend, x.j0, x.j1, x.flags);
+          mbar_arrive(&x_full[at]);
+        }
+        __syncwarp();
+        if (++at == QUEUE) { at = 0; at_phase ^= 1; }
+        if (x.j1 == 0) break;
+        if (x.j0 == 0 && lane == 0)        // for the joining launch
+          p.part[walk.index] = make_int2(x.flags & PIECE_CUT ? deal.owner(walk.last) - static_cast<int>(blockIdx.x) + 1 : 1,
+                                         2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1));
+        k.piece(p, x, x.h, first);
       }
-      __syncwarp();
-      if (++at == QUEUE) { at = 0; at_phase ^= 1; }
-      if (!more) break;
-      if (x.j0 == 0 && lane == 0)          // for the joining launch
-        p.part[walk.index] = make_int2(x.flags & PIECE_CUT ? deal.owner(walk.last) - static_cast<int>(blockIdx.x) + 1 : 1,
-                                       2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1));
+      if (walk.next(y)) first = Ring::first(p, y);
+      else y.j0 = y.j1 = 0;
+      if (!begun) {
+        begun = true;
+        continue;
+      }
       const bool two = x.n_tok > p.TT;
-      k.piece(p, x, x.h);
 #pragma unroll 1
       for (int j = x.j0; j < x.j1 && ok; ++j) {
         ok = k.template load<DH>(p, tmap, x, j);
@@ -625,13 +699,13 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           // The box of a tile brings its tokens and, behind the last of them, rows of others that no one reads.
           const bool one = x.n_tok == 1 && p.by_token;
           const int tiles = two ? 2 : 1, bytes = (one ? 1 : p.q_tokens) * p.G * 128;
+          const CUtensorMap* map = one ? &q_token : &q_tile;
           uint64_t* bar = &q_full[n_pieces & 1];
           mbar_arrive_expect_tx(bar, tiles * C::NCH * bytes);
 #pragma unroll 1
           for (int i = 0; i < tiles * C::NCH; ++i) {
             const int tile = i / C::NCH, c = i % C::NCH;
-            tma_load_3d(sQ + (two ? tile : n_pieces & 1) * q_bytes + c * q_chunk, one ? &q_token : &q_tile, bar, c * 64, x.h * p.G,
-                        x.t0 + tile * p.TT);
+            tma_load_3d(sQ + (two ? tile : n_pieces & 1) * q_bytes + c * q_chunk, map, bar, c * 64, x.h * p.G, x.t0 + tile * p.TT);
           }
         }
         __syncwarp();
@@ -643,7 +717,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     Ring v(sV, v_full, v_empty, VS);
     bool ok = true;
     while (ok && take(x)) {
-      v.piece(p, x, p.Hkv + x.h);
+      v.piece(p, x, p.Hkv + x.h, Ring::first(p, x));
 #pragma unroll 1
       for (int j = x.j0; j < x.j1 && ok; ++j) ok = v.template load<DH>(p, tmap, x, j);
     }
@@ -653,9 +727,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     // tensor core spends on the other's. The warp walks its loop as a whole and one lane issues; what an instruction is given comes from
     // lane 0 by a shuffle, so that it is known to be the same for the warp and stays in uniform registers.
     const bool leader = elect_one();
-    constexpr uint32_t idesc = make_idesc_bf16(BM, BN, false, false);
     constexpr uint64_t desc = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16);
-    const uint32_t a_q = smem_u32(sQ), a_k = smem_u32(sK), chunk = same(q_chunk >> 4);
+    constexpr uint64_t desc_same = desc & ~(0x3fffull << 32);        // every eight rows are the same eight
+    const uint32_t at_q = smem_u32(sQ), at_k = smem_u32(sK), q_step = same(q_chunk >> 4);
+    constexpr uint32_t k_step = BN * 8;
     int ks = 0, n_pieces = 0, steps = 0;
     uint32_t kph = 0;
     bool ok = true;
@@ -663,33 +738,44 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       const int half = n_pieces & 1;
       const bool two = same(x.n_tok > p.TT ? 1 : 0);
       const int n = same((x.j1 - x.j0) << (two ? 1 : 0));
-      // eight rows for every eight of the tile, where its four quarters take the same rows
-      const uint64_t desc_q = desc & ~(same(is_split(p, x) ? 1 : 0) ? 0x3fffull << 32 : 0ull);
+      // few rows: a product of 16 columns at least, of which eight are the others again
       ok = wait(&q_full[half], (n_pieces >> 1) & 1, p.status, ST_TIMEOUT_MISC);
+      auto steps_of = [&](auto kind) {
+      constexpr bool few = decltype(kind)::value;
 #pragma unroll 1
       for (int i = 0; i < n && ok; ++i, ++steps) {
         const int L = steps & 1;
         const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;      // the block's first step, its last
         const int before = C::SB == 1 ? steps : steps >> 1;                        // scores that were in this accumulator
-        const uint32_t q_lo = same((a_q + (two ? L : half) * q_bytes) >> 4), k_lo = same((a_k + ks * C::KV_BYTES) >> 4);
+        const uint32_t q_lo = same((at_q + (two ? L : half) * q_bytes) >> 4), k_lo = same((at_k + ks * C::KV_BYTES) >> 4);
         const uint32_t to = same(tmem + (C::SB == 1 ? 0 : L * BN));
         if (uses) ok = wait(&k_full[ks], kph, p.status, ST_TIMEOUT_FULL);
         if (before > 0) ok = ok && wait(&s_free[C::SB == 1 ? 0 : L], (before - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
+          if (few) {
 #pragma unroll
-          for (int k = 0; k < DH / 16; ++k)
-            umma_bf16_ss(to, desc_q | (q_lo + (k >> 2) * chunk + (k & 3) * 2), desc | (k_lo + (k >> 2) * (BN * 8) + (k & 3) * 2), idesc,
-                         k > 0 ? 1u : 0u);
+            for (int k = 0; k < DH / 16; ++k)
+              umma_bf16_ss(to, desc | (k_lo + (k >> 2) * k_step + (k & 3) * 2), desc_same | (q_lo + (k >> 2) * q_step + (k & 3) * 2),
+                           make_idesc_bf16(BM, 2 * FEW, false, false), k > 0 ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int k = 0; k < DH / 16; ++k)
+              umma_bf16_ss(to, desc | (q_lo + (k >> 2) * q_step + (k & 3) * 2), desc | (k_lo + (k >> 2) * k_step + (k & 3) * 2),
+                           make_idesc_bf16(BM, BN, false, false), k > 0 ? 1u : 0u);
+          }
           umma_commit(&s_full[L]);
-          if (frees) umma_commit(&k_empty[ks]);
+          if (frees && !few) umma_commit(&k_empty[ks]);
           if (i == n - 1) umma_commit(&q_empty[half]);
         }
         if (frees) {
           if (++ks == KS) { ks = 0; kph ^= 1; }
         }
       }
+      };
+      if (!PLANNED && same(few_rows<PLANNED>(p, x) ? 1 : 0)) steps_of(std::bool_constant<!PLANNED>{});
+      else steps_of(std::false_type{});
       ++n_pieces;
     }
   } else {
@@ -697,19 +783,25 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const bool leader = elect_one();
     constexpr uint32_t idesc = make_idesc_bf16(BM, DH, false, true);
     constexpr uint64_t desc = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61) | (static_cast<uint64_t>(BN * 8) << 16);
-    const uint32_t a_v = smem_u32(sV);
-    int vs = 0, steps = 0;
+    // few rows: V^T has 128 rows (at dh 64 each of them twice), P^T lies in the block of K, eight rows of a position behind one another
+    constexpr uint32_t idesc_few = make_idesc_bf16(BM, 2 * FEW, true, true);
+    constexpr uint64_t desc_few = DH == 128 ? desc : desc & ~(0x3fffull << 16);
+    constexpr uint64_t desc_p = (1ull << 46) | (static_cast<uint64_t>(8 * FEW * 2 >> 4) << 16);
+    const uint32_t a_v = smem_u32(sV), a_k = smem_u32(sK);
+    int vs = 0, ks = 0, steps = 0;
     uint32_t vph = 0;
     bool ok = true;
     while (ok && take(x)) {
       const bool two = same(x.n_tok > p.TT ? 1 : 0);
       const int n = same((x.j1 - x.j0) << (two ? 1 : 0)), first_live = same(x.kend - x.kbase - x.j0 * BN);
+      auto steps_of = [&](auto kind) {
+      constexpr bool few = decltype(kind)::value;
 #pragma unroll 1
       for (int i = 0; i < n && ok; ++i, ++steps) {
         const int L = steps & 1, turn = steps >> 1;            // every second step is this lane's
         const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;
         const int live = min(BN, first_live - (two ? i >> 1 : i) * BN);            // positions that count
-        const uint32_t v_lo = same((a_v + vs * C::KV_BYTES) >> 4), o = same(tmem + C::COL_O + L * DH),
+        const uint32_t v_lo = same((a_v + vs * C::KV_BYTES) >> 4), p_lo = same((a_k + ks * C::KV_BYTES) >> 4), o = same(tmem + C::COL_O + L * DH),
                        w = same(tmem + C::COL_P + L * (BN / 2)), begins = same(i < 2 ? 1 : 0);
         if (uses) {
           ok = wait(&v_full[vs], vph, p.status, ST_TIMEOUT_FULL);
@@ -735,7 +827,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
 #pragma unroll
             for (int k2 = 0; k2 < HALF / 16; ++k2) {
               const int k = h * (HALF / 16) + k2;
-              if (k * 16 < live) umma_bf16_ts(o, w + k * 8, desc | (v_lo + k * 128), idesc, (!begins || k > 0) ? 1u : 0u);
+              if (k * 16 < live) {
+                if (few) umma_bf16_ss(o, desc_few | (v_lo + k * 128), desc_p | (p_lo + k * FEW * 2), idesc_few, (!begins || k > 0) ? 1u : 0u);
+                else umma_bf16_ts(o, w + k * 8, desc | (v_lo + k * 128), idesc, (!begins || k > 0) ? 1u : 0u);
+              }
             }
           }
         }
@@ -743,11 +838,16 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         if (leader) {
           umma_commit(&pv_done[L]);
           if (frees) umma_commit(&v_empty[vs]);
+          if (few) umma_commit(&k_empty[ks]);
         }
         if (frees) {
+          if (++ks == KS) ks = 0;
           if (++vs == VS) { vs = 0; vph ^= 1; }
         }
       }
+      };
+      if (!PLANNED && same(few_rows<PLANNED>(p, x) ? 1 : 0)) steps_of(std::bool_constant<!PLANNED>{});
+      else steps_of(std::false_type{});
     }
   }
   } else {
@@ -757,31 +857,213 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int quarter = warp & 3;          // lanes of tensor memory that this warp may read
     const int r = quarter * 32 + lane;     // row of the tile
     const int tile_tok = quotient(r, p.G), tile_g = r - tile_tok * p.G;
-    const int lane_tok = quotient(lane, p.G), lane_g = lane - lane_tok * p.G;      // split
+    const int few_tok = quotient(lane & (FEW - 1), p.G);       // of row lane & 7
     const uint32_t tm = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t tm_S = tm + (C::SB == 1 ? 0 : L * BN), tm_P = tm + C::COL_P + L * (BN / 2), tm_O = tm + C::COL_O + L * DH;
     const float sl2 = p.scale_log2;
     int n = 0, steps = 0, n_join = 0;      // this lane's blocks; both lanes'; pieces whose lanes were joined
+    int slot0 = 0, told = 0;               // few rows: where the piece's first block of K lies; phases of r_full
     bool pending = false;                  // lane 1: its O waits to be read by lane 0
     while (take(x)) {
       const bool two = x.n_tok > p.TT;
       const int nb = x.j1 - x.j0;
       const int first = two ? 0 : (L ^ steps) & 1, step = two ? 1 : 2;           // this lane's blocks
       steps += two ? 2 * nb : nb;
+      int slot = 0;
+      if (!PLANNED && p.few) {
+        slot = slot0 + first;
+        if (slot >= KS) slot -= KS;
+        slot0 += nb;
+        slot0 -= quotient(slot0, KS) * KS;
+      }
       if (first >= nb) continue;
-      const bool split = is_split(p, x);
-      const int row_tok = split ? lane_tok : tile_tok, g = split ? lane_g : tile_g;
-      const int toks = two ? min(p.TT, x.n_tok - L * p.TT) : x.n_tok, tok = row_tok + (two ? L * p.TT : 0);
-      const bool active = split || quarter * 32 < toks * p.G;      // whether any row of this warp counts
-      const bool valid = row_tok < toks;
+      if (few_rows<PLANNED>(p, x)) {
+        // A thread has position r of a block, and then column r of O, of all rows.
+        const int rows = x.n_tok * p.G;
+        int limit = x.kend;                // of row lane & 7
+        if ((x.flags & (PIECE_SHARED | PIECE_SHORT)) == (PIECE_SHARED | PIECE_SHORT) && few_tok < x.n_tok)
+          limit = min(limit, p.seq_len[x.t0 + few_tok]);
+        float m_ref[FEW], l[FEW];
+#pragma unroll
+        for (int e = 0; e < FEW; ++e) { m_ref[e] = LOWEST; l[e] = 0.f; }
+        // What the lane's warps wrote is there for all of them.
+        auto meet = [&]() {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&r_full[L]);
+          wait(&r_full[L], told & 1, p.status, ST_TIMEOUT_MISC);
+          ++told;
+        };
+#pragma unroll 1
+        for (int i = first; i < nb; i += step, ++n) {
+          // the same waits as below, which do not end the loop either
+          wait(&s_full[L], n & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+          tc_fence_after();
+          uint32_t v[FEW], o[FEW];
+          tmem_ld_32x8(tm_S, v);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
+          const int pos = x.kbase + (x.j0 + i) * BN + r;
+          if (__any_sync(0xffffffffu, limit <= pos - lane + 31)) {
+#pragma unroll
+            for (int e = 0; e < FEW; ++e)
+              if (pos >= __shfl_sync(0xffffffffu, limit, e)) v[e] = 0xff800000u;
+          }
+          float4* top = reinterpret_cast<float4*>(s_max + (L * 2 + (n & 1)) * 4 * FEW);
+          float m[FEW];
+#pragma unroll
+          for (int e = 0; e < FEW; ++e) m[e] = warp_max(__uint_as_float(v[e]));
+          if (lane == 0) {
+            top[quarter * 2] = make_float4(m[0], m[1], m[2], m[3]);
+            top[quarter * 2 + 1] = make_float4(m[4], m[5], m[6], m[7]);
+          }
+          meet();
+          bool grow = false, huge = false;
+          float alpha[FEW];
+#pragma unroll
+          for (int e = 0; e < FEW; ++e) m[e] = LOWEST;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float4 a = top[w * 2], b = top[w * 2 + 1];
+            m[0] = fmaxf(m[0], a.x); m[1] = fmaxf(m[1], a.y); m[2] = fmaxf(m[2], a.z); m[3] = fmaxf(m[3], a.w);
+            m[4] = fmaxf(m[4], b.x); m[5] = fmaxf(m[5], b.y); m[6] = fmaxf(m[6], b.z); m[7] = fmaxf(m[7], b.w);
+          }
+#pragma unroll
+          for (int e = 0; e < FEW; ++e) {
+            const float now = fmaxf(m[e] * sl2, m_ref[e]);
+            grow |= e < rows && now > m_ref[e];        // what lies in columns behind the last row decides nothing
+            alpha[e] = ex2(m_ref[e] - now);
+            m_ref[e] = now;
+            huge |= e < rows && fabsf(now) > 16777216.f && now != LOWEST;
+          }
+          if (n > 0) {
+            wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+            tc_fence_after();
+            if (i > first && grow) {       // all threads of the lane have the same maxima
+              tmem_ld_32x8(tm_O, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < FEW; e += 2) mul2(o[e], o[e + 1], alpha[e], alpha[e + 1]);
+              tmem_st_32x8(tm_O, o);
+              tmem_st_wait();
+            }
+          }
+          if (pending) {
+            wait(&o_free[quarter], (n_join - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
+            pending = false;
+          }
+          float factor = sl2;
+          if (huge) {                      // scaled beforehand, as below
+#pragma unroll
+            for (int e = 0; e < FEW; e += 2) mul2(v[e], v[e + 1], sl2, sl2);
+            factor = 1.f;
+          }
+          float w[FEW];
+#pragma unroll
+          for (int e = 0; e < FEW; ++e) {
+            w[e] = ex2(__fmaf_rn(__uint_as_float(v[e]), factor, -m_ref[e]));
+            l[e] = __fmaf_rn(l[e], alpha[e], w[e]);
+          }
+          *reinterpret_cast<uint4*>(sK + slot * C::KV_BYTES + r * 16) =
+              make_uint4(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7]));
+          slot += step;
+          if (slot >= KS) slot -= KS;
+          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) { mbar_arrive(&p_full[2 * L]); mbar_arrive(&p_full[2 * L + 1]); }
+        }
+        // Sums over the warp: a lane passes on what it has of the rows that the other keeps. Row `own` ends in every fourth lane.
+        const int own = lane >> 2;
+        const bool up16 = lane & 16, up8 = lane & 8, up4 = lane & 4;
+        float a4[4], b4[4], a2[2], b2[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a4[e] = (up16 ? l[e + 4] : l[e]) + __shfl_xor_sync(0xffffffffu, up16 ? l[e] : l[e + 4], 16);
+          b4[e] = up16 ? m_ref[e + 4] : m_ref[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          a2[e] = (up8 ? a4[e + 2] : a4[e]) + __shfl_xor_sync(0xffffffffu, up8 ? a4[e] : a4[e + 2], 8);
+          b2[e] = up8 ? b4[e + 2] : b4[e];
+        }
+        float sum = (up4 ? a2[1] : a2[0]) + __shfl_xor_sync(0xffffffffu, up4 ? a2[0] : a2[1], 4), m_own = up4 ? b2[1] : b2[0];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        const bool joins = nb > 1;
+        wait(&pv_done[L], (n - 1) & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+        tc_fence_after();
+        float2* ml = s_ml + (L * 4 + quarter) * FEW;
+        uint32_t o[FEW];
+        if (joins && L == 1) {
+          if ((lane & 3) == 0) ml[own] = make_float2(m_own, sum);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_full[quarter]);
+          ++n_join;
+          pending = true;
+          continue;
+        }
+        tmem_ld_32x8(tm_O, o);
+        if (joins) {
+          const float2* other = s_ml + (4 + quarter) * FEW;
+          uint32_t o1[FEW];
+          wait(&o_full[quarter], n_join & 1, p.status, ST_TIMEOUT_TMEM_FULL);
+          tc_fence_after();
+          tmem_ld_32x8(tm_O + DH, o1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < FEW; ++e) {
+            const float y = other[e].x, m = fmaxf(m_ref[e], y);
+            o[e] = __float_as_uint(__fmaf_rn(ex2(m_ref[e] - m), __uint_as_float(o[e]), __fmul_rn(ex2(y - m), __uint_as_float(o1[e]))));
+          }
+          const float2 y = other[own];
+          const float m = fmaxf(m_own, y.x);
+          sum = __fmaf_rn(ex2(m_own - m), sum, __fmul_rn(ex2(y.x - m), y.y));
+          m_own = m;
+          __syncwarp();
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&o_free[quarter]);
+          ++n_join;
+        }
+        if ((lane & 3) == 0) ml[own] = make_float2(m_own, sum);
+        meet();
+        // Rows of a shared item go where pieces go though it may not be cut: there they lie behind one another.
+        const bool cut = x.flags & (PIECE_CUT | PIECE_SHARED);
+        const unsigned row = cut ? (2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1)) * (2 * BM) : (own_slot(p) * p.NT + x.t0) * p.H + x.h * p.G;
+        const size_t n_rows = cut ? static_cast<size_t>(2) * gridDim.x * (2 * BM) : static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
+        float* base = cut ? p.cut : p.whole;
+        if (quarter == 0 && lane < rows) {
+          float2 y = s_ml[L * 4 * FEW + lane];
+#pragma unroll
+          for (int w = 1; w < 4; ++w) y.y += s_ml[(L * 4 + w) * FEW + lane].y;
+          reinterpret_cast<float2*>(base + n_rows * DH)[row + lane] = y;
+        }
+        tmem_ld_wait();
+        float* to = base + static_cast<size_t>(row) * DH + r;
+        if (r < DH) {
+#pragma unroll
+          for (int e = 0; e < FEW; ++e)
+            if (e < rows) to[e * DH] = __uint_as_float(o[e]);
+        }
+        __syncwarp();
+        tc_fence_before();
+        continue;
+      }
+      const int g = tile_g;
+      const int toks = two ? min(p.TT, x.n_tok - L * p.TT) : x.n_tok, tok = tile_tok + (two ? L * p.TT : 0);
+      const bool active = quarter * 32 < toks * p.G;      // whether any row of this warp counts
+      const bool valid = tile_tok < toks;
       const int t = x.t0 + tok;
       // positions that the row sees of this piece's
       int limit = x.kend;
       if (valid) {
         if (!(x.flags & PIECE_SHARED)) limit -= x.n_tok - 1 - tok;
-        else if (x.flags & PIECE_SHORT) limit = min(limit, p.pair ? p.row_limit[t] : p.seq_len[t]);
+        else if (x.flags & PIECE_SHORT) limit = min(limit, PLANNED ? p.row_limit[t] : p.seq_len[t]);
       }
       float m_ref = LOWEST, l = 0.f;
+#pragma unroll 1
       for (int i = first; i < nb; i += step, ++n) {
         // Waits in this loop may give up (the status word says so) but do not end it: lanes that left it one by one would be
         // missing at the warp barriers below.
@@ -834,7 +1116,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         // to half a step of it: nothing, unless scores are beyond 2^24. Those are scaled beforehand, rounded as the reference was.
         float factor = sl2;
         auto scaled_first = [&](uint32_t* u, auto count) {
-          if (__any_sync(0xffffffffu, fabsf(m_ref) > 16777216.f && m_ref != LOWEST)) {
+          if (__any_sync(0xffffffffu, valid && fabsf(m_ref) > 16777216.f && m_ref != LOWEST)) {
 #pragma unroll
             for (int c = 0; c < decltype(count)::value; c += 2) mul2(u[c], u[c + 1], sl2, sl2);
             factor = 1.f;
@@ -846,75 +1128,46 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           add2(sum4[c & 6], sum4[(c & 6) + 1], __float_as_uint(e0), __float_as_uint(e1));
           return pack_bf16x2(e0, e1);
         };
-        float alpha;
-        if (split) {
-          uint32_t v[32];
-          tmem_ld_32x32(tm_S + quarter * 32, v);
-          tmem_ld_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
-          m_blk = LOWEST;
+        uint32_t v[BN];
+        __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            if (quarter * 32 + c >= lim) v[c] = 0xff800000u;
-            if (quarter * 32 + c + 1 >= lim) v[c + 1] = 0xff800000u;
-            m_blk = max3(m_blk, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+        for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32_converged(tm_S + c * 32, v + c * 32);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
+        if (__any_sync(0xffffffffu, lim < BN)) {
+#pragma unroll
+          for (int w = 0; w < BN / 32; ++w) {
+            const int in = clampi(lim - w * 32, 0, 32);
+            const uint32_t seen = in == 32 ? 0xffffffffu : (1u << in) - 1;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!(seen >> c & 1)) v[w * 32 + c] = 0xff800000u;
           }
-          alpha = turn();
-          scaled_first(v, std::integral_constant<int, 32>{});
-          uint32_t pk[32];
-          if (i == first) {                // the weights of the others' positions stay zero
+        }
+        float m4[4] = {LOWEST, LOWEST, LOWEST, LOWEST};
 #pragma unroll
-            for (int c = 0; c < 32; ++c) pk[c] = 0;
-            tmem_st_32x32(tm_P, pk);
-            tmem_st_32x32(tm_P + 32, pk);
-            tmem_st_wait();
+        for (int c = 0; c < BN; c += 2)
+          m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+        m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float alpha = turn();
+        scaled_first(v, std::integral_constant<int, BN>{});
+        const int live = x.kend - (x.kbase + (x.j0 + i) * BN);      // positions that any row sees
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && live <= HALF) {    // nothing of it is multiplied
+            if (lane == 0) mbar_arrive(&p_full[2 * L + 1]);
+            break;
           }
+          uint32_t pk[HALF / 2];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) pk[c >> 1] = weigh(v[c], v[c + 1], c);
-          tmem_st_32x16(tm_P + quarter * 16, pk);
+          for (int c2 = 0; c2 < HALF; c2 += 2) pk[c2 >> 1] = weigh(v[h * HALF + c2], v[h * HALF + c2 + 1], h * HALF + c2);
+          tmem_st_32x32(tm_P + h * (HALF / 2), pk);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) { mbar_arrive(&p_full[2 * L]); mbar_arrive(&p_full[2 * L + 1]); }
-        } else {
-          uint32_t v[BN];
-          __syncwarp();
-#pragma unroll
-          for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32_converged(tm_S + c * 32, v + c * 32);
-          tmem_ld_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[C::SB == 1 ? 0 : L]);
-          if (__any_sync(0xffffffffu, lim < BN)) {
-#pragma unroll
-            for (int c = 0; c < BN; ++c)
-              if (c >= lim) v[c] = 0xff800000u;
-          }
-          float m4[4] = {LOWEST, LOWEST, LOWEST, LOWEST};
-#pragma unroll
-          for (int c = 0; c < BN; c += 2)
-            m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-          m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          alpha = turn();
-          scaled_first(v, std::integral_constant<int, BN>{});
-          const int live = x.kend - (x.kbase + (x.j0 + i) * BN);      // positions that any row sees
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h == 1 && live <= HALF) {    // nothing of it is multiplied
-              if (lane == 0) mbar_arrive(&p_full[2 * L + 1]);
-              break;
-            }
-            uint32_t pk[HALF / 2];
-#pragma unroll
-            for (int c2 = 0; c2 < HALF; c2 += 2) pk[c2 >> 1] = weigh(v[h * HALF + c2], v[h * HALF + c2 + 1], h * HALF + c2);
-            tmem_st_32x32(tm_P + h * (HALF / 2), pk);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * L + h]);
-          }
+          if (lane == 0) mbar_arrive(&p_full[2 * L + h]);
         }
         const float sum = ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) + ((sum4[4] + sum4[5]) + (sum4[6] + sum4[7]));
         l = __fadd_rn(__fmul_rn(l, alpha), sum);
@@ -945,7 +1198,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       }
       const int head = x.h * p.G + g;
       const bool cut = x.flags & PIECE_CUT;
-      const bool out_now = !cut && p.prefix == 0 && !split;
+      const bool out_now = !cut && p.prefix == 0;
       float* to = nullptr;
       if (valid && !out_now) {
         size_t row, rows;
@@ -955,8 +1208,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           rows = static_cast<size_t>(2) * gridDim.x * (2 * BM);
           base = p.cut;
         } else {
-          const int slot = (x.flags & PIECE_SHARED ? 0 : own_slot(p)) + (split ? quarter : 0);
-          row = (static_cast<size_t>(slot) * p.NT + t) * p.H + head;
+          row = (static_cast<size_t>(x.flags & PIECE_SHARED ? 0 : own_slot(p)) * p.NT + t) * p.H + head;
           rows = static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
           base = p.whole;
         }
@@ -965,25 +1217,23 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       }
       const float inv_l = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
-      for (int c0 = 0; c0 < DH; c0 += 64) {
-        uint32_t o[64];
+      for (int c0 = 0; c0 < DH; c0 += 32) {
+        uint32_t o[32];
         __syncwarp();
-#pragma unroll
-        for (int c = 0; c < 64; c += 32) tmem_ld_32x32_converged(tm_O + c0 + c, o + c);
+        tmem_ld_32x32_converged(tm_O + c0, o);
         if (joins) {
-          uint32_t o1[64];
-#pragma unroll
-          for (int c = 0; c < 64; c += 32) tmem_ld_32x32_converged(tm_O + DH + c0 + c, o1 + c);
+          uint32_t o1[32];
+          tmem_ld_32x32_converged(tm_O + DH + c0, o1);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < 32; ++e)
             o[e] = __float_as_uint(__fmaf_rn(w0, __uint_as_float(o[e]), __fmul_rn(w1, __uint_as_float(o1[e]))));
         }
         tmem_ld_wait();
         if (valid && out_now) {
           __nv_bfloat16* orow = p.out + t * p.ldo + head * DH + c0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
+          for (int e = 0; e < 4; ++e) {
             uint4 w;
             w.x = pack_bf16x2(__uint_as_float(o[e * 8 + 0]) * inv_l, __uint_as_float(o[e * 8 + 1]) * inv_l);
             w.y = pack_bf16x2(__uint_as_float(o[e * 8 + 2]) * inv_l, __uint_as_float(o[e * 8 + 3]) * inv_l);
@@ -993,7 +1243,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           }
         } else if (valid) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 8) st_global_v8(to + c0 + e, o + e);
+          for (int e = 0; e < 32; e += 8) st_global_v8(to + c0 + e, o + e);
         }
       }
       __syncwarp();
@@ -1024,7 +1274,7 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
   __shared__ float2 s_ml[ROWS][WAYS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS, slot = PACKED ? 0 : warp / WAYS;
   const int job = PACKED ? blockIdx.x * 4 + warp : blockIdx.x;
-  const int t = quotient(job, p.Hkv), h = job - t * p.Hkv;
+  const int t = p.by_heads.of(job), h = job - t * p.Hkv;
   pdl_trigger();
   pdl_wait();
   if (t >= p.NT) return;
@@ -1049,34 +1299,31 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
   int2 common = make_int2(0, 0);
   int first = 0;                           // token of the shared item
   if (p.prefix > 0) {
-    const int tile = quotient(t - q_lo, 2 * p.TT);
-    common = p.part[h * quotient(q_hi - q_lo + 2 * p.TT - 1, 2 * p.TT) + tile];
+    const int tile = p.by_span.of(t - q_lo);
+    common = p.part[h * p.by_span.of(q_hi - q_lo + 2 * p.TT - 1) + tile];
     first = q_lo + tile * 2 * p.TT;
   }
   int n[2];
   const float* from[2];
   const float2* ml[2];
   int jump[2];                             // rows from the first part to the second, which is 4 * BM in front of the third
-  int fold[2], apart[2];                   // log2 of the parts that a CTA has of an item, rows between them
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     // in bounds even where a wait of the other launch has given up and the entry is none
     int2 x = i ? own : common;
     x.y = clampi(x.y, 0, 2 * ctas - 1);
-    const int count = i && kend <= p.prefix ? 0 : clampi(x.x, 0, ctas - (x.y >> 1)), tok = t - (i ? t0 : first), log = p.split & (i ? 1 : 2) ? 2 : 0;
-    const bool cut = count > 1;
+    const int count = i && kend <= p.prefix ? 0 : clampi(x.x, 0, ctas - (x.y >> 1)), tok = t - (i ? t0 : first);
+    const bool cut = count > 1 || (!i && p.few & 2);
     const size_t at = cut ? static_cast<size_t>(x.y) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
                           : (static_cast<size_t>(i ? own_slot(p) : 0) * p.NT + t) * p.H + h * p.G;
     const size_t rows = cut ? static_cast<size_t>(4) * ctas * BM : static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
     const float* base = cut ? p.cut : p.whole;
-    n[i] = count << log;
+    n[i] = count;
     from[i] = base + at * DH + lane * F;
     ml[i] = reinterpret_cast<const float2*>(base + rows * DH) + at;
     jump[i] = x.y & 1 ? 2 * BM : 4 * BM;
-    fold[i] = log;
-    apart[i] = cut ? 32 : p.NT * p.H;
   }
-  if (p.prefix == 0 && !p.split && n[1] == 1) return;  // written out by its CTA
+  if (p.prefix == 0 && !p.few && n[1] == 1) return;  // written out by its CTA
   const int parts = n[0] + n[1];
 #pragma unroll 1
   for (int g0 = 0; g0 < p.G; g0 += ROWS * AT_ONCE) {
@@ -1097,8 +1344,8 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
       for (int b = 0; b < BATCH; ++b) {
         const int k = k0 + b * WAYS;
         const bool own = k >= n[0];
-        const int e = own ? k - n[0] : k, log = own ? fold[1] : fold[0], c = e >> log;
-        const int row = g + (e - (c << log)) * (own ? apart[1] : apart[0]) + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
+        const int c = own ? k - n[0] : k;
+        const int row = g + (c > 0 ? (own ? jump[1] : jump[0]) + (c - 1) * (4 * BM) : 0);
         const float* at_o = (own ? from[1] : from[0]) + static_cast<long long>(row) * DH;
         const float2* at_ml = (own ? ml[1] : ml[0]) + row;
 #pragma unroll
@@ -1201,13 +1448,15 @@ static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
   if (!rc && p.by_token) rc = make_tmap_3d_bf16_box(&q_token, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, 1);
   if (rc) return rc;
   if (!p.by_token) q_token = q_tile;
-  static PerDeviceOnce attr;
-  if (allow_smem(attr, attend_kernel<DH>, 227 * 1024, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  static PerDeviceOnce attr[2];
+  if (allow_smem(attr[0], attend_kernel<DH, false>, 227 * 1024, SB_ERR_LAUNCH) ||
+      allow_smem(attr[1], attend_kernel<DH, true>, 227 * 1024, SB_ERR_LAUNCH))
+    return SB_ERR_LAUNCH;
   const int slots = Cfg<DH>::slots(p.q_rows);
   p.vs = slots / 2;
   p.ks = slots - p.vs;
   if (p.pair && launch_dep(plan_kernel, dim3(1), dim3(1024), 0, s, p) != cudaSuccess) return SB_ERR_LAUNCH;
-  if (launch_dep(attend_kernel<DH>, dim3(ctas), dim3(THREADS), Cfg<DH>::smem_bytes(p.q_rows), s, tm, q_tile, q_token, p) != cudaSuccess) return SB_ERR_LAUNCH;
+  if (launch_dep(p.pair ? attend_kernel<DH, true> : attend_kernel<DH, false>, dim3(ctas), dim3(THREADS), Cfg<DH>::smem_bytes(p.q_rows), s, tm, q_tile, q_token, p) != cudaSuccess) return SB_ERR_LAUNCH;
   const long long jobs = static_cast<long long>(p.NT) * p.Hkv;
   // few rows have many parts each
   return (p.pair        ? launch_dep(join_kernel<DH, 1, true>, dim3((jobs + 3) / 4), dim3(128), 0, s, p, ctas)
@@ -1233,9 +1482,9 @@ static void sizes(spa::Params& p, int NT, int B, int H, int Hkv, int prefix, boo
   p.q_rows = (p.G * p.q_tokens + 7) / 8 * 8;
   p.max_pairs = ragged ? B + NT / (2 * p.TT) : B;
   p.shared_items = prefix > 0 ? Hkv * (NT / (2 * p.TT) + 1) : 0;
-  p.split = ragged || p.G > 8 ? 0 : NT * p.G > 8 ? 1 : 3;
+  p.few = ragged || p.G > spa::FEW ? 0 : NT * p.G > spa::FEW ? 1 : 3;
 }
-static int slots_of(const spa::Params& p) { return p.prefix > 0 || p.split ? spa::whole_slots(p) : 0; }
+static int slots_of(const spa::Params& p) { return p.prefix > 0 || p.few ? spa::whole_slots(p) : 0; }
 
 // Bytes of workspace that sb_shared_prefix_attention needs (32-byte aligned); 0 where it would refuse the sizes.
 extern "C" size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv, int dh, int ragged, int prefix) {
@@ -1277,15 +1526,16 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   const int ctas = spa::ctas_for(max_units);
   const spa::Layout at(NT, H, Hkv, dh, ctas, max_pairs, p.shared_items, planned, slots_of(p));
   if (at.total > workspace_bytes) return SB_ERR_ARG;
-  int box = 64;
-  while (page % box) box >>= 1;
+  int box_log = 6;
+  while (page % (1 << box_log)) --box_log;
   CUtensorMap tm;
-  const int rc = make_tmap_2d_bf16(&tm, pool, dh, rows, dh, 64, box);
+  const int rc = make_tmap_2d_bf16(&tm, pool, dh, rows, dh, 64, 1 << box_log);
   if (rc) return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq;
   p.block_table = block_table; p.max_blocks = max_blocks; p.seq_len = seq_len; p.prefix_table = prefix_table; p.cu_q = cu_q;
-  p.page = page; p.n_blocks = n_blocks; p.box = box;
+  p.page = page; p.n_blocks = n_blocks; p.box_log = box_log;
+  p.by_page.set(page); p.by_heads.set(Hkv); p.by_span.set(2 * p.TT);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo; p.fill = fill;
   p.hdr = planned ? reinterpret_cast<spa::Header*>(ws) : nullptr;
