@@ -42,8 +42,8 @@ static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * 168, "the shares draw on the 
 constexpr int TMEM_COLS = 512;
 constexpr int FEW = 8;         // rows of an item whose products are taken the other way round
 constexpr int QUEUE = 4;       // pieces that the producer may be ahead
-// What an item costs besides its blocks, in units (below): of few rows, of one tile, of two.
-constexpr int ITEM_FEW = 2, ITEM_ONE = 3, ITEM_TWO = 5;
+// Units (below) of a block of few rows, of one tile and of two, and of what an item costs besides its blocks.
+constexpr int BLOCK_FEW = 3, BLOCK_ONE = 2, BLOCK_TWO = 4, ITEM_FEW = 1, ITEM_ONE = 4, ITEM_TWO = 10;
 // A row's reference is its running maximum, so its largest weight is 1 and loses nothing when weights become bf16, and the sum is one of
 // weights before that. A reference that may lag behind by 2^8 saves rescales of O: 2 us of 64 (64 sequences behind 16384 positions), for an
 // error of 2.2e-3 in place of 2.0e-3 on unit scores and 1.3e-3 in place of 0.5e-3 on scores of four times the spread; with a sum of the
@@ -173,18 +173,22 @@ __device__ __forceinline__ int quotient(int a, int d) {
 }
 
 __device__ __forceinline__ int blocks_of(int positions) { return positions > 0 ? (positions + BN - 1) / BN : 0; }
-// An item lies in the line with one unit for a block of one tile of rows, two for a block of two, and in front of them what it costs
-// besides its blocks.
+// An item lies in the line with the units of its blocks, in front of which are those for what it costs besides.
+__device__ __forceinline__ int block_units(int n_tok, int TT, bool few) { return few ? BLOCK_FEW : n_tok > TT ? BLOCK_TWO : BLOCK_ONE; }
 __device__ __forceinline__ int head_units(int n_tok, int TT, bool few) { return few ? ITEM_FEW : n_tok > TT ? ITEM_TWO : ITEM_ONE; }
 __device__ __forceinline__ int units_of(int positions, int n_tok, int TT, bool few) {
-  return positions > 0 ? (blocks_of(positions) << (n_tok > TT ? 1 : 0)) + head_units(n_tok, TT, few) : 0;
+  return positions > 0 ? blocks_of(positions) * block_units(n_tok, TT, few) + head_units(n_tok, TT, few) : 0;
+}
+// a / block_units
+__device__ __forceinline__ int blocks_in(int units, int each) {
+  return each == BLOCK_FEW ? static_cast<int>(__umulhi(units, 0xaaaaaaabu) >> 1) : units >> (each >> 1);
 }
 
 // The deal of the line over the CTAs: shared items to the first of them, own ones to the others, the units of either evenly. A CTA also
 // has to begin a piece that its neighbour's share has cut, which is dearer for shared items (of two tiles) than for own ones (of a few
 // rows). With U and V units, `more` units dearer: U / n + more = V / (ctas - n) for n CTAs.
-// At least two units a CTA, so that one between the ends of an item has a block of it, whose two units may lie with two CTAs (the first
-// unit's CTA has the block).
+// At least the units of a block a CTA, so that one between the ends of an item has a block of it, whose units may lie with two CTAs (the
+// first unit's CTA has the block).
 struct Deal {                              // the part of it that CTA c has a share of
   int from, units, first, per, rem;        // where it begins in the line, its units, its first CTA
   __device__ Deal(int units_shared, int units_own, int grid, int c, int more) {
@@ -197,7 +201,7 @@ struct Deal {                              // the part of it that CTA c has a sh
     from = own ? units_shared : 0;
     units = own ? units_own : units_shared;
     first = own ? n : 0;
-    const int share = max(1, min(own ? grid - n : n, units >> 1));
+    const int share = max(1, min(own ? grid - n : n, units / BLOCK_TWO));
     per = units / share;                   // may be large
     rem = units - per * share;
   }
@@ -366,13 +370,13 @@ struct Walk {
       const int stop = min(size, off + (u1 - u)), begin = u - off;
       u += stop - off;
       // a block belongs to the CTA that has its first unit
-      const int two = x.n_tok > p.TT ? 1 : 0;
-      const int head = head_units(x.n_tok, p.TT, few_rows<PLANNED>(p, x)), blocks = (size - head) >> two;
-      x.j0 = (max(0, off - head) + two) >> two;
-      x.j1 = (max(0, stop - head) + two) >> two;
+      const bool few = few_rows<PLANNED>(p, x);
+      const int head = head_units(x.n_tok, p.TT, few), each = block_units(x.n_tok, p.TT, few), blocks = blocks_in(size - head, each);
+      x.j0 = blocks_in(max(0, off - head) + each - 1, each);
+      x.j1 = blocks_in(max(0, stop - head) + each - 1, each);
       if (x.j1 == x.j0) continue;
       if (x.j1 - x.j0 != blocks) x.flags |= PIECE_CUT;
-      last = begin + head + ((blocks - 1) << two);
+      last = begin + head + (blocks - 1) * each;
       return true;
     }
   }
@@ -1520,7 +1524,7 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   sizes(p, NT, B, H, Hkv, prefix, planned);
   const int TT = p.TT, max_pairs = p.max_pairs;
   const uint64_t cap = static_cast<uint64_t>(max_blocks) * page;
-  const uint64_t own = 2 * cap / spa::BN + 2 + spa::ITEM_TWO, common = 2 * prefix / spa::BN + 2 + spa::ITEM_TWO;     // units of an item
+  const uint64_t own = spa::BLOCK_TWO * (cap / spa::BN + 1) + spa::ITEM_TWO, common = spa::BLOCK_TWO * (prefix / spa::BN + 1) + spa::ITEM_TWO;     // units of an item
   if (Hkv * (max_pairs * own + (NT / (2 * TT) + 1) * common) >= (1ull << 31))
     return SB_ERR_TOO_LARGE;
   const int ctas = spa::ctas_for(max_units);
