@@ -5,18 +5,19 @@
 // destination pools; no destination is a source or another copy's destination, so the order of copies does not matter. Ids outside their
 // pools are skipped.
 //
-// Bound by memory: each byte is read and written once. A CTA copies up to 32 KB of one page of one layer, eight 16-byte words a thread, all
+// Bound by memory: each byte is read and written once. A CTA copies up to 16 KB of one page of one layer, four 16-byte words a thread, all
 // of whose loads are under way before the first store; layers are the slowest grid index, so a page that goes to many (a fork) is read
-// from L2 by all but the first. 128 pages of 256 KB in eight layers 83 us, 0.99 of the copy rate; 301 pages of 8 KB in 32 layers 26.9, 0.90;
-// 40 of 64 positions to 16 pages in 32 layers 18.5, of which 84 MB are writes (four copies a CTA, which hold a source that stays the same
-// in registers, gained nothing and cost the first of these 2 us).
+// from L2 by all but the first. What is written is marked as the first to leave L2: a fork of all layers is more than fits beside what the
+// next steps read. 128 pages of 256 KB in eight layers 83 us, 0.99 of the copy rate; 301 pages of 8 KB in 32 layers 26.3, 0.92; 40 of 64
+// positions to 16 pages in 32 layers 15.0, of which 84 MB are writes, 0.91 (stores without the mark 17.1; two words a thread 18.2, eight
+// 21.3; copies as the fastest index 19.2; four copies a CTA, which hold a source that stays the same in registers, gain nothing).
 #include "api.h"
 #include "dependent.cuh"
 
 namespace sb {
 namespace pages {
 
-constexpr int MAX_LAYERS = 64, THREADS = 256, WORDS = 8;      // pools of a launch; words of a thread
+constexpr int MAX_LAYERS = 64, THREADS = 256, WORDS = 4;      // pools of a launch; words of a thread
 
 struct Params {
   const void* src[MAX_LAYERS];
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(THREADS) copy_pages_kernel(const __grid_consta
       if (first + k * THREADS < words) v[k] = s[at[k]];
 #pragma unroll
     for (int k = 0; k < WORDS; ++k)
-      if (first + k * THREADS < words) d[at[k]] = v[k];
+      if (first + k * THREADS < words) __stcs(d + at[k], v[k]);
   }
 }
 
