@@ -6,14 +6,29 @@
 // sequences against one copy of K and V, and each sequence's rows against what it has for itself. Parts (m_i, l_i, o_i) of a row,
 // o_i not divided by l_i, join as m = max m_i, w_i = 2^(m_i - m), o = sum w_i o_i / sum w_i l_i (scores in units of log 2).
 //
-// Both parts are the same work for a CTA: a tile of 128 rows (tokens times the query heads of one kv head), a table of pages and a
-// range of 128-position blocks of keys. An item is all of that for one tile of rows:
-//   shared: (kv head, tile of consecutive tokens, whatever their sequences), blocks [0, P / 128)
-//   own:    (sequence, tile of its tokens, kv head), blocks of [P, limit of its last row)
+// Both parts are the same work for a CTA: up to two tiles of 128 rows (tokens times the query heads of one kv head), a table of pages and
+// a range of 128-position blocks of keys. An item is all of that for one set of rows:
+//   shared: (kv head, consecutive tokens, whatever their sequences), blocks [0, P / 128)
+//   own:    (sequence, tokens of it, kv head), blocks of [P, limit of its last row)
 // Where the sequences bring a whole tile of rows each there is nothing to share, and their own items start at position 0.
-// The blocks of all items form one line, which is dealt out evenly over the CTAs; what lies in a CTA's share of an item is a piece.
+// The blocks of all items form one line, which is dealt out over the CTAs, one a SM; what lies in a CTA's share of an item is a piece.
 // An item that is not cut and has no other part is written out at once, pieces of the others go to a workspace and a second,
-// dependent launch joins them in a fixed order.
+// dependent launch joins them in a fixed order, so that answers do not depend on what ran when.
+//
+// In a CTA a warp brings rows and K by TMA, one V, one issues S = Q K^T, one O += P V, and two lanes of four warps each turn scores into
+// weights: lane by lane a tile each, or every second block of one tile, so that one lane's exponentials (128 x 128 of them take 1024
+// cycles) run beside the products of the other. Scores, weights and both sums are in tensor memory, K and V in rings of blocks.
+//
+// What bounds it, B200, 32 / 8 heads of 128, a call in a graph:
+//   many rows and a long prefix: the exponentials and what lies between them. A block of two tiles takes some 3700 cycles, 2048 of them
+//     exponentials on each SM sub-partition and 1024 products: 520 tokens of 16 sequences behind 8192 positions 83 us, 0.54 of the matrix rate.
+//   one token a sequence: 64 sequences behind 16384 positions, up to 512 of their own, 60.5 us where memory would take 21: the sequences'
+//     own items, 512 of two or three blocks, are as many starts and ends, and what they fetch of their own code; shared blocks are read
+//     once, but a CTA's ten of them bring a new maximum, thus a pass over O, almost every time.
+//   few sequences: latency. 4 samples behind 512 positions 10.8 us: 7 until the last CTA is done (3 of them until the first block has
+//     come), 1 to the joining launch, 2 for that to find and to add up its parts.
+// Code counts: pieces of one block go through most of the kernel once each. From 148 KB to 107 (and 76 where the batch is ragged, by a
+// kernel of its own) the times above fell by 5 to 15 %.
 #include "sm100_ptx.cuh"
 #include "api.h"
 #include "dependent.cuh"
@@ -40,14 +55,16 @@ constexpr int THREADS = 384;   // loaders of rows and K, and of V, issuers of bo
 constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * 168, "the shares draw on the registers of the launch");
 constexpr int TMEM_COLS = 512;
-constexpr int FEW = 8;         // rows of an item whose products are taken the other way round
+constexpr int FEW = 8;         // rows of an item whose products are taken the other way round (few_rows)
 constexpr int QUEUE = 4;       // pieces that the producer may be ahead
-// Units (below) of a block of few rows, of one tile and of two, and of what an item costs besides its blocks.
+// Units (below) of a block of few rows, of one tile and of two, and of what an item costs besides its blocks, about half a microsecond each.
+// 16 sequences behind 4000 positions 17.6 us, 33 behind 5003 32.1, 64 behind 16384 60.5, 256 of a block each behind 1024 76; with blocks of
+// 2, 2, 4 and items of 4, 6, 10 they take 18.2, 32.9, 59.0 and 82, with 3, 2, 4 and 3, 5, 10 18.9, 32.9, 63.1 and 82.
 constexpr int BLOCK_FEW = 3, BLOCK_ONE = 2, BLOCK_TWO = 4, ITEM_FEW = 1, ITEM_ONE = 4, ITEM_TWO = 10;
 // A row's reference is its running maximum, so its largest weight is 1 and loses nothing when weights become bf16, and the sum is one of
-// weights before that. A reference that may lag behind by 2^8 saves rescales of O: 2 us of 64 (64 sequences behind 16384 positions), for an
-// error of 2.2e-3 in place of 2.0e-3 on unit scores and 1.3e-3 in place of 0.5e-3 on scores of four times the spread; with a sum of the
-// rounded weights that is 1.0e-3, but the sum costs 5 to 12 us of 65 to 105.
+// weights before that. A reference that may lag behind by 2^8 saves rescales of O (520 tokens behind 8192 positions 77 us for 83, 64
+// sequences behind 16384 positions 58 for 60), for an error of 2.2e-3 in place of 2.0e-3 on unit scores and 1.3e-3 in place of 0.5e-3 on
+// scores of four times the spread; with a sum of the rounded weights that is 1.0e-3, but the sum costs more than the rescales.
 constexpr float LOWEST = -3.402823466e38f;   // reference of a row that has seen nothing: 2^(-inf - LOWEST) is 0
 
 template <int DH>
@@ -109,7 +126,6 @@ struct Params {
   int B, NT, H, Hkv, G, TT;
   int few;             // items whose products are taken the other way round: 1 a sequence's own, 2 shared ones (few_rows)
   int q_tokens;        // of the box that brings a tile of rows
-  int by_token;        // whether there is a box of one token too
   int q_rows;          // of a tile in shared memory, a multiple of 8; the tensor core reads 128, those behind are rows of no one
   int ks, vs;          // blocks of K and V in shared memory
   float scale_log2;
@@ -121,7 +137,8 @@ struct Params {
   Pair* pair;
   int* row_limit;      // [NT]
   int* row_pair;       // [NT], -1: of no sequence
-  int2* part;          // [Hkv][shared tiles] and then [pairs][Hkv]: CTAs that have a piece of the item; the first of these, times two, 1 for its second piece
+  int2* part;          // [Hkv][shared tiles] and then [pairs][Hkv]: CTAs that have a piece of the item; twice the first of these, 1 more for
+                       // its second piece
   int* row_t0;         // [NT] first token of its pair
   float* whole;        // [slots][NT][H][dh], and [slots][NT][H][2] behind it: items that were not cut, shared and then own
   float* cut;          // [2 * CTAs][256][dh], and [2 * CTAs][256][2] behind it: first and last pieces of the CTAs
@@ -147,8 +164,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 constexpr int kTries = 1 << 21;
-// Wait of a whole warp, all lanes with one result; bounded like mbar_wait, in fewer instructions: the kernel below is bound by what it
-// has to fetch of its own code where a CTA goes through many short pieces (with mbar_wait at every wait 136 KB).
+// Wait of a whole warp, all lanes with one result; bounded like mbar_wait, in a third of the instructions, since there are some
+// forty in the kernel.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status, int code) {
   int tries = 0;
 #pragma unroll 1
@@ -186,7 +203,8 @@ __device__ __forceinline__ int blocks_in(int units, int each) {
 
 // The deal of the line over the CTAs: shared items to the first of them, own ones to the others, the units of either evenly. A CTA also
 // has to begin a piece that its neighbour's share has cut, which is dearer for shared items (of two tiles) than for own ones (of a few
-// rows). With U and V units, `more` units dearer: U / n + more = V / (ctas - n) for n CTAs.
+// rows). With U and V units, `more` units dearer: U / n + more = V / (ctas - n) for n CTAs. Shares that do not mind the border leave some
+// CTAs with many ends of shared items, others with none: 12.5 us in place of 10.9 (4 samples behind 512), 20.0 / 18.6 (16 behind 4000).
 // At least the units of a block a CTA, so that one between the ends of an item has a block of it, whose units may lie with two CTAs (the
 // first unit's CTA has the block).
 struct Deal {                              // the part of it that CTA c has a share of
@@ -249,22 +267,23 @@ struct Piece {
 // CUT: not all of its item; FIRST: begins where the CTA's share does; SHORT: some row may end inside
 constexpr int PIECE_SHARED = 1, PIECE_CUT = 2, PIECE_FIRST = 4, PIECE_SHORT = 8, SEQUENCE = 4;
 
-// A CTA's pieces, found by a whole warp. The plan of a batch of one token a sequence is summed up on the way, 32 sequences at a time;
-// anything else has been planned (plan_kernel).
 // Slots of the rows of items that were not cut: of shared items, then of own ones.
 __host__ __device__ __forceinline__ int own_slot(const Params& p) { return p.prefix == 0 ? 0 : 1; }
 __host__ __device__ __forceinline__ int whole_slots(const Params& p) { return own_slot(p) + 1; }
 
 // Whether the products are taken the other way round, S^T = K Q^T and O^T = V^T P^T, of up to eight rows (a sequence of one token has as
 // many as query heads share a kv head). In a tile of 128 rows they would be lanes 0 to 7 of one warp, which would go through 128 columns
-// of scores and dh of O one by one; here a thread has a position, or a column of O, of all rows, an eighth of the instructions.
+// of scores and dh of O one by one; here a thread has a position, or a column of O, of all rows, an eighth of the instructions. 64
+// sequences behind 16384 positions, 500 of their own: 57 us, as tiles of 128 rows 65 to 71; 64 of their own, a block each, where the code
+// of both weighs more than what it saves, 55 and 50; 16 sequences with 1 of their own 27.5 and 25.
 template <bool PLANNED>
 __device__ __forceinline__ bool few_rows(const Params& p, const Piece& x) {
   return !PLANNED && (x.flags & PIECE_SHARED ? p.few & 2 : p.few & 1) != 0;
 }
 
-// The items from one on are gone through without a division or a search: a warp that looks for every piece anew takes 4000 cycles for
-// one, as long as the others take for a piece of one block.
+// A CTA's pieces, found by a whole warp. The plan of a batch of one token a sequence is summed up on the way, 32 sequences at a time; a
+// ragged one has been planned (plan_kernel). From one item to the next there is no division and no search, which took 4000 cycles a piece,
+// as long as the others take for one of one block.
 template <bool PLANNED>
 struct Walk {
   const Params& p;
@@ -382,14 +401,14 @@ struct Walk {
   }
 };
 
-// Plan of a ragged batch, or of more sequences than the CTAs plan for themselves: one CTA.
+// Plan of a ragged batch: one CTA.
 __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   __shared__ int s_warp[32];
   __shared__ int s_hi, s_pairs, s_sum, s_least;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   pdl_wait();
-  if (tid == 0) { s_hi = p.cu_q ? clampi(p.cu_q[0], 0, p.NT) : 0; s_pairs = 0; s_sum = 0; s_least = INT_MAX; }
+  if (tid == 0) { s_hi = clampi(p.cu_q[0], 0, p.NT); s_pairs = 0; s_sum = 0; s_least = INT_MAX; }
   for (int t = tid; t < p.NT; t += 1024) { p.row_limit[t] = 0; p.row_pair[t] = -1; }
   __syncthreads();
   const int q_lo = s_hi;
@@ -398,8 +417,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
     const int b = b0 + tid;
     int start = 0, end = 0;
     if (b < p.B) {
-      start = p.cu_q ? clampi(p.cu_q[b], 0, p.NT) : b;
-      end = p.cu_q ? clampi(p.cu_q[b + 1], 0, p.NT) : b + 1;
+      start = clampi(p.cu_q[b], 0, p.NT);
+      end = clampi(p.cu_q[b + 1], 0, p.NT);
     }
     // offsets that fall back would give rows to two sequences: the largest end so far is where a sequence starts at least
     int top = b < p.B ? max(start, end) : 0;
@@ -541,7 +560,7 @@ struct Ring {
 
 template <int DH, bool PLANNED>
 __global__ void __launch_bounds__(THREADS, 1)
-attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap q_tile, const __grid_constant__ CUtensorMap q_token,
+attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap q_tile,
               const __grid_constant__ Params p) {
   using C = Cfg<DH>;
   const int KS = p.ks, VS = p.vs;
@@ -598,7 +617,6 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     fence_proxy_async_smem();
     prefetch_tmap(&tmap);
     prefetch_tmap(&q_tile);
-    prefetch_tmap(&q_token);
   }
   if (warp == 1) {
     tmem_alloc(tmem_holder, TMEM_COLS);
@@ -700,16 +718,15 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         }
         both = two;
         if (ok && lane == 0) {
-          // The box of a tile brings its tokens and, behind the last of them, rows of others that no one reads.
-          const bool one = x.n_tok == 1 && p.by_token;
-          const int tiles = two ? 2 : 1, bytes = (one ? 1 : p.q_tokens) * p.G * 128;
-          const CUtensorMap* map = one ? &q_token : &q_tile;
+          // The box of a tile brings its tokens and, behind the last of them, rows of others that no one reads. For one token a box of its
+          // own gains nothing (256 sequences behind 1024 positions 78.8 us with it, 75.5 without).
+          const int tiles = two ? 2 : 1, bytes = p.q_tokens * p.G * 128;
           uint64_t* bar = &q_full[n_pieces & 1];
           mbar_arrive_expect_tx(bar, tiles * C::NCH * bytes);
 #pragma unroll 1
           for (int i = 0; i < tiles * C::NCH; ++i) {
             const int tile = i / C::NCH, c = i % C::NCH;
-            tma_load_3d(sQ + (two ? tile : n_pieces & 1) * q_bytes + c * q_chunk, map, bar, c * 64, x.h * p.G, x.t0 + tile * p.TT);
+            tma_load_3d(sQ + (two ? tile : n_pieces & 1) * q_bytes + c * q_chunk, &q_tile, bar, c * 64, x.h * p.G, x.t0 + tile * p.TT);
           }
         }
         __syncwarp();
@@ -1267,7 +1284,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
 
 // Joins the parts of rows. The heads of a (token, kv head) have the same parts, so they are looked up once. PACKED, for many rows of few
 // parts: a warp has the rows of a (token, kv head), two at a time, and a CTA four of these. Otherwise a CTA has them, four at a time, a
-// row to WAYS warps, which share its parts; their sums meet in shared memory.
+// row to WAYS warps, which share its parts; their sums meet in shared memory. What an item's parts are has been left by the CTA that has its
+// first block (Params::part): worked out here it takes 1.5 us longer.
 template <int DH, int WAYS, bool PACKED>
 __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant__ Params p, int ctas) {
   constexpr int F = DH / 32;               // columns of a lane
@@ -1444,14 +1462,10 @@ struct Layout {
 
 template <int DH>
 static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
-  CUtensorMap q_tile, q_token;
+  CUtensorMap q_tile;
   // (64 columns, the query heads of a kv head, tokens): the rows of a tile in the order in which it has them
-  int rc = make_tmap_3d_bf16_box(&q_tile, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, p.q_tokens);
-  // a map takes a microsecond to make: up to eight tokens a box of one saves less
-  p.by_token = p.q_tokens > 8;
-  if (!rc && p.by_token) rc = make_tmap_3d_bf16_box(&q_token, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, 1);
+  const int rc = make_tmap_3d_bf16_box(&q_tile, p.q, DH, p.H, p.NT, DH, p.ldq, 64, p.G, p.q_tokens);
   if (rc) return rc;
-  if (!p.by_token) q_token = q_tile;
   static PerDeviceOnce attr[2];
   if (allow_smem(attr[0], attend_kernel<DH, false>, 227 * 1024, SB_ERR_LAUNCH) ||
       allow_smem(attr[1], attend_kernel<DH, true>, 227 * 1024, SB_ERR_LAUNCH))
@@ -1460,12 +1474,19 @@ static int launch(const CUtensorMap& tm, Params p, int ctas, cudaStream_t s) {
   p.vs = slots / 2;
   p.ks = slots - p.vs;
   if (p.pair && launch_dep(plan_kernel, dim3(1), dim3(1024), 0, s, p) != cudaSuccess) return SB_ERR_LAUNCH;
-  if (launch_dep(p.pair ? attend_kernel<DH, true> : attend_kernel<DH, false>, dim3(ctas), dim3(THREADS), Cfg<DH>::smem_bytes(p.q_rows), s, tm, q_tile, q_token, p) != cudaSuccess) return SB_ERR_LAUNCH;
+  if (launch_dep(p.pair ? attend_kernel<DH, true> : attend_kernel<DH, false>, dim3(ctas), dim3(THREADS), Cfg<DH>::smem_bytes(p.q_rows), s,
+                 tm, q_tile, p) != cudaSuccess)
+    return SB_ERR_LAUNCH;
   const long long jobs = static_cast<long long>(p.NT) * p.Hkv;
-  // few rows have many parts each
-  return (p.pair        ? launch_dep(join_kernel<DH, 1, true>, dim3((jobs + 3) / 4), dim3(128), 0, s, p, ctas)
-          : jobs <= 256 ? launch_dep(join_kernel<DH, 4, false>, dim3(jobs), dim3(512), 0, s, p, ctas)
-                        : launch_dep(join_kernel<DH, 1, false>, dim3(jobs), dim3(128), 0, s, p, ctas)) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  // Few rows of many parts have a warp for every fourth part, many rows half a warp each, us of a call: 16 sequences behind 4000 positions
+  // 17.4 with four ways, 18.4 with one, 4 behind 2048 12.9 / 13.8, 4 behind 1024 (four parts) 12.2 / 10.9, 32 behind 4000 23.9 / 23.4; 2
+  // sequences of 4 tokens packed 20.5, else 16.5, 32 of 4 30.3 / 28.0, 64 of 6 50.6 / 54.2. The parts of a shared item: as many as CTAs
+  // for each of them, of two blocks at least.
+  const long long items = p.Hkv * ((p.NT + 2LL * p.TT - 1) / (2 * p.TT)), blocks = p.prefix / BN;
+  const long long parts = blocks / 2 < ctas / items ? blocks / 2 : ctas / items;
+  return (jobs > 1024 && p.pair        ? launch_dep(join_kernel<DH, 1, true>, dim3((jobs + 3) / 4), dim3(128), 0, s, p, ctas)
+          : jobs <= 192 && parts >= 7 ? launch_dep(join_kernel<DH, 4, false>, dim3(jobs), dim3(512), 0, s, p, ctas)
+                                      : launch_dep(join_kernel<DH, 1, false>, dim3(jobs), dim3(128), 0, s, p, ctas)) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 static int ctas_for(long long units) {
@@ -1524,7 +1545,8 @@ extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const vo
   sizes(p, NT, B, H, Hkv, prefix, planned);
   const int TT = p.TT, max_pairs = p.max_pairs;
   const uint64_t cap = static_cast<uint64_t>(max_blocks) * page;
-  const uint64_t own = spa::BLOCK_TWO * (cap / spa::BN + 1) + spa::ITEM_TWO, common = spa::BLOCK_TWO * (prefix / spa::BN + 1) + spa::ITEM_TWO;     // units of an item
+  const uint64_t own = spa::BLOCK_TWO * (cap / spa::BN + 1) + spa::ITEM_TWO;           // units of an item
+  const uint64_t common = spa::BLOCK_TWO * (prefix / spa::BN + 1) + spa::ITEM_TWO;
   if (Hkv * (max_pairs * own + (NT / (2 * TT) + 1) * common) >= (1ull << 31))
     return SB_ERR_TOO_LARGE;
   const int ctas = spa::ctas_for(max_units);

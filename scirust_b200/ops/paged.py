@@ -143,7 +143,10 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
         return out.zero_() if fill or cu_q is None else out
     per_tile = TILE_ROWS // (H // Hkv)
     if cu_q is not None and n >= B * per_tile:
-        prefix = 0                                  # the sequences fill tiles by themselves: nothing to gain from a part in common
+        # The sequences fill tiles by themselves: a part in common saves no tile, and its sums have to be joined. us, own / in common, 16
+        # sequences of 16, 24, 32, 64, 128 tokens behind 4096 positions (32 / 8 heads): 49.9 / 44.0, 51.8 / 50.7, 53.7 / 57.2, 89.4 / 97.5,
+        # 161 / 180; of 48, whose second tile is half empty, 86.4 / 77.5; 4 sequences of 32 26.2 / 28.2
+        prefix = 0
     L = max_blocks * page if max_len is None else min(int(max_len), max_blocks * page)
     pairs = B if cu_q is None else B + n // per_tile
     units = Hkv * (-(-n // per_tile) * -(-prefix // BLOCK) + pairs * max(0, -(-(L - prefix) // BLOCK)))
