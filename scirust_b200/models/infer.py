@@ -571,12 +571,15 @@ class InferenceEngine:
 
     def _shares(self, B: int, P: int) -> bool:
         """Whether the attention that reads a common prefix of ``P`` positions once beats ``decode_attention``, which reads it for each of
-        ``B`` sequences (from the cache of the chip, while it fits). Its second launch costs about 5 us, so what the others need not read
-        again has to be worth that. us in a graph, 32 positions behind the prefix, decode / shared, 32 / 8 heads of 128:
-        4 x 2048 13.8 / 14.1, 4 x 4096 18.1 / 16.8, 8 x 1024 13.9 / 15.3, 8 x 2048 18.4 / 15.5, 16 x 512 14.3 / 15.6, 16 x 1024 18.9 / 16.4,
-        64 x 256 22.7 / 29.7, 64 x 1024 49.4 / 31.6, 64 x 8192 304 / 42.7, 2 x 8192 17.3 / 20.2; 16 / 16 heads of 64: 16 x 512 15.1 / 15.4,
-        16 x 1024 21.6 / 19.3, 64 x 512 29.5 / 39.4, 64 x 1024 51.8 / 42.4; 8 / 1 heads of 128: 64 x 1024 16.7 / 19.3, 64 x 2048 21.2 / 21.0."""
-        return P >= 1024 and (B - 1) * P * self.Hkv * self.cfg.head_dim * 4 >= 45 << 20
+        ``B`` sequences (from the cache of the chip, while it fits), but is one launch. us in a graph, 32 positions behind the prefix,
+        decode / shared. 32 / 8 heads of 128: 2 x 64 5.3 / 8.3, 2 x 256 9.9 / 8.8, 2 x 2048 11.2 / 11.0, 16 x 64 7.1 / 11.4, 16 x 256 13.4 /
+        12.3, 64 x 256 22.8 / 18.3, 16 x 8192 82.1 / 19.7, 64 x 8192 305 / 40.6; 16 / 8 heads: 2 x 256 8.1 / 8.7, 16 x 256 11.2 / 12.0, 2 x
+        512 8.9 / 8.9, 16 x 512 14.0 / 12.2; 8 / 1 heads: 2 x 256 13.4 / 11.0, 4 x 8192 13.6 / 14.4, 64 x 8192 48.0 / 24.7. Heads of 64, one
+        or three query heads a kv head: 16 / 16 2 x 2048 11.2 / 11.4, 4 x 1024 10.3 / 11.0, 8 x 1024 13.9 / 11.6, 4 x 2048 14.5 / 11.5, 64 x
+        512 29.5 / 30.5, 64 x 1024 51.8 / 35.2; 12 / 4 4 x 1024 9.2 / 10.3, 8 x 1024 11.5 / 10.3, 32 x 512 11.0 / 12.2."""
+        if self.cfg.head_dim == 128:
+            return B > 1 and P >= (256 if self.H >= 4 * self.Hkv else 512)
+        return P >= 1024 and (B - 1) * P >= 4096
 
     def generate_shared(self, prefix: torch.Tensor, suffixes, max_new: int, params: SamplingParams | None = None, seed: int = 0):
         """Generation for sequences that begin alike. ``prefix`` [P] goes through the model once, and its pages of the cache are shared;

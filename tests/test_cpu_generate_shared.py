@@ -72,10 +72,11 @@ def test_command_prints_a_line_for_each_sample(model, tmp_path, capsys):
     assert cli.run(args + ["--samples", "0"]) != 0
 
 
-@pytest.mark.parametrize("H, Hkv, B, P, want", [(32, 8, 4, 2048, False), (32, 8, 4, 4096, True), (32, 8, 2, 8192, False), (32, 8, 8, 1024, False),
-                                                (32, 8, 16, 1024, True), (32, 8, 64, 512, False), (8, 1, 64, 1024, False), (8, 1, 64, 2048, True)])
-def test_rule_of_which_attention_runs(H, Hkv, B, P, want):
-    eng = InferenceEngine(GQADecoder(SciAgentConfig(16, 128 * H, 0, H, Hkv, 16, 64, 10000.0)), max_batch=1, max_seq=8, page=8)
+@pytest.mark.parametrize("H, Hkv, dh, B, P, want", [(32, 8, 128, 2, 255, False), (32, 8, 128, 2, 256, True), (32, 8, 128, 1, 4096, False),
+                                                    (16, 8, 128, 16, 511, False), (16, 8, 128, 2, 512, True), (16, 16, 64, 4, 1024, False),
+                                                    (16, 16, 64, 8, 1024, True), (16, 16, 64, 64, 1000, False), (12, 4, 64, 2, 4096, True)])
+def test_rule_of_which_attention_runs(H, Hkv, dh, B, P, want):
+    eng = InferenceEngine(GQADecoder(SciAgentConfig(16, dh * H, 0, H, Hkv, 16, 64, 10000.0)), max_batch=1, max_seq=8, page=8)
     assert eng._shares(B, P) is want
 
 
