@@ -56,30 +56,27 @@ int32_t sbrt_balloc_alloc(SbBlockAlloc* a, int32_t n, int32_t* out) {
   return 0;
 }
 // Gives up one owner of each block (an id may occur several times); the last owner's returns to the pool. Ids outside the pool, and more
-// blocks than are out, are rejected (-1) and nothing is freed.
+// owners of a block than it has, are rejected (-1) and nothing is freed.
 int32_t sbrt_balloc_free(SbBlockAlloc* a, const int32_t* ids, int32_t n) {
   for (int32_t i = 0; i < n; ++i)
     if (ids[i] < 0 || ids[i] >= a->n_blocks) return -1;
-  std::vector<int32_t> back;
-  try {
-    back.reserve(n > 0 ? n : 0);
-  } catch (...) {
-    return -1;
-  }
   for (int32_t i = 0; i < n; ++i) {
-    if (a->more[ids[i]] > 0) --a->more[ids[i]];
-    else back.push_back(ids[i]);
+    const int32_t id = ids[i];
+    if (!a->used[id]) {                   // one owner more than it has: as they were, from the last on
+      while (i-- > 0) {
+        if (a->used[ids[i]]) ++a->more[ids[i]];
+        else a->used[ids[i]] = 1;
+      }
+      return -1;
+    }
+    if (a->more[id] > 0) --a->more[id];
+    else a->used[id] = 0;
   }
-  if (a->free_list.size() + back.size() > static_cast<size_t>(a->n_blocks)) {
-    // as they were: an id keeps its last owner in `back`, so what it had beyond is the times that it occurs less those
-    for (int32_t i = 0; i < n; ++i) ++a->more[ids[i]];
-    for (int32_t id : back) --a->more[id];
-    return -1;
-  }
-  for (int32_t id : back) {
-    a->free_list.push_back(id);           // within what is reserved
-    a->used[id] = 0;
-  }
+  // Freed ids go back in the order in which their last owners are given up: `more` marks the ones that are not in the list yet.
+  for (int32_t i = 0; i < n; ++i)
+    if (!a->used[ids[i]]) ++a->more[ids[i]];
+  for (int32_t i = 0; i < n; ++i)
+    if (!a->used[ids[i]] && --a->more[ids[i]] == 0) a->free_list.push_back(ids[i]);        // within what is reserved
   return 0;
 }
 // One more owner for each block (an id may occur several times); -1, and none, if one of them is not in use.

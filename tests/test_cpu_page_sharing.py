@@ -28,6 +28,18 @@ def test_a_page_is_free_with_its_last_owner():
         a.owners(4)
 
 
+def test_more_owners_than_a_page_has_are_refused():
+    a = BlockAllocator(4)
+    one, two = a.alloc(2)
+    a.share([two])
+    for ids in ([one, one], [two, two, two], [one, two, one], [3], [two, 3]):
+        with pytest.raises(ValueError):
+            a.free(ids)
+        assert (a.owners(one), a.owners(two), a.num_free()) == (1, 2, 2)
+    a.free([two, one, two])
+    assert sorted(a.alloc(4)) == [0, 1, 2, 3]            # each once
+
+
 def test_random_histories_of_owners():
     rng = random.Random(3)
     for _ in range(20):
