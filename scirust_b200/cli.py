@@ -188,6 +188,9 @@ def cmd_sciagent(a):
         return EXIT_OK
     if a.action == "generate":
         return cmd_infer(a)
+    if a.samples != 1:
+        sys.stderr.write("error: --samples is for generate\n")
+        return EXIT_USAGE
     if a.action == "quantize":
         import torch
         from . import quantization as Q
@@ -760,7 +763,7 @@ def build_parser():
     s.add_argument("--group", type=int, default=32)
     s.add_argument("--path", default="")
     s.add_argument("--lines", default="")
-    s.set_defaults(fn=lambda a: cmd_sciagent_text(a) if a.action in ("ask", "chat", "explain") else cmd_sciagent(a))
+    s.set_defaults(fn=lambda a: cmd_sciagent_text(a) if a.action in ("ask", "chat", "explain") and a.samples == 1 else cmd_sciagent(a))
     lm = sub.add_parser("lm")
     lm.add_argument("tokens", nargs="?", default="1,2,3,4,2,5")
     lm.add_argument("--seed", type=int, default=123)

@@ -588,11 +588,13 @@ class InferenceEngine:
 
         The same tokens as ``generate`` on the whole prompts, but for roundings (another kernel reads the prefix)."""
         params = params or SamplingParams()
-        prefix = prefix.reshape(-1)
+        if prefix.dim() > 1 and prefix.shape[-1] != prefix.numel():
+            raise ValueError("one prefix")
+        prefix = prefix.reshape(-1).to(self.dev)
         P = prefix.numel()
         if isinstance(suffixes, int):
             suffixes = [prefix[:0]] * suffixes
-        suffixes = [torch.as_tensor(s).reshape(-1).to(prefix.dtype) for s in suffixes]
+        suffixes = [torch.as_tensor(s).reshape(-1).to(self.dev, prefix.dtype) for s in suffixes]
         B, lens = len(suffixes), [s.numel() for s in suffixes]
         if B < 1 or P < 1 or max_new < 1:
             raise ValueError("a prefix, one sequence and one new token at least")
@@ -616,9 +618,9 @@ class InferenceEngine:
             D.argmax_rows(logits, out_tokens=self.tokens[:B])
         else:
             sampler = DeviceSampler(params, B, self.cfg.vocab_size, [seed + b for b in range(B)], dev, history_len=longest + max_new)
-            sampler.history[:, :P] = prefix.to(dev)
+            sampler.history[:, :P] = prefix
             for b, s in enumerate(suffixes):
-                sampler.history[b, P:P + lens[b]] = s.to(dev)
+                sampler.history[b, P:P + lens[b]] = s
             sampler.n_hist.copy_(torch.tensor([P + n for n in lens], dtype=torch.int32))
             sampler.sample(logits, out_tokens=self.tokens[:B])
             sampler.push(self.tokens[:B])
@@ -637,14 +639,15 @@ class InferenceEngine:
         out.copy_(logits)
         if sum(lens) == 0:
             return out
-        tok = torch.cat(suffixes).to(dev)
+        tok = torch.cat(suffixes)
         n = torch.tensor(lens, dtype=torch.int32)
         ends = torch.cat([n[:1] * 0, n.cumsum(0, dtype=torch.int32)])
         seq_of = torch.arange(B, dtype=torch.int32).repeat_interleave(n.long())
         pos = torch.arange(tok.numel(), dtype=torch.int32) - ends[:-1].repeat_interleave(n.long()) + P
         seq_of, pos, cu, total = seq_of.to(dev), pos.to(torch.int32).to(dev), ends.to(dev), (n + P).to(dev)
         x = self._prompt_layers(tok, seq_of, pos, lambda li, qkv: paged.shared_prefix_attention(
-            qkv, cache.pools[li], cache.block_table[:B], cache.page, total, *shared, self.H, self.Hkv, self.cfg.head_dim, cu_q=cu, max_len=P + max(lens)))
+            qkv, cache.pools[li], cache.block_table[:B], cache.page, total, *shared, self.H, self.Hkv, self.cfg.head_dim, cu_q=cu,
+            max_len=P + max(lens)))
         some = [b for b in range(B) if lens[b]]
         last = x[torch.tensor([int(ends[b + 1]) - 1 for b in some], device=dev)].contiguous()
         got = torch.empty((len(some), out.shape[1]), dtype=out.dtype, device=dev)

@@ -84,16 +84,17 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     zero (an empty slot) gives zeros, and so does a row in front of position 0. ``max_len`` bounds the lengths (default: the table);
     it is for the size of the launch only. Rows of ``out`` that belong to no sequence stay as they are; without ``out`` they are zero.
 
-    Positions that no row of a sequence sees may hold anything, infinities and NaN included. Among the new tokens of one call that
-    holds for keys; a value that is not finite reaches the rows in front of it too, as in ``attention_fwd``."""
+    Positions that no row of the call sees may hold anything, infinities and NaN included. Among the new tokens of a sequence, and in the
+    prefix for a sequence that ends inside it, what a row does not see may be any key; a value that is not finite reaches the row all the
+    same, as in ``attention_fwd``. ``out`` may not lie in what the call reads."""
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
     (n, width), (B,), (rows, max_blocks) = q.shape, seq_len.shape, block_table.shape
     n_blocks, *layout = pool.shape
     prefix = int(prefix_len) // page * page if prefix_table is not None else 0
     if H <= 0 or H % Hkv or page <= 0 or prefix_len < 0 or not scale > 0.0:
         raise ValueError("shared_prefix_attention: heads must divide by kv heads, page and scale be positive")
-    if layout != [2, Hkv, page, dh] or rows != B:
-        raise ValueError("shared_prefix_attention: pool must be [n_blocks, 2, Hkv, page, dh] and block_table [B, pages]")
+    if layout != [2, Hkv, page, dh] or rows != B or (B and not max_blocks):
+        raise ValueError("shared_prefix_attention: pool must be [n_blocks, 2, Hkv, page, dh] and block_table [B, pages >= 1]")
     if width < H * dh or (n != B if cu_q is None else cu_q.shape != (B + 1,)):
         raise ValueError("shared_prefix_attention: q must be [rows, >= H*dh], one row a sequence or rows counted by cu_q [B + 1]")
     if prefix and prefix_table.numel() * page < prefix:
@@ -128,19 +129,22 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
             and (cu_q is None or cu_q.device == device) and (out is None or out.device == device)):
         raise ValueError("shared_prefix_attention: all tensors must be on the device of q")
     (ldq, unit), q_at = q.stride(), q.data_ptr()
-    if unit != 1 or ldq % 8 or q_at % 16 or not pool.is_contiguous():
-        raise ValueError("shared_prefix_attention: pool must be contiguous, rows of q contiguous and 16-byte aligned")
+    if n == 1:
+        ldq = H * dh                                # a dimension of one has any stride
+    if unit != 1 or ldq % 8 or ldq < H * dh or q_at % 16 or not pool.is_contiguous():
+        raise ValueError("shared_prefix_attention: pool must be contiguous, rows of q contiguous, apart and 16-byte aligned")
     if out is None:
         fill, ldo = 1, H * dh
         out = _lib.empty((n, ldo), BF, device)
     else:
         fill, (ldo, unit) = 0, out.stride()
-        if unit != 1 or ldo % 8 or out.data_ptr() % 16:
-            raise ValueError("shared_prefix_attention: rows of out must be contiguous and 16-byte aligned")
+        ldo = H * dh if n == 1 else ldo
+        if unit != 1 or ldo % 8 or ldo < H * dh or out.data_ptr() % 16:
+            raise ValueError("shared_prefix_attention: rows of out must be contiguous, apart and 16-byte aligned")
     if n == 0:
         return out
-    if B == 0 or max_blocks == 0:
-        return out.zero_() if fill or cu_q is None else out
+    if B == 0:
+        return out.zero_() if fill else out
     per_tile = TILE_ROWS // (H // Hkv)
     if cu_q is not None and n >= B * per_tile:
         # The sequences fill tiles by themselves: a part in common saves no tile, and its sums have to be joined. us, own / in common, 16
@@ -191,6 +195,12 @@ def _page_ids(ids, n_blocks, what):
     return ids
 
 
+def _overlap(pools, to) -> bool:
+    """Whether a pool of ``to`` shares memory with one of ``pools`` that does not begin where it does."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for p in (pools, to) for t in p.pools)
+    return any(a[0] != b[0] and b[0] < a[1] for a, b in zip(spans, spans[1:]))
+
+
 def copy_pages(pools, src, dst, rows=None, out=None):
     """Copies page ``src[i]`` to page ``dst[i]`` in every layer's pool, or to ``dst[i]`` of the pools ``out``; with ``rows`` only the first
     ``rows`` positions of each page. ``pools`` (and ``out``) is a ``PagePools`` or a list of pools.
@@ -215,6 +225,8 @@ def copy_pages(pools, src, dst, rows=None, out=None):
         if len(src) != len(dst) or len(set(dst)) != len(dst):
             raise ValueError("copy_pages: as many destinations as sources, each once")
         same = {t.data_ptr() for t in pools.pools} & {t.data_ptr() for t in to.pools}
+        if to is not pools and _overlap(pools, to):
+            raise ValueError("copy_pages: pools reach into one another")
         if same and set(src) & set(dst):
             raise ValueError("copy_pages: a page is both source and destination")
     n = len(src)

@@ -55,7 +55,7 @@ def test_samples_of_one_prompt_share_its_pages(model):
 def test_refusals(model):
     eng = InferenceEngine(model, max_batch=2, max_seq=16, page=8)
     p = torch.arange(1, 6)
-    for args in ((p, 3, 4), (p, 2, 12), (p, [torch.ones(9, dtype=torch.int64)], 3), (p, 0, 4), (p[:0], 2, 4), (p, 2, 0), (p, [], 2)):
+    for args in ((p, 3, 4), (p, 2, 12), (p, [torch.ones(9, dtype=torch.int64)], 3), (p, 0, 4), (p[:0], 2, 4), (p, 2, 0), (p, [], 2), (torch.ones(2, 2, dtype=torch.int64), 2, 3)):
         with pytest.raises(ValueError):
             eng.generate_shared(*args)
 
@@ -70,6 +70,7 @@ def test_command_prints_a_line_for_each_sample(model, tmp_path, capsys):
     assert cli.run(args + ["--samples", "3"]) == 0
     assert capsys.readouterr().out.splitlines() == one * 3           # greedy
     assert cli.run(args + ["--samples", "0"]) != 0
+    assert cli.run(["sciagent", "ask"] + args[1:] + ["--samples", "2"]) != 0
 
 
 @pytest.mark.parametrize("H, Hkv, dh, B, P, want", [(32, 8, 128, 2, 255, False), (32, 8, 128, 2, 256, True), (32, 8, 128, 1, 4096, False),

@@ -60,7 +60,7 @@ def test_empty_sequences_and_rows_of_no_sequence():
     dict(H=3), dict(page=16), dict(dh=32), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(prefix_len=-1),
     dict(prefix_len=30), dict(seq_len=torch.ones(2, dtype=torch.int32)), dict(cu_q=torch.zeros(3, dtype=torch.int32)),
     dict(q=torch.zeros(4, 256, dtype=BF)), dict(q=torch.zeros(3, 255, dtype=BF)), dict(out=torch.zeros(3, 255, dtype=BF)),
-    dict(block_table=torch.zeros(3, dtype=torch.int32))])
+    dict(block_table=torch.zeros(3, dtype=torch.int32)), dict(block_table=torch.zeros(3, 0, dtype=torch.int32))])
 def test_refusals(change):
     with pytest.raises(ValueError):
         paged.shared_prefix_attention(**{**batch(), **change})
@@ -102,6 +102,17 @@ def test_copy_pages_statement():
 def test_copy_pages_refusals(args, kw):
     with pytest.raises(ValueError):
         paged.copy_pages([torch.zeros(6, 2, 1, 4, 8) for _ in range(2)], *args, **kw)
+
+
+def test_copies_between_pools_that_reach_into_one_another_are_refused():
+    memory = torch.zeros(9, 2, 1, 4, 8)
+    pools, other = [memory[:5]], [memory[3:]]
+    with pytest.raises(ValueError):
+        paged.copy_pages(pools, [0], [1], out=other)
+    memory[0] = 1.0
+    paged.copy_pages(pools, [0], [3], out=[memory[5:]])             # beside it
+    paged.copy_pages(pools, [0], [2], out=[memory[:4]])             # the same pool, by fewer pages
+    assert [bool(p.any()) for p in memory] == [True, False, True, False, False, False, False, False, True]
 
 
 def test_page_pools_refusals():

@@ -125,6 +125,37 @@ def test_what_no_row_sees_may_hold_anything(new, junk):
     check(a)
 
 
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("G", [1, 2, 3, 5, 7, 8, 9])
+def test_rows_of_a_sequence_of_one_token(G, dh):
+    """Few rows for each kv head, shared by few or many tokens, blocks that end everywhere, maxima that grow and lie beyond 2^24."""
+    for B, prefix, tails in ((1, 0, [1]), (1, 256, [129]), (2, 128, [127, 128]), (3, 0, [500, 1, 256]), (8, 640, [1, 2, 15, 16, 17, 129, 255, 640]),
+                             (9, 8, [300 + 60 * b for b in range(9)])):
+        a = batch(B, 2 * G, 2, dh, 8, prefix, tails, seed=B)
+        check(a, max_len=prefix + max(tails))
+        a["pool"][:, 0] *= torch.linspace(0.2, 3.0, a["pool"].shape[0], device=DEV)[:, None, None, None].to(BF)
+        check(a)
+        a["pool"][:, 0] *= 2.0 ** 14
+        a["q"] *= 2.0 ** 14
+        check_order(a)
+
+
+def check_order(a):
+    """Scores so far apart that a row's answer is the value of its largest one."""
+    out = paged.shared_prefix_attention(**a).to(F64)
+    o, _ = statement(a)
+    H, Hkv, dh, page = a["H"], a["Hkv"], a["dh"], a["page"]
+    for b, length in enumerate(a["seq_len"].tolist()):
+        pos = torch.arange(length, device=DEV)
+        k = a["pool"][a["block_table"][b].long()[pos // page], 0, :, pos % page].to(F64)
+        q = a["q"][b, :H * dh].to(F64).reshape(Hkv, H // Hkv, dh)
+        two = torch.einsum("kgd,jkd->kgj", q, k).topk(min(2, length), -1).values
+        off = 2 * dh * 2.0 ** -23 * torch.einsum("kgd,jkd->kgj", q.abs(), k.abs()).amax(-1)       # of a score in 32 bits
+        clear = two[..., 0] - two[..., -1] > 2 * off if length > 1 else torch.ones_like(off, dtype=torch.bool)
+        rows = (out[b] - o[b]).reshape(Hkv, H // Hkv, dh)[clear]
+        assert bool((rows.abs() <= 2.0 ** -8 * o[b].reshape(Hkv, H // Hkv, dh)[clear].abs() + 1e-6).all())
+
+
 def test_scores_far_apart():
     a = batch(6, 16, 4, 64, 64, 320, [1, 9, 50, 30, 77, 128])
     a["q"] *= 20                                   # scores of a few hundred: one position has all the weight
@@ -182,6 +213,17 @@ def test_strides_of_rows_and_of_the_answer():
     assert torch.equal(out, want) and not answer[:, :512].any() and not answer[:, 1536:].any()
 
 
+def test_rows_that_overlap_are_refused_and_one_row_has_any_stride():
+    a = batch(3, 8, 2, 64, 16, 100, [5, 9, 1])
+    with pytest.raises(ValueError):
+        paged.shared_prefix_attention(**{**a, "q": a["q"][:1].expand(3, -1)})
+    with pytest.raises(ValueError):
+        paged.shared_prefix_attention(**a, out=torch.zeros((1, 512), dtype=BF, device=DEV).expand(3, -1))
+    one = batch(1, 8, 2, 64, 16, 100, [5])
+    one["q"] = one["q"].as_strided((1, 512), (0, 1))
+    check(one, out=torch.zeros(600, dtype=BF, device=DEV).as_strided((1, 512), (7, 1)))
+
+
 def test_long_prefix_many_sequences():
     check(batch(64, 8, 2, 64, 64, 6000, [1 + 7 * b % 190 for b in range(64)]))
     check(batch(130, 4, 1, 128, 64, 700, [1 + 11 * b % 300 for b in range(130)]))
@@ -230,6 +272,34 @@ def test_same_bits_again_on_another_stream_and_in_a_graph():
     torch.cuda.synchronize()
     want = check(a, max_len=1300)
     assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want)
+
+
+def test_two_calls_at_once():
+    """On two streams, and graphs captured on one stream and replayed on two: each has a workspace of its own."""
+    ab = [batch(16, 32, 8, 128, 64, 4000, [1 + 17 * b for b in range(16)], seed=1),
+          batch(7, 32, 8, 128, 64, 2000, [40 + b for b in range(7)], [1 + 5 * b for b in range(7)], seed=2)]
+    want = [check(a) for a in ab]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in ab], [], [torch.zeros_like(w) for w in want]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, a, o in zip(streams, ab, outs):
+            with torch.cuda.stream(s):
+                paged.shared_prefix_attention(**a, out=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    for a, o in zip(ab, outs):
+        o.zero_()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            paged.shared_prefix_attention(**a, out=o)
+        graphs.append(g)
+    for _ in range(10):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    _lib.check_status(torch.device(DEV, 0))
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
 def test_what_a_bound_of_the_lengths_is_for():
