@@ -21,7 +21,8 @@
 //
 // What bounds it, B200, 32 / 8 heads of 128, a call in a graph:
 //   many rows and a long prefix: the exponentials and what lies between them. A block of two tiles takes some 3700 cycles, 2048 of them
-//     exponentials on each SM sub-partition and 1024 products: 520 tokens of 16 sequences behind 8192 positions 83 us, 0.54 of the matrix rate.
+//     exponentials on each SM sub-partition and 1024 products: 520 tokens of 16 sequences behind 8192 positions 83 us, 0.54 of the matrix
+//     rate.
 //   one token a sequence: 64 sequences behind 16384 positions, up to 512 of their own, 60.5 us where memory would take 21: the sequences'
 //     own items, 512 of two or three blocks, are as many starts and ends, and what they fetch of their own code; shared blocks are read
 //     once, but a CTA's ten of them bring a new maximum, thus a pass over O, almost every time.
@@ -762,38 +763,38 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       // few rows: a product of 16 columns at least, of which eight are the others again
       ok = wait(&q_full[half], (n_pieces >> 1) & 1, p.status, ST_TIMEOUT_MISC);
       auto steps_of = [&](auto kind) {
-      constexpr bool few = decltype(kind)::value;
+        constexpr bool few = decltype(kind)::value;
 #pragma unroll 1
-      for (int i = 0; i < n && ok; ++i, ++steps) {
-        const int L = steps & 1;
-        const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;      // the block's first step, its last
-        const int before = C::SB == 1 ? steps : steps >> 1;                        // scores that were in this accumulator
-        const uint32_t q_lo = same((at_q + (two ? L : half) * q_bytes) >> 4), k_lo = same((at_k + ks * C::KV_BYTES) >> 4);
-        const uint32_t to = same(tmem + (C::SB == 1 ? 0 : L * BN));
-        if (uses) ok = wait(&k_full[ks], kph, p.status, ST_TIMEOUT_FULL);
-        if (before > 0) ok = ok && wait(&s_free[C::SB == 1 ? 0 : L], (before - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
-        if (!ok) break;
-        tc_fence_after();
-        if (leader) {
-          if (few) {
+        for (int i = 0; i < n && ok; ++i, ++steps) {
+          const int L = steps & 1;
+          const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;      // the block's first step, its last
+          const int before = C::SB == 1 ? steps : steps >> 1;                        // scores that were in this accumulator
+          const uint32_t q_lo = same((at_q + (two ? L : half) * q_bytes) >> 4), k_lo = same((at_k + ks * C::KV_BYTES) >> 4);
+          const uint32_t to = same(tmem + (C::SB == 1 ? 0 : L * BN));
+          if (uses) ok = wait(&k_full[ks], kph, p.status, ST_TIMEOUT_FULL);
+          if (before > 0) ok = ok && wait(&s_free[C::SB == 1 ? 0 : L], (before - 1) & 1, p.status, ST_TIMEOUT_TMEM_EMPTY);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            if (few) {
 #pragma unroll
-            for (int k = 0; k < DH / 16; ++k)
-              umma_bf16_ss(to, desc | (k_lo + (k >> 2) * k_step + (k & 3) * 2), desc_same | (q_lo + (k >> 2) * q_step + (k & 3) * 2),
-                           make_idesc_bf16(BM, 2 * FEW, false, false), k > 0 ? 1u : 0u);
-          } else {
+              for (int k = 0; k < DH / 16; ++k)
+                umma_bf16_ss(to, desc | (k_lo + (k >> 2) * k_step + (k & 3) * 2), desc_same | (q_lo + (k >> 2) * q_step + (k & 3) * 2),
+                             make_idesc_bf16(BM, 2 * FEW, false, false), k > 0 ? 1u : 0u);
+            } else {
 #pragma unroll
-            for (int k = 0; k < DH / 16; ++k)
-              umma_bf16_ss(to, desc | (q_lo + (k >> 2) * q_step + (k & 3) * 2), desc | (k_lo + (k >> 2) * k_step + (k & 3) * 2),
-                           make_idesc_bf16(BM, BN, false, false), k > 0 ? 1u : 0u);
+              for (int k = 0; k < DH / 16; ++k)
+                umma_bf16_ss(to, desc | (q_lo + (k >> 2) * q_step + (k & 3) * 2), desc | (k_lo + (k >> 2) * k_step + (k & 3) * 2),
+                             make_idesc_bf16(BM, BN, false, false), k > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[L]);
+            if (frees && !few) umma_commit(&k_empty[ks]);
+            if (i == n - 1) umma_commit(&q_empty[half]);
           }
-          umma_commit(&s_full[L]);
-          if (frees && !few) umma_commit(&k_empty[ks]);
-          if (i == n - 1) umma_commit(&q_empty[half]);
+          if (frees) {
+            if (++ks == KS) { ks = 0; kph ^= 1; }
+          }
         }
-        if (frees) {
-          if (++ks == KS) { ks = 0; kph ^= 1; }
-        }
-      }
       };
       if (!PLANNED && same(few_rows<PLANNED>(p, x) ? 1 : 0)) steps_of(std::bool_constant<!PLANNED>{});
       else steps_of(std::false_type{});
@@ -816,56 +817,56 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       const bool two = same(x.n_tok > p.TT ? 1 : 0);
       const int n = same((x.j1 - x.j0) << (two ? 1 : 0)), first_live = same(x.kend - x.kbase - x.j0 * BN);
       auto steps_of = [&](auto kind) {
-      constexpr bool few = decltype(kind)::value;
+        constexpr bool few = decltype(kind)::value;
 #pragma unroll 1
-      for (int i = 0; i < n && ok; ++i, ++steps) {
-        const int L = steps & 1, turn = steps >> 1;            // every second step is this lane's
-        const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;
-        const int live = min(BN, first_live - (two ? i >> 1 : i) * BN);            // positions that count
-        const uint32_t v_lo = same((a_v + vs * C::KV_BYTES) >> 4), p_lo = same((a_k + ks * C::KV_BYTES) >> 4), o = same(tmem + C::COL_O + L * DH),
-                       w = same(tmem + C::COL_P + L * (BN / 2)), begins = same(i < 2 ? 1 : 0);
-        if (uses) {
-          ok = wait(&v_full[vs], vph, p.status, ST_TIMEOUT_FULL);
-          if (ok && (live & 15)) {
-            // A product takes 16 positions. The weights of those behind the end are zero, but what lies there may be no number, and zero
-            // times it would be none either.
-            uint8_t* v = sV + vs * C::KV_BYTES;
+        for (int i = 0; i < n && ok; ++i, ++steps) {
+          const int L = steps & 1, turn = steps >> 1;            // every second step is this lane's
+          const bool uses = !two || (i & 1) == 0, frees = !two || (i & 1) == 1;
+          const int live = min(BN, first_live - (two ? i >> 1 : i) * BN);            // positions that count
+          const uint32_t v_lo = same((a_v + vs * C::KV_BYTES) >> 4), p_lo = same((a_k + ks * C::KV_BYTES) >> 4), o = same(tmem + C::COL_O + L * DH),
+                         w = same(tmem + C::COL_P + L * (BN / 2)), begins = same(i < 2 ? 1 : 0);
+          if (uses) {
+            ok = wait(&v_full[vs], vph, p.status, ST_TIMEOUT_FULL);
+            if (ok && (live & 15)) {
+              // A product takes 16 positions. The weights of those behind the end are zero, but what lies there may be no number, and zero
+              // times it would be none either.
+              uint8_t* v = sV + vs * C::KV_BYTES;
 #pragma unroll 1
-            for (int c = lane; c < (16 - (live & 15)) * (DH / 8); c += 32) {
-              const int row = live + c / (DH / 8), e = c % (DH / 8);       // rows are whole, so their swizzle does not matter
-              *reinterpret_cast<uint4*>(v + (e >> 3) * (BN * 128) + row * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+              for (int c = lane; c < (16 - (live & 15)) * (DH / 8); c += 32) {
+                const int row = live + c / (DH / 8), e = c % (DH / 8);       // rows are whole, so their swizzle does not matter
+                *reinterpret_cast<uint4*>(v + (e >> 3) * (BN * 128) + row * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
             }
-            fence_proxy_async_smem();
-            __syncwarp();
           }
-        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          ok = ok && wait(&p_full[2 * L + h], turn & 1, p.status, ST_TIMEOUT_MISC);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && wait(&p_full[2 * L + h], turn & 1, p.status, ST_TIMEOUT_MISC);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int k2 = 0; k2 < HALF / 16; ++k2) {
-              const int k = h * (HALF / 16) + k2;
-              if (k * 16 < live) {
-                if (few) umma_bf16_ss(o, desc_few | (v_lo + k * 128), desc_p | (p_lo + k * FEW * 2), idesc_few, (!begins || k > 0) ? 1u : 0u);
-                else umma_bf16_ts(o, w + k * 8, desc | (v_lo + k * 128), idesc, (!begins || k > 0) ? 1u : 0u);
+              for (int k2 = 0; k2 < HALF / 16; ++k2) {
+                const int k = h * (HALF / 16) + k2;
+                if (k * 16 < live) {
+                  if (few) umma_bf16_ss(o, desc_few | (v_lo + k * 128), desc_p | (p_lo + k * FEW * 2), idesc_few, (!begins || k > 0) ? 1u : 0u);
+                  else umma_bf16_ts(o, w + k * 8, desc | (v_lo + k * 128), idesc, (!begins || k > 0) ? 1u : 0u);
+                }
               }
             }
           }
+          if (!ok) break;
+          if (leader) {
+            umma_commit(&pv_done[L]);
+            if (frees) umma_commit(&v_empty[vs]);
+            if (few) umma_commit(&k_empty[ks]);
+          }
+          if (frees) {
+            if (++ks == KS) ks = 0;
+            if (++vs == VS) { vs = 0; vph ^= 1; }
+          }
         }
-        if (!ok) break;
-        if (leader) {
-          umma_commit(&pv_done[L]);
-          if (frees) umma_commit(&v_empty[vs]);
-          if (few) umma_commit(&k_empty[ks]);
-        }
-        if (frees) {
-          if (++ks == KS) ks = 0;
-          if (++vs == VS) { vs = 0; vph ^= 1; }
-        }
-      }
       };
       if (!PLANNED && same(few_rows<PLANNED>(p, x) ? 1 : 0)) steps_of(std::bool_constant<!PLANNED>{});
       else steps_of(std::false_type{});
@@ -1136,10 +1137,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         // Weights of two columns, as bf16. Scale and difference are one fused step, whose exponent is off from the rounded reference by up
         // to half a step of it: nothing, unless scores are beyond 2^24. Those are scaled beforehand, rounded as the reference was.
         float factor = sl2;
-        auto scaled_first = [&](uint32_t* u, auto count) {
+        auto scaled_first = [&](uint32_t* u) {
           if (__any_sync(0xffffffffu, valid && fabsf(m_ref) > 16777216.f && m_ref != LOWEST)) {
 #pragma unroll
-            for (int c = 0; c < decltype(count)::value; c += 2) mul2(u[c], u[c + 1], sl2, sl2);
+            for (int c = 0; c < BN; c += 2) mul2(u[c], u[c + 1], sl2, sl2);
             factor = 1.f;
           }
         };
@@ -1173,7 +1174,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         m_blk = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         const float alpha = turn();
-        scaled_first(v, std::integral_constant<int, BN>{});
+        scaled_first(v);
         const int live = x.kend - (x.kbase + (x.j0 + i) * BN);      // positions that any row sees
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

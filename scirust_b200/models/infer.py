@@ -577,6 +577,8 @@ class InferenceEngine:
         512 8.9 / 8.9, 16 x 512 14.0 / 12.2; 8 / 1 heads: 2 x 256 13.4 / 11.0, 4 x 8192 13.6 / 14.4, 64 x 8192 48.0 / 24.7. Heads of 64, one
         or three query heads a kv head: 16 / 16 2 x 2048 11.2 / 11.4, 4 x 1024 10.3 / 11.0, 8 x 1024 13.9 / 11.6, 4 x 2048 14.5 / 11.5, 64 x
         512 29.5 / 30.5, 64 x 1024 51.8 / 35.2; 12 / 4 4 x 1024 9.2 / 10.3, 8 x 1024 11.5 / 10.3, 32 x 512 11.0 / 12.2."""
+        if self.cache.page % 8:                        # which the kernel does not take
+            return False
         if self.cfg.head_dim == 128:
             return B > 1 and P >= (256 if self.H >= 4 * self.Hkv else 512)
         return P >= 1024 and (B - 1) * P >= 4096
@@ -602,6 +604,8 @@ class InferenceEngine:
         if B > self.max_batch or longest + max_new > self.max_seq:
             raise ValueError("request exceeds the engine's max_batch / max_seq")
         cache, dev = self.cache, self.dev
+        if longest > P and dev.type == "cuda" and cache.page % 8:
+            raise ValueError("suffixes need a cache with pages of a multiple of 8")
         for b in range(self.max_batch):                # pages that another generation has left
             if cache.owned[b]:
                 cache.release(b)

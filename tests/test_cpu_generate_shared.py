@@ -79,6 +79,8 @@ def test_command_prints_a_line_for_each_sample(model, tmp_path, capsys):
 def test_rule_of_which_attention_runs(H, Hkv, dh, B, P, want):
     eng = InferenceEngine(GQADecoder(SciAgentConfig(16, dh * H, 0, H, Hkv, 16, 64, 10000.0)), max_batch=1, max_seq=8, page=8)
     assert eng._shares(B, P) is want
+    eng.cache.page = 12
+    assert not eng._shares(B, P)
 
 
 def test_rule_keeps_the_answers(model):

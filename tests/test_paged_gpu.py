@@ -430,3 +430,15 @@ def test_generation_behind_a_shared_prefix(monkeypatch, P, lens):
         whole = graph.prefill(torch.cat([prefix, suffixes[b]])[None])[0].float()
         assert (seen[0][b] - whole).norm() <= 0.034 * whole.norm()
         graph.cache.release(0)
+
+
+def test_generation_with_pages_that_the_kernel_does_not_take():
+    from scirust_b200.models.infer import InferenceEngine
+    from scirust_b200.models.sciagent import GQADecoder, SciAgentConfig
+    model = GQADecoder(SciAgentConfig(64, 128, 1, 2, 1, 128, 2048, 10000.0), device=DEV, seed=5, init_std=0.08)
+    eng = InferenceEngine(model, max_batch=8, max_seq=1600, page=12)
+    prefix = torch.arange(1500) % 63 + 1
+    out = eng.generate_shared(prefix, 8, 4)
+    assert torch.equal(out, out[:1].expand(8, -1))
+    with pytest.raises(ValueError):
+        eng.generate_shared(prefix, [prefix[:2]], 4)
