@@ -125,8 +125,10 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
             and block_table.is_contiguous() and seq_len.is_contiguous() and (not prefix or prefix_table.is_contiguous())
             and (cu_q is None or cu_q.is_contiguous())):
         raise ValueError("shared_prefix_attention: tables, lengths and offsets must be contiguous and int32")
-    if not (block_table.device == seq_len.device == pool.device == device and (not prefix or prefix_table.device == device)
-            and (cu_q is None or cu_q.device == device) and (out is None or out.device == device)):
+    index = q.get_device()
+    if not (block_table.get_device() == seq_len.get_device() == pool.get_device() == index
+            and (not prefix or prefix_table.get_device() == index) and (cu_q is None or cu_q.get_device() == index)
+            and (out is None or out.get_device() == index)):
         raise ValueError("shared_prefix_attention: all tensors must be on the device of q")
     (ldq, unit), q_at = q.stride(), q.data_ptr()
     if n == 1:
@@ -135,7 +137,7 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
         raise ValueError("shared_prefix_attention: pool must be contiguous, rows of q contiguous, apart and 16-byte aligned")
     if out is None:
         fill, ldo = 1, H * dh
-        out = _lib.empty((n, ldo), BF, device)
+        out = _lib.empty((n, ldo), BF, device) if _lib.DEBUG_POISON else q.new_empty((n, ldo))       # two thirds of torch.empty's time
     else:
         fill, (ldo, unit) = 0, out.stride()
         ldo = H * dh if n == 1 else ldo
@@ -155,7 +157,7 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     pairs = B if cu_q is None else B + n // per_tile
     units = Hkv * (-(-n // per_tile) * -(-prefix // BLOCK) + pairs * max(0, -(-(L - prefix) // BLOCK)))
     stream = _lib.stream()
-    ws, ws_bytes = _workspace(_workspace_bytes(device.index, n, B, H, Hkv, dh, cu_q is not None, prefix), device, stream)
+    ws, ws_bytes = _workspace(_workspace_bytes(index, n, B, H, Hkv, dh, cu_q is not None, prefix), device, stream)
     _lib.call("sb_shared_prefix_attention", q_at, ldq, pool.data_ptr(), n_blocks, block_table.data_ptr(), max_blocks, page,
               seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
               B, n, H, Hkv, dh, units, scale, ws.data_ptr(), ws_bytes, out.data_ptr(), ldo, fill,
