@@ -21,7 +21,7 @@
 //
 // What bounds it, B200, 32 / 8 heads of 128, a call in a graph:
 //   many rows and a long prefix: the exponentials and what lies between them. A block of two tiles takes some 3700 cycles, 2048 of them
-//     exponentials on each SM sub-partition and 1024 products: 520 tokens of 16 sequences behind 8192 positions 83 us, 0.54 of the matrix
+//     exponentials on each SM sub-partition, and 2048 products beside them: 520 tokens of 16 sequences behind 8192 positions 83 us, 0.54 of the matrix
 //     rate.
 //   one token a sequence: 64 sequences behind 16384 positions, up to 512 of their own, 60.5 us where memory would take 21: the sequences'
 //     own items, 512 of two or three blocks, are as many starts and ends, and what they fetch of their own code; shared blocks are read
