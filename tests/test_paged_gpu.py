@@ -318,6 +318,17 @@ def test_many_short_pieces_a_cta(B, tail):
     check(batch(B, 8, 2, 64, 16, 300, tails, new))
 
 
+@pytest.mark.parametrize("H,Hkv,dh,B,prefix,tails,max_len", [
+    (32, 32, 128, 8, 512, [257] * 8, None), (32, 32, 128, 8, 512, [2000] * 8, None), (32, 32, 64, 4, 512, [513, 600, 1, 900], None),
+    (16, 16, 64, 8, 1024, [2000, 1, 3000, 40, 2500, 7, 129, 1800], None), (32, 8, 128, 2, 256, [8192, 8192], None),
+    (32, 8, 128, 2, 256, [12000, 1], None), (32, 8, 128, 2, 128, [300, 300], 1), (32, 8, 128, 2, 128, [1, 1], 1), (16, 4, 64, 1, 128, [9000], 1)])
+def test_shared_items_of_few_rows_beside_long_own_parts(H, Hkv, dh, B, prefix, tails, max_len):
+    """A CTA has more shared items than it has slots for what is cut."""
+    a = batch(B, H, Hkv, dh, 64, prefix, tails)
+    check(a, max_len=prefix + max(tails) if max_len is None else max_len)
+    check(a)
+
+
 # ---------------------------------------------------------------------------------------------- copies of pages
 def _copied(pools, src, dst, rows, out=None):
     """Each pool as it should be, one copy at a time."""
