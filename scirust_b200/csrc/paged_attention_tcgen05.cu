@@ -1065,6 +1065,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           for (int w = 1; w < 4; ++w) y.y += s_ml[(L * 4 + w) * FEW + lane].y;
           reinterpret_cast<float2*>(base + n_rows * DH)[row + lane + few_tok * skip] = y;
         }
+        __syncwarp();                      // an aligned instruction behind stores of some lanes
         tmem_ld_wait();
         float* to = base + static_cast<size_t>(row) * DH + r;
         if (r < DH) {
