@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import threading
 
 import torch
 
@@ -49,19 +50,30 @@ def shared_prefix_attention_ref(q, pool, block_table, page, seq_len, prefix_tabl
     return out
 
 
+class _Workspace:
+    """The workspace of a stream's calls. The launches of a call hand their parts on in it, so ``lock`` is held around them: of two threads
+    on one stream one would launch between the other's, whose second launch then read what is not its own."""
+    __slots__ = ("lock", "buffer", "bytes")
+
+    def __init__(self):
+        self.lock, self.buffer, self.bytes = threading.Lock(), None, 0
+
+    def at_least(self, n, device):
+        if self.bytes < n:                  # the buffer before goes back to the stream whose launches use it
+            self.buffer, self.bytes = _lib.empty(n, torch.uint8, device), n
+        return self.buffer.data_ptr()
+
+
 _ws: dict = {}
 
 
-def _workspace(n, device, stream):
-    """``(buffer, its bytes)`` of at least ``n`` bytes. Calls on one stream follow one another and share one; what is being captured into
-    a graph gets its own from the graph's pool, since graphs captured on one stream may be replayed at once on two."""
+def _workspace(device, stream):
+    """Calls on one stream follow one another and share one; what is being captured into a graph gets its own from the graph's pool, since
+    graphs captured on one stream may be replayed at once on two."""
     if _lib.DEBUG_POISON or torch._C._cuda_isCurrentStreamCapturing():
-        return _lib.empty(n, torch.uint8, device), n
+        return _Workspace()
     key = (device.index, stream)
-    w = _ws.get(key)
-    if w is None or w[1] < n:
-        w = _ws[key] = (torch.empty(n, dtype=torch.uint8, device=device), n)
-    return w
+    return _ws.get(key) or _ws.setdefault(key, _Workspace())
 
 
 @functools.lru_cache(maxsize=4096)       # a function of the device and the sizes
@@ -157,11 +169,12 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     pairs = B if cu_q is None else B + n // per_tile
     units = Hkv * (-(-n // per_tile) * -(-prefix // BLOCK) + pairs * max(0, -(-(L - prefix) // BLOCK)))
     stream = _lib.stream()
-    ws, ws_bytes = _workspace(_workspace_bytes(index, n, B, H, Hkv, dh, cu_q is not None, prefix), device, stream)
-    _lib.call("sb_shared_prefix_attention", q_at, ldq, pool.data_ptr(), n_blocks, block_table.data_ptr(), max_blocks, page,
-              seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
-              B, n, H, Hkv, dh, units, scale, ws.data_ptr(), ws_bytes, out.data_ptr(), ldo, fill,
-              _lib.status_word(device).data_ptr(), stream)
+    need, ws = _workspace_bytes(index, n, B, H, Hkv, dh, cu_q is not None, prefix), _workspace(device, stream)
+    with ws.lock:
+        at = ws.at_least(need, device)
+        _lib.call("sb_shared_prefix_attention", q_at, ldq, pool.data_ptr(), n_blocks, block_table.data_ptr(), max_blocks, page,
+                  seq_len.data_ptr(), prefix_table.data_ptr() if prefix else None, prefix, cu_q.data_ptr() if cu_q is not None else None,
+                  B, n, H, Hkv, dh, units, scale, at, ws.bytes, out.data_ptr(), ldo, fill, _lib.status_word(device).data_ptr(), stream)
     _g.launch_count += 2 if cu_q is None else 3
     return out
 
