@@ -557,6 +557,7 @@ class InferenceEngine:
                     continue
                 graphs[-1].replay()
                 out[:, i] = self.tokens[:B]
+            paged.drop_workspace(self.dev, s.cuda_stream)       # of the eager step; the graphs have their own
         else:
             for i in range(1, max_new):
                 if crosses(i):

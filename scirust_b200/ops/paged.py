@@ -76,6 +76,12 @@ def _workspace(device, stream):
     return _ws.get(key) or _ws.setdefault(key, _Workspace())
 
 
+def drop_workspace(device, stream):
+    """Gives back what calls on ``stream`` (a handle) work in, some 40 MB, where no more of them are to come. Launches under way keep it: it
+    goes to that stream's next allocations."""
+    _ws.pop((device.index, stream), None)
+
+
 @functools.lru_cache(maxsize=4096)       # a function of the device and the sizes
 def _workspace_bytes(device, NT, B, H, Hkv, dh, ragged, prefix):
     fn = _lib.cuda().sb_shared_prefix_attention_bytes

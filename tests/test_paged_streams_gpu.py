@@ -127,3 +127,17 @@ def test_threads_on_one_stream():
 
     in_threads(lambda: run(0), lambda: run(3), lambda: run(5))
     assert len(paged._ws) == 1
+
+
+def test_a_generation_leaves_no_workspace_with_its_stream():
+    from scirust_b200.models.infer import InferenceEngine
+    from scirust_b200.models.sciagent import GQADecoder, SciAgentConfig
+    eng = InferenceEngine(GQADecoder(SciAgentConfig(64, 512, 1, 4, 1, 128, 512, 10000.0), device=DEV, seed=5, init_std=0.08), max_batch=3, max_seq=400, page=16)
+    prefix = torch.arange(300) % 63 + 1
+    outs = []
+    assert eng._shares(3, 300)                       # the steps go through the workspace
+    for _ in range(3):
+        outs.append(eng.generate_shared(prefix, 3, 6))
+        outs.append(eng.generate_shared(prefix, [prefix[:5], prefix[:9]], 6)[:1])
+        assert set(paged._ws) == {(0, torch.cuda.current_stream().cuda_stream)}       # the suffixes' pass
+    assert all(torch.equal(o, w) for o, w in zip(outs[2:], outs))
