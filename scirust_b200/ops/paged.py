@@ -185,6 +185,11 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     return out
 
 
+def _overlap(spans) -> bool:
+    """Whether one of the address ranges, sorted, reaches into another that does not begin where it does."""
+    return any(a[0] != b[0] and b[0] < a[1] for a, b in zip(spans, spans[1:]))
+
+
 class PagePools:
     """The pools of a cache's layers, checked once: tensors of one shape ``[n_blocks, ..., page, width]``, type and device, each contiguous.
     It holds on to the tensors; one that is replaced in the cache needs a new handle."""
@@ -202,6 +207,10 @@ class PagePools:
         self.heads = math.prod(self.shape[1:-2])                      # of K and of V
         self.row_bytes = self.shape[-1] * p.element_size()            # of a position of a head
         self.page_bytes = self.heads * self.page * self.row_bytes
+        size = self.n_blocks * self.page_bytes
+        self.spans = sorted((t.data_ptr(), t.data_ptr() + size) for t in self.pools)
+        if _overlap(self.spans):
+            raise ValueError("PagePools: pools reach into one another")
         self._table = (C.c_void_p * len(self.pools))(*[t.data_ptr() for t in self.pools])
         self.table = C.addressof(self._table)
 
@@ -216,23 +225,20 @@ def _page_ids(ids, n_blocks, what):
     return ids
 
 
-def _overlap(pools, to) -> bool:
-    """Whether a pool of ``to`` shares memory with one of ``pools`` that does not begin where it does."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for p in (pools, to) for t in p.pools)
-    return any(a[0] != b[0] and b[0] < a[1] for a, b in zip(spans, spans[1:]))
-
-
 def copy_pages(pools, src, dst, rows=None, out=None):
     """Copies page ``src[i]`` to page ``dst[i]`` in every layer's pool, or to ``dst[i]`` of the pools ``out``; with ``rows`` only the first
     ``rows`` positions of each page. ``pools`` (and ``out``) is a ``PagePools`` or a list of pools.
 
-    A source may be copied many times; a destination must occur once and, in the same pools, be no source. Ids from the host (a list, a CPU
+    A source may be copied many times; a destination must occur once and, in the same pools, be no source. Pools may not reach into one another,
+    nor may one occur twice in ``out``. Ids from the host (a list, a CPU
     tensor) are checked for that. Ids on the device (int32) are taken as they are, so that a captured call can be replayed with others;
     ids outside the pools are skipped there, as padding may be."""
     pools = pools if isinstance(pools, PagePools) else PagePools(pools)
     to = pools if out is None else out if isinstance(out, PagePools) else PagePools(out)
     if to is not pools and (len(to) != len(pools) or to.shape[1:] != pools.shape[1:] or to.dtype != pools.dtype or to.device != pools.device):
         raise ValueError("copy_pages: out must be as many pools of the same pages, type and device")
+    if to is not pools and (_overlap(sorted(pools.spans + to.spans)) or any(a[0] == b[0] < a[1] for a, b in zip(to.spans, to.spans[1:]))):
+        raise ValueError("copy_pages: pools reach into one another, or out has one twice")
     if rows is not None and not 0 <= rows <= pools.page:
         raise ValueError("copy_pages: rows must be between 0 and the positions of a page")
     device = pools.device
@@ -245,9 +251,7 @@ def copy_pages(pools, src, dst, rows=None, out=None):
         src, dst = _page_ids(src, pools.n_blocks, "source"), _page_ids(dst, to.n_blocks, "destination")
         if len(src) != len(dst) or len(set(dst)) != len(dst):
             raise ValueError("copy_pages: as many destinations as sources, each once")
-        same = {t.data_ptr() for t in pools.pools} & {t.data_ptr() for t in to.pools}
-        if to is not pools and _overlap(pools, to):
-            raise ValueError("copy_pages: pools reach into one another")
+        same = {at for at, _ in pools.spans} & {at for at, _ in to.spans}
         if same and set(src) & set(dst):
             raise ValueError("copy_pages: a page is both source and destination")
     n = len(src)

@@ -115,6 +115,23 @@ def test_copies_between_pools_that_reach_into_one_another_are_refused():
     assert [bool(p.any()) for p in memory] == [True, False, True, False, False, False, False, False, True]
 
 
+def test_copies_into_one_pool_from_two_are_refused():
+    pools, into = [torch.full((6, 2, 1, 4, 8), float(i)) for i in range(2)], torch.zeros(6, 2, 1, 4, 8)
+    with pytest.raises(ValueError):
+        paged.copy_pages(pools, [0], [1], out=[into, into])
+    assert not into.any()
+    paged.copy_pages([pools[1], pools[1]], [0], [1], out=[into, pools[0]])         # from one pool to two
+    assert bool(into[1].eq(1).all()) and bool(pools[0][1].eq(1).all()) and not pools[0][0].any()
+    paged.copy_pages(pools, [], [], out=[into[:0], into[:0]])                      # of nothing
+
+
+def test_pools_of_a_cache_that_reach_into_one_another_are_refused():
+    memory = torch.zeros(9, 2, 1, 4, 8)
+    with pytest.raises(ValueError):
+        paged.PagePools([memory[:5], memory[3:8]])
+    assert len(paged.PagePools([memory[4:8], memory[:4]])) == 2
+
+
 def test_page_pools_refusals():
     for bad in ([], [torch.zeros(3, 4)], [torch.zeros(3, 2, 4, 8), torch.zeros(3, 2, 4, 7)], [torch.zeros(3, 2, 8, 4).transpose(2, 3)],
                 [torch.zeros(3, 2, 4, 8), torch.zeros(3, 2, 4, 8, dtype=BF)]):

@@ -393,6 +393,17 @@ def test_copies_in_a_graph_take_new_ids():
     assert all(torch.equal(a, b) for a, b in zip(pools, want))
 
 
+def test_copies_between_pools_that_reach_into_one_another_are_refused_for_ids_on_the_device_too():
+    memory = torch.zeros((9, 2, 1, 4, 8), dtype=BF, device=DEV)
+    ids = [torch.tensor([i], dtype=torch.int32, device=DEV) for i in (0, 1)]
+    for pools, out in (([memory[:5]], [memory[3:]]), ([memory[:3], memory[3:6]], [memory[6:]] * 2)):
+        with pytest.raises(ValueError):
+            paged.copy_pages(pools, *ids, out=out)
+    memory[0] = 1.0
+    paged.copy_pages([memory[:5]], *ids, out=[memory[5:]])
+    assert [bool(p.any()) for p in memory] == [True] + [False] * 5 + [True] + [False] * 2
+
+
 def test_many_copies():
     """More copies than a grid has rows."""
     pool = torch.arange(140000, device=DEV, dtype=torch.int32).reshape(-1, 1, 1, 1).repeat(1, 1, 2, 4)
