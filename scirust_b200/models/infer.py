@@ -607,7 +607,7 @@ class InferenceEngine:
         cache, dev = self.cache, self.dev
         if longest > P and dev.type == "cuda" and cache.page % 8:
             raise ValueError("suffixes need a cache with pages of a multiple of 8")
-        for b in range(self.max_batch):                # pages that another generation has left
+        for b in range(B):                             # pages that another generation has left
             if cache.owned[b]:
                 cache.release(b)
         logits = self.prefill(prefix[None]).clone()

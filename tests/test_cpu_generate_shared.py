@@ -52,6 +52,16 @@ def test_samples_of_one_prompt_share_its_pages(model):
     assert torch.equal(matrix[0], matrix[1])
 
 
+def test_sequences_that_do_not_take_part_keep_their_pages(model):
+    eng = InferenceEngine(model, max_batch=4, max_seq=32, page=8)
+    eng.prefill(torch.arange(1, 41).view(4, 10))
+    kept, held = eng.cache.owned[3][:], eng.cache.pools[0][eng.cache.owned[3]].clone()
+    out = eng.generate_shared(torch.arange(1, 20), 3, 5)
+    assert out.tolist() == [alone(model, list(range(1, 20)), 5)] * 3
+    assert eng.cache.owned[3] == kept and eng.cache.block_table[3, :2].tolist() == kept
+    assert torch.equal(eng.cache.pools[0][kept], held)
+
+
 def test_refusals(model):
     eng = InferenceEngine(model, max_batch=2, max_seq=16, page=8)
     p = torch.arange(1, 6)
