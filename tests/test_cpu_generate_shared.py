@@ -1,4 +1,9 @@
 """Generation of sequences with a common prefix against generation of each prompt by itself (CPU statements)."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -97,3 +102,13 @@ def test_rule_keeps_the_answers(model):
     eng = InferenceEngine(model, max_batch=3, max_seq=32, page=8)
     out = eng.generate_shared(torch.arange(1, 12), 3, 4)               # too little for the other kernel
     assert eng._shared is None and out.tolist() == [alone(model, list(range(1, 12)), 4)] * 3
+
+
+@pytest.mark.parametrize("world, kv", [(2, 4), (4, 1)])
+def test_tensor_parallel_ranks(world, kv):
+    """Sharded heads, and kv heads that ranks hold in common."""
+    root = Path(__file__).resolve().parents[1]
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={world}", "--master-addr", "127.0.0.1",
+           "--master-port", str(29780 + world), str(root / "tests" / "mp" / "mp_tp_generate_shared.py")]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=600, env=dict(os.environ, PYTHONPATH=str(root), SB_TP_KV=str(kv)))
+    assert r.returncode == 0 and "TP_GENERATE_SHARED_OK" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
