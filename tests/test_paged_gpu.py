@@ -173,6 +173,31 @@ def test_weights_of_the_lowest_value_mask():
     assert bool(out.any())
 
 
+@pytest.mark.parametrize("H,Hkv,dh", [(4, 4, 64), (16, 2, 128), (18, 2, 64)])
+@pytest.mark.parametrize("new", [None, [5, 60, 1]])
+def test_equal_scores_near_the_lowest_value_weigh_all_positions_alike(H, Hkv, dh, new):
+    """Scores of -2^127, in units of log 2 -3.387e38, where the type ends at -3.403e38: the answer is the mean of the values that a row sees.
+    Weights are 1 and their sum a whole number, both exact; a value's sum is off by a step of 2^-23 of the magnitudes for each addition,
+    the division by two steps, and the answer is rounded to bf16."""
+    a = batch(3, H, Hkv, dh, 64, 320, [5, 270, 1], new)
+    a["q"].zero_()
+    a["q"][:, :H * dh:dh] = -2.0 ** 63
+    a["pool"][:, 0] = 0
+    a["pool"][:, 0, ..., 0] = 2.0 ** 64
+    scale = 3.387e38 / 2.0 ** 127 / 1.4426950408889634
+    out = paged.shared_prefix_attention(**a, scale=scale).to(F64).view(-1, Hkv, H // Hkv, dh)
+    _lib.check_status(out.device)
+    t = 0
+    for b, length in enumerate(a["seq_len"].tolist()):
+        for limit in range(length - (1 if new is None else new[b]) + 1, length + 1):
+            pos = torch.arange(limit, device=DEV)
+            v = a["pool"][a["block_table"][b].long()[pos // 64], 1, :, pos % 64].to(F64)              # [limit, Hkv, dh]
+            mean, size = v.mean(0), v.abs().mean(0)
+            bound = 2.0 ** -8 * mean.abs() + (limit + 2) * 2.0 ** -23 * size
+            assert bool(((out[t] - mean[:, None]).abs() <= bound[:, None]).all())
+            t += 1
+
+
 def test_rows_of_no_sequence():
     a = batch(3, 16, 4, 64, 64, 256, [9, 5, 20], [9, 5, 20])
     a["q"] = torch.cat([a["q"], a["q"][:7]])
