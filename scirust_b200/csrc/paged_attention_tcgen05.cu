@@ -268,7 +268,8 @@ struct Piece {
 // CUT: not all of its item; FIRST: begins where the CTA's share does; SHORT: some row may end inside
 constexpr int PIECE_SHARED = 1, PIECE_CUT = 2, PIECE_FIRST = 4, PIECE_SHORT = 8, SEQUENCE = 4;
 
-// Slots of the rows of items that were not cut: of shared items, then of own ones.
+// Slots of the rows of items that were not cut: of shared items (of few rows by kv head, token and query head, of others as the batch has
+// them), then of own ones.
 __host__ __device__ __forceinline__ int own_slot(const Params& p) { return p.prefix == 0 ? 0 : 1; }
 __host__ __device__ __forceinline__ int whole_slots(const Params& p) { return own_slot(p) + 1; }
 
@@ -1051,29 +1052,28 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         }
         if ((lane & 3) == 0) ml[own] = make_float2(m_own, sum);
         meet();
-        // A piece of an item that is cut has a slot of its CTA, its rows behind one another. A CTA has two slots, for its first and its last
-        // piece; what lies between is not cut, and of that a CTA may have any number, so its rows go where those of the batch lie.
+        // Rows of a piece lie behind one another. A CTA has two slots, for its first and its last piece, the only ones that can be cut. What
+        // lies between has a place of its own, since a CTA may have any number of these: a shared item, of all tokens, among those of the kv
+        // heads, an own one, of one token, where its rows are in the batch.
         const bool cut = x.flags & PIECE_CUT;
-        const unsigned row = cut ? (2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1)) * (2 * BM)
-                                 : ((x.flags & PIECE_SHARED ? 0 : own_slot(p)) * p.NT + x.t0) * p.H + x.h * p.G;
-        const unsigned skip = cut ? 0 : p.H - p.G;         // rows between a token's last and the next one's first
+        const unsigned row = cut                      ? (2 * blockIdx.x + (x.flags & PIECE_FIRST ? 0 : 1)) * (2 * BM)
+                             : x.flags & PIECE_SHARED ? x.h * p.NT * p.G
+                                                      : (own_slot(p) * p.NT + x.t0) * p.H + x.h * p.G;
         const size_t n_rows = cut ? static_cast<size_t>(2) * gridDim.x * (2 * BM) : static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
         float* base = cut ? p.cut : p.whole;
         if (quarter == 0 && lane < rows) {
           float2 y = s_ml[L * 4 * FEW + lane];
 #pragma unroll
           for (int w = 1; w < 4; ++w) y.y += s_ml[(L * 4 + w) * FEW + lane].y;
-          reinterpret_cast<float2*>(base + n_rows * DH)[row + lane + few_tok * skip] = y;
+          reinterpret_cast<float2*>(base + n_rows * DH)[row + lane] = y;
         }
         __syncwarp();                      // an aligned instruction behind stores of some lanes
         tmem_ld_wait();
         float* to = base + static_cast<size_t>(row) * DH + r;
         if (r < DH) {
 #pragma unroll
-          for (int e = 0, g = p.G; e < FEW; ++e, to += DH) {
-            if (e == g) { to += static_cast<size_t>(skip) * DH; g += p.G; }
-            if (e < rows) *to = __uint_as_float(o[e]);
-          }
+          for (int e = 0; e < FEW; ++e)
+            if (e < rows) to[e * DH] = __uint_as_float(o[e]);
         }
         __syncwarp();
         tc_fence_before();
@@ -1343,8 +1343,9 @@ __global__ void __launch_bounds__(128 * WAYS) join_kernel(const __grid_constant_
     x.y = clampi(x.y, 0, 2 * ctas - 1);
     const int count = i && kend <= p.prefix ? 0 : clampi(x.x, 0, ctas - (x.y >> 1)), tok = t - (i ? t0 : first);
     const bool cut = count > 1;
-    const size_t at = cut ? static_cast<size_t>(x.y) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
-                          : (static_cast<size_t>(i ? own_slot(p) : 0) * p.NT + t) * p.H + h * p.G;
+    const size_t at = cut               ? static_cast<size_t>(x.y) * (2 * BM) + (tok < p.TT ? tok * p.G : BM + (tok - p.TT) * p.G)
+                      : !i && p.few & 2 ? (static_cast<size_t>(h) * p.NT + t) * p.G
+                                        : (static_cast<size_t>(i ? own_slot(p) : 0) * p.NT + t) * p.H + h * p.G;
     const size_t rows = cut ? static_cast<size_t>(4) * ctas * BM : static_cast<size_t>(whole_slots(p)) * p.NT * p.H;
     const float* base = cut ? p.cut : p.whole;
     n[i] = count;
