@@ -89,6 +89,19 @@ def _workspace_bytes(device, NT, B, H, Hkv, dh, ragged, prefix):
     return fn(NT, B, H, Hkv, dh, int(ragged), prefix)
 
 
+def _in_common(n, B, per_tile, prefix, longest=0) -> bool:
+    """Whether the rows of ``B`` sequences, ``n`` tokens in all, ``per_tile`` of which fill a tile, go over the prefix together. That takes as
+    many tiles as all rows fill, apart each sequence's last one is partly empty; but parts in common have to be joined. us, apart / in common,
+    32 / 8 heads, 32 tokens a tile. 16 sequences behind 4096: of 16 tokens 49.9 / 44.0, 24 51.8 / 50.7, 32 53.4 / 57.1, 48 86.4 / 77.2, 64
+    89.9 / 97.3. Behind 8192 and 16384: 33 136 / 93, 261 / 169, 1 to 64 112 / 91, 214 / 163, 64 149 / 156, 265 / 294, 100 267 / 236, 501 / 458, 1
+    to 300 286 / 282, 501 / 510; one of 1000 beside 31 of one token 486 / 298. Behind 512: 33 30.4 / 31.8, 64 35.3 / 41.4, 100 50.5 / 63.1; behind
+    2048 33 53.6 / 46.6, 64 59.5 / 66.4, 100 96.2 / 101.5; one of 1000 beside 31 behind 1024 73.5 / 73.8. The host knows the tokens' sum and,
+    where the caller says how long sequences are, the ``longest`` run: behind a long prefix they go apart only where all fill their tiles or
+    the last tiles are few beside the others, which also bounds the workspace (1 KB a row and head)."""
+    full = n == B * longest and longest % per_tile == 0
+    return n < B * per_tile or (prefix >= 4096 and n < 4 * B * per_tile and not full)
+
+
 def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, prefix_len, H, Hkv, dh, scale=None, cu_q=None,
                             max_len=None, out=None):
     """GQA attention of a batch over its paged KV, where all sequences begin with the same ``prefix_len`` positions: the pages that
@@ -100,7 +113,8 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     ``block_table`` [B, *] holds all pages of each sequence and ``prefix_table`` those of the prefix, of which whole pages are shared:
     the positions behind the last whole page come from each sequence's own table. ``seq_len`` [B] counts the new tokens; a length of
     zero (an empty slot) gives zeros, and so does a row in front of position 0. ``max_len`` bounds the lengths (default: the table);
-    it is for the size of the launch only. Rows of ``out`` that belong to no sequence stay as they are; without ``out`` they are zero.
+    it is for the size of the launch and how the work is split only. Rows of ``out`` that belong to no sequence stay as they are; without
+    ``out`` they are zero.
 
     Positions that no row of the call sees may hold anything, infinities and NaN included. Among the new tokens of a sequence, and in the
     prefix for a sequence that ends inside it, what a row does not see may be any key; a value that is not finite reaches the row all the
@@ -166,10 +180,7 @@ def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, p
     if B == 0:
         return out.zero_() if fill else out
     per_tile = TILE_ROWS // (H // Hkv)
-    if cu_q is not None and n >= B * per_tile:
-        # The sequences fill tiles by themselves: a part in common saves no tile, and its sums have to be joined. us, own / in common, 16
-        # sequences of 16, 24, 32, 64, 128 tokens behind 4096 positions (32 / 8 heads): 49.9 / 44.0, 51.8 / 50.7, 53.7 / 57.2, 89.4 / 97.5,
-        # 161 / 180; of 48, whose second tile is half empty, 86.4 / 77.5; 4 sequences of 32 26.2 / 28.2
+    if cu_q is not None and not _in_common(n, B, per_tile, prefix, 0 if max_len is None else max_len - prefix_len):
         prefix = 0
     L = max_blocks * page if max_len is None else min(int(max_len), max_blocks * page)
     pairs = B if cu_q is None else B + n // per_tile
@@ -229,8 +240,8 @@ def copy_pages(pools, src, dst, rows=None, out=None):
     """Copies page ``src[i]`` to page ``dst[i]`` in every layer's pool, or to ``dst[i]`` of the pools ``out``; with ``rows`` only the first
     ``rows`` positions of each page. ``pools`` (and ``out``) is a ``PagePools`` or a list of pools.
 
-    A source may be copied many times; a destination must occur once and, in the same pools, be no source. Pools may not reach into one another,
-    nor may one occur twice in ``out``. Ids from the host (a list, a CPU
+    A source may be copied many times; a destination must occur once and, in the same pools, be no source. Pools may not reach into one
+    another, nor may one occur twice in ``out``. Ids from the host (a list, a CPU
     tensor) are checked for that. Ids on the device (int32) are taken as they are, so that a captured call can be replayed with others;
     ids outside the pools are skipped there, as padding may be."""
     pools = pools if isinstance(pools, PagePools) else PagePools(pools)

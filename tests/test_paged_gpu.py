@@ -343,6 +343,15 @@ def test_many_short_pieces_a_cta(B, tail):
     check(batch(B, 8, 2, 64, 16, 300, tails, new))
 
 
+@pytest.mark.parametrize("new", [[300] + [1] * 7, [33] * 6, [64] * 4, [0, 130, 1, 77]])
+def test_runs_of_uneven_length_behind_a_long_prefix(new):
+    """As many tokens as fill the sequences' tiles, and rows of all of them in a tile of the prefix."""
+    a = batch(len(new), 8, 2, 128, 64, 4100, [n + 3 for n in new], new)
+    assert sum(new) >= len(new) * 32 and paged._in_common(sum(new), len(new), 32, 4096, max(new) + 3)
+    check(a, max_len=4100 + max(new) + 3)
+    check(a, max_len=4100 + max(new))               # where all have 64, apart
+
+
 @pytest.mark.parametrize("H,Hkv,dh,B,prefix,tails,max_len", [
     (32, 32, 128, 8, 512, [257] * 8, None), (32, 32, 128, 8, 512, [2000] * 8, None), (32, 32, 64, 4, 512, [513, 600, 1, 900], None),
     (16, 16, 64, 8, 1024, [2000, 1, 3000, 40, 2500, 7, 129, 1800], None), (32, 8, 128, 2, 256, [8192, 8192], None),
