@@ -1529,8 +1529,8 @@ extern "C" size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv
 
 // q: bf16 [NT, ldq], query heads first, positions already rotated in. pool: n_blocks pages [2, Hkv, page, dh], page a multiple of 8.
 // cu_q: [B + 1] rows of the sequences, or null: one row each (NT == B). seq_len: positions of each sequence, its rows' among them.
-// prefix_table: pages of the first `prefix` positions, which all sequences share (prefix a multiple of page; 0: none). max_units bounds
-// the blocks of 64 positions of all (sequence, kv head, tile of rows), which caps the grid.
+// prefix_table: pages of the first `prefix` positions, which all sequences share (prefix a multiple of page; 0: none). max_units, about
+// the blocks of 128 positions of all items, caps the grid; lengths beyond what it was counted for are answered all the same.
 extern "C" int sb_shared_prefix_attention(const void* q, long long ldq, const void* pool, int n_blocks, const int* block_table,
                                           int max_blocks, int page, const int* seq_len, const int* prefix_table, int prefix,
                                           const int* cu_q, int B, int NT, int H, int Hkv, int dh, long long max_units, float scale,

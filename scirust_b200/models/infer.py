@@ -577,7 +577,13 @@ class InferenceEngine:
         12.3, 64 x 256 22.8 / 18.3, 16 x 8192 82.1 / 19.7, 64 x 8192 305 / 40.6; 16 / 8 heads: 2 x 256 8.1 / 8.7, 16 x 256 11.2 / 12.0, 2 x
         512 8.9 / 8.9, 16 x 512 14.0 / 12.2; 8 / 1 heads: 2 x 256 13.4 / 11.0, 4 x 8192 13.6 / 14.4, 64 x 8192 48.0 / 24.7. Heads of 64, one
         or three query heads a kv head: 16 / 16 2 x 2048 11.2 / 11.4, 4 x 1024 10.3 / 11.0, 8 x 1024 13.9 / 11.6, 4 x 2048 14.5 / 11.5, 64 x
-        512 29.5 / 30.5, 64 x 1024 51.8 / 35.2; 12 / 4 4 x 1024 9.2 / 10.3, 8 x 1024 11.5 / 10.3, 32 x 512 11.0 / 12.2."""
+        512 29.5 / 30.5, 64 x 1024 51.8 / 35.2; 12 / 4 4 x 1024 9.2 / 10.3, 8 x 1024 11.5 / 10.3, 32 x 512 11.0 / 12.2.
+
+        Far behind a short prefix both read about the same, and a generation that grows to there keeps what it began with. Prefix + own
+        positions, 32 / 8 heads of 128: 2 x 256 + 2048 11.2 / 12.7, 2 x 1024 + 8192 17.8 / 18.2, 4 x 256 + 8192 28.5 / 31.5, 16 x 256 + 2048
+        31.8 / 31.2, 16 x 1024 + 8192 92.7 / 101.9, 64 x 1024 + 8192 345 / 320, 4 x 4096 + 8192 36.2 / 38.2, 16 x 4096 + 8192 120 / 92; 4 / 1
+        heads 4 x 1024 + 8192 12.0 / 15.4, 64 x 1024 + 8192 51.7 / 50.0; 16 / 4 heads of 64 4 x 1024 + 8192 21.8 / 19.3, 16 x 1024 + 8192 40.6 /
+        51.7, 64 x 1024 + 8192 135 / 98."""
         if self.cache.page % 8:                        # which the kernel does not take
             return False
         if self.cfg.head_dim == 128:

@@ -241,9 +241,8 @@ def copy_pages(pools, src, dst, rows=None, out=None):
     ``rows`` positions of each page. ``pools`` (and ``out``) is a ``PagePools`` or a list of pools.
 
     A source may be copied many times; a destination must occur once and, in the same pools, be no source. Pools may not reach into one
-    another, nor may one occur twice in ``out``. Ids from the host (a list, a CPU
-    tensor) are checked for that. Ids on the device (int32) are taken as they are, so that a captured call can be replayed with others;
-    ids outside the pools are skipped there, as padding may be."""
+    another, nor may one occur twice in ``out``. Ids from the host (a list, a CPU tensor) are checked. Ids on the device (int32) are taken
+    as they are, so that a captured call can be replayed with others; ids outside the pools are skipped there, as padding may be."""
     pools = pools if isinstance(pools, PagePools) else PagePools(pools)
     to = pools if out is None else out if isinstance(out, PagePools) else PagePools(out)
     if to is not pools and (len(to) != len(pools) or to.shape[1:] != pools.shape[1:] or to.dtype != pools.dtype or to.device != pools.device):
