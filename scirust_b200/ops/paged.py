@@ -97,9 +97,10 @@ def _in_common(n, B, per_tile, prefix, longest=0) -> bool:
     to 300 286 / 282, 501 / 510; one of 1000 beside 31 of one token 486 / 298. Behind 512: 33 30.4 / 31.8, 64 35.3 / 41.4, 100 50.5 / 63.1; behind
     2048 33 53.6 / 46.6, 64 59.5 / 66.4, 100 96.2 / 101.5; one of 1000 beside 31 behind 1024 73.5 / 73.8. The host knows the tokens' sum and,
     where the caller says how long sequences are, the ``longest`` run: behind a long prefix they go apart only where all fill their tiles or
-    the last tiles are few beside the others, which also bounds the workspace (1 KB a row and head)."""
+    the last tiles are few beside the others. A part in common takes 1 KB of workspace a row and head, so batches of more than 8192 tokens do
+    not ask for it beyond where they did not fill tiles."""
     full = n == B * longest and longest % per_tile == 0
-    return n < B * per_tile or (prefix >= 4096 and n < 4 * B * per_tile and not full)
+    return n < B * per_tile or (prefix >= 4096 and n < min(4 * B * per_tile, 8193) and not full)
 
 
 def shared_prefix_attention(q, pool, block_table, page, seq_len, prefix_table, prefix_len, H, Hkv, dh, scale=None, cu_q=None,

@@ -84,7 +84,7 @@ def test_entry_point_refuses():
 @pytest.mark.parametrize("n, B, prefix, longest, want", [
     (511, 16, 512, 0, True), (512, 16, 512, 0, False), (512, 16, 4095, 0, False), (512, 16, 4096, 0, True), (1031, 32, 16384, 1000, True),
     (2047, 16, 8192, 0, True), (2048, 16, 8192, 0, False), (1, 1, 8, 1, True), (32, 1, 64, 32, False), (1024, 16, 8192, 64, False),
-    (1024, 16, 8192, 65, True), (768, 16, 8192, 48, True)])
+    (1024, 16, 8192, 65, True), (768, 16, 8192, 48, True), (8192, 128, 8192, 0, True), (8193, 128, 8192, 0, False), (8193, 300, 8192, 0, True)])
 def test_rule_of_which_rows_go_over_the_prefix_together(n, B, prefix, longest, want):
     assert paged._in_common(n, B, 32, prefix, longest) is want
 
