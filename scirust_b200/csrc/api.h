@@ -132,6 +132,13 @@ int sb_copy_pages(const void* const* src, void* const* dst, int layers, const in
 size_t sb_shared_prefix_attention_bytes(int NT, int B, int H, int Hkv, int dh, int ragged, int prefix);
 int sb_shared_prefix_attention(const void* q, long long ldq, const void* pool, int n_blocks, const int* block_table, int max_blocks, int page, const int* seq_len, const int* prefix_table, int prefix, const int* cu_q, int B, int NT, int H, int Hkv, int dh, long long max_units, float scale, void* workspace, size_t workspace_bytes, void* out, long long ldo, int fill, int* status, void* stream);
 
+// quantized_kv.cu
+int sb_quant_kv_append(void* qkv, long long ld, int n, int H, int Hkv, int dh, const float* cos_t, const float* sin_t, int n_pos, void* codes, int e4m3, float* scales, int n_blocks, int page, int block, const int* table, int max_blocks, const int* seq_len, const int* cu_q, int B, int chunk, void* stream_);
+int sb_quant_kv_read(const void* codes, int e4m3, const float* scales, int n_blocks, int Hkv, int page, int block, int dh, const int* pages, int n, void* out, void* stream_);
+
+// quantized_kv_attention.cu
+int sb_quant_kv_attention(const void* q, long long ldq, const void* codes, int e4m3, const float* scales, int n_blocks, int page, int block, const int* table, int max_blocks, const int* seq_len, int B, int H, int Hkv, int dh, float scale, void* out, long long ldo, void* stream_);
+
 // sampler.cu
 int sb_sample_rows(const float* logits, int ld, int rows, int V, float temperature, int top_k, float top_p, float rep_penalty, int rep_window, const int64_t* recent, int recent_ld, const int* n_recent, uint64_t* rng_state, int64_t* out_tokens, int64_t* generated, int gen_stride, int step, uint32_t* work, void* stream);
 

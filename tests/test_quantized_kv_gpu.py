@@ -1,0 +1,405 @@
+"""Operators on a paged KV cache in 8 bits on the GPU: what is written against the statement, to the bit, attention against 64 bits."""
+import math
+
+import pytest
+import torch
+
+from scirust_b200 import ops
+from scirust_b200.ops import _lib, quantized_kv as Q
+
+pytestmark = pytest.mark.gpu
+BF, F64 = torch.bfloat16, torch.float64
+DEV = "cuda"
+KINDS = ["int8", "e4m3"]
+CU = "cu_q"
+
+
+@pytest.fixture(autouse=True)
+def _poisoned(monkeypatch):
+    """Workspaces and answers begin as NaN and between fences, so that a part which is read and was not written shows."""
+    monkeypatch.setattr(_lib, "DEBUG_POISON", True)
+    yield
+    torch.cuda.synchronize()
+    _lib.check_canaries()
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def bits(t):
+    return t.contiguous().view({1: torch.int8, 2: torch.int16, 4: torch.int32}[t.element_size()])
+
+
+def random_pool(n, Hkv, page, dh, kind, block, seed=0):
+    """A pool as earlier writes leave it: codes of all magnitudes, scales that are powers of two."""
+    g = gen(seed)
+    x = torch.randn((n, 2, Hkv, page, dh), generator=g, device=DEV)
+    codes = (x * 40).round().clamp(-127, 127).to(torch.int8) if kind == "int8" else (x * 150).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.exp2(torch.randint(-8, 0, (n, 2, Hkv, page // block), generator=g, device=DEV).float())
+    return Q.QuantPool(codes, scales)
+
+
+def on_cpu(pool):
+    return Q.QuantPool(pool.codes.cpu(), pool.scales.cpu())
+
+
+def tables(pages, seed=0, spare=3):
+    """A table with as many pages a sequence as asked for, every page in one sequence; unused entries name no page."""
+    order = torch.randperm(sum(pages) + spare, generator=gen(seed), device=DEV).int()
+    table = torch.full((len(pages), max(max(pages), 1)), -1, dtype=torch.int32, device=DEV)
+    at = 0
+    for b, n in enumerate(pages):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return table, len(order)
+
+
+# ---------------------------------------------------------------------------------------------------------------- writing
+def write(kind, H, Hkv, dh, page, block, held, new, rope=True, cu=True, chunk=None, monkeypatch=None, seed=0, pad=8, first=0, scale=1.0):
+    """One write on the GPU and by the statement on the CPU: rotated rows, codes and scales have to be the same bits."""
+    if chunk is not None:
+        monkeypatch.setattr(Q, "_chunk", lambda n, B, block: chunk)
+    total = [h + n for h, n in zip(held, new)]
+    table, n_pages = tables([-(-t // page) for t in total], seed)
+    pool = random_pool(n_pages, Hkv, page, dh, kind, block, seed)
+    lens = torch.tensor(total, dtype=torch.int32, device=DEV)
+    n = first + sum(new) + (2 if cu else 0)                              # rows of no sequence in front and behind
+    g = gen(seed + 1)
+    x = torch.randn((n, (H + 2 * Hkv) * dh + pad), generator=g, device=DEV)
+    x = (x * torch.exp2(torch.randint(-3, 4, (n, 1), generator=g, device=DEV).float()) * scale).to(BF)
+    cu_q = (torch.tensor([0] + new).cumsum(0) + first).int().to(DEV) if cu else None
+    other, y = on_cpu(pool), x.cpu()
+    c = cu_q.cpu() if cu else None
+    if rope:
+        cos, sin = ops.rope_table(max(total) + 1, dh, 10000.0, DEV)
+        Q.rope_kv_append(x, H, Hkv, dh, cos, sin, pool, table, lens, cu_q=cu_q)
+        Q.rope_kv_append(y, H, Hkv, dh, cos.cpu(), sin.cpu(), other, table.cpu(), lens.cpu(), cu_q=c)
+    else:
+        Q.kv_append(x, H, Hkv, dh, pool, table, lens, cu_q=cu_q)
+        Q.kv_append(y, H, Hkv, dh, other, table.cpu(), lens.cpu(), cu_q=c)
+    assert torch.equal(bits(x.cpu()), bits(y))
+    assert torch.equal(bits(pool.scales.cpu()), bits(other.scales))
+    assert torch.equal(bits(pool.codes.cpu()), bits(other.codes))
+    return pool
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,Hkv,dh", [(16, 4, 64), (4, 1, 128), (3, 3, 64), (5, 5, 128), (0, 2, 128)])
+def test_single_tokens(kind, H, Hkv, dh):
+    held = [0, 1, 15, 16, 17, 63, 64, 100, 5]
+    write(kind, H, Hkv, dh, 64, 16, held, [1] * len(held), cu=False)
+    write(kind, H, Hkv, dh, 64, 16, held, [1] * len(held), cu=False, rope=False, scale=8.0)       # every block's scale grows
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page,block", [(8, 8), (16, 8), (32, 32), (64, 16), (64, 64), (128, 64), (192, 64)])
+@pytest.mark.parametrize("chunk", [1, 4, 16])
+def test_ragged_runs(kind, page, block, chunk, monkeypatch):
+    held, new = [0, 3, 0, 61, 130, 7, 64], [1, 200, 64, 67, 2, 0, 129]
+    write(kind, 4, 2, 128, page, block, held, new, chunk=chunk, monkeypatch=monkeypatch, first=3)
+    write(kind, 6, 2, 64, page, block, held, new, rope=False, chunk=chunk, monkeypatch=monkeypatch, scale=16.0)
+
+
+def test_many_sequences():
+    """More than one step of the search for a row's sequence: 33 times 32 of them, empty ones among them."""
+    g = torch.Generator().manual_seed(4)
+    new = torch.randint(0, 4, (1056,), generator=g).tolist()
+    held = torch.randint(0, 9, (1056,), generator=g).tolist()
+    write("int8", 2, 1, 64, 8, 8, held, new)
+
+
+def test_long_prompt():
+    write("e4m3", 4, 2, 128, 64, 16, [0, 5], [3000, 1111])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_writing_in_parts_agrees_where_blocks_are_whole(kind):
+    """A prompt in pieces that end with blocks gives the same pool as the whole of it."""
+    H, Hkv, dh, page, block = 4, 2, 64, 64, 16
+    table, n = tables([4])
+    x = torch.randn((200, (H + 2 * Hkv) * dh), generator=gen(0), device=DEV).to(BF)
+    one, two = random_pool(n, Hkv, page, dh, kind, block), random_pool(n, Hkv, page, dh, kind, block)
+    ends = lambda *e: torch.tensor(e, dtype=torch.int32, device=DEV)
+    Q.kv_append(x, H, Hkv, dh, one, table, ends(200), cu_q=ends(0, 200))
+    for a, b in ((0, 48), (48, 64), (64, 192), (192, 200)):
+        Q.kv_append(x[a:b], H, Hkv, dh, two, table, ends(b), cu_q=ends(0, b - a))
+    assert torch.equal(bits(one.codes), bits(two.codes)) and torch.equal(one.scales, two.scales)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_without_a_place_stay(kind):
+    """Rows in front of position 0, behind the table or the rotation's tables, of an empty slot, and ids outside the pool."""
+    H, Hkv, dh, page, block = 2, 1, 128, 16, 16
+    pool = random_pool(4, Hkv, page, dh, kind, block)
+    kept = Q.QuantPool(pool.codes.clone(), pool.scales.clone())
+    i = lambda *e: torch.tensor(e, dtype=torch.int32, device=DEV)
+    x = torch.randn((14, (H + 2 * Hkv) * dh), generator=gen(1), device=DEV).to(BF)
+    before = x.clone()
+    cos, sin = ops.rope_table(40, dh, 10000.0, DEV)
+    # 4 rows for 2 positions; a table of two pages and a length of 34; an empty slot; a page outside; one below; a length behind the rotation
+    table = torch.stack([i(0, 1), i(2, 3), i(1, 1), i(4, 4), i(-1, 0), i(3, 3)])
+    Q.rope_kv_append(x, H, Hkv, dh, cos, sin, pool, table, i(2, 34, 0, 2, 1, 2 ** 31 - 1), cu_q=i(0, 4, 8, 9, 11, 12, 14))
+    turned = (x != before).any(1)
+    # row 3 is position 1 and turns; position 0 does not; rows 4 and 5 are positions 30 and 31; row 10 position 1 of a sequence without a page
+    assert turned.nonzero().flatten().tolist() == [3, 4, 5, 10]
+    changed = (bits(pool.codes) != bits(kept.codes)).flatten(1).any(1)
+    assert changed.tolist() == [True, False, False, True]
+    assert torch.equal(pool.scales[[1, 2]], kept.scales[[1, 2]])
+    assert torch.equal(bits(pool.codes[0, :, :, 2:]), bits(kept.codes[0, :, :, 2:]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_not_finite(kind):
+    H, Hkv, dh, page, block = 1, 2, 64, 32, 16
+    table, n = tables([2])
+    pool = random_pool(n, Hkv, page, dh, kind, block)
+    x = torch.randn((40, (H + 2 * Hkv) * dh), generator=gen(1), device=DEV).to(BF)
+    x[3, H * dh + 5] = math.inf
+    x[20, -1] = math.nan
+    x[33, H * dh + dh] = 3.4e38 if kind == "e4m3" else -math.inf
+    i = lambda *e: torch.tensor(e, dtype=torch.int32, device=DEV)
+    Q.kv_append(x, H, Hkv, dh, pool, table, i(40), cu_q=i(0, 40))
+    bad = pool.scales[table[0].long()].isnan().nonzero().tolist()              # page, k or v, head, block
+    assert bad == [[0, 0, 0, 0], [0, 1, 1, 1], [1, 0, 1, 0]]
+    back = Q.read_pages(pool, table[0])
+    assert torch.equal(back.isnan().view(2, 2, Hkv, 2, block * dh).all(-1), pool.scales[table[0].long()].isnan())
+    # in a block that is not begun anew it stays, in one that is it goes
+    Q.kv_append(x[:1], H, Hkv, dh, pool, table, i(10))
+    assert bool(pool.scales[table[0, 0].long(), 0, 0, 0].isnan())
+    Q.kv_append(x[:1], H, Hkv, dh, pool, table, i(1))
+    assert not bool(pool.scales[table[0, 0].long(), 0, 0, 0].isnan())
+
+
+# ---------------------------------------------------------------------------------------------------------------- reading back
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page,block,dh,Hkv", [(8, 8, 64, 1), (64, 16, 128, 8), (128, 64, 64, 3), (48, 16, 128, 5)])
+def test_pages_read_back(kind, page, block, dh, Hkv):
+    pool = random_pool(9, Hkv, page, dh, kind, block)
+    ids = torch.tensor([3, 0, 8, 3, 9, -1, 7], dtype=torch.int32, device=DEV)                    # twice the same; two outside the pool
+    want = pool.codes.to(F64) * pool.scales.to(F64).repeat_interleave(block, -1)[..., None]
+    got = Q.read_pages(pool, ids)
+    assert torch.equal(got[[0, 1, 2, 3, 6]].to(F64), want[[3, 0, 8, 3, 7]])                      # exact: powers of two
+    assert not bool(got[4:6].any())
+    out = torch.full((2, 2, Hkv, page, dh), math.nan, dtype=BF, device=DEV)
+    assert Q.read_pages(pool, [5, 1], out=out) is out and torch.equal(out.to(F64), want[[5, 1]])
+    # scales that are no powers of two: one rounding to fp32 and one to bf16
+    odd = Q.QuantPool(pool.codes, pool.scales * 1.3)
+    want = pool.codes.to(F64) * odd.scales.to(F64).repeat_interleave(block, -1)[..., None]
+    assert bool(((Q.read_pages(odd, list(range(9))).to(F64) - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -23)).all())
+    assert Q.read_pages(pool, []).shape[0] == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------- attention
+def batch(kind, H, Hkv, dh, page, block, lens, seed=0, pad=8, dirty=True):
+    """A batch of sequences of these lengths. What lies behind a sequence's last position is the largest code, NaN where the type has one,
+    and NaN as scale of blocks that hold no position."""
+    table, n = tables([-(-t // page) for t in lens], seed)
+    pool = random_pool(n, Hkv, page, dh, kind, block, seed)
+    if dirty:
+        b8 = pool.codes.view(torch.int8)
+        used = torch.zeros(n, dtype=torch.bool, device=DEV)
+        for b, length in enumerate(lens):
+            if length % page:
+                at = int(table[b, length // page])
+                b8[at, :, :, length % page:] = 127
+                pool.scales[at, :, :, -(-(length % page) // block):] = math.nan
+            used[table[b, :-(-length // page)].long()] = True
+        b8[~used] = 127
+        pool.scales[~used] = math.nan
+    q = (torch.randn((len(lens), H * dh + pad), generator=gen(seed + 1), device=DEV) * 1.5).to(BF)
+    return dict(q=q, pool=pool, block_table=table, seq_len=torch.tensor(lens, dtype=torch.int32, device=DEV), H=H, Hkv=Hkv, dh=dh)
+
+
+def statement(a, scale=None):
+    """(o, bound): 64 bits, and how far an element may be off. A weight is rounded to fp16 (half a step of 2^-11, none finer than 2^-25 of
+    2^-9 of the largest) and weighs v, the answer is rounded once to bf16; a score is a sum of dh products in 32 bits, each addition off by
+    a step of 2^-23 of the sum of magnitudes, which the exponential passes on as a relative error of a weight and of their sum."""
+    H, Hkv, dh, pool = a["H"], a["Hkv"], a["dh"], a["pool"]
+    page, block = pool.codes.shape[3], pool.block
+    scale = dh ** -0.5 if scale is None else scale
+    B = a["q"].shape[0]
+    o, bound = torch.zeros((B, Hkv, H // Hkv, dh), dtype=F64, device=DEV), torch.zeros((B, Hkv, H // Hkv, dh), dtype=F64, device=DEV)
+    for b, length in enumerate(a["seq_len"].tolist()):
+        if length <= 0:
+            continue
+        pos = torch.arange(length, device=DEV)
+        at = a["block_table"][b].long()[pos // page]
+        kv = pool.codes.view(torch.int8)[at, :, :, pos % page].view(pool.codes.dtype).to(F64) * pool.scales[at, :, :, pos % page // block].to(F64)[..., None]
+        q = a["q"][b, :H * dh].to(F64).reshape(Hkv, H // Hkv, dh)
+        s = torch.einsum("kgd,jkd->kgj", q, kv[:, 0]) * scale
+        size = torch.einsum("kgd,jkd->kgj", q.abs(), kv[:, 0].abs()) * scale
+        p = torch.softmax(s, -1)
+        o[b] = torch.einsum("kgj,jkd->kgd", p, kv[:, 1])
+        mean = torch.einsum("kgj,jkd->kgd", p, kv[:, 1].abs())
+        slip = 2 * dh * 2.0 ** -23 * size.amax(-1, keepdim=True) + 2.0 ** -11 + 2.0 ** -20
+        tiny = 2.0 ** -33 * kv[:, 1].abs().amax(0)[:, None] * length * p.amax(-1, keepdim=True)
+        bound[b] = 2.0 ** -8 * o[b].abs() + slip * mean + tiny + 1e-30
+    return o.reshape(B, -1), bound.reshape(B, -1)
+
+
+def check(a, scale=None, **kw):
+    out = Q.decode_attention(**a, scale=scale, **kw)
+    _lib.check_status(out.device)
+    want, bound = statement(a, scale)
+    off = (out.to(F64) - want).abs() / bound.clamp_min(1e-30)
+    assert bool((off <= 1).all()), f"off by up to {float(off.nan_to_num(9e9).max()):.2f} of the bound"
+    return out
+
+
+HEADS = [(16, 4, 64), (32, 8, 128), (4, 1, 128), (12, 12, 64), (5, 5, 128), (20, 1, 128), (16, 1, 64), (9, 1, 128), (34, 2, 64), (14, 2, 128)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,Hkv,dh", HEADS)
+def test_attention_head_layouts(kind, H, Hkv, dh):
+    check(batch(kind, H, Hkv, dh, 64, 16, [1, 200, 0, 64, 65, 15, 130]))
+    check(batch(kind, H, Hkv, dh, 64, 32, [777]), scale=0.3, max_len=1000)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page,block", [(8, 8), (16, 8), (16, 16), (32, 8), (64, 8), (64, 64), (128, 64), (192, 32)])
+def test_attention_pages_and_blocks(kind, page, block):
+    lens = [1, 7, 8, 9, 63, 64, 65, 191, 193, 500, 0, 1025]
+    check(batch(kind, 8, 2, 128, page, block, lens))
+    check(batch(kind, 8, 2, 64, page, block, lens, seed=3))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_long_and_ragged(kind):
+    check(batch(kind, 32, 8, 128, 64, 16, [20000], dirty=False))
+    check(batch(kind, 16, 4, 64, 16, 16, [9000, 1, 4321, 2], dirty=False))
+    check(batch(kind, 8, 2, 128, 64, 16, [3000, 1, 0, 17, 64, 2900, 640, 1500, 3, 0], dirty=True))
+
+
+@pytest.mark.parametrize("B", [149, 300, 1025, 2100])
+def test_attention_many_sequences(B):
+    lens = [(7 * b * b + 3) % 200 for b in range(B)]
+    check(batch("int8", 4, 2, 64, 16, 16, lens))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_wide_scales(kind):
+    """Scales of keys and values that differ by many powers of two between blocks, rising, falling and mixed: a small value with a large
+    weight beside a large one with a small weight."""
+    a = batch(kind, 8, 2, 128, 64, 16, [700, 700, 700], dirty=False)
+    n = a["pool"].scales.shape[0]
+    e = torch.zeros_like(a["pool"].scales)
+    for b in range(3):
+        ids = a["block_table"][b].long()
+        ramp = torch.arange(len(ids) * 4, device=DEV).view(-1, 1, 1, 4).float()
+        e[ids] = {0: ramp, 1: -ramp, 2: torch.randint(-20, 20, (len(ids), 2, 2, 4), generator=gen(7), device=DEV).float()}[b]
+    a["pool"].scales.copy_(torch.exp2(-7 + e * torch.tensor([0.1, 1.0], device=DEV).view(1, 2, 1, 1)))
+    assert n >= 33
+    check(a)
+    # and scales that are no powers of two
+    a["pool"].scales.mul_(1.37)
+    check(a)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_large_scores(kind):
+    """Scores in the hundreds, one position far above the others, in the first, a middle and the last place."""
+    for at in (0, 333, 699):
+        a = batch(kind, 4, 2, 64, 64, 16, [700], dirty=False)
+        a["pool"].scales[:, 0] = 2.0 ** -2
+        a["pool"].scales[a["block_table"][0, at // 64].long(), 0, :, at % 64 // 16] = 2.0
+        check(a)
+
+
+def test_attention_queries_of_any_size():
+    """bf16 has eight bits of exponent, fp16 five: rows of queries near the ends of the range, and one of zeros."""
+    a = batch("int8", 4, 1, 128, 64, 16, [300] * 5, dirty=False)
+    for row, size in enumerate((2.0 ** 30, 2.0 ** -30, 0.0, 2.0 ** 100, 2.0 ** -120)):
+        a["q"][row] *= size
+    # at 2^30 and 2^100 one position takes all the weight; the statement's bound of a score would let any other have it
+    out = Q.decode_attention(**a)
+    want, bound = statement(a)
+    for row in (1, 2, 4):
+        assert bool(((out[row].to(F64) - want[row]).abs() <= bound[row]).all())
+    for row in (0, 3):
+        assert bool(((out[row].to(F64) - want[row]).abs() <= 2.0 ** -7 * want[row].abs()).all())
+
+
+def test_attention_not_finite():
+    """A NaN or an infinity in a query spoils that head alone; a NaN scale of a position that is read spoils the kv head's rows of that
+    sequence alone."""
+    a = batch("int8", 4, 2, 64, 16, 16, [100, 50, 60], dirty=False)
+    a["q"][0, 70] = math.nan
+    a["q"][1, 0] = math.inf
+    a["pool"].scales[a["block_table"][2, 1].long(), 1, 1, 0] = math.nan
+    out = Q.decode_attention(**a).view(3, 4, 64)
+    bad = torch.zeros((3, 4), dtype=torch.bool, device=DEV)
+    bad[0, 1] = bad[1, 0] = bad[2, 2] = bad[2, 3] = True
+    assert torch.equal(out.isnan().all(-1), bad) and torch.equal(out.isnan().any(-1), bad)
+
+
+def test_attention_page_ids_outside_the_pool():
+    """They count as zeros: a score of 0 and a value of 0."""
+    a = batch("int8", 4, 2, 64, 16, 16, [40, 40], dirty=False)
+    zeroed = Q.QuantPool(torch.cat([a["pool"].codes, torch.zeros_like(a["pool"].codes[:1])]), torch.cat([a["pool"].scales, torch.ones_like(a["pool"].scales[:1])]))
+    n = a["pool"].codes.shape[0]
+    for bad in (n, 2 ** 31 - 1, -1, -2 ** 31):
+        t = a["block_table"].clone()
+        t[1, 1] = bad
+        got = Q.decode_attention(**{**a, "block_table": t})
+        t[1, 1] = n
+        want = Q.decode_attention(**{**a, "block_table": t, "pool": zeroed})
+        assert torch.equal(got, want)
+
+
+def test_attention_output_rows_and_repeats():
+    a = batch("e4m3", 8, 2, 128, 64, 16, [300, 1, 0, 2000])
+    want = check(a)
+    wide = torch.full((4, 8 * 128 + 24), 7.0, dtype=BF, device=DEV)
+    got = Q.decode_attention(**a, out=wide[:, 8:8 + 1024])
+    assert torch.equal(got, want) and bool((wide[:, :8] == 7).all()) and bool((wide[:, 1032:] == 7).all())
+    for _ in range(5):
+        assert torch.equal(Q.decode_attention(**a), want)                   # the same bits every time
+    one = {**a, "q": a["q"][3:4], "block_table": a["block_table"][3:4], "seq_len": a["seq_len"][3:4]}
+    check(one)
+    assert Q.decode_attention(**{**a, "q": a["q"][:0], "block_table": a["block_table"][:0], "seq_len": a["seq_len"][:0]}).shape == (0, 1024)
+
+
+def test_lengths_behind_the_table_are_cut():
+    a = batch("int8", 4, 2, 64, 16, 16, [48, 32], dirty=False)
+    want = Q.decode_attention(**a)
+    t = a["block_table"].clone()
+    t[1, 2] = t[1, 1]
+    want2 = Q.decode_attention(**{**a, "block_table": t, "seq_len": torch.tensor([48, 48], dtype=torch.int32, device=DEV)})
+    got = Q.decode_attention(**{**a, "block_table": t, "seq_len": torch.tensor([2 ** 31 - 1, 49], dtype=torch.int32, device=DEV)})
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want2[1])
+
+
+def test_refusals():
+    H, Hkv, dh, page = 4, 2, 64, 16
+    pool = random_pool(3, Hkv, page, dh, "int8", 16)
+    x = torch.randn((2, (H + 2 * Hkv) * dh), generator=gen(0), device=DEV).to(BF)
+    table, lens = torch.zeros((2, 1), dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    good = dict(H=H, Hkv=Hkv, dh=dh, pool=pool, block_table=table, seq_len=lens)
+    cos, sin = ops.rope_table(8, dh, 10000.0, DEV)
+
+    def refused(fn, *a, **kw):
+        with pytest.raises(ValueError):
+            fn(*a, **kw)
+
+    for fn in (Q.kv_append, Q.decode_attention):
+        for bad in (dict(block_table=table.long()), dict(seq_len=lens.long()), dict(seq_len=lens.cpu()), dict(block_table=table.cpu()),
+                    dict(block_table=torch.zeros((2, 2), dtype=torch.int32, device=DEV)[:, ::2]), dict(pool=on_cpu(pool)),
+                    dict(pool=(pool.codes, pool.scales.cpu())), dict(pool=(pool.codes.transpose(0, 1).contiguous().transpose(0, 1), pool.scales))):
+            refused(fn, x, **{**good, **bad})
+        refused(fn, x[:, 4:], **good)                                        # rows that are not 16-byte aligned, or too short
+        refused(fn, x.repeat(1, 2)[:, ::2], **good)
+        refused(fn, x[:1].expand(2, -1), **good)
+    refused(Q.kv_append, x, **good, cu_q=torch.zeros(3, dtype=torch.int64, device=DEV))
+    refused(Q.rope_kv_append, x, H, Hkv, dh, cos.cpu(), sin.cpu(), pool, table, lens)
+    refused(Q.rope_kv_append, x, H, Hkv, dh, cos.t().contiguous().t(), sin, pool, table, lens)
+    small = random_pool(3, Hkv, page, 32, "int8", 16)
+    refused(Q.kv_append, x, H, Hkv, 32, small, table, lens)
+    refused(Q.decode_attention, x, small, table, lens, H, Hkv, 32)
+    refused(Q.read_pages, small, [0])
+    refused(Q.read_pages, pool, [3])
+    refused(Q.read_pages, pool, torch.zeros(1, dtype=torch.int64, device=DEV))
+    refused(Q.read_pages, pool, torch.zeros(4, dtype=torch.int32, device=DEV)[::2])
+    refused(Q.decode_attention, x, **good, out=torch.empty((2, H * dh), dtype=BF))
+    refused(Q.decode_attention, x, **good, out=torch.empty((2, H * dh + 4), dtype=BF, device=DEV)[:, 4:])
