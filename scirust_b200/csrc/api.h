@@ -137,7 +137,9 @@ int sb_quant_kv_append(void* qkv, long long ld, int n, int H, int Hkv, int dh, c
 int sb_quant_kv_read(const void* codes, int e4m3, const float* scales, int n_blocks, int Hkv, int page, int block, int dh, const int* pages, int n, void* out, void* stream_);
 
 // quantized_kv_attention.cu
-int sb_quant_kv_attention(const void* q, long long ldq, const void* codes, int e4m3, const float* scales, int n_blocks, int page, int block, const int* table, int max_blocks, const int* seq_len, int B, int H, int Hkv, int dh, float scale, void* out, long long ldo, void* stream_);
+int sb_quant_kv_attention_floats(int dh);
+int sb_quant_kv_attention(const void* q, long long ldq, const void* codes, int e4m3, const float* scales, int n_blocks, int page, int block, const int* table, int max_blocks, const int* seq_len, int B, int H, int Hkv, int dh, long long max_tiles, float scale, float* part, unsigned int* counters, void* out, long long ldo, int* status, void* stream_);
+int sb_stream_capture_id(void* stream_, unsigned long long* id);
 
 // sampler.cu
 int sb_sample_rows(const float* logits, int ld, int rows, int V, float temperature, int top_k, float top_p, float rep_penalty, int rep_window, const int64_t* recent, int recent_ld, const int* n_recent, uint64_t* rng_state, int64_t* out_tokens, int64_t* generated, int gen_stride, int step, uint32_t* work, void* stream);

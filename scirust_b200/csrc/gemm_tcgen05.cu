@@ -437,6 +437,21 @@ int make_tmap_2d_u16_plain(CUtensorMap* out, const void* base, uint64_t inner, u
   return r == CUDA_SUCCESS ? 0 : SB_ERR_DRIVER;
 }
 
+// 2-D tensor map over bytes whose rows of 64 or 128 are swizzled as wide as they are. Out-of-range parts of a box are filled with zeros.
+int make_tmap_2d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return SB_ERR_DRIVER;
+  if (reinterpret_cast<uintptr_t>(base) & 15) return SB_ERR_ALIGN;
+  cuuint64_t dims[2] = {row_bytes, rows};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {row_bytes, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : SB_ERR_DRIVER;
+}
+
 // Patches of an NHWC tensor [B, H, W, C]: boxes of 64 channels x `box` output pixels (ow per row, whole rows, whole
 // images when an image is smaller than the box) at element stride `stride`. 0 when the shape does not tile.
 static int make_tmap_patches(CUtensorMap* out, const void* base, int B, int H, int W, int C, int ow, int oh, int stride,

@@ -1,85 +1,494 @@
 // Attention of single tokens over the paged KV cache in 8 bits (its layout: quantized_kv.cu).
 //
-// o = sum_j w_j s_v(j) c_v(j) / sum_j w_j with w_j = exp(scale * s_k(j) * (q . c_k(j)) - m): codes c, scales s of the position's block. One CTA
-// for a query head of a sequence; each of its warps takes every fourth position, lanes hold dimensions, and the warps' running maxima,
-// sums and values are joined at the end.
+//   o = sum_j w_j s_v(j) c_v(j) / sum_j w_j,   w_j = exp(scale * s_k(j) * (q . c_k(j)) - m),
+// with codes c and the scales s of the position's block and head.
+//
+// Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time. One CTA per SM holds a ring of
+// tiles of 64 positions (keys and values, 8 or 16 KB) that one warp fills by TMA and another with the tile's sixteen scales; the tiles of all
+// jobs (a sequence and up to 16 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer
+// warps take the tiles in groups of four, warp w of a group 16 positions of the tile:
+//  - Codes become fp16, which holds every one of either type exactly: int8 by a byte permute (a byte behind 0x64 is 1024 + it) and one
+//    subtraction of two halves, e4m3 by its conversion. mma.sync takes them as the A operand, 16 positions (S = K q) or 16
+//    dimensions (O = V w) by 16, and eight query heads as columns: a warp's 16 positions times 16 query rows would be half empty
+//    with eight query heads a kv head or fewer. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of
+//    two halves of the A operand, and for K the dimensions of a step are in another order, in which q is loaded.
+//  - q is scaled by a power of two so that its row's largest magnitude is just below 2^15: fp16 then holds its bf16 values without loss.
+//  - The reference of the exponentials is a score seen before, not the maximum: it moves when a score exceeds it by 2^6, so that few
+//    tiles need a reduction over positions and a pass over O. Weights are 2^9 at the reference: at most 2^15, and what lies 2^-33 below the
+//    reference is still a number of fp16. Their sum is taken in 32 bits before they are rounded (half a step of 2^-11) and weighed.
+//  - A value's scale goes into its weight, as a ratio to the largest scale that the warp has seen of the piece, which weighs the sums at the
+//    end: a product of its own for each block of 16 positions would need a pass over O for each.
+// A job that is cut has its pieces joined by the CTA that ends last, in the order of the tiles (a counter, no atomics on data).
 #include <cuda_bf16.h>
 #include "api.h"
 #include "dependent.cuh"
+#include "per_device.h"
 #include "quantized_kv.cuh"
 #include "sm100_ptx.cuh"
 
 namespace sb {
+int num_sms();                                                 // gemm_tcgen05.cu
+int make_tmap_2d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes, uint64_t rows, uint32_t box_rows);
+
 namespace kv8 {
+
+constexpr int TK = 64;                       // positions of a tile
+constexpr int MAX_B = 1024;                  // sequences of a launch, whose offsets lie in shared memory
+constexpr int STAGES_MAX = 16;
+constexpr int HEADS_MAX = 16;                // query heads of a job
+constexpr int SMEM = 226 * 1024;
 
 struct AttendParams {
   const __nv_bfloat16* q; long long ldq;
-  const uint8_t* codes; const float* scales;
-  int n_blocks, page, block;
+  const float* scales;
+  int n_blocks, page, page_bits, block_bits;         // page_bits: 3, 4 or 5, or for multiples of 64 6
   const int* table; int max_blocks;
   const int* seq_len;
-  int H, Hkv;
-  float scale;
+  int B, Hkv, G, subs, heads;                // a kv head's G query heads in `subs` jobs of `heads`
+  float scale_log2;
+  float* part;                               // [2 * grid][HEADS_MAX][DH + 2]
+  unsigned int* counters;                    // [B * Hkv * subs], zero between calls
   __nv_bfloat16* out; long long ldo;
+  int* status;
+  int stages;
 };
 
-template <int DH, bool E4M3>
-__global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ AttendParams p) {
-  constexpr int LANES = DH / 4;                                // lanes that hold a position: all, or half of them
+template <int DH, int NH>
+struct Cfg {
+  static constexpr int CONSUMERS = NH == 1 ? 16 : 8;           // warps; with twice the accumulators, half of them
+  static constexpr int GROUPS = CONSUMERS / 4;
+  static constexpr int THREADS = CONSUMERS * 32 + 64;
+  static constexpr int TILE = TK * DH;                         // bytes of a tile's keys, and of its values
+  static constexpr int PITCH = DH + 4;                         // of a head's sums between warps: four heads of a pair of rows on different banks
+  static constexpr int merge_bytes(int heads) { return CONSUMERS * heads * (PITCH + 2) * 4; }
+  static constexpr int fixed_bytes(int heads) { return merge_bytes(heads) + (2 * MAX_B + 2) * 4 + STAGES_MAX * (64 + 16) + 1024; }
+  // A stage is always taken by one group: a parity wait tells a fill from the one after next only by whoever has seen the one between.
+  static constexpr int stages(int heads) {
+    const int n = (SMEM - fixed_bytes(heads)) / (2 * TILE) / GROUPS * GROUPS;
+    return n < STAGES_MAX ? n : STAGES_MAX;
+  }
+  static constexpr int smem_bytes(int heads) { return stages(heads) * 2 * TILE + fixed_bytes(heads); }
+};
+static_assert(Cfg<128, 1>::stages(8) >= 8 && Cfg<128, 2>::stages(16) >= 8, "128 KB in flight");
+
+__device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Bytes (0, 1) and (2, 3) of w as pairs of halves, or with APART (0, 2) and (1, 3).
+template <bool E4M3, bool APART>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& x, uint32_t& y) {
+  if constexpr (E4M3) {
+    if (APART) w = __byte_perm(w, 0, 0x3120);
+    asm("{\n"
+        ".reg .b16 lo, hi;\n"
+        "mov.b32 {lo, hi}, %2;\n"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n"
+        "}\n" : "=r"(x), "=r"(y) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    x = __byte_perm(u, 0x64646464u, APART ? 0x4240 : 0x4140);
+    y = __byte_perm(u, 0x64646464u, APART ? 0x4341 : 0x4342);
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64806480u));          // 1152
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y) : "r"(0x64806480u));
+  }
+}
+
+// Tiles of one sequence: an empty one keeps a tile without positions, whose job writes zeros.
+__device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + TK - 1) / TK : 1; }
+
+template <int DH, bool E4M3, int NH>
+__global__ void __launch_bounds__(Cfg<DH, NH>::THREADS, 1)
+attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
+  using C = Cfg<DH, NH>;
+  constexpr int CHUNKS = DH / 16, GROUPS = C::GROUPS, CONSUMERS = C::CONSUMERS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stages = p.stages, heads = p.heads, jobs_b = p.Hkv * p.subs;
+  float* sc = reinterpret_cast<float*>(ring + stages * 2 * C::TILE);                // [stages][k: 8 | v: 8], of 8 positions each
+  uint64_t* full = reinterpret_cast<uint64_t*>(sc + STAGES_MAX * 16);
+  uint64_t* empty = full + STAGES_MAX;
+  float* sm_o = reinterpret_cast<float*>(empty + STAGES_MAX);                       // [warps][heads][PITCH]
+  float* sm_ml = sm_o + CONSUMERS * heads * C::PITCH;                               // [warps][heads][2]
+  int* prefix = reinterpret_cast<int*>(sm_ml + CONSUMERS * heads * 2);              // [B + 1] tiles before sequence b
+  int* lens = prefix + MAX_B + 1;                                                   // [B]
+  __shared__ int s_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap);
+    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 17); mbar_init(&empty[s], 4); }
+    fence_barrier_init();
+  }
   pdl_trigger();
   pdl_wait();
-  const int head = blockIdx.x, b = blockIdx.y, kvh = head / (p.H / p.Hkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane % LANES * 4, part = lane / LANES;
-  const long long cap = static_cast<long long>(p.max_blocks) * p.page;
-  const int len = static_cast<int>(min(static_cast<long long>(p.seq_len[b]), cap));
-  const __nv_bfloat16* q = p.q + b * p.ldq + head * DH + d;
-  float4 qv;
-  qv.x = __bfloat162float(q[0]); qv.y = __bfloat162float(q[1]); qv.z = __bfloat162float(q[2]); qv.w = __bfloat162float(q[3]);
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0, 0, 0, 0);
-  constexpr int STEP = 4 * (32 / LANES);
-  for (int j0 = warp * (32 / LANES); j0 < len; j0 += STEP) {
-    const int j = j0 + part;
-    const bool live = j < len;
-    const int id = live ? p.table[static_cast<size_t>(b) * p.max_blocks + j / p.page] : 0;
-    const bool known = live && static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
-    const size_t row = known ? (static_cast<size_t>(id) * 2 * p.Hkv + kvh) : 0;
-    const int slot = j % p.page, blocks = p.page / p.block;
-    float4 k = make_float4(0, 0, 0, 0), v = k;
-    float ks = 0.f, vs = 0.f;
-    if (known) {
-      const size_t vrow = row + p.Hkv;
-      k = from_codes<E4M3>(*reinterpret_cast<const uint32_t*>(p.codes + (row * p.page + slot) * DH + d));
-      v = from_codes<E4M3>(*reinterpret_cast<const uint32_t*>(p.codes + (vrow * p.page + slot) * DH + d));
-      ks = p.scales[row * blocks + slot / p.block];
-      vs = p.scales[vrow * blocks + slot / p.block];
-    }
-    float s = qv.x * k.x + qv.y * k.y + qv.z * k.z + qv.w * k.w;
+  if (warp == 0) {
+    const int cap = static_cast<int>(min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll - TK));
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int len = b0 + lane < p.B ? min(p.seq_len[b0 + lane], cap) : 0;
+      const int n = b0 + lane < p.B ? tiles_of(len) : 0;
+      int inc = n;
 #pragma unroll
-    for (int x = 1; x < LANES; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s = live ? s * ks * p.scale : -INFINITY;
-    if (!live) continue;                                       // the upper half of a warp, at the last position only
-    const float top = fmaxf(m, s), w = s == top && top == m ? 1.f : expf(s - top), a = top == m ? 1.f : expf(m - top);
-    m = top;
-    l = l * a + w;
-    o.x = o.x * a + w * vs * v.x; o.y = o.y * a + w * vs * v.y; o.z = o.z * a + w * vs * v.z; o.w = o.w * a + w * vs * v.w;
-  }
-  __shared__ float sm_m[8], sm_l[8], sm_o[8][DH];
-  const int who = warp * (32 / LANES) + part;
-  sm_o[who][d] = o.x; sm_o[who][d + 1] = o.y; sm_o[who][d + 2] = o.z; sm_o[who][d + 3] = o.w;
-  if (d == 0) { sm_m[who] = m; sm_l[who] = l; }
-  __syncthreads();
-  if (threadIdx.x < DH) {
-    float top = -INFINITY, lt = 0.f, ot = 0.f;
-    for (int w = 0; w < STEP; ++w) top = fmaxf(top, sm_m[w]);
-    for (int w = 0; w < STEP; ++w) {
-      if (w >= len) break;                                     // it has seen no position
-      const float a = sm_m[w] == top ? 1.f : expf(sm_m[w] - top);
-      lt += sm_l[w] * a;
-      ot += sm_o[w][threadIdx.x] * a;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (b0 + lane < p.B) { prefix[b0 + lane] = base + inc - n; lens[b0 + lane] = len; }
+      base += __shfl_sync(0xffffffffu, inc, 31);
     }
-    p.out[b * p.ldo + head * DH + threadIdx.x] = __float2bfloat16_rn(len > 0 ? ot / lt : 0.f);
+    if (lane == 0) prefix[p.B] = base;
   }
+  __syncthreads();
+  // unit u = tile u - S of job (b, j), jobs in (b, j) order; this CTA takes units [u0, u1)
+  const long long T = static_cast<long long>(prefix[p.B]) * jobs_b;
+  const long long grid = min(static_cast<long long>(gridDim.x), (T + GROUPS - 1) / GROUPS);
+  if (blockIdx.x >= grid) return;
+  // divisions of whole 64-bit numbers take hundreds of cycles; up to 29 million tiles on 148 CTAs 32 bits hold every dividend
+  const bool narrow = (T + 1) * grid <= 0xffffffffll;
+  auto quotient = [&](long long a, long long d) -> long long {
+    return narrow ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(d)) : a / d;
+  };
+  const long long u0 = quotient(blockIdx.x * T, grid), u1 = quotient((blockIdx.x + 1) * T, grid);
+  int b = 0, len = 0, nt = 0, job = 0, t_beg = 0, t_end = 0;
+  long long s_job = 0;
+  {
+    int lo = 0, hi = p.B - 1;                  // last sequence whose first unit is <= u0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (static_cast<long long>(prefix[mid]) * jobs_b <= u0) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+  }
+  // A piece: the tiles [t_beg, t_end) of a job that lie in this CTA's range. Producer and consumers walk over the same pieces.
+  auto locate = [&](long long u) {
+    long long s_b = 0;
+    for (;; ++b) {
+      len = lens[b];
+      nt = tiles_of(len);
+      s_b = static_cast<long long>(prefix[b]) * jobs_b;
+      if (u < s_b + static_cast<long long>(nt) * jobs_b) break;
+    }
+    const long long off = u - s_b;                       // below nt * jobs_b
+    job = static_cast<int>(quotient(off, nt));
+    s_job = s_b + static_cast<long long>(job) * nt;
+    t_beg = static_cast<int>(u - s_job);
+    t_end = static_cast<int>(min(static_cast<long long>(nt), t_beg + (u1 - u)));
+  };
+
+  if (warp >= CONSUMERS) {
+    // ------------------------------ producers: one warp brings codes, one scales ------------------------------
+    const bool brings_codes = warp == CONSUMERS;
+    const int box_bits = min(p.page_bits, 6), box = 1 << box_bits, nbx = TK >> box_bits;    // positions of a TMA box, boxes of a tile
+    // of a tile, a lane has one box of codes of keys or values (eight boxes of each at most), or one scale, of eight positions
+    const int v = brings_codes ? lane & 1 : (lane >> 3) & 1;
+    const int first = brings_codes ? (lane >> 1) << box_bits : (lane & 7) * 8;              // its first position in the tile
+    const int x = first >> box_bits;
+    const int unit = brings_codes ? p.page : p.page >> p.block_bits;                        // rows or scales of a page and head
+    const int step = v * p.Hkv * unit + (brings_codes ? 0 : (first & (box - 1)) >> p.block_bits);
+    const int none = brings_codes ? p.n_blocks * 2 * p.Hkv * p.page : -1;                   // for ids outside the pool: a row behind the last one
+    const int slot_bits = brings_codes ? 0 : p.block_bits;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (long long u = u0; u < u1 && ok; u += t_end - t_beg) {
+      locate(u);
+      const int kvh = job / p.subs;
+      const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
+      int at_of_lane = -1;                               // of box (fetched + lane): its first row of keys, or their scale
+      int fetched = -1000000;
+      for (int t = t_beg; t < t_end; ++t) {
+        const int bx0 = t * nbx;
+        if (bx0 + nbx > fetched + 32) {                  // nbx divides 32: a tile's boxes are fetched together
+          fetched = bx0;
+          const long long pos = static_cast<long long>(fetched + lane) << box_bits;
+          at_of_lane = -1;
+          if (pos < len) {
+            const int at = static_cast<int>(pos) / p.page, slot = static_cast<int>(pos) - at * p.page, id = table[at];
+            if (static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks)) at_of_lane = (id * 2 * p.Hkv + kvh) * unit + (slot >> slot_bits);
+          }
+        }
+        const int base = __shfl_sync(0xffffffffu, at_of_lane, bx0 + x - fetched);
+        const int at = base < 0 ? none : base + step, left = len - t * TK;                  // positions of the tile that exist, or more
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        if (brings_codes) {
+          const int live = left >= TK ? nbx : max(0, (left + box - 1) >> box_bits);         // boxes with a position that exists
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
+          __syncwarp();
+          if (x < live) tma_load_2d(ring + stage * 2 * C::TILE + v * C::TILE + first * DH, &tmap, &full[stage], 0, at);
+        } else if (lane < 16) {
+          const bool real = first < left && at >= 0;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 16 + lane)), "l"(p.scales + (real ? at : 0)),
+                       "r"(real ? 4 : 0) : "memory");
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
+        }
+        __syncwarp();
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+
+  // ------------------------------ consumers -----------------------------
+  const int quad = lane >> 2, tq = lane & 3, mi = lane >> 3;
+  const int group = warp >> 2, pw = warp & 3;
+  const int wrow = pw * 16 + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
+  const int swz = DH == 128 ? (wrow & 7) : ((wrow >> 1) & 3);
+  long long it = 0;                          // tiles of the CTA before the piece
+  int stage = group;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (long long u = u0; u < u1;) {
+    locate(u);
+    const int h0 = (job / p.subs) * p.G + (job % p.subs) * heads, live = min(heads, p.G - (job % p.subs) * heads);
+    // q as B fragments: column `quad` is a query head; of a step of 16 dimensions the lane's four are 4 tq .. 4 tq + 3, as K's bytes come
+    uint32_t qb[NH][CHUNKS][2];
+    float qf[NH][2];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const int h = n * 8 + quad;
+      const __nv_bfloat16* src = p.q + b * p.ldq + static_cast<long long>(h0 + h) * DH + tq * 4;
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const uint2 v = h < live ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
+        qb[n][c][0] = v.x;
+        qb[n][c][1] = v.y;
+        top = __vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+      }
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 15u);               // the exponent of the largest, biased
+      const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);      // 2^(14 - (e - 127)), and back
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        qb[n][c][0] = half2_bits(bf16_lo(qb[n][c][0]) * up, bf16_hi(qb[n][c][0]) * up);
+        qb[n][c][1] = half2_bits(bf16_lo(qb[n][c][1]) * up, bf16_hi(qb[n][c][1]) * up);
+      }
+      const float f = down * p.scale_log2;
+      qf[n][0] = __shfl_sync(0xffffffffu, f, tq * 8);                                // of heads 2 tq and 2 tq + 1, the columns of a result
+      qf[n][1] = __shfl_sync(0xffffffffu, f, tq * 8 + 4);
+    }
+    float m[NH][2], l[NH][2], o[CHUNKS][NH][4];
+    float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
+#pragma unroll
+    for (int n = 0; n < NH; ++n) m[n][0] = m[n][1] = -1.0e30f, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+      for (int n = 0; n < NH; ++n) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
+
+    for (int t = t_beg + static_cast<int>((group - it) & (GROUPS - 1)); t < t_end; t += GROUPS) {
+      const int st = stage;
+      const uint32_t ph = phase;
+      stage += GROUPS;
+      if (stage >= stages) { stage -= stages; phase ^= 1; }
+      if (ok && !mbar_wait_warp(&full[st], ph, p.status, ST_TIMEOUT_FULL)) ok = false;
+      if (!ok) continue;
+      const uint32_t kt = smem_u32(ring + st * 2 * C::TILE) + wrow * DH, vt = kt + C::TILE;
+      const float2 ks = *reinterpret_cast<const float2*>(sc + st * 16 + pw * 2), vs = *reinterpret_cast<const float2*>(sc + st * 16 + 8 + pw * 2);
+      const int valid = len - t * TK - pw * 16;                                      // positions of this warp's 16 that exist
+      float s[NH][4];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c += 2) {
+        uint32_t r[4], a[4];
+        ldsm(kt + (((c + (mi >> 1)) ^ swz) << 4), r);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          widen<E4M3, false>(r[2 * i], a[0], a[2]);
+          widen<E4M3, false>(r[2 * i + 1], a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_f16(s[n], a[0], a[1], a[2], a[3], qb[n][c + i][0], qb[n][c + i][1]);
+        }
+      }
+      bool over = vs.x > vref || vs.y > vref;
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[n][e] *= ks.x * qf[n][e];
+          s[n][2 + e] *= ks.y * qf[n][e];
+          if (valid < 16) {
+            if (quad >= valid) s[n][e] = -INFINITY;
+            if (quad + 8 >= valid) s[n][2 + e] = -INFINITY;
+          }
+          over |= s[n][e] - m[n][e] > 15.f || s[n][2 + e] - m[n][e] > 15.f;
+        }
+      }
+      if (__any_sync(0xffffffffu, over)) {
+        const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
+        vref = v_new;
+        vinv = 1.f / v_new;
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[n][e], s[n][2 + e]) - 9.f;
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float m_new = fmaxf(m[n][e], top), a = ex2(m[n][e] - m_new);
+            m[n][e] = m_new;
+            l[n][e] *= a;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+              o[c][n][e] *= a * v_ratio;
+              o[c][n][2 + e] *= a * v_ratio;
+            }
+          }
+        }
+      }
+      uint32_t w[NH][2];
+      {
+        const float v0 = vs.x * vinv, v1 = vs.y * vinv;
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = ex2(s[n][i] - m[n][i & 1]);
+          l[n][0] += e[0] + e[2];
+          l[n][1] += e[1] + e[3];
+          w[n][0] = transpose8x8(half2_bits(e[0] * v0, e[1] * v0));
+          w[n][1] = transpose8x8(half2_bits(e[2] * v1, e[3] * v1));
+        }
+      }
+      // what lies behind the last position may be NaN, which a weight of zero does not make zero
+      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+      if (E4M3 && valid < 16) {
+        keep0 = (2 * tq < valid ? 0xffffu : 0u) | (2 * tq + 1 < valid ? 0xffff0000u : 0u);
+        keep1 = (2 * tq + 8 < valid ? 0xffffu : 0u) | (2 * tq + 9 < valid ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c += 2) {
+        uint32_t r[4], a[4];
+        ldsm_t(vt + (((c + (mi >> 1)) ^ swz) << 4), r);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (E4M3) { r[2 * i] &= keep0; r[2 * i + 1] &= keep1; }
+          widen<E4M3, true>(r[2 * i], a[0], a[1]);
+          widen<E4M3, true>(r[2 * i + 1], a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_f16(o[c + i][n], a[0], a[1], a[2], a[3], w[n][0], w[n][1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    it += t_end - t_beg;
+    u += t_end - t_beg;
+
+    // ---- the warps' sums are joined in the order of the warps ----
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = n * 8 + 2 * tq + e;
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+        if (h >= live) continue;
+        float* dst = sm_o + (warp * heads + h) * C::PITCH + 2 * quad;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float2*>(dst + c * 16) = make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
+        if (quad == 0) { sm_ml[(warp * heads + h) * 2] = m[n][e]; sm_ml[(warp * heads + h) * 2 + 1] = l[n][e]; }
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
+    const bool whole = t_beg == 0 && t_end == nt;
+    float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (t_beg == 0)) * (HEADS_MAX * (DH + 2));
+    auto write_out = [&](int h, int d, float4 v, float sum) {
+      if (len > 0) { v.x /= sum; v.y /= sum; v.z /= sum; v.w /= sum; }
+      *reinterpret_cast<uint2*>(p.out + b * p.ldo + static_cast<long long>(h0 + h) * DH + d) =
+          make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    };
+    for (int i = threadIdx.x; i < live * (DH / 4); i += CONSUMERS * 32) {
+      const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+      float top = -1.0e30f, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < CONSUMERS; ++x) top = fmaxf(top, sm_ml[(x * heads + h) * 2]);
+#pragma unroll
+      for (int x = 0; x < CONSUMERS; ++x) {
+        const float a = ex2(sm_ml[(x * heads + h) * 2] - top);
+        const float4 e = *reinterpret_cast<const float4*>(sm_o + (x * heads + h) * C::PITCH + d);
+        sum += sm_ml[(x * heads + h) * 2 + 1] * a;
+        v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
+      }
+      if (whole) {
+        write_out(h, d, v, sum);
+      } else {
+        float* dst = part + h * (DH + 2);
+        *reinterpret_cast<float2*>(dst + d) = make_float2(v.x, v.y);
+        *reinterpret_cast<float2*>(dst + d + 2) = make_float2(v.z, v.w);
+        if (d == 0) { dst[DH] = top; dst[DH + 1] = sum; }
+      }
+    }
+    if (whole) {
+      asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
+      continue;
+    }
+    // ---- the CTA that ends last joins the pieces, in the order of the tiles ----
+    const long long c0 = quotient((s_job + 1) * grid - 1, T), c1 = quotient((s_job + nt) * grid - 1, T);
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
+    if (threadIdx.x == 0) {
+      unsigned int* ctr = p.counters + static_cast<size_t>(b) * jobs_b + job;
+      const unsigned int before = atomicAdd(ctr, 1u);
+      s_last = before == static_cast<unsigned int>(c1 - c0);
+      if (s_last) *ctr = 0;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
+    if (!s_last) continue;
+    __threadfence();
+    for (int i = threadIdx.x; i < live * (DH / 4); i += CONSUMERS * 32) {
+      const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+      float top = -1.0e30f, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (long long c = c0; c <= c1; ++c)
+        top = fmaxf(top, __ldcg(p.part + static_cast<size_t>(2 * c + (c == c0)) * (HEADS_MAX * (DH + 2)) + h * (DH + 2) + DH));
+#pragma unroll 4
+      for (long long c = c0; c <= c1; ++c) {
+        const float* src = p.part + static_cast<size_t>(2 * c + (c == c0)) * (HEADS_MAX * (DH + 2)) + h * (DH + 2);
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(src + d)), y = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + DH));
+        const float a = ex2(ml.x - top);
+        sum += ml.y * a;
+        v.x += x.x * a; v.y += x.y * a; v.z += y.x * a; v.w += y.y * a;
+      }
+      write_out(h, d, v, sum);
+    }
+  }
+}
+
+template <int DH, bool E4M3, int NH>
+static int launch_attend(const CUtensorMap& tm, AttendParams p, int grid, cudaStream_t s) {
+  using C = Cfg<DH, NH>;
+  static PerDeviceOnce attr;
+  if (allow_smem(attr, attend_kernel<DH, E4M3, NH>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  p.stages = C::stages(p.heads);
+  return launch_dep(attend_kernel<DH, E4M3, NH>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.heads), s, tm, p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 }  // namespace kv8
@@ -87,22 +496,57 @@ __global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ Att
 
 using namespace sb;
 
-// q: [B, ldq] bf16 (H * dh used, rotated); out: [B, ldo] bf16. A sequence of no positions gets zeros; ids outside the pool count as zeros.
+// Floats of `part` for launches on the current device at head dimension dh.
+extern "C" int sb_quant_kv_attention_floats(int dh) { return 2 * num_sms() * kv8::HEADS_MAX * (dh + 2); }
+
+// q: [B, ldq] bf16 (H * dh used, rotated), out: [B, ldo] bf16, rows 16-byte aligned. A sequence of no positions gets zeros; ids outside the
+// pool count as zeros. page 8, 16, 32 or a multiple of 64; B <= 1024. max_tiles: an upper bound of the 64-position tiles of all
+// jobs, which only caps the grid. counters: B * Hkv * ceil(H / Hkv / 16) words, zero before the first call (every call leaves them zero).
 extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* codes, int e4m3, const float* scales, int n_blocks, int page,
                                      int block, const int* table, int max_blocks, const int* seq_len, int B, int H, int Hkv, int dh,
-                                     float scale, void* out, long long ldo, void* stream_) {
-  if (!q || !codes || !scales || !table || !seq_len || !out || B <= 0 || H <= 0 || max_blocks <= 0 || !kv8::layout_ok(Hkv, dh, n_blocks, page, block) ||
-      H % Hkv)
+                                     long long max_tiles, float scale, float* part, unsigned int* counters, void* out, long long ldo,
+                                     int* status, void* stream_) {
+  if (!q || !codes || !scales || !table || !seq_len || !out || !part || !counters || !status || B <= 0 || B > kv8::MAX_B || H <= 0 ||
+      max_blocks <= 0 || max_tiles <= 0 || !kv8::layout_ok(Hkv, dh, n_blocks, page, block) || H % Hkv)
     return SB_ERR_ARG;
-  if (B > 65535) return SB_ERR_TOO_LARGE;
+  if (page != 8 && page != 16 && page != 32 && page % 64) return SB_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || (ldq & 7) || (ldo & 7)) return SB_ERR_ALIGN;
+  const uint64_t rows = static_cast<uint64_t>(n_blocks) * 2 * Hkv * page;
+  if (rows > 0x7fffffffull - kv8::TK) return SB_ERR_TOO_LARGE;
+  CUtensorMap tm;
+  const int rc = make_tmap_2d_u8_rows(&tm, codes, dh, rows, page < kv8::TK ? page : kv8::TK);
+  if (rc) return rc;
   kv8::AttendParams p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq;
-  p.codes = static_cast<const uint8_t*>(codes); p.scales = scales;
-  p.n_blocks = n_blocks; p.page = page; p.block = block;
+  p.scales = scales;
+  p.n_blocks = n_blocks; p.page = page;
+  for (p.page_bits = 3; p.page_bits < 6 && (1 << p.page_bits) < page;) ++p.page_bits;
+  for (p.block_bits = 3; (1 << p.block_bits) < block;) ++p.block_bits;
   p.table = table; p.max_blocks = max_blocks; p.seq_len = seq_len;
-  p.H = H; p.Hkv = Hkv; p.scale = scale;
+  p.B = B; p.Hkv = Hkv; p.G = H / Hkv;
+  p.subs = (p.G + kv8::HEADS_MAX - 1) / kv8::HEADS_MAX;
+  p.heads = (p.G + p.subs - 1) / p.subs;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part = part; p.counters = counters;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  auto kern = dh == 64 ? (e4m3 ? kv8::attend_kernel<64, true> : kv8::attend_kernel<64, false>)
-                       : (e4m3 ? kv8::attend_kernel<128, true> : kv8::attend_kernel<128, false>);
-  return launch_dep(kern, dim3(H, B), dim3(128), 0, static_cast<cudaStream_t>(stream_), p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  p.status = status;
+  // a tile for each group of consumers at least
+  const long long want = (max_tiles + 3) / 4;
+  const int grid = want < num_sms() ? static_cast<int>(want) : num_sms();
+  cudaStream_t s = static_cast<cudaStream_t>(stream_);
+  const bool two = p.heads > 8;
+  if (dh == 64)
+    return e4m3 ? (two ? kv8::launch_attend<64, true, 2>(tm, p, grid, s) : kv8::launch_attend<64, true, 1>(tm, p, grid, s))
+                : (two ? kv8::launch_attend<64, false, 2>(tm, p, grid, s) : kv8::launch_attend<64, false, 1>(tm, p, grid, s));
+  return e4m3 ? (two ? kv8::launch_attend<128, true, 2>(tm, p, grid, s) : kv8::launch_attend<128, true, 1>(tm, p, grid, s))
+              : (two ? kv8::launch_attend<128, false, 2>(tm, p, grid, s) : kv8::launch_attend<128, false, 1>(tm, p, grid, s));
+}
+
+// The capture that `stream` is in, 0 where it is in none: what a graph's launches share is apart from every other graph's.
+extern "C" int sb_stream_capture_id(void* stream_, unsigned long long* id) {
+  cudaStreamCaptureStatus status;
+  unsigned long long capture = 0;
+  if (!id || cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream_), &status, &capture) != cudaSuccess) return SB_ERR_RUNTIME;
+  *id = status == cudaStreamCaptureStatusActive ? capture : 0;
+  return 0;
 }

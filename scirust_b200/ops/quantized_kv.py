@@ -9,7 +9,10 @@ rounded to the new steps; a code stays within one step of its value, e4m3 loses 
 is given an infinity or a NaN (e4m3: or what rounds to an infinity) reads as NaN until its first position is written again."""
 from __future__ import annotations
 
+import ctypes as C
+import functools
 import math
+import threading
 from typing import NamedTuple
 
 import torch
@@ -21,7 +24,8 @@ BF = torch.bfloat16
 vp, i32, i64, f32 = _lib.vp, _lib.i32, _lib.i64, _lib.f32
 _lib.register("sb_quant_kv_append", [vp, i64, i32, i32, i32, i32, vp, vp, i32, vp, i32, vp, i32, i32, i32, vp, i32, vp, vp, i32, i32, vp])
 _lib.register("sb_quant_kv_read", [vp, i32, vp, i32, i32, i32, i32, i32, vp, i32, vp, vp])
-_lib.register("sb_quant_kv_attention", [vp, i64, vp, i32, vp, i32, i32, i32, vp, i32, vp, i32, i32, i32, i32, f32, vp, i64, vp])
+_lib.register("sb_quant_kv_attention", [vp, i64, vp, i32, vp, i32, i32, i32, vp, i32, vp, i32, i32, i32, i32, i64, f32, vp, vp, vp, i64, vp, vp])
+_lib.register("sb_stream_capture_id", [vp, vp])
 
 CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 LARGEST = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
@@ -262,6 +266,52 @@ def read_pages(pool, pages, out=None):
 
 
 # ---------------------------------------------------------------------------------------------------------------- attention
+TILE, JOB_HEADS, LAUNCH_SEQUENCES = 64, 16, 1024          # positions of a tile, query heads of a job, sequences of a launch
+
+
+class _Workspace:
+    """Parts of jobs that are cut, and a counter for each job, which every launch leaves at zero."""
+    __slots__ = ("part", "counters", "capture")
+
+    def __init__(self, floats, counters, device, capture):
+        self.part = _lib.empty(floats, torch.float32, device)
+        self.counters = torch.zeros(counters, dtype=torch.int32, device=device)
+        self.capture = capture
+
+
+_ws: dict = {}
+_ws_lock = threading.Lock()
+
+
+@functools.lru_cache(maxsize=64)
+def _part_floats(device_index, dh):
+    return _lib.cuda().sb_quant_kv_attention_floats(dh)
+
+
+def _workspace(device, stream, floats, counters):
+    """Launches on one stream follow one another and share one. Those of a graph share one of the graph's memory, whose counters it clears
+    itself: graphs captured on one stream may be replayed at once on two."""
+    capture = 0
+    if torch._C._cuda_isCurrentStreamCapturing():
+        word = (C.c_ulonglong * 1)()
+        _lib.call("sb_stream_capture_id", stream, word)
+        capture = word[0]
+    key = (device.index, stream, capture != 0)
+    w = _ws.get(key)
+    if w is None or w.capture != capture or w.counters.shape[0] < counters or w.part.shape[0] < floats or _lib.DEBUG_POISON:
+        with _ws_lock:
+            w = _ws.get(key)
+            if w is None or w.capture != capture or w.counters.shape[0] < counters or w.part.shape[0] < floats or _lib.DEBUG_POISON:
+                w = _ws[key] = _Workspace(floats, max(counters, 4096), device, capture)
+    return w
+
+
+def drop_workspace(device, stream):
+    """Gives back what calls on ``stream`` (a handle) work in, some 4 MB, where no more of them are to come."""
+    for captured in (False, True):
+        _ws.pop((device.index, stream, captured), None)
+
+
 def decode_attention_ref(q, pool, block_table, seq_len, H, Hkv, dh, scale=None):
     """fp32 statement, one sequence at a time; a sequence of no positions gets zeros."""
     codes, scales, _, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
@@ -315,7 +365,24 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
         return out
     if n_blocks == 0:
         raise ValueError("decode_attention: the pool has no pages")
-    _lib.call("sb_quant_kv_attention", q_at, ldq, codes.data_ptr(), codes.dtype is not torch.int8, scales.data_ptr(), n_blocks, page, block,
-              block_table.data_ptr(), max_blocks, seq_len.data_ptr(), B, H, Hkv, dh, scale, out.data_ptr(), ldo, _lib.stream())
-    _g.launch_count += 1
+    if page not in (8, 16, 32) and page % TILE:
+        raise ValueError("decode_attention: pages of 8, 16, 32 or a multiple of 64 positions")
+    if n_blocks * 2 * Hkv * page >= (1 << 31) - TILE:
+        raise ValueError("decode_attention: more rows of codes than 31 bits count")
+    tiles = -(-max_blocks * page // TILE)                       # of a sequence, at most
+    at_once = min(B, LAUNCH_SEQUENCES, ((1 << 31) - 1) // tiles)
+    jobs = Hkv * -(-(H // Hkv) // JOB_HEADS)
+    if max_len is not None:
+        tiles = min(tiles, max(1, -(-int(max_len) // TILE)))
+    stream = _lib.stream()
+    ws = _workspace(device, stream, _part_floats(device.index, dh), at_once * jobs)
+    part, counters, status = ws.part.data_ptr(), ws.counters.data_ptr(), _lib.status_word(device).data_ptr()
+    codes_at, e4m3, scales_at, table_at, lens_at, o_at = (codes.data_ptr(), codes.dtype is not torch.int8, scales.data_ptr(),
+                                                          block_table.data_ptr(), seq_len.data_ptr(), out.data_ptr())
+    for b in range(0, B, at_once):
+        n = min(at_once, B - b)
+        _lib.call("sb_quant_kv_attention", q_at + b * ldq * 2, ldq, codes_at, e4m3, scales_at, n_blocks, page, block,
+                  table_at + b * max_blocks * 4, max_blocks, lens_at + b * 4, n, H, Hkv, dh, n * jobs * tiles, scale, part, counters,
+                  o_at + b * ldo * 2, ldo, status, stream)
+        _g.launch_count += 1
     return out
