@@ -37,6 +37,7 @@ constexpr int MAX_B = 1024;                  // sequences of a launch, whose off
 constexpr int STAGES_MAX = 16;
 constexpr int HEADS_MAX = 16;                // query heads of a job
 constexpr int SMEM = 226 * 1024;
+constexpr int GRID_MAX = 160;
 
 struct AttendParams {
   const __nv_bfloat16* q; long long ldq;
@@ -46,7 +47,7 @@ struct AttendParams {
   const int* seq_len;
   int B, Hkv, G, subs, heads;                // a kv head's G query heads in `subs` jobs of `heads`
   float scale_log2;
-  float* part;                               // [2 * grid][HEADS_MAX][DH + 2]
+  float* part;                               // [2 * grid] of [HEADS_MAX][DH] values and [HEADS_MAX][2] maxima and sums
   unsigned int* counters;                    // [B * Hkv * subs], zero between calls
   __nv_bfloat16* out; long long ldo;
   int* status;
@@ -60,6 +61,7 @@ struct Cfg {
   static constexpr int THREADS = CONSUMERS * 32 + 64;
   static constexpr int TILE = TK * DH;                         // bytes of a tile's keys, and of its values
   static constexpr int PITCH = DH + 4;                         // of a head's sums between warps: four heads of a pair of rows on different banks
+  static constexpr int SETS = NH == 1 ? 8 : 4;                 // that share the pieces of a job which is joined
   static constexpr int merge_bytes(int heads) { return CONSUMERS * heads * (PITCH + 2) * 4; }
   static constexpr int fixed_bytes(int heads) { return merge_bytes(heads) + (2 * MAX_B + 2) * 4 + STAGES_MAX * (64 + 16) + 1024; }
   // A stage is always taken by one group: a parity wait tells a fill from the one after next only by whoever has seen the one between.
@@ -69,6 +71,9 @@ struct Cfg {
   }
   static constexpr int smem_bytes(int heads) { return stages(heads) * 2 * TILE + fixed_bytes(heads); }
 };
+// The weights of a job's pieces (one for each CTA at most) and the sets' values lie where the warps' sums have lain.
+static_assert(GRID_MAX + 4 + Cfg<64, 1>::SETS * 64 <= 16 * Cfg<64, 1>::PITCH && GRID_MAX + 4 + Cfg<128, 1>::SETS * 128 <= 16 * Cfg<128, 1>::PITCH &&
+              GRID_MAX + 4 + Cfg<64, 2>::SETS * 64 <= 8 * Cfg<64, 2>::PITCH && GRID_MAX + 4 + Cfg<128, 2>::SETS * 128 <= 8 * Cfg<128, 2>::PITCH, "");
 static_assert(Cfg<128, 1>::stages(8) >= 8 && Cfg<128, 2>::stages(16) >= 8, "128 KB in flight");
 
 __device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
@@ -417,7 +422,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     }
     asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
     const bool whole = t_beg == 0 && t_end == nt;
-    float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (t_beg == 0)) * (HEADS_MAX * (DH + 2));
+    auto part_of = [&](long long c) { return p.part + static_cast<size_t>(c) * (HEADS_MAX * (DH + 2)); };
     auto write_out = [&](int h, int d, float4 v, float sum) {
       if (len > 0) { v.x /= sum; v.y /= sum; v.z /= sum; v.w /= sum; }
       *reinterpret_cast<uint2*>(p.out + b * p.ldo + static_cast<long long>(h0 + h) * DH + d) =
@@ -439,10 +444,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       if (whole) {
         write_out(h, d, v, sum);
       } else {
-        float* dst = part + h * (DH + 2);
-        *reinterpret_cast<float2*>(dst + d) = make_float2(v.x, v.y);
-        *reinterpret_cast<float2*>(dst + d + 2) = make_float2(v.z, v.w);
-        if (d == 0) { dst[DH] = top; dst[DH + 1] = sum; }
+        float* dst = part_of(2 * blockIdx.x + (t_beg == 0));
+        *reinterpret_cast<float4*>(dst + h * DH + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(dst + HEADS_MAX * DH + 2 * h) = make_float2(top, sum);
       }
     }
     if (whole) {
@@ -450,35 +454,63 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       continue;
     }
     // ---- the CTA that ends last joins the pieces, in the order of the tiles ----
-    const long long c0 = quotient((s_job + 1) * grid - 1, T), c1 = quotient((s_job + nt) * grid - 1, T);
-    __threadfence();
+    const long long c0 = quotient((s_job + 1) * grid - 1, T);
+    const int pieces = static_cast<int>(quotient((s_job + nt) * grid - 1, T) - c0) + 1;
     asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
     if (threadIdx.x == 0) {
+      __threadfence();
       unsigned int* ctr = p.counters + static_cast<size_t>(b) * jobs_b + job;
-      const unsigned int before = atomicAdd(ctr, 1u);
-      s_last = before == static_cast<unsigned int>(c1 - c0);
+      s_last = atomicAdd(ctr, 1u) == static_cast<unsigned int>(pieces) - 1;
       if (s_last) *ctr = 0;
+      __threadfence();
     }
     asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
     if (!s_last) continue;
-    __threadfence();
-    for (int i = threadIdx.x; i < live * (DH / 4); i += CONSUMERS * 32) {
-      const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+    // weights of the pieces: a warp for each head
+    auto piece = [&](int i) { return part_of(2 * (c0 + i) + (i == 0)); };
+    float* sm_a = sm_o;                                          // [heads][pieces], then [sets][heads][DH] of values
+    float* sm_v = sm_o + ((heads * pieces + 3) & ~3);
+    for (int h = warp; h < live; h += CONSUMERS) {
       float top = -1.0e30f, sum = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (long long c = c0; c <= c1; ++c)
-        top = fmaxf(top, __ldcg(p.part + static_cast<size_t>(2 * c + (c == c0)) * (HEADS_MAX * (DH + 2)) + h * (DH + 2) + DH));
-#pragma unroll 4
-      for (long long c = c0; c <= c1; ++c) {
-        const float* src = p.part + static_cast<size_t>(2 * c + (c == c0)) * (HEADS_MAX * (DH + 2)) + h * (DH + 2);
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(src + d)), y = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + DH));
+      for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(piece(i) + HEADS_MAX * DH + 2 * h));
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      for (int i = lane; i < pieces; i += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(i) + HEADS_MAX * DH + 2 * h));
         const float a = ex2(ml.x - top);
+        sm_a[h * pieces + i] = a;
         sum += ml.y * a;
-        v.x += x.x * a; v.y += x.y * a; v.z += y.x * a; v.w += y.y * a;
       }
-      write_out(h, d, v, sum);
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (lane == 0) sm_ml[h] = sum;
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
+    const int items = live * (DH / 4), sets = min(C::SETS, max(1, CONSUMERS * 32 / items));
+    for (int i = threadIdx.x; i < items * sets; i += CONSUMERS * 32) {
+      const int set = i / items, at = (i - set * items) * 4, h = at / DH;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = set; c < pieces; c += sets) {
+        const float4 e = __ldcg(reinterpret_cast<const float4*>(piece(c) + at));
+        const float a = sm_a[h * pieces + c];
+        v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
+      }
+      if (sets == 1) write_out(h, at % DH, v, sm_ml[h]);
+      else *reinterpret_cast<float4*>(sm_v + set * heads * DH + at) = v;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
+    if (sets == 1) continue;
+    if (threadIdx.x < items) {
+      const int at = threadIdx.x * 4, h = at / DH;
+      float4 v = *reinterpret_cast<const float4*>(sm_v + at);
+      for (int x = 1; x < sets; ++x) {
+        const float4 e = *reinterpret_cast<const float4*>(sm_v + x * heads * DH + at);
+        v.x += e.x; v.y += e.y; v.z += e.z; v.w += e.w;
+      }
+      write_out(h, at % DH, v, sm_ml[h]);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
   }
 }
 
@@ -532,7 +564,7 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   p.status = status;
   // a tile for each group of consumers at least
   const long long want = (max_tiles + 3) / 4;
-  const int grid = want < num_sms() ? static_cast<int>(want) : num_sms();
+  const int most = num_sms() < kv8::GRID_MAX ? num_sms() : kv8::GRID_MAX, grid = want < most ? static_cast<int>(want) : most;
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   const bool two = p.heads > 8;
   if (dh == 64)
