@@ -18,7 +18,11 @@
 //    reference is still a number of fp16. Their sum is taken in 32 bits before they are rounded (half a step of 2^-11) and weighed.
 //  - A value's scale goes into its weight, as a ratio to the largest scale that the warp has seen of the piece, which weighs the sums at the
 //    end: a product of its own for each block of 16 positions would need a pass over O for each.
-// A job that is cut has its pieces joined by the CTA that ends last, in the order of the tiles (a counter, no atomics on data).
+//  - A warp takes its positions' bytes into registers and gives the stage back before it computes, so that nearly the whole ring is always
+//    under way from memory.
+// At the end of a piece of a job the warps leave their sums in shared memory and go on; two finishing warps join them. A job that is cut
+// has its pieces joined by the CTA that ends last, in the order of the tiles (a counter, no atomics on data). Only the warp that brings the codes
+// works out which piece is next; the others find its sequence, heads and tiles beside its queries.
 #include <cuda_bf16.h>
 #include "api.h"
 #include "dependent.cuh"
@@ -34,7 +38,7 @@ namespace kv8 {
 
 constexpr int TK = 64;                       // positions of a tile
 constexpr int MAX_B = 1024;                  // sequences of a launch, whose offsets lie in shared memory
-constexpr int STAGES_MAX = 16;
+constexpr int STAGES_MAX = 24;
 constexpr int HEADS_MAX = 16;                // query heads of a job
 constexpr int SMEM = 226 * 1024;
 constexpr int GRID_MAX = 160;
@@ -54,33 +58,45 @@ struct AttendParams {
   int stages;
 };
 
+// The tiles [t_beg, t_end) of a job that lie in a CTA's range.
+struct __align__(16) Piece {
+  int b, h0, live, len;                      // sequence, query heads [h0, h0 + live), positions
+  int t_beg, t_end, nt, last;                // nt: tiles of the job; last: of the CTA
+  int start, counter, pad[2];                // the job's first unit, its counter
+};
+
 template <int DH, int NH>
 struct Cfg {
-  static constexpr int CONSUMERS = NH == 1 ? 16 : 8;           // warps; with twice the accumulators, half of them
+  static constexpr int CONSUMERS = NH == 1 ? 12 : 8;           // warps; with twice the accumulators, fewer
   static constexpr int GROUPS = CONSUMERS / 4;
-  static constexpr int THREADS = CONSUMERS * 32 + 64;
+  static constexpr int CODES = CONSUMERS, SCALES = CONSUMERS + 1, FINISHERS = CONSUMERS + 2;      // two producers, two finishers
+  static constexpr int THREADS = CONSUMERS * 32 + 128;
   static constexpr int TILE = TK * DH;                         // bytes of a tile's keys, and of its values
   static constexpr int PITCH = DH + 4;                         // of a head's sums between warps: four heads of a pair of rows on different banks
-  static constexpr int SETS = NH == 1 ? 8 : 4;                 // that share the pieces of a job which is joined
-  static constexpr int merge_bytes(int heads) { return CONSUMERS * heads * (PITCH + 2) * 4; }
-  static constexpr int fixed_bytes(int heads) { return merge_bytes(heads) + (2 * MAX_B + 2) * 4 + STAGES_MAX * (64 + 16) + 1024; }
-  // A stage is always taken by one group: a parity wait tells a fill from the one after next only by whoever has seen the one between.
-  static constexpr int stages(int heads) {
-    const int n = (SMEM - fixed_bytes(heads)) / (2 * TILE) / GROUPS * GROUPS;
-    return n < STAGES_MAX ? n : STAGES_MAX;
+  static constexpr int SETS = 4;                               // that share the pieces of a job which is joined
+  static constexpr int QSLOTS = NH == 1 ? 4 : 2;               // pieces whose queries lie in shared memory
+  static constexpr int fixed_bytes(int heads, int B) {
+    return CONSUMERS * heads * (PITCH + 2) * 4 + QSLOTS * (heads * DH * 2 + static_cast<int>(sizeof(Piece))) + (2 * B + 1) * 4 +
+           STAGES_MAX * (64 + 16) + (2 * QSLOTS + 2) * 8 + 1024;
   }
-  static constexpr int smem_bytes(int heads) { return stages(heads) * 2 * TILE + fixed_bytes(heads); }
+  // A stage is always taken by one group: a parity wait tells a fill from the one after next only by whoever has seen the one between.
+  static constexpr int stages(int heads, int B) {
+    const int n = (SMEM - fixed_bytes(heads, B)) / (2 * TILE), most = n < STAGES_MAX ? n : STAGES_MAX;
+    return most / GROUPS * GROUPS;
+  }
+  static constexpr int smem_bytes(int heads, int B) { return stages(heads, B) * 2 * TILE + fixed_bytes(heads, B); }
+  // the sets' values lie where the warps' sums have lain
+  static_assert(SETS * (DH + 2) <= CONSUMERS * (PITCH + 2), "");
 };
-// The weights of a job's pieces (one for each CTA at most) and the sets' values lie where the warps' sums have lain.
-static_assert(GRID_MAX + 4 + Cfg<64, 1>::SETS * 64 <= 16 * Cfg<64, 1>::PITCH && GRID_MAX + 4 + Cfg<128, 1>::SETS * 128 <= 16 * Cfg<128, 1>::PITCH &&
-              GRID_MAX + 4 + Cfg<64, 2>::SETS * 64 <= 8 * Cfg<64, 2>::PITCH && GRID_MAX + 4 + Cfg<128, 2>::SETS * 128 <= 8 * Cfg<128, 2>::PITCH, "");
-static_assert(Cfg<128, 1>::stages(8) >= 8 && Cfg<128, 2>::stages(16) >= 8, "128 KB in flight");
+static_assert(Cfg<128, 1>::stages(8, MAX_B) >= 8 && Cfg<128, 2>::stages(16, MAX_B) >= 8, "128 KB in flight");
 
-__device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+__device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&a)[2], uint32_t (&b)[2]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+__device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&a)[2], uint32_t (&b)[2]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -123,6 +139,16 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& x, uint32_t& y) {
 // Tiles of one sequence: an empty one keeps a tile without positions, whose job writes zeros.
 __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + TK - 1) / TK : 1; }
 
+// How the units (tiles of all jobs, end to end) are dealt out: the first `more` CTAs have one more than the others.
+struct Deal {
+  int units, ctas, each, more;
+  __device__ __forceinline__ int first(int c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int cta(int u) const {
+    const int at = more * (each + 1);
+    return u < at ? u / (each + 1) : more + (u - at) / each;
+  }
+};
+
 template <int DH, bool E4M3, int NH>
 __global__ void __launch_bounds__(Cfg<DH, NH>::THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
@@ -132,79 +158,76 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stages = p.stages, heads = p.heads, jobs_b = p.Hkv * p.subs;
   float* sc = reinterpret_cast<float*>(ring + stages * 2 * C::TILE);                // [stages][k: 8 | v: 8], of 8 positions each
-  uint64_t* full = reinterpret_cast<uint64_t*>(sc + STAGES_MAX * 16);
-  uint64_t* empty = full + STAGES_MAX;
-  float* sm_o = reinterpret_cast<float*>(empty + STAGES_MAX);                       // [warps][heads][PITCH]
+  __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 16);     // [slots][heads][DH]
+  Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * heads * DH);          // [slots]
+  float* sm_o = reinterpret_cast<float*>(pieces + C::QSLOTS);                       // [warps][heads][PITCH]
   float* sm_ml = sm_o + CONSUMERS * heads * C::PITCH;                               // [warps][heads][2]
-  int* prefix = reinterpret_cast<int*>(sm_ml + CONSUMERS * heads * 2);              // [B + 1] tiles before sequence b
-  int* lens = prefix + MAX_B + 1;                                                   // [B]
-  __shared__ int s_last;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ml + CONSUMERS * heads * 2);
+  uint64_t* empty = full + STAGES_MAX;
+  uint64_t* q_full = empty + STAGES_MAX;
+  uint64_t* q_empty = q_full + C::QSLOTS;
+  uint64_t* o_full = q_empty + C::QSLOTS;                                           // the warps' sums of a piece, but for the last one's
+  uint64_t* o_empty = o_full + 1;
+  int* prefix = reinterpret_cast<int*>(o_empty + 1);                                // [B + 1] tiles before sequence b
+  int* lens = prefix + p.B + 1;                                                     // [B]
+  __shared__ int s_last[2];
+  __shared__ Deal s_deal;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    prefetch_tmap(&tmap);
-    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 17); mbar_init(&empty[s], 4); }
-    fence_barrier_init();
-  }
-  pdl_trigger();
-  pdl_wait();
   if (warp == 0) {
-    const int cap = static_cast<int>(min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll - TK));
-    int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int len = b0 + lane < p.B ? min(p.seq_len[b0 + lane], cap) : 0;
-      const int n = b0 + lane < p.B ? tiles_of(len) : 0;
-      int inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (b0 + lane < p.B) { prefix[b0 + lane] = base + inc - n; lens[b0 + lane] = len; }
-      base += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    if (lane == 0) prefix[p.B] = base;
+    if (lane < stages) { mbar_init(&full[lane], 17); mbar_init(&empty[lane], 4); }
+    if (lane < C::QSLOTS) { mbar_init(&q_full[lane], 1); mbar_init(&q_empty[lane], CONSUMERS + 2); }
+    if (lane == 0) { mbar_init(o_full, CONSUMERS); mbar_init(o_empty, 1); }
+    fence_barrier_init();
+  } else if (threadIdx.x == C::CODES * 32) {
+    prefetch_tmap(&tmap);
   }
   __syncthreads();
-  // unit u = tile u - S of job (b, j), jobs in (b, j) order; this CTA takes units [u0, u1)
-  const long long T = static_cast<long long>(prefix[p.B]) * jobs_b;
-  const long long grid = min(static_cast<long long>(gridDim.x), (T + GROUPS - 1) / GROUPS);
-  if (blockIdx.x >= grid) return;
-  // divisions of whole 64-bit numbers take hundreds of cycles; up to 29 million tiles on 148 CTAs 32 bits hold every dividend
-  const bool narrow = (T + 1) * grid <= 0xffffffffll;
-  auto quotient = [&](long long a, long long d) -> long long {
-    return narrow ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(d)) : a / d;
-  };
-  const long long u0 = quotient(blockIdx.x * T, grid), u1 = quotient((blockIdx.x + 1) * T, grid);
-  int b = 0, len = 0, nt = 0, job = 0, t_beg = 0, t_end = 0;
-  long long s_job = 0;
-  {
-    int lo = 0, hi = p.B - 1;                  // last sequence whose first unit is <= u0
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<long long>(prefix[mid]) * jobs_b <= u0) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
-  }
-  // A piece: the tiles [t_beg, t_end) of a job that lie in this CTA's range. Producer and consumers walk over the same pieces.
-  auto locate = [&](long long u) {
-    long long s_b = 0;
-    for (;; ++b) {
-      len = lens[b];
-      nt = tiles_of(len);
-      s_b = static_cast<long long>(prefix[b]) * jobs_b;
-      if (u < s_b + static_cast<long long>(nt) * jobs_b) break;
-    }
-    const long long off = u - s_b;                       // below nt * jobs_b
-    job = static_cast<int>(quotient(off, nt));
-    s_job = s_b + static_cast<long long>(job) * nt;
-    t_beg = static_cast<int>(u - s_job);
-    t_end = static_cast<int>(min(static_cast<long long>(nt), t_beg + (u1 - u)));
-  };
+  pdl_trigger();
+  pdl_wait();
 
-  if (warp >= CONSUMERS) {
-    // ------------------------------ producers: one warp brings codes, one scales ------------------------------
-    const bool brings_codes = warp == CONSUMERS;
+  if (warp == C::CODES || warp == C::SCALES) {
+    // ------------------------------ producers: one warp brings queries and codes, one scales ------------------------------
+    const bool brings_codes = warp == C::CODES;
+    Deal deal;
+    if (brings_codes) {
+      const int cap = static_cast<int>(min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll - TK));
+      int base = 0;
+      for (int b0 = 0; b0 < p.B; b0 += 32) {
+        const int len = b0 + lane < p.B ? min(p.seq_len[b0 + lane], cap) : 0;
+        const int n = b0 + lane < p.B ? tiles_of(len) : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += v;
+        }
+        if (b0 + lane < p.B) { prefix[b0 + lane] = base + inc - n; lens[b0 + lane] = len; }
+        base += __shfl_sync(0xffffffffu, inc, 31);
+      }
+      deal.units = base * jobs_b;
+      deal.ctas = min(static_cast<int>(gridDim.x), (deal.units + GROUPS - 1) / GROUPS);
+      deal.each = deal.units / deal.ctas;
+      deal.more = deal.units - deal.each * deal.ctas;
+      if (lane == 0) { prefix[p.B] = base; s_deal = deal; }
+    }
+    asm volatile("bar.sync 3, 64;" ::: "memory");
+    deal = s_deal;
+    const bool idle = static_cast<int>(blockIdx.x) >= deal.ctas;
+    int left = idle ? 0 : deal.first(blockIdx.x + 1) - deal.first(blockIdx.x);              // units of the CTA to come
+    // the first piece: the last sequence whose first unit is not behind it, by steps of a 32nd of those left
+    const int u0 = idle ? 0 : deal.first(blockIdx.x);
+    int b = 0;
+    for (int n = p.B - 1; n > 0;) {
+      const int step = (n + 31) / 32, at = b + (lane + 1) * step;
+      const int c = __popc(__ballot_sync(0xffffffffu, at <= b + n && prefix[min(at, p.B)] * jobs_b <= u0));
+      b += c * step;
+      n = min(step - 1, n - c * step);
+    }
+    int len = lens[b], nt = tiles_of(len), start = prefix[b] * jobs_b, job = (u0 - start) / nt;
+    start += job * nt;
+    int t_beg = u0 - start, kvh = job / p.subs, sub = job - kvh * p.subs;
+
     const int box_bits = min(p.page_bits, 6), box = 1 << box_bits, nbx = TK >> box_bits;    // positions of a TMA box, boxes of a tile
     // of a tile, a lane has one box of codes of keys or values (eight boxes of each at most), or one scale, of eight positions
     const int v = brings_codes ? lane & 1 : (lane >> 3) & 1;
@@ -214,15 +237,32 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int step = v * p.Hkv * unit + (brings_codes ? 0 : (first & (box - 1)) >> p.block_bits);
     const int none = brings_codes ? p.n_blocks * 2 * p.Hkv * p.page : -1;                   // for ids outside the pool: a row behind the last one
     const int slot_bits = brings_codes ? 0 : p.block_bits;
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (long long u = u0; u < u1 && ok; u += t_end - t_beg) {
-      locate(u);
-      const int kvh = job / p.subs;
+    int stage = 0, q_slot = 0;
+    uint32_t phase = 0, q_phase = 0;
+    do {
+      const int t_end = min(nt, t_beg + left);
+      left -= t_end - t_beg;
+      if (brings_codes) {
+        if (!mbar_wait_warp(&q_empty[q_slot], q_phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) break;
+        if (lane == 0) {
+          const int h0 = kvh * p.G + sub * heads, live = min(heads, p.G - sub * heads);
+          Piece* to = pieces + q_slot;
+          to->b = b; to->h0 = h0; to->live = live; to->len = len;
+          to->t_beg = t_beg; to->t_end = t_end; to->nt = nt; to->last = left == 0;
+          to->start = start; to->counter = b * jobs_b + job;
+          mbar_arrive_expect_tx(&q_full[q_slot], idle ? 0 : live * DH * 2);
+          if (!idle)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(smem_u32(sm_q + q_slot * heads * DH)), "l"(p.q + b * p.ldq + static_cast<long long>(h0) * DH), "r"(live * DH * 2),
+                         "r"(smem_u32(&q_full[q_slot])) : "memory");
+        }
+        if (++q_slot == C::QSLOTS) { q_slot = 0; q_phase ^= 1; }
+      }
+      if (idle) break;
       const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
       int at_of_lane = -1;                               // of box (fetched + lane): its first row of keys, or their scale
       int fetched = -1000000;
+      bool ok = true;
       for (int t = t_beg; t < t_end; ++t) {
         const int bx0 = t * nbx;
         if (bx0 + nbx > fetched + 32) {                  // nbx divides 32: a tile's boxes are fetched together
@@ -235,15 +275,15 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           }
         }
         const int base = __shfl_sync(0xffffffffu, at_of_lane, bx0 + x - fetched);
-        const int at = base < 0 ? none : base + step, left = len - t * TK;                  // positions of the tile that exist, or more
+        const int at = base < 0 ? none : base + step, rest = len - t * TK;                  // positions of the tile that exist, or more
         if (!mbar_wait_warp(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
         if (brings_codes) {
-          const int live = left >= TK ? nbx : max(0, (left + box - 1) >> box_bits);         // boxes with a position that exists
+          const int live = rest >= TK ? nbx : max(0, (rest + box - 1) >> box_bits);         // boxes with a position that exists
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
           __syncwarp();
           if (x < live) tma_load_2d(ring + stage * 2 * C::TILE + v * C::TILE + first * DH, &tmap, &full[stage], 0, at);
         } else if (lane < 16) {
-          const bool real = first < left && at >= 0;
+          const bool real = first < rest && at >= 0;
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 16 + lane)), "l"(p.scales + (real ? at : 0)),
                        "r"(real ? 4 : 0) : "memory");
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
@@ -251,184 +291,233 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         __syncwarp();
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
-    }
+      if (!ok) break;
+      start += nt;                                       // the next job's
+      t_beg = 0;
+      if (++sub == p.subs) { sub = 0; ++kvh; }
+      if (++job == jobs_b) {
+        job = kvh = 0;
+        if (++b < p.B) { len = lens[b]; nt = tiles_of(len); }
+      }
+    } while (left > 0);
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
 
-  // ------------------------------ consumers -----------------------------
+  // ------------------------------ consumers, and finishers: these join the warps' sums of all pieces but the last -----------------------
+  const bool consumes = warp < CONSUMERS;
   const int quad = lane >> 2, tq = lane & 3, mi = lane >> 3;
   const int group = warp >> 2, pw = warp & 3;
   const int wrow = pw * 16 + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
   const int swz = DH == 128 ? (wrow & 7) : ((wrow >> 1) & 3);
-  long long it = 0;                          // tiles of the CTA before the piece
-  int stage = group;
-  uint32_t phase = 0;
+  const int team = consumes ? CONSUMERS * 32 : 64, tid = consumes ? threadIdx.x : threadIdx.x - C::FINISHERS * 32;
+  auto team_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(consumes ? 1 : 2), "r"(team) : "memory"); };
+  int stage = group, q_slot = 0;
+  uint32_t phase = 0, q_phase = 0, o_phase = 0;
   bool ok = true;
-  for (long long u = u0; u < u1;) {
-    locate(u);
-    const int h0 = (job / p.subs) * p.G + (job % p.subs) * heads, live = min(heads, p.G - (job % p.subs) * heads);
-    // q as B fragments: column `quad` is a query head; of a step of 16 dimensions the lane's four are 4 tq .. 4 tq + 3, as K's bytes come
-    uint32_t qb[NH][CHUNKS][2];
-    float qf[NH][2];
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      const int h = n * 8 + quad;
-      const __nv_bfloat16* src = p.q + b * p.ldq + static_cast<long long>(h0 + h) * DH + tq * 4;
-      uint32_t top = 0;
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const uint2 v = h < live ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
-        qb[n][c][0] = v.x;
-        qb[n][c][1] = v.y;
-        top = __vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
-      }
-      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 15u);               // the exponent of the largest, biased
-      const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);      // 2^(14 - (e - 127)), and back
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        qb[n][c][0] = half2_bits(bf16_lo(qb[n][c][0]) * up, bf16_hi(qb[n][c][0]) * up);
-        qb[n][c][1] = half2_bits(bf16_lo(qb[n][c][1]) * up, bf16_hi(qb[n][c][1]) * up);
-      }
-      const float f = down * p.scale_log2;
-      qf[n][0] = __shfl_sync(0xffffffffu, f, tq * 8);                                // of heads 2 tq and 2 tq + 1, the columns of a result
-      qf[n][1] = __shfl_sync(0xffffffffu, f, tq * 8 + 4);
-    }
-    float m[NH][2], l[NH][2], o[CHUNKS][NH][4];
-    float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
-#pragma unroll
-    for (int n = 0; n < NH; ++n) m[n][0] = m[n][1] = -1.0e30f, l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-      for (int n = 0; n < NH; ++n) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
-
-    for (int t = t_beg + static_cast<int>((group - it) & (GROUPS - 1)); t < t_end; t += GROUPS) {
-      const int st = stage;
-      const uint32_t ph = phase;
-      stage += GROUPS;
-      if (stage >= stages) { stage -= stages; phase ^= 1; }
-      if (ok && !mbar_wait_warp(&full[st], ph, p.status, ST_TIMEOUT_FULL)) ok = false;
-      if (!ok) continue;
-      const uint32_t kt = smem_u32(ring + st * 2 * C::TILE) + wrow * DH, vt = kt + C::TILE;
-      const float2 ks = *reinterpret_cast<const float2*>(sc + st * 16 + pw * 2), vs = *reinterpret_cast<const float2*>(sc + st * 16 + 8 + pw * 2);
-      const int valid = len - t * TK - pw * 16;                                      // positions of this warp's 16 that exist
-      float s[NH][4];
-#pragma unroll
-      for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < CHUNKS; c += 2) {
-        uint32_t r[4], a[4];
-        ldsm(kt + (((c + (mi >> 1)) ^ swz) << 4), r);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          widen<E4M3, false>(r[2 * i], a[0], a[2]);
-          widen<E4M3, false>(r[2 * i + 1], a[1], a[3]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma_f16(s[n], a[0], a[1], a[2], a[3], qb[n][c + i][0], qb[n][c + i][1]);
-        }
-      }
-      bool over = vs.x > vref || vs.y > vref;
+  int turn = group;                          // tiles of the next piece before the first that this group takes
+  for (bool last = false; !last;) {
+    if (!mbar_wait_warp(&q_full[q_slot], q_phase, p.status, ST_TIMEOUT_FULL)) return;
+    const Piece* piece = pieces + q_slot;                // the last one stays
+    const int t_beg = piece->t_beg, t_end = piece->t_end, len = piece->len, live = piece->live;
+    last = piece->last;
+    Piece to;
+    const __nv_bfloat16* my_q = sm_q + q_slot * heads * DH;
+    uint64_t* q_done = &q_empty[q_slot];
+    if (++q_slot == C::QSLOTS) { q_slot = 0; q_phase ^= 1; }
+    if (consumes) {
+      // q as B fragments: column `quad` is a query head; of a step of 16 dimensions the lane's four are 4 tq .. 4 tq + 3, as K's bytes come
+      uint32_t qb[NH][CHUNKS][2];
+      float qf[NH][2];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
+        const int h = n * 8 + quad;
+        const __nv_bfloat16* src = my_q + h * DH + tq * 4;
+        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[n][e] *= ks.x * qf[n][e];
-          s[n][2 + e] *= ks.y * qf[n][e];
-          if (valid < 16) {
-            if (quad >= valid) s[n][e] = -INFINITY;
-            if (quad + 8 >= valid) s[n][2 + e] = -INFINITY;
-          }
-          over |= s[n][e] - m[n][e] > 15.f || s[n][2 + e] - m[n][e] > 15.f;
+        for (int c = 0; c < CHUNKS; ++c) {
+          const uint2 v = h < live ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
+          qb[n][c][0] = v.x;
+          qb[n][c][1] = v.y;
+          top = __vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
         }
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 15u);               // the exponent of the largest, biased
+        const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);      // 2^(14 - (e - 127)), and back
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          qb[n][c][0] = half2_bits(bf16_lo(qb[n][c][0]) * up, bf16_hi(qb[n][c][0]) * up);
+          qb[n][c][1] = half2_bits(bf16_lo(qb[n][c][1]) * up, bf16_hi(qb[n][c][1]) * up);
+        }
+        const float f = down * p.scale_log2;
+        qf[n][0] = __shfl_sync(0xffffffffu, f, tq * 8);                                // of heads 2 tq and 2 tq + 1, the columns of a result
+        qf[n][1] = __shfl_sync(0xffffffffu, f, tq * 8 + 4);
       }
-      if (__any_sync(0xffffffffu, over)) {
-        const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
-        vref = v_new;
-        vinv = 1.f / v_new;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_done);
+      float m[NH][2], l[NH][2], o[CHUNKS][NH][4];
+      float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
+#pragma unroll
+      for (int n = 0; n < NH; ++n) m[n][0] = m[n][1] = -1.0e30f, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int n = 0; n < NH; ++n) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
+
+      int t = t_beg + turn;
+      for (; t < t_end; t += GROUPS) {
+        const int st = stage;
+        const uint32_t ph = phase;
+        stage += GROUPS;
+        if (stage >= stages) { stage -= stages; phase ^= 1; }
+        if (ok && !mbar_wait_warp(&full[st], ph, p.status, ST_TIMEOUT_FULL)) ok = false;
+        if (!ok) continue;
+        const uint32_t kt = smem_u32(ring + st * 2 * C::TILE) + wrow * DH, vt = kt + C::TILE;
+        const float2 ks = *reinterpret_cast<const float2*>(sc + st * 16 + pw * 2), vs = *reinterpret_cast<const float2*>(sc + st * 16 + 8 + pw * 2);
+        const int valid = len - t * TK - pw * 16;                                      // positions of this warp's 16 that exist
+        // the bytes of the warp's 16 positions go to registers, and the stage back to the producers
+        uint32_t rk[CHUNKS][2], rv[CHUNKS][2];
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c += 2) ldsm(kt + (((c + (mi >> 1)) ^ swz) << 4), rk[c], rk[c + 1]);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c += 2) ldsm_t(vt + (((c + (mi >> 1)) ^ swz) << 4), rv[c], rv[c + 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+        float s[NH][4], s1[NH][4];                                                     // two sums of products, so that they need not wait so long
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = s1[n][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          uint32_t a[4];
+          widen<E4M3, false>(rk[c][0], a[0], a[2]);
+          widen<E4M3, false>(rk[c][1], a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_f16(c & 1 ? s1[n] : s[n], a[0], a[1], a[2], a[3], qb[n][c][0], qb[n][c][1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] += s1[n][e];
+        bool over = vs.x > vref || vs.y > vref;
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(s[n][e], s[n][2 + e]) - 9.f;
+            s[n][e] *= ks.x * qf[n][e];
+            s[n][2 + e] *= ks.y * qf[n][e];
+            if (valid < 16) {
+              if (quad >= valid) s[n][e] = -INFINITY;
+              if (quad + 8 >= valid) s[n][2 + e] = -INFINITY;
+            }
+            over |= s[n][e] - m[n][e] > 15.f || s[n][2 + e] - m[n][e] > 15.f;
+          }
+        }
+        if (__any_sync(0xffffffffu, over)) {
+          const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
+          vref = v_new;
+          vinv = 1.f / v_new;
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float m_new = fmaxf(m[n][e], top), a = ex2(m[n][e] - m_new);
-            m[n][e] = m_new;
-            l[n][e] *= a;
+          for (int n = 0; n < NH; ++n) {
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-              o[c][n][e] *= a * v_ratio;
-              o[c][n][2 + e] *= a * v_ratio;
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[n][e], s[n][2 + e]) - 9.f;
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              const float m_new = fmaxf(m[n][e], top), a = ex2(m[n][e] - m_new);
+              m[n][e] = m_new;
+              l[n][e] *= a;
+#pragma unroll
+              for (int c = 0; c < CHUNKS; ++c) {
+                o[c][n][e] *= a * v_ratio;
+                o[c][n][2 + e] *= a * v_ratio;
+              }
             }
           }
         }
-      }
-      uint32_t w[NH][2];
-      {
-        const float v0 = vs.x * vinv, v1 = vs.y * vinv;
+        uint32_t w[NH][2];
+        {
+          const float v0 = vs.x * vinv, v1 = vs.y * vinv;
 #pragma unroll
-        for (int n = 0; n < NH; ++n) {
-          float e[4];
+          for (int n = 0; n < NH; ++n) {
+            float e[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[i] = ex2(s[n][i] - m[n][i & 1]);
-          l[n][0] += e[0] + e[2];
-          l[n][1] += e[1] + e[3];
-          w[n][0] = transpose8x8(half2_bits(e[0] * v0, e[1] * v0));
-          w[n][1] = transpose8x8(half2_bits(e[2] * v1, e[3] * v1));
+            for (int i = 0; i < 4; ++i) e[i] = ex2(s[n][i] - m[n][i & 1]);
+            l[n][0] += e[0] + e[2];
+            l[n][1] += e[1] + e[3];
+            w[n][0] = transpose8x8(half2_bits(e[0] * v0, e[1] * v0));
+            w[n][1] = transpose8x8(half2_bits(e[2] * v1, e[3] * v1));
+          }
+        }
+        // what lies behind the last position may be NaN, which a weight of zero does not make zero
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (E4M3 && valid < 16) {
+          keep0 = (2 * tq < valid ? 0xffffu : 0u) | (2 * tq + 1 < valid ? 0xffff0000u : 0u);
+          keep1 = (2 * tq + 8 < valid ? 0xffffu : 0u) | (2 * tq + 9 < valid ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          uint32_t a[4];
+          if (E4M3) { rv[c][0] &= keep0; rv[c][1] &= keep1; }
+          widen<E4M3, true>(rv[c][0], a[0], a[1]);
+          widen<E4M3, true>(rv[c][1], a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_f16(o[c][n], a[0], a[1], a[2], a[3], w[n][0], w[n][1]);
         }
       }
-      // what lies behind the last position may be NaN, which a weight of zero does not make zero
-      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-      if (E4M3 && valid < 16) {
-        keep0 = (2 * tq < valid ? 0xffffu : 0u) | (2 * tq + 1 < valid ? 0xffff0000u : 0u);
-        keep1 = (2 * tq + 8 < valid ? 0xffffu : 0u) | (2 * tq + 9 < valid ? 0xffff0000u : 0u);
-      }
-#pragma unroll
-      for (int c = 0; c < CHUNKS; c += 2) {
-        uint32_t r[4], a[4];
-        ldsm_t(vt + (((c + (mi >> 1)) ^ swz) << 4), r);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (E4M3) { r[2 * i] &= keep0; r[2 * i + 1] &= keep1; }
-          widen<E4M3, true>(r[2 * i], a[0], a[1]);
-          widen<E4M3, true>(r[2 * i + 1], a[2], a[3]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma_f16(o[c + i][n], a[0], a[1], a[2], a[3], w[n][0], w[n][1]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
-    }
-    it += t_end - t_beg;
-    u += t_end - t_beg;
+      turn = t - t_end;
 
-    // ---- the warps' sums are joined in the order of the warps ----
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int h = n * 8 + 2 * tq + e;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
-        if (h >= live) continue;
-        float* dst = sm_o + (warp * heads + h) * C::PITCH + 2 * quad;
+          for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+      if (ok && !mbar_wait_warp(o_empty, o_phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) ok = false;      // those of the piece before have been read
+      o_phase ^= 1;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float2*>(dst + c * 16) = make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
-        if (quad == 0) { sm_ml[(warp * heads + h) * 2] = m[n][e]; sm_ml[(warp * heads + h) * 2 + 1] = l[n][e]; }
+      for (int n = 0; n < NH; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int h = n * 8 + 2 * tq + e;
+          if (h >= live) continue;
+          float* dst = sm_o + (warp * heads + h) * C::PITCH + 2 * quad;
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float2*>(dst + c * 16) = make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
+          if (quad == 0) *reinterpret_cast<float2*>(sm_ml + (warp * heads + h) * 2) = make_float2(m[n][e], l[n][e]);
+        }
       }
+      if (!last) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_full);
+        continue;
+      }
+    } else {
+      to = *piece;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_done);
+      if (last) return;
+      if (!mbar_wait_warp(o_full, o_phase, p.status, ST_TIMEOUT_FULL)) return;
+      o_phase ^= 1;
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
-    const bool whole = t_beg == 0 && t_end == nt;
-    auto part_of = [&](long long c) { return p.part + static_cast<size_t>(c) * (HEADS_MAX * (DH + 2)); };
-    auto write_out = [&](int h, int d, float4 v, float sum) {
+    if (t_beg == t_end) return;                          // a CTA without units
+
+    if (consumes) to = *piece;
+    const bool whole = t_beg == 0 && t_end == to.nt;
+    const Deal deal = s_deal;
+    const int c0 = whole ? 0 : deal.cta(to.start), n_pieces = whole ? 1 : deal.cta(to.start + to.nt - 1) - c0 + 1;
+    auto part_of = [&](int c) { return p.part + static_cast<size_t>(c) * (HEADS_MAX * (DH + 2)); };
+    auto write_out = [&](int at, float4 v, float sum) {
       if (len > 0) { v.x /= sum; v.y /= sum; v.z /= sum; v.w /= sum; }
-      *reinterpret_cast<uint2*>(p.out + b * p.ldo + static_cast<long long>(h0 + h) * DH + d) =
+      *reinterpret_cast<uint2*>(p.out + to.b * p.ldo + static_cast<long long>(to.h0) * DH + at) =
           make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
     };
-    for (int i = threadIdx.x; i < live * (DH / 4); i += CONSUMERS * 32) {
+    const int items = live * (DH / 4);                   // of four values each
+    if (consumes) team_sync();
+    // ---- the warps' sums are joined in the order of the warps ----
+    for (int i = tid; i < items; i += team) {
       const int h = i / (DH / 4), d = i % (DH / 4) * 4;
       float top = -1.0e30f, sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -436,81 +525,92 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       for (int x = 0; x < CONSUMERS; ++x) top = fmaxf(top, sm_ml[(x * heads + h) * 2]);
 #pragma unroll
       for (int x = 0; x < CONSUMERS; ++x) {
-        const float a = ex2(sm_ml[(x * heads + h) * 2] - top);
+        const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (x * heads + h) * 2);
+        const float a = ex2(ml.x - top);
         const float4 e = *reinterpret_cast<const float4*>(sm_o + (x * heads + h) * C::PITCH + d);
-        sum += sm_ml[(x * heads + h) * 2 + 1] * a;
+        sum += ml.y * a;
         v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
       }
       if (whole) {
-        write_out(h, d, v, sum);
+        write_out(i * 4, v, sum);
       } else {
         float* dst = part_of(2 * blockIdx.x + (t_beg == 0));
-        *reinterpret_cast<float4*>(dst + h * DH + d) = v;
+        *reinterpret_cast<float4*>(dst + i * 4) = v;
         if (d == 0) *reinterpret_cast<float2*>(dst + HEADS_MAX * DH + 2 * h) = make_float2(top, sum);
       }
     }
-    if (whole) {
-      asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
-      continue;
-    }
+    if (whole && last) return;
+    team_sync();
+    if (!consumes && tid == 0) mbar_arrive(o_empty);
+    if (whole) continue;
     // ---- the CTA that ends last joins the pieces, in the order of the tiles ----
-    const long long c0 = quotient((s_job + 1) * grid - 1, T);
-    const int pieces = static_cast<int>(quotient((s_job + nt) * grid - 1, T) - c0) + 1;
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
-    if (threadIdx.x == 0) {
-      __threadfence();
-      unsigned int* ctr = p.counters + static_cast<size_t>(b) * jobs_b + job;
-      s_last = atomicAdd(ctr, 1u) == static_cast<unsigned int>(pieces) - 1;
-      if (s_last) *ctr = 0;
-      __threadfence();
+    if (tid == 0) {
+      unsigned int before;
+      asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + to.counter) : "memory");
+      s_last[consumes] = before == static_cast<unsigned int>(n_pieces) - 1;
+      if (s_last[consumes]) p.counters[to.counter] = 0;
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
-    if (!s_last) continue;
-    // weights of the pieces: a warp for each head
-    auto piece = [&](int i) { return part_of(2 * (c0 + i) + (i == 0)); };
-    float* sm_a = sm_o;                                          // [heads][pieces], then [sets][heads][DH] of values
-    float* sm_v = sm_o + ((heads * pieces + 3) & ~3);
-    for (int h = warp; h < live; h += CONSUMERS) {
+    team_sync();
+    if (!s_last[consumes]) continue;
+    const int sets = consumes ? min(C::SETS, max(1, team / items)) : 1;      // the sums have been read, by the consumers of the last piece anyway
+    float* sm_v = sm_o;                                                      // [sets][live][DH], then [sets][live][2]
+    float* sm_vml = sm_o + sets * live * DH;
+    for (int i = tid; i < items * sets; i += team) {
+      int set = 0, at = i;
+      while (at >= items) { at -= items; ++set; }
+      const int h = at / (DH / 4);
       float top = -1.0e30f, sum = 0.f;
-      for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(piece(i) + HEADS_MAX * DH + 2 * h));
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      for (int i = lane; i < pieces; i += 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(i) + HEADS_MAX * DH + 2 * h));
-        const float a = ex2(ml.x - top);
-        sm_a[h * pieces + i] = a;
-        sum += ml.y * a;
-      }
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (lane == 0) sm_ml[h] = sum;
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
-    const int items = live * (DH / 4), sets = min(C::SETS, max(1, CONSUMERS * 32 / items));
-    for (int i = threadIdx.x; i < items * sets; i += CONSUMERS * 32) {
-      const int set = i / items, at = (i - set * items) * 4, h = at / DH;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int c = set; c < pieces; c += sets) {
-        const float4 e = __ldcg(reinterpret_cast<const float4*>(piece(c) + at));
-        const float a = sm_a[h * pieces + c];
+      for (int c = set; c < n_pieces; c += 8 * sets) {   // the loads of eight pieces are under way together
+        float2 ml[8];
+        float4 e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at_c = c + k * sets;
+          ml[k] = make_float2(-1.0e30f, 0.f);
+          if (at_c >= n_pieces) continue;
+          const float* src = part_of(2 * (c0 + at_c) + (at_c == 0));
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(src + HEADS_MAX * DH + 2 * h));
+          e[k] = __ldcg(reinterpret_cast<const float4*>(src + at * 4));
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) now = fmaxf(now, ml[k].x);
+        const float keep = ex2(top - now);
+        top = now;
+        sum *= keep;
+        v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (c + k * sets >= n_pieces) continue;
+          const float a = ex2(ml[k].x - top);
+          sum += ml[k].y * a;
+          v.x += e[k].x * a; v.y += e[k].y * a; v.z += e[k].z * a; v.w += e[k].w * a;
+        }
+      }
+      if (sets == 1) {
+        write_out(at * 4, v, sum);
+      } else {
+        *reinterpret_cast<float4*>(sm_v + (set * items + at) * 4) = v;
+        if (at % (DH / 4) == 0) *reinterpret_cast<float2*>(sm_vml + (set * live + h) * 2) = make_float2(top, sum);
+      }
+    }
+    if (sets == 1) continue;
+    team_sync();
+    if (tid < items) {
+      const int h = tid / (DH / 4);
+      float top = -1.0e30f, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x = 0; x < sets; ++x) top = fmaxf(top, sm_vml[(x * live + h) * 2]);
+      for (int x = 0; x < sets; ++x) {
+        const float2 ml = *reinterpret_cast<const float2*>(sm_vml + (x * live + h) * 2);
+        const float a = ex2(ml.x - top);
+        const float4 e = *reinterpret_cast<const float4*>(sm_v + (x * items + tid) * 4);
+        sum += ml.y * a;
         v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
       }
-      if (sets == 1) write_out(h, at % DH, v, sm_ml[h]);
-      else *reinterpret_cast<float4*>(sm_v + set * heads * DH + at) = v;
+      write_out(tid * 4, v, sum);
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
-    if (sets == 1) continue;
-    if (threadIdx.x < items) {
-      const int at = threadIdx.x * 4, h = at / DH;
-      float4 v = *reinterpret_cast<const float4*>(sm_v + at);
-      for (int x = 1; x < sets; ++x) {
-        const float4 e = *reinterpret_cast<const float4*>(sm_v + x * heads * DH + at);
-        v.x += e.x; v.y += e.y; v.z += e.z; v.w += e.w;
-      }
-      write_out(h, at % DH, v, sm_ml[h]);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
   }
 }
 
@@ -519,8 +619,8 @@ static int launch_attend(const CUtensorMap& tm, AttendParams p, int grid, cudaSt
   using C = Cfg<DH, NH>;
   static PerDeviceOnce attr;
   if (allow_smem(attr, attend_kernel<DH, E4M3, NH>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
-  p.stages = C::stages(p.heads);
-  return launch_dep(attend_kernel<DH, E4M3, NH>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.heads), s, tm, p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  p.stages = C::stages(p.heads, p.B);
+  return launch_dep(attend_kernel<DH, E4M3, NH>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.heads, p.B), s, tm, p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 }  // namespace kv8
@@ -558,12 +658,13 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   p.B = B; p.Hkv = Hkv; p.G = H / Hkv;
   p.subs = (p.G + kv8::HEADS_MAX - 1) / kv8::HEADS_MAX;
   p.heads = (p.G + p.subs - 1) / p.subs;
+  if (static_cast<double>(B) * ((static_cast<double>(max_blocks) * page + kv8::TK - 1) / kv8::TK) * Hkv * p.subs > 2147483647.0) return SB_ERR_TOO_LARGE;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = part; p.counters = counters;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.status = status;
-  // a tile for each group of consumers at least
-  const long long want = (max_tiles + 3) / 4;
+  // the kernel leaves a tile to each group of consumers
+  const long long want = (max_tiles + 1) / 2;
   const int most = num_sms() < kv8::GRID_MAX ? num_sms() : kv8::GRID_MAX, grid = want < most ? static_cast<int>(want) : most;
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   const bool two = p.heads > 8;

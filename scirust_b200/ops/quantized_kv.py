@@ -370,8 +370,10 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     if n_blocks * 2 * Hkv * page >= (1 << 31) - TILE:
         raise ValueError("decode_attention: more rows of codes than 31 bits count")
     tiles = -(-max_blocks * page // TILE)                       # of a sequence, at most
-    at_once = min(B, LAUNCH_SEQUENCES, ((1 << 31) - 1) // tiles)
     jobs = Hkv * -(-(H // Hkv) // JOB_HEADS)
+    at_once = min(B, LAUNCH_SEQUENCES, ((1 << 31) - 1) // (tiles * jobs))
+    if at_once == 0:
+        raise ValueError("decode_attention: a table of more tiles and heads than 31 bits count")
     if max_len is not None:
         tiles = min(tiles, max(1, -(-int(max_len) // TILE)))
     stream = _lib.stream()
