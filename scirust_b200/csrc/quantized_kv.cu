@@ -15,13 +15,16 @@
 #include "sm100_ptx.cuh"
 
 namespace sb {
+int num_sms();                                                                 // gemm_tcgen05.cu
+
 namespace kv8 {
 
 // ---- writing -------------------------------------------------------------------------------------------------------------------
-// A warp takes one head of a chunk of rows and walks over the blocks of positions that begin in it; a block's rows that reach into the next
-// chunk are its own. Which sequence and position a row has follows from cu_q and seq_len, so that no two warps can write one block.
-// Sixteen rows at a time stay in registers between the maximum and the codes; of larger blocks the rows are read twice, the second time
-// from L2.
+// A warp takes one key or value head of a chunk of rows (or several, where there are more than enough warps) and walks over the blocks of
+// positions that begin in it; a block's rows that reach into the next chunk are its own. Which sequence and position a row has follows from cu_q and seq_len, so that no two warps can write one
+// block. Sixteen rows at a time stay in registers between the maximum and the codes; of larger blocks the rows are read twice, the second
+// time from L2. Query heads are only turned: a warp has one row, or as many as fill it, with their part of the rotation's table in registers
+// for a quarter of the heads.
 // Bound by memory for prompts and by latency for single tokens.
 constexpr int WARPS = 4;
 
@@ -34,6 +37,7 @@ struct AppendParams {
   const int* table; int max_blocks;
   const int *seq_len, *cu_q;                   // cu_q null: row b is sequence b's only one
   int B, chunk;
+  int head_ctas, kv_ctas;                      // CTAs of a chunk's key and value heads, and of all chunks; queries' CTAs come behind
 };
 
 // The sequence that row t belongs to: how many of cu[1 .. B] are at most t, by steps of a 32nd of what is left.
@@ -62,7 +66,8 @@ __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d)
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
            static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16;
   } else {
-    auto code = [](float x) { return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f))); };
+    // 1.5 * 2^23 + x is rounded to a whole number, whose last byte is x's (a conversion takes four times as long)
+    auto code = [](float x) { return __float_as_uint(fminf(fmaxf(x, -127.f), 127.f) + 12582912.f); };
     return __byte_perm(__byte_perm(code(a), code(b), 0x0040), __byte_perm(code(c), code(d), 0x0040), 0x5410);
   }
 }
@@ -78,17 +83,77 @@ __device__ __forceinline__ float scale_for(uint32_t bits) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-template <int DH, bool E4M3>
-__global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int LANES = DH / 8, ROWS = 32 / LANES, WORDS = 16 / ROWS;          // lanes of a row, rows of a load, loads of 16 rows
+struct Place { int rows, pos; };               // rows of a sequence from some row on, the first one's position; rows 0: that has no place
+
+// Where row t of sequence b is, which its first row is not behind and which has more.
+__device__ __forceinline__ Place place_of(const AppendParams& p, int b, int t, int stop, int& skip) {
+  const int rows = min(stop, p.n) - t;
+  const long long at = static_cast<long long>(p.seq_len[b]) - (stop - t);
+  long long limit = min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll);
+  if (p.cos_t) limit = min(limit, static_cast<long long>(p.n_pos));
+  if (at < 0 || at >= limit) {
+    skip = at < 0 ? static_cast<int>(min(-at, static_cast<long long>(rows))) : rows;
+    return {0, 0};
+  }
+  return {min(rows, static_cast<int>(limit - at)), static_cast<int>(at)};
+}
+
+__device__ __forceinline__ uint4 rotate8(uint4 v, const float4& c, const float4& s) {
+  return make_uint4(rotate(v.x, c.x, s.x), rotate(v.y, c.y, s.y), rotate(v.z, c.z, s.z), rotate(v.w, c.w, s.w));
+}
+
+template <int DH>
+__device__ __forceinline__ void turn_queries(const AppendParams& p, int cta) {
+  constexpr int LANES = DH / 8, ROWS = 32 / LANES, AHEAD = 8;                  // lanes of a row, rows of a warp, heads under way
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, ch = lane % LANES;
+  const int t0 = cta * ROWS, t = t0 + sub;
+  __nv_bfloat16* x = p.qkv + min(t, p.n - 1) * p.ld + ch * 8;
+  uint4 v[AHEAD];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (h0 + i * WARPS < p.H) v[i] = *reinterpret_cast<const uint4*>(x + (h0 + i * WARPS) * DH);
+  };
+  load(warp);                                  // while the row's place is looked for
+  int b = p.cu_q ? find_sequence(p.cu_q, p.B, t0) : t;
+  if (t >= p.n) return;
+  int stop = t + 1;
+  if (p.cu_q) {
+    while (b < p.B && p.cu_q[b + 1] <= t) ++b;
+    if (b >= p.B || t < p.cu_q[b]) return;
+    stop = p.cu_q[b + 1];
+  } else if (b >= p.B) {
+    return;
+  }
+  int skip;
+  const Place at = place_of(p, b, t, stop, skip);
+  if (at.rows == 0) return;
+  const size_t a = static_cast<size_t>(at.pos) * (DH / 2) + ch * 4;
+  const float4 c = *reinterpret_cast<const float4*>(p.cos_t + a), s = *reinterpret_cast<const float4*>(p.sin_t + a);
+  for (int h0 = warp;;) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (h0 + i * WARPS < p.H) *reinterpret_cast<uint4*>(x + (h0 + i * WARPS) * DH) = rotate8(v[i], c, s);
+    h0 += WARPS * AHEAD;
+    if (h0 >= p.H) break;
+    load(h0);
+  }
+}
+
+// BATCH: rows at a time, 8 for blocks of 8 and else 16
+template <int DH, bool E4M3, int BATCH>
+__global__ void __launch_bounds__(WARPS * 32, 6) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int LANES = DH / 8, ROWS = 32 / LANES, WORDS = BATCH / ROWS;       // lanes of a row, rows of a load, loads of a batch
   pdl_trigger();
   pdl_wait();
+  if (static_cast<int>(blockIdx.x) >= p.kv_ctas) {
+    turn_queries<DH>(p, blockIdx.x - p.kv_ctas);
+    return;
+  }
   const int lane = threadIdx.x & 31, sub = lane / LANES, ch = lane % LANES;
-  const int head = blockIdx.y * WARPS + (threadIdx.x >> 5) + (p.cos_t ? 0 : p.H);
-  if (head >= p.H + 2 * p.Hkv) return;
-  const bool is_q = head < p.H, turns = p.cos_t && head < p.H + p.Hkv;
-  const int kv = head >= p.H + p.Hkv, h = head - p.H - kv * p.Hkv;
-  int t = blockIdx.x * p.chunk;
+  const int chunk = blockIdx.x / p.head_ctas, first_head = (blockIdx.x - chunk * p.head_ctas) * WARPS + (threadIdx.x >> 5);
+  if (first_head >= 2 * p.Hkv) return;
+  int t = chunk * p.chunk;
   const int end = min(p.n - t, p.chunk) + t;
   int b = p.cu_q ? find_sequence(p.cu_q, p.B, t) : t;
   while (t < end) {
@@ -103,94 +168,85 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
       b = t;
       if (b >= p.B) return;
     }
-    const int rows = min(stop, p.n) - t;
-    const long long at = static_cast<long long>(p.seq_len[b]) - (stop - t);
-    long long limit = min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll);
-    if (p.cos_t) limit = min(limit, static_cast<long long>(p.n_pos));
-    if (at < 0 || at >= limit) {
-      t += static_cast<int>(at < 0 ? min(-at, static_cast<long long>(rows)) : rows);
-      continue;
-    }
-    const int pos = static_cast<int>(at), off = pos & (p.block - 1);
-    int cnt = min(min(p.block - off, rows), static_cast<int>(limit - pos));
-    const int t0 = t;
+    int skip;
+    const Place place = place_of(p, b, t, stop, skip);
+    if (place.rows == 0) { t += skip; continue; }
+    const int pos = place.pos, off = pos & (p.block - 1), cnt = min(p.block - off, place.rows), t0 = t;
     t += cnt;
-    if (is_q) cnt = min(cnt, end - t0);
-    else if (off && t0 != start) continue;                                     // a block that began in an earlier chunk
+    if (off && t0 != start) continue;                                          // a block that began in an earlier chunk
 
-    __nv_bfloat16* x = p.qkv + t0 * p.ld + head * DH + ch * 8;
-    uint4 v[WORDS];
-    auto load = [&](int r0) {
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) {
-        const int r = r0 + i * ROWS + sub;
-        v[i] = r < cnt ? *reinterpret_cast<const uint4*>(x + r * p.ld) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    uint32_t top = 0;
-    for (int r0 = 0; r0 < cnt; r0 += 16) {
-      load(r0);
-      if (turns) {
+    const int at = pos / p.page, slot = pos - at * p.page, id = p.table[static_cast<size_t>(b) * p.max_blocks + at];
+    const bool known = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
+    for (int head = first_head; head < 2 * p.Hkv; head += p.head_ctas * WARPS) {
+      const int kv = head >= p.Hkv, h = head - kv * p.Hkv;
+      const bool turns = p.cos_t && !kv;
+      __nv_bfloat16* x = p.qkv + (t0 + sub) * p.ld + (p.H + head) * DH + ch * 8;
+      uint4 v[WORDS];
+      auto load = [&](int r0) {
 #pragma unroll
         for (int i = 0; i < WORDS; ++i) {
-          const int r = r0 + i * ROWS + sub;
-          if (r >= cnt) continue;
-          const size_t a = static_cast<size_t>(pos + r) * (DH / 2) + ch * 4;
-          const float4 c = *reinterpret_cast<const float4*>(p.cos_t + a), s = *reinterpret_cast<const float4*>(p.sin_t + a);
-          v[i] = make_uint4(rotate(v[i].x, c.x, s.x), rotate(v[i].y, c.y, s.y), rotate(v[i].z, c.z, s.z), rotate(v[i].w, c.w, s.w));
-          *reinterpret_cast<uint4*>(x + r * p.ld) = v[i];
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r0 + i * ROWS + sub < cnt) v[i] = *reinterpret_cast<const uint4*>(x + (r0 + i * ROWS) * p.ld);
         }
+      };
+      load(0);
+      // while the rows are under way: the scale of what the block holds
+      const size_t row = (static_cast<size_t>(known ? id : 0) * 2 + kv) * p.Hkv + h;
+      float* scale_at = p.scales + row * (p.page / p.block) + slot / p.block;
+      const float old = off && known ? *scale_at : 0.f;
+      uint32_t top = 0;
+      for (int r0 = 0; r0 < cnt; r0 += BATCH) {
+        if (r0) load(r0);
+        if (turns) {
+          const size_t a = static_cast<size_t>(pos + r0 + sub) * (DH / 2) + ch * 4;
+#pragma unroll
+          for (int i = 0; i < WORDS; ++i) {
+            const bool in = r0 + i * ROWS + sub < cnt;
+            float4 c = make_float4(0, 0, 0, 0), s = c;
+            if (in) c = *reinterpret_cast<const float4*>(p.cos_t + a + i * ROWS * (DH / 2)), s = *reinterpret_cast<const float4*>(p.sin_t + a + i * ROWS * (DH / 2));
+            v[i] = rotate8(v[i], c, s);
+            if (in) *reinterpret_cast<uint4*>(x + (r0 + i * ROWS) * p.ld) = v[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i)
+          top = max16x2(top, max16x2(max16x2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), max16x2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
       }
+      if (!known) continue;
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i)
-        top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
-    }
-    if (is_q) continue;
+      for (int o = 1; o < 32; o <<= 1) top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = max(top & 0xffffu, top >> 16);
+      const float need = scale_for<E4M3>(top);
+      const float scale = off && (old > need || old != old) ? old : need;
+      if (lane == 0) *scale_at = scale;                                          // all lanes have read it: they have met since
+      const bool holds = scale == scale;
+      const float inv = 1.f / scale;
+      uint8_t* dst = p.codes + (row * p.page + slot) * DH;
+      for (int r0 = 0; r0 < cnt; r0 += BATCH) {
+        if (cnt > BATCH) load(r0);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top = max(top & 0xffffu, top >> 16);
-
-    const int id = p.table[static_cast<size_t>(b) * p.max_blocks + pos / p.page];
-    if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.n_blocks)) continue;
-    const int slot = pos % p.page;
-    const size_t row = (static_cast<size_t>(id) * 2 + kv) * p.Hkv + h;
-    float* scale_at = p.scales + row * (p.page / p.block) + slot / p.block;
-    uint8_t* dst = p.codes + (row * p.page + slot) * DH;
-    float scale = scale_for<E4M3>(top), old = scale;
-    if (off) {
-      old = *scale_at;
-      if (old > scale || old != old) scale = old;
-    }
-    __syncwarp();                                                              // all lanes have read it
-    if (lane == 0) *scale_at = scale;
-    const bool holds = scale == scale;
-    const float inv = 1.f / scale;
-    for (int r0 = 0; r0 < cnt; r0 += 16) {
-      if (cnt > 16) load(r0);
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) {
-        const int r = r0 + i * ROWS + sub;
-        if (r >= cnt) continue;
-        uint2 c = make_uint2(0, 0);
-        if (holds) {
+        for (int i = 0; i < WORDS; ++i) {
+          uint2 c;
           c.x = to_codes<E4M3>(bf16_lo(v[i].x) * inv, bf16_hi(v[i].x) * inv, bf16_lo(v[i].y) * inv, bf16_hi(v[i].y) * inv);
           c.y = to_codes<E4M3>(bf16_lo(v[i].z) * inv, bf16_hi(v[i].z) * inv, bf16_lo(v[i].w) * inv, bf16_hi(v[i].w) * inv);
+          if (!holds) c = make_uint2(0, 0);
+          if (r0 + i * ROWS + sub < cnt) *reinterpret_cast<uint2*>(dst + (r0 + i * ROWS + sub) * DH + ch * 8) = c;
         }
-        *reinterpret_cast<uint2*>(dst + r * DH + ch * 8) = c;
       }
-    }
-    if (off && holds && old != scale) {                                        // what the block holds, in the new steps
-      const float ratio = old * inv;
-      uint4* before = reinterpret_cast<uint4*>(dst - off * DH);
-      for (int i = lane; i < off * (DH / 16); i += 32) {
-        uint4 w = before[i];
-        uint32_t* e = &w.x;
+      if (off && holds && old != scale) {                                        // what the block holds, in the new steps
+        const float ratio = old * inv;
+        uint4* before = reinterpret_cast<uint4*>(dst - off * DH);
+#pragma unroll 4
+        for (int i = lane; i < off * (DH / 16); i += 32) {
+          uint4 w = before[i];
+          uint32_t* e = &w.x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 f = from_codes<E4M3>(e[j]);
-          e[j] = to_codes<E4M3>(f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio);
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = from_codes<E4M3>(e[j]);
+            e[j] = to_codes<E4M3>(f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio);
+          }
+          before[i] = w;
         }
-        before[i] = w;
       }
     }
   }
@@ -256,10 +312,19 @@ extern "C" int sb_quant_kv_append(void* qkv, long long ld, int n, int H, int Hkv
   p.codes = static_cast<uint8_t*>(codes); p.scales = scales;
   p.n_blocks = n_blocks; p.page = page; p.block = block;
   p.table = table; p.max_blocks = max_blocks; p.seq_len = seq_len; p.cu_q = cu_q; p.B = B; p.chunk = chunk;
-  const int heads = (cos_t ? H : 0) + 2 * Hkv;
-  const dim3 grid((n + chunk - 1) / chunk, (heads + kv8::WARPS - 1) / kv8::WARPS);
-  auto kern = dh == 64 ? (e4m3 ? kv8::append_kernel<64, true> : kv8::append_kernel<64, false>)
-                       : (e4m3 ? kv8::append_kernel<128, true> : kv8::append_kernel<128, false>);
+  const long long chunks = (static_cast<long long>(n) + chunk - 1) / chunk, rows = 256 / dh;                     // rows of a warp of queries
+  // A warp finds its place by five loads, each of which waits for the one before: beyond two rounds of CTAs it takes more heads with that.
+  const long long most = (2 * Hkv + kv8::WARPS - 1) / kv8::WARPS, rounds = chunks * most / (num_sms() * 12ll);
+  p.head_ctas = static_cast<int>(rounds < 2 ? most : rounds < most ? (most + rounds - 1) / rounds : 1);
+  const long long kv_ctas = chunks * p.head_ctas, ctas = kv_ctas + (cos_t && H ? (n + rows - 1) / rows : 0);
+  if (ctas > 0x7fffffffll) return SB_ERR_TOO_LARGE;
+  p.kv_ctas = static_cast<int>(kv_ctas);
+  const dim3 grid(static_cast<unsigned>(ctas));
+  using Kernel = void (*)(kv8::AppendParams);
+  static const Kernel kernels[8] = {kv8::append_kernel<64, false, 16>, kv8::append_kernel<64, false, 8>, kv8::append_kernel<64, true, 16>,
+                                    kv8::append_kernel<64, true, 8>, kv8::append_kernel<128, false, 16>, kv8::append_kernel<128, false, 8>,
+                                    kv8::append_kernel<128, true, 16>, kv8::append_kernel<128, true, 8>};
+  const Kernel kern = kernels[(dh == 128) * 4 + (e4m3 != 0) * 2 + (block == 8)];
   return launch_dep(kern, grid, dim3(kv8::WARPS * 32), 0, static_cast<cudaStream_t>(stream_), p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 

@@ -7,6 +7,13 @@
 namespace sb {
 namespace kv8 {
 
+// The larger ones of two pairs of 16-bit numbers.
+__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
 // Four codes as numbers.
 template <bool E4M3>
 __device__ __forceinline__ float4 from_codes(uint32_t w) {

@@ -184,6 +184,12 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   }
   __syncthreads();
   pdl_trigger();
+  {
+    // lengths and tables are the first things read, one after the other: L2 has them when they are
+    const size_t line = (static_cast<size_t>(blockIdx.x) * C::THREADS + threadIdx.x) * 128, bytes = static_cast<size_t>(p.B) * 4;
+    if (line < bytes * p.max_blocks) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.table) + line));
+    if (line < bytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.seq_len) + line));
+  }
   pdl_wait();
 
   if (warp == C::CODES || warp == C::SCALES) {
@@ -193,8 +199,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     if (brings_codes) {
       const int cap = static_cast<int>(min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll - TK));
       int base = 0;
+      int next = lane < p.B ? p.seq_len[lane] : 0;
       for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const int len = b0 + lane < p.B ? min(p.seq_len[b0 + lane], cap) : 0;
+        const int len = min(next, cap);
+        next = b0 + 32 + lane < p.B ? p.seq_len[b0 + 32 + lane] : 0;
         const int n = b0 + lane < p.B ? tiles_of(len) : 0;
         int inc = n;
 #pragma unroll
@@ -226,7 +234,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     }
     int len = lens[b], nt = tiles_of(len), start = prefix[b] * jobs_b, job = (u0 - start) / nt;
     start += job * nt;
-    int t_beg = u0 - start, kvh = job / p.subs, sub = job - kvh * p.subs;
+    int t_beg = u0 - start, kvh = p.subs == 1 ? job : job / p.subs, sub = job - kvh * p.subs;
 
     const int box_bits = min(p.page_bits, 6), box = 1 << box_bits, nbx = TK >> box_bits;    // positions of a TMA box, boxes of a tile
     // of a tile, a lane has one box of codes of keys or values (eight boxes of each at most), or one scale, of eight positions
@@ -339,10 +347,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           const uint2 v = h < live ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
           qb[n][c][0] = v.x;
           qb[n][c][1] = v.y;
-          top = __vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+          top = max16x2(top, max16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
         }
-        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 15u);               // the exponent of the largest, biased
         const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);      // 2^(14 - (e - 127)), and back
 #pragma unroll
@@ -510,7 +518,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int c0 = whole ? 0 : deal.cta(to.start), n_pieces = whole ? 1 : deal.cta(to.start + to.nt - 1) - c0 + 1;
     auto part_of = [&](int c) { return p.part + static_cast<size_t>(c) * (HEADS_MAX * (DH + 2)); };
     auto write_out = [&](int at, float4 v, float sum) {
-      if (len > 0) { v.x /= sum; v.y /= sum; v.z /= sum; v.w /= sum; }
+      const float inv = len > 0 ? 1.f / sum : 0.f;
+      v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
       *reinterpret_cast<uint2*>(p.out + to.b * p.ldo + static_cast<long long>(to.h0) * DH + at) =
           make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
     };
@@ -521,9 +530,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       const int h = i / (DH / 4), d = i % (DH / 4) * 4;
       float top = -1.0e30f, sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
+#pragma unroll 4
       for (int x = 0; x < CONSUMERS; ++x) top = fmaxf(top, sm_ml[(x * heads + h) * 2]);
-#pragma unroll
+#pragma unroll 4                             // code that runs once comes from L2: short loops are faster than long straight lines
       for (int x = 0; x < CONSUMERS; ++x) {
         const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (x * heads + h) * 2);
         const float a = ex2(ml.x - top);

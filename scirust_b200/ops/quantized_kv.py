@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from . import gemm as _g
 
-BF = torch.bfloat16
+BF, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 vp, i32, i64, f32 = _lib.vp, _lib.i32, _lib.i64, _lib.f32
 _lib.register("sb_quant_kv_append", [vp, i64, i32, i32, i32, i32, vp, vp, i32, vp, i32, vp, i32, i32, i32, vp, i32, vp, vp, i32, i32, vp])
 _lib.register("sb_quant_kv_read", [vp, i32, vp, i32, i32, i32, i32, i32, vp, i32, vp, vp])
@@ -60,44 +60,45 @@ class QuantPool(NamedTuple):
 def _layout(what, pool, Hkv=None, dh=None):
     """(codes, scales, n_blocks, Hkv, page, dh, block) of a pool, or ValueError."""
     codes, scales = pool
-    if codes.dim() != 5 or scales.dim() != 4:
+    shape, per_block = codes.shape, scales.shape
+    if len(shape) != 5 or len(per_block) != 4 or shape[:3] != per_block[:3] or shape[1] != 2 or (Hkv is not None and (shape[2] != Hkv or shape[4] != dh)):
         raise ValueError(f"{what}: pool must be codes [n_blocks, 2, Hkv, page, dh] and scales [n_blocks, 2, Hkv, page / block]")
-    n_blocks, two, heads, page, width = codes.shape
-    sn, s2, sh, per_page = scales.shape
-    if two != 2 or s2 != 2 or sn != n_blocks or sh != heads or (Hkv is not None and (heads != Hkv or width != dh)):
-        raise ValueError(f"{what}: pool must be codes [n_blocks, 2, Hkv, page, dh] and scales [n_blocks, 2, Hkv, page / block]")
-    block = page // per_page if per_page else 0
-    if block not in BLOCKS or block * per_page != page:
+    n_blocks, _, heads, page, width = shape
+    block = page // per_block[3] if per_block[3] else 0
+    if block not in BLOCKS or block * per_block[3] != page:
         raise ValueError(f"{what}: a scale for each 8, 16, 32 or 64 positions, which divide the page")
-    if codes.dtype not in LARGEST or scales.dtype is not torch.float32:
+    if codes.dtype not in LARGEST or scales.dtype is not F32:
         raise ValueError(f"{what}: codes must be int8 or float8_e4m3fn, scales fp32")
-    if codes.device != scales.device:
+    if codes.get_device() != scales.get_device():
         raise ValueError(f"{what}: codes and scales must be on one device")
     return codes, scales, n_blocks, heads, page, width, block
 
 
-def _on_device(what, device, codes, scales, dh, tensors):
-    """What the kernels ask of a pool and of the int32 tensors beside it, whose addresses they are given."""
+def _on_device(what, index, codes, scales, dh, tensors):
+    """What the kernels ask of a pool and of the int32 tensors beside it, whose addresses they are given: the codes' address."""
     if dh != 64 and dh != 128:
         raise ValueError(f"{what}: head dimension 64 or 128")
-    if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
+    at = codes.data_ptr()
+    if not codes.is_contiguous() or not scales.is_contiguous() or at % 16:
         raise ValueError(f"{what}: codes and scales must be contiguous, codes 16-byte aligned")
-    if codes.get_device() != device.index:
+    if codes.get_device() != index:
         raise ValueError(f"{what}: all tensors must be on one device")
     for t in tensors:
-        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != device.index):
+        if t.dtype is not I32 or t.get_device() != index or not t.is_contiguous():
             raise ValueError(f"{what}: tables, lengths, offsets and page ids must be contiguous, int32 and on the pool's device")
+    return at
 
 
 def _batch(what, n, seq_len, block_table, cu_q):
-    if seq_len.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != seq_len.shape[0]:
+    lens, table = seq_len.shape, block_table.shape
+    if len(lens) != 1 or len(table) != 2 or table[0] != lens[0]:
         raise ValueError(f"{what}: seq_len [B] and block_table [B, pages]")
-    B = seq_len.shape[0]
-    if B and not block_table.shape[1]:
+    B, max_blocks = table
+    if B and not max_blocks:
         raise ValueError(f"{what}: block_table has no pages")
     if n != B if cu_q is None else tuple(cu_q.shape) != (B + 1,):
         raise ValueError(f"{what}: one row a sequence, or rows counted by cu_q [B + 1]")
-    return B, block_table.shape[1]
+    return B, max_blocks
 
 
 # ---------------------------------------------------------------------------------------------------------------- writing
@@ -161,9 +162,9 @@ def _append_ref(qkv, H, Hkv, dh, rope, codes, scales, block, block_table, seq_le
 
 
 def _chunk(n, B, block):
-    """Rows that a warp looks for blocks in: the whole of a block of sixteen where sequences are long, one row where they are short, so that
-    the blocks of a chunk, which one warp writes one after the other, are few."""
-    return 1 if n < 4 * B else 4 if n < 64 * B else 16
+    """Rows that a warp looks for blocks in: a block's worth where sequences are long, one row where they are short, so that the blocks of a
+    chunk, which one warp writes one after the other, are few."""
+    return 1 if n < 4 * B else 4 if n < 64 * B else block
 
 
 def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
@@ -174,16 +175,17 @@ def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
     B, max_blocks = _batch(what, n, seq_len, block_table, cu_q)
     if qkv.dtype is not BF:
         raise ValueError(f"{what}: qkv must be bf16")
-    if rope is not None and (rope[0].shape != rope[1].shape or rope[0].dim() != 2 or rope[0].shape[1] * 2 != dh
-                             or rope[0].dtype is not torch.float32 or rope[1].dtype is not torch.float32):
-        raise ValueError(f"{what}: the rotation's tables must be fp32 [positions, dh / 2]")
-    device = qkv.device
-    if device.type != "cuda":
+    if rope is not None:
+        turns = rope[0].shape
+        if len(turns) != 2 or turns[1] * 2 != dh or rope[1].shape != turns or rope[0].dtype is not F32 or rope[1].dtype is not F32:
+            raise ValueError(f"{what}: the rotation's tables must be fp32 [positions, dh / 2]")
+    index = qkv.get_device()
+    if index < 0:
         return _append_ref(qkv, H, Hkv, dh, rope, codes, scales, block, block_table, seq_len, cu_q)
-    if device.index != _lib.current_device():
-        with torch.cuda.device(device):
+    if index != _lib.current_device():
+        with torch.cuda.device(index):
             return _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q)
-    _on_device(what, device, codes, scales, dh, (block_table, seq_len, cu_q))
+    codes_at = _on_device(what, index, codes, scales, dh, (block_table, seq_len) if cu_q is None else (block_table, seq_len, cu_q))
     (ld, unit), at = qkv.stride(), qkv.data_ptr()
     if n == 1:
         ld = (H + 2 * Hkv) * dh                        # a dimension of one has any stride
@@ -193,14 +195,16 @@ def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
     n_pos = 0
     if rope is not None:
         cos, sin = rope
-        if not (cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == device.index):
+        if cos.get_device() != index or sin.get_device() != index or not (cos.is_contiguous() and sin.is_contiguous()):
             raise ValueError(f"{what}: the rotation's tables must be contiguous and on the device of qkv")
         n_pos, cos, sin = cos.shape[0], cos.data_ptr(), sin.data_ptr()
+        if (cos | sin) % 16:
+            raise ValueError(f"{what}: the rotation's tables must be 16-byte aligned")
     if n == 0 or B == 0 or n_blocks == 0:
         return
-    _lib.call("sb_quant_kv_append", at, ld, n, H, Hkv, dh, cos, sin, n_pos, codes.data_ptr(), codes.dtype is not torch.int8, scales.data_ptr(),
-              n_blocks, page, block, block_table.data_ptr(), max_blocks, seq_len.data_ptr(), cu_q.data_ptr() if cu_q is not None else None,
-              B, _chunk(n, B, block), _lib.stream())
+    _lib.call("sb_quant_kv_append", at, ld, n, H, Hkv, dh, cos, sin, n_pos, codes_at, codes.dtype is not torch.int8, scales.data_ptr(), n_blocks,
+              page, block, block_table.data_ptr(), max_blocks, seq_len.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B,
+              _chunk(n, B, block), _lib.stream())
     _g.launch_count += 1
 
 
@@ -230,37 +234,37 @@ def read_pages(pool, pages, out=None):
     ``pages[i]``, so that with ``arange(n)`` as table it is a pool for the attention over bf16 pages. The same page may be asked for more
     than once. Ids on the host are checked; of those on the device (int32) one outside the pool reads as zeros."""
     codes, scales, n_blocks, Hkv, page, dh, block = _layout("read_pages", pool)
-    device = codes.device
-    if not torch.is_tensor(pages) or (pages.device.type != "cuda" and device.type == "cuda"):
+    index = codes.get_device()
+    if not torch.is_tensor(pages) or (index >= 0 and not pages.is_cuda):
         ids = [int(i) for i in (pages.tolist() if torch.is_tensor(pages) else pages)]
         if any(not 0 <= i < n_blocks for i in ids):
             raise ValueError("read_pages: page outside the pool")
-        pages = torch.tensor(ids, dtype=torch.int32, device=device)
+        pages = torch.tensor(ids, dtype=I32, device=codes.device)
     if pages.dim() != 1:
         raise ValueError("read_pages: a vector of page ids")
     shape = (pages.shape[0], 2, Hkv, page, dh)
-    if out is not None and (tuple(out.shape) != shape or out.dtype is not BF or not out.is_contiguous() or out.device != device):
+    if out is not None and (tuple(out.shape) != shape or out.dtype is not BF or not out.is_contiguous() or out.device != codes.device):
         raise ValueError("read_pages: out must be contiguous bf16 [pages, 2, Hkv, page, dh] beside the pool")
-    if device.type != "cuda":
+    if index < 0:
         if pages.numel() and not 0 <= int(pages.min()) <= int(pages.max()) < n_blocks:
             raise ValueError("read_pages: page outside the pool")
-        got = _values(codes[pages.long()] if codes.dtype is torch.int8 else codes.view(torch.int8)[pages.long()].view(codes.dtype),
-                      scales[pages.long()], block).to(BF)
+        got = _values(codes.view(torch.int8)[pages.long()].view(codes.dtype), scales[pages.long()], block).to(BF)
         return got if out is None else out.copy_(got)
-    if device.index != _lib.current_device():
-        with torch.cuda.device(device):
+    if index != _lib.current_device():
+        with torch.cuda.device(index):
             return read_pages(pool, pages, out)
-    _on_device("read_pages", device, codes, scales, dh, (pages,))
+    codes_at = _on_device("read_pages", index, codes, scales, dh, (pages,))
     if out is None:
-        out = _lib.empty(shape, BF, device)
-    elif out.data_ptr() % 16:
+        out = _lib.empty(shape, BF, codes.device) if _lib.DEBUG_POISON else codes.new_empty(shape, dtype=BF)      # cheaper than torch.empty
+    out_at = out.data_ptr()
+    if out_at % 16:
         raise ValueError("read_pages: out must be 16-byte aligned")
-    if out.numel() == 0:
+    if shape[0] == 0:
         return out
     if n_blocks == 0:
         return out.zero_()
-    _lib.call("sb_quant_kv_read", codes.data_ptr(), codes.dtype is not torch.int8, scales.data_ptr(), n_blocks, Hkv, page, block, dh,
-              pages.data_ptr(), shape[0], out.data_ptr(), _lib.stream())
+    _lib.call("sb_quant_kv_read", codes_at, codes.dtype is not torch.int8, scales.data_ptr(), n_blocks, Hkv, page, block, dh, pages.data_ptr(),
+              shape[0], out_at, _lib.stream())
     _g.launch_count += 1
     return out
 
@@ -271,12 +275,13 @@ TILE, JOB_HEADS, LAUNCH_SEQUENCES = 64, 16, 1024          # positions of a tile,
 
 class _Workspace:
     """Parts of jobs that are cut, and a counter for each job, which every launch leaves at zero."""
-    __slots__ = ("part", "counters", "capture")
+    __slots__ = ("part", "counters", "capture", "floats", "jobs", "part_at", "counters_at")
 
-    def __init__(self, floats, counters, device, capture):
+    def __init__(self, floats, jobs, device, capture):
         self.part = _lib.empty(floats, torch.float32, device)
-        self.counters = torch.zeros(counters, dtype=torch.int32, device=device)
-        self.capture = capture
+        self.counters = torch.zeros(jobs, dtype=torch.int32, device=device)
+        self.capture, self.floats, self.jobs = capture, floats, jobs
+        self.part_at, self.counters_at = self.part.data_ptr(), self.counters.data_ptr()
 
 
 _ws: dict = {}
@@ -284,11 +289,11 @@ _ws_lock = threading.Lock()
 
 
 @functools.lru_cache(maxsize=64)
-def _part_floats(device_index, dh):
+def _part_floats(index, dh):                      # a function of the device and the head dimension
     return _lib.cuda().sb_quant_kv_attention_floats(dh)
 
 
-def _workspace(device, stream, floats, counters):
+def _workspace(index, stream, floats, jobs):
     """Launches on one stream follow one another and share one. Those of a graph share one of the graph's memory, whose counters it clears
     itself: graphs captured on one stream may be replayed at once on two."""
     capture = 0
@@ -296,13 +301,13 @@ def _workspace(device, stream, floats, counters):
         word = (C.c_ulonglong * 1)()
         _lib.call("sb_stream_capture_id", stream, word)
         capture = word[0]
-    key = (device.index, stream, capture != 0)
+    key = (index, stream, capture != 0)
     w = _ws.get(key)
-    if w is None or w.capture != capture or w.counters.shape[0] < counters or w.part.shape[0] < floats or _lib.DEBUG_POISON:
+    if w is None or w.capture != capture or w.jobs < jobs or w.floats < floats or _lib.DEBUG_POISON:
         with _ws_lock:
             w = _ws.get(key)
-            if w is None or w.capture != capture or w.counters.shape[0] < counters or w.part.shape[0] < floats or _lib.DEBUG_POISON:
-                w = _ws[key] = _Workspace(floats, max(counters, 4096), device, capture)
+            if w is None or w.capture != capture or w.jobs < jobs or w.floats < floats or _lib.DEBUG_POISON:
+                w = _ws[key] = _Workspace(floats, max(jobs, 4096), torch.device("cuda", index), capture)
     return w
 
 
@@ -336,36 +341,38 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     may hold any code and any scale. Returns bf16 [B, H * dh], ``out`` if that is given; ``out`` may not lie in what the call reads."""
     codes, scales, n_blocks, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    if q.dim() != 2 or H <= 0 or H % Hkv or q.shape[1] < H * dh or not scale > 0.0:
+    shape = q.shape
+    if len(shape) != 2 or H <= 0 or H % Hkv or shape[1] < H * dh or not scale > 0.0:
         raise ValueError("decode_attention: q must be [B, >= H * dh], heads a multiple of kv heads, scale positive")
-    B, max_blocks = _batch("decode_attention", q.shape[0], seq_len, block_table, None)
+    B, max_blocks = _batch("decode_attention", shape[0], seq_len, block_table, None)
     if q.dtype is not BF or (out is not None and (out.dtype is not BF or tuple(out.shape) != (B, H * dh))):
         raise ValueError("decode_attention: q must be bf16, out bf16 [B, H * dh]")
-    device = q.device
-    if device.type != "cuda":
+    index = q.get_device()
+    if index < 0:
         o = decode_attention_ref(q, pool, block_table, seq_len, H, Hkv, dh, scale).to(BF)
         return o if out is None else out.copy_(o)
-    if device.index != _lib.current_device():
-        with torch.cuda.device(device):
+    if index != _lib.current_device():
+        with torch.cuda.device(index):
             return decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale, max_len, out)
-    _on_device("decode_attention", device, codes, scales, dh, (block_table, seq_len))
+    codes_at = _on_device("decode_attention", index, codes, scales, dh, (block_table, seq_len))
     (ldq, unit), q_at = q.stride(), q.data_ptr()
     if B == 1:
         ldq = H * dh
     if unit != 1 or ldq % 8 or ldq < H * dh or q_at % 16:
         raise ValueError("decode_attention: rows of q must be contiguous, apart and 16-byte aligned")
     if out is None:
-        out, ldo = _lib.empty((B, H * dh), BF, device), H * dh
+        out = _lib.empty((B, H * dh), BF, q.device) if _lib.DEBUG_POISON else q.new_empty((B, H * dh))       # cheaper than torch.empty
+        ldo, o_at = H * dh, out.data_ptr()
     else:
-        ldo, unit = out.stride()
+        (ldo, unit), o_at = out.stride(), out.data_ptr()
         ldo = H * dh if B == 1 else ldo
-        if unit != 1 or ldo % 8 or ldo < H * dh or out.data_ptr() % 16 or out.get_device() != device.index:
+        if unit != 1 or ldo % 8 or ldo < H * dh or o_at % 16 or out.get_device() != index:
             raise ValueError("decode_attention: rows of out must be contiguous, apart, 16-byte aligned and on the device of q")
     if B == 0:
         return out
     if n_blocks == 0:
         raise ValueError("decode_attention: the pool has no pages")
-    if page not in (8, 16, 32) and page % TILE:
+    if page % TILE and page not in (8, 16, 32):
         raise ValueError("decode_attention: pages of 8, 16, 32 or a multiple of 64 positions")
     if n_blocks * 2 * Hkv * page >= (1 << 31) - TILE:
         raise ValueError("decode_attention: more rows of codes than 31 bits count")
@@ -377,14 +384,12 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     if max_len is not None:
         tiles = min(tiles, max(1, -(-int(max_len) // TILE)))
     stream = _lib.stream()
-    ws = _workspace(device, stream, _part_floats(device.index, dh), at_once * jobs)
-    part, counters, status = ws.part.data_ptr(), ws.counters.data_ptr(), _lib.status_word(device).data_ptr()
-    codes_at, e4m3, scales_at, table_at, lens_at, o_at = (codes.data_ptr(), codes.dtype is not torch.int8, scales.data_ptr(),
-                                                          block_table.data_ptr(), seq_len.data_ptr(), out.data_ptr())
+    ws = _workspace(index, stream, _part_floats(index, dh), at_once * jobs)
+    status, table_at, lens_at = _lib.status_word(q.device).data_ptr(), block_table.data_ptr(), seq_len.data_ptr()
     for b in range(0, B, at_once):
         n = min(at_once, B - b)
-        _lib.call("sb_quant_kv_attention", q_at + b * ldq * 2, ldq, codes_at, e4m3, scales_at, n_blocks, page, block,
-                  table_at + b * max_blocks * 4, max_blocks, lens_at + b * 4, n, H, Hkv, dh, n * jobs * tiles, scale, part, counters,
+        _lib.call("sb_quant_kv_attention", q_at + b * ldq * 2, ldq, codes_at, codes.dtype is not torch.int8, scales.data_ptr(), n_blocks, page, block,
+                  table_at + b * max_blocks * 4, max_blocks, lens_at + b * 4, n, H, Hkv, dh, n * jobs * tiles, scale, ws.part_at, ws.counters_at,
                   o_at + b * ldo * 2, ldo, status, stream)
         _g.launch_count += 1
     return out
