@@ -5,12 +5,12 @@
 //
 // Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time. One CTA per SM holds a ring of
 // tiles of 64 positions (keys and values, 8 or 16 KB) that one warp fills by TMA and another with the tile's sixteen scales; the tiles of all
-// jobs (a sequence and up to 16 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer
+// jobs (a sequence and up to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer
 // warps take the tiles in groups of four, warp w of a group 16 positions of the tile:
 //  - Codes become fp16, which holds every one of either type exactly: int8 by a byte permute (a byte behind 0x64 is 1024 + it) and one
 //    subtraction of two halves, e4m3 by its conversion. mma.sync takes them as the A operand, 16 positions (S = K q) or 16
 //    dimensions (O = V w) by 16, and eight query heads as columns: a warp's 16 positions times 16 query rows would be half empty
-//    with eight query heads a kv head or fewer. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of
+//    with eight query heads a kv head or fewer. With more, each group takes all tiles for eight of them. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of
 //    two halves of the A operand, and for K the dimensions of a step are in another order, in which q is loaded.
 //  - q is scaled by a power of two so that its row's largest magnitude is just below 2^15: fp16 then holds its bf16 values without loss.
 //  - The reference of the exponentials is a score seen before, not the maximum: it moves when a score exceeds it by 2^6, so that few
@@ -39,7 +39,7 @@ namespace kv8 {
 constexpr int TK = 64;                       // positions of a tile
 constexpr int MAX_B = 1024;                  // sequences of a launch, whose offsets lie in shared memory
 constexpr int STAGES_MAX = 24;
-constexpr int HEADS_MAX = 16;                // query heads of a job
+constexpr int SET = 8, HEADS_MAX = 3 * SET;  // query heads of a set, which is what a warp takes, and of a job
 constexpr int SMEM = 226 * 1024;
 constexpr int GRID_MAX = 160;
 
@@ -49,7 +49,8 @@ struct AttendParams {
   int n_blocks, page, page_bits, block_bits;         // page_bits: 3, 4 or 5, or for multiples of 64 6
   const int* table; int max_blocks;
   const int* seq_len;
-  int B, Hkv, G, subs, heads;                // a kv head's G query heads in `subs` jobs of `heads`
+  int B, Hkv, G, subs;                       // a kv head's G query heads in `subs` jobs
+  int sets, heads;                           // of so many sets of so many heads
   float scale_log2;
   float* part;                               // [2 * grid] of [HEADS_MAX][DH] values and [HEADS_MAX][2] maxima and sums
   unsigned int* counters;                    // [B * Hkv * subs], zero between calls
@@ -65,38 +66,35 @@ struct __align__(16) Piece {
   int start, counter, pad[2];                // the job's first unit, its counter
 };
 
-template <int DH, int NH>
+template <int DH>
 struct Cfg {
-  static constexpr int CONSUMERS = NH == 1 ? 12 : 8;           // warps; with twice the accumulators, fewer
-  static constexpr int GROUPS = CONSUMERS / 4;
+  static constexpr int GROUPS = 3, CONSUMERS = 4 * GROUPS;     // of four warps, and warps
   static constexpr int CODES = CONSUMERS, SCALES = CONSUMERS + 1, FINISHERS = CONSUMERS + 2;      // two producers, two finishers
   static constexpr int THREADS = CONSUMERS * 32 + 128;
   static constexpr int TILE = TK * DH;                         // bytes of a tile's keys, and of its values
   static constexpr int PITCH = DH + 4;                         // of a head's sums between warps: four heads of a pair of rows on different banks
-  static constexpr int SETS = 4;                               // that share the pieces of a job which is joined
-  static constexpr int QSLOTS = NH == 1 ? 4 : 2;               // pieces whose queries lie in shared memory
-  static constexpr int fixed_bytes(int heads, int B) {
-    return CONSUMERS * heads * (PITCH + 2) * 4 + QSLOTS * (heads * DH * 2 + static_cast<int>(sizeof(Piece))) + (2 * B + 1) * 4 +
+  static constexpr int QSLOTS = 4;                             // pieces whose queries lie in shared memory
+  static constexpr int fixed_bytes(int sets, int heads, int B) {
+    return CONSUMERS * heads * (PITCH + 2) * 4 + QSLOTS * (sets * heads * DH * 2 + static_cast<int>(sizeof(Piece))) + (2 * B + 1) * 4 +
            STAGES_MAX * (64 + 16) + (2 * QSLOTS + 2) * 8 + 1024;
   }
-  // A stage is always taken by one group: a parity wait tells a fill from the one after next only by whoever has seen the one between.
-  static constexpr int stages(int heads, int B) {
-    const int n = (SMEM - fixed_bytes(heads, B)) / (2 * TILE), most = n < STAGES_MAX ? n : STAGES_MAX;
-    return most / GROUPS * GROUPS;
+  // A stage is always taken by the same groups: a parity wait tells a fill from the one after next only by whoever has seen the one between.
+  static constexpr int stages(int sets, int heads, int B) {
+    const int n = (SMEM - fixed_bytes(sets, heads, B)) / (2 * TILE), most = n < STAGES_MAX ? n : STAGES_MAX;
+    return sets == 1 ? most / GROUPS * GROUPS : most;
   }
-  static constexpr int smem_bytes(int heads, int B) { return stages(heads, B) * 2 * TILE + fixed_bytes(heads, B); }
-  // the sets' values lie where the warps' sums have lain
-  static_assert(SETS * (DH + 2) <= CONSUMERS * (PITCH + 2), "");
+  static constexpr int smem_bytes(int sets, int heads, int B) { return stages(sets, heads, B) * 2 * TILE + fixed_bytes(sets, heads, B); }
 };
-static_assert(Cfg<128, 1>::stages(8, MAX_B) >= 8 && Cfg<128, 2>::stages(16, MAX_B) >= 8, "128 KB in flight");
+static_assert(Cfg<128>::stages(1, 8, MAX_B) >= 9 && Cfg<128>::stages(3, 8, MAX_B) >= 8, "128 KB in flight");
 
 __device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&a)[2], uint32_t (&b)[2]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr) : "memory");
 }
+template <int OFFSET>
 __device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&a)[2], uint32_t (&b)[2]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr), "n"(OFFSET) : "memory");
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -149,17 +147,17 @@ struct Deal {
   }
 };
 
-template <int DH, bool E4M3, int NH>
-__global__ void __launch_bounds__(Cfg<DH, NH>::THREADS, 1)
+template <int DH, bool E4M3>
+__global__ void __launch_bounds__(Cfg<DH>::THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
-  using C = Cfg<DH, NH>;
+  using C = Cfg<DH>;
   constexpr int CHUNKS = DH / 16, GROUPS = C::GROUPS, CONSUMERS = C::CONSUMERS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stages = p.stages, heads = p.heads, jobs_b = p.Hkv * p.subs;
+  const int stages = p.stages, sets = p.sets, heads = p.heads, jobs_b = p.Hkv * p.subs;
   float* sc = reinterpret_cast<float*>(ring + stages * 2 * C::TILE);                // [stages][k: 8 | v: 8], of 8 positions each
-  __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 16);     // [slots][heads][DH]
-  Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * heads * DH);          // [slots]
+  __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 16);     // [slots][sets * heads][DH]
+  Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * sets * heads * DH);          // [slots]
   float* sm_o = reinterpret_cast<float*>(pieces + C::QSLOTS);                       // [warps][heads][PITCH]
   float* sm_ml = sm_o + CONSUMERS * heads * C::PITCH;                               // [warps][heads][2]
   uint64_t* full = reinterpret_cast<uint64_t*>(sm_ml + CONSUMERS * heads * 2);
@@ -175,7 +173,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0) {
-    if (lane < stages) { mbar_init(&full[lane], 17); mbar_init(&empty[lane], 4); }
+    if (lane < stages) { mbar_init(&full[lane], 17); mbar_init(&empty[lane], 4 * sets); }
     if (lane < C::QSLOTS) { mbar_init(&q_full[lane], 1); mbar_init(&q_empty[lane], CONSUMERS + 2); }
     if (lane == 0) { mbar_init(o_full, CONSUMERS); mbar_init(o_empty, 1); }
     fence_barrier_init();
@@ -214,7 +212,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         base += __shfl_sync(0xffffffffu, inc, 31);
       }
       deal.units = base * jobs_b;
-      deal.ctas = min(static_cast<int>(gridDim.x), (deal.units + GROUPS - 1) / GROUPS);
+      deal.ctas = min(static_cast<int>(gridDim.x), sets == 1 ? (deal.units + GROUPS - 1) / GROUPS : deal.units);
       deal.each = deal.units / deal.ctas;
       deal.more = deal.units - deal.each * deal.ctas;
       if (lane == 0) { prefix[p.B] = base; s_deal = deal; }
@@ -253,7 +251,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       if (brings_codes) {
         if (!mbar_wait_warp(&q_empty[q_slot], q_phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) break;
         if (lane == 0) {
-          const int h0 = kvh * p.G + sub * heads, live = min(heads, p.G - sub * heads);
+          const int h0 = kvh * p.G + sub * sets * heads, live = min(sets * heads, p.G - sub * sets * heads);
           Piece* to = pieces + q_slot;
           to->b = b; to->h0 = h0; to->live = live; to->len = len;
           to->t_beg = t_beg; to->t_end = t_end; to->nt = nt; to->last = left == 0;
@@ -261,7 +259,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           mbar_arrive_expect_tx(&q_full[q_slot], idle ? 0 : live * DH * 2);
           if (!idle)
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                         ::"r"(smem_u32(sm_q + q_slot * heads * DH)), "l"(p.q + b * p.ldq + static_cast<long long>(h0) * DH), "r"(live * DH * 2),
+                         ::"r"(smem_u32(sm_q + q_slot * sets * heads * DH)), "l"(p.q + b * p.ldq + static_cast<long long>(h0) * DH), "r"(live * DH * 2),
                          "r"(smem_u32(&q_full[q_slot])) : "memory");
         }
         if (++q_slot == C::QSLOTS) { q_slot = 0; q_phase ^= 1; }
@@ -316,37 +314,38 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   const bool consumes = warp < CONSUMERS;
   const int quad = lane >> 2, tq = lane & 3, mi = lane >> 3;
   const int group = warp >> 2, pw = warp & 3;
+  // the groups take turns at the tiles, or, with more than one set of heads, each takes all tiles for a set of its own
+  const int my_set = sets == 1 ? 0 : group, stride = sets == 1 ? GROUPS : 1;
   const int wrow = pw * 16 + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
-  const int swz = DH == 128 ? (wrow & 7) : ((wrow >> 1) & 3);
+  // its first sixteen bytes of that row, swizzled; those of step c are at this address ^ (c << 4)
+  const uint32_t my_row = smem_u32(ring) + wrow * DH + (((mi >> 1) ^ (DH == 128 ? wrow & 7 : (wrow >> 1) & 3)) << 4);
+  const uint32_t my_scales = smem_u32(sc) + pw * 8;
   const int team = consumes ? CONSUMERS * 32 : 64, tid = consumes ? threadIdx.x : threadIdx.x - C::FINISHERS * 32;
   auto team_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(consumes ? 1 : 2), "r"(team) : "memory"); };
-  int stage = group, q_slot = 0;
+  int turn = group - my_set;                 // tiles of the next piece before the first that this group takes
+  int stage = turn, q_slot = 0;
   uint32_t phase = 0, q_phase = 0, o_phase = 0;
-  bool ok = true;
-  int turn = group;                          // tiles of the next piece before the first that this group takes
   for (bool last = false; !last;) {
     if (!mbar_wait_warp(&q_full[q_slot], q_phase, p.status, ST_TIMEOUT_FULL)) return;
     const Piece* piece = pieces + q_slot;                // the last one stays
-    const int t_beg = piece->t_beg, t_end = piece->t_end, len = piece->len, live = piece->live;
+    const int t_beg = piece->t_beg, t_end = piece->t_end, len = piece->len, live = piece->live, mine = min(heads, live - my_set * heads);
     last = piece->last;
     Piece to;
-    const __nv_bfloat16* my_q = sm_q + q_slot * heads * DH;
+    const __nv_bfloat16* my_q = sm_q + (q_slot * sets + my_set) * heads * DH;
     uint64_t* q_done = &q_empty[q_slot];
     if (++q_slot == C::QSLOTS) { q_slot = 0; q_phase ^= 1; }
     if (consumes) {
       // q as B fragments: column `quad` is a query head; of a step of 16 dimensions the lane's four are 4 tq .. 4 tq + 3, as K's bytes come
-      uint32_t qb[NH][CHUNKS][2];
-      float qf[NH][2];
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        const int h = n * 8 + quad;
-        const __nv_bfloat16* src = my_q + h * DH + tq * 4;
+      uint32_t qb[CHUNKS][2];
+      float qf[2];
+      {
+        const __nv_bfloat16* src = my_q + quad * DH + tq * 4;
         uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-          const uint2 v = h < live ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
-          qb[n][c][0] = v.x;
-          qb[n][c][1] = v.y;
+          const uint2 v = quad < mine ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
+          qb[c][0] = v.x;
+          qb[c][1] = v.y;
           top = max16x2(top, max16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
         }
         top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -355,109 +354,96 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);      // 2^(14 - (e - 127)), and back
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-          qb[n][c][0] = half2_bits(bf16_lo(qb[n][c][0]) * up, bf16_hi(qb[n][c][0]) * up);
-          qb[n][c][1] = half2_bits(bf16_lo(qb[n][c][1]) * up, bf16_hi(qb[n][c][1]) * up);
+          qb[c][0] = half2_bits(bf16_lo(qb[c][0]) * up, bf16_hi(qb[c][0]) * up);
+          qb[c][1] = half2_bits(bf16_lo(qb[c][1]) * up, bf16_hi(qb[c][1]) * up);
         }
         const float f = down * p.scale_log2;
-        qf[n][0] = __shfl_sync(0xffffffffu, f, tq * 8);                                // of heads 2 tq and 2 tq + 1, the columns of a result
-        qf[n][1] = __shfl_sync(0xffffffffu, f, tq * 8 + 4);
+        qf[0] = __shfl_sync(0xffffffffu, f, tq * 8);                                   // of heads 2 tq and 2 tq + 1, the columns of a result
+        qf[1] = __shfl_sync(0xffffffffu, f, tq * 8 + 4);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(q_done);
-      float m[NH][2], l[NH][2], o[CHUNKS][NH][4];
+      float m[2] = {-1.0e30f, -1.0e30f}, l[2] = {0.f, 0.f}, o[CHUNKS][4];
       float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
 #pragma unroll
-      for (int n = 0; n < NH; ++n) m[n][0] = m[n][1] = -1.0e30f, l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-        for (int n = 0; n < NH; ++n) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
+      for (int c = 0; c < CHUNKS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
 
-      int t = t_beg + turn;
-      for (; t < t_end; t += GROUPS) {
+      int t = my_set < sets ? t_beg + turn : t_end;                                    // with two sets one group has none
+      for (; t < t_end; t += stride) {
         const int st = stage;
         const uint32_t ph = phase;
-        stage += GROUPS;
+        stage += stride;
         if (stage >= stages) { stage -= stages; phase ^= 1; }
-        if (ok && !mbar_wait_warp(&full[st], ph, p.status, ST_TIMEOUT_FULL)) ok = false;
-        if (!ok) continue;
-        const uint32_t kt = smem_u32(ring + st * 2 * C::TILE) + wrow * DH, vt = kt + C::TILE;
-        const float2 ks = *reinterpret_cast<const float2*>(sc + st * 16 + pw * 2), vs = *reinterpret_cast<const float2*>(sc + st * 16 + 8 + pw * 2);
+        mbar_wait_converged(&full[st], ph, p.status, ST_TIMEOUT_FULL);
+        const uint32_t row = my_row + st * (2 * C::TILE);
+        float2 ks, vs;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks.x), "=f"(ks.y) : "r"(my_scales + st * 64) : "memory");
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2+32];" : "=f"(vs.x), "=f"(vs.y) : "r"(my_scales + st * 64) : "memory");
         const int valid = len - t * TK - pw * 16;                                      // positions of this warp's 16 that exist
         // the bytes of the warp's 16 positions go to registers, and the stage back to the producers
         uint32_t rk[CHUNKS][2], rv[CHUNKS][2];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) ldsm(kt + (((c + (mi >> 1)) ^ swz) << 4), rk[c], rk[c + 1]);
+        for (int c = 0; c < CHUNKS; c += 2) ldsm(row ^ (c << 4), rk[c], rk[c + 1]);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) ldsm_t(vt + (((c + (mi >> 1)) ^ swz) << 4), rv[c], rv[c + 1]);
+        for (int c = 0; c < CHUNKS; c += 2) ldsm_t<C::TILE>(row ^ (c << 4), rv[c], rv[c + 1]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
-        float s[NH][4], s1[NH][4];                                                     // two sums of products, so that they need not wait so long
-#pragma unroll
-        for (int n = 0; n < NH; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = s1[n][e] = 0.f;
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};               // two sums of products, so that they need not wait so long
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           uint32_t a[4];
           widen<E4M3, false>(rk[c][0], a[0], a[2]);
           widen<E4M3, false>(rk[c][1], a[1], a[3]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma_f16(c & 1 ? s1[n] : s[n], a[0], a[1], a[2], a[3], qb[n][c][0], qb[n][c][1]);
+          mma_f16(c & 1 ? s1 : s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
         }
 #pragma unroll
-        for (int n = 0; n < NH; ++n)
+        for (int e = 0; e < 4; ++e) s[e] += s1[e];
+        float x[4], top = -INFINITY;                                                   // scores less the reference
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] += s1[n][e];
-        bool over = vs.x > vref || vs.y > vref;
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            s[n][e] *= ks.x * qf[n][e];
-            s[n][2 + e] *= ks.y * qf[n][e];
-            if (valid < 16) {
-              if (quad >= valid) s[n][e] = -INFINITY;
-              if (quad + 8 >= valid) s[n][2 + e] = -INFINITY;
-            }
-            over |= s[n][e] - m[n][e] > 15.f || s[n][2 + e] - m[n][e] > 15.f;
-          }
+        for (int e = 0; e < 2; ++e) {
+          s[e] *= ks.x * qf[e];
+          s[2 + e] *= ks.y * qf[e];
         }
-        if (__any_sync(0xffffffffu, over)) {
+        if (valid < 16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (quad + (e >> 1) * 8 >= valid) s[e] = -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = s[e] - m[e & 1];
+          top = fmaxf(top, x[e]);
+        }
+        if (__any_sync(0xffffffffu, top > 15.f || fmaxf(vs.x, vs.y) > vref)) {
           const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
           vref = v_new;
           vinv = 1.f / v_new;
 #pragma unroll
-          for (int n = 0; n < NH; ++n) {
+          for (int e = 0; e < 2; ++e) {
+            float most = fmaxf(s[e], s[2 + e]) - 9.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(s[n][e], s[n][2 + e]) - 9.f;
+            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            const float m_new = fmaxf(m[e], most), a = ex2(m[e] - m_new);
+            m[e] = m_new;
+            l[e] *= a;
+            x[e] = s[e] - m_new;
+            x[2 + e] = s[2 + e] - m_new;
 #pragma unroll
-              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-              const float m_new = fmaxf(m[n][e], top), a = ex2(m[n][e] - m_new);
-              m[n][e] = m_new;
-              l[n][e] *= a;
-#pragma unroll
-              for (int c = 0; c < CHUNKS; ++c) {
-                o[c][n][e] *= a * v_ratio;
-                o[c][n][2 + e] *= a * v_ratio;
-              }
+            for (int c = 0; c < CHUNKS; ++c) {
+              o[c][e] *= a * v_ratio;
+              o[c][2 + e] *= a * v_ratio;
             }
           }
         }
-        uint32_t w[NH][2];
+        uint32_t w[2];
         {
           const float v0 = vs.x * vinv, v1 = vs.y * vinv;
 #pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            float e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = ex2(s[n][i] - m[n][i & 1]);
-            l[n][0] += e[0] + e[2];
-            l[n][1] += e[1] + e[3];
-            w[n][0] = transpose8x8(half2_bits(e[0] * v0, e[1] * v0));
-            w[n][1] = transpose8x8(half2_bits(e[2] * v1, e[3] * v1));
-          }
+          for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
+          l[0] += x[0] + x[2];
+          l[1] += x[1] + x[3];
+          w[0] = transpose8x8(half2_bits(x[0] * v0, x[1] * v0));
+          w[1] = transpose8x8(half2_bits(x[2] * v1, x[3] * v1));
         }
         // what lies behind the last position may be NaN, which a weight of zero does not make zero
         uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -471,31 +457,25 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           if (E4M3) { rv[c][0] &= keep0; rv[c][1] &= keep1; }
           widen<E4M3, true>(rv[c][0], a[0], a[1]);
           widen<E4M3, true>(rv[c][1], a[2], a[3]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma_f16(o[c][n], a[0], a[1], a[2], a[3], w[n][0], w[n][1]);
+          mma_f16(o[c], a[0], a[1], a[2], a[3], w[0], w[1]);
         }
       }
       turn = t - t_end;
 
 #pragma unroll
-      for (int n = 0; n < NH; ++n)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
-      if (ok && !mbar_wait_warp(o_empty, o_phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) ok = false;      // those of the piece before have been read
+        for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+      mbar_wait_converged(o_empty, o_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);           // those of the piece before have been read
       o_phase ^= 1;
 #pragma unroll
-      for (int n = 0; n < NH; ++n) {
+      for (int e = 0; e < 2; ++e) {
+        const int h = 2 * tq + e;
+        if (h >= mine) continue;
+        float* dst = sm_o + (warp * heads + h) * C::PITCH + 2 * quad;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = n * 8 + 2 * tq + e;
-          if (h >= live) continue;
-          float* dst = sm_o + (warp * heads + h) * C::PITCH + 2 * quad;
-#pragma unroll
-          for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float2*>(dst + c * 16) = make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
-          if (quad == 0) *reinterpret_cast<float2*>(sm_ml + (warp * heads + h) * 2) = make_float2(m[n][e], l[n][e]);
-        }
+        for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float2*>(dst + c * 16) = make_float2(o[c][e] * vref, o[c][2 + e] * vref);
+        if (quad == 0) *reinterpret_cast<float2*>(sm_ml + (warp * heads + h) * 2) = make_float2(m[e], l[e]);
       }
       if (!last) {
         __syncwarp();
@@ -528,15 +508,16 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     // ---- the warps' sums are joined in the order of the warps ----
     for (int i = tid; i < items; i += team) {
       const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+      const int set = h / heads, from = sets == 1 ? 0 : 4 * set, to_warp = sets == 1 ? CONSUMERS : from + 4, at = h - set * heads;
       float top = -1.0e30f, sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int x = 0; x < CONSUMERS; ++x) top = fmaxf(top, sm_ml[(x * heads + h) * 2]);
 #pragma unroll 4                             // code that runs once comes from L2: short loops are faster than long straight lines
-      for (int x = 0; x < CONSUMERS; ++x) {
-        const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (x * heads + h) * 2);
+      for (int x = from; x < to_warp; ++x) top = fmaxf(top, sm_ml[(x * heads + at) * 2]);
+#pragma unroll 4
+      for (int x = from; x < to_warp; ++x) {
+        const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (x * heads + at) * 2);
         const float a = ex2(ml.x - top);
-        const float4 e = *reinterpret_cast<const float4*>(sm_o + (x * heads + h) * C::PITCH + d);
+        const float4 e = *reinterpret_cast<const float4*>(sm_o + (x * heads + at) * C::PITCH + d);
         sum += ml.y * a;
         v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
       }
@@ -561,21 +542,22 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     }
     team_sync();
     if (!s_last[consumes]) continue;
-    const int sets = consumes ? min(C::SETS, max(1, team / items)) : 1;      // the sums have been read, by the consumers of the last piece anyway
-    float* sm_v = sm_o;                                                      // [sets][live][DH], then [sets][live][2]
-    float* sm_vml = sm_o + sets * live * DH;
-    for (int i = tid; i < items * sets; i += team) {
-      int set = 0, at = i;
-      while (at >= items) { at -= items; ++set; }
+    // The consumers of the last piece have room where the sums were, which have been read: several shares of the pieces at a time.
+    const int shares = consumes ? min(4, max(1, team / items)) : 1;
+    float* sm_v = sm_o;                                  // [shares][live][DH], then [shares][live][2]
+    float* sm_vml = sm_o + shares * live * DH;
+    for (int i = tid; i < items * shares; i += team) {
+      int share = 0, at = i;
+      while (at >= items) { at -= items; ++share; }
       const int h = at / (DH / 4);
       float top = -1.0e30f, sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = set; c < n_pieces; c += 8 * sets) {   // the loads of eight pieces are under way together
+      for (int c = share; c < n_pieces; c += 8 * shares) {   // the loads of eight pieces are under way together
         float2 ml[8];
         float4 e[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int at_c = c + k * sets;
+          const int at_c = c + k * shares;
           ml[k] = make_float2(-1.0e30f, 0.f);
           if (at_c >= n_pieces) continue;
           const float* src = part_of(2 * (c0 + at_c) + (at_c == 0));
@@ -591,27 +573,27 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          if (c + k * sets >= n_pieces) continue;
+          if (c + k * shares >= n_pieces) continue;
           const float a = ex2(ml[k].x - top);
           sum += ml[k].y * a;
           v.x += e[k].x * a; v.y += e[k].y * a; v.z += e[k].z * a; v.w += e[k].w * a;
         }
       }
-      if (sets == 1) {
+      if (shares == 1) {
         write_out(at * 4, v, sum);
       } else {
-        *reinterpret_cast<float4*>(sm_v + (set * items + at) * 4) = v;
-        if (at % (DH / 4) == 0) *reinterpret_cast<float2*>(sm_vml + (set * live + h) * 2) = make_float2(top, sum);
+        *reinterpret_cast<float4*>(sm_v + (share * items + at) * 4) = v;
+        if (at % (DH / 4) == 0) *reinterpret_cast<float2*>(sm_vml + (share * live + h) * 2) = make_float2(top, sum);
       }
     }
-    if (sets == 1) continue;
+    if (shares == 1) continue;
     team_sync();
     if (tid < items) {
       const int h = tid / (DH / 4);
       float top = -1.0e30f, sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int x = 0; x < sets; ++x) top = fmaxf(top, sm_vml[(x * live + h) * 2]);
-      for (int x = 0; x < sets; ++x) {
+      for (int x = 0; x < shares; ++x) top = fmaxf(top, sm_vml[(x * live + h) * 2]);
+      for (int x = 0; x < shares; ++x) {
         const float2 ml = *reinterpret_cast<const float2*>(sm_vml + (x * live + h) * 2);
         const float a = ex2(ml.x - top);
         const float4 e = *reinterpret_cast<const float4*>(sm_v + (x * items + tid) * 4);
@@ -623,13 +605,13 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   }
 }
 
-template <int DH, bool E4M3, int NH>
+template <int DH, bool E4M3>
 static int launch_attend(const CUtensorMap& tm, AttendParams p, int grid, cudaStream_t s) {
-  using C = Cfg<DH, NH>;
+  using C = Cfg<DH>;
   static PerDeviceOnce attr;
-  if (allow_smem(attr, attend_kernel<DH, E4M3, NH>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
-  p.stages = C::stages(p.heads, p.B);
-  return launch_dep(attend_kernel<DH, E4M3, NH>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.heads, p.B), s, tm, p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  if (allow_smem(attr, attend_kernel<DH, E4M3>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  p.stages = C::stages(p.sets, p.heads, p.B);
+  return launch_dep(attend_kernel<DH, E4M3>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.sets, p.heads, p.B), s, tm, p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 }  // namespace kv8
@@ -642,7 +624,7 @@ extern "C" int sb_quant_kv_attention_floats(int dh) { return 2 * num_sms() * kv8
 
 // q: [B, ldq] bf16 (H * dh used, rotated), out: [B, ldo] bf16, rows 16-byte aligned. A sequence of no positions gets zeros; ids outside the
 // pool count as zeros. page 8, 16, 32 or a multiple of 64; B <= 1024. max_tiles: an upper bound of the 64-position tiles of all
-// jobs, which only caps the grid. counters: B * Hkv * ceil(H / Hkv / 16) words, zero before the first call (every call leaves them zero).
+// jobs, which only caps the grid. counters: B * Hkv * ceil(H / Hkv / 24) words, zero before the first call (every call leaves them zero).
 extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* codes, int e4m3, const float* scales, int n_blocks, int page,
                                      int block, const int* table, int max_blocks, const int* seq_len, int B, int H, int Hkv, int dh,
                                      long long max_tiles, float scale, float* part, unsigned int* counters, void* out, long long ldo,
@@ -666,22 +648,20 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   p.table = table; p.max_blocks = max_blocks; p.seq_len = seq_len;
   p.B = B; p.Hkv = Hkv; p.G = H / Hkv;
   p.subs = (p.G + kv8::HEADS_MAX - 1) / kv8::HEADS_MAX;
-  p.heads = (p.G + p.subs - 1) / p.subs;
+  const int per_job = (p.G + p.subs - 1) / p.subs;
+  p.sets = (per_job + kv8::SET - 1) / kv8::SET;
+  p.heads = (per_job + p.sets - 1) / p.sets;
   if (static_cast<double>(B) * ((static_cast<double>(max_blocks) * page + kv8::TK - 1) / kv8::TK) * Hkv * p.subs > 2147483647.0) return SB_ERR_TOO_LARGE;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = part; p.counters = counters;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.status = status;
   // the kernel leaves a tile to each group of consumers
-  const long long want = (max_tiles + 1) / 2;
+  const long long want = p.sets == 1 ? (max_tiles + 2) / 3 : max_tiles;
   const int most = num_sms() < kv8::GRID_MAX ? num_sms() : kv8::GRID_MAX, grid = want < most ? static_cast<int>(want) : most;
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  const bool two = p.heads > 8;
-  if (dh == 64)
-    return e4m3 ? (two ? kv8::launch_attend<64, true, 2>(tm, p, grid, s) : kv8::launch_attend<64, true, 1>(tm, p, grid, s))
-                : (two ? kv8::launch_attend<64, false, 2>(tm, p, grid, s) : kv8::launch_attend<64, false, 1>(tm, p, grid, s));
-  return e4m3 ? (two ? kv8::launch_attend<128, true, 2>(tm, p, grid, s) : kv8::launch_attend<128, true, 1>(tm, p, grid, s))
-              : (two ? kv8::launch_attend<128, false, 2>(tm, p, grid, s) : kv8::launch_attend<128, false, 1>(tm, p, grid, s));
+  if (dh == 64) return e4m3 ? kv8::launch_attend<64, true>(tm, p, grid, s) : kv8::launch_attend<64, false>(tm, p, grid, s);
+  return e4m3 ? kv8::launch_attend<128, true>(tm, p, grid, s) : kv8::launch_attend<128, false>(tm, p, grid, s);
 }
 
 // The capture that `stream` is in, 0 where it is in none: what a graph's launches share is apart from every other graph's.

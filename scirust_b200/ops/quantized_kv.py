@@ -270,7 +270,7 @@ def read_pages(pool, pages, out=None):
 
 
 # ---------------------------------------------------------------------------------------------------------------- attention
-TILE, JOB_HEADS, LAUNCH_SEQUENCES = 64, 16, 1024          # positions of a tile, query heads of a job, sequences of a launch
+TILE, JOB_HEADS, LAUNCH_SEQUENCES = 64, 24, 1024          # positions of a tile, query heads of a job, sequences of a launch
 
 
 class _Workspace:

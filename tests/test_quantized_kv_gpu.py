@@ -247,7 +247,7 @@ def check(a, scale=None, **kw):
     return out
 
 
-HEADS = [(16, 4, 64), (32, 8, 128), (4, 1, 128), (12, 12, 64), (5, 5, 128), (20, 1, 128), (16, 1, 64), (9, 1, 128), (34, 2, 64), (14, 2, 128)]
+HEADS = [(16, 4, 64), (32, 8, 128), (4, 1, 128), (12, 12, 64), (5, 5, 128), (20, 1, 128), (16, 1, 64), (9, 1, 128), (34, 2, 64), (14, 2, 128), (24, 1, 64), (50, 2, 64), (97, 1, 64), (71, 1, 128)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
