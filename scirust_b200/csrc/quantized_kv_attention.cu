@@ -7,12 +7,15 @@
 // tiles of 64 positions (keys and values, 8 or 16 KB) that one warp fills by TMA and another with the tile's sixteen scales; the tiles of all
 // jobs (a sequence and up to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer
 // warps take the tiles in groups of four, warp w of a group 16 positions of the tile:
+//  - mma.sync takes codes as the A operand, 16 positions (S = K q) or 16 dimensions (O = V w), and eight query heads as columns: a warp's
+//    16 positions times 16 query rows would be half empty with eight query heads a kv head or fewer. With more, each group takes all tiles for
+//    eight of them. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of two halves of the A operand,
+//    and for K the dimensions of a step are in another order, in which q is loaded.
 //  - Codes become fp16, which holds every one of either type exactly: int8 by a byte permute (a byte behind 0x64 is 1024 + it) and one
-//    subtraction of two halves, e4m3 by its conversion. mma.sync takes them as the A operand, 16 positions (S = K q) or 16
-//    dimensions (O = V w) by 16, and eight query heads as columns: a warp's 16 positions times 16 query rows would be half empty
-//    with eight query heads a kv head or fewer. With more, each group takes all tiles for eight of them. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of
-//    two halves of the A operand, and for K the dimensions of a step are in another order, in which q is loaded.
-//  - q is scaled by a power of two so that its row's largest magnitude is just below 2^15: fp16 then holds its bf16 values without loss.
+//    subtraction of two halves, e4m3 by its conversion. K in int8 goes into the product as it is: q, scaled by a power of two so that its
+//    row's largest magnitude is just below 2^14 and rounded to whole numbers, is two bytes, whose products are summed apart, exactly. That
+//    rounding is off by 2^-14 of the row's largest at most, and bf16 values from 2^-6 of it on are kept as they are; 50 conversions a tile and
+//    lane of 130 are saved (1 x 131072 int8 52 -> 49 us). For e4m3 q's largest is just below 2^15, and fp16 holds it without loss.
 //  - The reference of the exponentials is a score seen before, not the maximum: it moves when a score exceeds it by 2^6, so that few
 //    tiles need a reduction over positions and a pass over O. Weights are 2^9 at the reference: at most 2^15, and what lies 2^-33 below the
 //    reference is still a number of fp16. Their sum is taken in 32 bits before they are rounded (half a step of 2^-11) and weighed.
@@ -96,13 +99,28 @@ __device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&a)[2], uint32_t
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
                : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr), "n"(OFFSET) : "memory");
 }
+// c += a b, or with FIRST c = a b
+template <bool FIRST>
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (FIRST)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool FIRST>
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[2], const uint32_t (&a_next)[2], uint32_t b0, uint32_t b1) {
+  if constexpr (FIRST)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a_next[0]), "r"(a_next[1]), "r"(b0), "r"(b1), "r"(0));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a_next[0]), "r"(a_next[1]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -351,11 +369,27 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 15u);               // the exponent of the largest, biased
-        const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);      // 2^(14 - (e - 127)), and back
+        float down;
+        if constexpr (E4M3) {
+          const float up = __uint_as_float((268u - e) << 23);                          // 2^(14 - (e - 127)), and back
+          down = __uint_as_float((e - 14u) << 23);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          qb[c][0] = half2_bits(bf16_lo(qb[c][0]) * up, bf16_hi(qb[c][0]) * up);
-          qb[c][1] = half2_bits(bf16_lo(qb[c][1]) * up, bf16_hi(qb[c][1]) * up);
+          for (int c = 0; c < CHUNKS; ++c) {
+            qb[c][0] = half2_bits(bf16_lo(qb[c][0]) * up, bf16_hi(qb[c][0]) * up);
+            qb[c][1] = half2_bits(bf16_lo(qb[c][1]) * up, bf16_hi(qb[c][1]) * up);
+          }
+        } else {
+          // Whole numbers of up to 2^14: 1.5 * 2^23 + q is a float whose last bytes are it. The lower byte counts from -128 on, so that the
+          // upper one is that of q + 128.
+          const float up = __uint_as_float((267u - e) << 23);
+          down = e == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((e - 13u) << 23);      // no whole number is a NaN or an infinity
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c) {
+            const uint32_t w0 = __float_as_uint(fmaf(bf16_lo(qb[c][0]), up, 12582912.f)), w1 = __float_as_uint(fmaf(bf16_hi(qb[c][0]), up, 12582912.f));
+            const uint32_t w2 = __float_as_uint(fmaf(bf16_lo(qb[c][1]), up, 12582912.f)), w3 = __float_as_uint(fmaf(bf16_hi(qb[c][1]), up, 12582912.f));
+            qb[c][0] = __byte_perm(__byte_perm(w0 + 128, w1 + 128, 0x0051), __byte_perm(w2 + 128, w3 + 128, 0x0051), 0x5410);
+            qb[c][1] = __byte_perm(__byte_perm(w0, w1, 0x0040), __byte_perm(w2, w3, 0x0040), 0x5410);
+          }
         }
         const float f = down * p.scale_log2;
         qf[0] = __shfl_sync(0xffffffffu, f, tq * 8);                                   // of heads 2 tq and 2 tq + 1, the columns of a result
@@ -388,16 +422,38 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         for (int c = 0; c < CHUNKS; c += 2) ldsm_t<C::TILE>(row ^ (c << 4), rv[c], rv[c + 1]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};               // two sums of products, so that they need not wait so long
+        float s[4];
+        if constexpr (E4M3) {
+          float s1[4];                                                                 // two sums of products, so that they need not wait so long
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          uint32_t a[4];
-          widen<E4M3, false>(rk[c][0], a[0], a[2]);
-          widen<E4M3, false>(rk[c][1], a[1], a[3]);
-          mma_f16(c & 1 ? s1 : s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
+          for (int c = 0; c < CHUNKS; c += 2) {
+            uint32_t a[4];
+            widen<E4M3, false>(rk[c][0], a[0], a[2]);
+            widen<E4M3, false>(rk[c][1], a[1], a[3]);
+            if (c == 0) mma_f16<true>(s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
+            else mma_f16<false>(s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
+            widen<E4M3, false>(rk[c + 1][0], a[0], a[2]);
+            widen<E4M3, false>(rk[c + 1][1], a[1], a[3]);
+            if (c == 0) mma_f16<true>(s1, a[0], a[1], a[2], a[3], qb[c + 1][0], qb[c + 1][1]);
+            else mma_f16<false>(s1, a[0], a[1], a[2], a[3], qb[c + 1][0], qb[c + 1][1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] += s1[e];
+        } else {
+          int hi[4], lo[4];
+#pragma unroll
+          for (int c = 0; c < CHUNKS; c += 2) {
+            if (c == 0) {
+              mma_s8<true>(hi, rk[c], rk[c + 1], qb[c][0], qb[c + 1][0]);
+              mma_s8<true>(lo, rk[c], rk[c + 1], qb[c][1], qb[c + 1][1]);
+            } else {
+              mma_s8<false>(hi, rk[c], rk[c + 1], qb[c][0], qb[c + 1][0]);
+              mma_s8<false>(lo, rk[c], rk[c + 1], qb[c][1], qb[c + 1][1]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] = __int2float_rn(hi[e] * 256 + lo[e]);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += s1[e];
         float x[4], top = -INFINITY;                                                   // scores less the reference
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -457,7 +513,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           if (E4M3) { rv[c][0] &= keep0; rv[c][1] &= keep1; }
           widen<E4M3, true>(rv[c][0], a[0], a[1]);
           widen<E4M3, true>(rv[c][1], a[2], a[3]);
-          mma_f16(o[c], a[0], a[1], a[2], a[3], w[0], w[1]);
+          mma_f16<false>(o[c], a[0], a[1], a[2], a[3], w[0], w[1]);
         }
       }
       turn = t - t_end;

@@ -214,7 +214,9 @@ def batch(kind, H, Hkv, dh, page, block, lens, seed=0, pad=8, dirty=True):
 def statement(a, scale=None):
     """(o, bound): 64 bits, and how far an element may be off. A weight is rounded to fp16 (half a step of 2^-11, none finer than 2^-25 of
     2^-9 of the largest) and weighs v, the answer is rounded once to bf16; a score is a sum of dh products in 32 bits, each addition off by
-    a step of 2^-23 of the sum of magnitudes, which the exponential passes on as a relative error of a weight and of their sum."""
+    a step of 2^-23 of the sum of magnitudes, which the exponential passes on as a relative error of a weight and of their sum. With int8 codes
+    a query is rounded to whole numbers where its largest element is at least 2^13 of them: half of one, 2^-14 of the largest, for each
+    element, times the magnitude of the key's."""
     H, Hkv, dh, pool = a["H"], a["Hkv"], a["dh"], a["pool"]
     page, block = pool.codes.shape[3], pool.block
     scale = dh ** -0.5 if scale is None else scale
@@ -229,10 +231,11 @@ def statement(a, scale=None):
         q = a["q"][b, :H * dh].to(F64).reshape(Hkv, H // Hkv, dh)
         s = torch.einsum("kgd,jkd->kgj", q, kv[:, 0]) * scale
         size = torch.einsum("kgd,jkd->kgj", q.abs(), kv[:, 0].abs()) * scale
+        coarse = q.abs().amax(-1, keepdim=True) * 2.0 ** -14 if pool.codes.dtype is torch.int8 else torch.zeros_like(q[..., :1])
         p = torch.softmax(s, -1)
         o[b] = torch.einsum("kgj,jkd->kgd", p, kv[:, 1])
         mean = torch.einsum("kgj,jkd->kgd", p, kv[:, 1].abs())
-        slip = 2 * dh * 2.0 ** -23 * size.amax(-1, keepdim=True) + 2.0 ** -11 + 2.0 ** -20
+        slip = 2 * (dh * 2.0 ** -23 * size + coarse * scale * kv[:, 0].abs().sum(-1).T[:, None]).amax(-1, keepdim=True) + 2.0 ** -11 + 2.0 ** -20
         tiny = 2.0 ** -33 * kv[:, 1].abs().amax(0)[:, None] * length * p.amax(-1, keepdim=True)
         bound[b] = 2.0 ** -8 * o[b].abs() + slip * mean + tiny + 1e-30
     return o.reshape(B, -1), bound.reshape(B, -1)
