@@ -43,8 +43,8 @@ constexpr int TK = 64;                       // positions of a tile
 constexpr int MAX_B = 1024;                  // sequences of a launch, whose offsets lie in shared memory
 constexpr int STAGES_MAX = 24;
 constexpr int SET = 8, HEADS_MAX = 3 * SET;  // query heads of a set, which is what a warp takes, and of a job
-constexpr int SMEM = 226 * 1024;
-constexpr int GRID_MAX = 160;
+constexpr int SMEM = 225 * 1024;
+constexpr int SHARES = 4;                    // of the pieces of a job that is joined, at most
 
 struct AttendParams {
   const __nv_bfloat16* q; long long ldq;
@@ -75,10 +75,10 @@ struct Cfg {
   static constexpr int CODES = CONSUMERS, SCALES = CONSUMERS + 1, FINISHERS = CONSUMERS + 2;      // two producers, two finishers
   static constexpr int THREADS = CONSUMERS * 32 + 128;
   static constexpr int TILE = TK * DH;                         // bytes of a tile's keys, and of its values
-  static constexpr int PITCH = DH + 4;                         // of a head's sums between warps: four heads of a pair of rows on different banks
+  static constexpr int PITCH = DH + 4;                         // of a head's sums between warps
   static constexpr int QSLOTS = 4;                             // pieces whose queries lie in shared memory
   static constexpr int fixed_bytes(int sets, int heads, int B) {
-    return CONSUMERS * heads * (PITCH + 2) * 4 + QSLOTS * (sets * heads * DH * 2 + static_cast<int>(sizeof(Piece))) + (2 * B + 1) * 4 +
+    return CONSUMERS * heads * (PITCH + 4) * 4 + QSLOTS * (sets * heads * DH * 2 + static_cast<int>(sizeof(Piece))) + (2 * B + 1) * 4 +
            STAGES_MAX * (64 + 16) + (2 * QSLOTS + 2) * 8 + 1024;
   }
   // A stage is always taken by the same groups: a parity wait tells a fill from the one after next only by whoever has seen the one between.
@@ -165,6 +165,19 @@ struct Deal {
   }
 };
 
+// Four shares (reference and sum of weights, weighted values) as one; those of no piece have a sum of zero.
+__device__ __forceinline__ void join_shares(const float2 (&ml)[SHARES], const float4 (&e)[SHARES], float4& v, float& sum) {
+  const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+  sum = 0.f;
+  v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < SHARES; ++k) {
+    const float a = ex2(ml[k].x - top);
+    sum += ml[k].y * a;
+    v.x += e[k].x * a; v.y += e[k].y * a; v.z += e[k].z * a; v.w += e[k].w * a;
+  }
+}
+
 template <int DH, bool E4M3>
 __global__ void __launch_bounds__(Cfg<DH>::THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
@@ -177,8 +190,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 16);     // [slots][sets * heads][DH]
   Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * sets * heads * DH);          // [slots]
   float* sm_o = reinterpret_cast<float*>(pieces + C::QSLOTS);                       // [warps][heads][PITCH]
-  float* sm_ml = sm_o + CONSUMERS * heads * C::PITCH;                               // [warps][heads][2]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ml + CONSUMERS * heads * 2);
+  float4* sm_ml = reinterpret_cast<float4*>(sm_o + CONSUMERS * heads * C::PITCH);   // [warps][heads]: reference, sum, largest scale of values
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ml + CONSUMERS * heads);
   uint64_t* empty = full + STAGES_MAX;
   uint64_t* q_full = empty + STAGES_MAX;
   uint64_t* q_empty = q_full + C::QSLOTS;
@@ -186,14 +199,15 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   uint64_t* o_empty = o_full + 1;
   int* prefix = reinterpret_cast<int*>(o_empty + 1);                                // [B + 1] tiles before sequence b
   int* lens = prefix + p.B + 1;                                                     // [B]
-  __shared__ int s_last[2];
+  __shared__ int s_last[2], s_join[2][2];    // of the consumers and the finishers: whether their job's other pieces are there, its first CTA, its pieces
+  __shared__ int s_end, s_ready, s_ready_join[2];
   __shared__ Deal s_deal;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0) {
     if (lane < stages) { mbar_init(&full[lane], 17); mbar_init(&empty[lane], 4 * sets); }
     if (lane < C::QSLOTS) { mbar_init(&q_full[lane], 1); mbar_init(&q_empty[lane], CONSUMERS + 2); }
-    if (lane == 0) { mbar_init(o_full, CONSUMERS); mbar_init(o_empty, 1); }
+    if (lane == 0) { mbar_init(o_full, CONSUMERS); mbar_init(o_empty, 1); s_end = s_ready = 0; }
     fence_barrier_init();
   } else if (threadIdx.x == C::CODES * 32) {
     prefetch_tmap(&tmap);
@@ -524,14 +538,15 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
       mbar_wait_converged(o_empty, o_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);           // those of the piece before have been read
       o_phase ^= 1;
+      // a lane's values of a head lie behind one another: dimensions 16 c + 2 quad and the next, for all c
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = 2 * tq + e;
         if (h >= mine) continue;
-        float* dst = sm_o + (warp * heads + h) * C::PITCH + 2 * quad;
+        float4* dst = reinterpret_cast<float4*>(sm_o + (warp * heads + h) * C::PITCH + quad * (2 * CHUNKS));
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float2*>(dst + c * 16) = make_float2(o[c][e] * vref, o[c][2 + e] * vref);
-        if (quad == 0) *reinterpret_cast<float2*>(sm_ml + (warp * heads + h) * 2) = make_float2(m[e], l[e]);
+        for (int c = 0; c < CHUNKS; c += 2) dst[c / 2] = make_float4(o[c][e], o[c][2 + e], o[c + 1][e], o[c + 1][2 + e]);
+        if (quad == 0) sm_ml[warp * heads + h] = make_float4(m[e], l[e], vref, 0.f);
       }
       if (!last) {
         __syncwarp();
@@ -542,7 +557,27 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       to = *piece;
       __syncwarp();
       if (lane == 0) mbar_arrive(q_done);
-      if (last) return;
+      if (last) {
+        // Mostly the other piece of the job has long been there, at the start of the next CTA's range: then the consumers need neither write
+        // theirs nor ask for the count when they are done.
+        if (tid == 0 && t_beg != t_end && !(t_beg == 0 && t_end == to.nt)) {
+          const Deal deal = s_deal;
+          const int c0 = deal.cta(to.start), n = deal.cta(to.start + to.nt - 1) - c0 + 1;
+          for (int i = 0; i < (1 << 20) && !*const_cast<volatile int*>(&s_end); ++i) {
+            unsigned int there;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.counters + to.counter) : "memory");
+            if (there == static_cast<unsigned int>(n) - 1) {
+              s_ready_join[0] = c0;
+              s_ready_join[1] = n;
+              __threadfence_block();
+              *const_cast<volatile int*>(&s_ready) = 1;
+              break;
+            }
+            __nanosleep(200);
+          }
+        }
+        return;
+      }
       if (!mbar_wait_warp(o_full, o_phase, p.status, ST_TIMEOUT_FULL)) return;
       o_phase ^= 1;
     }
@@ -550,40 +585,82 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
 
     if (consumes) to = *piece;
     const bool whole = t_beg == 0 && t_end == to.nt;
-    const Deal deal = s_deal;
-    const int c0 = whole ? 0 : deal.cta(to.start), n_pieces = whole ? 1 : deal.cta(to.start + to.nt - 1) - c0 + 1;
     auto part_of = [&](int c) { return p.part + static_cast<size_t>(c) * (HEADS_MAX * (DH + 2)); };
-    auto write_out = [&](int at, float4 v, float sum) {
+    // item i: four values of a head, in the order in which the warps left them
+    auto write_out = [&](int i, float4 v, float sum) {
+      const int h = i / (DH / 4), j = i % (DH / 4), d = 32 * (j % (CHUNKS / 2)) + 2 * (j / (CHUNKS / 2));
       const float inv = len > 0 ? 1.f / sum : 0.f;
-      v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-      *reinterpret_cast<uint2*>(p.out + to.b * p.ldo + static_cast<long long>(to.h0) * DH + at) =
-          make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      __nv_bfloat16* dst = p.out + to.b * p.ldo + static_cast<long long>(to.h0 + h) * DH + d;
+      *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(v.x * inv, v.y * inv);
+      *reinterpret_cast<uint32_t*>(dst + 16) = pack_bf16x2(v.z * inv, v.w * inv);
     };
-    const int items = live * (DH / 4);                   // of four values each
-    if (consumes) team_sync();
-    // ---- the warps' sums are joined in the order of the warps ----
-    for (int i = tid; i < items; i += team) {
-      const int h = i / (DH / 4), d = i % (DH / 4) * 4;
-      const int set = h / heads, from = sets == 1 ? 0 : 4 * set, to_warp = sets == 1 ? CONSUMERS : from + 4, at = h - set * heads;
-      float top = -1.0e30f, sum = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4                             // code that runs once comes from L2: short loops are faster than long straight lines
-      for (int x = from; x < to_warp; ++x) top = fmaxf(top, sm_ml[(x * heads + at) * 2]);
-#pragma unroll 4
-      for (int x = from; x < to_warp; ++x) {
-        const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (x * heads + at) * 2);
-        const float a = ex2(ml.x - top);
-        const float4 e = *reinterpret_cast<const float4*>(sm_o + (x * heads + at) * C::PITCH + d);
-        sum += ml.y * a;
-        v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
+    const int items = live * (DH / 4);
+    // The pieces of a job are joined in shares, piece i in share i % shares, and these in their order; how many there are follows from the
+    // heads (as many as the consumers have threads for). So which CTA does it, and which of its warps, does not show in the result.
+    const int shares = items <= 96 ? 4 : items <= 192 ? 2 : 1;
+    bool ready = false;                                  // all other pieces are there
+    if (consumes) {
+      if (tid == 0) {
+        *const_cast<volatile int*>(&s_end) = 1;
+        s_last[1] = *const_cast<volatile int*>(&s_ready);
       }
-      if (whole) {
-        write_out(i * 4, v, sum);
+      team_sync();
+      ready = s_last[1];
+    }
+    const int r_c0 = s_ready_join[0], r_own = static_cast<int>(blockIdx.x) - r_c0, r_pieces = ready ? s_ready_join[1] : 0;
+    ready = ready && r_pieces <= (shares == 1 ? SHARES : shares);      // a piece a share, or one share: they can be joined at once
+    // ---- the warps' sums are joined in the order of the warps ----
+    for (int base = tid & ~31; base < items; base += team) {
+      const int i = min(base + lane, items - 1), h = i / (DH / 4), set = h / heads, at = h - set * heads;
+      const int from = sets == 1 ? 0 : 4 * set, count = sets == 1 ? CONSUMERS : 4, x = lane & 15;
+      float4 other[SHARES];
+      float2 other_ml[SHARES];
+#pragma unroll
+      for (int k = 0; k < SHARES; ++k) {
+        other_ml[k] = make_float2(-1.0e30f, 0.f);
+        other[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ready && k < r_pieces && k != r_own) {
+          const float* src = part_of(2 * (r_c0 + k) + (k == 0));
+          other_ml[k] = __ldcg(reinterpret_cast<const float2*>(src + HEADS_MAX * DH + 2 * h));
+          other[k] = __ldcg(reinterpret_cast<const float4*>(src + i * 4));
+        }
+      }
+      // lane x has the weight of warp x
+      const float4 ml = x < count ? sm_ml[(from + x) * heads + at] : make_float4(-1.0e30f, 0.f, 0.f, 0.f);
+      float top = ml.x;
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float a = ex2(ml.x - top), weight = x < count ? a * ml.z : 0.f;
+      float sum = ml.y * a;
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = 0; k0 < count; k0 += 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float w = __shfl_sync(0xffffffffu, weight, (lane & 16) + k0 + k);
+          const float4 e = *reinterpret_cast<const float4*>(sm_o + ((from + k0 + k) * heads + at) * C::PITCH + i % (DH / 4) * 4);
+          v.x += e.x * w; v.y += e.y * w; v.z += e.z * w; v.w += e.w * w;
+        }
+      }
+      if (ready) {
+#pragma unroll
+        for (int k = 0; k < SHARES; ++k)
+          if (k == r_own) { other_ml[k] = make_float2(top, sum); other[k] = v; }
+        join_shares(other_ml, other, v, sum);
+      }
+      if (base + lane >= items) continue;
+      if (whole || ready) {
+        write_out(i, v, sum);
       } else {
         float* dst = part_of(2 * blockIdx.x + (t_beg == 0));
         *reinterpret_cast<float4*>(dst + i * 4) = v;
-        if (d == 0) *reinterpret_cast<float2*>(dst + HEADS_MAX * DH + 2 * h) = make_float2(top, sum);
+        if (i % (DH / 4) == 0) *reinterpret_cast<float2*>(dst + HEADS_MAX * DH + 2 * h) = make_float2(top, sum);
       }
+    }
+    if (ready) {
+      if (tid == 0) p.counters[to.counter] = 0;
+      return;
     }
     if (whole && last) return;
     team_sync();
@@ -593,70 +670,90 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     if (tid == 0) {
       unsigned int before;
       asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + to.counter) : "memory");
-      s_last[consumes] = before == static_cast<unsigned int>(n_pieces) - 1;
+      const Deal deal = s_deal;                          // while the count is under way
+      const int c0 = deal.cta(to.start), n = deal.cta(to.start + to.nt - 1) - c0 + 1;
+      s_join[consumes][0] = c0;
+      s_join[consumes][1] = n;
+      s_last[consumes] = before == static_cast<unsigned int>(n) - 1;
       if (s_last[consumes]) p.counters[to.counter] = 0;
     }
     team_sync();
     if (!s_last[consumes]) continue;
-    // The consumers of the last piece have room where the sums were, which have been read: several shares of the pieces at a time.
-    const int shares = consumes ? min(4, max(1, team / items)) : 1;
-    float* sm_v = sm_o;                                  // [shares][live][DH], then [shares][live][2]
-    float* sm_vml = sm_o + shares * live * DH;
-    for (int i = tid; i < items * shares; i += team) {
-      int share = 0, at = i;
-      while (at >= items) { at -= items; ++share; }
-      const int h = at / (DH / 4);
-      float top = -1.0e30f, sum = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = share; c < n_pieces; c += 8 * shares) {   // the loads of eight pieces are under way together
-        float2 ml[8];
-        float4 e[8];
+    const int c0 = s_join[consumes][0], n_pieces = s_join[consumes][1];
+    // item i of a share of the pieces: the loads of eight pieces are under way together
+    auto join_share = [&](int i, int share, float2& ml, float4& v) {
+      const int h = i / (DH / 4);
+      ml = make_float2(-1.0e30f, 0.f);
+      v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = share; c < n_pieces; c += 8 * shares) {
+        float2 next_ml[8];
+        float4 next[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int at_c = c + k * shares;
-          ml[k] = make_float2(-1.0e30f, 0.f);
-          if (at_c >= n_pieces) continue;
-          const float* src = part_of(2 * (c0 + at_c) + (at_c == 0));
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(src + HEADS_MAX * DH + 2 * h));
-          e[k] = __ldcg(reinterpret_cast<const float4*>(src + at * 4));
+          const int at = c + k * shares;
+          next_ml[k] = make_float2(-1.0e30f, 0.f);
+          next[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (at < n_pieces) {
+            const float* src = part_of(2 * (c0 + at) + (at == 0));
+            next_ml[k] = __ldcg(reinterpret_cast<const float2*>(src + HEADS_MAX * DH + 2 * h));
+            next[k] = __ldcg(reinterpret_cast<const float4*>(src + i * 4));
+          }
         }
-        float now = top;
+        float top = ml.x;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) now = fmaxf(now, ml[k].x);
-        const float keep = ex2(top - now);
-        top = now;
-        sum *= keep;
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, next_ml[k].x);
+        const float keep = ex2(ml.x - top);
+        ml.x = top;
+        ml.y *= keep;
         v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          if (c + k * shares >= n_pieces) continue;
-          const float a = ex2(ml[k].x - top);
-          sum += ml[k].y * a;
-          v.x += e[k].x * a; v.y += e[k].y * a; v.z += e[k].z * a; v.w += e[k].w * a;
+          const float a = ex2(next_ml[k].x - top);
+          ml.y += next_ml[k].y * a;
+          v.x += next[k].x * a; v.y += next[k].y * a; v.z += next[k].z * a; v.w += next[k].w * a;
         }
       }
-      if (shares == 1) {
-        write_out(at * 4, v, sum);
-      } else {
-        *reinterpret_cast<float4*>(sm_v + (share * items + at) * 4) = v;
-        if (at % (DH / 4) == 0) *reinterpret_cast<float2*>(sm_vml + (share * live + h) * 2) = make_float2(top, sum);
+    };
+    float4* sm_v = reinterpret_cast<float4*>(sm_o);          // [shares][items], then [shares][live]
+    float2* sm_vml = reinterpret_cast<float2*>(sm_v + shares * items);
+    const bool spread = consumes && shares > 1;              // of the last piece: there is room where the sums were, which have been read
+    if (spread) {
+      if (tid < items * shares) {
+        const int share = tid / items, i = tid - share * items;
+        float2 ml;
+        float4 v;
+        join_share(i, share, ml, v);
+        sm_v[tid] = v;
+        if (i % (DH / 4) == 0) sm_vml[share * live + i / (DH / 4)] = ml;
       }
+      team_sync();
     }
-    if (shares == 1) continue;
-    team_sync();
-    if (tid < items) {
-      const int h = tid / (DH / 4);
-      float top = -1.0e30f, sum = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int x = 0; x < shares; ++x) top = fmaxf(top, sm_vml[(x * live + h) * 2]);
-      for (int x = 0; x < shares; ++x) {
-        const float2 ml = *reinterpret_cast<const float2*>(sm_vml + (x * live + h) * 2);
-        const float a = ex2(ml.x - top);
-        const float4 e = *reinterpret_cast<const float4*>(sm_v + (x * items + tid) * 4);
-        sum += ml.y * a;
-        v.x += e.x * a; v.y += e.y * a; v.z += e.z * a; v.w += e.w * a;
+    for (int i = tid; i < items; i += team) {
+      float2 ml[SHARES];
+      float4 e[SHARES], v;
+      float sum;
+#pragma unroll
+      for (int k = 0; k < SHARES; ++k) {
+        ml[k] = make_float2(-1.0e30f, 0.f);
+        e[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (spread && k < shares) {
+          e[k] = sm_v[k * items + i];
+          ml[k] = sm_vml[k * live + i / (DH / 4)];
+        }
       }
-      write_out(tid * 4, v, sum);
+      if (!spread) {
+#pragma unroll 1
+        for (int k = 0; k < shares; ++k) {
+          float2 next_ml;
+          float4 next;
+          join_share(i, k, next_ml, next);
+#pragma unroll
+          for (int x = 0; x < SHARES; ++x)
+            if (x == k) { ml[x] = next_ml; e[x] = next; }
+        }
+      }
+      join_shares(ml, e, v, sum);
+      write_out(i, v, sum);
     }
   }
 }
@@ -714,7 +811,7 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   p.status = status;
   // the kernel leaves a tile to each group of consumers
   const long long want = p.sets == 1 ? (max_tiles + 2) / 3 : max_tiles;
-  const int most = num_sms() < kv8::GRID_MAX ? num_sms() : kv8::GRID_MAX, grid = want < most ? static_cast<int>(want) : most;
+  const int grid = want < num_sms() ? static_cast<int>(want) : num_sms();
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   if (dh == 64) return e4m3 ? kv8::launch_attend<64, true>(tm, p, grid, s) : kv8::launch_attend<64, false>(tm, p, grid, s);
   return e4m3 ? kv8::launch_attend<128, true>(tm, p, grid, s) : kv8::launch_attend<128, false>(tm, p, grid, s);

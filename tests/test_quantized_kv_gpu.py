@@ -364,6 +364,23 @@ def test_attention_output_rows_and_repeats():
     assert Q.decode_attention(**{**a, "q": a["q"][:0], "block_table": a["block_table"][:0], "seq_len": a["seq_len"][:0]}).shape == (0, 1024)
 
 
+def test_attention_bits_do_not_depend_on_timing():
+    """Which CTA joins a job's pieces, and when it sees the others, is a matter of time; the bits are not. Pieces of two, a few and many CTAs, beside
+    a stream that delays some of them."""
+    a = batch("int8", 32, 8, 128, 64, 16, [3000, 10, 700, 5000] + [64 * i for i in range(12)], dirty=False)
+    long = batch("e4m3", 4, 1, 128, 64, 16, [30000, 17], dirty=False, seed=1)
+    twenty = batch("int8", 20, 1, 64, 64, 16, [9000, 4000, 1], dirty=False, seed=2)
+    other, x = torch.cuda.Stream(), torch.randn((2048, 2048), device=DEV)
+    for args in (a, long, twenty):
+        want = Q.decode_attention(**args)
+        for i in range(12):
+            if i % 2:
+                with torch.cuda.stream(other):
+                    x @ x
+            assert torch.equal(Q.decode_attention(**args), want)
+    torch.cuda.synchronize()
+
+
 def test_lengths_behind_the_table_are_cut():
     a = batch("int8", 4, 2, 64, 16, 16, [48, 32], dirty=False)
     want = Q.decode_attention(**a)
