@@ -155,9 +155,9 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& x, uint32_t& y) {
 // Tiles of one sequence: an empty one keeps a tile without positions, whose job writes zeros.
 __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + TK - 1) / TK : 1; }
 
-// How the units (tiles of all jobs, end to end) are dealt out: the first `more` CTAs have one more than the others.
+// How the units (tiles of all jobs, end to end; or whole jobs) are dealt out: the first `more` CTAs have one more than the others.
 struct Deal {
-  int units, ctas, each, more;
+  int ctas, each, more, whole;
   __device__ __forceinline__ int first(int c) const { return c * each + min(c, more); }
   __device__ __forceinline__ int cta(int u) const {
     const int at = more * (each + 1);
@@ -228,7 +228,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     Deal deal;
     if (brings_codes) {
       const int cap = static_cast<int>(min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll - TK));
-      int base = 0;
+      int base = 0, longest = 0;
       int next = lane < p.B ? p.seq_len[lane] : 0;
       for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int len = min(next, cap);
@@ -242,29 +242,51 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         }
         if (b0 + lane < p.B) { prefix[b0 + lane] = base + inc - n; lens[b0 + lane] = len; }
         base += __shfl_sync(0xffffffffu, inc, 31);
+        longest = max(longest, n);
       }
-      deal.units = base * jobs_b;
-      deal.ctas = min(static_cast<int>(gridDim.x), sets == 1 ? (deal.units + GROUPS - 1) / GROUPS : deal.units);
-      deal.each = deal.units / deal.ctas;
-      deal.more = deal.units - deal.each * deal.ctas;
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      const int tiles = base * jobs_b, jobs = p.B * jobs_b, grid = gridDim.x;
+      deal.ctas = min(grid, sets == 1 ? (tiles + GROUPS - 1) / GROUPS : tiles);
+      deal.each = tiles / deal.ctas;
+      deal.whole = 0;
+      // What it costs to cut jobs (writing sums, asking for the count, reading them), at the end, where nothing else is under way, is as long as
+      // sixteen tiles: up to there jobs are dealt out whole. us cut / whole, 32 / 8 heads of 128: 1 x 600 positions 10.6 / 7.6, 4 x 800 11.4 / 9.1, 4 x
+      // 1600 (21 tiles more) 11.9 / 12.6, 16 x 300 11.5 / 7.0, 16 x 1500 15.5 / 12.6, 16 x 2500 19.3 / 17.6, 9 x 5003 of 4 / 1 heads 13.3 / 29.1.
+      const int ctas = min(grid, jobs), most = (jobs + ctas - 1) / ctas;
+      if (longest <= 4096 && most * longest - deal.each <= 16) {
+        deal.ctas = ctas;
+        deal.each = jobs / ctas;
+        deal.whole = 1;
+      }
+      deal.more = (deal.whole ? jobs : tiles) - deal.each * deal.ctas;
       if (lane == 0) { prefix[p.B] = base; s_deal = deal; }
     }
     asm volatile("bar.sync 3, 64;" ::: "memory");
     deal = s_deal;
     const bool idle = static_cast<int>(blockIdx.x) >= deal.ctas;
-    int left = idle ? 0 : deal.first(blockIdx.x + 1) - deal.first(blockIdx.x);              // units of the CTA to come
-    // the first piece: the last sequence whose first unit is not behind it, by steps of a 32nd of those left
-    const int u0 = idle ? 0 : deal.first(blockIdx.x);
-    int b = 0;
-    for (int n = p.B - 1; n > 0;) {
-      const int step = (n + 31) / 32, at = b + (lane + 1) * step;
-      const int c = __popc(__ballot_sync(0xffffffffu, at <= b + n && prefix[min(at, p.B)] * jobs_b <= u0));
-      b += c * step;
-      n = min(step - 1, n - c * step);
+    int b = 0, job = 0, t_beg = 0, left = 0;                                                // the first piece; units of the CTA to come
+    if (!idle) {
+      const int u0 = deal.first(blockIdx.x);
+      left = deal.first(blockIdx.x + 1) - u0;
+      if (deal.whole) {
+        b = u0 / jobs_b;
+        job = u0 - b * jobs_b;
+      } else {
+        // the last sequence whose first unit is not behind the CTA's, by steps of a 32nd of those left
+        for (int n = p.B - 1; n > 0;) {
+          const int step = (n + 31) / 32, at = b + (lane + 1) * step;
+          const int c = __popc(__ballot_sync(0xffffffffu, at <= b + n && prefix[min(at, p.B)] * jobs_b <= u0));
+          b += c * step;
+          n = min(step - 1, n - c * step);
+        }
+        t_beg = u0 - prefix[b] * jobs_b;
+        job = t_beg / tiles_of(lens[b]);
+        t_beg -= job * tiles_of(lens[b]);
+      }
     }
-    int len = lens[b], nt = tiles_of(len), start = prefix[b] * jobs_b, job = (u0 - start) / nt;
+    int len = lens[b], nt = tiles_of(len), start = prefix[b] * jobs_b;
     start += job * nt;
-    int t_beg = u0 - start, kvh = p.subs == 1 ? job : job / p.subs, sub = job - kvh * p.subs;
+    int kvh = p.subs == 1 ? job : job / p.subs, sub = job - kvh * p.subs;
 
     const int box_bits = min(p.page_bits, 6), box = 1 << box_bits, nbx = TK >> box_bits;    // positions of a TMA box, boxes of a tile
     // of a tile, a lane has one box of codes of keys or values (eight boxes of each at most), or one scale, of eight positions
@@ -278,58 +300,59 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     int stage = 0, q_slot = 0;
     uint32_t phase = 0, q_phase = 0;
     do {
-      const int t_end = min(nt, t_beg + left);
-      left -= t_end - t_beg;
+      const int t_end = deal.whole ? nt : min(nt, t_beg + left);
+      left -= deal.whole ? 1 : t_end - t_beg;
+      const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
+      // of box (fetched + lane) of the sequence: its first row of keys, or their scale
+      int fetched = t_beg * nbx, at_of_lane;
+      auto fetch = [&] {
+        const long long pos = static_cast<long long>(fetched + lane) << box_bits;
+        at_of_lane = -1;
+        if (pos < len) {
+          const int at = static_cast<int>(pos) / p.page, slot = static_cast<int>(pos) - at * p.page, id = table[at];
+          if (static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks)) at_of_lane = (id * 2 * p.Hkv + kvh) * unit + (slot >> slot_bits);
+        }
+      };
+      if (!idle) fetch();                                // while the queries are seen to
       if (brings_codes) {
-        if (!mbar_wait_warp(&q_empty[q_slot], q_phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) break;
+        mbar_wait_converged(&q_empty[q_slot], q_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
         if (lane == 0) {
           const int h0 = kvh * p.G + sub * sets * heads, live = min(sets * heads, p.G - sub * sets * heads);
-          Piece* to = pieces + q_slot;
-          to->b = b; to->h0 = h0; to->live = live; to->len = len;
-          to->t_beg = t_beg; to->t_end = t_end; to->nt = nt; to->last = left == 0;
-          to->start = start; to->counter = b * jobs_b + job;
-          mbar_arrive_expect_tx(&q_full[q_slot], idle ? 0 : live * DH * 2);
           if (!idle)
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                         ::"r"(smem_u32(sm_q + q_slot * sets * heads * DH)), "l"(p.q + b * p.ldq + static_cast<long long>(h0) * DH), "r"(live * DH * 2),
-                         "r"(smem_u32(&q_full[q_slot])) : "memory");
+                         ::"r"(smem_u32(sm_q + q_slot * sets * heads * DH)), "l"(p.q + b * p.ldq + static_cast<long long>(h0) * DH),
+                         "r"(live * DH * 2), "r"(smem_u32(&q_full[q_slot])) : "memory");
+          Piece* to = pieces + q_slot;
+          to->b = b; to->h0 = h0; to->live = live; to->len = len;
+          to->t_beg = t_beg; to->t_end = idle ? t_beg : t_end; to->nt = nt; to->last = left <= 0;
+          to->start = start; to->counter = b * jobs_b + job;
+          mbar_arrive_expect_tx(&q_full[q_slot], idle ? 0 : live * DH * 2);
         }
         if (++q_slot == C::QSLOTS) { q_slot = 0; q_phase ^= 1; }
       }
       if (idle) break;
-      const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
-      int at_of_lane = -1;                               // of box (fetched + lane): its first row of keys, or their scale
-      int fetched = -1000000;
-      bool ok = true;
       for (int t = t_beg; t < t_end; ++t) {
         const int bx0 = t * nbx;
         if (bx0 + nbx > fetched + 32) {                  // nbx divides 32: a tile's boxes are fetched together
           fetched = bx0;
-          const long long pos = static_cast<long long>(fetched + lane) << box_bits;
-          at_of_lane = -1;
-          if (pos < len) {
-            const int at = static_cast<int>(pos) / p.page, slot = static_cast<int>(pos) - at * p.page, id = table[at];
-            if (static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks)) at_of_lane = (id * 2 * p.Hkv + kvh) * unit + (slot >> slot_bits);
-          }
+          fetch();
         }
         const int base = __shfl_sync(0xffffffffu, at_of_lane, bx0 + x - fetched);
         const int at = base < 0 ? none : base + step, rest = len - t * TK;                  // positions of the tile that exist, or more
-        if (!mbar_wait_warp(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        const int live = rest >= TK ? nbx : max(0, (rest + box - 1) >> box_bits);           // boxes with one of them
+        mbar_wait_converged(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
         if (brings_codes) {
-          const int live = rest >= TK ? nbx : max(0, (rest + box - 1) >> box_bits);         // boxes with a position that exists
-          if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
-          __syncwarp();
+          // the stage is not full before lane 0 has arrived, whichever comes first, its bytes or that they are expected
           if (x < live) tma_load_2d(ring + stage * 2 * C::TILE + v * C::TILE + first * DH, &tmap, &full[stage], 0, at);
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
         } else if (lane < 16) {
           const bool real = first < rest && at >= 0;
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 16 + lane)), "l"(p.scales + (real ? at : 0)),
                        "r"(real ? 4 : 0) : "memory");
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
         }
-        __syncwarp();
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
-      if (!ok) break;
       start += nt;                                       // the next job's
       t_beg = 0;
       if (++sub == p.subs) { sub = 0; ++kvh; }
@@ -611,7 +634,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     ready = ready && r_pieces <= (shares == 1 ? SHARES : shares);      // a piece a share, or one share: they can be joined at once
     // ---- the warps' sums are joined in the order of the warps ----
     for (int base = tid & ~31; base < items; base += team) {
-      const int i = min(base + lane, items - 1), h = i / (DH / 4), set = h / heads, at = h - set * heads;
+      const int i = min(base + lane, items - 1), h = i / (DH / 4), set = (h >= heads) + (h >= 2 * heads), at = h - set * heads;
       const int from = sets == 1 ? 0 : 4 * set, count = sets == 1 ? CONSUMERS : 4, x = lane & 15;
       float4 other[SHARES];
       float2 other_ml[SHARES];
@@ -810,7 +833,7 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.status = status;
   // the kernel leaves a tile to each group of consumers
-  const long long want = p.sets == 1 ? (max_tiles + 2) / 3 : max_tiles;
+  const long long shared = p.sets == 1 ? (max_tiles + 2) / 3 : max_tiles, jobs = static_cast<long long>(B) * Hkv * p.subs, want = shared > jobs ? shared : jobs;
   const int grid = want < num_sms() ? static_cast<int>(want) : num_sms();
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   if (dh == 64) return e4m3 ? kv8::launch_attend<64, true>(tm, p, grid, s) : kv8::launch_attend<64, false>(tm, p, grid, s);
