@@ -1,7 +1,7 @@
 #!/usr/bin/env python
 """Inference benchmark at Llama-3-8B shape (32 layers, d 4096, 32 query / 8 KV heads, head_dim 128,
 SwiGLU 14336, vocab 128256, RoPE theta 5e5, random-init bf16 weights): prefill of ``--prompt``
-synthetic tokens, then greedy decode of ``--new`` tokens with a paged bf16 KV cache, at batch
+synthetic tokens, then greedy decode of ``--new`` tokens with a paged KV cache (bf16, or 8 bits with ``--kv``), at batch
 ``--batch``; bf16 or int8 per-output-channel weights. Reports p50 time-to-first-token (prefill +
 first arg-max + device->host copy of the token) and decode tokens/s (CUDA-graph replay, device-side
 token feedback), timed with CUDA events.
@@ -35,6 +35,7 @@ def main():
     ap.add_argument("--prompt", type=int, default=2048)
     ap.add_argument("--new", type=int, default=256)
     ap.add_argument("--quant", default="none", choices=["none", "int8"])
+    ap.add_argument("--kv", default="none", choices=["none", "int8", "e4m3"], help="keys and values of the cache in 8 bits")
     ap.add_argument("--ttft-iters", type=int, default=5)
     ap.add_argument("--layers", type=int, default=0, help="override the layer count (smoke runs)")
     ap.add_argument("--graph", type=int, default=1, help="0: launch every decode step eagerly (for launch lists)")
@@ -58,13 +59,13 @@ def main():
     if a.tp > 1:
         from scirust_b200.models.infer_tp import TPInferenceEngine
         eng = TPInferenceEngine(model, quant=quant, max_batch=a.batch, max_seq=a.prompt + a.new + 1, page=64,
-                                use_graph=bool(a.graph), backend=a.comm)
+                                use_graph=bool(a.graph), backend=a.comm, kv=None if a.kv == "none" else a.kv)
         n_params = model.num_params()
         del model                      # the shards are copies; free the full weights
         torch.cuda.empty_cache()
     else:
         eng = InferenceEngine(model, quant=quant, max_batch=a.batch, max_seq=a.prompt + a.new + 1, page=64,
-                              use_graph=bool(a.graph))
+                              use_graph=bool(a.graph), kv=None if a.kv == "none" else a.kv)
         n_params = model.num_params()
     g = torch.Generator().manual_seed(0)
     prompts = torch.randint(0, cfg.vocab_size, (a.batch, a.prompt), generator=g).pin_memory()
@@ -103,7 +104,7 @@ def main():
     _lib.check_status(dev)
     if rank == 0:
         print(json.dumps({"metric": "inference", "model": a.model, "layers": cfg.n_layers, "batch": a.batch,
-                          "prompt": a.prompt, "new_tokens": a.new, "quant": a.quant, "tp": a.tp,
+                          "prompt": a.prompt, "new_tokens": a.new, "quant": a.quant, "kv": a.kv, "tp": a.tp,
                           "comm": a.comm if a.tp > 1 else "none", "ttft_p50_ms": p50,
                           "decode_tok_s": a.batch * (a.new - 1) / (decode_ms / 1e3),
                           "decode_ms_per_step": decode_ms / (a.new - 1), "total_ms": total_ms,

@@ -166,7 +166,7 @@ def cmd_infer(a):
     if samples < 1:
         sys.stderr.write("error: --samples must be positive\n")
         return EXIT_VALIDATION
-    eng = InferenceEngine(model, quant=a.quant, max_batch=samples, max_seq=len(ids) + a.max_new + 1)
+    eng = InferenceEngine(model, quant=a.quant, max_batch=samples, max_seq=len(ids) + a.max_new + 1, kv=a.kv)
     params = SamplingParams(a.temperature, a.top_k, a.top_p, a.repetition_penalty)
     if samples == 1:
         outs = eng.generate(torch.tensor([ids]), a.max_new, params, seed=a.seed).tolist()
@@ -654,7 +654,7 @@ def _sciagent_reply(a, prompt_text, max_new):
     ids = [min(i, model.cfg.vocab_size - 1) for i in ids][-(model.cfg.max_seq_len - max_new - 1):]
     if not ids:
         raise ValueError("empty prompt")
-    eng = InferenceEngine(model, quant=a.quant, max_batch=1, max_seq=len(ids) + max_new + 1)
+    eng = InferenceEngine(model, quant=a.quant, max_batch=1, max_seq=len(ids) + max_new + 1, kv=a.kv)
     params = SamplingParams(a.temperature, a.top_k, a.top_p, a.repetition_penalty)
     out = eng.generate(torch.tensor([ids]), max_new, params, seed=a.seed)[0].tolist()
     if 0 in out:
@@ -752,6 +752,7 @@ def build_parser():
         sp.add_argument("--repetition-penalty", type=float, default=1.0)
         sp.add_argument("--seed", type=int, default=0)
         sp.add_argument("--quant", default=None, choices=[None, "int8"])
+        sp.add_argument("--kv", default=None, choices=[None, "int8", "e4m3"], help="keys and values of the cache in 8 bits")
         sp.add_argument("--device", default="auto")
     i = sub.add_parser("infer")
     gen_args(i)

@@ -1,5 +1,5 @@
-"""Inference engine for the SciAgent / Llama-shaped GQA decoder: batched flash prefill, paged bf16
-KV cache, split-KV flash-decode, bf16 or int8 per-output-channel weights, device-side greedy
+"""Inference engine for the SciAgent / Llama-shaped GQA decoder: batched flash prefill, paged
+KV cache in bf16 or 8 bits, split-KV flash-decode, bf16 or int8 per-output-channel weights, device-side greedy
 feedback (no per-token device->host copy) and CUDA-graph replay of the decode step.
 
 Counterparts in the reference: ``CudaModel::prefill_cached`` / ``decode_step_cached`` /
@@ -24,7 +24,7 @@ import torch
 from .. import ops
 from ..generate import SamplingParams
 from ..ops.sampling import DeviceSampler
-from ..ops import _lib, attention as att, decode as D, gemm as G, paged
+from ..ops import _lib, attention as att, decode as D, gemm as G, paged, quantized_kv as Q
 from .sciagent import BF, GQADecoder, SciAgentConfig
 
 
@@ -103,12 +103,17 @@ class BlockAllocator:
 
 
 class PagedKVCache:
-    """Pools ``[n_layers][n_blocks, 2, Hkv, page, dh]`` (bf16) + block table + lengths."""
+    """Pools ``[n_layers][n_blocks, 2, Hkv, page, dh]`` (bf16, or with ``codes`` 8-bit ``QuantPool``s, whose scales count for ``block`` positions) +
+    block table + lengths."""
 
-    def __init__(self, n_layers, n_blocks, Hkv, dh, page, max_batch, max_seq, device):
+    def __init__(self, n_layers, n_blocks, Hkv, dh, page, max_batch, max_seq, device, codes=None, block=None):
         self.page, self.max_batch = page, max_batch
         self.max_blocks = (max_seq + page - 1) // page
-        self.pools = [torch.zeros((n_blocks, 2, Hkv, page, dh), dtype=BF, device=device) for _ in range(n_layers)]
+        self.quantized = codes is not None
+        if self.quantized:
+            self.pools = [Q.QuantPool.zeros(n_blocks, Hkv, page, dh, codes, block, device) for _ in range(n_layers)]
+        else:
+            self.pools = [torch.zeros((n_blocks, 2, Hkv, page, dh), dtype=BF, device=device) for _ in range(n_layers)]
         self.alloc = BlockAllocator(n_blocks)
         self.table_host = torch.zeros((max_batch, self.max_blocks), dtype=torch.int32)
         self.block_table = torch.zeros((max_batch, self.max_blocks), dtype=torch.int32, device=device)
@@ -134,6 +139,15 @@ class PagedKVCache:
         self.owned[seq] = []
         self.table_host[seq].zero_()
 
+    def _copy_pages(self, src, dst, rows=None, pools=None, to=None) -> None:
+        """``paged.copy_pages`` in the layers' pools, with 8 bits of codes (their first ``rows``) and of all scales."""
+        pools = self.pools if pools is None else pools
+        if not self.quantized:
+            return paged.copy_pages(paged.PagePools(pools), src, dst, rows=rows, out=paged.PagePools(to) if to is not None else None)
+        for part, n in ((0, rows), (1, None)):
+            parts = [[p[part].view(torch.uint8) if part == 0 else p[part] for p in side] if side is not None else None for side in (pools, to)]
+            paged.copy_pages(paged.PagePools(parts[0]), src, dst, rows=n, out=paged.PagePools(parts[1]) if to is not None else None)
+
     def fork(self, src: int, seqs, n_tokens: int) -> None:
         """Gives the sequences ``seqs``, which have no pages, the first ``n_tokens`` positions of ``src``. Whole pages are shared: each counts
         its owners and is free again with the last of them. A page that the positions do not fill is copied for every sequence, as far as it is
@@ -150,7 +164,7 @@ class PagedKVCache:
             self.owned[s] = self.owned[src][:whole] + last[i:i + 1]
             self.table_host[s, :len(self.owned[s])] = torch.tensor(self.owned[s], dtype=torch.int32)
         if last:
-            paged.copy_pages(paged.PagePools(self.pools), [self.owned[src][whole]] * len(seqs), last, rows=rest)
+            self._copy_pages([self.owned[src][whole]] * len(seqs), last, rows=rest)
 
     def _renumber(self, to) -> None:
         for s, ids in enumerate(self.owned):
@@ -164,7 +178,7 @@ class PagedKVCache:
         of a row of ``block_table``, the page ids of a shared prefix) have to be read again."""
         to = self.alloc.compact()
         moves = [(a, b) for a, b in enumerate(to) if b not in (-1, a)]
-        paged.copy_pages(paged.PagePools(self.pools), [a for a, _ in moves], [b for _, b in moves])
+        self._copy_pages([a for a, _ in moves], [b for _, b in moves])
         self._renumber(to)
         return sum(b >= 0 for b in to)
 
@@ -175,10 +189,14 @@ class PagedKVCache:
         live = self.alloc.n_blocks - self.alloc.num_free()
         if n_blocks < max(live, 1):
             raise MemoryError(f"{live} pages in use do not fit into {n_blocks}")
-        new = [torch.zeros((n_blocks, *p.shape[1:]), dtype=p.dtype, device=p.device) for p in old]
+        def empty(t):
+            return torch.zeros((n_blocks, *t.shape[1:]), dtype=torch.uint8, device=t.device).view(t.dtype) if t.element_size() == 1 else \
+                torch.zeros((n_blocks, *t.shape[1:]), dtype=t.dtype, device=t.device)
+
+        new = [Q.QuantPool(empty(p.codes), empty(p.scales)) if self.quantized else empty(p) for p in old]
         to = self.alloc.compact(n_blocks)
         pairs = [(a, b) for a, b in enumerate(to) if b >= 0]
-        paged.copy_pages(paged.PagePools(old), [a for a, _ in pairs], [b for _, b in pairs], out=paged.PagePools(new))
+        self._copy_pages([a for a, _ in pairs], [b for _, b in pairs], pools=old, to=new)
         self.pools[:] = new
         self._renumber(to)
 
@@ -252,7 +270,9 @@ class _WidenAhead:
 
 class InferenceEngine:
     def __init__(self, model: GQADecoder, quant: str | None = None, max_batch: int = 1, max_seq: int = 4096,
-                 page: int = 64, use_graph: bool = True):
+                 page: int = 64, use_graph: bool = True, kv: str | None = None, kv_block: int | None = None):
+        """``quant="int8"``: int8 weights. ``kv="int8"`` or ``"e4m3"``: a cache of half the size in 8 bits, one scale for ``kv_block`` positions of
+        a head (default: 16); decoding reads half the bytes, and what the cache holds is rounded once more."""
         cfg = model.cfg
         self.cfg, self.quant = cfg, quant
         dev = model.flat.device
@@ -263,7 +283,10 @@ class InferenceEngine:
         self.H, self.Hkv = cfg.n_heads, cfg.n_kv_heads      # heads held by this rank
         self._load_weights(model)
         n_blocks = max_batch * ((max_seq + page - 1) // page)
-        self.cache = PagedKVCache(cfg.n_layers, n_blocks, self.Hkv, cfg.head_dim, page, max_batch, max_seq, dev)
+        self.kv = kv
+        if kv is not None and dev.type == "cuda" and (page not in (8, 16, 32) and page % 64 or cfg.head_dim not in (64, 128)):
+            raise ValueError("a cache in 8 bits has pages of 8, 16, 32 or a multiple of 64 positions and heads of 64 or 128")
+        self.cache = PagedKVCache(cfg.n_layers, n_blocks, self.Hkv, cfg.head_dim, page, max_batch, max_seq, dev, kv, kv_block)
         self.cos, self.sin = ops.rope_table(max(cfg.max_seq_len, max_seq), cfg.head_dim, cfg.rope_theta, dev)
         self.tokens = torch.zeros(max_batch, dtype=torch.int64, device=dev)     # device feedback buffer
         self.logits = torch.zeros((max_batch, cfg.vocab_size), dtype=torch.float32, device=dev)
@@ -350,8 +373,10 @@ class InferenceEngine:
         cache.commit()
         seq_of = torch.arange(B, dtype=torch.int32, device=self.dev).repeat_interleave(P)
         pos = torch.arange(P, dtype=torch.int32, device=self.dev).repeat(B)
+        runs = (torch.full((B,), P, dtype=torch.int32, device=self.dev),
+                torch.arange(0, B * P + 1, P, dtype=torch.int32, device=self.dev)) if self.kv is not None else None
         x = self._prompt_layers(tok.reshape(-1), seq_of, pos,
-                                lambda li, qkv: att.attention_fwd(qkv, B, P, H, Hkv, dh, causal=True, want_lse=False)[0])
+                                lambda li, qkv: att.attention_fwd(qkv, B, P, H, Hkv, dh, causal=True, want_lse=False)[0], runs)
         last = x.view(B, P, -1)[:, -1, :].contiguous()
         logits = self.logits[:B]
         self._head(last, logits, rms_weight=self.rms_final)
@@ -359,9 +384,10 @@ class InferenceEngine:
         cache.seq_len[:B] = P
         return logits
 
-    def _prompt_layers(self, tok, seq_of, pos, attend):
+    def _prompt_layers(self, tok, seq_of, pos, attend, runs=None):
         """All layers over prompt tokens: ``tok`` [n], token i at position ``pos[i]`` of sequence ``seq_of[i]``. Keys and values go to the
-        cache, then ``attend(layer, qkv)`` is the attention. Returns the residual stream [n, d]."""
+        cache, then ``attend(layer, qkv)`` is the attention. ``runs``: the same places as each sequence's length with its tokens, and where in
+        ``tok`` it begins, [B + 1] (for a cache in 8 bits). Returns the residual stream [n, d]."""
         cfg, cache = self.cfg, self.cache
         H, Hkv, dh, n = self.H, self.Hkv, cfg.head_dim, tok.shape[0]
         x = ops.embed_fwd(self.embed, tok)
@@ -374,7 +400,10 @@ class InferenceEngine:
             h, _ = ops.rmsnorm_fwd(x, l["rms1"], cfg.eps, want_inv=False)
             w, kw = plan.product(l["wqkv"])
             qkv = self._linear(h, w, **kw)
-            D.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table, cache.page, seq_of, pos)
+            if self.kv is None:
+                D.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table, cache.page, seq_of, pos)
+            else:
+                Q.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table[:runs[0].shape[0]], *runs)
             a = attend(li, qkv)
             w, kw = plan.product(l["wo"])
             return self._proj_out(a, w, x, site="attn", **kw)
@@ -431,14 +460,19 @@ class InferenceEngine:
             else:
                 h, _ = ops.rmsnorm_fwd(x, l["rms1"], cfg.eps, want_inv=False)
                 qkv = self._linear(h, l["wqkv"])
-            D.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table, cache.page,
-                             seq_of, pos)
-            if self._shared is not None:
-                a = paged.shared_prefix_attention(qkv, cache.pools[li], cache.block_table[:B], cache.page, self._len_plus1[:B], *self._shared,
-                                                  H, Hkv, dh, max_len=max_len)
+            if self.kv is not None:
+                table, lens = cache.block_table[:B], self._len_plus1[:B]
+                Q.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], table, lens)
+                a = Q.decode_attention(qkv, cache.pools[li], table, lens, H, Hkv, dh, max_len=max_len)
             else:
-                a = D.decode_attention(qkv, cache.pools[li], cache.block_table, cache.page, self._len_plus1[:B], H, Hkv,
-                                       dh, max_len=max_len, stream=stream)
+                D.rope_kv_append(qkv, H, Hkv, dh, self.cos, self.sin, cache.pools[li], cache.block_table, cache.page,
+                                 seq_of, pos)
+                if self._shared is not None:
+                    a = paged.shared_prefix_attention(qkv, cache.pools[li], cache.block_table[:B], cache.page, self._len_plus1[:B],
+                                                      *self._shared, H, Hkv, dh, max_len=max_len)
+                else:
+                    a = D.decode_attention(qkv, cache.pools[li], cache.block_table, cache.page, self._len_plus1[:B], H, Hkv,
+                                           dh, max_len=max_len, stream=stream)
             x = self._proj_out(a, l["wo"], x, site="attn")
             if small:
                 gu = D.gemv(x, l["wgu"], rms_weight=l["rms2"], eps=cfg.eps)
@@ -475,7 +509,7 @@ class InferenceEngine:
     def _streams(self, B: int, held: int) -> bool:
         """Which of the two decode-attention kernels suits ``B`` sequences of ``held`` positions (the cap that they may grow
         to does not count: the first part of a long generation is short)."""
-        return (self.dev.type == "cuda"
+        return (self.dev.type == "cuda" and self.kv is None
                 and D._stream_wins(held, B * self.Hkv, self.H // self.Hkv, self.cache.page, self.dev))
 
     # A generation that crosses the line between the two kernels captures its step anew (two or three milliseconds for eight
@@ -558,6 +592,7 @@ class InferenceEngine:
                 graphs[-1].replay()
                 out[:, i] = self.tokens[:B]
             paged.drop_workspace(self.dev, s.cuda_stream)       # of the eager step; the graphs have their own
+            Q.drop_workspace(self.dev, s.cuda_stream)
         else:
             for i in range(1, max_new):
                 if crosses(i):
@@ -636,7 +671,7 @@ class InferenceEngine:
             sampler.sample(logits, out_tokens=self.tokens[:B])
             sampler.push(self.tokens[:B])
         cache.seq_len[:B] = torch.tensor([P + n for n in lens], dtype=torch.int32, device=dev)
-        self._shared = shared if self._shares(B, P) else None
+        self._shared = shared if self.kv is None and self._shares(B, P) else None      # that attention reads pages in bf16
         try:
             return self._decode_steps(B, longest, max_new, sampler)
         finally:
@@ -656,9 +691,24 @@ class InferenceEngine:
         seq_of = torch.arange(B, dtype=torch.int32).repeat_interleave(n.long())
         pos = torch.arange(tok.numel(), dtype=torch.int32) - ends[:-1].repeat_interleave(n.long()) + P
         seq_of, pos, cu, total = seq_of.to(dev), pos.to(torch.int32).to(dev), ends.to(dev), (n + P).to(dev)
+        table, (prefix_table, _), pool = cache.block_table[:B], shared, cache.pools.__getitem__
+        if self.kv is not None:
+            # the attention over runs of rows reads bf16: a layer's pages of these sequences are read back, under numbers of their own
+            pages = [cache.owned[b][:-(-(P + k) // cache.page)] for b, k in enumerate(lens)]
+            number = {page: i for i, page in enumerate(dict.fromkeys(sum(pages, [])))}
+            rows = torch.zeros((B, cache.max_blocks), dtype=torch.int32)
+            for b, ids in enumerate(pages):
+                rows[b, :len(ids)] = torch.tensor([number[page] for page in ids], dtype=torch.int32)
+            table = rows.to(dev)
+            prefix_table = table[0, :P // cache.page].contiguous()
+            ids = torch.tensor(list(number), dtype=torch.int32, device=dev)
+            back = torch.empty((len(number), 2, self.Hkv, cache.page, self.cfg.head_dim), dtype=BF, device=dev)
+
+            def pool(li):
+                return Q.read_pages(cache.pools[li], ids, out=back)
         x = self._prompt_layers(tok, seq_of, pos, lambda li, qkv: paged.shared_prefix_attention(
-            qkv, cache.pools[li], cache.block_table[:B], cache.page, total, *shared, self.H, self.Hkv, self.cfg.head_dim, cu_q=cu,
-            max_len=P + max(lens)))
+            qkv, pool(li), table, cache.page, total, prefix_table, P, self.H, self.Hkv, self.cfg.head_dim, cu_q=cu, max_len=P + max(lens)),
+            (total, cu))
         some = [b for b in range(B) if lens[b]]
         last = x[torch.tensor([int(ends[b + 1]) - 1 for b in some], device=dev)].contiguous()
         got = torch.empty((len(some), out.shape[1]), dtype=out.dtype, device=dev)

@@ -37,7 +37,8 @@ def _cols(w, parts):
 
 class TPInferenceEngine(InferenceEngine):
     def __init__(self, model: GQADecoder, group=None, quant: str | None = None, max_batch: int = 1,
-                 max_seq: int = 4096, page: int = 64, use_graph: bool = True, backend: str = "fused"):
+                 max_seq: int = 4096, page: int = 64, use_graph: bool = True, backend: str = "fused",
+                 kv: str | None = None, kv_block: int | None = None):
         self.group = group if group is not None else dist.group.WORLD
         self.rank = dist.get_rank(self.group)
         self.world = dist.get_world_size(self.group)
@@ -81,7 +82,7 @@ class TPInferenceEngine(InferenceEngine):
             from ..parallel.small_collectives import ArgmaxChannel
             self.amax_chan = ArgmaxChannel(self.region)
         super().__init__(model, quant=quant, max_batch=max_batch, max_seq=max_seq, page=page,
-                         use_graph=use_graph and self.backend == "fused")
+                         use_graph=use_graph and self.backend == "fused", kv=kv, kv_block=kv_block)
         self.vocab_local = cfg.vocab_size // W
         self.logits_local = self.coll.source("logits", (max_batch, self.vocab_local), torch.float32, device=dev)
 

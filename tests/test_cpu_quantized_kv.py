@@ -4,7 +4,10 @@ import math
 import pytest
 import torch
 
-from scirust_b200.ops import quantized_kv as Q
+from scirust_b200.generate import SamplingParams
+from scirust_b200.models.infer import InferenceEngine, PagedKVCache, teacher_forced_logits
+from scirust_b200.models.sciagent import GQADecoder, SciAgentConfig
+from scirust_b200.ops import decode as D, quantized_kv as Q
 
 BF, F64 = torch.bfloat16, torch.float64
 KINDS = ["int8", "e4m3"]
@@ -208,3 +211,131 @@ def test_refusals():
         refused(Q.QuantPool.zeros, **{**dict(n_blocks=1, Hkv=1, page=8, dh=16, device="cpu"), **bad})
     assert Q.read_pages(pool, []).shape == (0, 2, Hkv, page, dh)
     assert Q.QuantPool.zeros(3, 2, 64, 128, device="cpu").nbytes() == 3 * 2 * 2 * 64 * (128 + 4 / 16)
+
+
+# ---------------------------------------------------------------------------------------------------------------- the engine
+@pytest.fixture(scope="module")
+def model():
+    return GQADecoder(SciAgentConfig(64, 32, 2, 4, 2, 48, 64, 10000.0), seed=5, init_std=0.3)
+
+
+def read_all(pool):
+    return Q.read_pages(pool, list(range(pool.codes.shape[0])))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_engine_steps_attend_to_what_the_cache_holds(model, kind, monkeypatch):
+    """A step over the cache in 8 bits, and the same step of an engine whose bf16 cache is given the values that the codes stand for."""
+    prompts = torch.randint(1, 64, (3, 11), generator=torch.Generator().manual_seed(0))
+    tokens = torch.randint(1, 64, (3, 5), generator=torch.Generator().manual_seed(1))
+    eng = InferenceEngine(model, max_batch=3, max_seq=32, page=16, kv=kind, kv_block=8)
+    got = teacher_forced_logits(eng, prompts, tokens)
+    other = InferenceEngine(model, max_batch=3, max_seq=32, page=16)
+    other.prefill(prompts)
+    for b in range(3):
+        other.cache.reserve(b, 17)
+    other.cache.commit()
+    assert torch.equal(other.cache.block_table, eng.cache.block_table)
+    other.cache.pools[:] = [read_all(p) for p in eng.cache.pools]
+    other.cache.seq_len[:3] = 15
+    other._seq_of, other._len_plus1, other._generated = torch.arange(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), None
+    other.tokens[:3] = tokens[:, 4]
+    append = D.rope_kv_append
+
+    def only_rotate(qkv, H, Hkv, dh, cos, sin, pool, *rest):
+        append(qkv, H, Hkv, dh, cos, sin, pool.clone(), *rest)
+
+    monkeypatch.setattr(D, "rope_kv_append", only_rotate)
+    other._step_eager(3, 17, want_logits=True)
+    assert torch.equal(other.logits[:3].float(), got[:, 4])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_engine_generates(model, kind):
+    prompts = torch.randint(1, 64, (2, 13), generator=torch.Generator().manual_seed(2))
+    eng = InferenceEngine(model, max_batch=4, max_seq=40, page=8, kv=kind)
+    whole = eng.generate(prompts, 9)
+    assert whole.shape == (2, 9) and torch.equal(whole, eng.generate(prompts, 9))
+    alone = InferenceEngine(model, max_batch=1, max_seq=40, page=8, kv=kind)
+    assert torch.equal(alone.generate(prompts[1:], 9), whole[1:])
+    # sequences behind a common prefix: without suffixes the pages are the prompt's
+    assert torch.equal(eng.generate_shared(prompts[0], 3, 9), whole[:1].expand(3, -1))
+    suffixes = [torch.tensor([3, 4, 5]), torch.tensor([], dtype=torch.int64), torch.arange(1, 12)]
+    for params in (None, SamplingParams(0.8, 10, 0.9)):
+        out = eng.generate_shared(prompts[0], suffixes, 6, params, seed=1)
+        assert out.shape == (3, 6) and torch.equal(out, eng.generate_shared(prompts[0], suffixes, 6, params, seed=1))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_suffixes_attend_to_the_pages_read_back(model, kind, monkeypatch):
+    """The pass over suffixes gives what it gives on a bf16 cache that holds the codes' values, with the suffixes' own as well."""
+    from scirust_b200.ops import paged
+    prefix, suffixes = torch.arange(1, 20), [torch.tensor([3, 4, 5]), torch.arange(20, 31)]
+    seen = []
+    attend = paged.shared_prefix_attention
+
+    def watch(q, pool, table, page, total, prefix_table, P, *a, **kw):
+        out = attend(q, pool, table, page, total, prefix_table, P, *a, **kw)
+        seen.append((pool.clone(), table, prefix_table, out))
+        return out
+
+    monkeypatch.setattr(paged, "shared_prefix_attention", watch)
+    eng = InferenceEngine(model, max_batch=2, max_seq=40, page=8, kv=kind)
+    eng.generate_shared(prefix, suffixes, 1)
+    assert len(seen) == 2
+    c = eng.cache
+    for li, (pool, table, prefix_table, _) in enumerate(seen):
+        every = read_all(c.pools[li])
+        assert prefix_table.tolist() == table[0, :2].tolist() == table[1, :2].tolist()
+        for b, n in enumerate((22, 30)):
+            pages = -(-n // 8)
+            assert torch.equal(pool[table[b, :pages].long()], every[c.owned[b][:pages]])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_cache_forks_compacts_and_grows(kind):
+    H, Hkv, dh, page = 1, 2, 16, 16
+    cache = PagedKVCache(2, 9, Hkv, dh, page, 4, 48, torch.device("cpu"), kind, 8)
+    for seq, n in ((3, 5), (0, 43)):
+        cache.reserve(seq, n)
+    cache.commit()
+    lens, cu = torch.tensor([43, 0, 0, 5]).int(), torch.tensor([0, 43, 43, 43, 48]).int()
+    for li, pool in enumerate(cache.pools):
+        Q.kv_append(rows(48, H, Hkv, dh, seed=li), H, Hkv, dh, pool, cache.block_table, lens, cu_q=cu)
+
+    def held(li, seq, n):
+        v = Q.read_pages(cache.pools[li], cache.owned[seq]).permute(1, 2, 0, 3, 4).reshape(2, Hkv, -1, dh)
+        return v[:, :, :n].clone()
+
+    before = [(held(li, 0, 43), held(li, 3, 5)) for li in range(2)]
+    cache.fork(0, [1, 2], 41)
+    cache.commit()
+    assert cache.owned[1][:2] == cache.owned[0][:2] and cache.owned[1][2] != cache.owned[0][2]
+    for li in range(2):
+        assert torch.equal(held(li, 1, 41), before[li][0][:, :, :41])
+    cache.release(1)
+    assert cache.compact() == 5
+    cache.resize(12)
+    assert cache.pools[0].codes.shape[0] == 12 and cache.pools[0].codes.dtype is Q.CODES[kind] and cache.pools[0].scales.shape[0] == 12
+    cache.resize(5)
+    for li in range(2):
+        assert torch.equal(held(li, 0, 43), before[li][0]) and torch.equal(held(li, 3, 5), before[li][1])
+        assert torch.equal(held(li, 2, 41), before[li][0][:, :, :41])
+    # the forked sequence writes on in its own page: the other's stays
+    x = rows(1, H, Hkv, dh, seed=9, spread=False)
+    Q.kv_append(x * 64, H, Hkv, dh, cache.pools[0], cache.block_table[2:3], torch.tensor([42]).int())
+    assert torch.equal(held(0, 0, 43), before[0][0])
+
+
+def test_engine_refusals(model):
+    for bad in (dict(kv="int4"), dict(kv="int8", kv_block=12), dict(kv="int8", page=12), dict(kv="e4m3", page=8, kv_block=16)):
+        with pytest.raises(ValueError):
+            InferenceEngine(model, **{**dict(max_batch=1, max_seq=16, page=16), **bad})
+
+
+def test_command_takes_the_cache_type(model, tmp_path, capsys):
+    from scirust_b200 import cli
+    from scirust_b200.io import checkpoint as CK
+    CK.save_sciagent_checkpoint(model, tmp_path / "c", step=1, loss=0.0, lr=0.0)
+    assert cli.run(["infer", "--checkpoint", str(tmp_path / "c"), "--prompt", "1 2 3", "--max-new", "4", "--kv", "int8", "--device", "cpu"]) == 0
+    assert len(capsys.readouterr().out.splitlines()) == 1
