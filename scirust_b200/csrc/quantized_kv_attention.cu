@@ -648,8 +648,13 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           other[k] = __ldcg(reinterpret_cast<const float4*>(src + i * 4));
         }
       }
-      // lane x has the weight of warp x
+      // lane x has the weight of warp x; all sums are under way while the weights are worked out
       const float4 ml = x < count ? sm_ml[(from + x) * heads + at] : make_float4(-1.0e30f, 0.f, 0.f, 0.f);
+      const float* src = sm_o + (from * heads + at) * C::PITCH + i % (DH / 4) * 4;
+      float4 e[CONSUMERS];
+#pragma unroll
+      for (int k = 0; k < CONSUMERS; ++k)
+        e[k] = k < count ? *reinterpret_cast<const float4*>(src + k * (heads * C::PITCH)) : make_float4(0.f, 0.f, 0.f, 0.f);
       float top = ml.x;
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -658,13 +663,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k0 = 0; k0 < count; k0 += 4) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float w = __shfl_sync(0xffffffffu, weight, (lane & 16) + k0 + k);
-          const float4 e = *reinterpret_cast<const float4*>(sm_o + ((from + k0 + k) * heads + at) * C::PITCH + i % (DH / 4) * 4);
-          v.x += e.x * w; v.y += e.y * w; v.z += e.z * w; v.w += e.w * w;
-        }
+      for (int k = 0; k < CONSUMERS; ++k) {
+        const float w = __shfl_sync(0xffffffffu, weight, (lane & 16) + k);
+        v.x += e[k].x * w; v.y += e[k].y * w; v.z += e[k].z * w; v.w += e[k].w * w;
       }
       if (ready) {
 #pragma unroll
