@@ -437,16 +437,18 @@ int make_tmap_2d_u16_plain(CUtensorMap* out, const void* base, uint64_t inner, u
   return r == CUDA_SUCCESS ? 0 : SB_ERR_DRIVER;
 }
 
-// 2-D tensor map over bytes whose rows of 64 or 128 are swizzled as wide as they are. Out-of-range parts of a box are filled with zeros.
-int make_tmap_2d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes, uint64_t rows, uint32_t box_rows) {
+// Tensor map over bytes: `groups` of `rows` rows of 64 or 128, contiguous, swizzled as wide as a row is; a box is `box_rows` rows of `box_groups`
+// groups. Out-of-range parts of a box are filled with zeros.
+int make_tmap_3d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes, uint64_t rows, uint64_t groups, uint32_t box_rows,
+                         uint32_t box_groups) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return SB_ERR_DRIVER;
   if (reinterpret_cast<uintptr_t>(base) & 15) return SB_ERR_ALIGN;
-  cuuint64_t dims[2] = {row_bytes, rows};
-  cuuint64_t strides[1] = {row_bytes};
-  cuuint32_t box[2] = {row_bytes, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+  cuuint64_t dims[3] = {row_bytes, rows, groups};
+  cuuint64_t strides[2] = {row_bytes, rows * row_bytes};
+  cuuint32_t box[3] = {row_bytes, box_rows, box_groups};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : SB_ERR_DRIVER;

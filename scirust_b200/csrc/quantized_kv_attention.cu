@@ -35,7 +35,8 @@
 
 namespace sb {
 int num_sms();                                                 // gemm_tcgen05.cu
-int make_tmap_2d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes, uint64_t rows, uint32_t box_rows);
+int make_tmap_3d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes, uint64_t rows, uint64_t groups, uint32_t box_rows,
+                         uint32_t box_groups);
 
 namespace kv8 {
 
@@ -94,10 +95,9 @@ __device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&a)[2], uint32_t (
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr) : "memory");
 }
-template <int OFFSET>
 __device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&a)[2], uint32_t (&b)[2]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
-               : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr), "n"(OFFSET) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(b[0]), "=r"(b[1]) : "r"(addr) : "memory");
 }
 // c += a b, or with FIRST c = a b
 template <bool FIRST>
@@ -252,10 +252,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       // What it costs to cut jobs (writing sums, asking for the count, reading them), at the end, where nothing else is under way, is as long as
       // sixteen tiles: up to there jobs are dealt out whole. us cut / whole, 32 / 8 heads of 128: 1 x 600 positions 10.6 / 7.6, 4 x 800 11.4 / 9.1, 4 x
       // 1600 (21 tiles more) 11.9 / 12.6, 16 x 300 11.5 / 7.0, 16 x 1500 15.5 / 12.6, 16 x 2500 19.3 / 17.6, 9 x 5003 of 4 / 1 heads 13.3 / 29.1.
-      const int ctas = min(grid, jobs), most = (jobs + ctas - 1) / ctas;
+      const int each = jobs <= grid ? 1 : jobs / grid, most = each + (each * grid < jobs);
       if (longest <= 4096 && most * longest - deal.each <= 16) {
-        deal.ctas = ctas;
-        deal.each = jobs / ctas;
+        deal.ctas = min(grid, jobs);
+        deal.each = each;
         deal.whole = 1;
       }
       deal.more = (deal.whole ? jobs : tiles) - deal.each * deal.ctas;
@@ -289,31 +289,27 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     int kvh = p.subs == 1 ? job : job / p.subs, sub = job - kvh * p.subs;
 
     const int box_bits = min(p.page_bits, 6), box = 1 << box_bits, nbx = TK >> box_bits;    // positions of a TMA box, boxes of a tile
-    // of a tile, a lane has one box of codes of keys or values (eight boxes of each at most), or one scale, of eight positions
-    const int v = brings_codes ? lane & 1 : (lane >> 3) & 1;
-    const int first = brings_codes ? (lane >> 1) << box_bits : (lane & 7) * 8;              // its first position in the tile
+    // of a tile, a lane has one box of codes, of keys and of values, or one scale, of eight positions
+    const int first = brings_codes ? lane << box_bits : (lane & 7) * 8;                     // its first position in the tile
     const int x = first >> box_bits;
-    const int unit = brings_codes ? p.page : p.page >> p.block_bits;                        // rows or scales of a page and head
-    const int step = v * p.Hkv * unit + (brings_codes ? 0 : (first & (box - 1)) >> p.block_bits);
-    const int none = brings_codes ? p.n_blocks * 2 * p.Hkv * p.page : -1;                   // for ids outside the pool: a row behind the last one
-    const int slot_bits = brings_codes ? 0 : p.block_bits;
+    const int per_page = p.page >> p.block_bits;                                            // scales of a page and head
+    const int step = ((lane >> 3) & 1) * p.Hkv * per_page + ((first & (box - 1)) >> p.block_bits);
     int stage = 0, q_slot = 0;
     uint32_t phase = 0, q_phase = 0;
     do {
       const int t_end = deal.whole ? nt : min(nt, t_beg + left);
       left -= deal.whole ? 1 : t_end - t_beg;
       const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
-      // of box (fetched + lane) of the sequence: its first row of keys, or their scale
-      int fetched = t_beg * nbx, at_of_lane;
+      // of box (fetched + lane) of the sequence: its page, -1 outside the pool, and its first position there
+      int fetched = t_beg * nbx, id_of_lane, slot_of_lane;
       auto fetch = [&] {
         const long long pos = static_cast<long long>(fetched + lane) << box_bits;
-        at_of_lane = -1;
-        if (pos < len) {
-          const int at = static_cast<int>(pos) / p.page, slot = static_cast<int>(pos) - at * p.page, id = table[at];
-          if (static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks)) at_of_lane = (id * 2 * p.Hkv + kvh) * unit + (slot >> slot_bits);
-        }
+        const int at = pos < len ? static_cast<int>(pos) / p.page : 0;
+        slot_of_lane = static_cast<int>(pos) - at * p.page;
+        id_of_lane = -1;
+        if (pos < len) id_of_lane = table[at];
       };
-      if (!idle) fetch();                                // while the queries are seen to
+      if (!idle) fetch();                                // the ids come while the queries are seen to
       if (brings_codes) {
         mbar_wait_converged(&q_empty[q_slot], q_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
         if (lane == 0) {
@@ -337,16 +333,19 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           fetched = bx0;
           fetch();
         }
-        const int base = __shfl_sync(0xffffffffu, at_of_lane, bx0 + x - fetched);
-        const int at = base < 0 ? none : base + step, rest = len - t * TK;                  // positions of the tile that exist, or more
+        const int id = __shfl_sync(0xffffffffu, id_of_lane, bx0 + x - fetched), slot = __shfl_sync(0xffffffffu, slot_of_lane, bx0 + x - fetched);
+        const bool known = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
+        const int rest = len - t * TK;                                                      // positions of the tile that exist, or more
         const int live = rest >= TK ? nbx : max(0, (rest + box - 1) >> box_bits);           // boxes with one of them
         mbar_wait_converged(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
         if (brings_codes) {
-          // the stage is not full before lane 0 has arrived, whichever comes first, its bytes or that they are expected
-          if (x < live) tma_load_2d(ring + stage * 2 * C::TILE + v * C::TILE + first * DH, &tmap, &full[stage], 0, at);
+          // A box of keys and, behind it, that of values; ids outside the pool: one behind its last page, all zeros. The stage is not full before lane 0
+          // has arrived, whichever comes first, its bytes or that they are expected.
+          if (x < live) tma_load_3d(ring + stage * 2 * C::TILE + first * 2 * DH, &tmap, &full[stage], 0, kvh * p.page + slot, known ? 2 * id : 2 * p.n_blocks);
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
         } else if (lane < 16) {
-          const bool real = first < rest && at >= 0;
+          const bool real = first < rest && known;
+          const int at = (id * 2 * p.Hkv + kvh) * per_page + (slot >> p.block_bits) + step;
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 16 + lane)), "l"(p.scales + (real ? at : 0)),
                        "r"(real ? 4 : 0) : "memory");
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
@@ -372,8 +371,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   // the groups take turns at the tiles, or, with more than one set of heads, each takes all tiles for a set of its own
   const int my_set = sets == 1 ? 0 : group, stride = sets == 1 ? GROUPS : 1;
   const int wrow = pw * 16 + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
-  // its first sixteen bytes of that row, swizzled; those of step c are at this address ^ (c << 4)
-  const uint32_t my_row = smem_u32(ring) + wrow * DH + (((mi >> 1) ^ (DH == 128 ? wrow & 7 : (wrow >> 1) & 3)) << 4);
+  // its first sixteen bytes of that row, swizzled; those of step c are at this address ^ (c << 4), and those of values a box behind
+  const int box = 1 << p.page_bits;
+  const uint32_t my_row = smem_u32(ring) + ((wrow & ~(box - 1)) * 2 + (wrow & (box - 1))) * DH + (((mi >> 1) ^ (DH == 128 ? wrow & 7 : (wrow >> 1) & 3)) << 4);
   const uint32_t my_scales = smem_u32(sc) + pw * 8;
   const int team = consumes ? CONSUMERS * 32 : 64, tid = consumes ? threadIdx.x : threadIdx.x - C::FINISHERS * 32;
   auto team_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(consumes ? 1 : 2), "r"(team) : "memory"); };
@@ -456,7 +456,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
 #pragma unroll
         for (int c = 0; c < CHUNKS; c += 2) ldsm(row ^ (c << 4), rk[c], rk[c + 1]);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) ldsm_t<C::TILE>(row ^ (c << 4), rv[c], rv[c + 1]);
+        for (int c = 0; c < CHUNKS; c += 2) ldsm_t((row + box * DH) ^ (c << 4), rv[c], rv[c + 1]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
         float s[4];
@@ -812,10 +812,10 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
     return SB_ERR_ARG;
   if (page != 8 && page != 16 && page != 32 && page % 64) return SB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || (ldq & 7) || (ldo & 7)) return SB_ERR_ALIGN;
-  const uint64_t rows = static_cast<uint64_t>(n_blocks) * 2 * Hkv * page;
-  if (rows > 0x7fffffffull - kv8::TK) return SB_ERR_TOO_LARGE;
+  if (static_cast<double>(n_blocks) * 2 * Hkv * (page / block) > 2147483647.0 || static_cast<double>(Hkv) * page > 2147483647.0) return SB_ERR_TOO_LARGE;
   CUtensorMap tm;
-  const int rc = make_tmap_2d_u8_rows(&tm, codes, dh, rows, page < kv8::TK ? page : kv8::TK);
+  const int rc = make_tmap_3d_u8_rows(&tm, codes, dh, static_cast<uint64_t>(Hkv) * page, static_cast<uint64_t>(n_blocks) * 2,
+                                      page < kv8::TK ? page : kv8::TK, 2);
   if (rc) return rc;
   kv8::AttendParams p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq;

@@ -374,8 +374,8 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
         raise ValueError("decode_attention: the pool has no pages")
     if page % TILE and page not in (8, 16, 32):
         raise ValueError("decode_attention: pages of 8, 16, 32 or a multiple of 64 positions")
-    if n_blocks * 2 * Hkv * page >= (1 << 31) - TILE:
-        raise ValueError("decode_attention: more rows of codes than 31 bits count")
+    if scales.numel() >= 1 << 31:
+        raise ValueError("decode_attention: more scales than 31 bits count")
     tiles = -(-max_blocks * page // TILE)                       # of a sequence, at most
     jobs = Hkv * -(-(H // Hkv) // JOB_HEADS)
     at_once = min(B, LAUNCH_SEQUENCES, ((1 << 31) - 1) // (tiles * jobs))
