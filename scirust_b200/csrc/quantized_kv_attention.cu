@@ -4,9 +4,9 @@
 // with codes c and the scales s of the position's block and head.
 //
 // Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time. One CTA per SM holds a ring of
-// tiles of 64 positions (keys and values, 8 or 16 KB) that one warp fills by TMA and another with the tile's sixteen scales; the tiles of all
+// 16 KB tiles (keys and values of 64 positions, or 128 of heads of 64) that one warp fills by TMA and another with the tile's sixteen scales; the tiles of all
 // jobs (a sequence and up to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer
-// warps take the tiles in groups of four, warp w of a group 16 positions of the tile:
+// warps take the tiles in groups of four, warp w of a group a quarter of the tile's positions, in sixteens:
 //  - mma.sync takes codes as the A operand, 16 positions (S = K q) or 16 dimensions (O = V w), and eight query heads as columns: a warp's
 //    16 positions times 16 query rows would be half empty with eight query heads a kv head or fewer. With more, each group takes all tiles for
 //    eight of them. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of two halves of the A operand,
@@ -40,7 +40,6 @@ int make_tmap_3d_u8_rows(CUtensorMap* out, const void* base, uint32_t row_bytes,
 
 namespace kv8 {
 
-constexpr int TK = 64;                       // positions of a tile
 constexpr int MAX_B = 1024;                  // sequences of a launch, whose offsets lie in shared memory
 constexpr int STAGES_MAX = 24;
 constexpr int SET = 8, HEADS_MAX = 3 * SET;  // query heads of a set, which is what a warp takes, and of a job
@@ -75,12 +74,15 @@ struct Cfg {
   static constexpr int GROUPS = 3, CONSUMERS = 4 * GROUPS;     // of four warps, and warps
   static constexpr int CODES = CONSUMERS, SCALES = CONSUMERS + 1, FINISHERS = CONSUMERS + 2;      // two producers, two finishers
   static constexpr int THREADS = CONSUMERS * 32 + 128;
+  static constexpr int TK = 8192 / DH;                         // positions of a tile: 64, or 128 at half the head dimension
   static constexpr int TILE = TK * DH;                         // bytes of a tile's keys, and of its values
+  static constexpr int PARTS = TK / 64;                        // a warp's positions of a tile, in sixteens
+  static constexpr int SCALES_OF_V = TK / 8;                   // where values' scales begin: one for eight positions of keys, then of values
   static constexpr int PITCH = DH + 4;                         // of a head's sums between warps
   static constexpr int QSLOTS = 4;                             // pieces whose queries lie in shared memory
   static constexpr int fixed_bytes(int sets, int heads, int B) {
     return CONSUMERS * heads * (PITCH + 4) * 4 + QSLOTS * (sets * heads * DH * 2 + static_cast<int>(sizeof(Piece))) + (2 * B + 1) * 4 +
-           STAGES_MAX * (64 + 16) + (2 * QSLOTS + 2) * 8 + 1024;
+           STAGES_MAX * (2 * SCALES_OF_V * 4 + 16) + (2 * QSLOTS + 2) * 8 + 1024;
   }
   // A stage is always taken by the same groups: a parity wait tells a fill from the one after next only by whoever has seen the one between.
   static constexpr int stages(int sets, int heads, int B) {
@@ -153,6 +155,7 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& x, uint32_t& y) {
 }
 
 // Tiles of one sequence: an empty one keeps a tile without positions, whose job writes zeros.
+template <int TK>
 __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + TK - 1) / TK : 1; }
 
 // How the units (tiles of all jobs, end to end; or whole jobs) are dealt out: the first `more` CTAs have one more than the others.
@@ -182,12 +185,12 @@ template <int DH, bool E4M3>
 __global__ void __launch_bounds__(Cfg<DH>::THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
   using C = Cfg<DH>;
-  constexpr int CHUNKS = DH / 16, GROUPS = C::GROUPS, CONSUMERS = C::CONSUMERS;
+  constexpr int CHUNKS = DH / 16, GROUPS = C::GROUPS, CONSUMERS = C::CONSUMERS, TK = C::TK, PARTS = C::PARTS, SCALES_OF_V = C::SCALES_OF_V;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stages = p.stages, sets = p.sets, heads = p.heads, jobs_b = p.Hkv * p.subs;
-  float* sc = reinterpret_cast<float*>(ring + stages * 2 * C::TILE);                // [stages][k: 8 | v: 8], of 8 positions each
-  __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 16);     // [slots][sets * heads][DH]
+  float* sc = reinterpret_cast<float*>(ring + stages * 2 * C::TILE);                // [stages][keys | values], of 8 positions each
+  __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 2 * SCALES_OF_V);     // [slots][sets * heads][DH]
   Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * sets * heads * DH);          // [slots]
   float* sm_o = reinterpret_cast<float*>(pieces + C::QSLOTS);                       // [warps][heads][PITCH]
   float4* sm_ml = reinterpret_cast<float4*>(sm_o + CONSUMERS * heads * C::PITCH);   // [warps][heads]: reference, sum, largest scale of values
@@ -205,7 +208,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0) {
-    if (lane < stages) { mbar_init(&full[lane], 17); mbar_init(&empty[lane], 4 * sets); }
+    if (lane < stages) { mbar_init(&full[lane], 1 + 2 * SCALES_OF_V); mbar_init(&empty[lane], 4 * sets); }
     if (lane < C::QSLOTS) { mbar_init(&q_full[lane], 1); mbar_init(&q_empty[lane], CONSUMERS + 2); }
     if (lane == 0) { mbar_init(o_full, CONSUMERS); mbar_init(o_empty, 1); s_end = s_ready = 0; }
     fence_barrier_init();
@@ -233,7 +236,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int len = min(next, cap);
         next = b0 + 32 + lane < p.B ? p.seq_len[b0 + 32 + lane] : 0;
-        const int n = b0 + lane < p.B ? tiles_of(len) : 0;
+        const int n = b0 + lane < p.B ? tiles_of<TK>(len) : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -280,20 +283,20 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           n = min(step - 1, n - c * step);
         }
         t_beg = u0 - prefix[b] * jobs_b;
-        job = t_beg / tiles_of(lens[b]);
-        t_beg -= job * tiles_of(lens[b]);
+        job = t_beg / tiles_of<TK>(lens[b]);
+        t_beg -= job * tiles_of<TK>(lens[b]);
       }
     }
-    int len = lens[b], nt = tiles_of(len), start = prefix[b] * jobs_b;
+    int len = lens[b], nt = tiles_of<TK>(len), start = prefix[b] * jobs_b;
     start += job * nt;
     int kvh = p.subs == 1 ? job : job / p.subs, sub = job - kvh * p.subs;
 
     const int box_bits = min(p.page_bits, 6), box = 1 << box_bits, nbx = TK >> box_bits;    // positions of a TMA box, boxes of a tile
     // of a tile, a lane has one box of codes, of keys and of values, or one scale, of eight positions
-    const int first = brings_codes ? lane << box_bits : (lane & 7) * 8;                     // its first position in the tile
+    const int first = brings_codes ? lane << box_bits : lane % SCALES_OF_V * 8;                     // its first position in the tile
     const int x = first >> box_bits;
     const int per_page = p.page >> p.block_bits;                                            // scales of a page and head
-    const int step = ((lane >> 3) & 1) * p.Hkv * per_page + ((first & (box - 1)) >> p.block_bits);
+    const int step = lane / SCALES_OF_V * p.Hkv * per_page + ((first & (box - 1)) >> p.block_bits);
     int stage = 0, q_slot = 0;
     uint32_t phase = 0, q_phase = 0;
     do {
@@ -343,10 +346,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           // has arrived, whichever comes first, its bytes or that they are expected.
           if (x < live) tma_load_3d(ring + stage * 2 * C::TILE + first * 2 * DH, &tmap, &full[stage], 0, kvh * p.page + slot, known ? 2 * id : 2 * p.n_blocks);
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
-        } else if (lane < 16) {
+        } else if (lane < 2 * SCALES_OF_V) {
           const bool real = first < rest && known;
           const int at = (id * 2 * p.Hkv + kvh) * per_page + (slot >> p.block_bits) + step;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 16 + lane)), "l"(p.scales + (real ? at : 0)),
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 2 * SCALES_OF_V + lane)), "l"(p.scales + (real ? at : 0)),
                        "r"(real ? 4 : 0) : "memory");
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
         }
@@ -357,7 +360,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       if (++sub == p.subs) { sub = 0; ++kvh; }
       if (++job == jobs_b) {
         job = kvh = 0;
-        if (++b < p.B) { len = lens[b]; nt = tiles_of(len); }
+        if (++b < p.B) { len = lens[b]; nt = tiles_of<TK>(len); }
       }
     } while (left > 0);
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -370,11 +373,12 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   const int group = warp >> 2, pw = warp & 3;
   // the groups take turns at the tiles, or, with more than one set of heads, each takes all tiles for a set of its own
   const int my_set = sets == 1 ? 0 : group, stride = sets == 1 ? GROUPS : 1;
-  const int wrow = pw * 16 + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
+  const int wrow = pw * (16 * PARTS) + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
   // its first sixteen bytes of that row, swizzled; those of step c are at this address ^ (c << 4), and those of values a box behind
   const int box = 1 << p.page_bits;
   const uint32_t my_row = smem_u32(ring) + ((wrow & ~(box - 1)) * 2 + (wrow & (box - 1))) * DH + (((mi >> 1) ^ (DH == 128 ? wrow & 7 : (wrow >> 1) & 3)) << 4);
-  const uint32_t my_scales = smem_u32(sc) + pw * 8;
+  const uint32_t my_scales = smem_u32(sc) + pw * (8 * PARTS);
+  const int next_part = (box <= 16 ? 32 : 16) * DH;                                    // sixteen positions further on
   const int team = consumes ? CONSUMERS * 32 : 64, tid = consumes ? threadIdx.x : threadIdx.x - C::FINISHERS * 32;
   auto team_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(consumes ? 1 : 2), "r"(team) : "memory"); };
   int turn = group - my_set;                 // tiles of the next piece before the first that this group takes
@@ -447,110 +451,122 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         if (stage >= stages) { stage -= stages; phase ^= 1; }
         mbar_wait_converged(&full[st], ph, p.status, ST_TIMEOUT_FULL);
         const uint32_t row = my_row + st * (2 * C::TILE);
-        float2 ks, vs;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks.x), "=f"(ks.y) : "r"(my_scales + st * 64) : "memory");
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2+32];" : "=f"(vs.x), "=f"(vs.y) : "r"(my_scales + st * 64) : "memory");
-        const int valid = len - t * TK - pw * 16;                                      // positions of this warp's 16 that exist
-        // the bytes of the warp's 16 positions go to registers, and the stage back to the producers
-        uint32_t rk[CHUNKS][2], rv[CHUNKS][2];
+        float2 ks_of[PARTS], vs_of[PARTS];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) ldsm(row ^ (c << 4), rk[c], rk[c + 1]);
+        for (int i = 0; i < PARTS; ++i) {
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks_of[i].x), "=f"(ks_of[i].y) : "r"(my_scales + st * (8 * SCALES_OF_V) + i * 8) : "memory");
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                       : "=f"(vs_of[i].x), "=f"(vs_of[i].y) : "r"(my_scales + st * (8 * SCALES_OF_V) + i * 8 + 4 * SCALES_OF_V) : "memory");
+        }
+        // the bytes of the warp's positions go to registers, and the stage back to the producers
+        uint32_t k_of[PARTS][CHUNKS][2], v_of[PARTS][CHUNKS][2];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) ldsm_t((row + box * DH) ^ (c << 4), rv[c], rv[c + 1]);
+        for (int i = 0; i < PARTS; ++i) {
+#pragma unroll
+          for (int c = 0; c < CHUNKS; c += 2) ldsm((row + i * next_part) ^ (c << 4), k_of[i][c], k_of[i][c + 1]);
+#pragma unroll
+          for (int c = 0; c < CHUNKS; c += 2) ldsm_t((row + i * next_part + box * DH) ^ (c << 4), v_of[i][c], v_of[i][c + 1]);
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
-        float s[4];
-        if constexpr (E4M3) {
-          float s1[4];                                                                 // two sums of products, so that they need not wait so long
 #pragma unroll
-          for (int c = 0; c < CHUNKS; c += 2) {
-            uint32_t a[4];
-            widen<E4M3, false>(rk[c][0], a[0], a[2]);
-            widen<E4M3, false>(rk[c][1], a[1], a[3]);
-            if (c == 0) mma_f16<true>(s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
-            else mma_f16<false>(s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
-            widen<E4M3, false>(rk[c + 1][0], a[0], a[2]);
-            widen<E4M3, false>(rk[c + 1][1], a[1], a[3]);
-            if (c == 0) mma_f16<true>(s1, a[0], a[1], a[2], a[3], qb[c + 1][0], qb[c + 1][1]);
-            else mma_f16<false>(s1, a[0], a[1], a[2], a[3], qb[c + 1][0], qb[c + 1][1]);
-          }
+        for (int part = 0; part < PARTS; ++part) {
+          const float2 ks = ks_of[part], vs = vs_of[part];
+          uint32_t (&rk)[CHUNKS][2] = k_of[part], (&rv)[CHUNKS][2] = v_of[part];
+          const int valid = len - t * TK - (pw * PARTS + part) * 16;                     // positions of these 16 that exist
+          float s[4];
+          if constexpr (E4M3) {
+            float s1[4];                                                                 // two sums of products, so that they need not wait so long
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] += s1[e];
-        } else {
-          int hi[4], lo[4];
-#pragma unroll
-          for (int c = 0; c < CHUNKS; c += 2) {
-            if (c == 0) {
-              mma_s8<true>(hi, rk[c], rk[c + 1], qb[c][0], qb[c + 1][0]);
-              mma_s8<true>(lo, rk[c], rk[c + 1], qb[c][1], qb[c + 1][1]);
-            } else {
-              mma_s8<false>(hi, rk[c], rk[c + 1], qb[c][0], qb[c + 1][0]);
-              mma_s8<false>(lo, rk[c], rk[c + 1], qb[c][1], qb[c + 1][1]);
+            for (int c = 0; c < CHUNKS; c += 2) {
+              uint32_t a[4];
+              widen<E4M3, false>(rk[c][0], a[0], a[2]);
+              widen<E4M3, false>(rk[c][1], a[1], a[3]);
+              if (c == 0) mma_f16<true>(s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
+              else mma_f16<false>(s, a[0], a[1], a[2], a[3], qb[c][0], qb[c][1]);
+              widen<E4M3, false>(rk[c + 1][0], a[0], a[2]);
+              widen<E4M3, false>(rk[c + 1][1], a[1], a[3]);
+              if (c == 0) mma_f16<true>(s1, a[0], a[1], a[2], a[3], qb[c + 1][0], qb[c + 1][1]);
+              else mma_f16<false>(s1, a[0], a[1], a[2], a[3], qb[c + 1][0], qb[c + 1][1]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += s1[e];
+          } else {
+            int hi[4], lo[4];
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c += 2) {
+              if (c == 0) {
+                mma_s8<true>(hi, rk[c], rk[c + 1], qb[c][0], qb[c + 1][0]);
+                mma_s8<true>(lo, rk[c], rk[c + 1], qb[c][1], qb[c + 1][1]);
+              } else {
+                mma_s8<false>(hi, rk[c], rk[c + 1], qb[c][0], qb[c + 1][0]);
+                mma_s8<false>(lo, rk[c], rk[c + 1], qb[c][1], qb[c + 1][1]);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = __int2float_rn(hi[e] * 256 + lo[e]);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = __int2float_rn(hi[e] * 256 + lo[e]);
-        }
-        float x[4], top = -INFINITY;                                                   // scores less the reference
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[e] *= ks.x * qf[e];
-          s[2 + e] *= ks.y * qf[e];
-        }
-        if (valid < 16) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (quad + (e >> 1) * 8 >= valid) s[e] = -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = s[e] - m[e & 1];
-          top = fmaxf(top, x[e]);
-        }
-        if (__any_sync(0xffffffffu, top > 15.f || fmaxf(vs.x, vs.y) > vref)) {
-          const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
-          vref = v_new;
-          vinv = 1.f / v_new;
+          float x[4], top = -INFINITY;                                                   // scores less the reference
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float most = fmaxf(s[e], s[2 + e]) - 9.f;
+            s[e] *= ks.x * qf[e];
+            s[2 + e] *= ks.y * qf[e];
+          }
+          if (valid < 16) {
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            const float m_new = fmaxf(m[e], most), a = ex2(m[e] - m_new);
-            m[e] = m_new;
-            l[e] *= a;
-            x[e] = s[e] - m_new;
-            x[2 + e] = s[2 + e] - m_new;
+            for (int e = 0; e < 4; ++e)
+              if (quad + (e >> 1) * 8 >= valid) s[e] = -INFINITY;
+          }
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-              o[c][e] *= a * v_ratio;
-              o[c][2 + e] *= a * v_ratio;
+          for (int e = 0; e < 4; ++e) {
+            x[e] = s[e] - m[e & 1];
+            top = fmaxf(top, x[e]);
+          }
+          if (__any_sync(0xffffffffu, top > 15.f || fmaxf(vs.x, vs.y) > vref)) {
+            const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
+            vref = v_new;
+            vinv = 1.f / v_new;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float most = fmaxf(s[e], s[2 + e]) - 9.f;
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+              const float m_new = fmaxf(m[e], most), a = ex2(m[e] - m_new);
+              m[e] = m_new;
+              l[e] *= a;
+              x[e] = s[e] - m_new;
+              x[2 + e] = s[2 + e] - m_new;
+#pragma unroll
+              for (int c = 0; c < CHUNKS; ++c) {
+                o[c][e] *= a * v_ratio;
+                o[c][2 + e] *= a * v_ratio;
+              }
             }
           }
-        }
-        uint32_t w[2];
-        {
-          const float v0 = vs.x * vinv, v1 = vs.y * vinv;
+          uint32_t w[2];
+          {
+            const float v0 = vs.x * vinv, v1 = vs.y * vinv;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
-          l[0] += x[0] + x[2];
-          l[1] += x[1] + x[3];
-          w[0] = transpose8x8(half2_bits(x[0] * v0, x[1] * v0));
-          w[1] = transpose8x8(half2_bits(x[2] * v1, x[3] * v1));
-        }
-        // what lies behind the last position may be NaN, which a weight of zero does not make zero
-        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-        if (E4M3 && valid < 16) {
-          keep0 = (2 * tq < valid ? 0xffffu : 0u) | (2 * tq + 1 < valid ? 0xffff0000u : 0u);
-          keep1 = (2 * tq + 8 < valid ? 0xffffu : 0u) | (2 * tq + 9 < valid ? 0xffff0000u : 0u);
-        }
+            for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
+            l[0] += x[0] + x[2];
+            l[1] += x[1] + x[3];
+            w[0] = transpose8x8(half2_bits(x[0] * v0, x[1] * v0));
+            w[1] = transpose8x8(half2_bits(x[2] * v1, x[3] * v1));
+          }
+          // what lies behind the last position may be NaN, which a weight of zero does not make zero
+          uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+          if (E4M3 && valid < 16) {
+            keep0 = (2 * tq < valid ? 0xffffu : 0u) | (2 * tq + 1 < valid ? 0xffff0000u : 0u);
+            keep1 = (2 * tq + 8 < valid ? 0xffffu : 0u) | (2 * tq + 9 < valid ? 0xffff0000u : 0u);
+          }
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          uint32_t a[4];
-          if (E4M3) { rv[c][0] &= keep0; rv[c][1] &= keep1; }
-          widen<E4M3, true>(rv[c][0], a[0], a[1]);
-          widen<E4M3, true>(rv[c][1], a[2], a[3]);
-          mma_f16<false>(o[c], a[0], a[1], a[2], a[3], w[0], w[1]);
+          for (int c = 0; c < CHUNKS; ++c) {
+            uint32_t a[4];
+            if (E4M3) { rv[c][0] &= keep0; rv[c][1] &= keep1; }
+            widen<E4M3, true>(rv[c][0], a[0], a[1]);
+            widen<E4M3, true>(rv[c][1], a[2], a[3]);
+            mma_f16<false>(o[c], a[0], a[1], a[2], a[3], w[0], w[1]);
+          }
         }
       }
       turn = t - t_end;
@@ -815,7 +831,7 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   if (static_cast<double>(n_blocks) * 2 * Hkv * (page / block) > 2147483647.0 || static_cast<double>(Hkv) * page > 2147483647.0) return SB_ERR_TOO_LARGE;
   CUtensorMap tm;
   const int rc = make_tmap_3d_u8_rows(&tm, codes, dh, static_cast<uint64_t>(Hkv) * page, static_cast<uint64_t>(n_blocks) * 2,
-                                      page < kv8::TK ? page : kv8::TK, 2);
+                                      page < 64 ? page : 64, 2);
   if (rc) return rc;
   kv8::AttendParams p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq;
@@ -829,7 +845,7 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   const int per_job = (p.G + p.subs - 1) / p.subs;
   p.sets = (per_job + kv8::SET - 1) / kv8::SET;
   p.heads = (per_job + p.sets - 1) / p.sets;
-  if (static_cast<double>(B) * ((static_cast<double>(max_blocks) * page + kv8::TK - 1) / kv8::TK) * Hkv * p.subs > 2147483647.0) return SB_ERR_TOO_LARGE;
+  if (static_cast<double>(B) * ((static_cast<double>(max_blocks) * page + 63) / 64) * Hkv * p.subs > 2147483647.0) return SB_ERR_TOO_LARGE;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = part; p.counters = counters;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
