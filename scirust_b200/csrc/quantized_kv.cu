@@ -9,6 +9,7 @@
 // time, so that a code is off by less than one of its last steps, however often. A block that is given an infinity or a NaN gets NaN as its
 // scale and keeps it until its first position is written again: what the format cannot hold is not lost silently.
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "api.h"
 #include "dependent.cuh"
 #include "quantized_kv.cuh"
@@ -20,20 +21,22 @@ int num_sms();                                                                 /
 namespace kv8 {
 
 // ---- writing -------------------------------------------------------------------------------------------------------------------
-// A warp takes one key or value head of a chunk of rows (or several, where there are more than enough warps) and walks over the blocks of
-// positions that begin in it; a block's rows that reach into the next chunk are its own. Which sequence and position a row has follows from cu_q and seq_len, so that no two warps can write one
-// block. Sixteen rows at a time stay in registers between the maximum and the codes; of larger blocks the rows are read twice, the second
-// time from L2. Query heads are only turned: a warp has one row, or as many as fill it, with their part of the rotation's table in registers
-// for a quarter of the heads.
-// Bound by memory for prompts and by latency for single tokens.
-constexpr int WARPS = 4;
+// A warp, or two that exchange their maxima, takes one key or value head of a chunk of rows and walks over the blocks of positions that begin
+// in it; a block's rows that reach into the next chunk are its own. Which sequence and position a row has follows from cu_q and seq_len and is
+// looked for once a sequence and chunk (once a block: 17.2 for 15.4 us, for 16 sequences of 700 rows). No two warps can write one block. Eight
+// rows a warp stay in registers between the maximum and the codes; of larger blocks the rows are read twice, the second time from L2. (The
+// next block's or head's rows under way meanwhile take registers that more warps use better: 17.8 us.) Query heads are only turned: a warp has
+// one row, or as many as fill it, with their part of the rotation's table in registers for its share of the heads.
+// Bound by latency for single tokens: 2.3 us for one, 3.2 for 64 sequences of an 8B model; for prompts by memory, at 0.77 (2048 rows) to 0.94 (16
+// sequences of 700) of the copy rate.
+constexpr int HEADS = 4;                       // key or value heads of a CTA, with `SPLIT` warps each
 
 struct AppendParams {
   __nv_bfloat16* qkv; long long ld;
   int n, H, Hkv;
   const float *cos_t, *sin_t; int n_pos;       // null: the rows hold what is to be written
   uint8_t* codes; float* scales;
-  int n_blocks, page, block;
+  int n_blocks, page, block, block_bits, per_page;      // per_page: blocks of a page
   const int* table; int max_blocks;
   const int *seq_len, *cu_q;                   // cu_q null: row b is sequence b's only one
   int B, chunk;
@@ -43,6 +46,7 @@ struct AppendParams {
 // The sequence that row t belongs to: how many of cu[1 .. B] are at most t, by steps of a 32nd of what is left.
 __device__ __forceinline__ int find_sequence(const int* cu, int B, int t) {
   const int lane = threadIdx.x & 31;
+  if (B == 1) return cu[1] <= t;
   int lo = 0, n = B;
   while (n > 0) {
     const int step = (n + 31) / 32, at = lo + (lane + 1) * step;
@@ -60,14 +64,24 @@ __device__ __forceinline__ uint32_t rotate(uint32_t x, float c, float s) {
   return pack_bf16x2(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c)));
 }
 
-template <bool E4M3>
-__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d) {
+// The larger magnitudes of two pairs in bf16, NaN above all, under some sign.
+__device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+// x * f as codes. int8: 1.5 * 2^23 + x is rounded to a whole number, whose last byte is x's (a conversion takes four times as long); CLAMP: it
+// may be 128.
+template <bool E4M3, bool CLAMP>
+__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d, float f) {
   if constexpr (E4M3) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
-           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16;
+    return __nv_cvt_float2_to_fp8x2(make_float2(a * f, b * f), __NV_SATFINITE, __NV_E4M3) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c * f, d * f), __NV_SATFINITE, __NV_E4M3)) << 16;
   } else {
-    // 1.5 * 2^23 + x is rounded to a whole number, whose last byte is x's (a conversion takes four times as long)
-    auto code = [](float x) { return __float_as_uint(fminf(fmaxf(x, -127.f), 127.f) + 12582912.f); };
+    auto code = [f](float x) {
+      return __float_as_uint(CLAMP ? fminf(fmaxf(x * f, -127.f), 127.f) + 12582912.f : fmaf(x, f, 12582912.f));
+    };
     return __byte_perm(__byte_perm(code(a), code(b), 0x0040), __byte_perm(code(c), code(d), 0x0040), 0x5410);
   }
 }
@@ -83,26 +97,33 @@ __device__ __forceinline__ float scale_for(uint32_t bits) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-struct Place { int rows, pos; };               // rows of a sequence from some row on, the first one's position; rows 0: that has no place
+struct Place { int start, stop, rows, pos; };  // a sequence's rows; from some row on, those that have a place and the first one's position
 
-// Where row t of sequence b is, which its first row is not behind and which has more.
-__device__ __forceinline__ Place place_of(const AppendParams& p, int b, int t, int stop, int& skip) {
-  const int rows = min(stop, p.n) - t;
-  const long long at = static_cast<long long>(p.seq_len[b]) - (stop - t);
+// Where row t of sequence b is. Where it has no place, `rows` is 0 and `skip` how many rows have none.
+__device__ __forceinline__ Place place_of(const AppendParams& p, int b, int t, int& skip) {
+  Place at = {t, t + 1, 0, 0};
+  const int len = p.seq_len[b];                // three loads that do not wait for one another
+  if (p.cu_q) { at.start = p.cu_q[b]; at.stop = p.cu_q[b + 1]; }
+  if (t < at.start) { skip = at.start - t; return at; }
+  const int rows = min(at.stop, p.n) - t;
+  if (rows <= 0) { skip = 1; return at; }      // offsets that do not ascend
+  const long long pos = static_cast<long long>(len) - (at.stop - t);
   long long limit = min(static_cast<long long>(p.max_blocks) * p.page, 0x7fffffffll);
   if (p.cos_t) limit = min(limit, static_cast<long long>(p.n_pos));
-  if (at < 0 || at >= limit) {
-    skip = at < 0 ? static_cast<int>(min(-at, static_cast<long long>(rows))) : rows;
-    return {0, 0};
+  if (pos < 0 || pos >= limit) {
+    skip = pos < 0 ? static_cast<int>(min(-pos, static_cast<long long>(rows))) : rows;
+    return at;
   }
-  return {min(rows, static_cast<int>(limit - at)), static_cast<int>(at)};
+  at.rows = min(rows, static_cast<int>(limit - pos));
+  at.pos = static_cast<int>(pos);
+  return at;
 }
 
 __device__ __forceinline__ uint4 rotate8(uint4 v, const float4& c, const float4& s) {
   return make_uint4(rotate(v.x, c.x, s.x), rotate(v.y, c.y, s.y), rotate(v.z, c.z, s.z), rotate(v.w, c.w, s.w));
 }
 
-template <int DH>
+template <int DH, int WARPS>
 __device__ __forceinline__ void turn_queries(const AppendParams& p, int cta) {
   constexpr int LANES = DH / 8, ROWS = 32 / LANES, AHEAD = 8;                  // lanes of a row, rows of a warp, heads under way
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, ch = lane % LANES;
@@ -117,16 +138,11 @@ __device__ __forceinline__ void turn_queries(const AppendParams& p, int cta) {
   load(warp);                                  // while the row's place is looked for
   int b = p.cu_q ? find_sequence(p.cu_q, p.B, t0) : t;
   if (t >= p.n) return;
-  int stop = t + 1;
-  if (p.cu_q) {
+  if (p.cu_q && t > t0)
     while (b < p.B && p.cu_q[b + 1] <= t) ++b;
-    if (b >= p.B || t < p.cu_q[b]) return;
-    stop = p.cu_q[b + 1];
-  } else if (b >= p.B) {
-    return;
-  }
+  if (b >= p.B) return;
   int skip;
-  const Place at = place_of(p, b, t, stop, skip);
+  const Place at = place_of(p, b, t, skip);
   if (at.rows == 0) return;
   const size_t a = static_cast<size_t>(at.pos) * (DH / 2) + ch * 4;
   const float4 c = *reinterpret_cast<const float4*>(p.cos_t + a), s = *reinterpret_cast<const float4*>(p.sin_t + a);
@@ -140,151 +156,185 @@ __device__ __forceinline__ void turn_queries(const AppendParams& p, int cta) {
   }
 }
 
-// BATCH: rows at a time, 8 for blocks of 8 and else 16
-template <int DH, bool E4M3, int BATCH>
-__global__ void __launch_bounds__(WARPS * 32, 6) append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int LANES = DH / 8, ROWS = 32 / LANES, WORDS = BATCH / ROWS;       // lanes of a row, rows of a load, loads of a batch
+template <int DH, bool E4M3, int SPLIT>
+__global__ void __launch_bounds__(HEADS * SPLIT * 32, SPLIT == 1 ? 8 : 4) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int LANES = DH / 8, ROWS = 32 / LANES, WORDS = 8 / ROWS;           // lanes of a row, rows of a load, loads of eight rows
+  constexpr int BATCH = 8 * SPLIT;
   pdl_trigger();
   pdl_wait();
   if (static_cast<int>(blockIdx.x) >= p.kv_ctas) {
-    turn_queries<DH>(p, blockIdx.x - p.kv_ctas);
+    turn_queries<DH, HEADS * SPLIT>(p, blockIdx.x - p.kv_ctas);
     return;
   }
-  const int lane = threadIdx.x & 31, sub = lane / LANES, ch = lane % LANES;
-  const int chunk = blockIdx.x / p.head_ctas, first_head = (blockIdx.x - chunk * p.head_ctas) * WARPS + (threadIdx.x >> 5);
-  if (first_head >= 2 * p.Hkv) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ch = lane % LANES;
+  const int sub = lane / LANES + (SPLIT == 1 ? 0 : warp % SPLIT * 8);          // the lane's first row of a batch
+  const int chunk = blockIdx.x / p.head_ctas, head = (blockIdx.x - chunk * p.head_ctas) * HEADS + warp / SPLIT;
+  __shared__ uint32_t s_top[HEADS * SPLIT];
+  if (head >= 2 * p.Hkv) return;
+  const int kv = head >= p.Hkv, h = head - kv * p.Hkv;
+  const bool turns = p.cos_t && !kv;
+  __nv_bfloat16* const rows = p.qkv + sub * p.ld + (p.H + head) * DH + ch * 8;
   int t = chunk * p.chunk;
   const int end = min(p.n - t, p.chunk) + t;
   int b = p.cu_q ? find_sequence(p.cu_q, p.B, t) : t;
-  while (t < end) {
-    int start = t, stop = t + 1;                                               // rows of the sequence
-    if (p.cu_q) {
-      while (b < p.B && p.cu_q[b + 1] <= t) ++b;
-      if (b >= p.B) return;
-      start = p.cu_q[b];
-      stop = p.cu_q[b + 1];
-      if (t < start) { t = start; continue; }
-    } else {
-      b = t;
-      if (b >= p.B) return;
-    }
+  while (t < end) {                                                            // b: the sequence of row t, or the next one
+    if (!p.cu_q) b = t;
+    if (b >= p.B) return;
     int skip;
-    const Place place = place_of(p, b, t, stop, skip);
-    if (place.rows == 0) { t += skip; continue; }
-    const int pos = place.pos, off = pos & (p.block - 1), cnt = min(p.block - off, place.rows), t0 = t;
-    t += cnt;
-    if (off && t0 != start) continue;                                          // a block that began in an earlier chunk
-
-    const int at = pos / p.page, slot = pos - at * p.page, id = p.table[static_cast<size_t>(b) * p.max_blocks + at];
-    const bool known = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
-    for (int head = first_head; head < 2 * p.Hkv; head += p.head_ctas * WARPS) {
-      const int kv = head >= p.Hkv, h = head - kv * p.Hkv;
-      const bool turns = p.cos_t && !kv;
-      __nv_bfloat16* x = p.qkv + (t0 + sub) * p.ld + (p.H + head) * DH + ch * 8;
-      uint4 v[WORDS];
-      auto load = [&](int r0) {
+    const Place place = place_of(p, b, t, skip);
+    const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
+    int pos = place.pos;
+    const int stop = t + place.rows;                                           // of the sequence's rows that have a place
+    if (place.rows == 0) {
+      t += skip;
+    } else if ((pos & (p.block - 1)) && t != place.start) {                    // a block that began in an earlier chunk
+      const int rest = min(p.block - (pos & (p.block - 1)), place.rows);
+      t += rest;
+      pos += rest;
+    }
+    auto load = [&](uint4 (&to)[WORDS], int t0, int cnt) {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (r0 + i * ROWS + sub < cnt) v[i] = *reinterpret_cast<const uint4*>(x + (r0 + i * ROWS) * p.ld);
-        }
-      };
-      load(0);
-      // while the rows are under way: the scale of what the block holds
+      for (int i = 0; i < WORDS; ++i) {
+        to[i] = make_uint4(0, 0, 0, 0);
+        if (i * ROWS + sub < cnt) to[i] = *reinterpret_cast<const uint4*>(rows + (t0 + i * ROWS) * p.ld);
+      }
+    };
+    for (int cnt; t < end && t < stop; t += cnt, pos += cnt) {
+      const int off = pos & (p.block - 1), t0 = t;
+      cnt = min(p.block - off, stop - t);
+      uint4 v[WORDS];
+      load(v, t, cnt);
+      const int id = table[pos / p.page];
+      const bool known = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
+      const int slot = pos % p.page;
+      __nv_bfloat16* x = rows + t0 * p.ld;
       const size_t row = (static_cast<size_t>(known ? id : 0) * 2 + kv) * p.Hkv + h;
-      float* scale_at = p.scales + row * (p.page / p.block) + slot / p.block;
+      float* scale_at = p.scales + row * p.per_page + (slot >> p.block_bits);
       const float old = off && known ? *scale_at : 0.f;
       uint32_t top = 0;
       for (int r0 = 0; r0 < cnt; r0 += BATCH) {
-        if (r0) load(r0);
+        if (r0) load(v, t0 + r0, cnt - r0);
         if (turns) {
           const size_t a = static_cast<size_t>(pos + r0 + sub) * (DH / 2) + ch * 4;
 #pragma unroll
           for (int i = 0; i < WORDS; ++i) {
             const bool in = r0 + i * ROWS + sub < cnt;
             float4 c = make_float4(0, 0, 0, 0), s = c;
-            if (in) c = *reinterpret_cast<const float4*>(p.cos_t + a + i * ROWS * (DH / 2)), s = *reinterpret_cast<const float4*>(p.sin_t + a + i * ROWS * (DH / 2));
+            const size_t at = a + i * ROWS * (DH / 2);
+            if (in) {
+              c = *reinterpret_cast<const float4*>(p.cos_t + at);
+              s = *reinterpret_cast<const float4*>(p.sin_t + at);
+            }
             v[i] = rotate8(v[i], c, s);
             if (in) *reinterpret_cast<uint4*>(x + (r0 + i * ROWS) * p.ld) = v[i];
           }
         }
 #pragma unroll
         for (int i = 0; i < WORDS; ++i)
-          top = max16x2(top, max16x2(max16x2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), max16x2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
+          top = largest(top, largest(largest(v[i].x, v[i].y), largest(v[i].z, v[i].w)));
       }
       if (!known) continue;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = max(top & 0xffffu, top >> 16);
+      for (int o = 1; o < 32; o <<= 1) top = largest(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = max(top & 0x7fffu, top >> 16 & 0x7fffu);
+      if (SPLIT > 1) {                                                         // both warps of the head come here equally often
+        if (lane == 0) s_top[warp] = top;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / 2) : "memory");
+        top = max(top, s_top[warp ^ 1]);
+      }
       const float need = scale_for<E4M3>(top);
       const float scale = off && (old > need || old != old) ? old : need;
-      if (lane == 0) *scale_at = scale;                                          // all lanes have read it: they have met since
+      if (lane == 0 && sub == 0) *scale_at = scale;                            // all lanes have read it: they have met since
       const bool holds = scale == scale;
       const float inv = 1.f / scale;
       uint8_t* dst = p.codes + (row * p.page + slot) * DH;
-      for (int r0 = 0; r0 < cnt; r0 += BATCH) {
-        if (cnt > BATCH) load(r0);
+      auto write = [&](auto clamp) {
+        constexpr bool CLAMP = decltype(clamp)::value;
+        for (int r0 = 0; r0 < cnt; r0 += BATCH) {
+          if (cnt > BATCH) load(v, t0 + r0, cnt - r0);
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-          uint2 c;
-          c.x = to_codes<E4M3>(bf16_lo(v[i].x) * inv, bf16_hi(v[i].x) * inv, bf16_lo(v[i].y) * inv, bf16_hi(v[i].y) * inv);
-          c.y = to_codes<E4M3>(bf16_lo(v[i].z) * inv, bf16_hi(v[i].z) * inv, bf16_lo(v[i].w) * inv, bf16_hi(v[i].w) * inv);
-          if (!holds) c = make_uint2(0, 0);
-          if (r0 + i * ROWS + sub < cnt) *reinterpret_cast<uint2*>(dst + (r0 + i * ROWS + sub) * DH + ch * 8) = c;
+          for (int i = 0; i < WORDS; ++i) {
+            uint2 c;
+            c.x = to_codes<E4M3, CLAMP>(bf16_lo(v[i].x), bf16_hi(v[i].x), bf16_lo(v[i].y), bf16_hi(v[i].y), inv);
+            c.y = to_codes<E4M3, CLAMP>(bf16_lo(v[i].z), bf16_hi(v[i].z), bf16_lo(v[i].w), bf16_hi(v[i].w), inv);
+            if (!holds) c = make_uint2(0, 0);
+            if (r0 + i * ROWS + sub < cnt) *reinterpret_cast<uint2*>(dst + (r0 + i * ROWS + sub) * DH + ch * 8) = c;
+          }
         }
-      }
+      };
+      // only a mantissa of all ones is more than 127 steps of its own scale
+      if (!E4M3 && (top & 0x7f) == 0x7f) write(std::true_type());
+      else write(std::false_type());
       if (off && holds && old != scale) {                                        // what the block holds, in the new steps
         const float ratio = old * inv;
         uint4* before = reinterpret_cast<uint4*>(dst - off * DH);
 #pragma unroll 4
-        for (int i = lane; i < off * (DH / 16); i += 32) {
+        for (int i = lane + warp % SPLIT * 32; i < off * (DH / 16); i += 32 * SPLIT) {
           uint4 w = before[i];
           uint32_t* e = &w.x;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float4 f = from_codes<E4M3>(e[j]);
-            e[j] = to_codes<E4M3>(f.x * ratio, f.y * ratio, f.z * ratio, f.w * ratio);
+            e[j] = to_codes<E4M3, true>(f.x, f.y, f.z, f.w, ratio);
           }
           before[i] = w;
         }
       }
+      if (SPLIT > 1) asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / 2) : "memory");      // the maxima have been read
     }
+    if (p.cu_q && t < end)
+      while (b < p.B && p.cu_q[b + 1] <= t) ++b;
   }
 }
 
 // ---- reading back --------------------------------------------------------------------------------------------------------------
 // A page's codes and its values in bf16 lie in the same order, and the scale of an element is the one at its index / (block * dh). A thread
-// expands sixteen codes. Bound by memory: one byte read and two written an element.
+// expands two words of eight codes, or four where there are many, all of whose loads are under way before the first store; a warp's stores are
+// whole lines (sixteen codes a thread, whose stores are halves of lines: 66.5 us for 1000 pages). Bound by memory: one byte read and two written
+// an element. us for two / four / eight words a thread, 8 heads of 128: 1000 pages of 64 64.7 / 61.1 / 61.7 (0.98 of the copy rate), 100
+// 6.6 / 7.0 / 10.2, 30 3.2 / 3.8 / 5.5.
+constexpr int READ_THREADS = 256;
+
 struct ReadParams {
-  const uint8_t* codes; const float* scales;
+  const uint2* codes; const float* scales;
   const int* pages; int n, n_blocks;
-  long long page_words;                        // 16 codes each
+  long long page_words;                        // 8 codes each
   int shift;                                   // log2 of the words that share a scale
   int page_scales;
-  __nv_bfloat16* out;
+  uint4* out;
 };
 
-template <bool E4M3>
-__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams p) {
+template <bool E4M3, int READ_WORDS>
+__global__ void __launch_bounds__(READ_THREADS) read_kernel(const __grid_constant__ ReadParams p) {
   pdl_trigger();
   pdl_wait();
-  const long long w = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (w >= p.page_words) return;
+  const long long first = static_cast<long long>(blockIdx.x) * (READ_THREADS * READ_WORDS) + threadIdx.x;
   for (int i = blockIdx.y; i < p.n; i += gridDim.y) {
     const int id = p.pages[i];
-    uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks)) {
-      const uint4 c = *(reinterpret_cast<const uint4*>(p.codes) + id * p.page_words + w);
-      const float s = p.scales[static_cast<size_t>(id) * p.page_scales + (w >> p.shift)];
-      const float4 f0 = from_codes<E4M3>(c.x), f1 = from_codes<E4M3>(c.y), f2 = from_codes<E4M3>(c.z), f3 = from_codes<E4M3>(c.w);
-      o[0] = make_uint4(pack_bf16x2(f0.x * s, f0.y * s), pack_bf16x2(f0.z * s, f0.w * s), pack_bf16x2(f1.x * s, f1.y * s),
-                        pack_bf16x2(f1.z * s, f1.w * s));
-      o[1] = make_uint4(pack_bf16x2(f2.x * s, f2.y * s), pack_bf16x2(f2.z * s, f2.w * s), pack_bf16x2(f3.x * s, f3.y * s),
-                        pack_bf16x2(f3.z * s, f3.w * s));
+    const bool known = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
+    const uint2* src = p.codes + (known ? id : 0) * p.page_words;
+    const float* scales = p.scales + static_cast<size_t>(known ? id : 0) * p.page_scales;
+    uint4* dst = p.out + i * p.page_words;
+    uint2 c[READ_WORDS];
+    float s[READ_WORDS];
+#pragma unroll
+    for (int k = 0; k < READ_WORDS; ++k) {
+      const long long w = first + k * READ_THREADS;
+      c[k] = make_uint2(0, 0);
+      s[k] = 0.f;
+      if (known && w < p.page_words) {
+        c[k] = src[w];
+        s[k] = scales[w >> p.shift];
+      }
     }
-    uint4* dst = reinterpret_cast<uint4*>(p.out) + (i * p.page_words + w) * 2;
-    dst[0] = o[0];
-    dst[1] = o[1];
+#pragma unroll
+    for (int k = 0; k < READ_WORDS; ++k) {
+      const long long w = first + k * READ_THREADS;
+      const float4 f0 = from_codes<E4M3>(c[k].x), f1 = from_codes<E4M3>(c[k].y);
+      if (w < p.page_words)
+        dst[w] = make_uint4(pack_bf16x2(f0.x * s[k], f0.y * s[k]), pack_bf16x2(f0.z * s[k], f0.w * s[k]),
+                            pack_bf16x2(f1.x * s[k], f1.y * s[k]), pack_bf16x2(f1.z * s[k], f1.w * s[k]));
+    }
   }
 }
 
@@ -310,22 +360,26 @@ extern "C" int sb_quant_kv_append(void* qkv, long long ld, int n, int H, int Hkv
   p.qkv = static_cast<__nv_bfloat16*>(qkv); p.ld = ld; p.n = n; p.H = H; p.Hkv = Hkv;
   p.cos_t = cos_t; p.sin_t = sin_t; p.n_pos = n_pos;
   p.codes = static_cast<uint8_t*>(codes); p.scales = scales;
-  p.n_blocks = n_blocks; p.page = page; p.block = block;
+  p.n_blocks = n_blocks; p.page = page; p.block = block; p.per_page = page / block;
+  for (p.block_bits = 3; (1 << p.block_bits) < block;) ++p.block_bits;
   p.table = table; p.max_blocks = max_blocks; p.seq_len = seq_len; p.cu_q = cu_q; p.B = B; p.chunk = chunk;
   const long long chunks = (static_cast<long long>(n) + chunk - 1) / chunk, rows = 256 / dh;                     // rows of a warp of queries
-  // A warp finds its place by five loads, each of which waits for the one before: beyond two rounds of CTAs it takes more heads with that.
-  const long long most = (2 * Hkv + kv8::WARPS - 1) / kv8::WARPS, rounds = chunks * most / (num_sms() * 12ll);
-  p.head_ctas = static_cast<int>(rounds < 2 ? most : rounds < most ? (most + rounds - 1) / rounds : 1);
+  // Two warps a head: for blocks of more than sixteen, whose rows one warp would read in twice as many turns (16 sequences of 700 rows, blocks
+  // of 64: 19.1 against 25.3 us), and for blocks of sixteen where there are too few warps to hide how long a block takes (a prompt of 2048
+  // rows of an 8B model: 11.7 against 12.5 us; four of 1000: 18.4 against 16.9).
+  const int split = chunk > 8 && (block > 16 || (block > 8 && chunks * 2 * Hkv < num_sms() * 20ll)) ? 2 : 1;
+  const int warps = kv8::HEADS * split;
+  p.head_ctas = (2 * Hkv + kv8::HEADS - 1) / kv8::HEADS;
   const long long kv_ctas = chunks * p.head_ctas, ctas = kv_ctas + (cos_t && H ? (n + rows - 1) / rows : 0);
   if (ctas > 0x7fffffffll) return SB_ERR_TOO_LARGE;
   p.kv_ctas = static_cast<int>(kv_ctas);
   const dim3 grid(static_cast<unsigned>(ctas));
   using Kernel = void (*)(kv8::AppendParams);
-  static const Kernel kernels[8] = {kv8::append_kernel<64, false, 16>, kv8::append_kernel<64, false, 8>, kv8::append_kernel<64, true, 16>,
-                                    kv8::append_kernel<64, true, 8>, kv8::append_kernel<128, false, 16>, kv8::append_kernel<128, false, 8>,
-                                    kv8::append_kernel<128, true, 16>, kv8::append_kernel<128, true, 8>};
-  const Kernel kern = kernels[(dh == 128) * 4 + (e4m3 != 0) * 2 + (block == 8)];
-  return launch_dep(kern, grid, dim3(kv8::WARPS * 32), 0, static_cast<cudaStream_t>(stream_), p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  static const Kernel kernels[8] = {kv8::append_kernel<64, false, 1>, kv8::append_kernel<64, false, 2>, kv8::append_kernel<64, true, 1>,
+                                    kv8::append_kernel<64, true, 2>, kv8::append_kernel<128, false, 1>, kv8::append_kernel<128, false, 2>,
+                                    kv8::append_kernel<128, true, 1>, kv8::append_kernel<128, true, 2>};
+  const Kernel kern = kernels[(dh == 128) * 4 + (e4m3 != 0) * 2 + split - 1];
+  return launch_dep(kern, grid, dim3(warps * 32), 0, static_cast<cudaStream_t>(stream_), p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
 // out [n, 2, Hkv, page, dh] bf16: the pages' values; zeros for ids outside the pool.
@@ -334,14 +388,19 @@ extern "C" int sb_quant_kv_read(const void* codes, int e4m3, const float* scales
   if (!codes || !scales || !pages || !out || n <= 0 || !kv8::layout_ok(Hkv, dh, n_blocks, page, block)) return SB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15) return SB_ERR_ALIGN;
   kv8::ReadParams p;
-  p.codes = static_cast<const uint8_t*>(codes); p.scales = scales; p.pages = pages; p.n = n; p.n_blocks = n_blocks;
-  p.page_words = 2ll * Hkv * page * dh / 16;
+  p.codes = static_cast<const uint2*>(codes); p.scales = scales; p.pages = pages; p.n = n; p.n_blocks = n_blocks;
+  p.page_words = 2ll * Hkv * page * dh / 8;
   p.shift = 0;
-  while ((16 << p.shift) < block * dh) ++p.shift;
+  while ((8 << p.shift) < block * dh) ++p.shift;
   p.page_scales = 2 * Hkv * (page / block);
-  p.out = static_cast<__nv_bfloat16*>(out);
-  if (p.page_words > (1ll << 31) * 256 - 256) return SB_ERR_TOO_LARGE;
-  const dim3 grid(static_cast<unsigned>((p.page_words + 255) / 256), n < 65535 ? n : 65535);
-  auto kern = e4m3 ? kv8::read_kernel<true> : kv8::read_kernel<false>;
-  return launch_dep(kern, grid, dim3(256), 0, static_cast<cudaStream_t>(stream_), p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  p.out = static_cast<uint4*>(out);
+  const int words = n * static_cast<double>(p.page_words) < 4e6 ? 2 : 4;
+  const long long ctas = (p.page_words + kv8::READ_THREADS * words - 1) / (kv8::READ_THREADS * words);
+  if (ctas > 0x7fffffffll) return SB_ERR_TOO_LARGE;
+  const dim3 grid(static_cast<unsigned>(ctas), n < 65535 ? n : 65535);
+  using Kernel = void (*)(kv8::ReadParams);
+  static const Kernel kernels[4] = {kv8::read_kernel<false, 2>, kv8::read_kernel<false, 4>, kv8::read_kernel<true, 2>,
+                                    kv8::read_kernel<true, 4>};
+  const Kernel kern = kernels[(e4m3 != 0) * 2 + (words == 4)];
+  return launch_dep(kern, grid, dim3(kv8::READ_THREADS), 0, static_cast<cudaStream_t>(stream_), p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
