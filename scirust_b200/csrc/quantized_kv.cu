@@ -365,9 +365,11 @@ extern "C" int sb_quant_kv_append(void* qkv, long long ld, int n, int H, int Hkv
   p.table = table; p.max_blocks = max_blocks; p.seq_len = seq_len; p.cu_q = cu_q; p.B = B; p.chunk = chunk;
   const long long chunks = (static_cast<long long>(n) + chunk - 1) / chunk, rows = 256 / dh;                     // rows of a warp of queries
   // Two warps a head: for blocks of more than sixteen, whose rows one warp would read in twice as many turns (16 sequences of 700 rows, blocks
-  // of 64: 19.1 against 25.3 us), and for blocks of sixteen where there are too few warps to hide how long a block takes (a prompt of 2048
-  // rows of an 8B model: 11.7 against 12.5 us; four of 1000: 18.4 against 16.9).
-  const int split = chunk > 8 && (block > 16 || (block > 8 && chunks * 2 * Hkv < num_sms() * 20ll)) ? 2 : 1;
+  // of 64: 19.1 against 25.3 us), and for blocks of sixteen where there are too few warps to hide how long a block takes. us for two / one: 8
+  // heads of 128, 500 rows 5.9 / 7.8, 2048 rows 11.7 / 12.4, three sequences of 1000 14.3 / 14.0, four 18.4 / 16.8; 4 heads of 64, whose
+  // rows a warp loads in half the turns, 2048 rows 5.4 / 6.5, eight sequences of up to 1000 11.9 / 9.9.
+  const bool few = chunks * 2 * Hkv < num_sms() * (dh == 128 ? 20ll : 10ll);
+  const int split = chunk > 8 && (block > 16 || (block > 8 && few)) ? 2 : 1;
   const int warps = kv8::HEADS * split;
   p.head_ctas = (2 * Hkv + kv8::HEADS - 1) / kv8::HEADS;
   const long long kv_ctas = chunks * p.head_ctas, ctas = kv_ctas + (cos_t && H ? (n + rows - 1) / rows : 0);
