@@ -299,12 +299,12 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int step = lane / SCALES_OF_V * p.Hkv * per_page + ((first & (box - 1)) >> p.block_bits);
     int stage = 0, q_slot = 0;
     uint32_t phase = 0, q_phase = 0;
+    // of box (fetched + lane) of sequence b: its page, -1 outside the pool, and its first position there
+    int fetched = -1, id_of_lane = -1, slot_of_lane = 0;
     do {
       const int t_end = deal.whole ? nt : min(nt, t_beg + left);
       left -= deal.whole ? 1 : t_end - t_beg;
       const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
-      // of box (fetched + lane) of the sequence: its page, -1 outside the pool, and its first position there
-      int fetched = t_beg * nbx, id_of_lane, slot_of_lane;
       auto fetch = [&] {
         const long long pos = static_cast<long long>(fetched + lane) << box_bits;
         const int at = pos < len ? static_cast<int>(pos) / p.page : 0;
@@ -312,7 +312,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         id_of_lane = -1;
         if (pos < len) id_of_lane = table[at];
       };
-      if (!idle) fetch();                                // the ids come while the queries are seen to
+      if (!idle && fetched != t_beg * nbx) {             // the kv heads of a sequence have one table
+        fetched = t_beg * nbx;
+        fetch();                                         // the ids come while the queries are seen to
+      }
       if (brings_codes) {
         mbar_wait_converged(&q_empty[q_slot], q_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
         if (lane == 0) {
@@ -360,6 +363,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       if (++sub == p.subs) { sub = 0; ++kvh; }
       if (++job == jobs_b) {
         job = kvh = 0;
+        fetched = -1;
         if (++b < p.B) { len = lens[b]; nt = tiles_of<TK>(len); }
       }
     } while (left > 0);
