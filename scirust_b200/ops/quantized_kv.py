@@ -61,7 +61,8 @@ def _layout(what, pool, Hkv=None, dh=None):
     """(codes, scales, n_blocks, Hkv, page, dh, block) of a pool, or ValueError."""
     codes, scales = pool
     shape, per_block = codes.shape, scales.shape
-    if len(shape) != 5 or len(per_block) != 4 or shape[:3] != per_block[:3] or shape[1] != 2 or (Hkv is not None and (shape[2] != Hkv or shape[4] != dh)):
+    if (len(shape) != 5 or len(per_block) != 4 or shape[:3] != per_block[:3] or shape[1] != 2 or shape[2] == 0
+            or (Hkv is not None and (shape[2] != Hkv or shape[4] != dh))):
         raise ValueError(f"{what}: pool must be codes [n_blocks, 2, Hkv, page, dh] and scales [n_blocks, 2, Hkv, page / block]")
     n_blocks, _, heads, page, width = shape
     block = page // per_block[3] if per_block[3] else 0
@@ -175,6 +176,8 @@ def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
     B, max_blocks = _batch(what, n, seq_len, block_table, cu_q)
     if qkv.dtype is not BF:
         raise ValueError(f"{what}: qkv must be bf16")
+    if n_blocks == 0:
+        raise ValueError(f"{what}: the pool has no pages")
     if rope is not None:
         turns = rope[0].shape
         if len(turns) != 2 or turns[1] * 2 != dh or rope[1].shape != turns or rope[0].dtype is not F32 or rope[1].dtype is not F32:
@@ -200,7 +203,7 @@ def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
         n_pos, cos, sin = cos.shape[0], cos.data_ptr(), sin.data_ptr()
         if (cos | sin) % 16:
             raise ValueError(f"{what}: the rotation's tables must be 16-byte aligned")
-    if n == 0 or B == 0 or n_blocks == 0:
+    if n == 0 or B == 0:
         return
     _lib.call("sb_quant_kv_append", at, ld, n, H, Hkv, dh, cos, sin, n_pos, codes_at, codes.dtype is not torch.int8, scales.data_ptr(), n_blocks,
               page, block, block_table.data_ptr(), max_blocks, seq_len.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B,
@@ -318,7 +321,7 @@ def drop_workspace(device, stream):
 
 
 def decode_attention_ref(q, pool, block_table, seq_len, H, Hkv, dh, scale=None):
-    """fp32 statement, one sequence at a time; a sequence of no positions gets zeros."""
+    """fp32 statement, one sequence at a time; a sequence of no positions gets zeros, and pages outside the pool hold zeros."""
     codes, scales, _, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
     scale = 1.0 / math.sqrt(dh) if scale is None else scale
     out = torch.zeros((q.shape[0], H * dh), dtype=torch.float32, device=q.device)
@@ -327,7 +330,9 @@ def decode_attention_ref(q, pool, block_table, seq_len, H, Hkv, dh, scale=None):
         if length <= 0:
             continue
         ids = block_table[b, :(length + page - 1) // page].long()
-        kv = _values(codes.view(torch.int8)[ids].view(codes.dtype), scales[ids], block)
+        known = (ids >= 0) & (ids < codes.shape[0])
+        ids = ids.where(known, 0)
+        kv = _values(codes.view(torch.int8)[ids].view(codes.dtype), scales[ids], block).where(known[:, None, None, None, None], 0.0)
         k, v = kv.permute(1, 2, 0, 3, 4).reshape(2, Hkv, -1, dh)[:, :, :length]
         s = torch.einsum("hgd,hld->hgl", q[b, :H * dh].float().reshape(Hkv, H // Hkv, dh), k) * scale
         out[b] = torch.einsum("hgl,hld->hgd", torch.softmax(s, -1), v).reshape(-1)
@@ -338,13 +343,15 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     """GQA attention of one new token of each sequence over its paged KV in 8 bits. ``q`` [B, >= H * dh] bf16 holds the query heads (rotated);
     the token's own key and value are in ``pool`` already and counted by ``seq_len`` [B]. ``max_len`` bounds the lengths (default: the table);
     it is for the size of the launch only. A sequence of no positions (an empty slot) gets zeros. Positions behind a sequence's last one
-    may hold any code and any scale. Returns bf16 [B, H * dh], ``out`` if that is given; ``out`` may not lie in what the call reads."""
+    may hold any code and any scale; pages of no pool's (ids outside it) count as zeros. Returns bf16 [B, H * dh], ``out`` if that is given; ``out`` may not lie in what the call reads."""
     codes, scales, n_blocks, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
     shape = q.shape
     if len(shape) != 2 or H <= 0 or H % Hkv or shape[1] < H * dh or not scale > 0.0:
         raise ValueError("decode_attention: q must be [B, >= H * dh], heads a multiple of kv heads, scale positive")
     B, max_blocks = _batch("decode_attention", shape[0], seq_len, block_table, None)
+    if n_blocks == 0:
+        raise ValueError("decode_attention: the pool has no pages")
     if q.dtype is not BF or (out is not None and (out.dtype is not BF or tuple(out.shape) != (B, H * dh))):
         raise ValueError("decode_attention: q must be bf16, out bf16 [B, H * dh]")
     index = q.get_device()
@@ -370,8 +377,6 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
             raise ValueError("decode_attention: rows of out must be contiguous, apart, 16-byte aligned and on the device of q")
     if B == 0:
         return out
-    if n_blocks == 0:
-        raise ValueError("decode_attention: the pool has no pages")
     if page % TILE and page not in (8, 16, 32):
         raise ValueError("decode_attention: pages of 8, 16, 32 or a multiple of 64 positions")
     if scales.numel() >= 1 << 31:

@@ -153,6 +153,19 @@ def attention(q, pool, table, lens, H, Hkv, dh, scale=None):
     return out
 
 
+def test_pages_outside_the_pool_hold_zeros():
+    """Their scores are zeros and their values too: as a page of zeros in their place."""
+    H, Hkv, dh, page = 2, 1, 16, 8
+    g = torch.Generator().manual_seed(3)
+    pool = Q.QuantPool.zeros(4, Hkv, page, dh, "int8", device="cpu")
+    x = torch.randn((24, (H + 2 * Hkv) * dh), generator=g).to(BF)
+    lens = torch.tensor([24, 20]).int()
+    Q.kv_append(x, H, Hkv, dh, pool, torch.tensor([[0, 1, 2]]).int(), lens[:1], cu_q=torch.tensor([0, 24]).int())
+    q = torch.randn((2, H * dh), generator=g).to(BF)
+    got = Q.decode_attention(q, pool, torch.tensor([[0, -1, 2], [1, 2, 4]]).int(), lens, H, Hkv, dh)
+    assert torch.equal(got, Q.decode_attention(q, pool, torch.tensor([[0, 3, 2], [1, 2, 3]]).int(), lens, H, Hkv, dh))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_attention_and_reading_back(kind):
     H, Hkv, dh, page = 4, 2, 16, 8
@@ -209,6 +222,12 @@ def test_refusals():
     refused(Q.read_pages, pool, [0], out=torch.empty((2, 2, Hkv, page, dh), dtype=BF))
     for bad in (dict(codes="int4"), dict(block=4), dict(block=16), dict(page=12)):
         refused(Q.QuantPool.zeros, **{**dict(n_blocks=1, Hkv=1, page=8, dh=16, device="cpu"), **bad})
+    empty = Q.QuantPool.zeros(0, Hkv, page, dh, device="cpu")
+    refused(Q.kv_append, x, **{**good, "pool": empty})
+    refused(Q.decode_attention, q, **{**good, "pool": empty})
+    headless = Q.QuantPool.zeros(2, 0, page, dh, device="cpu")
+    refused(Q.kv_append, x, **{**good, "pool": headless, "Hkv": 0})
+    refused(Q.decode_attention, q, **{**good, "pool": headless, "Hkv": 0})
     assert Q.read_pages(pool, []).shape == (0, 2, Hkv, page, dh)
     assert Q.QuantPool.zeros(3, 2, 64, 128, device="cpu").nbytes() == 3 * 2 * 2 * 64 * (128 + 4 / 16)
 

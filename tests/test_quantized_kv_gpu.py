@@ -113,6 +113,11 @@ def test_long_prompt():
     write("e4m3", 4, 2, 128, 64, 16, [0, 5], [3000, 1111])
 
 
+@pytest.mark.parametrize("Hkv,dh", [(8, 64), (8, 128)])
+def test_more_blocks_than_two_warps_each_would_pay_for(Hkv, dh):
+    write("int8", 2, Hkv, dh, 64, 16, [7, 0], [2500, 700])
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_writing_in_parts_agrees_where_blocks_are_whole(kind):
     """A prompt in pieces that end with blocks gives the same pool as the whole of it."""
@@ -188,6 +193,15 @@ def test_pages_read_back(kind, page, block, dh, Hkv):
     want = pool.codes.to(F64) * odd.scales.to(F64).repeat_interleave(block, -1)[..., None]
     assert bool(((Q.read_pages(odd, list(range(9))).to(F64) - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -23)).all())
     assert Q.read_pages(pool, []).shape[0] == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_pages_read_back(kind):
+    pool = random_pool(9, 8, 64, 128, kind, 16)
+    ids = torch.randint(-1, 10, (300,), generator=gen(1), device=DEV).int()
+    got, known = Q.read_pages(pool, ids), (ids >= 0) & (ids < 9)
+    want = (pool.codes.float() * pool.scales.repeat_interleave(16, -1)[..., None]).to(BF)        # exact
+    assert torch.equal(got[known], want[ids[known].long()]) and not bool(got[~known].any())
 
 
 # ---------------------------------------------------------------------------------------------------------------- attention
