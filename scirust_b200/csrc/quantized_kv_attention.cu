@@ -3,10 +3,12 @@
 //   o = sum_j w_j s_v(j) c_v(j) / sum_j w_j,   w_j = exp(scale * s_k(j) * (q . c_k(j)) - m),
 // with codes c and the scales s of the position's block and head.
 //
-// Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time. One CTA per SM holds a ring of
-// 16 KB tiles (keys and values of 64 positions, or 128 of heads of 64) that one warp fills by TMA and another with the tile's sixteen scales; the tiles of all
-// jobs (a sequence and up to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer
-// warps take the tiles in groups of four, warp w of a group a quarter of the tile's positions, in sixteens:
+// Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time: 64 sequences of up to 2048 positions, 32
+// / 8 heads of 128, take 37.7 us (0.83 of the copy rate), one of 131072 46 (0.89). Calls of a few tiles a CTA are bound by latency, from 4.4 us on.
+// One CTA per SM holds a ring of 16 KB tiles (keys and values of 64 positions, or 128 of heads of 64: 32.9 us with tiles of 64, 25.5 so, for
+// 64 sequences of 16 / 4 such heads) that one warp fills by TMA and another with the tile's scales; the tiles of all jobs (a sequence and up
+// to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer warps take the tiles in
+// groups of four, warp w of a group a quarter of the tile's positions, in sixteens:
 //  - mma.sync takes codes as the A operand, 16 positions (S = K q) or 16 dimensions (O = V w), and eight query heads as columns: a warp's
 //    16 positions times 16 query rows would be half empty with eight query heads a kv head or fewer. With more, each group takes all tiles for
 //    eight of them. ldmatrix moves pairs of bytes, so the even and the odd dimensions of V come apart as rows of two halves of the A operand,
@@ -15,7 +17,8 @@
 //    subtraction of two halves, e4m3 by its conversion. K in int8 goes into the product as it is: q, scaled by a power of two so that its
 //    row's largest magnitude is just below 2^14 and rounded to whole numbers, is two bytes, whose products are summed apart, exactly. That
 //    rounding is off by 2^-14 of the row's largest at most, and bf16 values from 2^-6 of it on are kept as they are; 50 conversions a tile and
-//    lane of 130 are saved (1 x 131072 int8 52 -> 49 us). For e4m3 q's largest is just below 2^15, and fp16 holds it without loss.
+//    lane of 130 are saved (one sequence of 131072 positions: 52 us with halves, 49 so, as the rest then was). For e4m3 q's largest is just
+//    below 2^15, and fp16 holds it without loss.
 //  - The reference of the exponentials is a score seen before, not the maximum: it moves when a score exceeds it by 2^6, so that few
 //    tiles need a reduction over positions and a pass over O. Weights are 2^9 at the reference: at most 2^15, and what lies 2^-33 below the
 //    reference is still a number of fp16. Their sum is taken in 32 bits before they are rounded (half a step of 2^-11) and weighed.
@@ -23,9 +26,10 @@
 //    end: a product of its own for each block of 16 positions would need a pass over O for each.
 //  - A warp takes its positions' bytes into registers and gives the stage back before it computes, so that nearly the whole ring is always
 //    under way from memory.
-// At the end of a piece of a job the warps leave their sums in shared memory and go on; two finishing warps join them. A job that is cut
-// has its pieces joined by the CTA that ends last, in the order of the tiles (a counter, no atomics on data). Only the warp that brings the codes
-// works out which piece is next; the others find its sequence, heads and tiles beside its queries.
+// At the end of a piece of a job the warps leave their sums in shared memory and go on; two finishing warps join them, or, with more than
+// eight heads, all consumers, since two warps take ten turns for twenty heads (32 sequences of one kv head with 20 27.3 us so, 21.5
+// by all). A job that is cut has its pieces joined by the CTA that ends last, in the order of the tiles (a counter, no atomics on data).
+// Only the warp that brings the codes works out which piece is next; the others find its sequence, heads and tiles beside its queries.
 #include <cuda_bf16.h>
 #include "api.h"
 #include "dependent.cuh"
@@ -181,14 +185,15 @@ __device__ __forceinline__ void join_shares(const float2 (&ml)[SHARES], const fl
   }
 }
 
-template <int DH, bool E4M3>
+// MANY: jobs of more than one set of heads
+template <int DH, bool E4M3, bool MANY>
 __global__ void __launch_bounds__(Cfg<DH>::THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
   using C = Cfg<DH>;
   constexpr int CHUNKS = DH / 16, GROUPS = C::GROUPS, CONSUMERS = C::CONSUMERS, TK = C::TK, PARTS = C::PARTS, SCALES_OF_V = C::SCALES_OF_V;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stages = p.stages, sets = p.sets, heads = p.heads, jobs_b = p.Hkv * p.subs;
+  const int stages = p.stages, sets = MANY ? p.sets : 1, heads = p.heads, jobs_b = p.Hkv * p.subs;
   float* sc = reinterpret_cast<float*>(ring + stages * 2 * C::TILE);                // [stages][keys | values], of 8 positions each
   __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 2 * SCALES_OF_V);     // [slots][sets * heads][DH]
   Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * sets * heads * DH);          // [slots]
@@ -202,8 +207,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   uint64_t* o_empty = o_full + 1;
   int* prefix = reinterpret_cast<int*>(o_empty + 1);                                // [B + 1] tiles before sequence b
   int* lens = prefix + p.B + 1;                                                     // [B]
-  __shared__ int s_last[2], s_join[2][2];    // of the consumers and the finishers: whether their job's other pieces are there, its first CTA, its pieces
-  __shared__ int s_end, s_ready, s_ready_join[2];
+  // of the finishers and the consumers: whether their job's other pieces are there, its first CTA, its pieces
+  __shared__ int s_last[2], s_join[2][2];
+  __shared__ int s_end, s_ready, s_ready_now, s_ready_join[2];
   __shared__ Deal s_deal;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -249,12 +255,13 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       }
       longest = __reduce_max_sync(0xffffffffu, longest);
       const int tiles = base * jobs_b, jobs = p.B * jobs_b, grid = gridDim.x;
-      deal.ctas = min(grid, sets == 1 ? (tiles + GROUPS - 1) / GROUPS : tiles);
+      deal.ctas = min(grid, MANY ? tiles : (tiles + GROUPS - 1) / GROUPS);
       deal.each = tiles / deal.ctas;
       deal.whole = 0;
-      // What it costs to cut jobs (writing sums, asking for the count, reading them), at the end, where nothing else is under way, is as long as
-      // sixteen tiles: up to there jobs are dealt out whole. us cut / whole, 32 / 8 heads of 128: 1 x 600 positions 10.6 / 7.6, 4 x 800 11.4 / 9.1, 4 x
-      // 1600 (21 tiles more) 11.9 / 12.6, 16 x 300 11.5 / 7.0, 16 x 1500 15.5 / 12.6, 16 x 2500 19.3 / 17.6, 9 x 5003 of 4 / 1 heads 13.3 / 29.1.
+      // What it costs to cut jobs (writing sums, asking for the count, reading them), at the end, where nothing else is under way, is as long
+      // as sixteen tiles: up to there jobs are dealt out whole. us cut / whole, 32 / 8 heads of 128: 1 x 600 positions 10.1 / 7.1, 4 x 800 10.8 /
+      // 8.4, 4 x 1600 (21 tiles more) 11.4 / 12.0, 16 x 300 10.9 / 6.3, 16 x 1500 14.5 / 11.9, 16 x 2500 18.3 / 16.9, 64 x 1000 27.0 / 27.3, 9
+      // of up to 5003 on 4 / 1 heads 12.8 / 28.1.
       const int each = jobs <= grid ? 1 : jobs / grid, most = each + (each * grid < jobs);
       if (longest <= 4096 && most * longest - deal.each <= 16) {
         deal.ctas = min(grid, jobs);
@@ -339,21 +346,23 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           fetched = bx0;
           fetch();
         }
-        const int id = __shfl_sync(0xffffffffu, id_of_lane, bx0 + x - fetched), slot = __shfl_sync(0xffffffffu, slot_of_lane, bx0 + x - fetched);
+        const int id = __shfl_sync(0xffffffffu, id_of_lane, bx0 + x - fetched);
+        const int slot = __shfl_sync(0xffffffffu, slot_of_lane, bx0 + x - fetched);
         const bool known = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_blocks);
         const int rest = len - t * TK;                                                      // positions of the tile that exist, or more
         const int live = rest >= TK ? nbx : max(0, (rest + box - 1) >> box_bits);           // boxes with one of them
         mbar_wait_converged(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
         if (brings_codes) {
-          // A box of keys and, behind it, that of values; ids outside the pool: one behind its last page, all zeros. The stage is not full before lane 0
-          // has arrived, whichever comes first, its bytes or that they are expected.
-          if (x < live) tma_load_3d(ring + stage * 2 * C::TILE + first * 2 * DH, &tmap, &full[stage], 0, kvh * p.page + slot, known ? 2 * id : 2 * p.n_blocks);
+          // A box of keys and, behind it, that of values; ids outside the pool: one behind its last page, all zeros. The stage is not full
+          // before lane 0 has arrived, whichever comes first, its bytes or that they are expected.
+          if (x < live)
+            tma_load_3d(ring + stage * 2 * C::TILE + first * 2 * DH, &tmap, &full[stage], 0, kvh * p.page + slot, known ? 2 * id : 2 * p.n_blocks);
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
         } else if (lane < 2 * SCALES_OF_V) {
           const bool real = first < rest && known;
           const int at = (id * 2 * p.Hkv + kvh) * per_page + (slot >> p.block_bits) + step;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sc + stage * 2 * SCALES_OF_V + lane)), "l"(p.scales + (real ? at : 0)),
-                       "r"(real ? 4 : 0) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                       ::"r"(smem_u32(sc + stage * 2 * SCALES_OF_V + lane)), "l"(p.scales + (real ? at : 0)), "r"(real ? 4 : 0) : "memory");
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
         }
         if (++stage == stages) { stage = 0; phase ^= 1; }
@@ -376,11 +385,12 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   const int quad = lane >> 2, tq = lane & 3, mi = lane >> 3;
   const int group = warp >> 2, pw = warp & 3;
   // the groups take turns at the tiles, or, with more than one set of heads, each takes all tiles for a set of its own
-  const int my_set = sets == 1 ? 0 : group, stride = sets == 1 ? GROUPS : 1;
-  const int wrow = pw * (16 * PARTS) + (mi & 1) * 8 + (lane & 7);                              // the row of a tile that this lane addresses for ldmatrix
+  const int my_set = MANY ? group : 0, stride = MANY ? 1 : GROUPS;
+  const int wrow = pw * (16 * PARTS) + (mi & 1) * 8 + (lane & 7);                              // the lane's row of a tile, for ldmatrix
   // its first sixteen bytes of that row, swizzled; those of step c are at this address ^ (c << 4), and those of values a box behind
   const int box = 1 << p.page_bits;
-  const uint32_t my_row = smem_u32(ring) + ((wrow & ~(box - 1)) * 2 + (wrow & (box - 1))) * DH + (((mi >> 1) ^ (DH == 128 ? wrow & 7 : (wrow >> 1) & 3)) << 4);
+  const uint32_t my_row = smem_u32(ring) + ((wrow & ~(box - 1)) * 2 + (wrow & (box - 1))) * DH +
+                          (((mi >> 1) ^ (DH == 128 ? wrow & 7 : (wrow >> 1) & 3)) << 4);
   const uint32_t my_scales = smem_u32(sc) + pw * (8 * PARTS);
   const int next_part = (box <= 16 ? 32 : 16) * DH;                                    // sixteen positions further on
   const int team = consumes ? CONSUMERS * 32 : 64, tid = consumes ? threadIdx.x : threadIdx.x - C::FINISHERS * 32;
@@ -430,8 +440,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           down = e == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((e - 13u) << 23);      // no whole number is a NaN or an infinity
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t w0 = __float_as_uint(fmaf(bf16_lo(qb[c][0]), up, 12582912.f)), w1 = __float_as_uint(fmaf(bf16_hi(qb[c][0]), up, 12582912.f));
-            const uint32_t w2 = __float_as_uint(fmaf(bf16_lo(qb[c][1]), up, 12582912.f)), w3 = __float_as_uint(fmaf(bf16_hi(qb[c][1]), up, 12582912.f));
+            auto whole_number = [up](float x) { return __float_as_uint(fmaf(x, up, 12582912.f)); };
+            const uint32_t w0 = whole_number(bf16_lo(qb[c][0])), w1 = whole_number(bf16_hi(qb[c][0]));
+            const uint32_t w2 = whole_number(bf16_lo(qb[c][1])), w3 = whole_number(bf16_hi(qb[c][1]));
             qb[c][0] = __byte_perm(__byte_perm(w0 + 128, w1 + 128, 0x0051), __byte_perm(w2 + 128, w3 + 128, 0x0051), 0x5410);
             qb[c][1] = __byte_perm(__byte_perm(w0, w1, 0x0040), __byte_perm(w2, w3, 0x0040), 0x5410);
           }
@@ -441,7 +452,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         qf[1] = __shfl_sync(0xffffffffu, f, tq * 8 + 4);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_done);
+      if (lane == 0 && !MANY) mbar_arrive(q_done);
       float m[2] = {-1.0e30f, -1.0e30f}, l[2] = {0.f, 0.f}, o[CHUNKS][4];
       float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
 #pragma unroll
@@ -458,9 +469,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         float2 ks_of[PARTS], vs_of[PARTS];
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks_of[i].x), "=f"(ks_of[i].y) : "r"(my_scales + st * (8 * SCALES_OF_V) + i * 8) : "memory");
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
-                       : "=f"(vs_of[i].x), "=f"(vs_of[i].y) : "r"(my_scales + st * (8 * SCALES_OF_V) + i * 8 + 4 * SCALES_OF_V) : "memory");
+          const uint32_t at = my_scales + st * (8 * SCALES_OF_V) + i * 8;
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks_of[i].x), "=f"(ks_of[i].y) : "r"(at) : "memory");
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vs_of[i].x), "=f"(vs_of[i].y) : "r"(at + 4 * SCALES_OF_V) : "memory");
         }
         // the bytes of the warp's positions go to registers, and the stage back to the producers
         uint32_t k_of[PARTS][CHUNKS][2], v_of[PARTS][CHUNKS][2];
@@ -579,8 +590,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
-      mbar_wait_converged(o_empty, o_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);           // those of the piece before have been read
-      o_phase ^= 1;
+      if (!MANY) {
+        mbar_wait_converged(o_empty, o_phase ^ 1, p.status, ST_TIMEOUT_EMPTY);         // those of the piece before have been read
+        o_phase ^= 1;
+      }
       // a lane's values of a head lie behind one another: dimensions 16 c + 2 quad and the next, for all c
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -591,7 +604,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         for (int c = 0; c < CHUNKS; c += 2) dst[c / 2] = make_float4(o[c][e], o[c][2 + e], o[c + 1][e], o[c + 1][2 + e]);
         if (quad == 0) sm_ml[warp * heads + h] = make_float4(m[e], l[e], vref, 0.f);
       }
-      if (!last) {
+      if (!last && !MANY) {
         __syncwarp();
         if (lane == 0) mbar_arrive(o_full);
         continue;
@@ -621,12 +634,17 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         }
         return;
       }
+      if (MANY) continue;
       if (!mbar_wait_warp(o_full, o_phase, p.status, ST_TIMEOUT_FULL)) return;
       o_phase ^= 1;
     }
     if (t_beg == t_end) return;                          // a CTA without units
 
-    if (consumes) to = *piece;
+    if (consumes) {
+      to = *piece;
+      __syncwarp();
+      if (lane == 0 && MANY) mbar_arrive(q_done);
+    }
     const bool whole = t_beg == 0 && t_end == to.nt;
     auto part_of = [&](int c) { return p.part + static_cast<size_t>(c) * (HEADS_MAX * (DH + 2)); };
     // item i: four values of a head, in the order in which the warps left them
@@ -643,19 +661,20 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int shares = items <= 96 ? 4 : items <= 192 ? 2 : 1;
     bool ready = false;                                  // all other pieces are there
     if (consumes) {
-      if (tid == 0) {
+      if (tid == 0 && last) {
         *const_cast<volatile int*>(&s_end) = 1;
-        s_last[1] = *const_cast<volatile int*>(&s_ready);
+        s_ready_now = *const_cast<volatile int*>(&s_ready);
       }
       team_sync();
-      ready = s_last[1];
+      ready = last && s_ready_now;
     }
     const int r_c0 = s_ready_join[0], r_own = static_cast<int>(blockIdx.x) - r_c0, r_pieces = ready ? s_ready_join[1] : 0;
     ready = ready && r_pieces <= (shares == 1 ? SHARES : shares);      // a piece a share, or one share: they can be joined at once
     // ---- the warps' sums are joined in the order of the warps ----
+    constexpr int WARPS = MANY ? 4 : CONSUMERS;              // of a set
     for (int base = tid & ~31; base < items; base += team) {
       const int i = min(base + lane, items - 1), h = i / (DH / 4), set = (h >= heads) + (h >= 2 * heads), at = h - set * heads;
-      const int from = sets == 1 ? 0 : 4 * set, count = sets == 1 ? CONSUMERS : 4, x = lane & 15;
+      const int from = MANY ? 4 * set : 0, x = lane & 15;
       float4 other[SHARES];
       float2 other_ml[SHARES];
 #pragma unroll
@@ -669,22 +688,21 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         }
       }
       // lane x has the weight of warp x; all sums are under way while the weights are worked out
-      const float4 ml = x < count ? sm_ml[(from + x) * heads + at] : make_float4(-1.0e30f, 0.f, 0.f, 0.f);
+      const float4 ml = x < WARPS ? sm_ml[(from + x) * heads + at] : make_float4(-1.0e30f, 0.f, 0.f, 0.f);
       const float* src = sm_o + (from * heads + at) * C::PITCH + i % (DH / 4) * 4;
-      float4 e[CONSUMERS];
+      float4 e[WARPS];
 #pragma unroll
-      for (int k = 0; k < CONSUMERS; ++k)
-        e[k] = k < count ? *reinterpret_cast<const float4*>(src + k * (heads * C::PITCH)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < WARPS; ++k) e[k] = *reinterpret_cast<const float4*>(src + k * (heads * C::PITCH));
       float top = ml.x;
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float a = ex2(ml.x - top), weight = x < count ? a * ml.z : 0.f;
+      const float a = ex2(ml.x - top), weight = a * ml.z;
       float sum = ml.y * a;
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < CONSUMERS; ++k) {
+      for (int k = 0; k < WARPS; ++k) {
         const float w = __shfl_sync(0xffffffffu, weight, (lane & 16) + k);
         v.x += e[k].x * w; v.y += e[k].y * w; v.z += e[k].z * w; v.w += e[k].w * w;
       }
@@ -800,16 +818,18 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       join_shares(ml, e, v, sum);
       write_out(i, v, sum);
     }
+    if (consumes && !last) team_sync();                      // the next piece's sums go where the shares were
   }
 }
 
-template <int DH, bool E4M3>
+template <int DH, bool E4M3, bool MANY>
 static int launch_attend(const CUtensorMap& tm, AttendParams p, int grid, cudaStream_t s) {
   using C = Cfg<DH>;
   static PerDeviceOnce attr;
-  if (allow_smem(attr, attend_kernel<DH, E4M3>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  if (allow_smem(attr, attend_kernel<DH, E4M3, MANY>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
   p.stages = C::stages(p.sets, p.heads, p.B);
-  return launch_dep(attend_kernel<DH, E4M3>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.sets, p.heads, p.B), s, tm, p) == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  return launch_dep(attend_kernel<DH, E4M3, MANY>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.sets, p.heads, p.B), s, tm, p) == cudaSuccess
+             ? 0 : SB_ERR_LAUNCH;
 }
 
 }  // namespace kv8
@@ -832,7 +852,8 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
     return SB_ERR_ARG;
   if (page != 8 && page != 16 && page != 32 && page % 64) return SB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || (ldq & 7) || (ldo & 7)) return SB_ERR_ALIGN;
-  if (static_cast<double>(n_blocks) * 2 * Hkv * (page / block) > 2147483647.0 || static_cast<double>(Hkv) * page > 2147483647.0) return SB_ERR_TOO_LARGE;
+  if (static_cast<double>(n_blocks) * 2 * Hkv * (page / block) > 2147483647.0 || static_cast<double>(Hkv) * page > 2147483647.0)
+    return SB_ERR_TOO_LARGE;
   CUtensorMap tm;
   const int rc = make_tmap_3d_u8_rows(&tm, codes, dh, static_cast<uint64_t>(Hkv) * page, static_cast<uint64_t>(n_blocks) * 2,
                                       page < 64 ? page : 64, 2);
@@ -849,17 +870,23 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   const int per_job = (p.G + p.subs - 1) / p.subs;
   p.sets = (per_job + kv8::SET - 1) / kv8::SET;
   p.heads = (per_job + p.sets - 1) / p.sets;
-  if (static_cast<double>(B) * ((static_cast<double>(max_blocks) * page + 63) / 64) * Hkv * p.subs > 2147483647.0) return SB_ERR_TOO_LARGE;
+  const double most = static_cast<double>(B) * ((static_cast<double>(max_blocks) * page + 63) / 64) * Hkv * p.subs;
+  if (most > 2147483647.0) return SB_ERR_TOO_LARGE;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = part; p.counters = counters;
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.status = status;
   // the kernel leaves a tile to each group of consumers
-  const long long shared = p.sets == 1 ? (max_tiles + 2) / 3 : max_tiles, jobs = static_cast<long long>(B) * Hkv * p.subs, want = shared > jobs ? shared : jobs;
+  const long long shared = p.sets == 1 ? (max_tiles + 2) / 3 : max_tiles, jobs = static_cast<long long>(B) * Hkv * p.subs;
+  const long long want = shared > jobs ? shared : jobs;
   const int grid = want < num_sms() ? static_cast<int>(want) : num_sms();
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  if (dh == 64) return e4m3 ? kv8::launch_attend<64, true>(tm, p, grid, s) : kv8::launch_attend<64, false>(tm, p, grid, s);
-  return e4m3 ? kv8::launch_attend<128, true>(tm, p, grid, s) : kv8::launch_attend<128, false>(tm, p, grid, s);
+  using Launch = int (*)(const CUtensorMap&, kv8::AttendParams, int, cudaStream_t);
+  static const Launch launches[8] = {
+      kv8::launch_attend<64, false, false>, kv8::launch_attend<64, false, true>, kv8::launch_attend<64, true, false>,
+      kv8::launch_attend<64, true, true>, kv8::launch_attend<128, false, false>, kv8::launch_attend<128, false, true>,
+      kv8::launch_attend<128, true, false>, kv8::launch_attend<128, true, true>};
+  return launches[(dh == 128) * 4 + (e4m3 != 0) * 2 + (p.sets > 1)](tm, p, grid, s);
 }
 
 // The capture that `stream` is in, 0 where it is in none: what a graph's launches share is apart from every other graph's.

@@ -5,8 +5,8 @@ A pool is codes ``[n_blocks, 2, Hkv, page, dh]`` (int8 or float8_e4m3fn; keys, t
 (fp32): ``block`` consecutive positions of a head share one scale, and a value is code * scale. What is written gets the smallest power of
 two that the block's largest magnitude needs: 2^(k-6) for int8 where that lies in [2^k, 2^(k+1)), for e4m3 the least with 448 * scale no
 smaller (k is at least -90). A block that holds positions already keeps the larger of its scale and the new one, and what it holds is
-rounded to the new steps; a code stays within one step of its value, e4m3 loses nothing that way but below its smallest normal value. A block that
-is given an infinity or a NaN (e4m3: or what rounds to an infinity) reads as NaN until its first position is written again."""
+rounded to the new steps; a code stays within one step of its value, e4m3 loses nothing that way but below its smallest normal value. A
+block that is given an infinity or a NaN (e4m3: or what rounds to an infinity) reads as NaN until its first position is written again."""
 from __future__ import annotations
 
 import ctypes as C
@@ -343,7 +343,8 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     """GQA attention of one new token of each sequence over its paged KV in 8 bits. ``q`` [B, >= H * dh] bf16 holds the query heads (rotated);
     the token's own key and value are in ``pool`` already and counted by ``seq_len`` [B]. ``max_len`` bounds the lengths (default: the table);
     it is for the size of the launch only. A sequence of no positions (an empty slot) gets zeros. Positions behind a sequence's last one
-    may hold any code and any scale; pages of no pool's (ids outside it) count as zeros. Returns bf16 [B, H * dh], ``out`` if that is given; ``out`` may not lie in what the call reads."""
+    may hold any code and any scale; page ids outside the pool count as pages of zeros. Returns bf16 [B, H * dh], ``out`` if that is
+    given; ``out`` may not lie in what the call reads."""
     codes, scales, n_blocks, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
     shape = q.shape
