@@ -185,8 +185,8 @@ __device__ __forceinline__ void join_shares(const float2 (&ml)[SHARES], const fl
   }
 }
 
-// MANY: jobs of more than one set of heads
-template <int DH, bool E4M3, bool MANY>
+// MANY: jobs of more than one set of heads; SMALL: both producers ask for a tile's boxes
+template <int DH, bool E4M3, bool MANY, bool SMALL>
 __global__ void __launch_bounds__(Cfg<DH>::THREADS, 1)
 attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ AttendParams p) {
   using C = Cfg<DH>;
@@ -304,6 +304,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     const int x = first >> box_bits;
     const int per_page = p.page >> p.block_bits;                                            // scales of a page and head
     const int step = lane / SCALES_OF_V * p.Hkv * per_page + ((first & (box - 1)) >> p.block_bits);
+    // with SMALL every other box is the scales' warp's to ask for
+    const bool asks = brings_codes ? !(x & 1) : (x & 1) && lane < SCALES_OF_V && !(first & (box - 1));
     int stage = 0, q_slot = 0;
     uint32_t phase = 0, q_phase = 0;
     // of box (fetched + lane) of sequence b: its page, -1 outside the pool, and its first position there
@@ -352,11 +354,13 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         const int rest = len - t * TK;                                                      // positions of the tile that exist, or more
         const int live = rest >= TK ? nbx : max(0, (rest + box - 1) >> box_bits);           // boxes with one of them
         mbar_wait_converged(&empty[stage], phase ^ 1, p.status, ST_TIMEOUT_EMPTY);
+        auto ask = [&] {
+          tma_load_3d(ring + stage * 2 * C::TILE + first * 2 * DH, &tmap, &full[stage], 0, kvh * p.page + slot, known ? 2 * id : 2 * p.n_blocks);
+        };
         if (brings_codes) {
           // A box of keys and, behind it, that of values; ids outside the pool: one behind its last page, all zeros. The stage is not full
           // before lane 0 has arrived, whichever comes first, its bytes or that they are expected.
-          if (x < live)
-            tma_load_3d(ring + stage * 2 * C::TILE + first * 2 * DH, &tmap, &full[stage], 0, kvh * p.page + slot, known ? 2 * id : 2 * p.n_blocks);
+          if (SMALL ? asks && x < live : x < live) ask();
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], live * 2 * box * DH);
         } else if (lane < 2 * SCALES_OF_V) {
           const bool real = first < rest && known;
@@ -364,6 +368,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
                        ::"r"(smem_u32(sc + stage * 2 * SCALES_OF_V + lane)), "l"(p.scales + (real ? at : 0)), "r"(real ? 4 : 0) : "memory");
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
+          if (SMALL && asks && x < live) ask();
         }
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
@@ -822,14 +827,24 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   }
 }
 
-template <int DH, bool E4M3, bool MANY>
-static int launch_attend(const CUtensorMap& tm, AttendParams p, int grid, cudaStream_t s) {
+template <int DH, bool E4M3, bool MANY, bool SMALL>
+static int launch_kind(const CUtensorMap& tm, AttendParams p, int grid, cudaStream_t s) {
   using C = Cfg<DH>;
   static PerDeviceOnce attr;
-  if (allow_smem(attr, attend_kernel<DH, E4M3, MANY>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
+  if (allow_smem(attr, attend_kernel<DH, E4M3, MANY, SMALL>, SMEM, SB_ERR_LAUNCH)) return SB_ERR_LAUNCH;
   p.stages = C::stages(p.sets, p.heads, p.B);
-  return launch_dep(attend_kernel<DH, E4M3, MANY>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.sets, p.heads, p.B), s, tm, p) == cudaSuccess
+  return launch_dep(attend_kernel<DH, E4M3, MANY, SMALL>, dim3(grid), dim3(C::THREADS), C::smem_bytes(p.sets, p.heads, p.B), s, tm, p) == cudaSuccess
              ? 0 : SB_ERR_LAUNCH;
+}
+
+template <int DH, bool E4M3>
+static int launch_attend(const CUtensorMap& tm, const AttendParams& p, int grid, cudaStream_t s) {
+  // A box takes one warp some 90 cycles to ask for, whatever its size: a tile of four or more is shared by the two producers. us for one /
+  // two asking, 64 sequences of up to 2304 positions, 8 heads of 128, pages of 8 65.9 / 58.2, 16 52.4 / 50.3, 32 (two boxes) 46.5 / 47.1;
+  // 4 heads of 64, pages of 8 36.6 / 29.8, 16 25.9 / 22.9, 32 21.0 / 19.8, 64 (two boxes) 18.6 / 18.4.
+  const bool small = (Cfg<DH>::TK >> p.page_bits) >= 4;
+  if (p.sets > 1) return small ? launch_kind<DH, E4M3, true, true>(tm, p, grid, s) : launch_kind<DH, E4M3, true, false>(tm, p, grid, s);
+  return small ? launch_kind<DH, E4M3, false, true>(tm, p, grid, s) : launch_kind<DH, E4M3, false, false>(tm, p, grid, s);
 }
 
 }  // namespace kv8
@@ -881,12 +896,8 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   const long long want = shared > jobs ? shared : jobs;
   const int grid = want < num_sms() ? static_cast<int>(want) : num_sms();
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  using Launch = int (*)(const CUtensorMap&, kv8::AttendParams, int, cudaStream_t);
-  static const Launch launches[8] = {
-      kv8::launch_attend<64, false, false>, kv8::launch_attend<64, false, true>, kv8::launch_attend<64, true, false>,
-      kv8::launch_attend<64, true, true>, kv8::launch_attend<128, false, false>, kv8::launch_attend<128, false, true>,
-      kv8::launch_attend<128, true, false>, kv8::launch_attend<128, true, true>};
-  return launches[(dh == 128) * 4 + (e4m3 != 0) * 2 + (p.sets > 1)](tm, p, grid, s);
+  if (dh == 64) return e4m3 ? kv8::launch_attend<64, true>(tm, p, grid, s) : kv8::launch_attend<64, false>(tm, p, grid, s);
+  return e4m3 ? kv8::launch_attend<128, true>(tm, p, grid, s) : kv8::launch_attend<128, false>(tm, p, grid, s);
 }
 
 // The capture that `stream` is in, 0 where it is in none: what a graph's launches share is apart from every other graph's.
