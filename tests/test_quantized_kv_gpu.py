@@ -296,6 +296,38 @@ def test_attention_many_sequences(B):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,Hkv,dh", [(20, 1, 128), (24, 2, 64), (30, 1, 64), (8, 1, 128)])
+def test_attention_cut_and_whole_jobs_in_turn(kind, H, Hkv, dh):
+    """Long sequences among many short ones and empty slots: a CTA ends one job, has several whole ones and begins another."""
+    lens = [(13 * b * b + 5) % 300 if b % 7 else 0 for b in range(200)]
+    for at, n in ((0, 4000), (60, 2500), (61, 1), (199, 3333)):
+        lens[at] = n
+    a = batch(kind, H, Hkv, dh, 16, 8, lens)
+    want = check(a)
+    for _ in range(4):
+        assert torch.equal(Q.decode_attention(**a), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_more_bytes_than_32_bits_count(kind):
+    """The same three pages at the end of a pool of 4.5 GB as in a small one."""
+    H, Hkv, dh, page, block = 8, 8, 128, 64, 16
+    n = (9 << 29) // (2 * Hkv * page * dh)
+    codes = torch.empty((n, 2, Hkv, page, dh), dtype=torch.int8, device=DEV).view(Q.CODES[kind])
+    large = Q.QuantPool(codes, torch.zeros((n, 2, Hkv, page // block), device=DEV))
+    small = Q.QuantPool.zeros(3, Hkv, page, dh, kind, block)
+    codes[-3:].view(torch.int8).zero_()
+    x = torch.randn((150, (H + 2 * Hkv) * dh), generator=gen(0), device=DEV).to(BF)
+    lens, cu = torch.tensor([150], dtype=torch.int32, device=DEV), torch.tensor([0, 150], dtype=torch.int32, device=DEV)
+    tables_of = [torch.tensor([[n - 1, n - 3, n - 2]], dtype=torch.int32, device=DEV), torch.tensor([[2, 0, 1]], dtype=torch.int32, device=DEV)]
+    got = []
+    for pool, table in zip((large, small), tables_of):
+        Q.kv_append(x, H, Hkv, dh, pool, table, lens, cu_q=cu)
+        got.append((Q.decode_attention(x[:1, :H * dh], pool, table, lens, H, Hkv, dh), Q.read_pages(pool, table[0])))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and bool(got[0][0].any())
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_wide_scales(kind):
     """Scales of keys and values that differ by many powers of two between blocks, rising, falling and mixed: a small value with a large
     weight beside a large one with a small weight."""

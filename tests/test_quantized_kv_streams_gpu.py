@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from scirust_b200.generate import SamplingParams
-from scirust_b200.models.infer import InferenceEngine, teacher_forced_logits
+from scirust_b200.models.infer import InferenceEngine, PagedKVCache, teacher_forced_logits
 from scirust_b200.models.sciagent import GQADecoder, SciAgentConfig
 from scirust_b200.ops import _lib, decode as D, paged, quantized_kv as Q
 
@@ -228,6 +228,36 @@ def test_engine_behind_a_common_prefix(model, kv, monkeypatch):
             pages = -(-n // 16)
             assert torch.equal(pool[table[b, :pages].long()], every[eng.cache.owned[b][:pages]])
     _lib.check_status()
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("Hkv,page,block", [(1, 8, 8), (1, 16, 16), (3, 64, 16)])
+def test_cache_forks_compacts_and_grows(kv, Hkv, page, block):
+    """Down to a page whose scales are 8 bytes."""
+    H, dh, n = 4 * Hkv, 64, 5 * page // 2
+    cache = PagedKVCache(2, 9, Hkv, dh, page, 4, 3 * page, torch.device(DEV), kv, block)
+    cache.reserve(3, 5)
+    cache.reserve(0, n)
+    cache.commit()
+    lens, cu = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([n, 0, 0, 5], [0, n, n, n, n + 5]))
+    g = torch.Generator(device=DEV).manual_seed(0)
+    for pool in cache.pools:
+        Q.kv_append(torch.randn((n + 5, (H + 2 * Hkv) * dh), generator=g, device=DEV).to(BF), H, Hkv, dh, pool, cache.block_table, lens, cu_q=cu)
+    q = torch.randn((4, H * dh), generator=g, device=DEV).to(BF)[:1].repeat(4, 1)
+
+    def answers(lens):
+        return [Q.decode_attention(q, pool, cache.block_table, lens, H, Hkv, dh) for pool in cache.pools]
+
+    before = answers(lens)
+    cache.fork(0, [1, 2], n)
+    cache.release(1)
+    lens[2] = n
+    cache.compact()
+    cache.resize(12)
+    cache.resize(5)
+    cache.commit()
+    for a, b in zip(answers(lens), before):
+        assert torch.equal(a[[0, 3]], b[[0, 3]]) and torch.equal(a[2], b[0]) and not bool(a[1].any())
 
 
 def test_engine_refusals():
