@@ -64,13 +64,6 @@ __device__ __forceinline__ uint32_t rotate(uint32_t x, float c, float s) {
   return pack_bf16x2(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c)));
 }
 
-// The larger magnitudes of two pairs in bf16, NaN above all, under some sign.
-__device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
-  uint32_t y;
-  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
-  return y;
-}
-
 // x * f as codes. int8: 1.5 * 2^23 + x is rounded to a whole number, whose last byte is x's (a conversion takes four times as long); CLAMP: it
 // may be 128.
 template <bool E4M3, bool CLAMP>

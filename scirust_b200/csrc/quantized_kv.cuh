@@ -7,10 +7,10 @@
 namespace sb {
 namespace kv8 {
 
-// The larger ones of two pairs of 16-bit numbers.
-__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
+// The larger magnitudes of two pairs in bf16, NaN above all, under some sign.
+__device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
   uint32_t y;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
   return y;
 }
 

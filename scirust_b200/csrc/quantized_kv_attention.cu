@@ -54,6 +54,7 @@ struct AttendParams {
   const __nv_bfloat16* q; long long ldq;
   const float* scales;
   int n_blocks, page, page_bits, block_bits;         // page_bits: 3, 4 or 5, or for multiples of 64 6
+  int page_shift;                            // log2 of the page, -1 where it is no power of two
   const int* table; int max_blocks;
   const int* seq_len;
   int B, Hkv, G, subs;                       // a kv head's G query heads in `subs` jobs
@@ -316,7 +317,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       const int* table = p.table + static_cast<size_t>(b) * p.max_blocks;
       auto fetch = [&] {
         const long long pos = static_cast<long long>(fetched + lane) << box_bits;
-        const int at = pos < len ? static_cast<int>(pos) / p.page : 0;
+        const int at = pos >= len ? 0 : p.page_shift >= 0 ? static_cast<int>(pos) >> p.page_shift : static_cast<int>(pos) / p.page;
         slot_of_lane = static_cast<int>(pos) - at * p.page;
         id_of_lane = -1;
         if (pos < len) id_of_lane = table[at];
@@ -424,11 +425,11 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           const uint2 v = quad < mine ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
           qb[c][0] = v.x;
           qb[c][1] = v.y;
-          top = max16x2(top, max16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+          top = largest(top, largest(v.x, v.y));
         }
-        top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t e = max(max(top & 0xffffu, top >> 16) >> 7, 15u);               // the exponent of the largest, biased
+        top = largest(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = largest(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = max(max(top & 0x7fffu, top >> 16 & 0x7fffu) >> 7, 15u);     // the exponent of the largest, biased
         float down;
         if constexpr (E4M3) {
           const float up = __uint_as_float((268u - e) << 23);                          // 2^(14 - (e - 127)), and back
@@ -440,16 +441,17 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
           }
         } else {
           // Whole numbers of up to 2^14: 1.5 * 2^23 + q is a float whose last bytes are it. The lower byte counts from -128 on, so that the
-          // upper one is that of q + 128.
+          // upper one is that of q + 128, and the lower one that of q + 128 less 128, which is its first bit the other way.
           const float up = __uint_as_float((267u - e) << 23);
           down = e == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((e - 13u) << 23);      // no whole number is a NaN or an infinity
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
-            auto whole_number = [up](float x) { return __float_as_uint(fmaf(x, up, 12582912.f)); };
+            auto whole_number = [up](float x) { return __float_as_uint(fmaf(x, up, 12582912.f + 128.f)); };
             const uint32_t w0 = whole_number(bf16_lo(qb[c][0])), w1 = whole_number(bf16_hi(qb[c][0]));
             const uint32_t w2 = whole_number(bf16_lo(qb[c][1])), w3 = whole_number(bf16_hi(qb[c][1]));
-            qb[c][0] = __byte_perm(__byte_perm(w0 + 128, w1 + 128, 0x0051), __byte_perm(w2 + 128, w3 + 128, 0x0051), 0x5410);
-            qb[c][1] = __byte_perm(__byte_perm(w0, w1, 0x0040), __byte_perm(w2, w3, 0x0040), 0x5410);
+            const uint32_t w01 = __byte_perm(w0, w1, 0x5140), w23 = __byte_perm(w2, w3, 0x5140);      // lower bytes, upper bytes
+            qb[c][0] = __byte_perm(w01, w23, 0x7632);
+            qb[c][1] = __byte_perm(w01, w23, 0x5410) ^ 0x80808080u;
           }
         }
         const float f = down * p.scale_log2;
@@ -878,6 +880,9 @@ extern "C" int sb_quant_kv_attention(const void* q, long long ldq, const void* c
   p.scales = scales;
   p.n_blocks = n_blocks; p.page = page;
   for (p.page_bits = 3; p.page_bits < 6 && (1 << p.page_bits) < page;) ++p.page_bits;
+  p.page_shift = -1;
+  if (!(page & (page - 1)))
+    for (p.page_shift = 3; (1 << p.page_shift) < page;) ++p.page_shift;
   for (p.block_bits = 3; (1 << p.block_bits) < block;) ++p.block_bits;
   p.table = table; p.max_blocks = max_blocks; p.seq_len = seq_len;
   p.B = B; p.Hkv = Hkv; p.G = H / Hkv;
