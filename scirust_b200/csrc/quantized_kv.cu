@@ -26,8 +26,8 @@ namespace kv8 {
 // looked for once a sequence and chunk (once a block: 17.2 for 15.4 us, for 16 sequences of 700 rows). No two warps can write one block. Eight
 // rows a warp stay in registers between the maximum and the codes; of larger blocks the rows are read twice, the second time from L2. (The
 // next block's or head's rows under way meanwhile take registers that more warps use better: 17.8 us.) Query heads are only turned: a warp has
-// one row, or as many as fill it, with their part of the rotation's table in registers for its share of the heads.
-// Bound by latency for single tokens: 2.3 us for one, 3.2 for 64 sequences of an 8B model; for prompts by memory, at 0.77 (2048 rows) to 0.94 (16
+// one row, or as many as fill it, with their part of the rotation's table in registers for a quarter of the heads.
+// Bound by latency for single tokens: 2.3 us for one, 3.2 for 64 sequences of an 8B model; for prompts by memory, at 0.82 (2048 rows) to 0.94 (16
 // sequences of 700) of the copy rate.
 constexpr int HEADS = 4;                       // key or value heads of a CTA, with `SPLIT` warps each
 
@@ -116,11 +116,12 @@ __device__ __forceinline__ uint4 rotate8(uint4 v, const float4& c, const float4&
   return make_uint4(rotate(v.x, c.x, s.x), rotate(v.y, c.y, s.y), rotate(v.z, c.z, s.z), rotate(v.w, c.w, s.w));
 }
 
-template <int DH, int WARPS>
-__device__ __forceinline__ void turn_queries(const AppendParams& p, int cta) {
+template <int DH>
+__device__ __forceinline__ void turn_queries(const AppendParams& p, int team, int warp) {
+  constexpr int WARPS = HEADS;
   constexpr int LANES = DH / 8, ROWS = 32 / LANES, AHEAD = 8;                  // lanes of a row, rows of a warp, heads under way
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, ch = lane % LANES;
-  const int t0 = cta * ROWS, t = t0 + sub;
+  const int lane = threadIdx.x & 31, sub = lane / LANES, ch = lane % LANES;
+  const int t0 = team * ROWS, t = t0 + sub;
   __nv_bfloat16* x = p.qkv + min(t, p.n - 1) * p.ld + ch * 8;
   uint4 v[AHEAD];
   auto load = [&](int h0) {
@@ -156,7 +157,8 @@ __global__ void __launch_bounds__(HEADS * SPLIT * 32, SPLIT == 1 ? 8 : 4) append
   pdl_trigger();
   pdl_wait();
   if (static_cast<int>(blockIdx.x) >= p.kv_ctas) {
-    turn_queries<DH, HEADS * SPLIT>(p, blockIdx.x - p.kv_ctas);
+    const int warp = threadIdx.x >> 5;
+    turn_queries<DH>(p, (blockIdx.x - p.kv_ctas) * SPLIT + warp / HEADS, warp % HEADS);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ch = lane % LANES;
@@ -359,13 +361,13 @@ extern "C" int sb_quant_kv_append(void* qkv, long long ld, int n, int H, int Hkv
   const long long chunks = (static_cast<long long>(n) + chunk - 1) / chunk, rows = 256 / dh;                     // rows of a warp of queries
   // Two warps a head: for blocks of more than sixteen, whose rows one warp would read in twice as many turns (16 sequences of 700 rows, blocks
   // of 64: 19.1 against 25.3 us), and for blocks of sixteen where there are too few warps to hide how long a block takes. us for two / one: 8
-  // heads of 128, 500 rows 5.9 / 7.8, 2048 rows 11.7 / 12.4, three sequences of 1000 14.3 / 14.0, four 18.4 / 16.8; 4 heads of 64, whose
-  // rows a warp loads in half the turns, 2048 rows 5.4 / 6.5, eight sequences of up to 1000 11.9 / 9.9.
+  // heads of 128, 500 rows 5.9 / 7.8, 2048 rows 11.0 / 12.4, three sequences of 1000 14.3 / 14.0, four 18.4 / 16.8; 4 heads of 64, whose
+  // rows a warp loads in half the turns, 2048 rows 5.1 / 6.5, eight sequences of up to 1000 11.9 / 9.9.
   const bool few = chunks * 2 * Hkv < num_sms() * (dh == 128 ? 20ll : 10ll);
   const int split = chunk > 8 && (block > 16 || (block > 8 && few)) ? 2 : 1;
   const int warps = kv8::HEADS * split;
   p.head_ctas = (2 * Hkv + kv8::HEADS - 1) / kv8::HEADS;
-  const long long kv_ctas = chunks * p.head_ctas, ctas = kv_ctas + (cos_t && H ? (n + rows - 1) / rows : 0);
+  const long long kv_ctas = chunks * p.head_ctas, ctas = kv_ctas + (cos_t && H ? (n + rows * split - 1) / (rows * split) : 0);
   if (ctas > 0x7fffffffll) return SB_ERR_TOO_LARGE;
   p.kv_ctas = static_cast<int>(kv_ctas);
   const dim3 grid(static_cast<unsigned>(ctas));

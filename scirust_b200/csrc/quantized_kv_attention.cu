@@ -4,7 +4,7 @@
 // with codes c and the scales s of the position's block and head.
 //
 // Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time: 64 sequences of up to 2048 positions, 32
-// / 8 heads of 128, take 37.7 us (0.83 of the copy rate), one of 131072 46 (0.89). Calls of a few tiles a CTA are bound by latency, from 4.4 us on.
+// / 8 heads of 128, take 37.4 us (0.83 of the copy rate), one of 131072 46 (0.89). Calls of a few tiles a CTA are bound by latency, from 4.4 us on.
 // One CTA per SM holds a ring of 16 KB tiles (keys and values of 64 positions, or 128 of heads of 64: 32.9 us with tiles of 64, 25.5 so, for
 // 64 sequences of 16 / 4 such heads) that one warp fills by TMA and another with the tile's scales; the tiles of all jobs (a sequence and up
 // to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer warps take the tiles in
