@@ -203,7 +203,7 @@ def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
         n_pos, cos, sin = cos.shape[0], cos.data_ptr(), sin.data_ptr()
         if (cos | sin) % 16:
             raise ValueError(f"{what}: the rotation's tables must be 16-byte aligned")
-    if n == 0 or B == 0:
+    if n == 0 or B == 0 or (rope is not None and n_pos == 0):      # the address of tables without positions is null, as where there is no rotation
         return
     _lib.call("sb_quant_kv_append", at, ld, n, H, Hkv, dh, cos, sin, n_pos, codes_at, codes.dtype is not torch.int8, scales.data_ptr(), n_blocks,
               page, block, block_table.data_ptr(), max_blocks, seq_len.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B,

@@ -358,3 +358,13 @@ def test_command_takes_the_cache_type(model, tmp_path, capsys):
     CK.save_sciagent_checkpoint(model, tmp_path / "c", step=1, loss=0.0, lr=0.0)
     assert cli.run(["infer", "--checkpoint", str(tmp_path / "c"), "--prompt", "1 2 3", "--max-new", "4", "--kv", "int8", "--device", "cpu"]) == 0
     assert len(capsys.readouterr().out.splitlines()) == 1
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_rotation_without_positions_leaves_all_rows(kind):
+    H, Hkv, dh, page = 2, 1, 16, 8
+    x, pool = rows(3, H, Hkv, dh), Q.QuantPool.zeros(3, Hkv, page, dh, kind, device="cpu")
+    before, none = x.clone(), torch.empty((0, dh // 2))
+    for cu in (None, torch.arange(4).int()):
+        Q.rope_kv_append(x, H, Hkv, dh, none, none, pool, torch.arange(3).int()[:, None], torch.tensor([1, 3, 1]).int(), cu_q=cu)
+    assert torch.equal(x, before) and not bool(pool.codes.view(torch.int8).any()) and not bool(pool.scales.any())

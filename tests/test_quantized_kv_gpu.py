@@ -469,3 +469,20 @@ def test_refusals():
     refused(Q.read_pages, pool, torch.zeros(4, dtype=torch.int32, device=DEV)[::2])
     refused(Q.decode_attention, x, **good, out=torch.empty((2, H * dh), dtype=BF))
     refused(Q.decode_attention, x, **good, out=torch.empty((2, H * dh + 4), dtype=BF, device=DEV)[:, 4:])
+
+
+# ---------------------------------------------------------------------------------------------------------------- ends of the ranges
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("cu", [False, True])
+def test_a_rotation_without_positions_leaves_all_rows(kind, cu):
+    """Every row lies behind the end of tables that have no positions."""
+    H, Hkv, dh, page, block = 4, 2, 64, 16, 16
+    pool = random_pool(3, Hkv, page, dh, kind, block)
+    kept = Q.QuantPool(pool.codes.clone(), pool.scales.clone())
+    i = lambda *e: torch.tensor(e, dtype=torch.int32, device=DEV)
+    x = torch.randn((3, (H + 2 * Hkv) * dh), generator=gen(1), device=DEV).to(BF)
+    before, none = x.clone(), torch.empty((0, dh // 2), device=DEV)
+    table = torch.stack([i(0), i(1), i(2)])
+    Q.rope_kv_append(x, H, Hkv, dh, none, none, pool, table, i(1, 3, 1), cu_q=i(0, 1, 2, 3) if cu else None)
+    assert torch.equal(x, before)
+    assert torch.equal(bits(pool.codes), bits(kept.codes)) and torch.equal(bits(pool.scales), bits(kept.scales))
