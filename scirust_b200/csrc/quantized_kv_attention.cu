@@ -30,6 +30,7 @@
 // eight heads, all consumers, since two warps take ten turns for twenty heads (32 sequences of one kv head with 20 27.3 us so, 21.5
 // by all). A job that is cut has its pieces joined by the CTA that ends last, in the order of the tiles (a counter, no atomics on data).
 // Only the warp that brings the codes works out which piece is next; the others find its sequence, heads and tiles beside its queries.
+#include <cfloat>
 #include <cuda_bf16.h>
 #include "api.h"
 #include "dependent.cuh"
@@ -49,6 +50,7 @@ constexpr int STAGES_MAX = 24;
 constexpr int SET = 8, HEADS_MAX = 3 * SET;  // query heads of a set, which is what a warp takes, and of a job
 constexpr int SMEM = 225 * 1024;
 constexpr int SHARES = 4;                    // of the pieces of a job that is joined, at most
+constexpr float LOWEST = -FLT_MAX;           // reference of no score: no finite one lies below it, and what lies above by 15 moves it
 
 struct AttendParams {
   const __nv_bfloat16* q; long long ldq;
@@ -460,7 +462,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       }
       __syncwarp();
       if (lane == 0 && !MANY) mbar_arrive(q_done);
-      float m[2] = {-1.0e30f, -1.0e30f}, l[2] = {0.f, 0.f}, o[CHUNKS][4];
+      float m[2] = {LOWEST, LOWEST}, l[2] = {0.f, 0.f}, o[CHUNKS][4];
       float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
@@ -686,7 +688,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       float2 other_ml[SHARES];
 #pragma unroll
       for (int k = 0; k < SHARES; ++k) {
-        other_ml[k] = make_float2(-1.0e30f, 0.f);
+        other_ml[k] = make_float2(LOWEST, 0.f);
         other[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (ready && k < r_pieces && k != r_own) {
           const float* src = part_of(2 * (r_c0 + k) + (k == 0));
@@ -695,7 +697,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         }
       }
       // lane x has the weight of warp x; all sums are under way while the weights are worked out
-      const float4 ml = x < WARPS ? sm_ml[(from + x) * heads + at] : make_float4(-1.0e30f, 0.f, 0.f, 0.f);
+      const float4 ml = x < WARPS ? sm_ml[(from + x) * heads + at] : make_float4(LOWEST, 0.f, 0.f, 0.f);
       const float* src = sm_o + (from * heads + at) * C::PITCH + i % (DH / 4) * 4;
       float4 e[WARPS];
 #pragma unroll
@@ -753,7 +755,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
     // item i of a share of the pieces: the loads of eight pieces are under way together
     auto join_share = [&](int i, int share, float2& ml, float4& v) {
       const int h = i / (DH / 4);
-      ml = make_float2(-1.0e30f, 0.f);
+      ml = make_float2(LOWEST, 0.f);
       v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int c = share; c < n_pieces; c += 8 * shares) {
         float2 next_ml[8];
@@ -761,7 +763,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int at = c + k * shares;
-          next_ml[k] = make_float2(-1.0e30f, 0.f);
+          next_ml[k] = make_float2(LOWEST, 0.f);
           next[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (at < n_pieces) {
             const float* src = part_of(2 * (c0 + at) + (at == 0));
@@ -804,7 +806,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       float sum;
 #pragma unroll
       for (int k = 0; k < SHARES; ++k) {
-        ml[k] = make_float2(-1.0e30f, 0.f);
+        ml[k] = make_float2(LOWEST, 0.f);
         e[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (spread && k < shares) {
           e[k] = sm_v[k * items + i];

@@ -486,3 +486,35 @@ def test_a_rotation_without_positions_leaves_all_rows(kind, cu):
     Q.rope_kv_append(x, H, Hkv, dh, none, none, pool, table, i(1, 3, 1), cu_q=i(0, 1, 2, 3) if cu else None)
     assert torch.equal(x, before)
     assert torch.equal(bits(pool.codes), bits(kept.codes)) and torch.equal(bits(pool.scales), bits(kept.scales))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,Hkv,dh", [(8, 2, 128), (4, 4, 64), (20, 1, 128), (24, 1, 64)])
+def test_attention_scores_near_the_lowest_value(kind, H, Hkv, dh):
+    """All scores of a sequence are alike and -2^120 or lower: the answer is the mean of the values, and with one block far less low that of
+    its values. Equal keys give equal scores, bit for bit, and so weights of one power of two; what is left are the sums of up to n
+    terms in 32 bits, each addition off by a step of 2^-23 at most, and the rounding to bf16."""
+    lens = [1, 17, 300, 0, 5000]
+    a = batch(kind, H, Hkv, dh, 64, 16, lens, dirty=False)
+    pool = a["pool"]
+    pool.codes.view(torch.int8)[:, 0] = 1 if kind == "int8" else 0x38            # keys of 1
+    pool.scales[:, 0] = 2.0 ** 60
+    a["q"][:] = -2.0 ** 60
+    for least in (False, True):
+        if least:
+            for b, length in enumerate(lens):
+                if length:
+                    pool.scales[a["block_table"][b, length // 2 // 64].long(), 0, :, length // 2 % 64 // 16] = 2.0 ** 59
+        out = Q.decode_attention(**a).view(len(lens), Hkv, H // Hkv, dh)
+        for b, length in enumerate(lens):
+            if not length:
+                assert not bool(out[b].any())
+                continue
+            pos = torch.arange(length, device=DEV)
+            if least:
+                pos = pos[pos // 16 == length // 2 // 16]
+            at = a["block_table"][b].long()[pos // 64]
+            v = pool.codes.view(torch.int8)[at, 1, :, pos % 64].view(pool.codes.dtype).to(F64) * pool.scales[at, 1, :, pos % 64 // 16].to(F64)[..., None]
+            want, size = v.mean(0)[:, None], v.abs().mean(0)[:, None]
+            bound = 2.0 ** -8 * want.abs() + length * 2.0 ** -23 * size
+            assert bool(((out[b].to(F64) - want).abs() <= bound).all()), (least, length)
