@@ -22,8 +22,11 @@
 //  - The reference of the exponentials is a score seen before, not the maximum: it moves when a score exceeds it by 2^6, so that few
 //    tiles need a reduction over positions and a pass over O. Weights are 2^9 at the reference: at most 2^15, and what lies 2^-33 below the
 //    reference is still a number of fp16. Their sum is taken in 32 bits before they are rounded (half a step of 2^-11) and weighed.
-//  - A value's scale goes into its weight, as a ratio to the largest scale that the warp has seen of the piece, which weighs the sums at the
-//    end: a product of its own for each block of 16 positions would need a pass over O for each.
+//  - A value's scale goes into its weight, as a ratio to a power of two that weighs the sums at the end: a product of its own for each block of 16
+//    positions would need a pass over O for each. That power is a head's own and, where weights allow it, no less than the largest scale that the
+//    warp has seen of the piece, so that few tiles move it. But it is at most half of the largest product of a weight and a scale, so that
+//    what is rounded to fp16 loses no more than 2^-26 of that product (half of fp16's smallest step, 2^-25, against 2) wherever a
+//    scale without weight lies. Scales up to 2^100 times as large as another may lie beside it.
 //  - A warp takes its positions' bytes into registers and gives the stage back before it computes, so that nearly the whole ring is always
 //    under way from memory.
 // At the end of a piece of a job the warps leave their sums in shared memory and go on; two finishing warps join them, or, with more than
@@ -141,6 +144,20 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// One over a power of two between 2^-126 and 2^126.
+__device__ __forceinline__ float inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
+// The reference of values' scales, a power of two, after scales of up to `scale`, whose largest product with a weight is `product`, and a weight
+// of `a` for what was there: no less than the scales, so that nothing moves it before larger ones, but at most half of the largest product
+// so far (of which the old reference was at most half). A product is at most 2^15 of it: weights are, and where it lies below the scales it is
+// a quarter of the product or more. Numbers of one sign compare as their bits do.
+__device__ __forceinline__ float values_reference(float old, float scale, float product, float a) {
+  const uint32_t up = min((__float_as_uint(fmaxf(scale, old)) + 0x7fffffu) & 0x7f800000u, 0x7e800000u);
+  const uint32_t most = __float_as_uint(fmaxf(0.5f * product, a * old)) & 0x7f800000u;
+  const uint32_t least = __float_as_uint(fmaxf(scale * 0x1p-100f, 0x1p-126f)) & 0x7f800000u;      // the scales' ratio stays a number
+  return __uint_as_float(max(min(up, most), least));
+}
+
 // Bytes (0, 1) and (2, 3) of w as pairs of halves, or with APART (0, 2) and (1, 3).
 template <bool E4M3, bool APART>
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& x, uint32_t& y) {
@@ -201,7 +218,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
   __nv_bfloat16* sm_q = reinterpret_cast<__nv_bfloat16*>(sc + STAGES_MAX * 2 * SCALES_OF_V);     // [slots][sets * heads][DH]
   Piece* pieces = reinterpret_cast<Piece*>(sm_q + C::QSLOTS * sets * heads * DH);          // [slots]
   float* sm_o = reinterpret_cast<float*>(pieces + C::QSLOTS);                       // [warps][heads][PITCH]
-  float4* sm_ml = reinterpret_cast<float4*>(sm_o + CONSUMERS * heads * C::PITCH);   // [warps][heads]: reference, sum, largest scale of values
+  float4* sm_ml = reinterpret_cast<float4*>(sm_o + CONSUMERS * heads * C::PITCH);   // [warps][heads]: reference, sum, that of values' scales
   uint64_t* full = reinterpret_cast<uint64_t*>(sm_ml + CONSUMERS * heads);
   uint64_t* empty = full + STAGES_MAX;
   uint64_t* q_full = empty + STAGES_MAX;
@@ -463,7 +480,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       __syncwarp();
       if (lane == 0 && !MANY) mbar_arrive(q_done);
       float m[2] = {LOWEST, LOWEST}, l[2] = {0.f, 0.f}, o[CHUNKS][4];
-      float vref = 0x1p-100f, vinv = 0x1p100f;                                         // the largest scale of values so far
+      float vinv[2] = {0x1p126f, 0x1p126f};                                            // one over the references of values' scales
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
 
@@ -546,10 +563,8 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
             x[e] = s[e] - m[e & 1];
             top = fmaxf(top, x[e]);
           }
-          if (__any_sync(0xffffffffu, top > 15.f || fmaxf(vs.x, vs.y) > vref)) {
-            const float v_new = fmaxf(vref, fmaxf(vs.x, vs.y)), v_ratio = vref / v_new;
-            vref = v_new;
-            vinv = 1.f / v_new;
+          const float vs_top = fmaxf(vs.x, vs.y);
+          if (__any_sync(0xffffffffu, top > 15.f || vs_top * fmaxf(vinv[0], vinv[1]) > 1.f)) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float most = fmaxf(s[e], s[2 + e]) - 9.f;
@@ -560,22 +575,27 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
               l[e] *= a;
               x[e] = s[e] - m_new;
               x[2 + e] = s[2 + e] - m_new;
+              float product = fmaxf(ex2(x[e]) * vs.x, ex2(x[2 + e]) * vs.y);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) product = fmaxf(product, __shfl_xor_sync(0xffffffffu, product, d));
+              const float v_old = inverse(vinv[e]);
+              vinv[e] = inverse(values_reference(v_old, vs_top, product, a));
+              const float keep = a * v_old * vinv[e];                                  // v_old shrinks no faster than a
 #pragma unroll
               for (int c = 0; c < CHUNKS; ++c) {
-                o[c][e] *= a * v_ratio;
-                o[c][2 + e] *= a * v_ratio;
+                o[c][e] *= keep;
+                o[c][2 + e] *= keep;
               }
             }
           }
           uint32_t w[2];
           {
-            const float v0 = vs.x * vinv, v1 = vs.y * vinv;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
             l[0] += x[0] + x[2];
             l[1] += x[1] + x[3];
-            w[0] = transpose8x8(half2_bits(x[0] * v0, x[1] * v0));
-            w[1] = transpose8x8(half2_bits(x[2] * v1, x[3] * v1));
+            w[0] = transpose8x8(half2_bits(x[0] * (vs.x * vinv[0]), x[1] * (vs.x * vinv[1])));
+            w[1] = transpose8x8(half2_bits(x[2] * (vs.y * vinv[0]), x[3] * (vs.y * vinv[1])));
           }
           // what lies behind the last position may be NaN, which a weight of zero does not make zero
           uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -611,7 +631,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
         float4* dst = reinterpret_cast<float4*>(sm_o + (warp * heads + h) * C::PITCH + quad * (2 * CHUNKS));
 #pragma unroll
         for (int c = 0; c < CHUNKS; c += 2) dst[c / 2] = make_float4(o[c][e], o[c][2 + e], o[c + 1][e], o[c + 1][2 + e]);
-        if (quad == 0) sm_ml[warp * heads + h] = make_float4(m[e], l[e], vref, 0.f);
+        if (quad == 0) sm_ml[warp * heads + h] = make_float4(m[e], l[e], inverse(vinv[e]), 0.f);
       }
       if (!last && !MANY) {
         __syncwarp();

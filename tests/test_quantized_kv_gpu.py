@@ -518,3 +518,57 @@ def test_attention_scores_near_the_lowest_value(kind, H, Hkv, dh):
             want, size = v.mean(0)[:, None], v.abs().mean(0)[:, None]
             bound = 2.0 ** -8 * want.abs() + length * 2.0 ** -23 * size
             assert bool(((out[b].to(F64) - want).abs() <= bound).all()), (least, length)
+
+
+def spread_values(kind, H, Hkv, dh, lens, up, gap, seed=0):
+    """Sequences of positive values with a block of them 2^up times as large as the others, whose scores are ``gap`` (base 2) above the others'
+    for even query heads and below them for odd ones; in the middle of a sequence."""
+    a = batch(kind, H, Hkv, dh, 64, 16, lens, seed=seed, dirty=False)
+    pool, one = a["pool"], 1 if kind == "int8" else 0x38
+    v = pool.codes.view(torch.int8)[:, 1]
+    v.copy_(v.abs() if kind == "int8" else v & 0x7f)
+    pool.scales[:, 1] = torch.exp2(torch.randint(-3, 3, pool.scales[:, 1].shape, generator=gen(seed + 5), device=DEV).float())
+    pool.scales[:, 0] = 2.0 ** -7
+    pool.codes.view(torch.int8)[..., 0][:, 0] = 0
+    for b, length in enumerate(lens):
+        at, slot = a["block_table"][b, length // 2 // 64].long(), length // 2 % 64 // 16
+        pool.scales[at, 1, :, slot] *= 2.0 ** up
+        pool.scales[at, 0, :, slot] = 1.0
+        keys = pool.codes.view(torch.int8)[at, 0, :, slot * 16:slot * 16 + 16]
+        keys[:] = 0
+        keys[..., 0] = one
+    q = a["q"][:, :H * dh].view(len(lens), H, dh)
+    q[:, 0::2, 0] = gap * math.log(2.0) * math.sqrt(dh)
+    q[:, 1::2, 0] = -gap * math.log(2.0) * math.sqrt(dh)
+    return a
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,Hkv,dh", [(8, 2, 128), (4, 2, 64), (20, 1, 128)])
+@pytest.mark.parametrize("lens", [[40, 700, 512], [3000], [20000, 17]], ids=["whole", "cut", "long"])
+@pytest.mark.parametrize("up,gap", [(24, 60), (34, 40), (34, 34), (60, 90), (12, 8), (90, 90), (-40, 60), (60, 150), (100, 160)])
+def test_attention_values_of_one_block_far_from_the_others(kind, H, Hkv, dh, up, gap, lens):
+    """A weight counts by the value's scale that it has: a scale far above the others' takes nothing from them where its own weight
+    is small. As ``statement``, but what a product of a weight and a scale may lose below the numbers of fp16 is half a step of 2^-24 where
+    the largest such product of the sequence is 2 at least, times a code of 448 (127) at most: not a share of values without weight. The
+    scores here have the magnitudes that ``statement`` takes its slips from."""
+    a = spread_values(kind, H, Hkv, dh, lens, up, gap)
+    out = Q.decode_attention(**a).to(F64).view(len(lens), Hkv, H // Hkv, dh)
+    pool, scale = a["pool"], dh ** -0.5
+    largest = Q.LARGEST[pool.codes.dtype]
+    for b, length in enumerate(lens):
+        pos = torch.arange(length, device=DEV)
+        at = a["block_table"][b].long()[pos // 64]
+        steps = pool.scales[at, :, :, pos % 64 // 16].to(F64)
+        kv = pool.codes.view(torch.int8)[at, :, :, pos % 64].view(pool.codes.dtype).to(F64) * steps[..., None]
+        q = a["q"][b, :H * dh].to(F64).reshape(Hkv, H // Hkv, dh)
+        p = torch.softmax(torch.einsum("kgd,jkd->kgj", q, kv[:, 0]) * scale, -1)
+        size = torch.einsum("kgd,jkd->kgj", q.abs(), kv[:, 0].abs()) * scale
+        coarse = q.abs().amax(-1, keepdim=True) * 2.0 ** -14 * (kind == "int8")
+        want, mean = torch.einsum("kgj,jkd->kgd", p, kv[:, 1]), torch.einsum("kgj,jkd->kgd", p, kv[:, 1].abs())
+        # a score's own slip, before the exponential: of the positions with weight the largest counts
+        slip = 2 * (dh * 2.0 ** -23 * size + coarse * scale * kv[:, 0].abs().sum(-1).T[:, None]).amax(-1, keepdim=True) + 2.0 ** -11 + 2.0 ** -20
+        tiny = length * largest * 2.0 ** -26 * (p * steps[:, 1].T[:, None]).amax(-1, keepdim=True)
+        bound = 2.0 ** -8 * want.abs() + slip * mean + tiny
+        off = (out[b] - want).abs() / bound
+        assert bool((off <= 1).all()), (length, float(off.nan_to_num(9e9).max()))
