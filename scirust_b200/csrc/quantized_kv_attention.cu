@@ -725,8 +725,9 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       float top = ml.x;
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float a = ex2(ml.x - top), weight = a * ml.z;
-      float sum = ml.y * a;
+      // both 2^-24 times as large: a value near the largest number would leave the range beside a weight of 2^9 and more
+      const float a = ex2(ml.x - top), weight = a * (ml.z * 0x1p-24f);
+      float sum = a * (ml.y * 0x1p-24f);
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);

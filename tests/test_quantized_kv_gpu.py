@@ -572,3 +572,16 @@ def test_attention_values_of_one_block_far_from_the_others(kind, H, Hkv, dh, up,
         bound = 2.0 ** -8 * want.abs() + slip * mean + tiny
         off = (out[b] - want).abs() / bound
         assert bool((off <= 1).all()), (length, float(off.nan_to_num(9e9).max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,Hkv,dh", [(8, 2, 128), (20, 1, 64)])
+def test_attention_values_near_the_largest_number(kind, H, Hkv, dh):
+    """Values of up to 2^127, and down to the smallest scale that is written: 2^-96 (e4m3: 2^-98)."""
+    for scale in (2.0 ** (120 if kind == "int8" else 118), 2.0 ** (-96 if kind == "int8" else -98)):
+        a = batch(kind, H, Hkv, dh, 64, 16, [1, 16, 300, 2000], dirty=False)
+        a["pool"].scales[:, 1] = 2.0
+        want, bound = statement(a)
+        a["pool"].scales[:, 1] = 2 * scale
+        out = Q.decode_attention(**a).to(F64)
+        assert bool(((out / scale - want).abs() <= bound).all())
