@@ -585,3 +585,30 @@ def test_attention_values_near_the_largest_number(kind, H, Hkv, dh):
         a["pool"].scales[:, 1] = 2 * scale
         out = Q.decode_attention(**a).to(F64)
         assert bool(((out / scale - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** -30, 0.0, 2.0 ** 100, 2.0 ** -120, 2.0 ** -126, 2.0 ** 115])
+def test_attention_queries_of_any_size_e4m3(size):
+    """As whole numbers for int8 keys, queries are brought into fp16's range by a power of two for e4m3: near the ends of bf16's."""
+    a = batch("e4m3", 4, 1, 128, 64, 16, [300] * 2, dirty=False)
+    a["q"][0] = (a["q"][0].double().clamp(-3.9, 3.9) * size).to(BF)
+    out = Q.decode_attention(**a).to(F64)
+    want, bound = statement(a)
+    # of a large query one position takes all the weight; the statement's bound of a score would let any other have it
+    ok = (out - want).abs() <= (2.0 ** -7 * want.abs() if size > 2.0 ** 20 else bound)
+    assert bool(ok[0].all()) and bool(((out - want).abs() <= bound)[1].all())
+
+
+def test_attention_not_finite_e4m3():
+    """A NaN or an infinity in a query spoils that head alone; a NaN scale of a position that is read, or a NaN code of a value, the kv head's
+    rows of that sequence, the code one dimension of them."""
+    a = batch("e4m3", 4, 2, 64, 16, 16, [100, 50, 60, 70], dirty=False)
+    a["q"][0, 70] = math.nan
+    a["q"][1, 0] = math.inf
+    a["pool"].scales[a["block_table"][2, 1].long(), 1, 1, 0] = math.nan
+    a["pool"].codes.view(torch.int8)[a["block_table"][3, 4].long(), 1, 0, 5, 9] = 0x7f
+    out = Q.decode_attention(**a).view(4, 4, 64)
+    bad = torch.zeros((4, 4, 64), dtype=torch.bool, device=DEV)
+    bad[0, 1] = bad[1, 0] = bad[2, 2] = bad[2, 3] = True
+    bad[3, :2, 9] = True
+    assert torch.equal(out.isnan(), bad)
