@@ -1,5 +1,9 @@
 """The statements of the operators on a paged KV cache in 8 bits, against 64 bits, and what they refuse."""
 import math
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -368,3 +372,13 @@ def test_a_rotation_without_positions_leaves_all_rows(kind):
     for cu in (None, torch.arange(4).int()):
         Q.rope_kv_append(x, H, Hkv, dh, none, none, pool, torch.arange(3).int()[:, None], torch.tensor([1, 3, 1]).int(), cu_q=cu)
     assert torch.equal(x, before) and not bool(pool.codes.view(torch.int8).any()) and not bool(pool.scales.any())
+
+
+@pytest.mark.parametrize("world, kv", [(2, 4), (4, 1)])
+def test_tensor_parallel_ranks(world, kv):
+    """Sharded kv heads, and kv heads that ranks hold in common."""
+    root = Path(__file__).resolve().parents[1]
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={world}", "--master-addr", "127.0.0.1",
+           "--master-port", str(29840 + world), str(root / "tests" / "mp" / "mp_tp_quantized_kv.py")]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=600, env=dict(os.environ, PYTHONPATH=str(root), SB_TP_KV=str(kv)))
+    assert r.returncode == 0 and "TP_QUANTIZED_KV_OK" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
