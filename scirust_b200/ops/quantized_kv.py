@@ -90,6 +90,11 @@ def _on_device(what, index, codes, scales, dh, tensors):
     return at
 
 
+def _on_host(what, *tensors):
+    if any(t is not None and t.get_device() >= 0 for t in tensors):
+        raise ValueError(f"{what}: all tensors must be on one device")
+
+
 def _batch(what, n, seq_len, block_table, cu_q):
     lens, table = seq_len.shape, block_table.shape
     if len(lens) != 1 or len(table) != 2 or table[0] != lens[0]:
@@ -184,6 +189,7 @@ def _append(what, qkv, H, Hkv, dh, rope, pool, block_table, seq_len, cu_q):
             raise ValueError(f"{what}: the rotation's tables must be fp32 [positions, dh / 2]")
     index = qkv.get_device()
     if index < 0:
+        _on_host(what, codes, block_table, seq_len, cu_q, *(rope or ()))
         return _append_ref(qkv, H, Hkv, dh, rope, codes, scales, block, block_table, seq_len, cu_q)
     if index != _lib.current_device():
         with torch.cuda.device(index):
@@ -358,6 +364,7 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
         raise ValueError("decode_attention: q must be bf16, out bf16 [B, H * dh]")
     index = q.get_device()
     if index < 0:
+        _on_host("decode_attention", codes, block_table, seq_len, out)
         o = decode_attention_ref(q, pool, block_table, seq_len, H, Hkv, dh, scale).to(BF)
         return o if out is None else out.copy_(o)
     if index != _lib.current_device():

@@ -612,3 +612,23 @@ def test_attention_not_finite_e4m3():
     bad[0, 1] = bad[1, 0] = bad[2, 2] = bad[2, 3] = True
     bad[3, :2, 9] = True
     assert torch.equal(out.isnan(), bad)
+
+
+def test_rows_on_the_host_are_refused_beside_a_pool_on_the_device():
+    """Before anything is written."""
+    H, Hkv, dh, page = 4, 2, 64, 16
+    pool = random_pool(3, Hkv, page, dh, "int8", 16)
+    kept = pool.codes.clone()
+    x = torch.randn((5, (H + 2 * Hkv) * dh), generator=gen(0), device=DEV).to(BF).cpu()
+    table, lens, cu = torch.tensor([[1, 2]]).int(), torch.tensor([10]).int(), torch.tensor([0, 5]).int()
+    cos, sin = ops.rope_table(16, dh, 10000.0, DEV)
+    host = on_cpu(pool)
+    for bad in (dict(pool=pool), dict(pool=host, block_table=table.to(DEV)), dict(pool=host, seq_len=lens.to(DEV)), dict(pool=host, cu_q=cu.to(DEV))):
+        with pytest.raises(ValueError):
+            Q.kv_append(x, H, Hkv, dh, **{**dict(block_table=table, seq_len=lens, cu_q=cu), **bad})
+    with pytest.raises(ValueError):
+        Q.rope_kv_append(x, H, Hkv, dh, cos, sin, host, table, lens, cu_q=cu)
+    for bad in (dict(pool=pool), dict(block_table=table.to(DEV)), dict(seq_len=lens.to(DEV)), dict(out=torch.empty((1, H * dh), dtype=BF, device=DEV))):
+        with pytest.raises(ValueError):
+            Q.decode_attention(x[:1], **{**dict(pool=host, block_table=table, seq_len=lens, H=H, Hkv=Hkv, dh=dh), **bad})
+    assert torch.equal(pool.codes, kept)
