@@ -35,7 +35,7 @@ def main():
     ap.add_argument("--prompt", type=int, default=2048)
     ap.add_argument("--new", type=int, default=256)
     ap.add_argument("--quant", default="none", choices=["none", "int8"])
-    ap.add_argument("--kv", default="none", choices=["none", "int8", "e4m3"], help="keys and values of the cache in 8 bits")
+    ap.add_argument("--kv", default="none", choices=["none", "int8", "e4m3"], help="keys and values of the cache in 8 bits (faster for large batches, not for one sequence)")
     ap.add_argument("--ttft-iters", type=int, default=5)
     ap.add_argument("--layers", type=int, default=0, help="override the layer count (smoke runs)")
     ap.add_argument("--graph", type=int, default=1, help="0: launch every decode step eagerly (for launch lists)")

@@ -752,7 +752,8 @@ def build_parser():
         sp.add_argument("--repetition-penalty", type=float, default=1.0)
         sp.add_argument("--seed", type=int, default=0)
         sp.add_argument("--quant", default=None, choices=[None, "int8"])
-        sp.add_argument("--kv", default=None, choices=[None, "int8", "e4m3"], help="keys and values of the cache in 8 bits")
+        sp.add_argument("--kv", default=None, choices=[None, "int8", "e4m3"], help="keys and values of the cache in 8 bits: less memory, and faster for many sequences, "
+                        "but slower for many --samples of a long prompt, which each read it")
         sp.add_argument("--device", default="auto")
     i = sub.add_parser("infer")
     gen_args(i)

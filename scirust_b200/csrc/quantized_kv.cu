@@ -27,8 +27,10 @@ namespace kv8 {
 // rows a warp stay in registers between the maximum and the codes; of larger blocks the rows are read twice, the second time from L2. (The
 // next block's or head's rows under way meanwhile take registers that more warps use better: 17.8 us.) Query heads are only turned: a warp has
 // one row, or as many as fill it, with their part of the rotation's table in registers for a quarter of the heads.
-// Bound by latency for single tokens: 2.3 us for one, 3.2 for 64 sequences of an 8B model; for prompts by memory, at 0.82 (2048 rows) to 0.94 (16
-// sequences of 700) of the copy rate.
+// Bound by latency: 2.3 us for one token, 3.2 for one of each of 64 sequences of an 8B model. Runs of rows take longer than their bytes do, since a
+// warp sees to its blocks one after the other, each a chain of loads, a maximum, codes and stores: a prompt of 2048 rows 11.0 us (0.72 of
+// the copy rate), four of up to 1000 16.7 (0.80), 16 runs of up to 700 without rotation, 2080 CTAs for 1184 places, in blocks of 8 or 16
+// 14.2 and 15.0 (0.55, 0.52), in blocks of 64, whose rows are read twice, 19.0 (0.41).
 constexpr int HEADS = 4;                       // key or value heads of a CTA, with `SPLIT` warps each
 
 struct AppendParams {

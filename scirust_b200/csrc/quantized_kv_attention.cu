@@ -4,7 +4,7 @@
 // with codes c and the scales s of the position's block and head.
 //
 // Bound by the codes' bytes, half of a bf16 cache's, so everything done for a byte has half the time: 64 sequences of up to 2048 positions, 32
-// / 8 heads of 128, take 37.4 us (0.83 of the copy rate), one of 131072 46 (0.89). Calls of a few tiles a CTA are bound by latency, from 4.4 us on.
+// / 8 heads of 128, take 37.8 us (0.82 of the copy rate), one of 131072 46 (0.89). Calls of a few tiles a CTA are bound by latency, from 4.5 us on.
 // One CTA per SM holds a ring of 16 KB tiles (keys and values of 64 positions, or 128 of heads of 64: 32.9 us with tiles of 64, 25.5 so, for
 // 64 sequences of 16 / 4 such heads) that one warp fills by TMA and another with the tile's scales; the tiles of all jobs (a sequence and up
 // to 24 query heads of one kv head) lie end to end and are dealt out evenly, however ragged the lengths. Consumer warps take the tiles in
@@ -279,9 +279,13 @@ attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ 
       deal.each = tiles / deal.ctas;
       deal.whole = 0;
       // What it costs to cut jobs (writing sums, asking for the count, reading them), at the end, where nothing else is under way, is as long
-      // as sixteen tiles: up to there jobs are dealt out whole. us cut / whole, 32 / 8 heads of 128: 1 x 600 positions 10.1 / 7.1, 4 x 800 10.8 /
-      // 8.4, 4 x 1600 (21 tiles more) 11.4 / 12.0, 16 x 300 10.9 / 6.3, 16 x 1500 14.5 / 11.9, 16 x 2500 18.3 / 16.9, 64 x 1000 27.0 / 27.3, 9
-      // of up to 5003 on 4 / 1 heads 12.8 / 28.1.
+      // as sixteen tiles: up to there jobs are dealt out whole. us cut / whole, 32 / 8 heads of 128: 1 x 600 positions 9.9 / 7.1, 4 x 800 10.6 /
+      // 8.4, 4 x 1600 (21 tiles more) 11.1 / 12.0, 16 x 300 10.7 / 6.3, 16 x 1500 14.2 / 11.9, 16 x 2500 18.1 / 16.7, 64 x 1000 26.5 / 27.2, 9
+      // of up to 5003 on 4 / 1 heads 12.8 / 28.1; 16 / 4 heads of 64, whose tiles are twice as long: 1 x 600 8.1 / 5.5, 4 x 1600 8.5 / 8.3, 4 x
+      // 3000 8.9 / 12.4, 16 x 1500 9.7 / 8.5, 16 x 3000 11.0 / 12.7, 64 x 1000 14.5 / 11.5, 64 x 2000 17.3 / 16.8. A tile of several sets takes
+      // twice as long or more, so that with few such jobs sixteen are too many, at worst by a third: 20 / 1 heads of 128 1 x 600 9.9 / 10.9, 4
+      // x 800 10.2 / 12.8, 16 x 300 9.0 / 8.2, 16 x 1000 14.1 / 14.8, 32 x 400 11.7 / 9.4, 148 x 1000 23.2 / 17.5; 32 / 2 of 128 16 x 600
+      // 13.0 / 10.2, 74 x 1000 20.1 / 14.6; 24 / 2 of 64 8 x 1200 7.4 / 9.7, 16 x 2000 12.1 / 13.5, 74 x 1000 15.0 / 10.6.
       const int each = jobs <= grid ? 1 : jobs / grid, most = each + (each * grid < jobs);
       if (longest <= 4096 && most * longest - deal.each <= 16) {
         deal.ctas = min(grid, jobs);

@@ -272,7 +272,10 @@ class InferenceEngine:
     def __init__(self, model: GQADecoder, quant: str | None = None, max_batch: int = 1, max_seq: int = 4096,
                  page: int = 64, use_graph: bool = True, kv: str | None = None, kv_block: int | None = None):
         """``quant="int8"``: int8 weights. ``kv="int8"`` or ``"e4m3"``: a cache of half the size in 8 bits, one scale for ``kv_block`` positions of
-        a head (default: 16); decoding reads half the bytes, and what the cache holds is rounded once more."""
+        a head (default: 16); decoding reads half the bytes, and what the cache holds is rounded once more. Large batches gain by it, one
+        sequence of a few thousand positions does not (8B model behind 2048 positions, ms a step bf16 / int8: batch of 64 6.9 / 5.6, 16 4.2 / 3.9,
+        one 3.24 / 3.27), and many sequences behind a long common prefix (``generate_shared``) lose, since each reads the prefix for itself: 16
+        behind 2048 positions 3.8 / 3.8, 16 behind 8192 4.2 / 4.7, 64 behind 1024 4.4 / 4.6, 64 behind 8192 4.9 / 8.6."""
         cfg = model.cfg
         self.cfg, self.quant = cfg, quant
         dev = model.flat.device
@@ -671,7 +674,11 @@ class InferenceEngine:
             sampler.sample(logits, out_tokens=self.tokens[:B])
             sampler.push(self.tokens[:B])
         cache.seq_len[:B] = torch.tensor([P + n for n in lens], dtype=torch.int32, device=dev)
-        self._shared = shared if self.kv is None and self._shares(B, P) else None      # that attention reads pages in bf16
+        # That attention reads pages in bf16; over 8 bits each sequence reads the prefix, from the cache of the chip while it fits. us for the shared
+        # attention over bf16 / each sequence over 8 bits, 32 / 8 heads of 128: 2 x 2048 11.0 / 10.7, 16 x 1024 13.2 / 9.5, 16 x 8192 20.1 / 42.9, 64 x
+        # 1024 24.4 / 28.0, 64 x 8192 40.3 / 148; 16 / 4 heads of 64: 16 x 1024 10.7 / 6.9, 16 x 8192 14.8 / 17.3, 64 x 1024 16.3 / 11.3, 64 x 8192
+        # 26.8 / 48.8.
+        self._shared = shared if self.kv is None and self._shares(B, P) else None
         try:
             return self._decode_steps(B, longest, max_new, sampler)
         finally:
