@@ -355,7 +355,8 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     the token's own key and value are in ``pool`` already and counted by ``seq_len`` [B]. ``max_len`` bounds the lengths (default: the table);
     it is for the size of the launch only. A sequence of no positions (an empty slot) gets zeros. Positions behind a sequence's last one
     may hold any code and any scale; page ids outside the pool count as pages of zeros. Scores may lie
-    anywhere between -2^127 and 2^127. Returns bf16 [B, H * dh], ``out`` if that is
+    anywhere between -2^127 and 2^127, and the scales of a sequence's values, which are positive as those that are written, up to 2^100 times
+    one another. Queries over int8 codes are taken as whole numbers of 15 bits relative to each row's largest element. Returns bf16 [B, H * dh], ``out`` if that is
     given; ``out`` may not lie in what the call reads."""
     codes, scales, n_blocks, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
