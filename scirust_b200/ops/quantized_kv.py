@@ -354,10 +354,10 @@ def decode_attention(q, pool, block_table, seq_len, H, Hkv, dh, scale=None, max_
     """GQA attention of one new token of each sequence over its paged KV in 8 bits. ``q`` [B, >= H * dh] bf16 holds the query heads (rotated);
     the token's own key and value are in ``pool`` already and counted by ``seq_len`` [B]. ``max_len`` bounds the lengths (default: the table);
     it is for the size of the launch only. A sequence of no positions (an empty slot) gets zeros. Positions behind a sequence's last one
-    may hold any code and any scale; page ids outside the pool count as pages of zeros. Scores may lie
-    anywhere between -2^127 and 2^127, and the scales of a sequence's values, which are positive as those that are written, up to 2^100 times
-    one another. Queries over int8 codes are taken as whole numbers of 15 bits relative to each row's largest element. Returns bf16 [B, H * dh], ``out`` if that is
-    given; ``out`` may not lie in what the call reads."""
+    may hold any code and any scale; page ids outside the pool count as pages of zeros. Scores may lie anywhere between -2^127 and 2^127;
+    a sequence's scales of values, positive as those that are written, may be up to 2^100 times one another. A head's query is taken over int8 codes
+    as whole numbers of 15 bits, relative to its largest element. Returns bf16 [B, H * dh], ``out`` if that is given; ``out`` may not lie in
+    what the call reads."""
     codes, scales, n_blocks, _, page, _, block = _layout("decode_attention", pool, Hkv, dh)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
     shape = q.shape
